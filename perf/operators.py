@@ -284,7 +284,7 @@ def _prepare_kv4(case, g):
     s["lse"] = torch.empty(T, hq, device="cuda")
     if own:
         s["plan"] = _msa().fmha_sail_plan(torch.tensor(ql, dtype=torch.int32), torch.tensor(kl, dtype=torch.int32), hq, num_kv_heads=hk,
-                                          page_size=PAGE, kv_block_num=topk if topk else -1)
+                                          page_size=PAGE, kv_block_num=topk if topk else -1, use_kv4_cache=True)
     return s
 
 
