@@ -29,6 +29,9 @@ extern "C" {
 #define MSA_DT_BF16 0
 #define MSA_DT_E4M3 1
 #define MSA_DT_F32  2
+#define MSA_DT_KV4  3   /* caches only: e2m1 codes with an e4m3 scale for each 16 elements.  The tile of one (page, KV head) is
+                           9216 contiguous bytes: 128 rows of 64 bytes (element 2i in the low half of byte i), then
+                           128 rows of 8 scales.  Strides of such a cache are in bytes, multiples of 16 */
 
 /* msa_fmha_fwd mode bits (upstream SparseAttnMode, csrc/include/fmha_fusion.hpp:42-54) */
 #define MSA_FLAG_OUT_O      1   /* compute P.V and write O                      */
@@ -252,6 +255,85 @@ int msa_plan_device(const MsaPlanDeviceArgs* args, msa_stream_t stream);
 int msa_fmha_fwd_split_static(const MsaFmhaParams* params, const int32_t* splits_per_row,
                               msa_stream_t stream);
 
+/* msa_fmha_fwd with kv_dtype = MSA_DT_KV4: q bf16 or e4m3, paged k and v with page_size 128, MSA_FLAG_OUT_O only (with or
+ * without MSA_FLAG_SPARSE), block_m 16 / 64 / 128; up to 128 packed rows per work item.  Longer queries and scores: unpack
+ * the pages with msa_kv4_read and run on the copy.  A page table entry outside [0, kv_extent) is clamped. */
+
+/* Per-head RMS norm of q and k, rotary positions, and the write of k and v into a paged cache, in one pass over a step's
+ * tokens.  Any of q, k, v may be NULL (k needs k_out or k_cache; v needs v_cache).  q, k, v and the outputs are bf16 unless a
+ * dtype says otherwise, head_dim 128, strides in elements (a KV4 cache: bytes); in-place (q_out == q) is allowed.
+ *  - norm != 0: x / sqrt(mean(x^2) + eps) * weight; weights [128] (stride 0) or one row per head, f32 or bf16, NULL = 1.
+ *  - rotary elements (a multiple of 16, 0 = none) are rotated in pairs (i, i + rotary / 2), or (2i, 2i + 1) if interleaved,
+ *    by positions[axis[n]][token] * turns[n] for pair n; turns[n] = the frequency in turns per position, as a
+ *    64-bit fraction (modulo 1).
+ *  - cache: row of token t at slot_map[t] = page * page_size + offset; a negative slot, or one past num_pages, writes
+ *    nothing.  Slots of one call are distinct.  Keys are rounded to bf16, then divided by k_scale * k_scale_head[head]
+ *    and rounded to the cache's type (bf16 caches: as they are); values likewise.
+ * No upstream counterpart (upstream starts at the attention call). */
+typedef struct MsaNormRopeArgs {
+  const void* q; const void* k; const void* v;
+  const void* q_weight; const void* k_weight;
+  const void* positions;           /* int32 or int64, [axes][tokens] */
+  const int64_t* turns;            /* [rotary / 2] device */
+  const int32_t* axis;             /* [rotary / 2] device */
+  void* q_out; void* k_out; void* k_cache; void* v_cache;
+  const int32_t* slot_map;         /* [tokens] device */
+  const float* k_scale_head; const float* v_scale_head;   /* [num_kv_heads] or NULL */
+  int32_t* status;
+  int64_t pos_stride_axis;
+  int64_t q_stride_tok, q_stride_head, k_stride_tok, k_stride_head, v_stride_tok, v_stride_head;
+  int64_t q_out_stride_tok, q_out_stride_head, k_out_stride_tok, k_out_stride_head;
+  int64_t q_weight_stride, k_weight_stride;
+  int64_t k_cache_stride_page, k_cache_stride_head, k_cache_stride_tok;
+  int64_t v_cache_stride_page, v_cache_stride_head, v_cache_stride_tok;
+  int32_t tokens, num_qo_heads, num_kv_heads, rotary, interleaved, norm;
+  int32_t weight_dtype, q_out_dtype, cache_dtype, pos_int64, page_size, num_pages;
+  float eps, q_scale, k_scale, v_scale;
+} MsaNormRopeArgs;
+int msa_norm_rope(const MsaNormRopeArgs* args, msa_stream_t stream);
+
+/* Rows of a KV4 cache as bf16 (exact).  whole_pages == 0: out[i][head] = row slot_map[i] (zeros for a negative slot or one past
+ * num_pages); != 0: out[i][head][128][128] = page slot_map[i] (left as it was for a page outside [0, num_pages)). */
+typedef struct MsaKv4ReadArgs {
+  const void* cache;
+  void* out;
+  const int32_t* slot_map;         /* [rows] device: slots, or pages */
+  int32_t* status;
+  int64_t stride_page, stride_head;
+  int32_t rows, num_kv_heads, num_pages, whole_pages;
+} MsaKv4ReadArgs;
+int msa_kv4_read(const MsaKv4ReadArgs* args, msa_stream_t stream);
+
+/* The page table, slots and positions of a step from its requests' lengths, all on the device:
+ *  - kv_indices [max_total_pages] / kv_page_indptr [batch + 1]: the flat table that the attention call reads; entries
+ *    behind the last page are -1;
+ *  - slot_map / positions [max_total_q]: of every new token (the last qo_len keys of its request); -1 / 0 behind the last.
+ * With num_held, free_pages, num_free (all or none): pages that a request needs beyond the num_held[b] entries of its
+ * block_table row come from the top of the stack free_pages[0, num_free) in the order of the requests, and are written into
+ * the row; num_held_out / num_free_out (may be num_held / num_free) receive the new counts.  num_missing: pages and tokens
+ * that found no place (an empty stack, a row of the table or an output that is too short).  Such a page is 0 in
+ * kv_indices (attention over it stays in bounds but means nothing), -1 in block_table, and its tokens have slot -1. */
+typedef struct MsaPageTablesArgs {
+  const int32_t* qo_len;           /* [B] device: new tokens */
+  const int32_t* kv_len;           /* [B] device: keys with them */
+  int32_t* block_table;            /* [B][table_width] device, table_stride apart */
+  const int32_t* num_held;         /* [B] device or NULL */
+  const int32_t* free_pages;       /* [free_capacity] device or NULL */
+  const int32_t* num_free;         /* [1] device or NULL */
+  int32_t* kv_indices;
+  int32_t* kv_page_indptr;
+  int32_t* slot_map;
+  int32_t* positions;
+  int32_t* num_held_out;           /* [B] or NULL */
+  int32_t* num_free_out;           /* [1] or NULL */
+  int32_t* num_missing;            /* [1] or NULL */
+  int32_t* workspace;              /* msa_page_tables_workspace_bytes(batch) bytes */
+  int64_t table_stride;
+  int32_t batch, table_width, page_size, max_total_q, max_total_pages, free_capacity;
+} MsaPageTablesArgs;
+int64_t msa_page_tables_workspace_bytes(int32_t batch);
+int msa_page_tables(const MsaPageTablesArgs* args, msa_stream_t stream);
+
 /* Human-readable text of an MSA_ERR_* code. */
 const char* msa_status_string(int code);
 
@@ -259,7 +341,8 @@ const char* msa_status_string(int code);
 int msa_build_arch(void);
 
 /* sizeof() of the ABI structs as the library was compiled: 0 = MsaFmhaParams,
- * 1 = MsaWorkItem, 2 = MsaPlanArgs, 3 = MsaPlanDeviceArgs.  Lets a foreign-language binding verify its
+ * 1 = MsaWorkItem, 2 = MsaPlanArgs, 3 = MsaPlanDeviceArgs, 4 = MsaNormRopeArgs, 5 = MsaKv4ReadArgs,
+ * 6 = MsaPageTablesArgs.  Lets a foreign-language binding verify its
  * own struct declaration at load time. */
 int msa_sizeof(int which);
 

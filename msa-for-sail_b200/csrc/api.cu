@@ -15,6 +15,7 @@ int score_stream_supported(const MsaFmhaParams& p);
 int score_stream_launch(const MsaFmhaParams& p, cudaStream_t stream);
 int fmha_decode_tc_supported(const MsaFmhaParams& p);
 int fmha_decode_tc_launch(const MsaFmhaParams& p, cudaStream_t stream);
+int fmha_kv4_fwd(const MsaFmhaParams& p, cudaStream_t stream);
 int fmha_sparse_tc_supported(const MsaFmhaParams& p);
 int fmha_sparse_tc_launch(const MsaFmhaParams& p, cudaStream_t stream);
 int64_t fmha_sparse_tc_workspace_bytes(int64_t total_q, int num_qo_heads, int num_kv_heads, int kbn, int64_t num_pages);
@@ -73,8 +74,9 @@ extern "C" int msa_fmha_fwd(const MsaFmhaParams* pp, msa_stream_t stream_) {
   if (!pp) return MSA_ERR_BAD_ARG;
   msa::NvtxRange range("msa_fmha_fwd");
   const MsaFmhaParams& p = *pp;
-  if (const int rc = msa::validate_fmha(p, false)) return rc;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+  if (p.kv_dtype == MSA_DT_KV4) return msa::fmha_kv4_fwd(p, stream);
+  if (const int rc = msa::validate_fmha(p, false)) return rc;
   if (msa::fmha_sparse_tc_supported(p)) return msa::fmha_sparse_tc_launch(p, stream);
   if (msa::score_stream_supported(p)) return msa::score_stream_launch(p, stream);
   if (msa::fmha_decode_tc_supported(p)) return msa::fmha_decode_tc_launch(p, stream);
@@ -227,6 +229,9 @@ extern "C" int msa_sizeof(int which) {
     case 1: return static_cast<int>(sizeof(MsaWorkItem));
     case 2: return static_cast<int>(sizeof(MsaPlanArgs));
     case 3: return static_cast<int>(sizeof(MsaPlanDeviceArgs));
+    case 4: return static_cast<int>(sizeof(MsaNormRopeArgs));
+    case 5: return static_cast<int>(sizeof(MsaKv4ReadArgs));
+    case 6: return static_cast<int>(sizeof(MsaPageTablesArgs));
     default: return -1;
   }
 }

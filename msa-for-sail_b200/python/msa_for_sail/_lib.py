@@ -16,7 +16,7 @@ BOUNDS_CHECK = os.environ.get("MSA_BOUNDS_CHECK", "0") not in ("", "0")
 LIB_PATH = os.path.join(_HERE, "libmsa_b200_check.so" if BOUNDS_CHECK else "libmsa_b200.so")
 STATUS_OK, STATUS_TIMEOUT, STATUS_BOUNDS = 0, 1, 2
 
-MSA_DT_BF16, MSA_DT_E4M3, MSA_DT_F32 = 0, 1, 2
+MSA_DT_BF16, MSA_DT_E4M3, MSA_DT_F32, MSA_DT_KV4 = 0, 1, 2, 3
 FLAG_OUT_O, FLAG_OUT_SCORE, FLAG_SPARSE = 1, 2, 4
 
 _p = ctypes.c_void_p
@@ -66,10 +66,39 @@ class MsaPlanDeviceArgs(ctypes.Structure):
                 ("row_tiles", _i32)]
 
 
+class MsaNormRopeArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", _p), ("k", _p), ("v", _p), ("q_weight", _p), ("k_weight", _p), ("positions", _p), ("turns", _p), ("axis", _p),
+        ("q_out", _p), ("k_out", _p), ("k_cache", _p), ("v_cache", _p), ("slot_map", _p), ("k_scale_head", _p), ("v_scale_head", _p),
+        ("status", _p), ("pos_stride_axis", _i64),
+        ("q_stride_tok", _i64), ("q_stride_head", _i64), ("k_stride_tok", _i64), ("k_stride_head", _i64),
+        ("v_stride_tok", _i64), ("v_stride_head", _i64), ("q_out_stride_tok", _i64), ("q_out_stride_head", _i64),
+        ("k_out_stride_tok", _i64), ("k_out_stride_head", _i64), ("q_weight_stride", _i64), ("k_weight_stride", _i64),
+        ("k_cache_stride_page", _i64), ("k_cache_stride_head", _i64), ("k_cache_stride_tok", _i64),
+        ("v_cache_stride_page", _i64), ("v_cache_stride_head", _i64), ("v_cache_stride_tok", _i64),
+        ("tokens", _i32), ("num_qo_heads", _i32), ("num_kv_heads", _i32), ("rotary", _i32), ("interleaved", _i32), ("norm", _i32),
+        ("weight_dtype", _i32), ("q_out_dtype", _i32), ("cache_dtype", _i32), ("pos_int64", _i32), ("page_size", _i32), ("num_pages", _i32),
+        ("eps", _f32), ("q_scale", _f32), ("k_scale", _f32), ("v_scale", _f32),
+    ]
+
+
+class MsaKv4ReadArgs(ctypes.Structure):
+    _fields_ = [("cache", _p), ("out", _p), ("slot_map", _p), ("status", _p), ("stride_page", _i64), ("stride_head", _i64),
+                ("rows", _i32), ("num_kv_heads", _i32), ("num_pages", _i32), ("whole_pages", _i32)]
+
+
+class MsaPageTablesArgs(ctypes.Structure):
+    _fields_ = [("qo_len", _p), ("kv_len", _p), ("block_table", _p), ("num_held", _p), ("free_pages", _p), ("num_free", _p),
+                ("kv_indices", _p), ("kv_page_indptr", _p), ("slot_map", _p), ("positions", _p), ("num_held_out", _p),
+                ("num_free_out", _p), ("num_missing", _p), ("workspace", _p), ("table_stride", _i64), ("batch", _i32),
+                ("table_width", _i32), ("page_size", _i32), ("max_total_q", _i32), ("max_total_pages", _i32), ("free_capacity", _i32)]
+
+
 #: every symbol include/msa_b200.h declares
 EXPORTS = ("msa_fmha_fwd", "msa_lse_merge", "msa_topk_select", "msa_plan_dense",
            "msa_status_string", "msa_build_arch", "msa_sizeof", "msa_fmha_fwd_split_static",
-           "msa_sparse_workspace_bytes", "msa_plan_device", "msa_lse_merge_ex")
+           "msa_sparse_workspace_bytes", "msa_plan_device", "msa_lse_merge_ex", "msa_norm_rope", "msa_kv4_read",
+           "msa_page_tables", "msa_page_tables_workspace_bytes")
 
 
 def _load():
@@ -83,7 +112,8 @@ def _load():
             raise ImportError(f"{LIB_PATH} does not export {name}")
     lib.msa_sizeof.argtypes = [ctypes.c_int]
     lib.msa_sizeof.restype = ctypes.c_int
-    for which, st in ((0, MsaFmhaParams), (1, MsaWorkItem), (2, MsaPlanArgs)):
+    for which, st in ((0, MsaFmhaParams), (1, MsaWorkItem), (2, MsaPlanArgs), (3, MsaPlanDeviceArgs), (4, MsaNormRopeArgs),
+                      (5, MsaKv4ReadArgs), (6, MsaPageTablesArgs)):
         if lib.msa_sizeof(which) != ctypes.sizeof(st):
             raise ImportError(
                 f"ABI mismatch for {st.__name__}: library {lib.msa_sizeof(which)} bytes, "
@@ -105,6 +135,14 @@ def _load():
     lib.msa_sparse_workspace_bytes.restype = _i64
     lib.msa_plan_device.argtypes = [ctypes.POINTER(MsaPlanDeviceArgs), _p]
     lib.msa_plan_device.restype = ctypes.c_int
+    lib.msa_norm_rope.argtypes = [ctypes.POINTER(MsaNormRopeArgs), _p]
+    lib.msa_norm_rope.restype = ctypes.c_int
+    lib.msa_kv4_read.argtypes = [ctypes.POINTER(MsaKv4ReadArgs), _p]
+    lib.msa_kv4_read.restype = ctypes.c_int
+    lib.msa_page_tables.argtypes = [ctypes.POINTER(MsaPageTablesArgs), _p]
+    lib.msa_page_tables.restype = ctypes.c_int
+    lib.msa_page_tables_workspace_bytes.argtypes = [_i32]
+    lib.msa_page_tables_workspace_bytes.restype = _i64
     lib.msa_fmha_fwd_split_static.argtypes = [ctypes.POINTER(MsaFmhaParams), _p, _p]
     lib.msa_fmha_fwd_split_static.restype = ctypes.c_int
     return lib

@@ -15,8 +15,8 @@ from typing import Optional, Tuple, Union
 import numpy as np
 import torch
 
-from . import _lib
-from ._lib import FLAG_OUT_O, FLAG_OUT_SCORE, FLAG_SPARSE, MSA_DT_BF16, MSA_DT_E4M3, MSA_DT_F32
+from . import _lib, cache
+from ._lib import FLAG_OUT_O, FLAG_OUT_SCORE, FLAG_SPARSE, MSA_DT_BF16, MSA_DT_E4M3, MSA_DT_F32, MSA_DT_KV4
 
 __all__ = [
     "fmha_sail_plan", "fmha_sail", "sparse_topk_select",
@@ -25,6 +25,7 @@ __all__ = [
 ]
 
 KV_TILE = 128
+_KV4_CTAS = 3                           # CTAs of the 4-bit decode kernel that share an SM
 _USE_TC = True                          # route eligible prefill shapes to the tcgen05 kernel
 _FORCE_TC = False                       # ... even when the planner would rather split KV
 _USE_DECODE_TC = True                   # tcgen05 decode kernel for short-query bf16 shapes
@@ -115,7 +116,7 @@ def _compute_pack_factor(max_qo_len, num_qo_heads, num_kv_heads):
     return h_r
 
 
-def _sparse_splits(items, kv_block_num, num_kv_splits, num_sms, two_per_sm):
+def _sparse_splits(items, kv_block_num, num_kv_splits, num_sms, two_per_sm, ctas_per_sm=None):
     """Splits of the selected pages in token-major sparse attention, halved as often as pays.  A CTA takes its
     pages and about four page times more (dependent index loads, the first page's latency, the epilogue), the CTAs run in
     rounds of the slots there are (two e4m3 CTAs of at most 16 rows share an SM), and splits cost a merge, about four
@@ -132,7 +133,7 @@ def _sparse_splits(items, kv_block_num, num_kv_splits, num_sms, two_per_sm):
         s = 1
         while s * 2 <= min(kv_block_num, 8) and items * s < 2 * num_sms:
             s *= 2
-    slots = num_sms * (2 if two_per_sm else 1)
+    slots = num_sms * (ctas_per_sm or (2 if two_per_sm else 1))
     best, best_cost = 1, None
     while s >= 1:
         cost = -(-items * s // slots) * (-(-kv_block_num // s) + 4) + (4 if s > 1 else 0)
@@ -263,6 +264,7 @@ def _fmha_sail_plan(
     max_qo_len_override: int = -1,
     qo_len_uniform_override: Optional[bool] = None,
     max_kv_len_override: int = -1,
+    use_kv4_cache: bool = False,
 ):
     """Internal planner (upstream ``_fmha_sail_plan``, api.py:889-1217).
 
@@ -372,7 +374,7 @@ def _fmha_sail_plan(
     info["work"] = info["num_kv_splits_per_row"] = None
     if is_sparse:
         splits = _sparse_splits(total_q * hkv, kv_block_num, num_kv_splits, num_sms,
-                                use_fp8_kvcache and h_r <= 16)
+                                use_fp8_kvcache and h_r <= 16, _KV4_CTAS if use_kv4_cache and h_r <= 16 else None)
         up.add("token_batch", np.repeat(np.arange(batch, dtype=np.int32), a_q))
         up.add("page_batch", np.repeat(np.arange(batch, dtype=np.int32), pages_per))
         info["num_logical_pages"] = int(pages_per.sum())
@@ -398,7 +400,8 @@ def _fmha_sail_plan(
                 info["num_work_tc"] = n_tc
         # Two CTAs of the e4m3 decode kernel share an SM.  A cut at the average load may take more partials than a workspace
         # sized for the plain cut holds: such a workspace gets the plain cut.
-        for ctas in (2 if use_fp8_kvcache and max_qo * pack <= 16 else 1, -1):
+        shared = 1 if max_qo * pack > 16 else (_KV4_CTAS if use_kv4_cache else (2 if use_fp8_kvcache else 1))
+        for ctas in (shared, -1):
             args = _lib.MsaPlanArgs(
                 a_q.ctypes.data, a_k.ctypes.data, a_o.ctypes.data, batch, num_qo_heads, hkv, block_m, pack,
                 num_kv_splits if num_kv_splits >= 1 else -128, num_sms, ctas)
@@ -720,6 +723,9 @@ def _fmha_sail(
         kv_is_nhd, num_kv_heads, page_size = _detect_paged_kv_layout(k.shape, plan_page)
         head_dim_vo = v.shape[3]
         is_paged = True
+    if k.dtype == torch.uint8:
+        return _fmha_sail_kv4(q, k, v, plan_info, kv_indices, kv_block_indexes, q_offset_override, out, max_score, sm_scale,
+                              q_scale, k_scale, v_scale, o_scale, output_maxscore, output_o, check_input_valid, max_score_dtype, lse)
     if head_dim_qk != 128 or head_dim_vo != 128:
         raise ValueError("fmha_sail supports head_dim 128 only")
 
@@ -930,6 +936,139 @@ def _fmha_sail(
     elif kernel_out is not None and kernel_out is not out:
         out.copy_(kernel_out)
     return out, max_score
+
+
+def _fmha_sail_kv4(q, k, v, plan, kv_indices, kv_block_indexes, q_offset_override, out, max_score, sm_scale, q_scale, k_scale, v_scale,
+                   o_scale, output_maxscore, output_o, check_input_valid, max_score_dtype, lse):
+    """``_fmha_sail`` over a cache of ``allocate_kv4_cache``.
+
+    Work items of at most 128 rows (decode; sparse attention where few tokens share a page) read the codes themselves.  Longer
+    queries and scores run on a bf16 copy of the table's pages, which is exact: the products of a prompt take far longer than the
+    copy."""
+    if kv_indices is None:
+        raise ValueError("a 4-bit cache is paged: kv_indices is required")
+    if q.dim() != 3 or q.shape[2] != 128:
+        raise ValueError("fmha_sail supports head_dim 128 only")
+    if q.dtype not in (torch.bfloat16, torch.float8_e4m3fn):
+        raise ValueError(f"fmha_sail on a 4-bit cache requires q in bfloat16 or float8_e4m3fn, got {q.dtype}")
+    nnz_qo, num_qo_heads, _ = q.shape
+    if plan.get("page_size", -1) != cache.KV4_TILE:
+        raise ValueError(f"a 4-bit cache needs a plan with page_size={cache.KV4_TILE}")
+    num_kv_heads = k.shape[1] if k.dim() == 4 else -1
+    cache._check_kv4("k", k)
+    if v is None and output_o:
+        raise ValueError("v is required unless output_o=False")
+    if v is not None and output_o:
+        cache._check_kv4("v", v, num_kv_heads)
+        if v.shape[0] != k.shape[0]:
+            raise ValueError(f"k and v must have the same pages, got {k.shape[0]} and {v.shape[0]}")
+    if kv_indices.dtype != torch.int32 or kv_indices.dim() != 1 or not kv_indices.is_contiguous():
+        raise ValueError("kv_indices must be a contiguous int32 vector")
+    dev = q.device
+    cache._same_device(dev, k=k, v=v if output_o else None, kv_indices=kv_indices, kv_block_indexes=kv_block_indexes, out=out, lse=lse,
+                       max_score=max_score, plan=plan["qo_offset"])
+    if k.shape[0] == 0 and nnz_qo:
+        raise ValueError("the cache has no pages")
+    sparse = kv_block_indexes is not None
+    h_r = num_qo_heads // num_kv_heads
+    rows = plan["max_qo_len"] * plan["pack_factor"]
+    scores = output_maxscore and plan["max_k_tiles"] != -1
+    native = (output_o or not scores) and not scores and plan["pack_factor"] == h_r and (sparse or rows <= 128)
+    if native and sparse and plan["sparse_tc_preferred"] and 128 % h_r == 0 and kv_block_indexes.shape[2] <= 32:
+        native = False                        # the page-major kernel, on the copy
+    # the checks of the plan against the call, and of the other arguments, are those of any call
+    if plan["_host"] is None:
+        if nnz_qo > plan["total_qo_len"]:
+            raise ValueError(f"plan allows at most {plan['total_qo_len']} query tokens, q has {nnz_qo}")
+    elif plan["total_qo_len"] != nnz_qo:
+        raise ValueError(f"plan was made for {plan['total_qo_len']} query tokens, q has {nnz_qo}")
+    if not native:
+        with cache._on(dev):
+            table = torch.arange(kv_indices.shape[0], dtype=torch.int32, device=dev)
+            kb = cache.unpack_pages(k, kv_indices)
+            vb = cache.unpack_pages(v, kv_indices) if output_o or not scores else kb
+            return _fmha_sail(q if q.dtype == torch.bfloat16 else q.to(torch.bfloat16), kb, vb, plan, table, kv_block_indexes, q_offset_override, out,
+                              max_score, sm_scale, q_scale, k_scale, v_scale, o_scale, output_maxscore, output_o, check_input_valid,
+                              max_score_dtype, lse)
+    if plan["orig_num_qo_heads"] != num_qo_heads or plan["num_kv_heads"] != num_kv_heads:
+        raise ValueError("plan head counts do not match q / k")
+    if plan["is_sparse"] != sparse:
+        raise ValueError("plan sparse mode (kv_block_num) does not match kv_block_indexes")
+    qo_offset = plan["qo_offset"] if q_offset_override is None else q_offset_override
+    if isinstance(qo_offset, int):
+        if plan.get("graph_safe", False):
+            raise ValueError("graph_safe=True requires q_offset_override as a CUDA tensor; an int triggers an in-capture torch.full_like allocation")
+        qo_offset = torch.full_like(plan["qo_segment_lens"], qo_offset)
+    else:
+        cache._same_device(dev, qo_offset=qo_offset)
+        if qo_offset.dtype != torch.int32:
+            qo_offset = qo_offset.to(torch.int32)
+    if check_input_valid and plan["_host"] is not None:
+        _validate_fmha_inputs(q, k, v, plan, True, False, num_kv_heads, cache.KV4_TILE, kv_indices, kv_block_indexes, qo_offset)
+    if sm_scale is None:
+        sm_scale = 1.0 / math.sqrt(128)
+    q_s, _ = _scale_arg(q_scale, dev, num_kv_heads)
+    k_s, k_head = _scale_arg(k_scale, dev, num_kv_heads)
+    v_s, v_head = _scale_arg(v_scale, dev, num_kv_heads)
+    o_s, _ = _scale_arg(o_scale, dev, num_kv_heads)
+    if out is None:
+        out = torch.empty(nnz_qo, num_qo_heads, 128, device=dev, dtype=torch.bfloat16)
+    else:
+        assert out.dtype in (torch.bfloat16, torch.float32) and out.shape == (nnz_qo, num_qo_heads, 128)
+        assert out.stride(2) == 1
+    if lse is not None:
+        assert lse.dtype == torch.float32 and lse.is_contiguous() and lse.shape == (nnz_qo, num_qo_heads)
+    if nnz_qo == 0:
+        return out, None
+    assert q.stride(2) == 1, "q head_dim must be contiguous"
+    splits = plan["num_kv_splits"]
+    p = _lib.MsaFmhaParams()
+    p.q, p.k, p.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
+    p.q_stride_tok, p.q_stride_head = q.stride(0), q.stride(1)
+    p.k_stride_page, p.k_stride_head = k.stride(0), k.stride(1)
+    p.v_stride_page, p.v_stride_head = v.stride(0), v.stride(1)
+    p.kv_indices, p.kv_page_indptr, p.page_size = kv_indices.data_ptr(), plan["kv_page_indptr"].data_ptr(), cache.KV4_TILE
+    p.qo_start, p.kv_len, p.qo_offset = plan["qo_segment_offsets"].data_ptr(), plan["kv_segment_lens"].data_ptr(), qo_offset.data_ptr()
+    if sparse:
+        assert kv_block_indexes.dtype == torch.int32
+        if kv_block_indexes.dim() != 3 or kv_block_indexes.shape[:2] != (nnz_qo, num_kv_heads) or kv_block_indexes.stride(2) != 1:
+            raise ValueError(f"kv_block_indexes must be [total_qo_len, H_kv={num_kv_heads}, KVBlockNum], got {tuple(kv_block_indexes.shape)}")
+        p.kv_block_indexes, p.kv_block_num = kv_block_indexes.data_ptr(), kv_block_indexes.shape[2]
+        p.kbi_stride_tok, p.kbi_stride_head = kv_block_indexes.stride(0), kv_block_indexes.stride(1)
+        p.token_batch = plan["token_batch"].data_ptr()
+    else:
+        p.work, p.num_work = _ptr(plan["work"]), plan["num_work"]
+        p.decode_rows = rows
+    p.k_scale_head, p.v_scale_head = _ptr(k_head), _ptr(v_head)
+    p.total_q, p.num_qo_heads, p.num_kv_heads, p.batch = nnz_qo, num_qo_heads, num_kv_heads, plan["batch_size"]
+    p.block_m, p.pack, p.kv_extent = plan["qo_tile_size"], plan["pack_factor"], k.shape[0]
+    p.status = _status_word(dev).data_ptr()
+    p.q_dtype, p.kv_dtype = _dt_code(q.dtype), MSA_DT_KV4
+    p.flags = FLAG_OUT_O | (FLAG_SPARSE if sparse else 0)
+    p.sm_scale, p.out_scale = float(q_s * k_s * sm_scale), float(v_s * o_s)
+    if _SHOW_PARAMS:
+        _show_params(q, plan, True, cache.KV4_TILE, float(sm_scale), True, None, kv_block_indexes)
+    with cache._on(dev):
+        stream = _stream()
+        # partials of its own: two streams, or two captured graphs, may run one plan at the same time
+        kernel_out = out
+        if splits > 1:
+            part = torch.empty(splits * nnz_qo * num_qo_heads * 129, dtype=torch.float32, device=dev)
+            p.partial_o, p.num_splits = part.data_ptr(), splits
+            p.partial_lse = part.data_ptr() + splits * nnz_qo * num_qo_heads * 512
+        else:
+            if out.dtype == torch.float32:
+                kernel_out = torch.empty(out.shape, dtype=torch.bfloat16, device=dev)
+            p.num_splits, p.lse = 1, _ptr(lse)
+            p.out, p.out_stride_tok, p.out_stride_head = kernel_out.data_ptr(), kernel_out.stride(0), kernel_out.stride(1)
+        _lib.check(_lib.lib.msa_fmha_fwd(ctypes.byref(p), stream), "msa_fmha_fwd")
+        if splits > 1:
+            _lib.check(_lib.lib.msa_lse_merge_ex(
+                p.partial_o, MSA_DT_F32, p.partial_lse, _ptr(plan["num_kv_splits_per_row"]), out.data_ptr(), _dt_code(out.dtype), _ptr(lse),
+                splits, nnz_qo, num_qo_heads, 0, 0, out.stride(0), out.stride(1), float(v_s * o_s), stream), "msa_lse_merge_ex")
+        elif kernel_out is not out:
+            out.copy_(kernel_out)
+    return out, None
 
 
 def _decode_prefix(qo_segment_lens, sparse):

@@ -1,0 +1,494 @@
+"""Operators around the attention call of a serving step: page tables, norm and rotation with the cache write, 4-bit caches.
+
+* ``paged_kv_tables``: the flat page table, slots and positions of a step from the requests' lengths, on the GPU;
+* ``rope_plan`` / ``qk_norm_rope``: per-head norm of queries and keys, rotary positions (one axis or several) and the write of keys
+  and values into the paged cache, in one pass;
+* ``kv_cache_append``: the write alone;
+* ``allocate_kv4_cache`` / ``kv4_read``: a cache that holds 4 bits a value; ``fmha_sail`` takes it as ``k`` and ``v``.
+
+None of them has an upstream counterpart (upstream starts at the attention call, api.py:1480-1848).  All of them enqueue on the
+current stream of their tensors' device and read nothing back; what is allocated comes from torch's caching allocator, so
+they can be captured into CUDA graphs.
+"""
+import contextlib
+import ctypes
+import math
+from fractions import Fraction
+from typing import Optional, Sequence, Tuple, Union
+
+import torch
+
+from . import _lib
+from ._lib import MSA_DT_BF16, MSA_DT_E4M3, MSA_DT_F32, MSA_DT_KV4
+
+KV4_TILE = 128                          # tokens of a page
+KV4_ROW_BYTES = 72                      # 64 bytes of codes and 8 scales
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _stream():
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+
+
+def _on(device):
+    """A context in which `device` is the current one."""
+    return contextlib.nullcontext() if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
+
+
+def _same_device(device, **tensors):
+    for name, t in tensors.items():
+        if t is not None and t.device != device:
+            raise ValueError(f"{name} is on {t.device}, expected {device}")
+
+
+def _is_kv4(t):
+    return t is not None and t.dtype == torch.uint8
+
+
+# ----------------------------------------------------------------------------
+# 4-bit cache
+# ----------------------------------------------------------------------------
+
+def allocate_kv4_cache(num_pages: int, num_kv_heads: int, page_size: int = 128, device=None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Keys' and values' caches of 4 bits a value: two uint8 tensors ``[num_pages, num_kv_heads, 128, 72]``, zeros.
+
+    The 9 216 bytes of one page and head are one tile: 128 rows of 64 bytes (two e2m1 codes a byte, the even element in the low half),
+    then 128 rows of eight e4m3 scales, one for each 16 elements (so the last two dimensions are not rows of 72 bytes).  Views
+    of a larger allocation serve as well where the tiles stay contiguous and start at multiples of 16 bytes."""
+    if page_size != KV4_TILE:
+        raise ValueError(f"a 4-bit cache has pages of {KV4_TILE} tokens, got page_size={page_size}")
+    if num_pages < 0 or num_kv_heads < 1:
+        raise ValueError(f"num_pages={num_pages} must not be negative, num_kv_heads={num_kv_heads} must be positive")
+    device = torch.cuda.current_device() if device is None else device
+    shape = (num_pages, num_kv_heads, KV4_TILE, KV4_ROW_BYTES)
+    return torch.zeros(shape, dtype=torch.uint8, device=device), torch.zeros(shape, dtype=torch.uint8, device=device)
+
+
+def _check_kv4(name, t, num_kv_heads=None):
+    if t.dim() != 4 or t.dtype != torch.uint8 or tuple(t.shape[2:]) != (KV4_TILE, KV4_ROW_BYTES):
+        raise ValueError(f"{name}: a 4-bit cache is uint8 [pages, Hkv, {KV4_TILE}, {KV4_ROW_BYTES}], got {t.dtype} {tuple(t.shape)}")
+    if t.stride(3) != 1 or t.stride(2) != KV4_ROW_BYTES:
+        raise ValueError(f"{name}: the tile of a page and head of a 4-bit cache must be contiguous")
+    if t.stride(0) % 16 or t.stride(1) % 16 or t.data_ptr() % 16:
+        raise ValueError(f"{name}: the tiles of a 4-bit cache must start at multiples of 16 bytes")
+    if num_kv_heads is not None and t.shape[1] != num_kv_heads:
+        raise ValueError(f"{name} has {t.shape[1]} KV heads, expected {num_kv_heads}")
+
+
+def _status(device):
+    from .api import _status_word
+    return _status_word(device).data_ptr()
+
+
+def _read(cache, index, out, whole_pages):
+    if index.shape[0] == 0:
+        return out
+    if cache.shape[0] == 0:
+        return out.zero_()
+    a = _lib.MsaKv4ReadArgs()
+    a.cache, a.out, a.slot_map, a.status = cache.data_ptr(), out.data_ptr(), index.data_ptr(), _status(cache.device)
+    a.stride_page, a.stride_head = cache.stride(0), cache.stride(1)
+    a.rows, a.num_kv_heads, a.num_pages, a.whole_pages = index.shape[0], cache.shape[1], cache.shape[0], int(whole_pages)
+    with _on(cache.device):
+        _lib.check(_lib.lib.msa_kv4_read(ctypes.byref(a), _stream()), "msa_kv4_read")
+    return out
+
+
+def _check_index(name, t, device):
+    if t.dim() != 1 or t.dtype != torch.int32 or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 vector, got {t.dtype} {tuple(t.shape)}")
+    _same_device(device, **{name: t})
+
+
+def kv4_read(cache: torch.Tensor, slot_map: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Rows of a 4-bit cache as bf16 ``[tokens, Hkv, 128]`` (exact: code times scale; a scale per head is not applied).
+
+    ``slot_map``: int32, ``page * 128 + offset`` of each token; rows of a negative slot are zeros."""
+    _check_kv4("cache", cache)
+    if not cache.is_cuda:
+        raise RuntimeError("kv4_read needs CUDA tensors (there is no CPU path)")
+    _check_index("slot_map", slot_map, cache.device)
+    shape = (slot_map.shape[0], cache.shape[1], 128)
+    if out is None:
+        out = torch.empty(shape, dtype=torch.bfloat16, device=cache.device)
+    else:
+        _same_device(cache.device, out=out)
+        if out.dtype != torch.bfloat16 or tuple(out.shape) != shape or not out.is_contiguous():
+            raise ValueError(f"out must be contiguous bf16 {shape}, got {out.dtype} {tuple(out.shape)}")
+    return _read(cache, slot_map, out, False)
+
+
+def unpack_pages(cache, kv_indices):
+    """Pages of a 4-bit cache as bf16 ``[len(kv_indices), Hkv, 128, 128]``; pages outside the cache are left as they were."""
+    out = torch.empty(kv_indices.shape[0], cache.shape[1], KV4_TILE, 128, dtype=torch.bfloat16, device=cache.device)
+    return _read(cache, kv_indices, out, True)
+
+
+# ----------------------------------------------------------------------------
+# norm, rotation, cache write
+# ----------------------------------------------------------------------------
+
+class RopePlan(dict):
+    """Frequencies of a rotation, prepared by ``rope_plan``; pass it unchanged to ``qk_norm_rope``."""
+
+
+def rope_plan(rotary_dim: int = 128, base: float = 10000.0, inv_freq: Optional[Union[torch.Tensor, Sequence[float]]] = None,
+              sections: Optional[Sequence[int]] = None, interleaved: bool = False, device=None) -> RopePlan:
+    """Frequencies of a rotary embedding over the first ``rotary_dim`` elements of a head (a multiple of 16, at most 128).
+
+    ``inv_freq``: the angle per position of each of the ``rotary_dim / 2`` pairs (scaled variants bring their own); default
+    ``base ** (-2 i / rotary_dim)``.  ``sections``: pairs of each position axis, in order (time, height, width of a video token:
+    three numbers that add up to ``rotary_dim / 2``); default one axis.  ``interleaved``: pairs are neighbours (2 i, 2 i + 1)
+    instead of (i, i + rotary_dim / 2).
+
+    Frequencies are kept as 64-bit fractions of a turn, so angles are exact at any position."""
+    if rotary_dim % 16 or not 0 < rotary_dim <= 128:
+        raise ValueError(f"rotary_dim must be a multiple of 16 in (0, 128], got {rotary_dim}")
+    pairs = rotary_dim // 2
+    if inv_freq is None:
+        inv_freq = [base ** (-2 * i / rotary_dim) for i in range(pairs)]
+    else:
+        inv_freq = inv_freq.detach().double().cpu().tolist() if isinstance(inv_freq, torch.Tensor) else [float(x) for x in inv_freq]
+    if len(inv_freq) != pairs:
+        raise ValueError(f"inv_freq must have rotary_dim / 2 = {pairs} entries, got {len(inv_freq)}")
+    if not all(math.isfinite(f) for f in inv_freq):
+        raise ValueError("inv_freq must be finite")
+    sections = [pairs] if sections is None else [int(n) for n in sections]
+    if sum(sections) != pairs or min(sections) < 0:
+        raise ValueError(f"sections must add up to rotary_dim / 2 = {pairs}, got {sections}")
+    turns = []
+    for f in inv_freq:
+        n = round(Fraction(f) / _TWO_PI * (1 << 64)) % (1 << 64)
+        turns.append(n - (1 << 64) if n >= 1 << 63 else n)
+    axis = [i for i, n in enumerate(sections) for _ in range(n)]
+    device = torch.cuda.current_device() if device is None else device
+    return RopePlan(rotary_dim=rotary_dim, interleaved=bool(interleaved), axes=len(sections),
+                    turns=torch.tensor(turns, dtype=torch.int64, device=device), axis=torch.tensor(axis, dtype=torch.int32, device=device))
+
+
+# 2 pi to 39 digits: a frequency in turns is then as exact as the frequency
+_TWO_PI = Fraction(6283185307179586476925286766559005768394, 10 ** 39)
+
+
+def _rows(name, t, heads=None, tokens=None, dtypes=(torch.bfloat16,)):
+    if t.dim() != 3 or t.shape[2] != 128:
+        raise ValueError(f"{name} must be [tokens, heads, 128], got {tuple(t.shape)}")
+    if t.dtype not in dtypes:
+        raise ValueError(f"{name} must be {' or '.join(str(d) for d in dtypes)}, got {t.dtype}")
+    if t.stride(2) != 1:
+        raise ValueError(f"{name} head_dim must be contiguous")
+    unit = 8 * t.element_size()
+    if t.data_ptr() % unit or (t.stride(0) * t.element_size()) % unit or (t.stride(1) * t.element_size()) % unit:
+        raise ValueError(f"{name}: rows must start at multiples of {unit} bytes")
+    if (heads is not None and t.shape[1] != heads) or (tokens is not None and t.shape[0] != tokens):
+        raise ValueError(f"{name} must be [{tokens}, {heads}, 128], got {tuple(t.shape)}")
+
+
+def _weight(name, w, heads, device):
+    if w is None:
+        return None, 0
+    _same_device(device, **{name: w})
+    if w.dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError(f"{name} must be float32 or bfloat16, got {w.dtype}")
+    if tuple(w.shape) not in ((128,), (heads, 128)):
+        raise ValueError(f"{name} must be [128] or [{heads}, 128], got {tuple(w.shape)}")
+    if w.stride(-1) != 1 or (w.dim() == 2 and w.stride(0) % 8) or w.data_ptr() % 16:
+        raise ValueError(f"{name}: rows must be contiguous and start at multiples of 16 bytes")
+    return w.data_ptr(), w.stride(0) if w.dim() == 2 else 0
+
+
+def _scale(name, x, heads, device):
+    """A scale is a float, or an fp32 tensor with one value per KV head (it stays on the device)."""
+    if x is None:
+        return 1.0, None
+    if isinstance(x, torch.Tensor):
+        _same_device(device, **{name: x})
+        if x.dtype != torch.float32 or x.numel() != heads or not x.is_contiguous():
+            raise ValueError(f"{name} must be a float or a contiguous float32 tensor of {heads} values, got {x.dtype} {tuple(x.shape)}")
+        return 1.0, x.data_ptr()
+    return float(x), None
+
+
+def _cache_args(a, k_cache, v_cache, heads, slot_map, tokens, page_size, device):
+    """Fills the fields of the caches; both have the same type, layout and page count."""
+    first = k_cache if k_cache is not None else v_cache
+    if slot_map is None:
+        raise ValueError("a cache needs slot_map")
+    _check_index("slot_map", slot_map, device)
+    if slot_map.shape[0] != tokens:
+        raise ValueError(f"slot_map must have {tokens} entries, got {slot_map.shape[0]}")
+    _same_device(device, k_cache=k_cache, v_cache=v_cache)
+    if k_cache is not None and v_cache is not None and (k_cache.dtype != v_cache.dtype or k_cache.shape != v_cache.shape):
+        raise ValueError(f"k_cache and v_cache must be alike, got {k_cache.dtype} {tuple(k_cache.shape)} and {v_cache.dtype} {tuple(v_cache.shape)}")
+    codes = {torch.bfloat16: MSA_DT_BF16, torch.float8_e4m3fn: MSA_DT_E4M3, torch.uint8: MSA_DT_KV4}
+    if first.dtype not in codes:
+        raise ValueError(f"a cache is bfloat16, float8_e4m3fn or uint8 (4 bits), got {first.dtype}")
+    a.cache_dtype = codes[first.dtype]
+    for name, c in (("k_cache", k_cache), ("v_cache", v_cache)):
+        if c is None:
+            continue
+        if a.cache_dtype == MSA_DT_KV4:
+            _check_kv4(name, c, heads)
+            strides, size = (c.stride(0), c.stride(1), 0), KV4_TILE
+        else:
+            if c.dim() != 4 or c.shape[3] != 128 or c.stride(3) != 1:
+                raise ValueError(f"{name} must be [pages, Hkv, page, 128] or [pages, page, Hkv, 128], got {tuple(c.shape)}")
+            unit = 8 * c.element_size()
+            if c.data_ptr() % unit or any((c.stride(i) * c.element_size()) % unit for i in range(3)):
+                raise ValueError(f"{name}: rows must start at multiples of {unit} bytes")
+            if c.shape[2] == page_size and c.shape[1] == heads:
+                strides = (c.stride(0), c.stride(1), c.stride(2))
+            elif c.shape[1] == page_size and c.shape[2] == heads:
+                strides = (c.stride(0), c.stride(2), c.stride(1))
+            else:
+                raise ValueError(f"{name} must hold pages of {page_size} tokens and {heads} KV heads, got {tuple(c.shape)}")
+            size = page_size
+        if name == "k_cache":
+            a.k_cache, (a.k_cache_stride_page, a.k_cache_stride_head, a.k_cache_stride_tok) = c.data_ptr(), strides
+        else:
+            a.v_cache, (a.v_cache_stride_page, a.v_cache_stride_head, a.v_cache_stride_tok) = c.data_ptr(), strides
+        if size != page_size:
+            raise ValueError(f"a 4-bit cache has pages of {KV4_TILE} tokens, got page_size={page_size}")
+    if first.shape[0] * page_size > (1 << 31) - 1:
+        raise ValueError("slots of a cache of more than 2^31 - 1 tokens do not fit int32")
+    a.slot_map, a.page_size, a.num_pages = slot_map.data_ptr(), page_size, first.shape[0]
+
+
+def _cache_scales(a, cache, k_scale, v_scale, heads, device):
+    if cache is None or cache.dtype == torch.bfloat16:
+        if k_scale is not None or v_scale is not None:
+            raise ValueError("k_scale and v_scale belong to a quantised cache")
+    a.k_scale, a.k_scale_head = _scale("k_scale", k_scale, heads, device)
+    a.v_scale, a.v_scale_head = _scale("v_scale", v_scale, heads, device)
+
+
+def qk_norm_rope(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    positions: Optional[torch.Tensor],
+    rope: Optional[RopePlan],
+    *,
+    v: Optional[torch.Tensor] = None,
+    norm: bool = True,
+    q_weight: Optional[torch.Tensor] = None,
+    k_weight: Optional[torch.Tensor] = None,
+    eps: float = 1e-6,
+    q_out: Optional[torch.Tensor] = None,
+    k_out: Optional[torch.Tensor] = None,
+    q_scale: Optional[float] = None,
+    k_cache: Optional[torch.Tensor] = None,
+    v_cache: Optional[torch.Tensor] = None,
+    slot_map: Optional[torch.Tensor] = None,
+    page_size: int = 128,
+    k_scale=None,
+    v_scale=None,
+) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """Norm every query and key head, rotate them, and write keys and values into the paged cache, in one pass.
+
+    ``q [T, Hq, 128]``, ``k [T, Hkv, 128]`` bf16, any strides whose rows start at multiples of 16 bytes (slices of a fused projection's
+    output).  ``norm``: ``x / sqrt(mean(x^2) + eps) * weight`` over each head; weights ``[128]`` or one row per head, float32 or
+    bf16.  ``rope`` (from ``rope_plan``, None: no rotation) turns the pairs of a head by ``positions``: int32 or int64, ``[T]``, or
+    ``[axes, T]`` where the plan has several axes.
+
+    Without caches returns ``(q, k)`` in bf16.  With ``k_cache``, ``v_cache`` and ``v`` the rows go to ``slot_map[t]`` (int32,
+    ``page * page_size + offset``; a negative slot writes nothing; slots of one call are distinct) and the result is ``(q, None)``,
+    or ``(q, k_out)`` where that is given.  Caches are bf16 or e4m3 (HND or NHD, as ``fmha_sail`` takes them) or 4-bit
+    (``allocate_kv4_cache``); keys are rounded to bf16 before they are quantised.  ``k_scale`` / ``v_scale`` (quantised caches): what
+    the attention call will multiply by, a float or one float32 value per KV head.  ``q_out`` may be ``q`` (in place) or
+    float8_e4m3fn (then ``q / q_scale`` is stored)."""
+    if not q.is_cuda:
+        raise RuntimeError("qk_norm_rope needs CUDA tensors (there is no CPU path)")
+    dev = q.device
+    _rows("q", q)
+    T, hq = q.shape[0], q.shape[1]
+    _rows("k", k, tokens=T, heads=k.shape[1] if k.dim() == 3 else None)
+    hk = k.shape[1]
+    _same_device(dev, k=k, v=v, positions=positions, q_out=q_out, k_out=k_out)
+    a = _lib.MsaNormRopeArgs()
+    if rope is not None:
+        if positions is None:
+            raise ValueError("a rotation needs positions")
+        if positions.dtype not in (torch.int32, torch.int64):
+            raise ValueError(f"positions must be int32 or int64, got {positions.dtype}")
+        if tuple(positions.shape) != (rope["axes"], T) and not (rope["axes"] == 1 and tuple(positions.shape) == (T,)):
+            raise ValueError(f"positions must be [{rope['axes']}, {T}]" + (f" or [{T}]" if rope["axes"] == 1 else "") + f", got {tuple(positions.shape)}")
+        if T and positions.stride(-1) != 1 and T > 1:
+            raise ValueError("positions of one axis must be contiguous")
+        _same_device(dev, rope=rope["turns"])
+        a.positions, a.pos_int64 = positions.data_ptr(), int(positions.dtype == torch.int64)
+        a.pos_stride_axis = positions.stride(0) if positions.dim() == 2 else 0
+        a.turns, a.axis = rope["turns"].data_ptr(), rope["axis"].data_ptr()
+        a.rotary, a.interleaved = rope["rotary_dim"], int(rope["interleaved"])
+    if (k_cache is None) != (v_cache is None) or (v_cache is None) != (v is None):
+        raise ValueError("k_cache, v_cache and v go together")
+    if k_cache is not None:
+        _rows("v", v, tokens=T, heads=hk)
+        a.v, a.v_stride_tok, a.v_stride_head = v.data_ptr(), v.stride(0), v.stride(1)
+        _cache_args(a, k_cache, v_cache, hk, slot_map, T, page_size, dev)
+    _cache_scales(a, k_cache, k_scale, v_scale, hk, dev)
+    if q_out is None:
+        q_out = torch.empty(T, hq, 128, dtype=torch.bfloat16, device=dev)
+    else:
+        _rows("q_out", q_out, heads=hq, tokens=T, dtypes=(torch.bfloat16, torch.float8_e4m3fn))
+    if q_scale is not None and q_out.dtype != torch.float8_e4m3fn:
+        raise ValueError("q_scale belongs to an e4m3 q_out")
+    if k_out is None and k_cache is None:
+        k_out = torch.empty(T, hk, 128, dtype=torch.bfloat16, device=dev)
+    elif k_out is not None:
+        _rows("k_out", k_out, heads=hk, tokens=T)
+    a.q, a.q_stride_tok, a.q_stride_head = q.data_ptr(), q.stride(0), q.stride(1)
+    a.k, a.k_stride_tok, a.k_stride_head = k.data_ptr(), k.stride(0), k.stride(1)
+    a.q_out, a.q_out_stride_tok, a.q_out_stride_head = q_out.data_ptr(), q_out.stride(0), q_out.stride(1)
+    a.q_out_dtype = MSA_DT_E4M3 if q_out.dtype == torch.float8_e4m3fn else MSA_DT_BF16
+    if k_out is not None:
+        a.k_out, a.k_out_stride_tok, a.k_out_stride_head = k_out.data_ptr(), k_out.stride(0), k_out.stride(1)
+    if not norm and (q_weight is not None or k_weight is not None):
+        raise ValueError("weights belong to the norm")
+    if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
+        raise ValueError(f"q_weight and k_weight must have one dtype, got {q_weight.dtype} and {k_weight.dtype}")
+    a.q_weight, a.q_weight_stride = _weight("q_weight", q_weight, hq, dev)
+    a.k_weight, a.k_weight_stride = _weight("k_weight", k_weight, hk, dev)
+    w = q_weight if q_weight is not None else k_weight
+    a.weight_dtype = MSA_DT_BF16 if w is not None and w.dtype == torch.bfloat16 else MSA_DT_F32
+    a.tokens, a.num_qo_heads, a.num_kv_heads, a.norm, a.eps = T, hq, hk, int(bool(norm)), float(eps)
+    a.q_scale = 1.0 if q_scale is None else float(q_scale)
+    a.status = _status(dev)
+    if T == 0:
+        return q_out, k_out
+    with _on(dev):
+        _lib.check(_lib.lib.msa_norm_rope(ctypes.byref(a), _stream()), "msa_norm_rope")
+    return q_out, k_out
+
+
+def kv_cache_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, slot_map: torch.Tensor,
+                    page_size: int = 128, k_scale=None, v_scale=None) -> None:
+    """Write keys and values that are ready (``[T, Hkv, 128]`` bf16) into the paged cache at ``slot_map``; caches, slots and scales
+    as in ``qk_norm_rope``."""
+    if not k.is_cuda:
+        raise RuntimeError("kv_cache_append needs CUDA tensors (there is no CPU path)")
+    dev = k.device
+    _rows("k", k)
+    T, hk = k.shape[0], k.shape[1]
+    _rows("v", v, heads=hk, tokens=T)
+    _same_device(dev, v=v)
+    a = _lib.MsaNormRopeArgs()
+    _cache_args(a, k_cache, v_cache, hk, slot_map, T, page_size, dev)
+    _cache_scales(a, k_cache, k_scale, v_scale, hk, dev)
+    a.k, a.k_stride_tok, a.k_stride_head = k.data_ptr(), k.stride(0), k.stride(1)
+    a.v, a.v_stride_tok, a.v_stride_head = v.data_ptr(), v.stride(0), v.stride(1)
+    a.tokens, a.num_kv_heads, a.weight_dtype, a.status = T, hk, MSA_DT_F32, _status(dev)
+    if T == 0:
+        return
+    with _on(dev):
+        _lib.check(_lib.lib.msa_norm_rope(ctypes.byref(a), _stream()), "msa_norm_rope")
+
+
+# ----------------------------------------------------------------------------
+# page tables
+# ----------------------------------------------------------------------------
+
+class PageTables(dict):
+    """Tensors of a step's paged cache, made by ``paged_kv_tables``."""
+
+
+def paged_kv_tables(
+    qo_lens: torch.Tensor,
+    kv_lens: torch.Tensor,
+    block_table: torch.Tensor,
+    num_held: Optional[torch.Tensor] = None,
+    free_pages: Optional[torch.Tensor] = None,
+    num_free: Optional[torch.Tensor] = None,
+    *,
+    max_total_q: int,
+    max_total_pages: Optional[int] = None,
+    page_size: int = 128,
+    num_held_out: Optional[torch.Tensor] = None,
+    num_free_out: Optional[torch.Tensor] = None,
+    out: Optional[PageTables] = None,
+) -> PageTables:
+    """Page table, slots and positions of a step, built on the GPU from the requests' lengths (no host read, graph-safe).
+
+    ``qo_lens`` / ``kv_lens``: int32 ``[B]``, the new tokens of each request and its keys with them (as ``fmha_sail_plan`` takes them).
+    ``block_table``: int32 ``[B, width]``, the physical page of each logical page.  With ``num_held`` (int32 ``[B]``: entries of each
+    row that are set), ``free_pages`` (int32, a stack) and ``num_free`` (int32 ``[1]``) the pages that new tokens need are taken
+    from the top of the stack, in the order of the requests, and written into ``block_table``; without them the rows are complete.
+
+    Returns ``kv_indices`` (``[max_total_pages]``, default ``B * width``; -1 behind the last page) and ``kv_page_indptr`` for the attention
+    call, ``slot_map`` (``[max_total_q]``, -1 behind the last token) for the cache write, ``positions`` for the rotation, ``num_held``
+    and ``num_free`` (the counts after this step; pass ``num_held_out=num_held, num_free_out=num_free`` to update in place) and
+    ``num_missing``: pages and tokens that found no place.  Where that is not zero, missing pages are 0 in ``kv_indices`` and
+    their tokens' slots -1: nothing goes out of bounds, but attention over such a request means nothing.
+
+    ``out``: a former result of the same sizes, whose tensors are written again (a captured step's fixed addresses)."""
+    if not qo_lens.is_cuda:
+        raise RuntimeError("paged_kv_tables needs CUDA tensors (there is no CPU path)")
+    dev = qo_lens.device
+    _check_index("qo_lens", qo_lens, dev)
+    _check_index("kv_lens", kv_lens, dev)
+    B = qo_lens.shape[0]
+    if kv_lens.shape[0] != B:
+        raise ValueError(f"qo_lens and kv_lens must have the same length, got {B} and {kv_lens.shape[0]}")
+    if block_table.dim() != 2 or block_table.dtype != torch.int32 or block_table.shape[0] != B or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
+        raise ValueError(f"block_table must be int32 [{B}, width] with contiguous rows, got {block_table.dtype} {tuple(block_table.shape)}")
+    if B > 1 and block_table.stride(0) < block_table.shape[1]:
+        raise ValueError("rows of block_table must not overlap")
+    if page_size < 1 or max_total_q < 0:
+        raise ValueError(f"page_size={page_size} must be positive, max_total_q={max_total_q} must not be negative")
+    alloc = num_held is not None
+    if alloc != (free_pages is not None) or alloc != (num_free is not None):
+        raise ValueError("num_held, free_pages and num_free go together")
+    if not alloc and (num_held_out is not None or num_free_out is not None):
+        raise ValueError("num_held_out and num_free_out need num_held, free_pages and num_free")
+    width = block_table.shape[1]
+    total_pages = B * width if max_total_pages is None else int(max_total_pages)
+    if total_pages < 0 or total_pages > (1 << 31) - 1 or max_total_q > (1 << 31) - 1:
+        raise ValueError(f"max_total_pages={total_pages} and max_total_q={max_total_q} must fit int32")
+    sizes = {"kv_indices": total_pages, "kv_page_indptr": B + 1, "slot_map": max_total_q, "positions": max_total_q, "num_missing": 1}
+    if alloc:
+        for name, t, n in (("num_held", num_held, B), ("free_pages", free_pages, None), ("num_free", num_free, 1),
+                           ("num_held_out", num_held_out, B), ("num_free_out", num_free_out, 1)):
+            if t is None:
+                continue
+            _check_index(name, t, dev)
+            if n is not None and t.shape[0] != n:
+                raise ValueError(f"{name} must have {n} entries, got {t.shape[0]}")
+        sizes.update(num_held=B, num_free=1)
+    _same_device(dev, block_table=block_table)
+    if out is not None:
+        for name, n in sizes.items():
+            _check_index(f"out[{name!r}]", out[name], dev)
+            if out[name].shape[0] != n:
+                raise ValueError(f"out[{name!r}] must have {n} entries, got {out[name].shape[0]}")
+    res = PageTables()
+    given = {"num_held": num_held_out, "num_free": num_free_out}
+    need = [(name, n) for name, n in sizes.items() if given.get(name) is None and out is None]
+    ws_bytes = _lib.check(_lib.lib.msa_page_tables_workspace_bytes(B), "msa_page_tables_workspace_bytes")
+    with _on(dev):
+        # one allocation for the outputs (each on a 256-byte boundary) and the scans
+        at, total = {}, 0
+        for name, n in need + [("", ws_bytes // 4)]:
+            at[name] = total
+            total += (n + 63) & ~63
+        block = torch.empty(total, dtype=torch.int32, device=dev)
+        for name, n in sizes.items():
+            if given.get(name) is not None:
+                res[name] = given[name]
+            else:
+                res[name] = out[name] if out is not None else block[at[name]:at[name] + n]
+        a = _lib.MsaPageTablesArgs()
+        a.qo_len, a.kv_len, a.block_table = qo_lens.data_ptr(), kv_lens.data_ptr(), block_table.data_ptr()
+        a.kv_indices, a.kv_page_indptr = res["kv_indices"].data_ptr(), res["kv_page_indptr"].data_ptr()
+        a.slot_map, a.positions, a.num_missing = res["slot_map"].data_ptr(), res["positions"].data_ptr(), res["num_missing"].data_ptr()
+        if alloc:
+            a.num_held, a.free_pages, a.num_free = num_held.data_ptr(), free_pages.data_ptr(), num_free.data_ptr()
+            a.num_held_out, a.num_free_out = res["num_held"].data_ptr(), res["num_free"].data_ptr()
+            a.free_capacity = free_pages.shape[0]
+        a.workspace = block.data_ptr() + 4 * at[""]
+        a.table_stride = block_table.stride(0) if B > 1 else width
+        a.batch, a.table_width, a.page_size = B, width, page_size
+        a.max_total_q, a.max_total_pages = max_total_q, total_pages
+        _lib.check(_lib.lib.msa_page_tables(ctypes.byref(a), _stream()), "msa_page_tables")
+    return res
