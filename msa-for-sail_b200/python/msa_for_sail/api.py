@@ -25,7 +25,6 @@ __all__ = [
 ]
 
 KV_TILE = 128
-_KV4_CTAS = 3                           # CTAs of the 4-bit decode kernel that share an SM
 _USE_TC = True                          # route eligible prefill shapes to the tcgen05 kernel
 _FORCE_TC = False                       # ... even when the planner would rather split KV
 _USE_DECODE_TC = True                   # tcgen05 decode kernel for short-query bf16 shapes
@@ -141,6 +140,11 @@ def _sparse_splits(items, kv_block_num, num_kv_splits, num_sms, two_per_sm, ctas
             best, best_cost = s, cost
         s //= 2
     return best
+
+
+def _kv4_ctas(rows):
+    """CTAs of the 4-bit decode kernel that share an SM, by the rows of a work item (groups of 16 are CTAs of their own)."""
+    return 4 if rows <= 8 else 3
 
 
 def _block_m(rows):
@@ -374,7 +378,7 @@ def _fmha_sail_plan(
     info["work"] = info["num_kv_splits_per_row"] = None
     if is_sparse:
         splits = _sparse_splits(total_q * hkv, kv_block_num, num_kv_splits, num_sms,
-                                use_fp8_kvcache and h_r <= 16, _KV4_CTAS if use_kv4_cache and h_r <= 16 else None)
+                                use_fp8_kvcache and h_r <= 16, _kv4_ctas(h_r) if use_kv4_cache and h_r <= 16 else None)
         up.add("token_batch", np.repeat(np.arange(batch, dtype=np.int32), a_q))
         up.add("page_batch", np.repeat(np.arange(batch, dtype=np.int32), pages_per))
         info["num_logical_pages"] = int(pages_per.sum())
@@ -400,7 +404,7 @@ def _fmha_sail_plan(
                 info["num_work_tc"] = n_tc
         # Two CTAs of the e4m3 decode kernel share an SM.  A cut at the average load may take more partials than a workspace
         # sized for the plain cut holds: such a workspace gets the plain cut.
-        shared = 1 if max_qo * pack > 16 else (_KV4_CTAS if use_kv4_cache else (2 if use_fp8_kvcache else 1))
+        shared = 1 if max_qo * pack > 16 else (_kv4_ctas(max_qo * pack) if use_kv4_cache else (2 if use_fp8_kvcache else 1))
         for ctas in (shared, -1):
             args = _lib.MsaPlanArgs(
                 a_q.ctypes.data, a_k.ctypes.data, a_o.ctypes.data, batch, num_qo_heads, hkv, block_m, pack,
