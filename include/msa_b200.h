@@ -263,7 +263,7 @@ int msa_fmha_fwd_split_static(const MsaFmhaParams* params, const int32_t* splits
  * tokens.  Any of q, k, v may be NULL (k needs k_out or k_cache; v needs v_cache).  q, k, v and the outputs are bf16 unless a
  * dtype says otherwise, head_dim 128, strides in elements (a KV4 cache: bytes); in-place (q_out == q) is allowed.
  *  - norm != 0: x / sqrt(mean(x^2) + eps) * weight; weights [128] (stride 0) or one row per head, f32 or bf16, NULL = 1.
- *  - rotary elements (a multiple of 16, 0 = none) are rotated in pairs (i, i + rotary / 2), or (2i, 2i + 1) if interleaved,
+ *  - rotary elements (a multiple of 32, 0 = none) are rotated in pairs (i, i + rotary / 2), or (2i, 2i + 1) if interleaved,
  *    by positions[axis[n]][token] * turns[n] for pair n; turns[n] = the frequency in turns per position, as a
  *    64-bit fraction (modulo 1).
  *  - cache: row of token t at slot_map[t] = page * page_size + offset; a negative slot, or one past num_pages, writes

@@ -8,14 +8,15 @@
 // wrapping integer product, exact to 2^-64 turns times the position at any position; the cosine and sine of what is left
 // are taken once per token and pair and shared by all heads.
 //
-// Keys are normed and rotated in 64 bits and rounded to bf16 once, then quantised from there: which e4m3 or e2m1 value a key
-// next to a border gets does not depend on the order of a sum.  (They are a tenth of the rows or less; the pass is bound
-// by memory.)  Queries are computed in 32 bits.
+// Keys that are quantised are normed and rotated in 64 bits, rounded to bf16 once and quantised from there: which e4m3 or e2m1
+// value a key next to a border gets does not depend on the order of a sum.  (They are a tenth of the rows or less.)  All
+// else is computed in 32 bits and rounded once.
 //
 // 4-bit rows: 16 elements share an e4m3 scale s = round(max|x| / 6), at least 2^-9; the codes are the e2m1 roundings of x / s
 // (divisions as IEEE has them: an x on a border goes to the even code).  A NaN makes the scale of its 16 elements NaN.
 //
-// A row of 128 bf16 is read by 16 lanes, 16 bytes each; a warp works on two heads at a time.
+// A warp works on four heads at a time, 8 lanes each.  A lane has eight pairs: two chunks of eight elements (16 bytes), rotary / 2
+// apart (one after the other if interleaved, and in what is not rotated), so that a rotation needs no other lane.
 #include <algorithm>
 
 #include <cuda_fp4.h>
@@ -30,17 +31,30 @@ namespace {
 constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
 
-__device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&x)[8]) {
-  const uint4 r = *reinterpret_cast<const uint4*>(p);
+// Elements of a row that a lane has: x[0..7] at a, x[8..15] at b.
+struct Lane {
+  int a, b;
+  bool rotary;
+};
+template <bool PAIRS>
+__device__ __forceinline__ Lane lane_of(int l, int rotary) {
+  Lane v;
+  v.rotary = 16 * l < rotary;
+  v.a = v.rotary && !PAIRS ? 8 * l : 16 * l;
+  v.b = v.rotary && !PAIRS ? rotary / 2 + 8 * l : 16 * l + 8;
+  return v;
+}
+
+__device__ __forceinline__ void unpack8(const uint4& r, float* x) {
   const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) { x[2 * i] = __uint_as_float(w[i] << 16); x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
 }
-__device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
+__device__ __forceinline__ uint4 pack8(const float* x) {
   return make_uint4(pack2<false>(x[0], x[1]), pack2<false>(x[2], x[3]), pack2<false>(x[4], x[5]), pack2<false>(x[6], x[7]));
 }
 __device__ __forceinline__ float to_bf16(float x) { return __bfloat162float(__float2bfloat16_rn(x)); }
-__device__ __forceinline__ uint2 pack8_e4m3(const float (&x)[8], float scale) {
+__device__ __forceinline__ uint2 pack8_e4m3(const float* x, float scale) {
   uint32_t w[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i)
@@ -48,168 +62,313 @@ __device__ __forceinline__ uint2 pack8_e4m3(const float (&x)[8], float scale) {
   return make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
 }
 
-// Elements 8 * l .. + 7 of the weight of a head, 1 without one.
-__device__ __forceinline__ void load_weight(const void* w, int dtype, int64_t at, float (&x)[8]) {
+// A lane's elements of the weight of a head, 1 without one.
+__device__ __forceinline__ void load_weight(const void* w, int dtype, int64_t row, const Lane& v, float (&x)[16]) {
   if (!w) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = 1.f;
+    for (int i = 0; i < 16; ++i) x[i] = 1.f;
   } else if (dtype == MSA_DT_F32) {
-    const float4 a = *reinterpret_cast<const float4*>(static_cast<const float*>(w) + at);
-    const float4 b = *reinterpret_cast<const float4*>(static_cast<const float*>(w) + at + 4);
-    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-  } else {
-    load8(static_cast<const __nv_bfloat16*>(w) + at, x);
-  }
-}
-
-__device__ __forceinline__ float rsqrt_of(float x) { return rsqrtf(x); }
-__device__ __forceinline__ double rsqrt_of(double x) { return rsqrt(x); }
-
-// Norm and rotation of one head held by 16 lanes (lane l: elements 8 l .. 8 l + 7); cs: cosine and sine of every pair.
-template <typename F, typename F2>
-__device__ __forceinline__ void norm_rotate(F (&x)[8], const float (&w)[8], bool norm, float eps, const F2* cs, int rotary, bool interleaved,
-                                            int l) {
-  if (norm) {
-    F sum = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sum += x[i] * x[i];
-#pragma unroll
-    for (int d = 8; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d, 16);
-    const F r = rsqrt_of(sum * F(1.0 / kHeadDim) + F(eps));
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = x[i] * r * F(w[i]);
-  }
-  if (interleaved) {
-    if (8 * l < rotary) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const F2 t = cs[4 * l + i];
-        const F a = x[2 * i], b = x[2 * i + 1];
-        x[2 * i] = a * t.x - b * t.y;
-        x[2 * i + 1] = b * t.x + a * t.y;
-      }
+    for (int i = 0; i < 4; ++i) {
+      const float4 f = *reinterpret_cast<const float4*>(static_cast<const float*>(w) + row + (i < 2 ? v.a : v.b) + 4 * (i & 1));
+      x[4 * i] = f.x; x[4 * i + 1] = f.y; x[4 * i + 2] = f.z; x[4 * i + 3] = f.w;
     }
-    return;
-  }
-  const int off = rotary >> 4;                               // lanes from one half of the pairs to the other
-  const bool first = l < off, second = !first && l < 2 * off;
-  const int partner = first ? l + off : (second ? l - off : l);
-  const int pair0 = 8 * (first ? l : (second ? l - off : 0));
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const F other = __shfl_sync(0xffffffffu, x[i], partner, 16);
-    const F2 t = cs[pair0 + i];
-    if (first) x[i] = x[i] * t.x - other * t.y;
-    else if (second) x[i] = x[i] * t.x + other * t.y;
+  } else {
+    const __nv_bfloat16* p = static_cast<const __nv_bfloat16*>(w) + row;
+    unpack8(*reinterpret_cast<const uint4*>(p + v.a), x);
+    unpack8(*reinterpret_cast<const uint4*>(p + v.b), x + 8);
   }
 }
 
-// Writes 8 bf16-valued elements of a row of the cache.
-__device__ __forceinline__ void store_row(void* cache, int dtype, int64_t stride_page, int64_t stride_head, int64_t stride_tok, int page_size,
-                                          int slot, int head, int l, const float (&x)[8], float scale, bool write) {
-  const int page = slot / page_size, r = slot - page * page_size;
-  const int64_t at = page * stride_page + head * stride_head;
+// Norm and rotation of the head that 8 lanes hold.  The factor of the norm is the same for all elements, so it comes last and the
+// rotation does not wait for the sum.  32 bits: packed pairs, x[0..3] the first and x[4..7] the second elements of the pairs to turn.
+struct TurnF { uint64_t c[4], s[4]; };                     // cosines and sines
+__device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+template <bool NORM>
+__device__ __forceinline__ void norm_rotate_f(uint64_t (&x)[8], const uint64_t (&w)[8], float eps, bool turn, const TurnF& t) {
+  float r = 1.f;
+  if (NORM) {
+    uint64_t s0 = f2_mul(x[0], x[0]), s1 = f2_mul(x[1], x[1]);
+#pragma unroll
+    for (int i = 2; i < 8; i += 2) { s0 = f2_fma(x[i], x[i], s0); s1 = f2_fma(x[i + 1], x[i + 1], s1); }
+    float lo, hi;
+    f2_unpack(f2_add(s0, s1), lo, hi);
+    float sum = lo + hi;
+#pragma unroll
+    for (int d = 4; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d, 8);
+    r = rsqrtf(sum * (1.f / kHeadDim) + eps);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = f2_mul(x[i], w[i]);
+  }
+  if (turn) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint64_t p = x[i], q = x[i + 4];
+      x[i] = f2_fma(q, t.s[i] ^ 0x8000000080000000ull, f2_mul(p, t.c[i]));
+      x[i + 4] = f2_fma(p, t.s[i], f2_mul(q, t.c[i]));
+    }
+  }
+  if (NORM) {
+    const uint64_t rr = f2_pack(r, r);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = f2_mul(x[i], rr);
+  }
+}
+
+// 64 bits, rounded to bf16.  cs: of pair i of this lane at 8 i.
+template <bool PAIRS>
+__device__ __forceinline__ void norm_rotate_d(float (&x)[16], const float (&w)[16], bool norm, float eps, bool turn, const double2* cs) {
+  double z[16], r = 1.0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) z[i] = x[i];
+  if (norm) {
+    double sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sum += z[i] * z[i];
+#pragma unroll
+    for (int d = 4; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d, 8);
+    r = rsqrt(sum * (1.0 / kHeadDim) + static_cast<double>(eps));
+#pragma unroll
+    for (int i = 0; i < 16; ++i) z[i] *= static_cast<double>(w[i]);
+  }
+  if (turn) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const double2 t = cs[8 * i];
+      double& p = z[PAIRS ? 2 * i : i];
+      double& q = z[PAIRS ? 2 * i + 1 : i + 8];
+      const double p0 = p, q0 = q;
+      p = p0 * t.x - q0 * t.y;
+      q = q0 * t.x + p0 * t.y;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 16; ++i) x[i] = to_bf16(static_cast<float>(z[i] * r));
+}
+
+// Eight elements of a block of 16 as codes, and the block's scale; top: its largest magnitude.
+__device__ __forceinline__ uint32_t codes8(const float* y, uint32_t top, __nv_fp8_storage_t& sb) {
+  float s = __fdiv_rn(__uint_as_float(top), 6.f);
+  s = s < kKv4MinScale ? kKv4MinScale : s;
+  sb = __nv_cvt_float_to_fp8(s, __NV_SATFINITE, __NV_E4M3);
+  const __half_raw sh = __nv_cvt_fp8_to_halfraw(sb, __NV_E4M3);
+  const float sf = __half2float(*reinterpret_cast<const __half*>(&sh));
+  uint32_t codes = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    codes |= static_cast<uint32_t>(__nv_cvt_float2_to_fp4x2(make_float2(__fdiv_rn(y[2 * i], sf), __fdiv_rn(y[2 * i + 1], sf)), __NV_E2M1,
+                                                            cudaRoundNearest)) << (8 * i);
+  return codes;
+}
+
+// Writes a lane's bf16-valued elements of a row of the cache.  All lanes of the warp take part.
+__device__ __forceinline__ void store_row(void* cache, int dtype, int64_t at, int64_t stride_tok, int r, const Lane& v, int l, const float (&x)[16],
+                                          float scale, bool write) {
   if (dtype == MSA_DT_KV4) {
-    float y[8];
-    uint32_t top = 0;                                        // as integers: a NaN is above every number
+    float y[16];
+    uint32_t top[2] = {0, 0};                                // as integers: a NaN is above every number
 #pragma unroll
-    for (int i = 0; i < 8; ++i) { y[i] = __fdiv_rn(x[i], scale); top = max(top, __float_as_uint(y[i]) & 0x7fffffffu); }
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    float s = __fdiv_rn(__uint_as_float(top), 6.f);
-    s = s < kKv4MinScale ? kKv4MinScale : s;
-    const __nv_fp8_storage_t sb = __nv_cvt_float_to_fp8(s, __NV_SATFINITE, __NV_E4M3);
-    const __half_raw sh = __nv_cvt_fp8_to_halfraw(sb, __NV_E4M3);
-    const float sf = __half2float(*reinterpret_cast<const __half*>(&sh));
-    uint32_t codes = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      codes |= static_cast<uint32_t>(__nv_cvt_float2_to_fp4x2(make_float2(__fdiv_rn(y[2 * i], sf), __fdiv_rn(y[2 * i + 1], sf)), __NV_E2M1,
-                                                              cudaRoundNearest)) << (8 * i);
+    for (int i = 0; i < 16; ++i) { y[i] = __fdiv_rn(x[i], scale); top[i >> 3] = max(top[i >> 3], __float_as_uint(y[i]) & 0x7fffffffu); }
+    // 16 elements that share a scale: one chunk of two lanes, or both chunks of this one
+    const bool apart = v.b != v.a + 8;
+    const uint32_t far0 = __shfl_xor_sync(0xffffffffu, top[0], 1), far1 = __shfl_xor_sync(0xffffffffu, top[1], 1);
+    if (apart) { top[0] = max(top[0], far0); top[1] = max(top[1], far1); }
+    else top[0] = top[1] = max(top[0], top[1]);
+    __nv_fp8_storage_t sa, sb;
+    const uint32_t ca = codes8(y, top[0], sa), cb = codes8(y + 8, top[1], sb);
     if (write) {
       unsigned char* tile = static_cast<unsigned char*>(cache) + at;
-      *reinterpret_cast<uint32_t*>(tile + r * kKv4CodeBytes + 4 * l) = codes;
-      if (!(l & 1)) tile[kKv4ScaleOffset + r * kKv4ScaleBytes + (l >> 1)] = sb;
+      unsigned char* code = tile + r * kKv4CodeBytes;
+      unsigned char* sc = tile + kKv4ScaleOffset + r * kKv4ScaleBytes;
+      *reinterpret_cast<uint32_t*>(code + v.a / 2) = ca;
+      *reinterpret_cast<uint32_t*>(code + v.b / 2) = cb;
+      if (!apart || !(l & 1)) sc[v.a / 16] = sa;
+      if (apart && !(l & 1)) sc[v.b / 16] = sb;
     }
   } else if (write && dtype == MSA_DT_E4M3) {
-    *reinterpret_cast<uint2*>(static_cast<unsigned char*>(cache) + at + r * stride_tok + 8 * l) = pack8_e4m3(x, scale);
+    unsigned char* row = static_cast<unsigned char*>(cache) + at + r * stride_tok;
+    *reinterpret_cast<uint2*>(row + v.a) = pack8_e4m3(x, scale);
+    *reinterpret_cast<uint2*>(row + v.b) = pack8_e4m3(x + 8, scale);
   } else if (write) {
-    *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(cache) + at + r * stride_tok + 8 * l) = pack8(x);
+    __nv_bfloat16* row = static_cast<__nv_bfloat16*>(cache) + at + r * stride_tok;
+    *reinterpret_cast<uint4*>(row + v.a) = pack8(x);
+    *reinterpret_cast<uint4*>(row + v.b) = pack8(x + 8);
   }
 }
 
-__global__ void __launch_bounds__(kThreads) norm_rope_kernel(const MsaNormRopeArgs a) {
+// Elements of the two chunks <-> packed pairs, the first elements of the pairs to turn in x[0..3].
+template <bool PAIRS>
+__device__ __forceinline__ void pairs_of(const float (&y)[16], uint64_t (&x)[8]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (PAIRS) { x[i] = f2_pack(y[4 * i], y[4 * i + 2]); x[i + 4] = f2_pack(y[4 * i + 1], y[4 * i + 3]); }
+    else { x[i] = f2_pack(y[2 * i], y[2 * i + 1]); x[i + 4] = f2_pack(y[2 * i + 8], y[2 * i + 9]); }
+  }
+}
+template <bool PAIRS>
+__device__ __forceinline__ void elements_of(const uint64_t (&x)[8], float (&y)[16]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (PAIRS) { f2_unpack(x[i], y[4 * i], y[4 * i + 2]); f2_unpack(x[i + 4], y[4 * i + 1], y[4 * i + 3]); }
+    else { f2_unpack(x[i], y[2 * i], y[2 * i + 1]); f2_unpack(x[i + 4], y[2 * i + 8], y[2 * i + 9]); }
+  }
+}
+
+// A warp has one of `parts` parts of a token's heads, four heads (a unit) at a time: units part, part + parts, ... of the queries,
+// then of the keys, then of the values.  The next kBatch query units are on their way while as many are worked on.
+constexpr int kBatch = 2;
+
+template <bool PAIRS, bool NORM, bool Q8>
+__global__ void __launch_bounds__(kThreads, 2) norm_rope_kernel(const __grid_constant__ MsaNormRopeArgs a, int parts) {
   chain_begin();
-  __shared__ double2 s_cs[kHeadDim / 2];
-  __shared__ float2 s_csf[kHeadDim / 2];
-  const int t = blockIdx.x;
-  const int lane = threadIdx.x & 31, l = lane & 15, half = lane >> 4;
+  __shared__ double2 s_all[kWarps][kHeadDim / 2];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, l = lane & 7, sub = lane >> 3;
+  const int64_t id = static_cast<int64_t>(blockIdx.x) * kWarps + warp;
+  const int t = static_cast<int>(id / parts), part = static_cast<int>(id % parts);
+  if (t >= a.tokens) return;
+  double2* s_cs = s_all[warp];
+  const Lane v = lane_of<PAIRS>(l, a.rotary);
+  const int off = v.b - v.a;
+  const int q_units = a.q ? (a.num_qo_heads + 3) / 4 : 0, kv_units = (a.num_kv_heads + 3) / 4;
+  const int q_whole = a.q ? a.num_qo_heads / 4 : 0;          // units of four heads
+  const __nv_bfloat16* q_at = static_cast<const __nv_bfloat16*>(a.q) + t * a.q_stride_tok + (4 * part + sub) * a.q_stride_head + v.a;
+  const int64_t q_step = 4 * parts * a.q_stride_head;
+  uint4 raw[kBatch][2];
+  auto load_q = [&](const __nv_bfloat16* p, uint4 (&r)[kBatch][2]) {
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      r[i][0] = *reinterpret_cast<const uint4*>(p + i * q_step);
+      r[i][1] = *reinterpret_cast<const uint4*>(p + i * q_step + off);
+    }
+  };
+  if (part + (kBatch - 1) * parts < q_whole) load_q(q_at, raw);
+  const int slot = a.slot_map ? a.slot_map[t] : -1;
+  TurnF turn = {};
   if (a.rotary > 0) {
-    const int n = threadIdx.x;
-    if (n < a.rotary / 2) {
+    for (int n = lane; n < a.rotary / 2; n += 32) {
       const int64_t at = a.axis[n] * a.pos_stride_axis + t;
       const int64_t pos = a.pos_int64 ? static_cast<const int64_t*>(a.positions)[at] : static_cast<const int32_t*>(a.positions)[at];
       const int64_t turns = static_cast<int64_t>(static_cast<uint64_t>(pos) * static_cast<uint64_t>(a.turns[n]));   // modulo a turn
-      double2 cs;
-      sincospi(static_cast<double>(turns) * 0x1p-63, &cs.y, &cs.x);
-      s_cs[n] = cs;
-      s_csf[n] = make_float2(static_cast<float>(cs.x), static_cast<float>(cs.y));
+      double2 d;
+      sincospi(static_cast<double>(turns) * 0x1p-63, &d.y, &d.x);
+      s_cs[(n & 7) * 8 + (n >> 3)] = d;                      // pair i of lane l at 8 i + l
     }
-    __syncthreads();
+    __syncwarp();
+    if (v.rotary) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const double2 d = s_cs[16 * i + l], e = s_cs[16 * i + 8 + l];
+        turn.c[i] = f2_pack(static_cast<float>(d.x), static_cast<float>(e.x));
+        turn.s[i] = f2_pack(static_cast<float>(d.y), static_cast<float>(e.y));
+      }
+    }
   }
-  const int slot = a.slot_map ? a.slot_map[t] : -1;
-  const bool has_slot = slot >= 0 && slot / a.page_size < a.num_pages;
-#ifdef MSA_BOUNDS_CHECK
-  if (slot >= 0 && !has_slot) chk(slot, 0, 0, a.status);
-#endif
-  const int slot_in = has_slot ? slot : 0;
-  const int q_units = a.q ? (a.num_qo_heads + 1) / 2 : 0, kv_units = (a.num_kv_heads + 1) / 2;
-  const int k_end = q_units + (a.k ? kv_units : 0), v_end = k_end + (a.v ? kv_units : 0);
-  for (int u = blockIdx.y * kWarps + (threadIdx.x >> 5); u < v_end; u += gridDim.y * kWarps) {
-    float x[8], w[8];
-    if (u < q_units) {
-      const int head = 2 * u + half;
-      const bool real = head < a.num_qo_heads;
-      const int h = real ? head : head - 1;
-      load8(static_cast<const __nv_bfloat16*>(a.q) + t * a.q_stride_tok + h * a.q_stride_head + 8 * l, x);
-      load_weight(a.q_weight, a.weight_dtype, h * a.q_weight_stride + 8 * l, w);
-      norm_rotate(x, w, a.norm, a.eps, s_csf, a.rotary, a.interleaved, l);
-      if (real) {
-        const int64_t at = t * a.q_out_stride_tok + h * a.q_out_stride_head + 8 * l;
-        if (a.q_out_dtype == MSA_DT_E4M3) {
+  uint64_t w8[8] = {};
+  auto load_w8 = [&](const void* weight, int64_t row) {
+    float w[16];
+    load_weight(weight, a.weight_dtype, row, v, w);
+    pairs_of<PAIRS>(w, w8);
+  };
+  auto turned = [&](const uint4 (&r)[2], float (&y)[16]) {
+    uint64_t x[8];
+    unpack8(r[0], y);
+    unpack8(r[1], y + 8);
+    pairs_of<PAIRS>(y, x);
+    norm_rotate_f<NORM>(x, w8, a.eps, v.rotary, turn);
+    elements_of<PAIRS>(x, y);
+  };
+  const int64_t out_at = t * a.q_out_stride_tok + (4 * part + sub) * a.q_out_stride_head + v.a;
+  const int64_t out_step = 4 * parts * a.q_out_stride_head;
+  auto store_q = [&](int64_t at, float (&y)[16]) {
+    if (Q8) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) x[i] = to_bf16(x[i]);
-          *reinterpret_cast<uint2*>(static_cast<unsigned char*>(a.q_out) + at) = pack8_e4m3(x, a.q_scale);
-        } else {
-          *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.q_out) + at) = pack8(x);
-        }
-      }
-    } else if (u < k_end) {
-      const int head = 2 * (u - q_units) + half;
-      const bool real = head < a.num_kv_heads;
-      const int h = real ? head : head - 1;
-      load8(static_cast<const __nv_bfloat16*>(a.k) + t * a.k_stride_tok + h * a.k_stride_head + 8 * l, x);
-      if (a.norm || a.rotary > 0) {
-        load_weight(a.k_weight, a.weight_dtype, h * a.k_weight_stride + 8 * l, w);
-        double z[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) z[i] = x[i];
-        norm_rotate(z, w, a.norm, a.eps, s_cs, a.rotary, a.interleaved, l);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = to_bf16(static_cast<float>(z[i]));
-      }
-      if (a.k_out && real)
-        *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.k_out) + t * a.k_out_stride_tok + h * a.k_out_stride_head + 8 * l) = pack8(x);
-      if (a.k_cache)
-        store_row(a.k_cache, a.cache_dtype, a.k_cache_stride_page, a.k_cache_stride_head, a.k_cache_stride_tok, a.page_size, slot_in, h, l, x,
-                  a.k_scale * (a.k_scale_head ? a.k_scale_head[h] : 1.f), has_slot && real);
+      for (int n = 0; n < 16; ++n) y[n] = to_bf16(y[n]);
+      unsigned char* out = static_cast<unsigned char*>(a.q_out) + at;
+      *reinterpret_cast<uint2*>(out) = pack8_e4m3(y, a.q_scale);
+      *reinterpret_cast<uint2*>(out + off) = pack8_e4m3(y + 8, a.q_scale);
     } else {
-      const int head = 2 * (u - k_end) + half;
-      const bool real = head < a.num_kv_heads;
-      const int h = real ? head : head - 1;
-      load8(static_cast<const __nv_bfloat16*>(a.v) + t * a.v_stride_tok + h * a.v_stride_head + 8 * l, x);
-      store_row(a.v_cache, a.cache_dtype, a.v_cache_stride_page, a.v_cache_stride_head, a.v_cache_stride_tok, a.page_size, slot_in, h, l, x,
-                a.v_scale * (a.v_scale_head ? a.v_scale_head[h] : 1.f), has_slot && real);
+      __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.q_out) + at;
+      *reinterpret_cast<uint4*>(out) = pack8(y);
+      *reinterpret_cast<uint4*>(out + off) = pack8(y + 8);
     }
+  };
+  const bool w_head = NORM && a.q_weight_stride != 0;        // a weight for each head
+  if (NORM && a.q) load_w8(a.q_weight, 0);
+  int u = part, n_done = 0;                                  // n_done: units of this warp that are through
+  for (; u + (kBatch - 1) * parts < q_whole; u += kBatch * parts, n_done += kBatch) {
+    uint4 next[kBatch][2] = {};
+    const bool more = u + (2 * kBatch - 1) * parts < q_whole;
+    if (more) load_q(q_at + (n_done + kBatch) * q_step, next);
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      float y[16];
+      if (w_head) load_w8(a.q_weight, (4 * (u + i * parts) + sub) * a.q_weight_stride);
+      turned(raw[i], y);
+      store_q(out_at + (n_done + i) * out_step, y);
+    }
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) { raw[i][0] = next[i][0]; raw[i][1] = next[i][1]; }
+  }
+#pragma unroll 1
+  for (; u < q_units; u += parts, ++n_done) {                // what is left; lanes past the last head have that one once more
+    const int h = min(4 * u + sub, a.num_qo_heads - 1);
+    const bool real = 4 * u + sub < a.num_qo_heads;
+    const __nv_bfloat16* p = static_cast<const __nv_bfloat16*>(a.q) + t * a.q_stride_tok + h * a.q_stride_head + v.a;
+    const uint4 r[2] = {*reinterpret_cast<const uint4*>(p), *reinterpret_cast<const uint4*>(p + off)};
+    float y[16];
+    if (w_head) load_w8(a.q_weight, h * a.q_weight_stride);
+    turned(r, y);
+    if (real) store_q(out_at + n_done * out_step, y);
+  }
+  if (!a.k && !a.v) return;
+  const int page_size = max(a.page_size, 1), page = slot / page_size, row = slot - page * page_size;
+  const bool has_slot = slot >= 0 && page < a.num_pages;
+#ifdef MSA_BOUNDS_CHECK
+  if (slot >= 0 && a.slot_map && !has_slot) chk(slot, 0, 0, a.status);
+#endif
+  const bool fine = a.k_cache && a.cache_dtype != MSA_DT_BF16;   // keys are quantised
+  if (a.k && NORM && !fine) load_w8(a.k_weight, 0);
+#pragma unroll 1
+  for (u -= q_units; a.k && u < kv_units; u += parts) {
+    const int h = min(4 * u + sub, a.num_kv_heads - 1);
+    const bool real = 4 * u + sub < a.num_kv_heads;
+    const __nv_bfloat16* p = static_cast<const __nv_bfloat16*>(a.k) + t * a.k_stride_tok + h * a.k_stride_head + v.a;
+    const uint4 r[2] = {*reinterpret_cast<const uint4*>(p), *reinterpret_cast<const uint4*>(p + off)};
+    float x[16];
+    if (!fine && (NORM || a.rotary > 0)) {
+      if (NORM && a.k_weight_stride) load_w8(a.k_weight, h * a.k_weight_stride);
+      turned(r, x);
+    } else {
+      unpack8(r[0], x);
+      unpack8(r[1], x + 8);
+      if (NORM || a.rotary > 0) {
+        float w[16];
+        if (NORM) load_weight(a.k_weight, a.weight_dtype, h * a.k_weight_stride, v, w);
+        norm_rotate_d<PAIRS>(x, w, NORM, a.eps, v.rotary, s_cs + l);
+      }
+    }
+    if (a.k_out && real) {
+      __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.k_out) + t * a.k_out_stride_tok + h * a.k_out_stride_head + v.a;
+      *reinterpret_cast<uint4*>(out) = pack8(x);
+      *reinterpret_cast<uint4*>(out + off) = pack8(x + 8);
+    }
+    if (a.k_cache)
+      store_row(a.k_cache, a.cache_dtype, page * a.k_cache_stride_page + h * a.k_cache_stride_head, a.k_cache_stride_tok, row, v, l, x,
+                a.k_scale * (a.k_scale_head ? a.k_scale_head[h] : 1.f), has_slot && real);
+  }
+#pragma unroll 1
+  for (u -= a.k ? kv_units : 0; a.v && u < kv_units; u += parts) {
+    const int h = min(4 * u + sub, a.num_kv_heads - 1);
+    const __nv_bfloat16* p = static_cast<const __nv_bfloat16*>(a.v) + t * a.v_stride_tok + h * a.v_stride_head + v.a;
+    float x[16];
+    unpack8(*reinterpret_cast<const uint4*>(p), x);
+    unpack8(*reinterpret_cast<const uint4*>(p + off), x + 8);
+    store_row(a.v_cache, a.cache_dtype, page * a.v_cache_stride_page + h * a.v_cache_stride_head, a.v_cache_stride_tok, row, v, l, x,
+              a.v_scale * (a.v_scale_head ? a.v_scale_head[h] : 1.f), has_slot && 4 * u + sub < a.num_kv_heads);
   }
 }
 
@@ -273,7 +432,7 @@ extern "C" int msa_norm_rope(const MsaNormRopeArgs* pa, msa_stream_t stream) {
   if (!pa) return MSA_ERR_BAD_ARG;
   const MsaNormRopeArgs& a = *pa;
   if (a.tokens < 0 || a.num_qo_heads < 0 || a.num_kv_heads < 0 || (!a.q && !a.k && !a.v)) return MSA_ERR_BAD_ARG;
-  if (a.rotary < 0 || a.rotary > kHeadDim || a.rotary % 16) return MSA_ERR_UNSUPPORTED;
+  if (a.rotary < 0 || a.rotary > kHeadDim || a.rotary % 32) return MSA_ERR_UNSUPPORTED;
   if (a.rotary > 0 && (!a.positions || !a.turns || !a.axis)) return MSA_ERR_BAD_ARG;
   if (a.q) {
     if (!a.q_out || a.num_qo_heads < 1 || !rows_ok(a.q, a.q_stride_tok, a.q_stride_head, 2)) return MSA_ERR_BAD_ARG;
@@ -298,13 +457,18 @@ extern "C" int msa_norm_rope(const MsaNormRopeArgs* pa, msa_stream_t stream) {
   if (a.weight_dtype != MSA_DT_F32 && a.weight_dtype != MSA_DT_BF16) return MSA_ERR_UNSUPPORTED;
   if (a.tokens == 0) return MSA_OK;
   NvtxRange range("msa_norm_rope");
-  const int kv_units = (a.num_kv_heads + 1) / 2;
-  const int units = (a.q ? (a.num_qo_heads + 1) / 2 : 0) + (a.k ? kv_units : 0) + (a.v ? kv_units : 0);
-  // few tokens: the heads of one go to several CTAs, so that a warp has one unit
-  const int most = (units + kWarps - 1) / kWarps;
-  const int y = std::max(1, std::min(most, 2 * 148 / std::max(1, a.tokens)));
-  return launch_chained(norm_rope_kernel, dim3(a.tokens, y), kThreads, 0, static_cast<cudaStream_t>(stream), a) == cudaSuccess ? MSA_OK
-                                                                                                                           : MSA_ERR_LAUNCH;
+  const int kv_units = (a.num_kv_heads + 3) / 4;
+  const int units = (a.q ? (a.num_qo_heads + 3) / 4 : 0) + (a.k ? kv_units : 0) + (a.v ? kv_units : 0);
+  // few tokens: the heads of one go to several warps, until the SMs have 16 each or a warp has one unit
+  const int parts = std::max(1, std::min(units, 148 * 16 / a.tokens));
+  const int64_t blocks = (static_cast<int64_t>(a.tokens) * parts + kWarps - 1) / kWarps;
+  const bool q8 = a.q && a.q_out_dtype == MSA_DT_E4M3;
+#define MSA_ROPE_CASE(PAIRS) \
+  (a.norm ? (q8 ? norm_rope_kernel<PAIRS, true, true> : norm_rope_kernel<PAIRS, true, false>) \
+          : (q8 ? norm_rope_kernel<PAIRS, false, true> : norm_rope_kernel<PAIRS, false, false>))
+  return launch_chained(a.interleaved ? MSA_ROPE_CASE(true) : MSA_ROPE_CASE(false), dim3(static_cast<unsigned>(blocks)), kThreads, 0,
+                        static_cast<cudaStream_t>(stream), a, parts) == cudaSuccess ? MSA_OK : MSA_ERR_LAUNCH;
+#undef MSA_ROPE_CASE
 }
 
 extern "C" int msa_kv4_read(const MsaKv4ReadArgs* pa, msa_stream_t stream) {

@@ -137,7 +137,7 @@ class RopePlan(dict):
 
 def rope_plan(rotary_dim: int = 128, base: float = 10000.0, inv_freq: Optional[Union[torch.Tensor, Sequence[float]]] = None,
               sections: Optional[Sequence[int]] = None, interleaved: bool = False, device=None) -> RopePlan:
-    """Frequencies of a rotary embedding over the first ``rotary_dim`` elements of a head (a multiple of 16, at most 128).
+    """Frequencies of a rotary embedding over the first ``rotary_dim`` elements of a head (a multiple of 32, at most 128).
 
     ``inv_freq``: the angle per position of each of the ``rotary_dim / 2`` pairs (scaled variants bring their own); default
     ``base ** (-2 i / rotary_dim)``.  ``sections``: pairs of each position axis, in order (time, height, width of a video token:
@@ -145,8 +145,8 @@ def rope_plan(rotary_dim: int = 128, base: float = 10000.0, inv_freq: Optional[U
     instead of (i, i + rotary_dim / 2).
 
     Frequencies are kept as 64-bit fractions of a turn, so angles are exact at any position."""
-    if rotary_dim % 16 or not 0 < rotary_dim <= 128:
-        raise ValueError(f"rotary_dim must be a multiple of 16 in (0, 128], got {rotary_dim}")
+    if rotary_dim % 32 or not 0 < rotary_dim <= 128:
+        raise ValueError(f"rotary_dim must be a multiple of 32 in (0, 128], got {rotary_dim}")
     pairs = rotary_dim // 2
     if inv_freq is None:
         inv_freq = [base ** (-2 * i / rotary_dim) for i in range(pairs)]
