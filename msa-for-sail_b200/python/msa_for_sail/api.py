@@ -41,6 +41,9 @@ def _status_word(device):
     return _STATUS[idx]
 
 
+cache._status_word = _status_word
+
+
 def last_status(device=None, reset=True):
     """Read (synchronously) the device status word: 0 = ok, 1 = a kernel wait timed out, 2 = (bounds-checked
     build) a kernel found an out-of-range index in one of the caller's tables and clamped it."""
@@ -718,6 +721,9 @@ def _fmha_sail(
     split-KV merge directly, converted from the bf16 result otherwise)."""
     if not q.is_cuda:
         raise RuntimeError("fmha_sail needs CUDA tensors (there is no CPU path)")
+    if k.dtype == torch.uint8:
+        return _fmha_sail_kv4(q, k, v, plan_info, kv_indices, kv_block_indexes, q_offset_override, out, max_score, sm_scale,
+                              q_scale, k_scale, v_scale, o_scale, output_maxscore, output_o, check_input_valid, max_score_dtype, lse)
     nnz_qo, num_qo_heads, head_dim_qk = q.shape
     plan_page = plan_info.get("page_size", -1)
     if kv_indices is None:
@@ -727,9 +733,6 @@ def _fmha_sail(
         kv_is_nhd, num_kv_heads, page_size = _detect_paged_kv_layout(k.shape, plan_page)
         head_dim_vo = v.shape[3]
         is_paged = True
-    if k.dtype == torch.uint8:
-        return _fmha_sail_kv4(q, k, v, plan_info, kv_indices, kv_block_indexes, q_offset_override, out, max_score, sm_scale,
-                              q_scale, k_scale, v_scale, o_scale, output_maxscore, output_o, check_input_valid, max_score_dtype, lse)
     if head_dim_qk != 128 or head_dim_vo != 128:
         raise ValueError("fmha_sail supports head_dim 128 only")
 
@@ -958,12 +961,15 @@ def _fmha_sail_kv4(q, k, v, plan, kv_indices, kv_block_indexes, q_offset_overrid
     nnz_qo, num_qo_heads, _ = q.shape
     if plan.get("page_size", -1) != cache.KV4_TILE:
         raise ValueError(f"a 4-bit cache needs a plan with page_size={cache.KV4_TILE}")
-    num_kv_heads = k.shape[1] if k.dim() == 4 else -1
-    cache._check_kv4("k", k)
-    if v is None and output_o:
-        raise ValueError("v is required unless output_o=False")
-    if v is not None and output_o:
-        cache._check_kv4("v", v, num_kv_heads)
+    assert output_o or output_maxscore
+    scores = output_maxscore and plan["max_k_tiles"] != -1
+    output_o = output_o or not scores
+    k_stride = cache._check_kv4("k", k)
+    num_kv_heads = k.shape[1]
+    if output_o:
+        if v is None:
+            raise ValueError("v is required unless output_o=False")
+        v_stride = cache._check_kv4("v", v, num_kv_heads)
         if v.shape[0] != k.shape[0]:
             raise ValueError(f"k and v must have the same pages, got {k.shape[0]} and {v.shape[0]}")
     if kv_indices.dtype != torch.int32 or kv_indices.dim() != 1 or not kv_indices.is_contiguous():
@@ -973,11 +979,17 @@ def _fmha_sail_kv4(q, k, v, plan, kv_indices, kv_block_indexes, q_offset_overrid
                        max_score=max_score, plan=plan["qo_offset"])
     if k.shape[0] == 0 and nnz_qo:
         raise ValueError("the cache has no pages")
+    if num_qo_heads % num_kv_heads:
+        raise ValueError(f"num_qo_heads ({num_qo_heads}) must be divisible by num_kv_heads ({num_kv_heads})")
     sparse = kv_block_indexes is not None
+    if plan["is_sparse"] != sparse:
+        raise ValueError("plan sparse mode (kv_block_num) does not match kv_block_indexes")
+    if sparse and (kv_block_indexes.dtype != torch.int32 or kv_block_indexes.dim() != 3 or kv_block_indexes.shape[:2] != (nnz_qo, num_kv_heads)
+                   or kv_block_indexes.stride(2) != 1):
+        raise ValueError(f"kv_block_indexes must be int32 [total_qo_len, H_kv={num_kv_heads}, KVBlockNum], got {kv_block_indexes.dtype} {tuple(kv_block_indexes.shape)}")
     h_r = num_qo_heads // num_kv_heads
     rows = plan["max_qo_len"] * plan["pack_factor"]
-    scores = output_maxscore and plan["max_k_tiles"] != -1
-    native = (output_o or not scores) and not scores and plan["pack_factor"] == h_r and (sparse or rows <= 128)
+    native = not scores and plan["pack_factor"] == h_r and (sparse or rows <= 128)
     if native and sparse and plan["sparse_tc_preferred"] and 128 % h_r == 0 and kv_block_indexes.shape[2] <= 32:
         native = False                        # the page-major kernel, on the copy
     # the checks of the plan against the call, and of the other arguments, are those of any call
@@ -990,14 +1002,12 @@ def _fmha_sail_kv4(q, k, v, plan, kv_indices, kv_block_indexes, q_offset_overrid
         with cache._on(dev):
             table = torch.arange(kv_indices.shape[0], dtype=torch.int32, device=dev)
             kb = cache.unpack_pages(k, kv_indices)
-            vb = cache.unpack_pages(v, kv_indices) if output_o or not scores else kb
+            vb = cache.unpack_pages(v, kv_indices) if output_o else kb
             return _fmha_sail(q if q.dtype == torch.bfloat16 else q.to(torch.bfloat16), kb, vb, plan, table, kv_block_indexes, q_offset_override, out,
                               max_score, sm_scale, q_scale, k_scale, v_scale, o_scale, output_maxscore, output_o, check_input_valid,
                               max_score_dtype, lse)
     if plan["orig_num_qo_heads"] != num_qo_heads or plan["num_kv_heads"] != num_kv_heads:
         raise ValueError("plan head counts do not match q / k")
-    if plan["is_sparse"] != sparse:
-        raise ValueError("plan sparse mode (kv_block_num) does not match kv_block_indexes")
     qo_offset = plan["qo_offset"] if q_offset_override is None else q_offset_override
     if isinstance(qo_offset, int):
         if plan.get("graph_safe", False):
@@ -1026,30 +1036,21 @@ def _fmha_sail_kv4(q, k, v, plan, kv_indices, kv_block_indexes, q_offset_overrid
         return out, None
     assert q.stride(2) == 1, "q head_dim must be contiguous"
     splits = plan["num_kv_splits"]
-    p = _lib.MsaFmhaParams()
-    p.q, p.k, p.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
-    p.q_stride_tok, p.q_stride_head = q.stride(0), q.stride(1)
-    p.k_stride_page, p.k_stride_head = k.stride(0), k.stride(1)
-    p.v_stride_page, p.v_stride_head = v.stride(0), v.stride(1)
-    p.kv_indices, p.kv_page_indptr, p.page_size = kv_indices.data_ptr(), plan["kv_page_indptr"].data_ptr(), cache.KV4_TILE
-    p.qo_start, p.kv_len, p.qo_offset = plan["qo_segment_offsets"].data_ptr(), plan["kv_segment_lens"].data_ptr(), qo_offset.data_ptr()
+    q_stride, out_scale = q.stride(), float(v_s * o_s)
+    p = _lib.MsaFmhaParams(
+        q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), qo_start=plan["qo_segment_offsets"].data_ptr(), kv_len=plan["kv_segment_lens"].data_ptr(),
+        qo_offset=qo_offset.data_ptr(), kv_page_indptr=plan["kv_page_indptr"].data_ptr(), kv_indices=kv_indices.data_ptr(),
+        k_scale_head=_ptr(k_head), v_scale_head=_ptr(v_head), status=_status_word(dev).data_ptr(), q_stride_tok=q_stride[0], q_stride_head=q_stride[1],
+        k_stride_page=k_stride[0], k_stride_head=k_stride[1], v_stride_page=v_stride[0], v_stride_head=v_stride[1], kv_extent=k.shape[0],
+        total_q=nnz_qo, num_qo_heads=num_qo_heads, num_kv_heads=num_kv_heads, batch=plan["batch_size"], block_m=plan["qo_tile_size"],
+        pack=plan["pack_factor"], page_size=cache.KV4_TILE, num_splits=splits, q_dtype=_dt_code(q.dtype), kv_dtype=MSA_DT_KV4,
+        flags=FLAG_OUT_O | FLAG_SPARSE if sparse else FLAG_OUT_O, sm_scale=float(q_s * k_s * sm_scale), out_scale=out_scale)
     if sparse:
-        assert kv_block_indexes.dtype == torch.int32
-        if kv_block_indexes.dim() != 3 or kv_block_indexes.shape[:2] != (nnz_qo, num_kv_heads) or kv_block_indexes.stride(2) != 1:
-            raise ValueError(f"kv_block_indexes must be [total_qo_len, H_kv={num_kv_heads}, KVBlockNum], got {tuple(kv_block_indexes.shape)}")
         p.kv_block_indexes, p.kv_block_num = kv_block_indexes.data_ptr(), kv_block_indexes.shape[2]
         p.kbi_stride_tok, p.kbi_stride_head = kv_block_indexes.stride(0), kv_block_indexes.stride(1)
         p.token_batch = plan["token_batch"].data_ptr()
     else:
-        p.work, p.num_work = _ptr(plan["work"]), plan["num_work"]
-        p.decode_rows = rows
-    p.k_scale_head, p.v_scale_head = _ptr(k_head), _ptr(v_head)
-    p.total_q, p.num_qo_heads, p.num_kv_heads, p.batch = nnz_qo, num_qo_heads, num_kv_heads, plan["batch_size"]
-    p.block_m, p.pack, p.kv_extent = plan["qo_tile_size"], plan["pack_factor"], k.shape[0]
-    p.status = _status_word(dev).data_ptr()
-    p.q_dtype, p.kv_dtype = _dt_code(q.dtype), MSA_DT_KV4
-    p.flags = FLAG_OUT_O | (FLAG_SPARSE if sparse else 0)
-    p.sm_scale, p.out_scale = float(q_s * k_s * sm_scale), float(v_s * o_s)
+        p.work, p.num_work, p.decode_rows = _ptr(plan["work"]), plan["num_work"], rows
     if _SHOW_PARAMS:
         _show_params(q, plan, True, cache.KV4_TILE, float(sm_scale), True, None, kv_block_indexes)
     with cache._on(dev):
@@ -1058,18 +1059,18 @@ def _fmha_sail_kv4(q, k, v, plan, kv_indices, kv_block_indexes, q_offset_overrid
         kernel_out = out
         if splits > 1:
             part = torch.empty(splits * nnz_qo * num_qo_heads * 129, dtype=torch.float32, device=dev)
-            p.partial_o, p.num_splits = part.data_ptr(), splits
+            p.partial_o = part.data_ptr()
             p.partial_lse = part.data_ptr() + splits * nnz_qo * num_qo_heads * 512
         else:
             if out.dtype == torch.float32:
                 kernel_out = torch.empty(out.shape, dtype=torch.bfloat16, device=dev)
-            p.num_splits, p.lse = 1, _ptr(lse)
+            p.lse = _ptr(lse)
             p.out, p.out_stride_tok, p.out_stride_head = kernel_out.data_ptr(), kernel_out.stride(0), kernel_out.stride(1)
         _lib.check(_lib.lib.msa_fmha_fwd(ctypes.byref(p), stream), "msa_fmha_fwd")
         if splits > 1:
             _lib.check(_lib.lib.msa_lse_merge_ex(
                 p.partial_o, MSA_DT_F32, p.partial_lse, _ptr(plan["num_kv_splits_per_row"]), out.data_ptr(), _dt_code(out.dtype), _ptr(lse),
-                splits, nnz_qo, num_qo_heads, 0, 0, out.stride(0), out.stride(1), float(v_s * o_s), stream), "msa_lse_merge_ex")
+                splits, nnz_qo, num_qo_heads, 0, 0, out.stride(0), out.stride(1), out_scale, stream), "msa_lse_merge_ex")
         elif kernel_out is not out:
             out.copy_(kernel_out)
     return out, None
@@ -1132,7 +1133,7 @@ def _run_sub_batches(parts, q, k, v, kv_indices, kv_block_indexes, q_offset_over
     lse = kwargs.pop("lse", None)
     want_o = kwargs.get("output_o", True)
     if want_o and out is None:
-        out = torch.empty(nnz_qo, num_qo_heads, v.shape[-1], device=q.device, dtype=torch.bfloat16)
+        out = torch.empty(nnz_qo, num_qo_heads, q.shape[-1], device=q.device, dtype=torch.bfloat16)
     tok = kv = 0
     scores = []
     for plan, b0, b1 in parts:

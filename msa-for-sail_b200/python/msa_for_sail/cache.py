@@ -25,8 +25,7 @@ KV4_TILE = 128                          # tokens of a page
 KV4_ROW_BYTES = 72                      # 64 bytes of codes and 8 scales
 
 
-def _ptr(t):
-    return None if t is None else t.data_ptr()
+_status_word = None                     # of api.py, set when that is imported
 
 
 def _stream():
@@ -38,14 +37,19 @@ def _on(device):
     return contextlib.nullcontext() if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
 
 
+def _launch(device, fn, args, what):
+    """`fn` on the current stream of `device`."""
+    if device.index == torch._C._cuda_getDevice():
+        _lib.check(fn(ctypes.byref(args), torch._C._cuda_getCurrentRawStream(device.index)), what)
+    else:
+        with torch.cuda.device(device):
+            _lib.check(fn(ctypes.byref(args), _stream()), what)
+
+
 def _same_device(device, **tensors):
     for name, t in tensors.items():
-        if t is not None and t.device != device:
+        if t is not None and t.get_device() != device.index:
             raise ValueError(f"{name} is on {t.device}, expected {device}")
-
-
-def _is_kv4(t):
-    return t is not None and t.dtype == torch.uint8
 
 
 # ----------------------------------------------------------------------------
@@ -68,18 +72,19 @@ def allocate_kv4_cache(num_pages: int, num_kv_heads: int, page_size: int = 128, 
 
 
 def _check_kv4(name, t, num_kv_heads=None):
-    if t.dim() != 4 or t.dtype != torch.uint8 or tuple(t.shape[2:]) != (KV4_TILE, KV4_ROW_BYTES):
-        raise ValueError(f"{name}: a 4-bit cache is uint8 [pages, Hkv, {KV4_TILE}, {KV4_ROW_BYTES}], got {t.dtype} {tuple(t.shape)}")
-    if t.stride(3) != 1 or t.stride(2) != KV4_ROW_BYTES:
+    shape, stride = t.shape, t.stride()
+    if t.dtype != torch.uint8 or len(shape) != 4 or shape[2] != KV4_TILE or shape[3] != KV4_ROW_BYTES:
+        raise ValueError(f"{name}: a 4-bit cache is uint8 [pages, Hkv, {KV4_TILE}, {KV4_ROW_BYTES}], got {t.dtype} {tuple(shape)}")
+    if stride[3] != 1 or stride[2] != KV4_ROW_BYTES:
         raise ValueError(f"{name}: the tile of a page and head of a 4-bit cache must be contiguous")
-    if t.stride(0) % 16 or t.stride(1) % 16 or t.data_ptr() % 16:
+    if stride[0] % 16 or stride[1] % 16 or t.data_ptr() % 16:
         raise ValueError(f"{name}: the tiles of a 4-bit cache must start at multiples of 16 bytes")
-    if num_kv_heads is not None and t.shape[1] != num_kv_heads:
-        raise ValueError(f"{name} has {t.shape[1]} KV heads, expected {num_kv_heads}")
+    if num_kv_heads is not None and shape[1] != num_kv_heads:
+        raise ValueError(f"{name} has {shape[1]} KV heads, expected {num_kv_heads}")
+    return stride
 
 
 def _status(device):
-    from .api import _status_word
     return _status_word(device).data_ptr()
 
 
@@ -88,19 +93,18 @@ def _read(cache, index, out, whole_pages):
         return out
     if cache.shape[0] == 0:
         return out.zero_()
-    a = _lib.MsaKv4ReadArgs()
-    a.cache, a.out, a.slot_map, a.status = cache.data_ptr(), out.data_ptr(), index.data_ptr(), _status(cache.device)
-    a.stride_page, a.stride_head = cache.stride(0), cache.stride(1)
-    a.rows, a.num_kv_heads, a.num_pages, a.whole_pages = index.shape[0], cache.shape[1], cache.shape[0], int(whole_pages)
-    with _on(cache.device):
-        _lib.check(_lib.lib.msa_kv4_read(ctypes.byref(a), _stream()), "msa_kv4_read")
+    dev = cache.device
+    _launch(dev, _lib.lib.msa_kv4_read, _lib.MsaKv4ReadArgs(
+        cache.data_ptr(), out.data_ptr(), index.data_ptr(), _status(dev), cache.stride(0), cache.stride(1), index.shape[0], cache.shape[1],
+        cache.shape[0], whole_pages), "msa_kv4_read")
     return out
 
 
 def _check_index(name, t, device):
     if t.dim() != 1 or t.dtype != torch.int32 or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 vector, got {t.dtype} {tuple(t.shape)}")
-    _same_device(device, **{name: t})
+    if t.get_device() != device.index:
+        raise ValueError(f"{name} is on {t.device}, expected {device}")
 
 
 def kv4_read(cache: torch.Tensor, slot_map: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -173,31 +177,37 @@ def rope_plan(rotary_dim: int = 128, base: float = 10000.0, inv_freq: Optional[U
 _TWO_PI = Fraction(6283185307179586476925286766559005768394, 10 ** 39)
 
 
-def _rows(name, t, heads=None, tokens=None, dtypes=(torch.bfloat16,)):
-    if t.dim() != 3 or t.shape[2] != 128:
-        raise ValueError(f"{name} must be [tokens, heads, 128], got {tuple(t.shape)}")
+def _rows(name, t, heads, tokens, device, dtypes=(torch.bfloat16,)):
+    """Checks of [tokens, heads, 128]; the strides of tokens and heads."""
+    shape = t.shape
+    if len(shape) != 3 or shape[2] != 128 or (heads is not None and shape[1] != heads) or (tokens is not None and shape[0] != tokens):
+        raise ValueError(f"{name} must be [{'tokens' if tokens is None else tokens}, {'heads' if heads is None else heads}, 128], got {tuple(shape)}")
     if t.dtype not in dtypes:
         raise ValueError(f"{name} must be {' or '.join(str(d) for d in dtypes)}, got {t.dtype}")
-    if t.stride(2) != 1:
+    s0, s1, s2 = t.stride()
+    if s2 != 1:
         raise ValueError(f"{name} head_dim must be contiguous")
-    unit = 8 * t.element_size()
-    if t.data_ptr() % unit or (t.stride(0) * t.element_size()) % unit or (t.stride(1) * t.element_size()) % unit:
+    unit = 16 if t.dtype == torch.bfloat16 else 8
+    if t.data_ptr() % unit or s0 % 8 or s1 % 8:
         raise ValueError(f"{name}: rows must start at multiples of {unit} bytes")
-    if (heads is not None and t.shape[1] != heads) or (tokens is not None and t.shape[0] != tokens):
-        raise ValueError(f"{name} must be [{tokens}, {heads}, 128], got {tuple(t.shape)}")
+    if t.get_device() != device.index:
+        raise ValueError(f"{name} is on {t.device}, expected {device}")
+    return s0, s1
 
 
 def _weight(name, w, heads, device):
     if w is None:
         return None, 0
-    _same_device(device, **{name: w})
+    if w.get_device() != device.index:
+        raise ValueError(f"{name} is on {w.device}, expected {device}")
     if w.dtype not in (torch.float32, torch.bfloat16):
         raise ValueError(f"{name} must be float32 or bfloat16, got {w.dtype}")
-    if tuple(w.shape) not in ((128,), (heads, 128)):
-        raise ValueError(f"{name} must be [128] or [{heads}, 128], got {tuple(w.shape)}")
-    if w.stride(-1) != 1 or (w.dim() == 2 and w.stride(0) % 8) or w.data_ptr() % 16:
+    shape, stride = tuple(w.shape), w.stride()
+    if shape != (128,) and shape != (heads, 128):
+        raise ValueError(f"{name} must be [128] or [{heads}, 128], got {shape}")
+    if stride[-1] != 1 or (len(shape) == 2 and stride[0] % 8) or w.data_ptr() % 16:
         raise ValueError(f"{name}: rows must be contiguous and start at multiples of 16 bytes")
-    return w.data_ptr(), w.stride(0) if w.dim() == 2 else 0
+    return w.data_ptr(), stride[0] if len(shape) == 2 else 0
 
 
 def _scale(name, x, heads, device):
@@ -205,64 +215,64 @@ def _scale(name, x, heads, device):
     if x is None:
         return 1.0, None
     if isinstance(x, torch.Tensor):
-        _same_device(device, **{name: x})
         if x.dtype != torch.float32 or x.numel() != heads or not x.is_contiguous():
             raise ValueError(f"{name} must be a float or a contiguous float32 tensor of {heads} values, got {x.dtype} {tuple(x.shape)}")
+        if x.get_device() != device.index:
+            raise ValueError(f"{name} is on {x.device}, expected {device}")
         return 1.0, x.data_ptr()
     return float(x), None
 
 
-def _cache_args(a, k_cache, v_cache, heads, slot_map, tokens, page_size, device):
-    """Fills the fields of the caches; both have the same type, layout and page count."""
-    first = k_cache if k_cache is not None else v_cache
+_CACHE_DTYPES = {torch.bfloat16: MSA_DT_BF16, torch.float8_e4m3fn: MSA_DT_E4M3, torch.uint8: MSA_DT_KV4}
+
+
+def _cache_strides(name, c, dtype, heads, page_size, device):
+    """(pointer, strides of pages, heads, tokens) of one cache."""
+    if c.get_device() != device.index:
+        raise ValueError(f"{name} is on {c.device}, expected {device}")
+    if dtype == MSA_DT_KV4:
+        stride = _check_kv4(name, c, heads)
+        return c.data_ptr(), stride[0], stride[1], 0
+    shape, stride = c.shape, c.stride()
+    if len(shape) != 4 or shape[3] != 128 or stride[3] != 1:
+        raise ValueError(f"{name} must be [pages, Hkv, page, 128] or [pages, page, Hkv, 128], got {tuple(shape)}")
+    unit = 16 if dtype == MSA_DT_BF16 else 8
+    if c.data_ptr() % unit or stride[0] % 8 or stride[1] % 8 or stride[2] % 8:
+        raise ValueError(f"{name}: rows must start at multiples of {unit} bytes")
+    if shape[2] == page_size and shape[1] == heads:
+        return c.data_ptr(), stride[0], stride[1], stride[2]
+    if shape[1] == page_size and shape[2] == heads:
+        return c.data_ptr(), stride[0], stride[2], stride[1]
+    raise ValueError(f"{name} must hold pages of {page_size} tokens and {heads} KV heads, got {tuple(shape)}")
+
+
+def _cache_args(k_cache, v_cache, heads, slot_map, tokens, page_size, k_scale, v_scale, device):
+    """Checks of the caches of a call, which have one type, layout and page count; their type, strides and scales."""
     if slot_map is None:
         raise ValueError("a cache needs slot_map")
     _check_index("slot_map", slot_map, device)
     if slot_map.shape[0] != tokens:
         raise ValueError(f"slot_map must have {tokens} entries, got {slot_map.shape[0]}")
-    _same_device(device, k_cache=k_cache, v_cache=v_cache)
-    if k_cache is not None and v_cache is not None and (k_cache.dtype != v_cache.dtype or k_cache.shape != v_cache.shape):
+    if k_cache.dtype != v_cache.dtype or k_cache.shape != v_cache.shape:
         raise ValueError(f"k_cache and v_cache must be alike, got {k_cache.dtype} {tuple(k_cache.shape)} and {v_cache.dtype} {tuple(v_cache.shape)}")
-    codes = {torch.bfloat16: MSA_DT_BF16, torch.float8_e4m3fn: MSA_DT_E4M3, torch.uint8: MSA_DT_KV4}
-    if first.dtype not in codes:
-        raise ValueError(f"a cache is bfloat16, float8_e4m3fn or uint8 (4 bits), got {first.dtype}")
-    a.cache_dtype = codes[first.dtype]
-    for name, c in (("k_cache", k_cache), ("v_cache", v_cache)):
-        if c is None:
-            continue
-        if a.cache_dtype == MSA_DT_KV4:
-            _check_kv4(name, c, heads)
-            strides, size = (c.stride(0), c.stride(1), 0), KV4_TILE
-        else:
-            if c.dim() != 4 or c.shape[3] != 128 or c.stride(3) != 1:
-                raise ValueError(f"{name} must be [pages, Hkv, page, 128] or [pages, page, Hkv, 128], got {tuple(c.shape)}")
-            unit = 8 * c.element_size()
-            if c.data_ptr() % unit or any((c.stride(i) * c.element_size()) % unit for i in range(3)):
-                raise ValueError(f"{name}: rows must start at multiples of {unit} bytes")
-            if c.shape[2] == page_size and c.shape[1] == heads:
-                strides = (c.stride(0), c.stride(1), c.stride(2))
-            elif c.shape[1] == page_size and c.shape[2] == heads:
-                strides = (c.stride(0), c.stride(2), c.stride(1))
-            else:
-                raise ValueError(f"{name} must hold pages of {page_size} tokens and {heads} KV heads, got {tuple(c.shape)}")
-            size = page_size
-        if name == "k_cache":
-            a.k_cache, (a.k_cache_stride_page, a.k_cache_stride_head, a.k_cache_stride_tok) = c.data_ptr(), strides
-        else:
-            a.v_cache, (a.v_cache_stride_page, a.v_cache_stride_head, a.v_cache_stride_tok) = c.data_ptr(), strides
-        if size != page_size:
-            raise ValueError(f"a 4-bit cache has pages of {KV4_TILE} tokens, got page_size={page_size}")
-    if first.shape[0] * page_size > (1 << 31) - 1:
+    dtype = _CACHE_DTYPES.get(k_cache.dtype)
+    if dtype is None:
+        raise ValueError(f"a cache is bfloat16, float8_e4m3fn or uint8 (4 bits), got {k_cache.dtype}")
+    if dtype == MSA_DT_KV4 and page_size != KV4_TILE:
+        raise ValueError(f"a 4-bit cache has pages of {KV4_TILE} tokens, got page_size={page_size}")
+    if page_size < 1:
+        raise ValueError(f"page_size={page_size} must be positive")
+    if k_cache.shape[0] < 1:
+        raise ValueError("the cache has no pages")
+    if k_cache.shape[0] * page_size > (1 << 31) - 1:
         raise ValueError("slots of a cache of more than 2^31 - 1 tokens do not fit int32")
-    a.slot_map, a.page_size, a.num_pages = slot_map.data_ptr(), page_size, first.shape[0]
+    if dtype == MSA_DT_BF16 and (k_scale is not None or v_scale is not None):
+        raise ValueError("k_scale and v_scale belong to a quantised cache")
+    return (dtype, _cache_strides("k_cache", k_cache, dtype, heads, page_size, device), _cache_strides("v_cache", v_cache, dtype, heads, page_size, device),
+            _scale("k_scale", k_scale, heads, device), _scale("v_scale", v_scale, heads, device))
 
 
-def _cache_scales(a, cache, k_scale, v_scale, heads, device):
-    if cache is None or cache.dtype == torch.bfloat16:
-        if k_scale is not None or v_scale is not None:
-            raise ValueError("k_scale and v_scale belong to a quantised cache")
-    a.k_scale, a.k_scale_head = _scale("k_scale", k_scale, heads, device)
-    a.v_scale, a.v_scale_head = _scale("v_scale", v_scale, heads, device)
+_NO_CACHE = (MSA_DT_BF16, (None, 0, 0, 0), (None, 0, 0, 0), (1.0, None), (1.0, None))
 
 
 def qk_norm_rope(
@@ -302,64 +312,65 @@ def qk_norm_rope(
     if not q.is_cuda:
         raise RuntimeError("qk_norm_rope needs CUDA tensors (there is no CPU path)")
     dev = q.device
-    _rows("q", q)
+    q_strides = _rows("q", q, None, None, dev)
     T, hq = q.shape[0], q.shape[1]
-    _rows("k", k, tokens=T, heads=k.shape[1] if k.dim() == 3 else None)
+    k_strides = _rows("k", k, None, T, dev)
     hk = k.shape[1]
-    _same_device(dev, k=k, v=v, positions=positions, q_out=q_out, k_out=k_out)
-    a = _lib.MsaNormRopeArgs()
     if rope is not None:
         if positions is None:
             raise ValueError("a rotation needs positions")
-        if positions.dtype not in (torch.int32, torch.int64):
+        if positions.dtype != torch.int32 and positions.dtype != torch.int64:
             raise ValueError(f"positions must be int32 or int64, got {positions.dtype}")
-        if tuple(positions.shape) != (rope["axes"], T) and not (rope["axes"] == 1 and tuple(positions.shape) == (T,)):
-            raise ValueError(f"positions must be [{rope['axes']}, {T}]" + (f" or [{T}]" if rope["axes"] == 1 else "") + f", got {tuple(positions.shape)}")
-        if T and positions.stride(-1) != 1 and T > 1:
+        axes, shape = rope["axes"], tuple(positions.shape)
+        if shape != (axes, T) and not (axes == 1 and shape == (T,)):
+            raise ValueError(f"positions must be [{axes}, {T}]" + (f" or [{T}]" if axes == 1 else "") + f", got {shape}")
+        pos_stride = positions.stride()
+        if T > 1 and pos_stride[-1] != 1:
             raise ValueError("positions of one axis must be contiguous")
-        _same_device(dev, rope=rope["turns"])
-        a.positions, a.pos_int64 = positions.data_ptr(), int(positions.dtype == torch.int64)
-        a.pos_stride_axis = positions.stride(0) if positions.dim() == 2 else 0
-        a.turns, a.axis = rope["turns"].data_ptr(), rope["axis"].data_ptr()
-        a.rotary, a.interleaved = rope["rotary_dim"], int(rope["interleaved"])
+        turns, axis = rope["turns"], rope["axis"]
+        if positions.get_device() != dev.index or turns.get_device() != dev.index:
+            raise ValueError(f"positions are on {positions.device} and the rope plan is on {turns.device}, expected {dev}")
+        pos = (positions.data_ptr(), turns.data_ptr(), axis.data_ptr(), pos_stride[0] if len(shape) == 2 else 0, rope["rotary_dim"],
+               rope["interleaved"], positions.dtype == torch.int64)
+    else:
+        pos = (None, None, None, 0, 0, 0, 0)
     if (k_cache is None) != (v_cache is None) or (v_cache is None) != (v is None):
         raise ValueError("k_cache, v_cache and v go together")
     if k_cache is not None:
-        _rows("v", v, tokens=T, heads=hk)
-        a.v, a.v_stride_tok, a.v_stride_head = v.data_ptr(), v.stride(0), v.stride(1)
-        _cache_args(a, k_cache, v_cache, hk, slot_map, T, page_size, dev)
-    _cache_scales(a, k_cache, k_scale, v_scale, hk, dev)
-    if q_out is None:
-        q_out = torch.empty(T, hq, 128, dtype=torch.bfloat16, device=dev)
+        v_strides = _rows("v", v, hk, T, dev)
+        dtype, kc, vc, ks, vs = _cache_args(k_cache, v_cache, hk, slot_map, T, page_size, k_scale, v_scale, dev)
+        v_ptr, slots, num_pages = v.data_ptr(), slot_map.data_ptr(), k_cache.shape[0]
     else:
-        _rows("q_out", q_out, heads=hq, tokens=T, dtypes=(torch.bfloat16, torch.float8_e4m3fn))
-    if q_scale is not None and q_out.dtype != torch.float8_e4m3fn:
+        if k_scale is not None or v_scale is not None or slot_map is not None:
+            raise ValueError("slot_map, k_scale and v_scale belong to a cache")
+        dtype, kc, vc, ks, vs = _NO_CACHE
+        v_ptr, v_strides, slots, num_pages = None, (0, 0), None, 0
+    if q_out is None:
+        q_out = torch.empty(q.shape, dtype=torch.bfloat16, device=dev)
+        qo_strides = (hq * 128, 128)
+    else:
+        qo_strides = _rows("q_out", q_out, hq, T, dev, (torch.bfloat16, torch.float8_e4m3fn))
+    q8 = q_out.dtype == torch.float8_e4m3fn
+    if q_scale is not None and not q8:
         raise ValueError("q_scale belongs to an e4m3 q_out")
     if k_out is None and k_cache is None:
-        k_out = torch.empty(T, hk, 128, dtype=torch.bfloat16, device=dev)
-    elif k_out is not None:
-        _rows("k_out", k_out, heads=hk, tokens=T)
-    a.q, a.q_stride_tok, a.q_stride_head = q.data_ptr(), q.stride(0), q.stride(1)
-    a.k, a.k_stride_tok, a.k_stride_head = k.data_ptr(), k.stride(0), k.stride(1)
-    a.q_out, a.q_out_stride_tok, a.q_out_stride_head = q_out.data_ptr(), q_out.stride(0), q_out.stride(1)
-    a.q_out_dtype = MSA_DT_E4M3 if q_out.dtype == torch.float8_e4m3fn else MSA_DT_BF16
-    if k_out is not None:
-        a.k_out, a.k_out_stride_tok, a.k_out_stride_head = k_out.data_ptr(), k_out.stride(0), k_out.stride(1)
+        k_out = torch.empty(k.shape, dtype=torch.bfloat16, device=dev)
+    ko_strides = _rows("k_out", k_out, hk, T, dev) if k_out is not None else (0, 0)
     if not norm and (q_weight is not None or k_weight is not None):
         raise ValueError("weights belong to the norm")
     if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
         raise ValueError(f"q_weight and k_weight must have one dtype, got {q_weight.dtype} and {k_weight.dtype}")
-    a.q_weight, a.q_weight_stride = _weight("q_weight", q_weight, hq, dev)
-    a.k_weight, a.k_weight_stride = _weight("k_weight", k_weight, hk, dev)
+    qw, qw_stride = _weight("q_weight", q_weight, hq, dev)
+    kw, kw_stride = _weight("k_weight", k_weight, hk, dev)
     w = q_weight if q_weight is not None else k_weight
-    a.weight_dtype = MSA_DT_BF16 if w is not None and w.dtype == torch.bfloat16 else MSA_DT_F32
-    a.tokens, a.num_qo_heads, a.num_kv_heads, a.norm, a.eps = T, hq, hk, int(bool(norm)), float(eps)
-    a.q_scale = 1.0 if q_scale is None else float(q_scale)
-    a.status = _status(dev)
     if T == 0:
         return q_out, k_out
-    with _on(dev):
-        _lib.check(_lib.lib.msa_norm_rope(ctypes.byref(a), _stream()), "msa_norm_rope")
+    _launch(dev, _lib.lib.msa_norm_rope, _lib.MsaNormRopeArgs(
+        q.data_ptr(), k.data_ptr(), v_ptr, qw, kw, pos[0], pos[1], pos[2], q_out.data_ptr(), None if k_out is None else k_out.data_ptr(),
+        kc[0], vc[0], slots, ks[1], vs[1], _status(dev), pos[3], *q_strides, *k_strides, *v_strides, *qo_strides, *ko_strides, qw_stride, kw_stride,
+        kc[1], kc[2], kc[3], vc[1], vc[2], vc[3], T, hq, hk, pos[4], pos[5], 1 if norm else 0,
+        MSA_DT_BF16 if w is not None and w.dtype == torch.bfloat16 else MSA_DT_F32, MSA_DT_E4M3 if q8 else MSA_DT_BF16, dtype, pos[6],
+        page_size if slots is not None else 0, num_pages, eps, 1.0 if q_scale is None else q_scale, ks[0], vs[0]), "msa_norm_rope")
     return q_out, k_out
 
 
@@ -370,20 +381,22 @@ def kv_cache_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_c
     if not k.is_cuda:
         raise RuntimeError("kv_cache_append needs CUDA tensors (there is no CPU path)")
     dev = k.device
-    _rows("k", k)
+    k_strides = _rows("k", k, None, None, dev)
     T, hk = k.shape[0], k.shape[1]
-    _rows("v", v, heads=hk, tokens=T)
-    _same_device(dev, v=v)
-    a = _lib.MsaNormRopeArgs()
-    _cache_args(a, k_cache, v_cache, hk, slot_map, T, page_size, dev)
-    _cache_scales(a, k_cache, k_scale, v_scale, hk, dev)
-    a.k, a.k_stride_tok, a.k_stride_head = k.data_ptr(), k.stride(0), k.stride(1)
-    a.v, a.v_stride_tok, a.v_stride_head = v.data_ptr(), v.stride(0), v.stride(1)
-    a.tokens, a.num_kv_heads, a.weight_dtype, a.status = T, hk, MSA_DT_F32, _status(dev)
+    v_strides = _rows("v", v, hk, T, dev)
+    dtype, kc, vc, ks, vs = _cache_args(k_cache, v_cache, hk, slot_map, T, page_size, k_scale, v_scale, dev)
     if T == 0:
         return
-    with _on(dev):
-        _lib.check(_lib.lib.msa_norm_rope(ctypes.byref(a), _stream()), "msa_norm_rope")
+    a = _lib.MsaNormRopeArgs()
+    a.k, a.v, a.slot_map, a.status = k.data_ptr(), v.data_ptr(), slot_map.data_ptr(), _status(dev)
+    a.k_stride_tok, a.k_stride_head = k_strides
+    a.v_stride_tok, a.v_stride_head = v_strides
+    a.k_cache, a.k_cache_stride_page, a.k_cache_stride_head, a.k_cache_stride_tok = kc
+    a.v_cache, a.v_cache_stride_page, a.v_cache_stride_head, a.v_cache_stride_tok = vc
+    (a.k_scale, a.k_scale_head), (a.v_scale, a.v_scale_head) = ks, vs
+    a.cache_dtype, a.page_size, a.num_pages = dtype, page_size, k_cache.shape[0]
+    a.tokens, a.num_kv_heads, a.weight_dtype = T, hk, MSA_DT_F32
+    _launch(dev, _lib.lib.msa_norm_rope, a, "msa_norm_rope")
 
 
 # ----------------------------------------------------------------------------
@@ -456,39 +469,29 @@ def paged_kv_tables(
             if n is not None and t.shape[0] != n:
                 raise ValueError(f"{name} must have {n} entries, got {t.shape[0]}")
         sizes.update(num_held=B, num_free=1)
-    _same_device(dev, block_table=block_table)
+    if block_table.get_device() != dev.index:
+        raise ValueError(f"block_table is on {block_table.device}, expected {dev}")
     if out is not None:
         for name, n in sizes.items():
             _check_index(f"out[{name!r}]", out[name], dev)
             if out[name].shape[0] != n:
                 raise ValueError(f"out[{name!r}] must have {n} entries, got {out[name].shape[0]}")
-    res = PageTables()
-    given = {"num_held": num_held_out, "num_free": num_free_out}
-    need = [(name, n) for name, n in sizes.items() if given.get(name) is None and out is None]
-    ws_bytes = _lib.check(_lib.lib.msa_page_tables_workspace_bytes(B), "msa_page_tables_workspace_bytes")
-    with _on(dev):
-        # one allocation for the outputs (each on a 256-byte boundary) and the scans
-        at, total = {}, 0
-        for name, n in need + [("", ws_bytes // 4)]:
-            at[name] = total
-            total += (n + 63) & ~63
-        block = torch.empty(total, dtype=torch.int32, device=dev)
-        for name, n in sizes.items():
-            if given.get(name) is not None:
-                res[name] = given[name]
-            else:
-                res[name] = out[name] if out is not None else block[at[name]:at[name] + n]
-        a = _lib.MsaPageTablesArgs()
-        a.qo_len, a.kv_len, a.block_table = qo_lens.data_ptr(), kv_lens.data_ptr(), block_table.data_ptr()
-        a.kv_indices, a.kv_page_indptr = res["kv_indices"].data_ptr(), res["kv_page_indptr"].data_ptr()
-        a.slot_map, a.positions, a.num_missing = res["slot_map"].data_ptr(), res["positions"].data_ptr(), res["num_missing"].data_ptr()
-        if alloc:
-            a.num_held, a.free_pages, a.num_free = num_held.data_ptr(), free_pages.data_ptr(), num_free.data_ptr()
-            a.num_held_out, a.num_free_out = res["num_held"].data_ptr(), res["num_free"].data_ptr()
-            a.free_capacity = free_pages.shape[0]
-        a.workspace = block.data_ptr() + 4 * at[""]
-        a.table_stride = block_table.stride(0) if B > 1 else width
-        a.batch, a.table_width, a.page_size = B, width, page_size
-        a.max_total_q, a.max_total_pages = max_total_q, total_pages
-        _lib.check(_lib.lib.msa_page_tables(ctypes.byref(a), _stream()), "msa_page_tables")
+    ws_ints = (_lib.check(_lib.lib.msa_page_tables_workspace_bytes(B), "msa_page_tables_workspace_bytes") + 3) // 4
+    given = {"num_held": num_held_out, "num_free": num_free_out} if out is None else {**out, **{
+        name: t for name, t in (("num_held", num_held_out), ("num_free", num_free_out)) if t is not None}}
+    names = [name for name in sizes if given.get(name) is None]
+    # one allocation for the outputs and the scans
+    counts = [sizes[name] for name in names] + [ws_ints]
+    parts = torch.empty(sum(counts), dtype=torch.int32, device=dev).split_with_sizes(counts)
+    res = PageTables(zip(names, parts))
+    for name in sizes:
+        if name not in res:
+            res[name] = given[name]
+    null = (None, None, None, None, None, 0)
+    held = (num_held.data_ptr(), free_pages.data_ptr(), num_free.data_ptr(), res["num_held"].data_ptr(), res["num_free"].data_ptr(),
+            free_pages.shape[0]) if alloc else null
+    _launch(dev, _lib.lib.msa_page_tables, _lib.MsaPageTablesArgs(
+        qo_lens.data_ptr(), kv_lens.data_ptr(), block_table.data_ptr(), held[0], held[1], held[2], res["kv_indices"].data_ptr(),
+        res["kv_page_indptr"].data_ptr(), res["slot_map"].data_ptr(), res["positions"].data_ptr(), held[3], held[4], res["num_missing"].data_ptr(),
+        parts[-1].data_ptr(), block_table.stride(0) if B > 1 else width, B, width, page_size, max_total_q, total_pages, held[5]), "msa_page_tables")
     return res
