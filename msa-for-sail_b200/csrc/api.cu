@@ -166,8 +166,11 @@ extern "C" int msa_plan_dense(const MsaPlanArgs* a, MsaWorkItem* work, int32_t c
       for (int b = 0; b < a->batch; ++b) rows += static_cast<long long>(a->qo_len[b]) * a->num_qo_heads;
       rows = std::max(1LL, rows);
       const int plain_splits = (max_tiles + chunk - 1) / chunk;
-      long long most = std::min<long long>(ceiling, std::max<long long>(plain_splits, 4LL * sms * a->block_m / rows));
-      if (plain_splits * rows <= MSA_STATIC_SCRATCH_MAX_ROWS) most = std::min(most, MSA_STATIC_SCRATCH_MAX_ROWS / rows);
+      // (Three or more items to an SM: pieces so small that the cut they need has more rows, 0.5 KB each.  The kernel that runs
+      // so has partials of its own call, and no form with the library's scratch.)
+      const bool many = a->ctas_per_sm > 2;
+      long long most = std::min<long long>(ceiling, std::max<long long>(plain_splits, (many ? 16LL * slots : 4LL * sms) * a->block_m / rows));
+      if (!many && plain_splits * rows <= MSA_STATIC_SCRATCH_MAX_ROWS) most = std::min(most, MSA_STATIC_SCRATCH_MAX_ROWS / rows);
       cut = std::max(cut, static_cast<int>((max_tiles + most - 1) / most));
       if (cut < max_tiles && msa::makespan(protos, groups, cut, slots) < msa::makespan(protos, groups, chunk, slots)) chunk = cut;
     }
