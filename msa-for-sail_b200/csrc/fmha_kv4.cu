@@ -507,6 +507,8 @@ int launch(const MsaFmhaParams& p, int rows, cudaStream_t stream) {
 }  // namespace
 }  // namespace kv4
 
+int fmha_kv4_tc_launch(const MsaFmhaParams& p, int rows, cudaStream_t stream);
+
 // Checks of the fields that the 4-bit pass reads, and the launch.  Nothing here touches the device before the checks are through.
 int fmha_kv4_fwd(const MsaFmhaParams& p, cudaStream_t stream) {
   const bool sparse = (p.flags & MSA_FLAG_SPARSE) != 0;
@@ -537,6 +539,7 @@ int fmha_kv4_fwd(const MsaFmhaParams& p, cudaStream_t stream) {
       p.v_stride_head % 16 || (p.out && ((p.out_stride_tok * 2) % 16 || (p.out_stride_head * 2) % 16)))
     return MSA_ERR_BAD_ARG;
   if (p.total_q == 0 || p.kv_extent == 0) return p.total_q == 0 ? MSA_OK : MSA_ERR_BAD_ARG;
+  if (!sparse && rows > 16) return fmha_kv4_tc_launch(p, rows, stream);
   return rows <= 8 ? kv4::launch<1>(p, rows, stream) : kv4::launch<2>(p, rows, stream);
 }
 }  // namespace msa

@@ -146,7 +146,7 @@ def _sparse_splits(items, kv_block_num, num_kv_splits, num_sms, two_per_sm, ctas
 
 
 def _kv4_ctas(rows):
-    """CTAs of the 4-bit decode kernel that share an SM, by the rows of a work item (groups of 16 are CTAs of their own)."""
+    """CTAs of the 4-bit decode kernel of up to 16 rows that share an SM."""
     return 4 if rows <= 8 else 3
 
 
@@ -407,13 +407,11 @@ def _fmha_sail_plan(
                 info["num_work_tc"] = n_tc
         # Two CTAs of the e4m3 decode kernel share an SM.  A cut at the average load may take more partials than a workspace
         # sized for the plain cut holds: such a workspace gets the plain cut.
-        shared, plan_sms = 1 if max_qo * pack > 16 else (_kv4_ctas(max_qo * pack) if use_kv4_cache else (2 if use_fp8_kvcache else 1)), num_sms
-        if use_kv4_cache and max_qo * pack > 16:              # the 4-bit kernel has a CTA for each 16 rows of an item
-            plan_sms = max(1, num_sms * _kv4_ctas(16) // -(-max_qo * pack // 16))
+        shared = 1 if max_qo * pack > 16 else (_kv4_ctas(max_qo * pack) if use_kv4_cache else (2 if use_fp8_kvcache else 1))
         for ctas in (shared, -1):
             args = _lib.MsaPlanArgs(
                 a_q.ctypes.data, a_k.ctypes.data, a_o.ctypes.data, batch, num_qo_heads, hkv, block_m, pack,
-                num_kv_splits if num_kv_splits >= 1 else -128, plan_sms, ctas)
+                num_kv_splits if num_kv_splits >= 1 else -128, num_sms, ctas)
             cap = 1024
             spr = np.ones(max(1, total_q), np.int32)
             max_splits = _lib._i32(1)
