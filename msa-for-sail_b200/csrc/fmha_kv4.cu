@@ -112,6 +112,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::CTAS) kv4_decode_kernel(con
   const int h_r = p.num_qo_heads / p.num_kv_heads;
   const int rg = blockIdx.y * (8 * NT);                      // first row of this CTA's group
   Item it;
+  int first_blocks = -1;                                     // this lane's entry of a selection: on its way before the loads that depend on the batch item
   if (!sparse) {
     const MsaWorkItem w = p.work[blockIdx.x];
     it.b = chk(w.batch, 0, p.batch, p.status);
@@ -127,14 +128,15 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::CTAS) kv4_decode_kernel(con
     it.split = idx % p.num_splits; idx /= p.num_splits;
     it.kvh = idx % p.num_kv_heads;
     const int t = idx / p.num_kv_heads;
-    it.b = chk(p.token_batch[t], 0, p.batch, p.status);
-    it.head0 = it.kvh * h_r; it.pack = h_r;
-    it.tok0 = t - p.qo_start[it.b];
-    it.row0 = rg; it.nrows = min(8 * NT, h_r - rg);
     const int per = (p.kv_block_num + p.num_splits - 1) / p.num_splits;
     it.first = it.split * per;
     it.last = min(p.kv_block_num, it.first + per);
     it.blocks = p.kv_block_indexes + t * p.kbi_stride_tok + it.kvh * p.kbi_stride_head;
+    if (it.first + lane < it.last) first_blocks = it.blocks[it.first + lane];
+    it.b = chk(p.token_batch[t], 0, p.batch, p.status);
+    it.head0 = it.kvh * h_r; it.pack = h_r;
+    it.tok0 = t - p.qo_start[it.b];
+    it.row0 = rg; it.nrows = min(8 * NT, h_r - rg);
   }
   if (it.nrows <= 0) return;
   it.qo_base = p.qo_start[it.b];
@@ -156,7 +158,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::CTAS) kv4_decode_kernel(con
   int phys = -1, aux = -1;
   auto load_entries = [&](int j0) {
     if (it.blocks) {
-      aux = j0 + lane < n_tiles ? it.blocks[it.first + j0 + lane] : -1;
+      aux = j0 == 0 ? first_blocks : (j0 + lane < n_tiles ? it.blocks[it.first + j0 + lane] : -1);
       phys = aux >= 0 && aux < (lim_last + kKvTile - 1) / kKvTile ? physical(aux) : -1;
     } else {
       phys = j0 > 0 ? aux : (lane < n_tiles ? physical(it.first + lane) : -1);

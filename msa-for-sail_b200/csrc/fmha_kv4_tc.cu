@@ -41,7 +41,7 @@ constexpr int MMA_WARP = 4, PV_WARP = 5, CONVERT_WARP0 = 8, CONVERT_WARPS = 8;  
 constexpr int NTHREADS = 32 * (CONVERT_WARP0 + 2 * CONVERT_WARPS);
 // What the launch allocates (threads x compiled registers) must cover the registers after the moves, or the increase never
 // completes: the launcher checks it.
-constexpr int REGS_SOFTMAX = 152, REGS_MMA = 40, REGS_CONVERT = 64;
+constexpr int REGS_SOFTMAX = 208, REGS_MMA = 40, REGS_CONVERT = 56;
 constexpr int REGS_NEEDED = 128 * (REGS_SOFTMAX + REGS_MMA + 4 * REGS_CONVERT);
 static_assert(NTHREADS == 6 * 128, "warpgroups");
 constexpr int STAGES = 2;                                    // tiles of K and of V
@@ -248,235 +248,231 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv4_tc_kernel(const __grid_consta
     // =========================== softmax / epilogue ===========================
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_SOFTMAX));
     if (warp < n_active) {
-    const int trow = (warp << 5) | lane;                     // row of the tile, TMEM lane
-    const int r = trow % ROWS, part = trow / ROWS;           // row of the item, copy
-    const uint32_t lane_addr = static_cast<uint32_t>(warp << 5) << 16;
-    const uint32_t tO = tmem + O_COL + lane_addr;
-    const bool row_ok = r < nrows;
-    const int row = w.row0 + min(r, nrows - 1);
-    const int64_t tok = qo_base + row / G;
-    const int head = head0 + row % G;
-    const int limit = lim(min(r, nrows - 1));
-    float fac = 1.f;
-    {
-      const float scale = p.sm_scale * (p.k_scale_head ? p.k_scale_head[kvh] : 1.f) * kLog2e;
-      const int64_t at = tok * p.q_stride_tok + head * p.q_stride_head;
-      const bool e4m3 = p.q_dtype == MSA_DT_E4M3;
-      auto load8 = [&](int c, float (&x)[8]) {               // elements 8 c .. 8 c + 7
-        if (e4m3) {
-          const uint2 raw = *reinterpret_cast<const uint2*>(static_cast<const unsigned char*>(p.q) + at + 8 * c);
+      const int trow = (warp << 5) | lane;                     // row of the tile, TMEM lane
+      const int r = trow % ROWS, part = trow / ROWS;           // row of the item, copy
+      const uint32_t lane_addr = static_cast<uint32_t>(warp << 5) << 16;
+      const uint32_t tO = tmem + O_COL + lane_addr;
+      const bool row_ok = r < nrows;
+      const int row = w.row0 + min(r, nrows - 1);
+      const int64_t tok = qo_base + row / G;
+      const int head = head0 + row % G;
+      const int limit = lim(min(r, nrows - 1));
+      float fac = 1.f;
+      {
+        const float scale = p.sm_scale * (p.k_scale_head ? p.k_scale_head[kvh] : 1.f) * kLog2e;
+        const int64_t at = tok * p.q_stride_tok + head * p.q_stride_head;
+        const bool e4m3 = p.q_dtype == MSA_DT_E4M3;
+        auto load8 = [&](int c, float (&x)[8]) {               // elements 8 c .. 8 c + 7
+          if (e4m3) {
+            const uint2 raw = *reinterpret_cast<const uint2*>(static_cast<const unsigned char*>(p.q) + at + 8 * c);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t h = kv4_scales_to_half(static_cast<uint16_t>((i < 2 ? raw.x : raw.y) >> (16 * (i & 1))));
-            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
-            x[2 * i] = f.x; x[2 * i + 1] = f.y;
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t h = kv4_scales_to_half(static_cast<uint16_t>((i < 2 ? raw.x : raw.y) >> (16 * (i & 1))));
+              const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+              x[2 * i] = f.x; x[2 * i + 1] = f.y;
+            }
+          } else {
+            const uint4 raw = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.q) + at + 8 * c);
+            const uint32_t v[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) { x[2 * i] = __uint_as_float(v[i] << 16); x[2 * i + 1] = __uint_as_float(v[i] & 0xffff0000u); }
           }
-        } else {
-          const uint4 raw = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.q) + at + 8 * c);
-          const uint32_t v[4] = {raw.x, raw.y, raw.z, raw.w};
+        };
+        float top = 0.f;
+#pragma unroll 4
+        for (int c = 0; c < 16; ++c) {
+          float x[8];
+          load8(c, x);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) { x[2 * i] = __uint_as_float(v[i] << 16); x[2 * i + 1] = __uint_as_float(v[i] & 0xffff0000u); }
+          for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[i]));
         }
-      };
-      float top = 0.f;
+        // exponent of the largest element; a row of zeros or with an infinity is taken as it is.  The factor of the scores is made
+        // positive (its sign goes to Q), so that the largest score has the largest exponent.
+        int e = static_cast<int>(__float_as_uint(top) >> 23) - 127 - 14;
+        if (top == 0.f || !(top < INFINITY)) e = 0;
+        e = max(e, -126);
+        const float up = copysignf(scale == 0.f ? 0.f : __uint_as_float(static_cast<uint32_t>(127 - e) << 23), scale);
+        if (scale != 0.f) fac = fabsf(scale) * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
 #pragma unroll 4
-      for (int c = 0; c < 16; ++c) {
-        float x[8];
-        load8(c, x);
+        for (int c = 0; c < 16; ++c) {
+          float x[8];
+          load8(c, x);
+          *reinterpret_cast<uint4*>(smem + OFF_Q + tile_at(trow, c)) = make_uint4(pack2<true>(x[0] * up, x[1] * up), pack2<true>(x[2] * up, x[3] * up),
+                                                                            pack2<true>(x[4] * up, x[5] * up), pack2<true>(x[6] * up, x[7] * up));
+        }
+        fence_proxy_async_smem();
+        mbar_arrive(bar(Q_FULL));
+      }
+      float m = kNoMax, l = 0.f;                               // maximum - kPOffset, sum of P
+      bool alive = true;
+      for (int j = 0; j < n_tiles && alive; ++j) {
+        const uint32_t tS = tmem + (j & 1) * BN + lane_addr;
+        alive = mbar_wait_warp(bar(S_FULL + j % STAGES), (j / STAGES) & 1, abort_flag);
+        if (!alive) break;
+        tc_fence_after();
+        const int key0 = (first + j) * BN + part * COLS;       // of this thread
+        const bool edge = (first + j) * BN + BN > lim_first;
+        constexpr int CH = COLS / 32;
+        uint32_t sv[CH][32];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[i]));
-      }
-      // exponent of the largest element; a row of zeros or with an infinity is taken as it is.  The factor of the scores is made
-      // positive (its sign goes to Q), so that the largest score has the largest exponent.
-      int e = static_cast<int>(__float_as_uint(top) >> 23) - 127 - 14;
-      if (top == 0.f || !(top < INFINITY)) e = 0;
-      e = max(e, -126);
-      const float up = copysignf(scale == 0.f ? 0.f : __uint_as_float(static_cast<uint32_t>(127 - e) << 23), scale);
-      if (scale != 0.f) fac = fabsf(scale) * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
-#pragma unroll 4
-      for (int c = 0; c < 16; ++c) {
-        float x[8];
-        load8(c, x);
-        *reinterpret_cast<uint4*>(smem + OFF_Q + tile_at(trow, c)) = make_uint4(pack2<true>(x[0] * up, x[1] * up), pack2<true>(x[2] * up, x[3] * up),
-                                                                          pack2<true>(x[4] * up, x[5] * up), pack2<true>(x[6] * up, x[7] * up));
-      }
-      fence_proxy_async_smem();
-      mbar_arrive(bar(Q_FULL));
-    }
-    float m = kNoMax, l = 0.f;                               // maximum - kPOffset, sum of P
-    bool alive = true;
-    for (int j = 0; j < n_tiles && alive; ++j) {
-      const uint32_t tS = tmem + (j & 1) * BN + lane_addr;
-      alive = mbar_wait_warp(bar(S_FULL + j % STAGES), (j / STAGES) & 1, abort_flag);
-      if (!alive) break;
-      tc_fence_after();
-      const int key0 = (first + j) * BN + part * COLS;       // of this thread
-      const bool edge = (first + j) * BN + BN > lim_first;
-      constexpr int CH = COLS / 32;
-      constexpr bool TWICE = CH > 2;                         // a whole page of S does not stay in registers: it is read twice
-      uint32_t sv[TWICE ? 1 : CH][32];
-      auto load_s = [&](int c, uint32_t (&x)[32]) {
-        tmem_ld32(tS + part * COLS + 32 * c, x);
+        for (int c = 0; c < CH; ++c) tmem_ld32(tS + part * COLS + 32 * c, sv[c]);
         tmem_wait_ld();
         if (edge) {
 #pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (key0 + 32 * c + e >= limit) x[e] = 0xff800000u;
+          for (int c = 0; c < CH; ++c)
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (key0 + 32 * c + e >= limit) sv[c][e] = 0xff800000u;
+        }
+        float top = -INFINITY, t2 = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+#pragma unroll
+          for (int e = 0; e < 32; e += 4) {
+            top = max3(top, __uint_as_float(sv[c][e]), __uint_as_float(sv[c][e + 1]));
+            t2 = max3(t2, __uint_as_float(sv[c][e + 2]), __uint_as_float(sv[c][e + 3]));
+          }
+        top = fmaxf(top, t2) * fac;
+        const bool raise = top > m + (kPOffset + kRescale);
+        if (__any_sync(0xffffffffu, raise)) {
+          const float now = raise ? top - kPOffset : m;
+          const float keep = exp2_fast(m - now);
+          m = now;
+          l *= keep;
+          if (j > 0) {                                         // O may still be the target of P_{j-1} V_{j-1}
+            // (V_EMPTY of tile j - 3 was seen before S_{j-1} was computed: the phase is this one)
+            alive = mbar_wait_warp(bar(V_EMPTY + (j - 1) % STAGES), ((j - 1) / STAGES) & 1, abort_flag);
+            if (!alive) break;
+            tc_fence_after();
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              uint32_t v[32];
+              tmem_ld32(tO + c * 32, v);
+              tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * keep);
+              tmem_st32(tO + c * 32, v);
+            }
+          }
+        }
+        const uint64_t f2 = f2_pack(fac, fac), shift = f2_pack(-m, -m);
+        uint64_t l2 = 0;
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {                         // P overwrites the first half of S
+          uint32_t pk[16];
+          const uint32_t (&x)[32] = sv[c];
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            float x0, x1;
+            f2_unpack(f2_fma(f2_pack(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), f2, shift), x0, x1);
+            const float p0 = exp2_fast(x0), p1 = exp2_fast(x1);
+            l2 = f2_add(l2, f2_pack(p0, p1));
+            pk[e >> 1] = pack2<true>(p0, p1);
+          }
+          tmem_st16(tS + part * (COLS / 2) + c * 16, pk);
+        }
+        if constexpr (F > 1) {                                 // the keys of the other copies
+          uint32_t zero[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) zero[e] = 0u;
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            if (c / CH != part) tmem_st16(tS + c * 16, zero);
+        }
+        float la, lb;
+        f2_unpack(l2, la, lb);
+        l += la + lb;
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(bar(P_FULL + j % STAGES));
+      }
+      // ---- epilogue ----
+      if (alive && n_tiles > 0) alive = mbar_wait_warp(bar(O_DONE), 0, abort_flag);
+      const float vs = p.v_scale_head ? p.v_scale_head[kvh] : 1.f;
+      const int64_t prow = (static_cast<int64_t>(split) * p.total_q + tok) * p.num_qo_heads + head;
+      // columns c0 .. c0 + 7 of a row of the result; tok_, head_, prow_: the row
+      auto store8 = [&](const float (&v)[8], int c0, int64_t tok_, int head_, int64_t prow_) {
+        if (p.partial_o) {
+          float* dst = p.partial_o + prow_ * kHeadDim + c0;
+          *reinterpret_cast<float4*>(dst) = make_float4(v[0], v[1], v[2], v[3]);
+          *reinterpret_cast<float4*>(dst + 4) = make_float4(v[4], v[5], v[6], v[7]);
+        } else {
+          *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.out) + tok_ * p.out_stride_tok + head_ * p.out_stride_head + c0) =
+              make_uint4(pack2<false>(v[0], v[1]), pack2<false>(v[2], v[3]), pack2<false>(v[4], v[5]), pack2<false>(v[6], v[7]));
         }
       };
-      float top = -INFINITY, t2 = -INFINITY;
+      auto store_lse = [&](float lse, int64_t tok_, int head_, int64_t prow_) {
+        if (p.partial_o) p.partial_lse[prow_] = lse;
+        else if (p.lse) p.lse[tok_ * p.num_qo_heads + head_] = lse;
+      };
+      const float to_out = p.partial_o ? vs : vs * p.out_scale;
+      // F > 1: every MMA and conversion of the CTA is done, the tiles of K and V hold the F results of a row
+      float* stage = reinterpret_cast<float*>(smem + OFF_K);   // [128 rows of the tile][LD_O], then maximum and sum of each
+      constexpr int LD_O = kHeadDim + 4;
+      float* st_m = stage + BM * LD_O;
+      static_assert(BM * (LD_O + 2) * 4 <= 2 * STAGES * TILE_BYTES, "results fit the tiles");
+      if (alive) {
+        tc_fence_after();
+        const bool none = l == 0.f;
+        const float inv = F > 1 ? 1.f : (none ? 0.f : to_out / l);
 #pragma unroll
-      for (int c = 0; c < CH; ++c) {
-        uint32_t (&x)[32] = sv[TWICE ? 0 : c];
-        load_s(c, x);
-#pragma unroll
-        for (int e = 0; e < 32; e += 4) {
-          top = max3(top, __uint_as_float(x[e]), __uint_as_float(x[e + 1]));
-          t2 = max3(t2, __uint_as_float(x[e + 2]), __uint_as_float(x[e + 3]));
-        }
-      }
-      top = fmaxf(top, t2) * fac;
-      const bool raise = top > m + (kPOffset + kRescale);
-      if (__any_sync(0xffffffffu, raise)) {
-        const float now = raise ? top - kPOffset : m;
-        const float keep = exp2_fast(m - now);
-        m = now;
-        l *= keep;
-        if (j > 0) {                                         // O may still be the target of P_{j-1} V_{j-1}
-          // (V_EMPTY of tile j - 3 was seen before S_{j-1} was computed: the phase is this one)
-          alive = mbar_wait_warp(bar(V_EMPTY + (j - 1) % STAGES), ((j - 1) / STAGES) & 1, abort_flag);
-          if (!alive) break;
-          tc_fence_after();
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t v[32];
+        for (int c = 0; c < 4; ++c) {
+          uint32_t v[32];
+          if (n_tiles > 0) {
             tmem_ld32(tO + c * 32, v);
             tmem_wait_ld();
-#pragma unroll
-            for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * keep);
-            tmem_st32(tO + c * 32, v);
-          }
-        }
-      }
-      const uint64_t f2 = f2_pack(fac, fac), shift = f2_pack(-m, -m);
-      uint64_t l2 = 0;
-#pragma unroll
-      for (int c = 0; c < CH; ++c) {                         // P overwrites the first half of S, behind what has been read
-        uint32_t pk[16];
-        uint32_t (&x)[32] = sv[TWICE ? 0 : c];
-        if (TWICE) load_s(c, x);
-#pragma unroll
-        for (int e = 0; e < 32; e += 2) {
-          float x0, x1;
-          f2_unpack(f2_fma(f2_pack(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), f2, shift), x0, x1);
-          const float p0 = exp2_fast(x0), p1 = exp2_fast(x1);
-          l2 = f2_add(l2, f2_pack(p0, p1));
-          pk[e >> 1] = pack2<true>(p0, p1);
-        }
-        tmem_st16(tS + part * (COLS / 2) + c * 16, pk);
-      }
-      if constexpr (F > 1) {                                 // the keys of the other copies
-        uint32_t zero[16];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) zero[e] = 0u;
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-          if (c / CH != part) tmem_st16(tS + c * 16, zero);
-      }
-      float la, lb;
-      f2_unpack(l2, la, lb);
-      l += la + lb;
-      tmem_wait_st();
-      tc_fence_before();
-      mbar_arrive(bar(P_FULL + j % STAGES));
-    }
-    // ---- epilogue ----
-    if (alive && n_tiles > 0) alive = mbar_wait_warp(bar(O_DONE), 0, abort_flag);
-    const float vs = p.v_scale_head ? p.v_scale_head[kvh] : 1.f;
-    const int64_t prow = (static_cast<int64_t>(split) * p.total_q + tok) * p.num_qo_heads + head;
-    // columns c0 .. c0 + 7 of a row of the result; tok_, head_, prow_: the row
-    auto store8 = [&](const float (&v)[8], int c0, int64_t tok_, int head_, int64_t prow_) {
-      if (p.partial_o) {
-        float* dst = p.partial_o + prow_ * kHeadDim + c0;
-        *reinterpret_cast<float4*>(dst) = make_float4(v[0], v[1], v[2], v[3]);
-        *reinterpret_cast<float4*>(dst + 4) = make_float4(v[4], v[5], v[6], v[7]);
-      } else {
-        *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.out) + tok_ * p.out_stride_tok + head_ * p.out_stride_head + c0) =
-            make_uint4(pack2<false>(v[0], v[1]), pack2<false>(v[2], v[3]), pack2<false>(v[4], v[5]), pack2<false>(v[6], v[7]));
-      }
-    };
-    auto store_lse = [&](float lse, int64_t tok_, int head_, int64_t prow_) {
-      if (p.partial_o) p.partial_lse[prow_] = lse;
-      else if (p.lse) p.lse[tok_ * p.num_qo_heads + head_] = lse;
-    };
-    const float to_out = p.partial_o ? vs : vs * p.out_scale;
-    // F > 1: every MMA and conversion of the CTA is done, the tiles of K and V hold the F results of a row
-    float* stage = reinterpret_cast<float*>(smem + OFF_K);   // [128 rows of the tile][LD_O], then maximum and sum of each
-    constexpr int LD_O = kHeadDim + 4;
-    float* st_m = stage + BM * LD_O;
-    static_assert(BM * (LD_O + 2) * 4 <= 2 * STAGES * TILE_BYTES, "results fit the tiles");
-    if (alive) {
-      tc_fence_after();
-      const bool none = l == 0.f;
-      const float inv = F > 1 ? 1.f : (none ? 0.f : to_out / l);
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t v[32];
-        if (n_tiles > 0) {
-          tmem_ld32(tO + c * 32, v);
-          tmem_wait_ld();
-        } else {
-#pragma unroll
-          for (int e = 0; e < 32; ++e) v[e] = 0u;
-        }
-        if (!row_ok) continue;
-#pragma unroll
-        for (int e = 0; e < 32; e += 8) {
-          float x[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(v[e + i]) * inv;
-          if constexpr (F > 1) {
-            float* dst = stage + trow * LD_O + c * 32 + e;
-            *reinterpret_cast<float4*>(dst) = make_float4(x[0], x[1], x[2], x[3]);
-            *reinterpret_cast<float4*>(dst + 4) = make_float4(x[4], x[5], x[6], x[7]);
           } else {
-            store8(x, c * 32 + e, tok, head, prow);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) v[e] = 0u;
+          }
+          if (!row_ok) continue;
+#pragma unroll
+          for (int e = 0; e < 32; e += 8) {
+            float x[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(v[e + i]) * inv;
+            if constexpr (F > 1) {
+              float* dst = stage + trow * LD_O + c * 32 + e;
+              *reinterpret_cast<float4*>(dst) = make_float4(x[0], x[1], x[2], x[3]);
+              *reinterpret_cast<float4*>(dst + 4) = make_float4(x[4], x[5], x[6], x[7]);
+            } else {
+              store8(x, c * 32 + e, tok, head, prow);
+            }
+          }
+        }
+        if constexpr (F > 1) { st_m[trow] = m; st_m[BM + trow] = l; }
+        else if (row_ok) store_lse(none ? -INFINITY : (m + log2f(l)) * kLn2, tok, head, prow);
+      }
+      if constexpr (F > 1) {
+        asm volatile("bar.sync 1, 128;" ::: "memory");         // whatever came of the waits, all four warps come here
+        if (*abort_flag == 0) {
+          const int c8 = (trow & 15) * 8;                      // 16 threads a row, 8 columns each
+          for (int rr = trow >> 4; rr < nrows; rr += 8) {
+            float top = kNoMax, sum = 0.f, f[F], acc[8];
+#pragma unroll
+            for (int k = 0; k < F; ++k) top = fmaxf(top, st_m[k * ROWS + rr]);
+#pragma unroll
+            for (int k = 0; k < F; ++k) { f[k] = exp2_fast(st_m[k * ROWS + rr] - top); sum += f[k] * st_m[BM + k * ROWS + rr]; }
+            const bool none = sum == 0.f;
+            const float inv = none ? 0.f : to_out / sum;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) acc[i] = 0.f;
+#pragma unroll
+            for (int k = 0; k < F; ++k)
+#pragma unroll
+              for (int i = 0; i < 8; ++i) acc[i] += f[k] * stage[(k * ROWS + rr) * LD_O + c8 + i];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) acc[i] *= inv;
+            const int row2 = w.row0 + rr;
+            const int64_t tok2 = qo_base + row2 / G;
+            const int head2 = head0 + row2 % G;
+            const int64_t prow2 = (static_cast<int64_t>(split) * p.total_q + tok2) * p.num_qo_heads + head2;
+            store8(acc, c8, tok2, head2, prow2);
+            if (c8 == 0) store_lse(none ? -INFINITY : (top + log2f(sum)) * kLn2, tok2, head2, prow2);
           }
         }
       }
-      if constexpr (F > 1) { st_m[trow] = m; st_m[BM + trow] = l; }
-      else if (row_ok) store_lse(none ? -INFINITY : (m + log2f(l)) * kLn2, tok, head, prow);
     }
-    if constexpr (F > 1) {
-      asm volatile("bar.sync 1, 128;" ::: "memory");         // whatever came of the waits, all four warps come here
-      if (*abort_flag == 0) {
-        const int c8 = (trow & 15) * 8;                      // 16 threads a row, 8 columns each
-        for (int rr = trow >> 4; rr < nrows; rr += 8) {
-          float top = kNoMax, sum = 0.f, f[F], acc[8];
-#pragma unroll
-          for (int k = 0; k < F; ++k) top = fmaxf(top, st_m[k * ROWS + rr]);
-#pragma unroll
-          for (int k = 0; k < F; ++k) { f[k] = exp2_fast(st_m[k * ROWS + rr] - top); sum += f[k] * st_m[BM + k * ROWS + rr]; }
-          const bool none = sum == 0.f;
-          const float inv = none ? 0.f : to_out / sum;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) acc[i] = 0.f;
-#pragma unroll
-          for (int k = 0; k < F; ++k)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) acc[i] += f[k] * stage[(k * ROWS + rr) * LD_O + c8 + i];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) acc[i] *= inv;
-          const int row2 = w.row0 + rr;
-          const int64_t tok2 = qo_base + row2 / G;
-          const int head2 = head0 + row2 % G;
-          const int64_t prow2 = (static_cast<int64_t>(split) * p.total_q + tok2) * p.num_qo_heads + head2;
-          store8(acc, c8, tok2, head2, prow2);
-          if (c8 == 0) store_lse(none ? -INFINITY : (top + log2f(sum)) * kLn2, tok2, head2, prow2);
-        }
-      }
-    }
-  }
   }
 
   // ---------------- teardown ----------------

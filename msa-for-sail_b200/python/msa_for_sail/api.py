@@ -118,15 +118,9 @@ def _compute_pack_factor(max_qo_len, num_qo_heads, num_kv_heads):
     return h_r
 
 
-def _sparse_splits(items, kv_block_num, num_kv_splits, num_sms, two_per_sm, ctas_per_sm=None):
-    """Splits of the selected pages in token-major sparse attention, halved as often as pays.  A CTA takes its
-    pages and about four page times more (dependent index loads, the first page's latency, the epilogue), the CTAs run in
-    rounds of the slots there are (two e4m3 CTAs of at most 16 rows share an SM), and splits cost a merge, about four
-    page times.  Measured for 2 to 384 items of 4 to 32 pages in both types with every power of two up to 8: the count that
-    this gives is within 2 us (a step of the clock) of the best one at all 176 sizes; 24 tokens x 4 heads x 16 bf16 pages:
-    34 us uncut, 45 us in two, 59 us in eight, kernels alone on a cold L2."""
-    # The most splits, which partials in a caller's workspace are sized for: enough CTAs for two rounds, or of an explicit
-    # count what is left once halving it would leave an SM without a CTA.
+def _most_sparse_splits(items, kv_block_num, num_kv_splits, num_sms):
+    """The most splits, which partials in a caller's workspace are sized for: enough CTAs for two rounds, or of an explicit
+    count what is left once halving it would leave an SM without a CTA."""
     if num_kv_splits >= 1:
         s = min(num_kv_splits, kv_block_num)
         while s > 1 and items * (s // 2) >= num_sms:
@@ -135,7 +129,35 @@ def _sparse_splits(items, kv_block_num, num_kv_splits, num_sms, two_per_sm, ctas
         s = 1
         while s * 2 <= min(kv_block_num, 8) and items * s < 2 * num_sms:
             s *= 2
-    slots = num_sms * (ctas_per_sm or (2 if two_per_sm else 1))
+    return s
+
+
+def _kv4_sparse_splits(items, kv_block_num, num_kv_splits, num_sms, rows):
+    """Splits for the 4-bit decode kernel, whose CTAs share an SM's arithmetic.  In page times of an SM (0.53 us, 0.73 us with more than 8
+    rows): a page takes 1.3 in a CTA on its own, a round 9.5 (7) before its first and after its last page, a merge 6.5 (4.7).
+    Measured at seven sizes from 8 to 512 items, 8 to 32 pages, with 1, 2, 4 and 8 splits: the count that this gives is within
+    4 % of the best one; 256 items x 16 pages 23.6 us uncut, 26.6 us in two; 64 items 16.0, 13.3, 11.6, 12.4 us."""
+    slots, start, merge = num_sms * _kv4_ctas(rows), 9.5 if rows <= 8 else 7.0, 6.5 if rows <= 8 else 4.7
+    s = _most_sparse_splits(items, kv_block_num, num_kv_splits, num_sms)
+    best, best_cost = 1, None
+    while s >= 1:
+        pages = -(-kv_block_num // s)
+        cost = max(1.3 * pages, -(-items * s // num_sms) * pages) + start * -(-items * s // slots) + (merge if s > 1 else 0)
+        if best_cost is None or cost <= best_cost:
+            best, best_cost = s, cost
+        s //= 2
+    return best
+
+
+def _sparse_splits(items, kv_block_num, num_kv_splits, num_sms, two_per_sm):
+    """Splits of the selected pages in token-major sparse attention, halved as often as pays.  A CTA takes its
+    pages and about four page times more (dependent index loads, the first page's latency, the epilogue), the CTAs run in
+    rounds of the slots there are (two e4m3 CTAs of at most 16 rows share an SM), and splits cost a merge, about four
+    page times.  Measured for 2 to 384 items of 4 to 32 pages in both types with every power of two up to 8: the count that
+    this gives is within 2 us (a step of the clock) of the best one at all 176 sizes; 24 tokens x 4 heads x 16 bf16 pages:
+    34 us uncut, 45 us in two, 59 us in eight, kernels alone on a cold L2."""
+    s = _most_sparse_splits(items, kv_block_num, num_kv_splits, num_sms)
+    slots = num_sms * (2 if two_per_sm else 1)
     best, best_cost = 1, None
     while s >= 1:
         cost = -(-items * s // slots) * (-(-kv_block_num // s) + 4) + (4 if s > 1 else 0)
@@ -308,7 +330,7 @@ def _fmha_sail_plan(
             return _fmha_sail_plan_device(
                 qo_segment_lens, kv_segment_lens, num_qo_heads, hkv_, qo_offset, num_kv_splits, page_size,
                 output_maxscore, kv_block_num, usable_SM_count, causal, use_fp8_kvcache, dev, given_workspace,
-                max_total_q, max_qo_len_override, bool(qo_len_uniform_override), max_kv_len_override)
+                max_total_q, max_qo_len_override, bool(qo_len_uniform_override), max_kv_len_override, use_kv4_cache)
         # host-resident lengths: planned on the host below, which reads them
 
     qo_lens = _to_int_list(qo_segment_lens)
@@ -380,8 +402,10 @@ def _fmha_sail_plan(
     num_work = 0
     info["work"] = info["num_kv_splits_per_row"] = None
     if is_sparse:
-        splits = _sparse_splits(total_q * hkv, kv_block_num, num_kv_splits, num_sms,
-                                use_fp8_kvcache and h_r <= 16, _kv4_ctas(h_r) if use_kv4_cache and h_r <= 16 else None)
+        if use_kv4_cache:
+            splits = _kv4_sparse_splits(total_q * hkv * -(-h_r // 16), kv_block_num, num_kv_splits, num_sms, h_r)
+        else:
+            splits = _sparse_splits(total_q * hkv, kv_block_num, num_kv_splits, num_sms, use_fp8_kvcache and h_r <= 16)
         up.add("token_batch", np.repeat(np.arange(batch, dtype=np.int32), a_q))
         up.add("page_batch", np.repeat(np.arange(batch, dtype=np.int32), pages_per))
         info["num_logical_pages"] = int(pages_per.sum())
@@ -477,7 +501,7 @@ def _fmha_sail_plan(
 
 def _fmha_sail_plan_device(qo_segment_lens, kv_segment_lens, num_qo_heads, hkv, qo_offset, num_kv_splits,
                            page_size, output_maxscore, kv_block_num, usable_SM_count, causal, use_fp8_kvcache,
-                           dev, given_workspace, max_total_q, max_qo, qo_len_uniform, max_kv_len_override):
+                           dev, given_workspace, max_total_q, max_qo, qo_len_uniform, max_kv_len_override, use_kv4_cache=False):
     """Graph-safe planner (upstream graph_safe mode, api.py:916-941): the lengths stay on the GPU.
 
     Everything that sizes a launch comes from the arguments -- batch, ``max_qo_len_override`` (the
@@ -498,8 +522,10 @@ def _fmha_sail_plan_device(qo_segment_lens, kv_segment_lens, num_qo_heads, hkv, 
         num_sms = _num_sms(dev)
         if usable_SM_count > 0:
             num_sms = min(num_sms, usable_SM_count)
-        splits = _sparse_splits(max_total_q * hkv, kv_block_num, max(1, num_kv_splits), num_sms,
-                                use_fp8_kvcache and h_r <= 16)
+        if use_kv4_cache:
+            splits = _kv4_sparse_splits(max_total_q * hkv * -(-h_r // 16), kv_block_num, max(1, num_kv_splits), num_sms, h_r)
+        else:
+            splits = _sparse_splits(max_total_q * hkv, kv_block_num, max(1, num_kv_splits), num_sms, use_fp8_kvcache and h_r <= 16)
     else:
         pack = _compute_pack_factor(max_qo, num_qo_heads, hkv)
         block_m = _block_m(max_qo * pack)
@@ -653,6 +679,14 @@ def _validate_fmha_inputs(q, k, v, plan, is_paged, kv_is_nhd, num_kv_heads, page
 # ----------------------------------------------------------------------------
 # run
 # ----------------------------------------------------------------------------
+
+def _head_scale(x, device, hkv):
+    """Like ``_scale_arg``, without a read of the device: a tensor of one value is spread over the heads there."""
+    if not isinstance(x, torch.Tensor):
+        return 1.0 if x is None else float(x), None
+    assert x.numel() in (1, hkv), f"per-head scale must have {hkv} entries, got {x.numel()}"
+    return 1.0, x.reshape(-1).expand(hkv).to(device=device, dtype=torch.float32).contiguous()
+
 
 def _scale_arg(x, device, hkv):
     """A scale is a float, or an fp32 tensor with one value per KV head."""
@@ -1022,8 +1056,8 @@ def _fmha_sail_kv4(q, k, v, plan, kv_indices, kv_block_indexes, q_offset_overrid
     if sm_scale is None:
         sm_scale = 1.0 / math.sqrt(128)
     q_s, _ = _scale_arg(q_scale, dev, num_kv_heads)
-    k_s, k_head = _scale_arg(k_scale, dev, num_kv_heads)
-    v_s, v_head = _scale_arg(v_scale, dev, num_kv_heads)
+    k_s, k_head = _head_scale(k_scale, dev, num_kv_heads)
+    v_s, v_head = _head_scale(v_scale, dev, num_kv_heads)
     o_s, _ = _scale_arg(o_scale, dev, num_kv_heads)
     if out is None:
         out = torch.empty(nnz_qo, num_qo_heads, 128, device=dev, dtype=torch.bfloat16)

@@ -227,6 +227,43 @@ def test_scores_of_pages(qo, kv, output_o):
         ref.check_attention(out, None, b.want(), P_BF16, "with scores")
 
 
+def test_scales_of_one_head_in_a_graph():
+    """Scales stay on the device, also where there is one KV head or one value for all heads: nothing is read back."""
+    import msa_for_sail as msa
+    for hk in (1, 2):
+        b = Batch(61, [1, 1], [300, 200], 8 * hk, hk)
+        q, k, v, table = b.cuda()
+        plan, ks, vs = b.plan(num_kv_splits=2), torch.tensor([0.5], device=DEV), torch.tensor([3.0], device=DEV)
+        msa.fmha_sail(q, k, v, plan, kv_indices=table, k_scale=ks, v_scale=vs)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out, _ = msa.fmha_sail(q, k, v, plan, kv_indices=table, k_scale=ks, v_scale=vs)
+        vs.fill_(0.25)
+        graph.replay()
+        torch.cuda.synchronize()
+        ref.check_attention(out, None, b.want(k_scale=ks.expand(hk), v_scale=vs.expand(hk)), P_F16, f"{hk} heads")
+
+
+@pytest.mark.parametrize("rows", [1, 4])
+def test_a_reported_timeout_stops_the_tensor_core_kernel(rows):
+    """While the status word is set, the kernel with waits does not start; once it is cleared it gives the right result."""
+    import msa_for_sail as msa
+    from msa_for_sail import api
+    b = Batch(62, [rows, rows], [300, 200], 16, 2)
+    q, k, v, table = b.cuda()
+    plan = b.plan(num_kv_splits=1)
+    out = torch.full((b.T, 16, 128), 7.0, dtype=torch.bfloat16, device=DEV)
+    api._status_word(q.device).fill_(1)
+    msa.fmha_sail(q, k, v, plan, kv_indices=table, out=out)
+    torch.cuda.synchronize()
+    if rows * 8 > 16:
+        assert (out == 7.0).all()
+    assert api.last_status() == 1 and api.last_status() == 0
+    msa.fmha_sail(q, k, v, plan, kv_indices=table, out=out)
+    ref.check_attention(out, None, b.want(), P_F16, "after the status was cleared")
+
+
 @pytest.mark.parametrize("sparse", [False, True])
 def test_planned_and_run_in_a_graph(sparse):
     """graph_safe plan and call in one graph; lengths, table and selection change between replays; padded rows are left alone by nobody."""
