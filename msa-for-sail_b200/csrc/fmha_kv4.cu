@@ -96,10 +96,10 @@ struct Item {
   int head0, pack, tok0;           // row r: token tok0 + r / pack of the sequence, head head0 + r % pack
   int qo_base, kv_len, off, page_base;
   int first, last;                 // entries of the page list: logical pages, or places of the selection
-  const int32_t* blocks;           // selection, or nullptr
+  const int32_t* blocks;           // selection
 };
 
-template <int NT>
+template <int NT, bool SPARSE>
 __global__ void __launch_bounds__(kThreads, Cfg<NT>::CTAS) kv4_decode_kernel(const __grid_constant__ MsaFmhaParams p) {
   using C = Cfg<NT>;
   extern __shared__ __align__(16) unsigned char smem[];
@@ -108,12 +108,11 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::CTAS) kv4_decode_kernel(con
 
 
   // ---------------- the item ----------------
-  const bool sparse = (p.flags & MSA_FLAG_SPARSE) != 0;
   const int h_r = p.num_qo_heads / p.num_kv_heads;
   const int rg = blockIdx.y * (8 * NT);                      // first row of this CTA's group
   Item it;
   int first_blocks = -1;                                     // this lane's entry of a selection: on its way before the loads that depend on the batch item
-  if (!sparse) {
+  if constexpr (!SPARSE) {
     const MsaWorkItem w = p.work[blockIdx.x];
     it.b = chk(w.batch, 0, p.batch, p.status);
     it.head0 = chk(w.head0, 0, p.num_qo_heads, p.status);
@@ -121,7 +120,6 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::CTAS) kv4_decode_kernel(con
     it.pack = p.pack; it.tok0 = 0;
     it.row0 = w.row0 + rg; it.nrows = min(8 * NT, w.num_rows - rg);
     it.first = w.kv_tile_begin; it.last = w.kv_tile_end;
-    it.blocks = nullptr;
     it.kvh = it.head0 / h_r;
   } else {
     int idx = blockIdx.x;
@@ -148,7 +146,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::CTAS) kv4_decode_kernel(con
   const int lim_first = lim(0), lim_last = lim(it.nrows - 1);
 
   // ---------------- this warp's list of pages, and the copies ----------------
-  const int n_tiles = max(0, it.blocks ? it.last - it.first : min(it.last, (lim_last + kKvTile - 1) / kKvTile) - it.first);
+  const int n_tiles = max(0, SPARSE ? it.last - it.first : min(it.last, (lim_last + kKvTile - 1) / kKvTile) - it.first);
   // entries of the list, one a lane: physical pages, and logical pages of a selection or the next physical pages
   auto physical = [&](int lp) -> int {
     return min(max(chk(p.kv_indices[it.page_base + lp], 0, static_cast<int>(p.kv_extent), p.status), 0), static_cast<int>(p.kv_extent) - 1);
@@ -157,7 +155,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::CTAS) kv4_decode_kernel(con
   const unsigned char* const v_head = static_cast<const unsigned char*>(p.v) + it.kvh * p.v_stride_head + warp * kCodeBytes + 16 * lane;
   int phys = -1, aux = -1;
   auto load_entries = [&](int j0) {
-    if (it.blocks) {
+    if constexpr (SPARSE) {
       aux = j0 == 0 ? first_blocks : (j0 + lane < n_tiles ? it.blocks[it.first + j0 + lane] : -1);
       phys = aux >= 0 && aux < (lim_last + kKvTile - 1) / kKvTile ? physical(aux) : -1;
     } else {
@@ -169,7 +167,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::CTAS) kv4_decode_kernel(con
   auto fetch = [&](int j, int stage) {
     if ((j & 31) == 0) load_entries(j);
     const int page = __shfl_sync(0xffffffffu, phys, j & 31);
-    const int lp = it.blocks ? __shfl_sync(0xffffffffu, aux, j & 31) : it.first + j;
+    const int lp = SPARSE ? __shfl_sync(0xffffffffu, aux, j & 31) : it.first + j;
     if (page >= 0) {
       const uint32_t dst = smem_u32(ring) + stage * 2 * C::HALF + 16 * lane;
       const unsigned char* k = k_head + page * p.k_stride_page;
@@ -486,23 +484,23 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::CTAS) kv4_decode_kernel(con
   }
 }
 
-template <int NT>
+template <int NT, bool SPARSE>
 int launch(const MsaFmhaParams& p, int rows, cudaStream_t stream) {
   int device = 0;
   if (cudaGetDevice(&device) != cudaSuccess) return MSA_ERR_LAUNCH;
   static bool ready[64] = {};
   if (device < 0 || device >= 64 || !ready[device]) {
-    if (cudaFuncSetAttribute(kv4_decode_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<NT>::BYTES) != cudaSuccess) return MSA_ERR_LAUNCH;
+    if (cudaFuncSetAttribute(kv4_decode_kernel<NT, SPARSE>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<NT>::BYTES) != cudaSuccess) return MSA_ERR_LAUNCH;
     if (device >= 0 && device < 64) ready[device] = true;
   }
-  const int64_t items = (p.flags & MSA_FLAG_SPARSE) ? static_cast<int64_t>(p.total_q) * p.num_kv_heads * p.num_splits : p.num_work;
+  const int64_t items = SPARSE ? static_cast<int64_t>(p.total_q) * p.num_kv_heads * p.num_splits : p.num_work;
   if (items > 0x7fffffffLL) return MSA_ERR_TOO_LARGE;
   if (items == 0) return MSA_OK;
   const dim3 grid(static_cast<unsigned>(items), (rows + 8 * NT - 1) / (8 * NT));
   // A plain launch, and the next kernel comes up at the end of this one: CTAs that came up while the kernel before ends would fill
   // the SMs that are free first, three or four of the longest items on one (24 ragged sequences x 4 heads: 116 us instead of
   // 89), and a merge that came up early would take the place of CTAs here (82 us instead of 62, finer cut).
-  kv4_decode_kernel<NT><<<grid, kThreads, Cfg<NT>::BYTES, stream>>>(p);
+  kv4_decode_kernel<NT, SPARSE><<<grid, kThreads, Cfg<NT>::BYTES, stream>>>(p);
   return cudaGetLastError() == cudaSuccess ? MSA_OK : MSA_ERR_LAUNCH;
 }
 
@@ -542,6 +540,7 @@ int fmha_kv4_fwd(const MsaFmhaParams& p, cudaStream_t stream) {
     return MSA_ERR_BAD_ARG;
   if (p.total_q == 0 || p.kv_extent == 0) return p.total_q == 0 ? MSA_OK : MSA_ERR_BAD_ARG;
   if (!sparse && rows > 16) return fmha_kv4_tc_launch(p, rows, stream);
-  return rows <= 8 ? kv4::launch<1>(p, rows, stream) : kv4::launch<2>(p, rows, stream);
+  if (sparse) return rows <= 8 ? kv4::launch<1, true>(p, rows, stream) : kv4::launch<2, true>(p, rows, stream);
+  return rows <= 8 ? kv4::launch<1, false>(p, rows, stream) : kv4::launch<2, false>(p, rows, stream);
 }
 }  // namespace msa
