@@ -257,7 +257,9 @@ int msa_fmha_fwd_split_static(const MsaFmhaParams* params, const int32_t* splits
 
 /* msa_fmha_fwd with kv_dtype = MSA_DT_KV4: q bf16 or e4m3, paged k and v with page_size 128, MSA_FLAG_OUT_O only (with or
  * without MSA_FLAG_SPARSE), block_m 16 / 64 / 128; up to 128 packed rows per work item.  Longer queries and scores: unpack
- * the pages with msa_kv4_read and run on the copy.  A page table entry outside [0, kv_extent) is clamped. */
+ * the pages with msa_kv4_read and run on the copy.  num_logical_pages is the length of kv_indices; entries past it and pages
+ * outside [0, kv_extent) are clamped.  17 to 128 rows of dense items run on the tensor-core kernel, whose waits report to
+ * `status`. */
 
 /* Per-head RMS norm of q and k, rotary positions, and the write of k and v into a paged cache, in one pass over a step's
  * tokens.  Any of q, k, v may be NULL (k needs k_out or k_cache; v needs v_cache).  q, k, v and the outputs are bf16 unless a

@@ -106,7 +106,6 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::CTAS) kv4_decode_kernel(con
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   unsigned char* ring = smem + warp * C::STAGES * 2 * C::HALF;
 
-
   // ---------------- the item ----------------
   const int h_r = p.num_qo_heads / p.num_kv_heads;
   const int rg = blockIdx.y * (8 * NT);                      // first row of this CTA's group
@@ -146,10 +145,12 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::CTAS) kv4_decode_kernel(con
   const int lim_first = lim(0), lim_last = lim(it.nrows - 1);
 
   // ---------------- this warp's list of pages, and the copies ----------------
-  const int n_tiles = max(0, SPARSE ? it.last - it.first : min(it.last, (lim_last + kKvTile - 1) / kKvTile) - it.first);
+  // (none where the table is empty: `physical` then has nothing to read)
+  const int n_tiles = p.num_logical_pages <= 0 ? 0 : max(0, SPARSE ? it.last - it.first : min(it.last, (lim_last + kKvTile - 1) / kKvTile) - it.first);
   // entries of the list, one a lane: physical pages, and logical pages of a selection or the next physical pages
-  auto physical = [&](int lp) -> int {
-    return min(max(chk(p.kv_indices[it.page_base + lp], 0, static_cast<int>(p.kv_extent), p.status), 0), static_cast<int>(p.kv_extent) - 1);
+  auto physical = [&](int lp) -> int {                       // in bounds whatever the table holds, and however short it is
+    const int at = chk(it.page_base + lp, 0, p.num_logical_pages, p.status);
+    return min(max(chk(p.kv_indices[min(at, p.num_logical_pages - 1)], 0, static_cast<int>(p.kv_extent), p.status), 0), static_cast<int>(p.kv_extent) - 1);
   };
   const unsigned char* const k_head = static_cast<const unsigned char*>(p.k) + it.kvh * p.k_stride_head + warp * kCodeBytes + 16 * lane;
   const unsigned char* const v_head = static_cast<const unsigned char*>(p.v) + it.kvh * p.v_stride_head + warp * kCodeBytes + 16 * lane;
@@ -538,7 +539,8 @@ int fmha_kv4_fwd(const MsaFmhaParams& p, cudaStream_t stream) {
   if ((p.q_stride_tok * qe) % 16 || (p.q_stride_head * qe) % 16 || p.k_stride_page % 16 || p.k_stride_head % 16 || p.v_stride_page % 16 ||
       p.v_stride_head % 16 || (p.out && ((p.out_stride_tok * 2) % 16 || (p.out_stride_head * 2) % 16)))
     return MSA_ERR_BAD_ARG;
-  if (p.total_q == 0 || p.kv_extent == 0) return p.total_q == 0 ? MSA_OK : MSA_ERR_BAD_ARG;
+  if (p.total_q == 0) return MSA_OK;
+  if (p.kv_extent == 0 || p.num_logical_pages < 0) return MSA_ERR_BAD_ARG;
   if (!sparse && rows > 16) return fmha_kv4_tc_launch(p, rows, stream);
   if (sparse) return rows <= 8 ? kv4::launch<1, true>(p, rows, stream) : kv4::launch<2, true>(p, rows, stream);
   return rows <= 8 ? kv4::launch<1, false>(p, rows, stream) : kv4::launch<2, false>(p, rows, stream);

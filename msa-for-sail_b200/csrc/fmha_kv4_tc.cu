@@ -98,7 +98,8 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv4_tc_kernel(const __grid_consta
   auto lim = [&](int r) -> int { return min(kv_len, (w.row0 + r) / G + off + 1); };
   const int lim_first = lim(0), lim_last = lim(nrows - 1);
   const int first = w.kv_tile_begin;
-  const int n_tiles = max(0, min(w.kv_tile_end, (lim_last + BN - 1) / BN) - first);
+  // (none where the table is empty: the conversion then has nothing to read)
+  const int n_tiles = p.num_logical_pages <= 0 ? 0 : max(0, min(w.kv_tile_end, (lim_last + BN - 1) / BN) - first);
   const int n_active = F == 1 ? (nrows + 31) / 32 : 4;       // warps that have rows
 
   // a timeout reported earlier on this device (status word not cleared yet): do not start
@@ -136,7 +137,9 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv4_tc_kernel(const __grid_consta
                                              : static_cast<const unsigned char*>(p.k) + kvh * p.k_stride_head) + 16 * lane;
     const int64_t stride = is_v ? p.v_stride_page : p.k_stride_page;
     auto physical = [&](int j) -> int {
-      return j < n_tiles ? min(max(chk(p.kv_indices[page_base + first + j], 0, static_cast<int>(p.kv_extent), p.status), 0), static_cast<int>(p.kv_extent) - 1) : 0;
+      if (j >= n_tiles) return 0;
+      const int at = min(chk(page_base + first + j, 0, p.num_logical_pages, p.status), p.num_logical_pages - 1);
+      return min(max(chk(p.kv_indices[at], 0, static_cast<int>(p.kv_extent), p.status), 0), static_cast<int>(p.kv_extent) - 1);
     };
     int phys = physical(lane), next = physical(32 + lane);   // page-table entries, one a lane
     const uint32_t code_dst = smem_u32(ring) + code_at(lane >> 2, lane & 3), scale_dst = smem_u32(ring) + CODE_BYTES + 16 * lane;

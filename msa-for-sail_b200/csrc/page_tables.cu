@@ -75,7 +75,8 @@ __device__ void fill(const MsaPageTablesArgs& a, int num_free, int64_t first, in
       const int b = request_of(s.qo_start, a.batch, static_cast<int>(t));
       pos = a.kv_len[b] - (s.qo_start[b + 1] - static_cast<int>(t));
       const int page = pos >= 0 ? page_of(a, s, b, pos / a.page_size, num_free) : -1;
-      if (page >= 0) slot = page * a.page_size + pos % a.page_size;
+      const int64_t at = static_cast<int64_t>(page) * a.page_size + pos % a.page_size;
+      if (page >= 0 && at <= 0x7fffffff) slot = static_cast<int>(at);
       pos = max(pos, 0);
     }
     a.slot_map[t] = slot;

@@ -41,7 +41,15 @@ def _status_word(device):
     return _STATUS[idx]
 
 
-cache._status_word = _status_word
+def _status_ptr(device):
+    """Pointer of the status word, NULL (nothing is reported) where it would first be made inside a capture: it would live in the
+    graph's memory."""
+    if device.index not in _STATUS and torch.cuda.is_current_stream_capturing():
+        return None
+    return _status_word(device).data_ptr()
+
+
+cache._status_ptr = _status_ptr
 
 
 def last_status(device=None, reset=True):
@@ -684,6 +692,8 @@ def _head_scale(x, device, hkv):
     """Like ``_scale_arg``, without a read of the device: a tensor of one value is spread over the heads there."""
     if not isinstance(x, torch.Tensor):
         return 1.0 if x is None else float(x), None
+    if x.dtype == torch.float32 and x.numel() == hkv and x.get_device() == device.index and x.is_contiguous():
+        return 1.0, x
     assert x.numel() in (1, hkv), f"per-head scale must have {hkv} entries, got {x.numel()}"
     return 1.0, x.reshape(-1).expand(hkv).to(device=device, dtype=torch.float32).contiguous()
 
@@ -1009,8 +1019,10 @@ def _fmha_sail_kv4(q, k, v, plan, kv_indices, kv_block_indexes, q_offset_overrid
     if kv_indices.dtype != torch.int32 or kv_indices.dim() != 1 or not kv_indices.is_contiguous():
         raise ValueError("kv_indices must be a contiguous int32 vector")
     dev = q.device
-    cache._same_device(dev, k=k, v=v if output_o else None, kv_indices=kv_indices, kv_block_indexes=kv_block_indexes, out=out, lse=lse,
-                       max_score=max_score, plan=plan["qo_offset"])
+    index = dev.index
+    if any(t is not None and t.get_device() != index for t in (k, v, kv_indices, kv_block_indexes, out, lse, max_score, plan["qo_offset"])):
+        cache._same_device(dev, k=k, v=v, kv_indices=kv_indices, kv_block_indexes=kv_block_indexes, out=out, lse=lse, max_score=max_score,
+                           plan=plan["qo_offset"])
     if k.shape[0] == 0 and nnz_qo:
         raise ValueError("the cache has no pages")
     if num_qo_heads % num_kv_heads:
@@ -1037,20 +1049,28 @@ def _fmha_sail_kv4(q, k, v, plan, kv_indices, kv_block_indexes, q_offset_overrid
             table = torch.arange(kv_indices.shape[0], dtype=torch.int32, device=dev)
             kb = cache.unpack_pages(k, kv_indices)
             vb = cache.unpack_pages(v, kv_indices) if output_o else kb
+            # workspaces of its own: two streams, or two captured graphs, may run one plan at the same time
+            plan = PlanInfo(plan, sparse_ws=None)
+            for name in ("workspace_o", "workspace_lse"):
+                if plan[name] is not None:
+                    plan[name] = torch.empty_like(plan[name])
             return _fmha_sail(q if q.dtype == torch.bfloat16 else q.to(torch.bfloat16), kb, vb, plan, table, kv_block_indexes, q_offset_override, out,
                               max_score, sm_scale, q_scale, k_scale, v_scale, o_scale, output_maxscore, output_o, check_input_valid,
                               max_score_dtype, lse)
     if plan["orig_num_qo_heads"] != num_qo_heads or plan["num_kv_heads"] != num_kv_heads:
         raise ValueError("plan head counts do not match q / k")
-    qo_offset = plan["qo_offset"] if q_offset_override is None else q_offset_override
-    if isinstance(qo_offset, int):
-        if plan.get("graph_safe", False):
-            raise ValueError("graph_safe=True requires q_offset_override as a CUDA tensor; an int triggers an in-capture torch.full_like allocation")
-        qo_offset = torch.full_like(plan["qo_segment_lens"], qo_offset)
-    else:
-        cache._same_device(dev, qo_offset=qo_offset)
-        if qo_offset.dtype != torch.int32:
-            qo_offset = qo_offset.to(torch.int32)
+    qo_offset = plan["qo_offset"]
+    if q_offset_override is not None:
+        qo_offset = q_offset_override
+        if isinstance(qo_offset, int):
+            if plan.get("graph_safe", False):
+                raise ValueError("graph_safe=True requires q_offset_override as a CUDA tensor; an int triggers an in-capture torch.full_like allocation")
+            qo_offset = torch.full_like(plan["qo_segment_lens"], qo_offset)
+        else:
+            cache._same_device(dev, q_offset_override=qo_offset)
+            if tuple(qo_offset.shape) != (plan["batch_size"],):
+                raise ValueError(f"q_offset_override must be [batch_size={plan['batch_size']}], got {tuple(qo_offset.shape)}")
+            qo_offset = qo_offset.to(torch.int32).contiguous()
     if check_input_valid and plan["_host"] is not None:
         _validate_fmha_inputs(q, k, v, plan, True, False, num_kv_heads, cache.KV4_TILE, kv_indices, kv_block_indexes, qo_offset)
     if sm_scale is None:
@@ -1071,20 +1091,32 @@ def _fmha_sail_kv4(q, k, v, plan, kv_indices, kv_block_indexes, q_offset_overrid
     assert q.stride(2) == 1, "q head_dim must be contiguous"
     splits = plan["num_kv_splits"]
     q_stride, out_scale = q.stride(), float(v_s * o_s)
-    p = _lib.MsaFmhaParams(
-        q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), qo_start=plan["qo_segment_offsets"].data_ptr(), kv_len=plan["kv_segment_lens"].data_ptr(),
-        qo_offset=qo_offset.data_ptr(), kv_page_indptr=plan["kv_page_indptr"].data_ptr(), kv_indices=kv_indices.data_ptr(),
-        k_scale_head=_ptr(k_head), v_scale_head=_ptr(v_head), status=_status_word(dev).data_ptr(), q_stride_tok=q_stride[0], q_stride_head=q_stride[1],
-        k_stride_page=k_stride[0], k_stride_head=k_stride[1], v_stride_page=v_stride[0], v_stride_head=v_stride[1], kv_extent=k.shape[0],
-        total_q=nnz_qo, num_qo_heads=num_qo_heads, num_kv_heads=num_kv_heads, batch=plan["batch_size"], block_m=plan["qo_tile_size"],
-        pack=plan["pack_factor"], page_size=cache.KV4_TILE, num_splits=splits, q_dtype=_dt_code(q.dtype), kv_dtype=MSA_DT_KV4,
-        flags=FLAG_OUT_O | FLAG_SPARSE if sparse else FLAG_OUT_O, sm_scale=float(q_s * k_s * sm_scale), out_scale=out_scale)
+    base = plan.get("_kv4_params")            # the sizes that are the same in every call with this plan
+    if base is None:
+        plan["_kv4_pages"] = sum(-(-n // cache.KV4_TILE) for n in plan["_host"]["kv_lens"]) if plan["_host"] is not None else 0
+        base = plan["_kv4_params"] = bytes(_lib.MsaFmhaParams(
+            num_work=plan["num_work"], decode_rows=0 if sparse else rows, num_qo_heads=num_qo_heads, num_kv_heads=num_kv_heads,
+            batch=plan["batch_size"], block_m=plan["qo_tile_size"], pack=plan["pack_factor"], page_size=cache.KV4_TILE, num_splits=splits,
+            kv_dtype=MSA_DT_KV4, flags=FLAG_OUT_O | FLAG_SPARSE if sparse else FLAG_OUT_O))
+    if kv_indices.shape[0] < plan["_kv4_pages"]:
+        raise ValueError(f"kv_indices must have the {plan['_kv4_pages']} pages of the plan's sequences, got {kv_indices.shape[0]}")
+    p = _lib.MsaFmhaParams.from_buffer_copy(base)
+    p.qo_start, p.kv_len, p.qo_offset = plan["qo_segment_offsets"].data_ptr(), plan["kv_segment_lens"].data_ptr(), qo_offset.data_ptr()
+    p.kv_page_indptr, p.num_logical_pages, p.status = plan["kv_page_indptr"].data_ptr(), kv_indices.shape[0], _status_ptr(dev)
+    p.q, p.k, p.v, p.kv_indices = q.data_ptr(), k.data_ptr(), v.data_ptr(), kv_indices.data_ptr() or p.kv_page_indptr     # (an empty table is not read)
+    p.q_stride_tok, p.q_stride_head, p.total_q, p.q_dtype = q_stride[0], q_stride[1], nnz_qo, _dt_code(q.dtype)
+    p.k_stride_page, p.k_stride_head, p.v_stride_page, p.v_stride_head = k_stride[0], k_stride[1], v_stride[0], v_stride[1]
+    p.kv_extent, p.sm_scale, p.out_scale = k.shape[0], float(q_s * k_s * sm_scale), out_scale
+    if k_head is not None:
+        p.k_scale_head = k_head.data_ptr()
+    if v_head is not None:
+        p.v_scale_head = v_head.data_ptr()
     if sparse:
+        p.token_batch = plan["token_batch"].data_ptr()
         p.kv_block_indexes, p.kv_block_num = kv_block_indexes.data_ptr(), kv_block_indexes.shape[2]
         p.kbi_stride_tok, p.kbi_stride_head = kv_block_indexes.stride(0), kv_block_indexes.stride(1)
-        p.token_batch = plan["token_batch"].data_ptr()
     else:
-        p.work, p.num_work, p.decode_rows = _ptr(plan["work"]), plan["num_work"], rows
+        p.work = _ptr(plan["work"])
     if _SHOW_PARAMS:
         _show_params(q, plan, True, cache.KV4_TILE, float(sm_scale), True, None, kv_block_indexes)
     with cache._on(dev):

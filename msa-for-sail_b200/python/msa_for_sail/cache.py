@@ -25,7 +25,7 @@ KV4_TILE = 128                          # tokens of a page
 KV4_ROW_BYTES = 72                      # 64 bytes of codes and 8 scales
 
 
-_status_word = None                     # of api.py, set when that is imported
+_status_ptr = None                      # of api.py, set when that is imported
 
 
 def _stream():
@@ -84,10 +84,6 @@ def _check_kv4(name, t, num_kv_heads=None):
     return stride
 
 
-def _status(device):
-    return _status_word(device).data_ptr()
-
-
 def _read(cache, index, out, whole_pages):
     if index.shape[0] == 0:
         return out
@@ -95,7 +91,7 @@ def _read(cache, index, out, whole_pages):
         return out.zero_()
     dev = cache.device
     _launch(dev, _lib.lib.msa_kv4_read, _lib.MsaKv4ReadArgs(
-        cache.data_ptr(), out.data_ptr(), index.data_ptr(), _status(dev), cache.stride(0), cache.stride(1), index.shape[0], cache.shape[1],
+        cache.data_ptr(), out.data_ptr(), index.data_ptr(), _status_ptr(dev), cache.stride(0), cache.stride(1), index.shape[0], cache.shape[1],
         cache.shape[0], whole_pages), "msa_kv4_read")
     return out
 
@@ -367,7 +363,7 @@ def qk_norm_rope(
         return q_out, k_out
     _launch(dev, _lib.lib.msa_norm_rope, _lib.MsaNormRopeArgs(
         q.data_ptr(), k.data_ptr(), v_ptr, qw, kw, pos[0], pos[1], pos[2], q_out.data_ptr(), None if k_out is None else k_out.data_ptr(),
-        kc[0], vc[0], slots, ks[1], vs[1], _status(dev), pos[3], *q_strides, *k_strides, *v_strides, *qo_strides, *ko_strides, qw_stride, kw_stride,
+        kc[0], vc[0], slots, ks[1], vs[1], _status_ptr(dev), pos[3], *q_strides, *k_strides, *v_strides, *qo_strides, *ko_strides, qw_stride, kw_stride,
         kc[1], kc[2], kc[3], vc[1], vc[2], vc[3], T, hq, hk, pos[4], pos[5], 1 if norm else 0,
         MSA_DT_BF16 if w is not None and w.dtype == torch.bfloat16 else MSA_DT_F32, MSA_DT_E4M3 if q8 else MSA_DT_BF16, dtype, pos[6],
         page_size if slots is not None else 0, num_pages, eps, 1.0 if q_scale is None else q_scale, ks[0], vs[0]), "msa_norm_rope")
@@ -388,7 +384,7 @@ def kv_cache_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_c
     if T == 0:
         return
     a = _lib.MsaNormRopeArgs()
-    a.k, a.v, a.slot_map, a.status = k.data_ptr(), v.data_ptr(), slot_map.data_ptr(), _status(dev)
+    a.k, a.v, a.slot_map, a.status = k.data_ptr(), v.data_ptr(), slot_map.data_ptr(), _status_ptr(dev)
     a.k_stride_tok, a.k_stride_head = k_strides
     a.v_stride_tok, a.v_stride_head = v_strides
     a.k_cache, a.k_cache_stride_page, a.k_cache_stride_head, a.k_cache_stride_tok = kc

@@ -427,6 +427,97 @@ def test_step_of_a_serving_engine():
     assert num_free.tolist() == [24 - sum(-(-n // 128) for n in kl)]
 
 
+@pytest.mark.parametrize("rows", [1, 4])
+@pytest.mark.parametrize("sparse", [False, True])
+def test_a_table_shorter_than_the_lengths(rows, sparse):
+    """Lengths on the device may outgrow a table: the places behind its end are its last page, nothing behind it is read.  An empty one has
+    no keys."""
+    import msa_for_sail as msa
+    b = Batch(63, [rows], [600], 16, 2)
+    q, k, v, table = b.cuda()
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)
+    sel = i32([0, 2, 4]).expand(rows, 2, 3).contiguous()
+    ws = msa.allocate_graph_workspace(1, 16, num_kv_heads=2, page_size=128, num_kv_splits=2, kv_block_num=3 if sparse else -1, max_qo_len=rows)
+    plan = msa.fmha_sail_plan(i32([rows]), i32([600]), 16, num_kv_heads=2, page_size=128, kv_block_num=3 if sparse else -1, num_kv_splits=2,
+                              graph_safe=True, max_total_q=rows, max_qo_len_override=rows, qo_len_uniform_override=True, max_kv_len_override=700,
+                              qo_offset=i32([600 - rows]), given_workspace=ws, use_kv4_cache=True)
+    blocks = dict(kv_block_indexes=sel) if sparse else {}
+    short = table[:2].clone()
+    got = msa.fmha_sail(q, k, v, plan, kv_indices=short, **blocks)[0].clone()
+    b.table[2:] = b.table[1]
+    lse = torch.empty(rows, 16, device=DEV)
+    again, _ = msa.fmha_sail(q, k, v, plan, kv_indices=b.table.to(DEV), lse=lse, **blocks)
+    assert torch.equal(got, again)
+    ref.check_attention(got, lse, b.want(**(dict(blocks=sel.cpu()) if sparse else {})), P_F16, "short table")
+    none, _ = msa.fmha_sail(q, k, v, plan, kv_indices=table[:0].clone(), lse=lse, **blocks)
+    assert (none == 0).all() and torch.isinf(lse).all()
+
+
+def test_a_plan_keeps_no_pointer():
+    """The tensors of a plan may be replaced between calls."""
+    import msa_for_sail as msa
+    b = Batch(64, [1, 1], [300, 200], 16, 2)
+    q, k, v, table = b.cuda()
+    plan = b.plan(num_kv_splits=1)
+    msa.fmha_sail(q, k, v, plan, kv_indices=table)
+    b.kv = [300, 140]
+    b.offsets = [299, 139]
+    for name, value in (("kv_segment_lens", b.kv), ("qo_offset", b.offsets)):
+        plan[3][name] = torch.tensor(value, dtype=torch.int32, device=DEV)
+    out, _ = msa.fmha_sail(q, k, v, plan, kv_indices=table)
+    ref.check_attention(out, None, b.want(), P_F16, "replaced")
+
+
+def test_two_streams_share_a_plan_of_a_prompt():
+    """The copies and workspaces of the path over unpacked pages belong to the call."""
+    import msa_for_sail as msa
+    b = Batch(65, [300], [900], 8, 2)
+    q, k, v, table = b.cuda()
+    q2, blocks = q.flip(0).contiguous(), b.blocks(4).to(DEV)
+    plan = b.plan(kv_block_num=4)
+    want = [msa.fmha_sail(x, k, v, plan, kv_indices=table, kv_block_indexes=blocks)[0].clone() for x in (q, q2)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(20):
+        got = []
+        for s, x in zip(streams, (q, q2)):
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                got.append(msa.fmha_sail(x, k, v, plan, kv_indices=table, kv_block_indexes=blocks)[0])
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, w) for a, w in zip(got, want))
+
+
+def test_first_call_of_a_process_inside_a_capture(monkeypatch):
+    """The word that kernels report to is not made inside a capture, where it would belong to the graph's memory."""
+    import msa_for_sail as msa
+    from msa_for_sail import api
+    b = Batch(66, [1, 1], [300, 200], 16, 2)
+    q, k, v, table = b.cuda()
+    plan = b.plan(num_kv_splits=1)
+    msa.fmha_sail(q, k, v, plan, kv_indices=table)
+    torch.cuda.synchronize()
+    monkeypatch.setattr(api, "_STATUS", {})
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, _ = msa.fmha_sail(q, k, v, plan, kv_indices=table)
+    assert not api._STATUS
+    graph.replay()
+    torch.cuda.synchronize()
+    ref.check_attention(out, None, b.want(), P_F16, "captured")
+
+
+def test_refusals_of_tables_and_offsets():
+    import msa_for_sail as msa
+    b = Batch(67, [1, 1], [300, 200], 16, 2)
+    q, k, v, table = b.cuda()
+    plan = b.plan()
+    with pytest.raises(ValueError, match="kv_indices must have the 5 pages"):
+        msa.fmha_sail(q, k, v, plan, kv_indices=table[:4].clone())
+    with pytest.raises(ValueError, match="q_offset_override must be"):
+        msa.fmha_sail(q, k, v, plan, kv_indices=table, q_offset_override=torch.zeros(1, dtype=torch.int32, device=DEV))
+
+
 def test_refusals():
     import msa_for_sail as msa
     b = Batch(51, [1, 1], [300, 200], 16, 2)

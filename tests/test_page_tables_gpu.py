@@ -131,6 +131,15 @@ def test_steps_in_place_inside_a_graph():
         assert r["slot_map"].tolist() == slots and r["positions"].tolist() == pos
 
 
+def test_slots_that_pass_32_bits():
+    """A page whose tokens have no 32-bit slot gives -1, which nothing is written to."""
+    edge = 2 ** 31 // 128
+    r, _ = _run([3, 2], [3, 130], [[edge, 0], [edge - 1, 7]], None, None, 0, 6, 4, 128)
+    assert r["slot_map"].tolist() == [-1, -1, -1, 7 * 128, 7 * 128 + 1, -1]
+    r, _ = _run([2], [128], [[edge - 1]], None, None, 0, 2, 1, 128)
+    assert r["slot_map"].tolist() == [2 ** 31 - 2, 2 ** 31 - 1]
+
+
 def test_refusals():
     import msa_for_sail as msa
     q, k, t = _i32([1, 1]), _i32([5, 6]), torch.zeros(2, 4, dtype=torch.int32, device="cuda")
