@@ -89,6 +89,9 @@ __device__ __forceinline__ void load_words(const unsigned char* at, uint32_t (&w
   w[0] = v.x; w[1] = v.y;
 }
 
+// 0xff for each byte that is an e4m3 NaN.
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t x) { return __vcmpeq4(x & 0x7f7f7f7fu, 0x7f7f7f7fu); }
+
 // The item of a CTA: rows of one KV head against a list of pages.
 struct Item {
   int b, kvh, split;
@@ -138,7 +141,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::CTAS) kv4_decode_kernel(con
   if (it.nrows <= 0) return;
   it.qo_base = p.qo_start[it.b];
   it.kv_len = p.kv_len[it.b];
-  it.off = p.qo_offset[it.b];
+  it.off = min(p.qo_offset[it.b], it.kv_len);                // (no sum below passes 32 bits)
   it.page_base = p.kv_page_indptr[it.b];
   // keys that rows may see: row r sees keys below lim(r), which grows with r
   auto lim = [&](int r) -> int { return min(it.kv_len, it.tok0 + (it.row0 + min(r, it.nrows - 1)) / it.pack + it.off + 1); };
@@ -320,6 +323,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::CTAS) kv4_decode_kernel(con
         fac[n][0] = f.x; fac[n][1] = f.y;
       }
       if (key0 + kKeys > lim_first) {
+        uint32_t nx = 0, ny = 0;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           const int2 f = *reinterpret_cast<const int2*>(smem + C::OFF_LIM + 4 * (8 * n + 2 * t4));
@@ -329,8 +333,30 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::CTAS) kv4_decode_kernel(con
             for (int c = 0; c < 4; ++c)
               if (key0 + 16 * u + 8 * (c >> 1) + key_at(g) >= (c & 1 ? f.y : f.x)) s[u][n][c] = -INFINITY;
         }
-        // nobody wrote behind the last key: a scale of V may be NaN there, and 0 x NaN is not 0
-        if (key0 + lane >= it.kv_len) *reinterpret_cast<uint2*>(vt + kCodeBytes + 8 * lane) = make_uint2(0, 0);
+        // P is 0 where a row does not see a key, but 0 x NaN is not.  Behind the last row's keys, where maybe nobody wrote, V becomes
+        // zero; a NaN that some of the rows see is taken out of V and put into their sums.
+        uint2* vs = reinterpret_cast<uint2*>(vt + kCodeBytes + 8 * lane);
+        if (key0 + lane >= lim_last) *vs = make_uint2(0, 0);
+        else if (lim_first < lim_last && key0 + lane >= lim_first) nx = nan_bytes(vs->x), ny = nan_bytes(vs->y);
+        if (__any_sync(0xffffffffu, nx | ny)) {
+          if (nx | ny) *vs = make_uint2(vs->x & ~nx, vs->y & ~ny);
+          uint32_t at = 0;                                   // keys with a NaN in this thread's 16 elements
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const uint32_t v = __ballot_sync(0xffffffffu, ((i < 4 ? nx : ny) >> (8 * (i & 3))) & 1);
+            if (i == g) at = v;
+          }
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              const int seen = reinterpret_cast<const int*>(smem + C::OFF_LIM)[8 * n + 2 * t4 + c] - key0;
+              if (seen > 0 && (at & (0xffffffffu >> (32 - min(seen, 32)))) != 0) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) o[i][n][c] = o[i][n][c + 2] = __int_as_float(0x7fc00000);
+              }
+            }
+        }
         __syncwarp();
       }
       bool raise = false;

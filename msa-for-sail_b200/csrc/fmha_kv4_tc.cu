@@ -56,7 +56,8 @@ constexpr int OFF_V = OFF_K + STAGES * TILE_BYTES;
 constexpr int OFF_RING = OFF_V + STAGES * TILE_BYTES;
 constexpr int OFF_BAR = OFF_RING + 2 * CONVERT_WARPS * RING * HALF;
 enum Bar { Q_FULL = 0, K_FULL = 1, K_EMPTY = 3, V_FULL = 5, V_EMPTY = 7, S_FULL = 9, P_FULL = 11, O_DONE = 13, NUM_BARS = 14 };
-constexpr int SMEM_BYTES = OFF_BAR + NUM_BARS * 8 + 16 + 1024;           // + slack to align the base to 1 KB
+constexpr int OFF_NAN = OFF_BAR + NUM_BARS * 8 + 16;          // per 16 elements of V: first key with a NaN that not all rows see
+constexpr int SMEM_BYTES = OFF_NAN + 32 + 1024;           // + slack to align the base to 1 KB
 static_assert(SMEM_BYTES <= 227 * 1024 && HALF % 16 == 0 && OFF_BAR % 16 == 0, "shared memory");
 constexpr int TMEM_COLS = 512, O_COL = 256;
 constexpr float kPOffset = 7.f, kRescale = 8.f, kNoMax = -3e38f;
@@ -84,6 +85,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv4_tc_kernel(const __grid_consta
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + OFF_BAR + NUM_BARS * 8);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + OFF_BAR + NUM_BARS * 8 + 4);
   volatile int* skip_flag = abort_flag + 1;
+  int* const nan_key = reinterpret_cast<int*>(smem + OFF_NAN);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   // ---------------- the item ----------------
@@ -93,7 +95,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv4_tc_kernel(const __grid_consta
   const int nrows = min(w.num_rows, ROWS);
   if (nrows <= 0) return;
   const int G = p.pack, kvh = head0 / (p.num_qo_heads / p.num_kv_heads);
-  const int qo_base = p.qo_start[b], kv_len = p.kv_len[b], off = p.qo_offset[b], page_base = p.kv_page_indptr[b];
+  const int qo_base = p.qo_start[b], kv_len = p.kv_len[b], off = min(p.qo_offset[b], kv_len), page_base = p.kv_page_indptr[b];
   // row r sees keys below lim(r), which grows with r
   auto lim = [&](int r) -> int { return min(kv_len, (w.row0 + r) / G + off + 1); };
   const int lim_first = lim(0), lim_last = lim(nrows - 1);
@@ -114,6 +116,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv4_tc_kernel(const __grid_consta
     }
     mbar_init(bar(O_DONE), 1);
     *abort_flag = 0;
+    for (int i = 0; i < 8; ++i) nan_key[i] = 0x7fffffff;
     mbar_fence_init();
   }
   if (warp == MMA_WARP) {
@@ -167,13 +170,23 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv4_tc_kernel(const __grid_consta
       __syncwarp();
       uint4 code[KEYS / 8];
       uint32_t scale[KEYS / 8];
-      const int keys = is_v ? kv_len - (first + j) * BN - cw * KEYS : KEYS;   // behind the last key V is zero (a scale may be NaN there)
+      const int key0 = (first + j) * BN + cw * KEYS + r8;
 #pragma unroll
       for (int i = 0; i < KEYS / 8; ++i) {
         const unsigned char* src = ring + place * HALF;
         code[i] = *reinterpret_cast<const uint4*>(src + code_at(8 * i + r8, q));
         scale[i] = *reinterpret_cast<const uint16_t*>(src + CODE_BYTES + (8 * i + r8) * kKv4ScaleBytes + 2 * q);
-        if (8 * i + r8 >= keys) scale[i] = 0;
+        // P is 0 where a row does not see a key, but 0 x NaN is not.  Behind the last row's keys, where maybe nobody wrote, V becomes
+        // zero; a NaN that some of the rows see is taken out, and they get it at the end.
+        if (is_v && key0 + 8 * i >= lim_first) {
+          if (key0 + 8 * i >= lim_last) scale[i] = 0;
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            if ((scale[i] >> (8 * h) & 0x7f) == 0x7f) {
+              atomicMin(nan_key + 2 * q + h, key0 + 8 * i);  // a minimum: the order does not matter
+              scale[i] &= ~(0xffu << (8 * h));
+            }
+        }
       }
       __syncwarp();                                          // all lanes have read this place of the ring
       if (j + RING < n_tiles) fetch(j + RING, place);
@@ -391,6 +404,8 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv4_tc_kernel(const __grid_consta
       }
       // ---- epilogue ----
       if (alive && n_tiles > 0) alive = mbar_wait_warp(bar(O_DONE), 0, abort_flag);
+      // (it has completed: the wait makes what the converting warps wrote into nan_key visible)
+      if (alive && n_tiles > 0) alive = mbar_wait_warp(bar(V_FULL + (n_tiles - 1) % STAGES), ((n_tiles - 1) / STAGES) & 1, abort_flag);
       const float vs = p.v_scale_head ? p.v_scale_head[kvh] : 1.f;
       const int64_t prow = (static_cast<int64_t>(split) * p.total_q + tok) * p.num_qo_heads + head;
       // columns c0 .. c0 + 7 of a row of the result; tok_, head_, prow_: the row
@@ -434,6 +449,10 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv4_tc_kernel(const __grid_consta
             float x[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(v[e + i]) * inv;
+            if (F == 1 && nan_key[2 * c + e / 16] < limit) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) x[i] = __int_as_float(0x7fc00000);
+            }
             if constexpr (F > 1) {
               float* dst = stage + trow * LD_O + c * 32 + e;
               *reinterpret_cast<float4*>(dst) = make_float4(x[0], x[1], x[2], x[3]);
@@ -465,7 +484,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv4_tc_kernel(const __grid_consta
 #pragma unroll
               for (int i = 0; i < 8; ++i) acc[i] += f[k] * stage[(k * ROWS + rr) * LD_O + c8 + i];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) acc[i] *= inv;
+            for (int i = 0; i < 8; ++i) acc[i] = nan_key[c8 / 16] < lim(rr) ? __int_as_float(0x7fc00000) : acc[i] * inv;
             const int row2 = w.row0 + rr;
             const int64_t tok2 = qo_base + row2 / G;
             const int head2 = head0 + row2 % G;

@@ -416,8 +416,8 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const MsaKv4ReadArgs a) {
   *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.out) + row * kHeadDim + 8 * l) = out;
 }
 
-// Whole pages, in the order of a page table: out[e, head, 128, 128] = page kv_indices[e].  A warp takes a row of 4 tokens ... of
-// one (page, head): 8 lanes per row would leave scales to be loaded twice; 16 lanes a row as above, 16 rows a block step.
+// Whole pages, in the order of a page table: out[e, head, 128, 128] = page kv_indices[e].  A block has a (page, head), 16 lanes a row as
+// above, so that the writes of a warp are 512 contiguous bytes; memory bounds it.
 __global__ void __launch_bounds__(256) kv4_unpack_kernel(const MsaKv4ReadArgs a) {
   chain_begin();
   const int l = threadIdx.x & 15;

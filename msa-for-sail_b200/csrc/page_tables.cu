@@ -44,13 +44,13 @@ __device__ __forceinline__ int request_of(const int32_t* start, int batch, int x
   return lo;
 }
 
-// Physical page of logical page p of request b, -1 if there is none.
+// Physical page of logical page p of request b, -1 if there is none (or sums of the lengths passed 32 bits and p is one of no request).
 __device__ __forceinline__ int page_of(const MsaPageTablesArgs& a, const Scans& s, int b, int p, int num_free) {
-  if (p >= a.table_width) return -1;
+  if (static_cast<unsigned>(p) >= static_cast<unsigned>(a.table_width)) return -1;
   const int held = s.held[b];
   if (p < held) return a.block_table[b * a.table_stride + p];
   const int r = s.rank[b] + p - held;
-  return r < num_free ? a.free_pages[num_free - 1 - r] : -1;
+  return static_cast<unsigned>(r) < static_cast<unsigned>(num_free) ? a.free_pages[num_free - 1 - r] : -1;
 }
 
 // Entries [first, .) of the flat table and of the tokens, `step` apart.

@@ -427,6 +427,52 @@ def test_step_of_a_serving_engine():
     assert num_free.tolist() == [24 - sum(-(-n // 128) for n in kl)]
 
 
+def _poison(b, seq, key, head, block, which=("k", "v")):
+    page = int(b.table[b.indptr[seq] + key // 128])
+    for c in which:
+        getattr(b, c).view(b.k.shape[0], b.hk, -1)[page, head, 128 * 64 + 8 * (key % 128) + block] = 0x7F
+
+
+@pytest.mark.parametrize("n,hq,hk", [(1, 16, 2), (1, 32, 2), (2, 8, 2), (4, 8, 2), (4, 16, 2), (16, 8, 2), (16, 16, 2)])
+@pytest.mark.parametrize("splits", [1, 2])
+def test_not_a_number_in_places_that_rows_do_not_see(n, hq, hk, splits):
+    """Keys behind a row's last one may be NaN, behind the last row's (stale places below the sequence's length) and between the rows'
+    (tokens of the same step): only rows that see such a key have it, in the 16 elements that share its scale."""
+    import msa_for_sail as msa
+    kv = [300, 128 + n // 2, 500]
+    b = Batch(70 + n, [n] * 3, kv, hq, hk, offsets=[300 - n - 90, 128 + n // 2 - n, 500 - n])
+    q, k, v, table = b.cuda()
+    lse = torch.empty(b.T, hq, device=DEV)
+    want = b.want()
+    for key in range(210, 300):
+        for block in range(8):
+            _poison(b, 0, key, 0, block)
+            _poison(b, 0, key, 1, block)
+    hit = {1: kv[1] - 1, 2: 500 - max(1, n // 2)}               # the last token, and one in the middle
+    for seq, key in hit.items():
+        _poison(b, seq, key, 1, 3, "v")
+    q, k, v, table = b.cuda()
+    out, _ = msa.fmha_sail(q, k, v, b.plan(num_kv_splits=splits), kv_indices=table, lse=lse)
+    nan = torch.zeros(b.T, hq, 128, dtype=torch.bool)
+    for seq, key in hit.items():
+        for i in range(n):
+            if i + b.offsets[seq] >= key:
+                nan[seq * n + i, hq // hk:, 48:64] = True
+    assert nan.any() and torch.equal(torch.isnan(out.cpu()), nan)
+    ref.check_attention(torch.where(nan.to(DEV), 0.0, out), lse, (torch.where(nan, 0.0, want[0]),) + tuple(want[1:]), P_F16, f"{n} tokens")
+
+
+def test_offsets_past_every_key():
+    """An offset that no sum may add to: every row sees every key."""
+    import msa_for_sail as msa
+    for n, hq in ((1, 16), (4, 32)):
+        b = Batch(71, [n, n], [300, 200], hq, 2, offsets=[1000, 1000])
+        q, k, v, table = b.cuda()
+        far = torch.full((2,), 2 ** 31 - 1, dtype=torch.int32, device=DEV)
+        out, _ = msa.fmha_sail(q, k, v, b.plan(), kv_indices=table, q_offset_override=far)
+        ref.check_attention(out, None, b.want(), P_F16, f"{n} tokens")
+
+
 @pytest.mark.parametrize("rows", [1, 4])
 @pytest.mark.parametrize("sparse", [False, True])
 def test_a_table_shorter_than_the_lengths(rows, sparse):
