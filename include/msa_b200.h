@@ -153,6 +153,12 @@ int msa_lse_merge_ex(const void* partial_o, int32_t partial_dtype, const float* 
                      int64_t out_stride_tok, int64_t out_stride_head,
                      float out_scale, msa_stream_t stream);
 
+/* The merge of dense fp32 partials [S, total_q, H, 128] with a CTA for each row, for many splits of few rows: the time of
+ * msa_lse_merge grows with the number of splits, this one's hardly does.  Sums are taken in another (fixed) order. */
+int msa_lse_merge_many(const float* partial_o, const float* partial_lse, const int32_t* splits_per_row, void* out,
+                       int32_t out_dtype, float* lse_out, int32_t num_splits, int32_t total_q, int32_t num_heads,
+                       int64_t out_stride_tok, int64_t out_stride_head, float out_scale, msa_stream_t stream);
+
 /* Page top-k: per (head, token) row of scores[H, K, T] pick the `topk` best
  * pages of [0, num_valid_pages) by (score desc, index asc), emit them
  * ascending into out[T, H, topk] (int32), pad with -1.  Pages [0, force_begin)

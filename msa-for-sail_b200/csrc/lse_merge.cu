@@ -89,8 +89,102 @@ lse_merge_kernel(const void* po_, const float* pl, const int32_t* spr,
   if (lse_out && l16 == 0) lse_out[row] = sw > 0.f ? mxs + __logf(sw) : -INFINITY;
 }
 
+// A CTA per row, for many splits of few rows: half a warp would take eight splits after eight.  Warp w has splits w, w + 4, ...,
+// eight of them on their way at a time, a lane four columns; the four sums are added in their order.  Bound by the latency of
+// three dependent reads (weights, partials, sums of the warps).
+constexpr int kManyWarps = 4, kManyChunk = 128;               // splits whose weights are in shared memory at a time
+template <bool OF32>
+__global__ void __launch_bounds__(32 * kManyWarps)
+lse_merge_many_kernel(const float* po, const float* pl, const int32_t* spr, void* out_, float* lse_out, int num_splits, int64_t rows,
+                      int num_heads, int64_t out_stride_tok, int64_t out_stride_head, float out_scale) {
+  chain_begin();
+  __shared__ float s_w[kManyChunk];
+  __shared__ float s_red[2][kManyWarps];
+  __shared__ float4 s_acc[kManyWarps][32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t row = blockIdx.x;
+  const int t = static_cast<int>(row / num_heads), h = static_cast<int>(row % num_heads);
+  const int S = spr ? min(spr[t], num_splits) : num_splits;
+  float first = -INFINITY, mx = -INFINITY;
+  for (int s = threadIdx.x; s < S; s += 32 * kManyWarps) {
+    const float l = pl[s * rows + row];
+    if (s < kManyChunk) first = l;
+    mx = fmaxf(mx, l);
+  }
+#pragma unroll
+  for (int d = 16; d; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+  if (lane == 0) s_red[0][warp] = mx;
+  __syncthreads();
+  mx = fmaxf(fmaxf(s_red[0][0], s_red[0][1]), fmaxf(s_red[0][2], s_red[0][3]));
+  const float mxs = mx == -INFINITY ? 0.f : mx;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  float sw = 0.f;
+  for (int c0 = 0; c0 < S; c0 += kManyChunk) {
+    const int n = min(kManyChunk, S - c0);
+    if (c0 > 0) __syncthreads();                               // the weights before these are no longer read
+    if (threadIdx.x < n) {
+      const float l = c0 == 0 ? first : pl[(c0 + threadIdx.x) * rows + row];
+      const float w = l != -INFINITY ? __expf(l - mxs) : 0.f;
+      s_w[threadIdx.x] = w;
+      sw += w;
+    }
+    __syncthreads();
+    const float* src = po + (c0 * rows + row) * kHeadDim + 4 * lane;
+    constexpr int U = 8;
+    for (int s0 = warp; s0 < n; s0 += kManyWarps * U) {
+      float4 x[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) x[u] = *reinterpret_cast<const float4*>(src + min(s0 + kManyWarps * u, n - 1) * rows * kHeadDim);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const float w = s0 + kManyWarps * u < n ? s_w[s0 + kManyWarps * u] : 0.f;
+        if (w != 0.f) {                                        // the partial of an empty split is not looked at
+          acc.x = fmaf(w, x[u].x, acc.x); acc.y = fmaf(w, x[u].y, acc.y);
+          acc.z = fmaf(w, x[u].z, acc.z); acc.w = fmaf(w, x[u].w, acc.w);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int d = 16; d; d >>= 1) sw += __shfl_xor_sync(0xffffffffu, sw, d);
+  if (lane == 0) s_red[1][warp] = sw;
+  s_acc[warp][lane] = acc;
+  __syncthreads();
+  if (warp != 0) return;
+  sw = (s_red[1][0] + s_red[1][1]) + (s_red[1][2] + s_red[1][3]);
+  const float inv = sw > 0.f || isnan(sw) ? out_scale / sw : 0.f;
+#pragma unroll
+  for (int w = 1; w < kManyWarps; ++w) {
+    const float4 o = s_acc[w][lane];
+    acc.x += o.x; acc.y += o.y; acc.z += o.z; acc.w += o.w;
+  }
+  const int64_t at = t * out_stride_tok + h * out_stride_head + 4 * lane;
+  if (OF32) *reinterpret_cast<float4*>(static_cast<float*>(out_) + at) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+  else *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(out_) + at) = make_uint2(pack2<false>(acc.x * inv, acc.y * inv), pack2<false>(acc.z * inv, acc.w * inv));
+  if (lse_out && lane == 0) lse_out[row] = sw > 0.f || isnan(sw) ? mxs + __logf(sw) : -INFINITY;
+}
+
 }  // namespace
 }  // namespace msa
+
+extern "C" int msa_lse_merge_many(const float* partial_o, const float* partial_lse, const int32_t* splits_per_row, void* out,
+                                  int32_t out_dtype, float* lse_out, int32_t num_splits, int32_t total_q, int32_t num_heads,
+                                  int64_t out_stride_tok, int64_t out_stride_head, float out_scale, msa_stream_t stream) {
+  if (!partial_o || !partial_lse || !out || num_splits < 1 || total_q < 0 || num_heads <= 0) return MSA_ERR_BAD_ARG;
+  if (out_dtype != MSA_DT_F32 && out_dtype != MSA_DT_BF16) return MSA_ERR_UNSUPPORTED;
+  const int64_t rows = static_cast<int64_t>(total_q) * num_heads;
+  if (rows == 0) return MSA_OK;
+  if (rows > 0x7fffffffLL) return MSA_ERR_TOO_LARGE;
+  // rows of partials are read 16 bytes at a time, those of the result written 16 or 8
+  const int oe = out_dtype == MSA_DT_BF16 ? 2 : 4;
+  if ((reinterpret_cast<uintptr_t>(partial_o) & 15) || reinterpret_cast<uintptr_t>(out) % (4 * oe) || out_stride_tok % 4 || out_stride_head % 4)
+    return MSA_ERR_BAD_ARG;
+  msa::NvtxRange range("msa_lse_merge_many");
+  const auto kernel = out_dtype == MSA_DT_F32 ? msa::lse_merge_many_kernel<true> : msa::lse_merge_many_kernel<false>;
+  return msa::launch_chained(kernel, dim3(static_cast<unsigned>(rows)), 32 * msa::kManyWarps, 0, static_cast<cudaStream_t>(stream), partial_o,
+                             partial_lse, splits_per_row, out, lse_out, num_splits, rows, num_heads, out_stride_tok, out_stride_head,
+                             out_scale) == cudaSuccess ? MSA_OK : MSA_ERR_LAUNCH;
+}
 
 extern "C" int msa_lse_merge_ex(const void* partial_o, int32_t partial_dtype, const float* partial_lse,
                                 const int32_t* splits_per_row, void* out, int32_t out_dtype, float* lse_out,

@@ -68,6 +68,18 @@ def test_page_table_arguments():
         assert run(**kw) == BAD, kw
 
 
+def test_merge_of_many_splits_arguments():
+    L = _lib()
+    ok = dict(po=PTR, pl=PTR, spr=None, out=PTR, dt=L.MSA_DT_BF16, lse=None, S=2, T=0, H=4, st=512, sh=128)
+    run = lambda **kw: (lambda a: L.lib.msa_lse_merge_many(a["po"], a["pl"], a["spr"], a["out"], a["dt"], a["lse"], a["S"], a["T"], a["H"], a["st"], a["sh"],
+                                                             1.0, None))({**ok, **kw})
+    assert run() == 0
+    for kw in (dict(po=None), dict(pl=None), dict(out=None), dict(S=0), dict(T=-1), dict(H=0), dict(T=1, po=PTR + 8), dict(T=1, out=PTR + 4),
+               dict(T=1, st=514), dict(T=1, sh=130)):
+        assert run(**kw) == BAD, kw
+    assert run(dt=L.MSA_DT_E4M3) == UNSUPPORTED
+
+
 def test_attention_arguments_of_a_4_bit_cache():
     L = _lib()
     ok = dict(q=PTR, k=PTR, v=PTR, out=PTR, qo_start=PTR, kv_len=PTR, qo_offset=PTR, kv_page_indptr=PTR, kv_indices=PTR, work=PTR, q_stride_tok=1024,
