@@ -16,8 +16,19 @@
 // brings its largest element to [2^14, 2^15): exact in f16 down to 2^-28 of the largest.  P is written as 2^(x - m + 7), with m at
 // most 8 behind the true maximum: at most 2^15, 11 bits down to 2^-21 of the largest weight.
 //
-// A CTA has four warps.  Warp w has keys 32 w .. 32 w + 31 of every page, a ring of its own that it fills with 16-byte copies, and a softmax of its own; the four states are joined at the end.  So the warps of an SM run
-// past one another without barriers.
+// A CTA has four warps.  Warp w has keys 32 w .. 32 w + 31 of every page, a ring of its own that it fills with 16-byte copies, and a
+// softmax of its own; the four states are joined at the end.  So the warps of an SM run past one another without barriers.  (Rings
+// filled by bulk copies, sixteen small ones a page and warp: 281 us instead of 246 for a million keys; one ring a CTA with a warp
+// that loads: 250.)
+//
+// Up to 8 rows to a head (NT = 1): four CTAs an SM, two pages in a ring; to 16 (NT = 2): three CTAs with three, or registers run out.
+// More rows: fmha_kv4_tc.cu, or, where a selection is a token's own, groups of 16.
+//
+// Measured: one sequence of 1 048 576 keys, 64 / 8 heads: 219 us and 5 for the merge, 5.5 TB/s of codes and scales.  The copies alone take 186 us,
+// the conversions and products alone 213: the issue slots (55 % used, a conversion is an instruction of two clocks on the ALU
+// pipe) bound it, together with what the two leave one another.  24 ragged sequences, 64 / 4 heads (NT = 2): 56 us, 3.4 TB/s; a page
+// takes an SM 1 300 clocks, 830 would be the memory's.  32 x 16 selected pages of 1 024, 64 / 8 heads: 22 us, 3.4 TB/s; index
+// loads, first page and epilogue of one wave of CTAs.
 #include <algorithm>
 
 #include "kv4.cuh"
@@ -183,12 +194,14 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::CTAS) kv4_decode_kernel(con
       // scales: K by the first half of the warp, V by the second
       cp_async16(dst + kCodeBytes + (lane < 16 ? 0 : C::HALF - 256), (lane < 16 ? k : v - 256) + (kKv4ScaleOffset - warp * (kCodeBytes - kScaleBytes)));
     }
-    cp_async_commit();
     return page >= 0 ? lp * kKvTile + kKeys * warp : -1;
   };
   int keys[C::STAGES];
 #pragma unroll
-  for (int j = 0; j < C::STAGES; ++j) keys[j] = j < n_tiles ? fetch(j, j) : -1;
+  for (int j = 0; j < C::STAGES; ++j) {
+    keys[j] = j < n_tiles ? fetch(j, j) : -1;
+    cp_async_commit();                                       // of fewer pages too: the waits below count groups
+  }
 
   // Q^T: warp n converts rows 8 n .. 8 n + 7 for all warps.
   const int g = lane >> 2, t4 = lane & 3;
@@ -438,7 +451,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::CTAS) kv4_decode_kernel(con
 #pragma unroll
     for (int i = 0; i + 1 < C::STAGES; ++i) keys[i] = keys[i + 1];
     if (j + C::STAGES < n_tiles) keys[C::STAGES - 1] = fetch(j + C::STAGES, stage);
-    else cp_async_commit();                                  // an empty group: the wait above counts groups
+    cp_async_commit();                                       // an empty group at the end
     if (++stage == C::STAGES) stage = 0;
   }
   float sums[NT][2];

@@ -2,8 +2,8 @@
 //
 // The tile of one (page, KV head) is 9 216 contiguous bytes: 128 rows of 64 bytes, two e2m1 codes a byte (element 2 i in the low
 // half of byte i), then 128 rows of eight e4m3 scales, one for each 16 elements.  An element is code * scale; a scale per KV
-// head (the k_scale / v_scale of the attention call) comes on top.  Codes before scales, so that both are read in
-// 16-byte pieces and one bulk copy brings the tile; 16 elements a scale, 72 bytes a row: 0.56 of an e4m3 row.
+// head (the k_scale / v_scale of the attention call) comes on top.  Codes before scales, so that both are read in 16-byte pieces;
+// 16 elements a scale, 72 bytes a row: 0.56 of an e4m3 row.
 #pragma once
 
 #include "common.cuh"
@@ -13,7 +13,6 @@ namespace msa {
 constexpr int kKv4CodeBytes = kHeadDim / 2;                   // of a row
 constexpr int kKv4ScaleBytes = kHeadDim / 16;
 constexpr int kKv4ScaleOffset = kKvTile * kKv4CodeBytes;
-constexpr int kKv4TileBytes = kKvTile * (kKv4CodeBytes + kKv4ScaleBytes);
 constexpr float kKv4MinScale = 0x1p-9f;                       // the smallest e4m3 number: no block of small values is lost to a scale of zero
 
 // Four bytes of codes (8 elements) -> four f16 pairs, the low half of a byte in the low half of a pair.

@@ -8,9 +8,9 @@
 // wrapping integer product, exact to 2^-64 turns times the position at any position; the cosine and sine of what is left
 // are taken once per token and pair and shared by all heads.
 //
-// Keys that are quantised are normed and rotated in 64 bits, rounded to bf16 once and quantised from there: which e4m3 or e2m1
-// value a key next to a border gets does not depend on the order of a sum.  (They are a tenth of the rows or less.)  All
-// else is computed in 32 bits and rounded once.
+// Keys that go into a cache are normed and rotated in 64 bits, rounded to bf16 once and quantised from there: which bf16, e4m3 or
+// e2m1 value a key next to a border gets does not depend on the order of a sum.  (They are a tenth of the rows or less.)
+// All else is computed in 32 bits and rounded once.
 //
 // 4-bit rows: 16 elements share an e4m3 scale s = round(max|x| / 6), at least 2^-9; the codes are the e2m1 roundings of x / s
 // (divisions as IEEE has them: an x on a border goes to the even code).  A NaN makes the scale of its 16 elements NaN.
@@ -353,7 +353,7 @@ __global__ void __launch_bounds__(32, kCtas) norm_rope_kernel(const __grid_const
 #ifdef MSA_BOUNDS_CHECK
   if (slot >= 0 && a.slot_map && !has_slot) chk(slot, 0, 0, a.status);
 #endif
-  const bool fine = a.k_cache && a.cache_dtype != MSA_DT_BF16;   // keys are quantised
+  const bool fine = a.k_cache != nullptr;                    // keys in 64 bits
   if (a.k && NORM && !fine) load_w8(a.k_weight, 0);
 #pragma unroll 1
   for (u -= q_units; a.k && u < kv_units; u += parts) {

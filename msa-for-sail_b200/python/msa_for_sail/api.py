@@ -1173,7 +1173,9 @@ def fmha_sail_plan(
     (forwarded to ``_fmha_sail_plan``): ``num_kv_heads``, ``num_kv_splits``,
     ``page_size``, ``output_maxscore``, ``kv_block_num``, ``usable_SM_count``,
     ``causal``, ``use_fp8_kvcache``, ``device``, ``stream``, ``given_workspace``,
-    ``max_total_q``, ``graph_safe`` and the ``*_override`` hints.  With
+    ``max_total_q``, ``graph_safe``, ``use_kv4_cache`` (a cache of
+    ``allocate_kv4_cache``: ``page_size=128``; how the work is cut depends on it, not the
+    result) and the ``*_override`` hints.  With
     ``split_prefill_decode`` a decode-first batch is planned as two sub-batches, each with
     the tile shape that suits it.
     """
@@ -1261,6 +1263,13 @@ def fmha_sail(
     ``q_scale``, ``k_scale``, ``v_scale``, ``o_scale``, ``output_maxscore``, ``output_o``,
     ``max_score_dtype``, ``check_input_valid``.  Returns ``(out, max_score)``; either may be
     ``None`` when that output is disabled.
+
+    ``k``/``v`` may also be the uint8 tensors of ``allocate_kv4_cache`` (4 bits a value), with a plan
+    of ``page_size=128`` (and ``use_kv4_cache=True``, which cuts the work for them).  Decode and sparse
+    decode read the 4 bits themselves, with up to 128 rows (tokens x query heads) to a KV head; longer
+    queries, page scores and sparse prefill run on bf16 copies of the pages in ``kv_indices``, which
+    live for the call (``len(kv_indices) * Hkv * 32`` KB each for keys and values; planned pages and a
+    fixed-address table alike, so a captured prefill has a table no longer than its use).
     """
     mixed, cut, batch_size, first, second = plan_info
     if not mixed:

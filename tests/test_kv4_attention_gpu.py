@@ -586,3 +586,18 @@ def test_refusals():
         with pytest.raises((ValueError, AssertionError)):
             f()
             print("not refused:", i)
+
+
+@pytest.mark.parametrize("hq", [8, 16])
+def test_lists_of_fewer_pages_than_stages(hq):
+    """One to three pages an item, pages that are not in a cache of the device, many items at once."""
+    import msa_for_sail as msa
+    kv = [1 + 37 * i % 384 for i in range(600)]
+    b = Batch(81, [1] * len(kv), kv, hq, 1)
+    q, k, v, table = b.cuda()
+    plan, want = b.plan(num_kv_splits=1), b.want()
+    flush = torch.zeros(1 << 28, dtype=torch.uint8, device=DEV)
+    for _ in range(8):
+        flush.add_(1)
+        out, _ = msa.fmha_sail(q, k, v, plan, kv_indices=table)
+        ref.check_attention(out, None, want, P_F16, f"{hq} rows")

@@ -34,3 +34,17 @@ def test_register_moves_are_checked_before_the_launch():
 @pytest.mark.parametrize("name", ["fmha_kv4.cu", "fmha_kv4_tc.cu"])
 def test_kernels_read_coherently(name):
     assert not re.search(r"__restrict__|__ldg\b|\.nc\b", code(name))
+
+
+@pytest.mark.parametrize("name", ["fmha_kv4.cu", "fmha_kv4_tc.cu"])
+def test_every_stage_is_a_group_of_copies(name):
+    """A warp waits for all but the newest groups of its copies: a list of fewer pages than stages has a group for each stage all the same,
+    or its last pages would be read while they are on their way."""
+    text = code(name)
+    before = text.split("cp_async_wait<")[0]
+    prologue = re.search(r"for \(int j = 0; j < (?:C::STAGES|RING); \+\+j\) \{(.*?)\n\s*\}", before, flags=re.S).group(1)
+    assert re.search(r"^\s*cp_async_commit\(\);", prologue, flags=re.M)
+    loop = text.split("cp_async_wait<", 1)[1]
+    assert len(re.findall(r"^\s*cp_async_commit\(\);", loop, flags=re.M)) == 1 and "else cp_async_commit" not in loop
+    fetch = re.search(r"auto fetch = (.*?)\n    \};|auto fetch = (.*?)\n  \};", text, flags=re.S).group(0)
+    assert "cp_async_commit" not in fetch

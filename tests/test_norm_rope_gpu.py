@@ -301,3 +301,22 @@ def test_refusals():
     bf = torch.zeros(2, 2, 128, 128, dtype=torch.bfloat16, device=DEV)
     with pytest.raises(ValueError):
         msa.kv_cache_append(k, v, bf, bf.clone(), sl, k_scale=0.5)
+
+
+def test_keys_of_a_bf16_cache_are_rounded_once():
+    """Cached keys are computed in 64 bits: they are the nearest bf16 numbers, also where 32 bits would fall on the other side of a border."""
+    import msa_for_sail as msa
+    T, hk = 900, 4
+    q, k, v, g = _inputs(91, T, 4, hk)
+    w = torch.rand(128, generator=g) + 0.5
+    pos, inv = torch.randint(0, 100_000, (1, T), generator=g), [1e4 ** (-2 * i / 128) for i in range(64)]
+    kc, vc = _cache("bf16", 8, hk)
+    slots = torch.randperm(1024, generator=g)[:T].to(torch.int32)
+    msa.qk_norm_rope(q, k, pos.to(DEV), msa.rope_plan(128), v=v, q_weight=w.to(DEV), k_weight=w.to(DEV), k_cache=kc, v_cache=vc, slot_map=slots.to(DEV))
+    want, _ = ref.norm_rope(k, pos, inv, [64], False, w)
+    # 64-bit angles of the reference are good to 1e5 x 2^-53: borders that close are left out
+    near = (want.float().to(torch.bfloat16).double() - want).abs()
+    step = 2.0 ** (torch.floor(torch.log2(want.abs().clamp(min=1e-30))) - 7)
+    clear = (near / step - 0.5).abs() > 1e-7
+    got = _rows(kc, slots, "bf16", False)
+    assert clear.float().mean() > 0.999 and torch.equal(got[clear], want.float().to(torch.bfloat16)[clear])
