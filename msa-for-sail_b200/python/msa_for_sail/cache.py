@@ -39,8 +39,11 @@ def _on(device):
 
 def _launch(device, fn, args, what):
     """`fn` on the current stream of `device`."""
-    if device.index == torch._C._cuda_getDevice():
-        _lib.check(fn(ctypes.byref(args), torch._C._cuda_getCurrentRawStream(device.index)), what)
+    index = device.index
+    if index == torch._C._cuda_getDevice():
+        rc = fn(ctypes.byref(args), torch._C._cuda_getCurrentRawStream(index))
+        if rc:
+            _lib.check(rc, what)
     else:
         with torch.cuda.device(device):
             _lib.check(fn(ctypes.byref(args), _stream()), what)
@@ -84,15 +87,16 @@ def _check_kv4(name, t, num_kv_heads=None):
     return stride
 
 
-def _read(cache, index, out, whole_pages):
-    if index.shape[0] == 0:
+def _read(cache, stride, index, out, whole_pages):
+    rows, shape = index.shape[0], cache.shape
+    if rows == 0:
         return out
-    if cache.shape[0] == 0:
+    if shape[0] == 0:
         return out.zero_()
     dev = cache.device
-    _launch(dev, _lib.lib.msa_kv4_read, _lib.MsaKv4ReadArgs(
-        cache.data_ptr(), out.data_ptr(), index.data_ptr(), _status_ptr(dev), cache.stride(0), cache.stride(1), index.shape[0], cache.shape[1],
-        cache.shape[0], whole_pages), "msa_kv4_read")
+    _launch(dev, _lib.lib.msa_kv4_read, _lib.kv4_read_args(
+        cache.data_ptr(), out.data_ptr(), index.data_ptr(), _status_ptr(dev) or 0, stride[0], stride[1], rows, shape[1], shape[0], whole_pages),
+        "msa_kv4_read")
     return out
 
 
@@ -107,24 +111,25 @@ def kv4_read(cache: torch.Tensor, slot_map: torch.Tensor, out: Optional[torch.Te
     """Rows of a 4-bit cache as bf16 ``[tokens, Hkv, 128]`` (exact: code times scale; a scale per head is not applied).
 
     ``slot_map``: int32, ``page * 128 + offset`` of each token; rows of a negative slot are zeros."""
-    _check_kv4("cache", cache)
+    stride = _check_kv4("cache", cache)
     if not cache.is_cuda:
         raise RuntimeError("kv4_read needs CUDA tensors (there is no CPU path)")
-    _check_index("slot_map", slot_map, cache.device)
+    dev = cache.device
+    _check_index("slot_map", slot_map, dev)
     shape = (slot_map.shape[0], cache.shape[1], 128)
     if out is None:
-        out = torch.empty(shape, dtype=torch.bfloat16, device=cache.device)
+        out = torch.empty(shape, dtype=torch.bfloat16, device=dev)
     else:
-        _same_device(cache.device, out=out)
+        _same_device(dev, out=out)
         if out.dtype != torch.bfloat16 or tuple(out.shape) != shape or not out.is_contiguous():
             raise ValueError(f"out must be contiguous bf16 {shape}, got {out.dtype} {tuple(out.shape)}")
-    return _read(cache, slot_map, out, False)
+    return _read(cache, stride, slot_map, out, 0)
 
 
 def unpack_pages(cache, kv_indices):
     """Pages of a 4-bit cache as bf16 ``[len(kv_indices), Hkv, 128, 128]``; pages outside the cache are left as they were."""
     out = torch.empty(kv_indices.shape[0], cache.shape[1], KV4_TILE, 128, dtype=torch.bfloat16, device=cache.device)
-    return _read(cache, kv_indices, out, True)
+    return _read(cache, cache.stride(), kv_indices, out, 1)
 
 
 # ----------------------------------------------------------------------------
@@ -193,14 +198,14 @@ def _rows(name, t, heads, tokens, device, dtypes=(torch.bfloat16,)):
 
 def _weight(name, w, heads, device):
     if w is None:
-        return None, 0
+        return 0, 0
     if w.get_device() != device.index:
         raise ValueError(f"{name} is on {w.device}, expected {device}")
     if w.dtype not in (torch.float32, torch.bfloat16):
         raise ValueError(f"{name} must be float32 or bfloat16, got {w.dtype}")
-    shape, stride = tuple(w.shape), w.stride()
+    shape, stride = w.shape, w.stride()
     if shape != (128,) and shape != (heads, 128):
-        raise ValueError(f"{name} must be [128] or [{heads}, 128], got {shape}")
+        raise ValueError(f"{name} must be [128] or [{heads}, 128], got {tuple(shape)}")
     if stride[-1] != 1 or (len(shape) == 2 and stride[0] % 8) or w.data_ptr() % 16:
         raise ValueError(f"{name}: rows must be contiguous and start at multiples of 16 bytes")
     return w.data_ptr(), stride[0] if len(shape) == 2 else 0
@@ -209,14 +214,14 @@ def _weight(name, w, heads, device):
 def _scale(name, x, heads, device):
     """A scale is a float, or an fp32 tensor with one value per KV head (it stays on the device)."""
     if x is None:
-        return 1.0, None
+        return 1.0, 0
     if isinstance(x, torch.Tensor):
         if x.dtype != torch.float32 or x.numel() != heads or not x.is_contiguous():
             raise ValueError(f"{name} must be a float or a contiguous float32 tensor of {heads} values, got {x.dtype} {tuple(x.shape)}")
         if x.get_device() != device.index:
             raise ValueError(f"{name} is on {x.device}, expected {device}")
         return 1.0, x.data_ptr()
-    return float(x), None
+    return float(x), 0
 
 
 _CACHE_DTYPES = {torch.bfloat16: MSA_DT_BF16, torch.float8_e4m3fn: MSA_DT_E4M3, torch.uint8: MSA_DT_KV4}
@@ -268,7 +273,7 @@ def _cache_args(k_cache, v_cache, heads, slot_map, tokens, page_size, k_scale, v
             _scale("k_scale", k_scale, heads, device), _scale("v_scale", v_scale, heads, device))
 
 
-_NO_CACHE = (MSA_DT_BF16, (None, 0, 0, 0), (None, 0, 0, 0), (1.0, None), (1.0, None))
+_NO_CACHE = (MSA_DT_BF16, (0, 0, 0, 0), (0, 0, 0, 0), (1.0, 0), (1.0, 0))
 
 
 def qk_norm_rope(
@@ -317,9 +322,9 @@ def qk_norm_rope(
             raise ValueError("a rotation needs positions")
         if positions.dtype != torch.int32 and positions.dtype != torch.int64:
             raise ValueError(f"positions must be int32 or int64, got {positions.dtype}")
-        axes, shape = rope["axes"], tuple(positions.shape)
+        axes, shape = rope["axes"], positions.shape
         if shape != (axes, T) and not (axes == 1 and shape == (T,)):
-            raise ValueError(f"positions must be [{axes}, {T}]" + (f" or [{T}]" if axes == 1 else "") + f", got {shape}")
+            raise ValueError(f"positions must be [{axes}, {T}]" + (f" or [{T}]" if axes == 1 else "") + f", got {tuple(shape)}")
         pos_stride = positions.stride()
         if T > 1 and pos_stride[-1] != 1:
             raise ValueError("positions of one axis must be contiguous")
@@ -329,7 +334,7 @@ def qk_norm_rope(
         pos = (positions.data_ptr(), turns.data_ptr(), axis.data_ptr(), pos_stride[0] if len(shape) == 2 else 0, rope["rotary_dim"],
                rope["interleaved"], positions.dtype == torch.int64)
     else:
-        pos = (None, None, None, 0, 0, 0, 0)
+        pos = (0, 0, 0, 0, 0, 0, 0)
     if (k_cache is None) != (v_cache is None) or (v_cache is None) != (v is None):
         raise ValueError("k_cache, v_cache and v go together")
     if k_cache is not None:
@@ -340,7 +345,7 @@ def qk_norm_rope(
         if k_scale is not None or v_scale is not None or slot_map is not None:
             raise ValueError("slot_map, k_scale and v_scale belong to a cache")
         dtype, kc, vc, ks, vs = _NO_CACHE
-        v_ptr, v_strides, slots, num_pages = None, (0, 0), None, 0
+        v_ptr, v_strides, slots, num_pages = 0, (0, 0), 0, 0
     if q_out is None:
         q_out = torch.empty(q.shape, dtype=torch.bfloat16, device=dev)
         qo_strides = (hq * 128, 128)
@@ -361,12 +366,12 @@ def qk_norm_rope(
     w = q_weight if q_weight is not None else k_weight
     if T == 0:
         return q_out, k_out
-    _launch(dev, _lib.lib.msa_norm_rope, _lib.MsaNormRopeArgs(
-        q.data_ptr(), k.data_ptr(), v_ptr, qw, kw, pos[0], pos[1], pos[2], q_out.data_ptr(), None if k_out is None else k_out.data_ptr(),
-        kc[0], vc[0], slots, ks[1], vs[1], _status_ptr(dev), pos[3], *q_strides, *k_strides, *v_strides, *qo_strides, *ko_strides, qw_stride, kw_stride,
-        kc[1], kc[2], kc[3], vc[1], vc[2], vc[3], T, hq, hk, pos[4], pos[5], 1 if norm else 0,
+    _launch(dev, _lib.lib.msa_norm_rope, _lib.norm_rope_args(
+        q.data_ptr(), k.data_ptr(), v_ptr, qw, kw, pos[0], pos[1], pos[2], q_out.data_ptr(), 0 if k_out is None else k_out.data_ptr(),
+        kc[0], vc[0], slots, ks[1], vs[1], _status_ptr(dev) or 0, pos[3], *q_strides, *k_strides, *v_strides, *qo_strides, *ko_strides, qw_stride,
+        kw_stride, kc[1], kc[2], kc[3], vc[1], vc[2], vc[3], T, hq, hk, pos[4], pos[5], 1 if norm else 0,
         MSA_DT_BF16 if w is not None and w.dtype == torch.bfloat16 else MSA_DT_F32, MSA_DT_E4M3 if q8 else MSA_DT_BF16, dtype, pos[6],
-        page_size if slots is not None else 0, num_pages, eps, 1.0 if q_scale is None else q_scale, ks[0], vs[0]), "msa_norm_rope")
+        page_size if slots else 0, num_pages, eps, 1.0 if q_scale is None else q_scale, ks[0], vs[0]), "msa_norm_rope")
     return q_out, k_out
 
 
@@ -401,6 +406,9 @@ def kv_cache_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_c
 
 class PageTables(dict):
     """Tensors of a step's paged cache, made by ``paged_kv_tables``."""
+
+
+_TABLES = ("kv_indices", "kv_page_indptr", "slot_map", "positions", "num_missing", "num_held", "num_free")
 
 
 def paged_kv_tables(
@@ -444,8 +452,8 @@ def paged_kv_tables(
         raise ValueError(f"block_table must be int32 [{B}, width] with contiguous rows, got {block_table.dtype} {tuple(block_table.shape)}")
     if B > 1 and block_table.stride(0) < block_table.shape[1]:
         raise ValueError("rows of block_table must not overlap")
-    if page_size < 1 or max_total_q < 0:
-        raise ValueError(f"page_size={page_size} must be positive, max_total_q={max_total_q} must not be negative")
+    if not 1 <= page_size <= (1 << 31) - 1 or max_total_q < 0:
+        raise ValueError(f"page_size={page_size} must be positive and fit int32, max_total_q={max_total_q} must not be negative")
     alloc = num_held is not None
     if alloc != (free_pages is not None) or alloc != (num_free is not None):
         raise ValueError("num_held, free_pages and num_free go together")
@@ -455,7 +463,6 @@ def paged_kv_tables(
     total_pages = B * width if max_total_pages is None else int(max_total_pages)
     if total_pages < 0 or total_pages > (1 << 31) - 1 or max_total_q > (1 << 31) - 1:
         raise ValueError(f"max_total_pages={total_pages} and max_total_q={max_total_q} must fit int32")
-    sizes = {"kv_indices": total_pages, "kv_page_indptr": B + 1, "slot_map": max_total_q, "positions": max_total_q, "num_missing": 1}
     if alloc:
         for name, t, n in (("num_held", num_held, B), ("free_pages", free_pages, None), ("num_free", num_free, 1),
                            ("num_held_out", num_held_out, B), ("num_free_out", num_free_out, 1)):
@@ -464,29 +471,31 @@ def paged_kv_tables(
             _check_index(name, t, dev)
             if n is not None and t.shape[0] != n:
                 raise ValueError(f"{name} must have {n} entries, got {t.shape[0]}")
-        sizes.update(num_held=B, num_free=1)
     if block_table.get_device() != dev.index:
         raise ValueError(f"block_table is on {block_table.device}, expected {dev}")
+    names, counts = (_TABLES, [total_pages, B + 1, max_total_q, max_total_q, 1, B, 1]) if alloc else (_TABLES[:5], [total_pages, B + 1, max_total_q, max_total_q, 1])
+    given = {"num_held": num_held_out, "num_free": num_free_out} if num_held_out is not None or num_free_out is not None else {}
     if out is not None:
-        for name, n in sizes.items():
+        for name, n in zip(names, counts):
             _check_index(f"out[{name!r}]", out[name], dev)
             if out[name].shape[0] != n:
                 raise ValueError(f"out[{name!r}] must have {n} entries, got {out[name].shape[0]}")
+        given = {**out, **{name: t for name, t in given.items() if t is not None}}
     ws_ints = (_lib.check(_lib.lib.msa_page_tables_workspace_bytes(B), "msa_page_tables_workspace_bytes") + 3) // 4
-    given = {"num_held": num_held_out, "num_free": num_free_out} if out is None else {**out, **{
-        name: t for name, t in (("num_held", num_held_out), ("num_free", num_free_out)) if t is not None}}
-    names = [name for name in sizes if given.get(name) is None]
     # one allocation for the outputs and the scans
-    counts = [sizes[name] for name in names] + [ws_ints]
-    parts = torch.empty(sum(counts), dtype=torch.int32, device=dev).split_with_sizes(counts)
-    res = PageTables(zip(names, parts))
-    for name in sizes:
-        if name not in res:
-            res[name] = given[name]
-    null = (None, None, None, None, None, 0)
+    if given:
+        kept = {name: given[name] for name in names if given.get(name) is not None}
+        fresh = [(name, n) for name, n in zip(names, counts) if name not in kept]
+        counts = [n for _, n in fresh] + [ws_ints]
+        parts = torch.empty(sum(counts), dtype=torch.int32, device=dev).split_with_sizes(counts)
+        res = PageTables(zip([name for name, _ in fresh], parts), **kept)
+    else:
+        counts.append(ws_ints)
+        parts = torch.empty(sum(counts), dtype=torch.int32, device=dev).split_with_sizes(counts)
+        res = PageTables(zip(names, parts))
     held = (num_held.data_ptr(), free_pages.data_ptr(), num_free.data_ptr(), res["num_held"].data_ptr(), res["num_free"].data_ptr(),
-            free_pages.shape[0]) if alloc else null
-    _launch(dev, _lib.lib.msa_page_tables, _lib.MsaPageTablesArgs(
+            free_pages.shape[0]) if alloc else (0, 0, 0, 0, 0, 0)
+    _launch(dev, _lib.lib.msa_page_tables, _lib.page_tables_args(
         qo_lens.data_ptr(), kv_lens.data_ptr(), block_table.data_ptr(), held[0], held[1], held[2], res["kv_indices"].data_ptr(),
         res["kv_page_indptr"].data_ptr(), res["slot_map"].data_ptr(), res["positions"].data_ptr(), held[3], held[4], res["num_missing"].data_ptr(),
         parts[-1].data_ptr(), block_table.stride(0) if B > 1 else width, B, width, page_size, max_total_q, total_pages, held[5]), "msa_page_tables")
