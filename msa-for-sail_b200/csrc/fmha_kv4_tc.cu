@@ -3,11 +3,11 @@
 // With so many rows to a KV head the products outgrow mma.sync, and the conversion of a page should be shared by all of them.  One CTA =
 // one work item; its packed rows are the rows of a 128-row MMA tile.
 //
-//   warps 0-3    softmax and epilogue: thread r owns row r; at first they convert Q.  With at most 128 / F rows (F = 2, 4) the rows stand
+//   warps 0-3    softmax and epilogue: thread r owns row r; at first they convert Q into TMEM.  With at most 128 / F rows (F = 2, 4) the rows stand
 //                F times in the tile, and copy f has keys 128 / F * f .. of every page, with a maximum and a sum of its own and zeros in
 //                P elsewhere: all four warps work on a page (32 sequences x 4 tokens x 16 heads: 94 us with half of the threads idle).
 //                The F states of a row are joined at the end
-//   warp 4       issues S[j & 1] = Q K_j^T (tcgen05, f16 operands, accumulators in TMEM)
+//   warp 4       issues S[j & 1] = Q K_j^T (tcgen05, f16 operands, Q and accumulators in TMEM: 75.0 us with Q in shared memory)
 //   warp 5       issues O += P_j V_j (P from TMEM).  (One warp for both took 2 150 clocks a page: 1 350 to issue, which is what
 //                the tensor pipe takes, and 250 for each of three waits, ready or not.)
 //   warps 8-23   conversion, eight warps for K and eight for V: warp w has keys 16 w .. 16 w + 15 of every page.  16-byte copies bring
@@ -21,11 +21,13 @@
 // lags by at most 8.
 //
 // A page costs 64 KB written to shared memory and as much read by the MMAs, about 1 000 clocks of its bandwidth, 500 clocks of conversions
-// per scheduler, and with 128 rows 1 000 clocks of exponentials; its 18 KB from memory are 810.  Measured: 32 sequences of 131 to 16 384
-// keys x 4 tokens, 64 / 4 heads, 64 rows to a head: 68 us and 7 for the merge, 2 130 clocks a page (149 us in groups of 16 rows on fmha_kv4.cu,
-// which convert every page four times); with 128 rows 2 600.  The chain of a page through one warpgroup bounds it: read S, mask, maximum, exponentials,
-// write P, wait for the next S.  Two warpgroups that take turns (one buffer of S each, or registers run out) and one warp that
-// hands over K and V together were slower.  Every wait is bounded (tc_ptx.cuh).
+// per scheduler, and with 128 rows 1 000 clocks of exponentials; its 18 KB from memory are 810.  Measured: 32 sequences of 131 to
+// 16 384 keys x 4 tokens, 64 / 4 heads, 64 rows to a head: 67 us and 7 for the merge, 2 100 clocks a page (149 us in groups of 16 rows on
+// fmha_kv4.cu, which convert every page four times); with 128 rows 2 600, with 32 rows 1 900.  From 64 rows on the softmax
+// warpgroup bounds it, which is never without work: 550 clocks to read S, take the maximum and vote, 1 100 for exponentials and P; below that the
+// converting warps: 600 clocks to read codes and order more, 400 for a free tile, 650 to convert and fence.  Two softmax warpgroups that take
+// turns (one buffer of S each, or registers run out), one warp that hands over K and V together, a fourth page on its way: slower or no gain.
+// Every wait is bounded (tc_ptx.cuh).
 #include <algorithm>
 
 #include "kv4.cuh"
@@ -54,8 +56,7 @@ constexpr int KEYS = BN / CONVERT_WARPS;                     // of a page that a
 constexpr int CODE_BYTES = KEYS * kKv4CodeBytes, SCALE_BYTES = KEYS * kKv4ScaleBytes;
 constexpr int HALF = CODE_BYTES + SCALE_BYTES;               // of a warp's keys
 
-constexpr int OFF_Q = 0;
-constexpr int OFF_K = TILE_BYTES;
+constexpr int OFF_K = 0;
 constexpr int OFF_V = OFF_K + STAGES * TILE_BYTES;
 constexpr int OFF_RING = OFF_V + STAGES * TILE_BYTES;
 constexpr int OFF_BAR = OFF_RING + 2 * CONVERT_WARPS * RING * HALF;
@@ -63,7 +64,7 @@ enum Bar { Q_FULL = 0, K_FULL = 1, K_EMPTY = 3, V_FULL = 5, V_EMPTY = 7, S_FULL 
 constexpr int OFF_NAN = OFF_BAR + NUM_BARS * 8 + 16;          // per 16 elements of V: first key with a NaN that not all rows see
 constexpr int SMEM_BYTES = OFF_NAN + 32 + 1024;           // + slack to align the base to 1 KB
 static_assert(SMEM_BYTES <= 227 * 1024 && HALF % 16 == 0 && OFF_BAR % 16 == 0, "shared memory");
-constexpr int TMEM_COLS = 512, O_COL = 256;
+constexpr int TMEM_COLS = 512, O_COL = 256, Q_COL = 384;        // S twice, O, Q
 constexpr float kPOffset = 7.f, kRescale = 8.f, kNoMax = -3e38f;
 
 // kind::f16 with f16 operands and f32 accumulation
@@ -225,6 +226,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv4_tc_kernel(const __grid_consta
     if (warp == MMA_WARP) {
       constexpr uint32_t IDESC_QK = idesc_f16(BM, BN, false);
       bool alive = n_tiles > 0 && mbar_wait_warp(bar(Q_FULL), 0, abort_flag);
+      tc_fence_after();
       for (int j = 0; j < n_tiles && alive; ++j) {
         const int st = j % STAGES;
         // V_EMPTY: P_{j-2} V_{j-2} is done, which read P from this buffer of S
@@ -233,11 +235,11 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv4_tc_kernel(const __grid_consta
         if (!alive) break;
         tc_fence_after();
         if (elect_one()) {
-          const uint32_t qa = (base + OFF_Q) >> 4, ka = (base + OFF_K + st * TILE_BYTES) >> 4;
+          const uint32_t ka = (base + OFF_K + st * TILE_BYTES) >> 4;
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
             const uint32_t o = ((k >> 2) * SUB_BYTES + (k & 3) * 32) >> 4;
-            mma_ss(tmem + st * BN, dk_hi | ((qa + o) & 0x3FFF), dk_hi | ((ka + o) & 0x3FFF), IDESC_QK, k > 0);
+            mma_ts(tmem + st * BN, tmem + Q_COL + k * 8, dk_hi | ((ka + o) & 0x3FFF), IDESC_QK, k > 0);
           }
           mma_commit(bar(S_FULL + st));
           mma_commit(bar(K_EMPTY + st));
@@ -313,14 +315,20 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv4_tc_kernel(const __grid_consta
         e = max(e, -126);
         const float up = copysignf(scale == 0.f ? 0.f : __uint_as_float(static_cast<uint32_t>(127 - e) << 23), scale);
         if (scale != 0.f) fac = fabsf(scale) * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
-#pragma unroll 4
-        for (int c = 0; c < 16; ++c) {
-          float x[8];
-          load8(c, x);
-          *reinterpret_cast<uint4*>(smem + OFF_Q + tile_at(trow, c)) = make_uint4(pack2<true>(x[0] * up, x[1] * up), pack2<true>(x[2] * up, x[3] * up),
-                                                                            pack2<true>(x[4] * up, x[5] * up), pack2<true>(x[6] * up, x[7] * up));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            float x[8];
+            load8(4 * i + c, x);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) pk[4 * c + e] = pack2<true>(x[2 * e] * up, x[2 * e + 1] * up);
+          }
+          tmem_st16(tmem + Q_COL + 16 * i + lane_addr, pk);
         }
-        fence_proxy_async_smem();
+        tmem_wait_st();
+        tc_fence_before();
         mbar_arrive(bar(Q_FULL));
       }
       float m = kNoMax, l = 0.f;                               // maximum - kPOffset, sum of P
