@@ -265,7 +265,7 @@ int msa_fmha_fwd_split_static(const MsaFmhaParams* params, const int32_t* splits
  * without MSA_FLAG_SPARSE), block_m 16 / 64 / 128; up to 128 packed rows per work item.  Longer queries and scores: unpack
  * the pages with msa_kv4_read and run on the copy.  num_logical_pages is the length of kv_indices; entries past it and pages
  * outside [0, kv_extent) are clamped.  17 to 128 rows of dense items run on the tensor-core kernel, whose waits report to
- * `status`. */
+ * `status`.  msa_fmha_fwd_split_static does not take it. */
 
 /* Per-head RMS norm of q and k, rotary positions, and the write of k and v into a paged cache, in one pass over a step's
  * tokens.  Any of q, k, v may be NULL (k needs k_out or k_cache; v needs v_cache).  q, k, v and the outputs are bf16 unless a
@@ -275,7 +275,7 @@ int msa_fmha_fwd_split_static(const MsaFmhaParams* params, const int32_t* splits
  *    by positions[axis[n]][token] * turns[n] for pair n; turns[n] = the frequency in turns per position, as a
  *    64-bit fraction (modulo 1).
  *  - cache: row of token t at slot_map[t] = page * page_size + offset; a negative slot, or one past num_pages, writes
- *    nothing.  Slots of one call are distinct.  Keys are rounded to bf16, then divided by k_scale * k_scale_head[head]
+ *    nothing.  Slots of one call are distinct.  Keys are computed in 64 bits and rounded to bf16, then divided by k_scale * k_scale_head[head]
  *    and rounded to the cache's type (bf16 caches: as they are); values likewise.
  * No upstream counterpart (upstream starts at the attention call). */
 typedef struct MsaNormRopeArgs {

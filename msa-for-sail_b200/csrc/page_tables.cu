@@ -10,8 +10,8 @@
 // binary search of the scans and is computed on its own: neither one very long request nor many short ones leave
 // threads without work.  Pages are handed out in the order of the requests, whatever the order of the threads.
 //
-// Bound by launches and by dependent reads (lengths, scans, the table, the slots): 8 requests 4.0 us in one launch, 2 048 requests of up to
-// 32 768 keys with 263 113 pages 12 us in two; their bytes would take 0.1.
+// Bound by launches and by dependent reads (lengths, scans, the table, the slots): 8 requests 4.2 us in one launch, 2 048 requests of up to
+// 32 768 keys with 263 113 pages 13 us in two; their bytes would take 0.1.
 #include <algorithm>
 
 #include "common.cuh"

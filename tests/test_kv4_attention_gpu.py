@@ -555,6 +555,53 @@ def test_first_call_of_a_process_inside_a_capture(monkeypatch):
     ref.check_attention(out, None, b.want(), P_F16, "captured")
 
 
+def test_checked_inputs_and_the_line_of_a_call(monkeypatch, capfd):
+    import msa_for_sail as msa
+    from msa_for_sail import api
+    monkeypatch.setattr(api, "_SHOW_PARAMS", True)
+    b = Batch(68, [1, 2], [300, 700], 16, 2)
+    q, k, v, table = b.cuda()
+    out, _ = msa.fmha_sail(q, k, v, b.plan(), kv_indices=table, check_input_valid=True)
+    ref.check_attention(out, None, b.want(), P_F16, "checked")
+    assert "[MSA] --format=" in capfd.readouterr().out
+    bad = table.clone()
+    bad[1] = 10 ** 6
+    with pytest.raises(AssertionError, match="outside"):
+        msa.fmha_sail(q, k, v, b.plan(), kv_indices=bad, check_input_valid=True)
+    blocks = b.blocks(3)
+    out, _ = msa.fmha_sail(q, k, v, b.plan(kv_block_num=3), kv_indices=table, kv_block_indexes=blocks.to(DEV), check_input_valid=True)
+    ref.check_attention(out, None, b.want(blocks=blocks), P_F16, "checked selection")
+
+
+@pytest.mark.parametrize("hq,hk", [(256, 1), (130, 1), (144, 1)])
+def test_more_than_128_heads_to_a_kv_head(hq, hk):
+    """A dense plan has no items for a token of so many heads, whatever the cache; where pages are selected they are groups of 16 rows."""
+    import msa_for_sail as msa
+    b = Batch(69, [1, 1], [300, 200], hq, hk)
+    q, k, v, table = b.cuda()
+    with pytest.raises(RuntimeError, match="bad argument"):
+        b.plan()
+    blocks = b.blocks(2)
+    out, _ = msa.fmha_sail(q, k, v, b.plan(kv_block_num=2), kv_indices=table, kv_block_indexes=blocks.to(DEV))
+    ref.check_attention(out, None, b.want(blocks=blocks), P_F16, f"{hq} heads, selected")
+
+
+def test_strides_the_kernels_read():
+    """Queries inside a wider buffer, a selection whose rows are apart, a cache whose pages hold more than keys and values."""
+    import msa_for_sail as msa
+    for n, hq in ((1, 16), (2, 32)):
+        b = Batch(70, [n] * 3, [300, 129, 700], hq, 2)
+        q, k, v, table = b.cuda()
+        wide = torch.full((b.T, hq + 5, 128), torch.nan, dtype=torch.bfloat16, device=DEV)
+        wide[:, 2:2 + hq] = q
+        big = torch.full((k.shape[0], 5, 128, 72), 0x7F, dtype=torch.uint8, device=DEV)
+        big[:, 1:3], big[:, 3:5] = k, v
+        out = torch.full((b.T, hq + 3, 128), 7.0, dtype=torch.bfloat16, device=DEV)
+        msa.fmha_sail(wide[:, 2:2 + hq], big[:, 1:3], big[:, 3:5], b.plan(), kv_indices=table, out=out[:, 1:1 + hq])
+        ref.check_attention(out[:, 1:1 + hq], None, b.want(), P_F16, f"{n} tokens")
+        assert (out[:, 0] == 7).all() and (out[:, 1 + hq:] == 7).all()
+
+
 def test_refusals_of_tables_and_offsets():
     import msa_for_sail as msa
     b = Batch(67, [1, 1], [300, 200], 16, 2)
