@@ -27,7 +27,8 @@
 // Measured: one sequence of 1 048 576 keys, 64 / 8 heads: 219 us and 5 for the merge, 5.5 TB/s of codes and scales.  The copies alone take 186 us,
 // the conversions and products alone 213: the issue slots (55 % used, a conversion is an instruction of two clocks on the ALU
 // pipe) bound it, together with what the two leave one another.  24 ragged sequences, 64 / 4 heads (NT = 2): 56 us, 3.4 TB/s; a page
-// takes an SM 1 300 clocks, 830 would be the memory's.  32 x 16 selected pages of 1 024, 64 / 8 heads: 22 us, 3.4 TB/s; index
+// takes an SM 1 300 clocks, 830 would be the memory's (its two steps of 16 keys one after the other, which spares registers: 62 us with
+// three CTAs an SM, 67 with four).  32 x 16 selected pages of 1 024, 64 / 8 heads: 22 us, 3.4 TB/s; index
 // loads, first page and epilogue of one wave of CTAs.
 #include <algorithm>
 
@@ -144,6 +145,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<NT>::CTAS) kv4_decode_kernel(con
     it.last = min(p.kv_block_num, it.first + per);
     it.blocks = p.kv_block_indexes + t * p.kbi_stride_tok + it.kvh * p.kbi_stride_head;
     if (it.first + lane < it.last) first_blocks = it.blocks[it.first + lane];
+    if (t >= p.qo_start[p.batch]) return;                    // a padded row, behind the last sequence: left as it was
     it.b = chk(p.token_batch[t], 0, p.batch, p.status);
     it.head0 = it.kvh * h_r; it.pack = h_r;
     it.tok0 = t - p.qo_start[it.b];

@@ -302,6 +302,32 @@ def test_planned_and_run_in_a_graph(sparse):
         ref.check_attention(out, lse, n.want(blocks=blocks) if sparse else n.want(), P_F16, f"replay {seed}")
 
 
+@pytest.mark.parametrize("sparse", [False, True])
+@pytest.mark.parametrize("splits", [1, 2])
+@pytest.mark.parametrize("n", [1, 3])
+def test_rows_behind_the_last_sequence(sparse, splits, n):
+    """A padded batch of a graph-safe plan: the rows behind the last sequence stay as they were, or become empty rows in the merge of splits."""
+    import msa_for_sail as msa
+    qo, pad = [n, 1, 0], 4
+    b = Batch(72, qo, [500, 130, 0], 16, 2)
+    q, k, v, table = b.cuda()
+    T = b.T + pad
+    q = torch.cat([q, torch.ones(pad, 16, 128, dtype=torch.bfloat16, device=DEV)])
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)
+    blocks = torch.cat([b.blocks(3), torch.zeros(pad, 2, 3, dtype=torch.int32)])
+    ws = msa.allocate_graph_workspace(3, 16, num_kv_heads=2, page_size=128, num_kv_splits=2, kv_block_num=3 if sparse else -1, max_qo_len=n + 2)
+    plan = msa.fmha_sail_plan(i32(qo), i32(b.kv), 16, num_kv_heads=2, page_size=128, kv_block_num=3 if sparse else -1, num_kv_splits=splits,
+                              graph_safe=True, max_total_q=T, max_qo_len_override=n, qo_len_uniform_override=False, max_kv_len_override=600,
+                              qo_offset=i32([-1] * 3), given_workspace=ws, use_kv4_cache=True)
+    out, lse = torch.full((T, 16, 128), 7.0, dtype=torch.bfloat16, device=DEV), torch.full((T, 16), 7.0, device=DEV)
+    msa.fmha_sail(q, k, v, plan, kv_indices=table, out=out, lse=lse, **(dict(kv_block_indexes=blocks.to(DEV)) if sparse else {}))
+    ref.check_attention(out[:b.T], lse[:b.T], b.want(**(dict(blocks=blocks[:b.T]) if sparse else {})), P_F16, "real rows")
+    if plan[3]["num_kv_splits"] == 1:
+        assert (out[b.T:] == 7).all() and (lse[b.T:] == 7).all()
+    else:
+        assert (out[b.T:] == 0).all() and torch.isinf(lse[b.T:]).all()
+
+
 def test_two_streams_share_a_plan():
     """The partials of a call are its own: one plan may run on two streams at the same time."""
     import msa_for_sail as msa
