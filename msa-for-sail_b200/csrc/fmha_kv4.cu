@@ -26,7 +26,7 @@
 //
 // Measured: one sequence of 1 048 576 keys, 64 / 8 heads: 219 us and 5 for the merge, 5.5 TB/s of codes and scales.  The copies alone take 186 us,
 // the conversions and products alone 213: the issue slots (55 % used, a conversion is an instruction of two clocks on the ALU
-// pipe) bound it, together with what the two leave one another.  24 ragged sequences, 64 / 4 heads (NT = 2): 56 us, 3.4 TB/s; a page
+// pipe) bound it, together with what the two leave one another.  (Under the 1 000 W cap, after some hundreds of passes, 260 at 1.68 GHz.)  24 ragged sequences, 64 / 4 heads (NT = 2): 56 us, 3.4 TB/s; a page
 // takes an SM 1 300 clocks, 830 would be the memory's (its two steps of 16 keys one after the other, which spares registers: 62 us with
 // three CTAs an SM, 67 with four).  32 x 16 selected pages of 1 024, 64 / 8 heads: 22 us, 3.4 TB/s; index
 // loads, first page and epilogue of one wave of CTAs.
