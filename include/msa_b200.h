@@ -153,8 +153,8 @@ int msa_lse_merge_ex(const void* partial_o, int32_t partial_dtype, const float* 
                      int64_t out_stride_tok, int64_t out_stride_head,
                      float out_scale, msa_stream_t stream);
 
-/* The merge of dense fp32 partials [S, total_q, H, 128] with a CTA for each row, for many splits of few rows: the time of
- * msa_lse_merge grows with the number of splits, this one's hardly does.  Sums are taken in another (fixed) order. */
+/* The merge of dense fp32 partials [S, total_q, H, 128] with a warp for each row, or a CTA where there are many splits of few
+ * rows: 0.2 to 0.7 of the time of msa_lse_merge.  Sums are taken in another (fixed) order. */
 int msa_lse_merge_many(const float* partial_o, const float* partial_lse, const int32_t* splits_per_row, void* out,
                        int32_t out_dtype, float* lse_out, int32_t num_splits, int32_t total_q, int32_t num_heads,
                        int64_t out_stride_tok, int64_t out_stride_head, float out_scale, msa_stream_t stream);

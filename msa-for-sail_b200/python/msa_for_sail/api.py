@@ -1134,17 +1134,9 @@ def _fmha_sail_kv4(q, k, v, plan, kv_indices, kv_block_indexes, q_offset_overrid
             p.out, p.out_stride_tok, p.out_stride_head = kernel_out.data_ptr(), kernel_out.stride(0), kernel_out.stride(1)
         _lib.check(_lib.lib.msa_fmha_fwd(ctypes.byref(p), stream), "msa_fmha_fwd")
         if splits > 1:
-            # a CTA or half a warp per row: 64 rows x 72 splits 3.8 and 11.4 us, 512 x 8 2.9 and 3.0, 1 536 x 16 5.0 and 4.2, x 37
-            # 6.8 and 8.1, 8 192 x 8 15.0 and 6.4
-            spr, rows_out = _ptr(plan["num_kv_splits_per_row"]), nnz_qo * num_qo_heads
-            if rows_out <= max(512, 48 * splits):
-                _lib.check(_lib.lib.msa_lse_merge_many(
-                    p.partial_o, p.partial_lse, spr, out.data_ptr(), _dt_code(out.dtype), _ptr(lse), splits, nnz_qo, num_qo_heads,
-                    out.stride(0), out.stride(1), out_scale, stream), "msa_lse_merge_many")
-            else:
-                _lib.check(_lib.lib.msa_lse_merge_ex(
-                    p.partial_o, MSA_DT_F32, p.partial_lse, spr, out.data_ptr(), _dt_code(out.dtype), _ptr(lse), splits, nnz_qo,
-                    num_qo_heads, 0, 0, out.stride(0), out.stride(1), out_scale, stream), "msa_lse_merge_ex")
+            _lib.check(_lib.lib.msa_lse_merge_many(
+                p.partial_o, p.partial_lse, _ptr(plan["num_kv_splits_per_row"]), out.data_ptr(), _dt_code(out.dtype), _ptr(lse),
+                splits, nnz_qo, num_qo_heads, out.stride(0), out.stride(1), out_scale, stream), "msa_lse_merge_many")
         elif kernel_out is not out:
             out.copy_(kernel_out)
     return out, None

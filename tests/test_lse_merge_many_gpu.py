@@ -57,6 +57,25 @@ def test_against_64_bits(S, out_dtype):
         assert ((got - wl).abs()[ok] <= 2.0 ** -17 + 2.0 ** -22 * wl.abs()[ok]).all()
 
 
+@pytest.mark.parametrize("S,T,H", [(1, 1100, 1), (3, 300, 7), (17, 600, 2), (33, 1025, 1), (100, 20, 64)])
+def test_many_rows(S, T, H):
+    g = torch.Generator("cuda").manual_seed(S)
+    po, pl = torch.randn(S, T, H, 128, device="cuda", generator=g), 3 * torch.randn(S, T, H, device="cuda", generator=g)
+    empty = torch.rand(S, T, H, device="cuda", generator=g) < 0.3
+    pl[empty], po[empty] = -torch.inf, torch.nan
+    pl[:, 1] = -torch.inf
+    spr = torch.randint(1, S + 1, (T,), device="cuda", generator=g, dtype=torch.int32)
+    spr[3] = 0                                                  # a padded row
+    for limit in (None, spr):
+        out, lse = _run(po, pl, limit)
+        want, spread, wl = _want(po, pl, limit, 1.0)
+        tol = 2.0 ** -24 * want.abs() + (2 * (30 * 2.0 ** -23 + 2.0 ** -21) + (S + 8) * 2.0 ** -24) * spread + 1e-30
+        assert ((out.double() - want).abs() <= tol).all()
+        ok = ~torch.isinf(wl)
+        assert torch.equal(torch.isinf(lse), ~ok) and (out[1] == 0).all()
+        assert ((lse.double() - wl).abs()[ok] <= 2.0 ** -17 + 2.0 ** -22 * wl.abs()[ok]).all()
+
+
 def test_not_a_number_and_large_differences():
     po = torch.ones(40, 1, 3, 128, device="cuda")
     pl = torch.zeros(40, 1, 3, device="cuda")
@@ -66,6 +85,8 @@ def test_not_a_number_and_large_differences():
     out, lse = _run(po, pl)
     assert (out[0, 0] == 1).all() and torch.isnan(out[0, 1]).all() and torch.isnan(lse[0, 1]) and (out[0, 2] == 5).all()
     assert float(lse[0, 2]) == pytest.approx(1e30)
+    out, lse = _run(po[5:15].contiguous(), pl[5:15].contiguous())    # few splits: the other kernel
+    assert (out[0, 0] == 1).all() and torch.isnan(out[0, 1]).all() and torch.isnan(lse[0, 1]) and (out[0, 2] == 5).all()
 
 
 def test_runs_are_repeatable_and_lse_is_optional():
