@@ -7,7 +7,8 @@
 //                F times in the tile, and copy f has keys 128 / F * f .. of every page, with a maximum and a sum of its own and zeros in
 //                P elsewhere: all four warps work on a page (32 sequences x 4 tokens x 16 heads: 94 us with half of the threads idle).
 //                The F states of a row are joined at the end
-//   warp 4       issues S[j & 1] = Q K_j^T (tcgen05, f16 operands, Q and accumulators in TMEM: 75.0 us with Q in shared memory)
+//   warp 4       issues S[j & 1] = Q K_j^T (tcgen05, f16 operands, Q and accumulators in TMEM; Q in shared memory costs 1.4 us more
+//                of 32 sequences x 4 tokens x 64 heads)
 //   warp 5       issues O += P_j V_j (P from TMEM).  (One warp for both took 2 150 clocks a page: 1 350 to issue, which is what
 //                the tensor pipe takes, and 250 for each of three waits, ready or not.)
 //   warps 8-23   conversion, eight warps for K and eight for V: warp w has keys 16 w .. 16 w + 15 of every page.  16-byte copies bring
@@ -22,7 +23,7 @@
 //
 // A page costs 64 KB written to shared memory and as much read by the MMAs, about 1 000 clocks of its bandwidth, 500 clocks of conversions
 // per scheduler, and with 128 rows 1 000 clocks of exponentials; its 18 KB from memory are 810.  Measured: 32 sequences of 131 to
-// 16 384 keys x 4 tokens, 64 / 4 heads, 64 rows to a head: 67 us and 7 for the merge, 2 100 clocks a page (149 us in groups of 16 rows on
+// 16 384 keys x 4 tokens, 64 / 4 heads, 64 rows to a head: 67 us and 4 for the merge, 2 100 clocks a page (149 us in groups of 16 rows on
 // fmha_kv4.cu, which convert every page four times); with 128 rows 2 600, with 32 rows 1 900.  From 64 rows on the softmax
 // warpgroup bounds it, which is never without work: 550 clocks to read S, take the maximum and vote, 1 100 for exponentials and P; below that the
 // converting warps: 600 clocks to read codes and order more, 400 for a free tile, 650 to convert and fence.  Two softmax warpgroups that take
