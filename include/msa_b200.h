@@ -111,6 +111,8 @@ typedef struct MsaFmhaParams {
   int32_t flags;           /* MSA_FLAG_*                                                     */
   float   sm_scale;        /* q_scale * k_scale * softmax scale                              */
   float   out_scale;       /* v_scale * o_scale                                              */
+  int32_t num_page_entries; /* length of kv_indices: places past its end read as its last entry; 0 = not given,
+                              every place that the lengths reach is read (kv_dtype = MSA_DT_KV4: num_logical_pages) */
 } MsaFmhaParams;
 
 /* FMHA forward: dense ragged / dense paged / sparse, optional split-KV partials.
@@ -320,7 +322,9 @@ int msa_kv4_read(const MsaKv4ReadArgs* args, msa_stream_t stream);
  * block_table row come from the top of the stack free_pages[0, num_free) in the order of the requests, and are written into
  * the row; num_held_out / num_free_out (may be num_held / num_free) receive the new counts.  num_missing: pages and tokens
  * that found no place (an empty stack, a row of the table or an output that is too short).  Such a page is 0 in
- * kv_indices (attention over it stays in bounds but means nothing), -1 in block_table, and its tokens have slot -1. */
+ * kv_indices (attention over it stays in bounds but means nothing), -1 in block_table, and its tokens have slot -1.
+ * kv_page_indptr counts the pages that a kv_indices of max_total_pages has no place for as well: give the attention call
+ * num_page_entries = max_total_pages, and they read as its last entry. */
 typedef struct MsaPageTablesArgs {
   const int32_t* qo_len;           /* [B] device: new tokens */
   const int32_t* kv_len;           /* [B] device: keys with them */

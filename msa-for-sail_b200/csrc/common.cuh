@@ -31,6 +31,16 @@ __device__ __forceinline__ int chk(int v, int lo, int hi, int32_t* status) {
 __device__ __forceinline__ int chk(int v, int, int, int32_t*) { return v; }
 #endif
 
+// Entry `at` of the flat page table.  Lengths that live on the device may outgrow the table: the places behind its end are its last
+// entry, and nothing behind it is read.  (num_page_entries = 0: the caller did not say how long it is.)
+__device__ __forceinline__ int page_entry(const MsaFmhaParams& p, int at) {
+#ifdef MSA_BOUNDS_CHECK
+  if (p.num_page_entries > 0) at = chk(at, 0, p.num_page_entries, p.status);
+#endif
+  const unsigned place = min(static_cast<unsigned>(at), static_cast<unsigned>(p.num_page_entries) - 1u);
+  return chk(p.kv_indices[place], 0, static_cast<int>(p.kv_extent), p.status);
+}
+
 // ---- kernels of one stream without a gap between them ----
 // A kernel launched with launch_chained() may start while the kernel before it in the stream still runs: once every CTA of
 // that one has called chain_begin() or ended.  chain_begin() comes before anything that touches global memory: it waits

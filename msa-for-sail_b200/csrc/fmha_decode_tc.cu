@@ -224,7 +224,7 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
         }
         const int pos = n + incl - nu;
         if (nu > 0 && pos + nu <= MAX_SPARSE_TILES * UPP) {
-          const int ph = chk(p.kv_indices[page_base + blk], 0, static_cast<int>(p.kv_extent), p.status);
+          const int ph = page_entry(p, page_base + blk);
           for (int u = 0; u < nu; ++u) { s_tiles[pos + u] = blk * UPP + u; s_phys[pos + u] = ph; }
         }
         n += __shfl_sync(0xffffffffu, incl, 31);
@@ -275,8 +275,8 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
     int phys_cur = 0, phys_next = 0;
     const int n_pages = (n_tiles + UPP - 1) / UPP;
     if (!sparse) {
-      phys_cur = lane < n_pages ? chk(p.kv_indices[page_base + tb + lane], 0, static_cast<int>(p.kv_extent), p.status) : 0;
-      phys_next = 32 + lane < n_pages ? chk(p.kv_indices[page_base + tb + 32 + lane], 0, static_cast<int>(p.kv_extent), p.status) : 0;
+      phys_cur = lane < n_pages ? page_entry(p, page_base + tb + lane) : 0;
+      phys_next = 32 + lane < n_pages ? page_entry(p, page_base + tb + 32 + lane) : 0;
     }
     uint32_t fix_phase = 0;
     bool alive = do_k || do_v;
@@ -287,7 +287,7 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
       const int pg = j / UPP;                                // dense: page index within this item
       if (!sparse && j > 0 && (j % (32 * UPP)) == 0) {
         phys_cur = phys_next;
-        phys_next = pg + 32 + lane < n_pages ? chk(p.kv_indices[page_base + tb + pg + 32 + lane], 0, static_cast<int>(p.kv_extent), p.status) : 0;
+        phys_next = pg + 32 + lane < n_pages ? page_entry(p, page_base + tb + pg + 32 + lane) : 0;
       }
       const int phys = sparse ? s_phys[j] : __shfl_sync(0xffffffffu, phys_cur, pg & 31);
       const int valid_rows = min(TK, kv_len - key0);

@@ -156,7 +156,7 @@ fmha_mma_kernel(const __grid_constant__ MsaFmhaParams p) {
         if (ps > 0) {
           const int lp = sparse ? s.lpage : pos / ps;
           const int in_page = sparse ? r : pos - lp * ps;
-          const int64_t pg = chk(p.kv_indices[page_base + lp], 0, static_cast<int>(p.kv_extent), p.status);
+          const int64_t pg = page_entry(p, page_base + lp);
           ko = pg * p.k_stride_page + static_cast<int64_t>(kvh) * p.k_stride_head + static_cast<int64_t>(in_page) * p.k_stride_tok;
           vo = pg * p.v_stride_page + static_cast<int64_t>(kvh) * p.v_stride_head + static_cast<int64_t>(in_page) * p.v_stride_tok;
         } else {

@@ -457,7 +457,7 @@ sparse_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
   const int kvh = item.x / NP, gp = item.x % NP;
   const int b = chk(p.page_batch[gp], 0, p.batch, p.status);
   const int lpage = gp - p.kv_page_indptr[b];
-  const int phys = chk(p.kv_indices[gp], 0, static_cast<int>(p.kv_extent), p.status);
+  const int phys = page_entry(p, gp);
   const int G = p.num_qo_heads / p.num_kv_heads;
   const int tpc = BM / G;                                  // tokens per chunk
   const int n_ent = item.z - item.y;

@@ -227,8 +227,8 @@ fmha_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant__ 
           const int ks = tile % KSTAGES, tiles = min(2, n_total - j);
           int page[2] = {0, 0};
           if (paged) {
-            page[0] = chk(p.kv_indices[page_base + j], 0, static_cast<int>(p.kv_extent), p.status);
-            if (tiles == 2) page[1] = chk(p.kv_indices[page_base + j + 1], 0, static_cast<int>(p.kv_extent), p.status);
+            page[0] = page_entry(p, page_base + j);
+            if (tiles == 2) page[1] = page_entry(p, page_base + j + 1);
           }
           alive = mbar_wait_warp(bar(K_EMPTY + ks), ((tile / KSTAGES) & 1) ^ 1, abort_flag, spin_limit);
           if (!alive) break;
@@ -252,7 +252,7 @@ fmha_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant__ 
           if (j == stall_tile) { alive = false; break; }    // test hook: whoever waits for this tile runs out of polls
           if (j == max(0, n_total - NEXT_LEAD) && lane == 0) mbar_arrive(bar(NEXT_REQ));
           const int ks = tile % KSTAGES, vs = tile % VSTAGES;
-          const int page = paged ? chk(p.kv_indices[page_base + j], 0, static_cast<int>(p.kv_extent), p.status) : 0;
+          const int page = paged ? page_entry(p, page_base + j) : 0;
           const int valid_rows = min(BN, kv_len - j * BN);
           const bool fix = valid_rows < BN;                 // tail tile: rows past kv_len must read as 0 in V
           if (lane == 0) trace(3, j, 0);

@@ -157,7 +157,7 @@ score_stream_kernel(const __grid_constant__ MsaFmhaParams p) {
         l_tile = w.kv_tile_begin + (idx - s_pref[a]);
         const int b = chk(w.batch, 0, p.batch, p.status);
         const int kvh = chk(w.head0, 0, p.num_qo_heads, p.status) / h_r;
-        const int phys = chk(p.kv_indices[p.kv_page_indptr[b] + l_tile], 0, static_cast<int>(p.kv_extent), p.status);
+        const int phys = page_entry(p, p.kv_page_indptr[b] + l_tile);
         l_src += (static_cast<int64_t>(kvh) * p.k_stride_head + static_cast<int64_t>(phys) * p.k_stride_page) * e;
       }
       const uint64_t l_addr = reinterpret_cast<uint64_t>(l_src);

@@ -883,7 +883,7 @@ def _fmha_sail(
             p.v_stride_page, p.v_stride_head, p.v_stride_tok = v.stride(0), v.stride(1), v.stride(2)
         assert k.stride(3) == 1 and v.stride(3) == 1, "paged K/V head_dim must be contiguous"
         assert kv_indices.dtype == torch.int32 and kv_indices.is_cuda
-        p.kv_indices = kv_indices.data_ptr()
+        p.kv_indices, p.num_page_entries = kv_indices.data_ptr(), kv_indices.numel()
         p.kv_page_indptr = plan["kv_page_indptr"].data_ptr()
         p.page_size = page_size
     else:

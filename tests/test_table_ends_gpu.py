@@ -1,0 +1,105 @@
+"""Page tables that end before the lengths do (lengths on the device may outgrow a table of fixed size): the places behind the end are the
+last page, in every kernel and on every cache.  A short table gives what a full one gives whose last places are that page, bit for bit."""
+import pytest
+import torch
+
+import serving_ref as ref
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+KEYS, PAGES, KEPT = 600, 5, 2
+
+
+def _i32(x):
+    return torch.tensor(x, dtype=torch.int32, device=DEV)
+
+
+def _cache(kind, g, P, hk, page):
+    if kind == "kv4":
+        return [ref.random_kv4(g, P, hk).to(DEV) for _ in range(2)]
+    x = [torch.randn(P, hk, page, 128, generator=g).to(DEV) for _ in range(2)]
+    return [t.to(torch.bfloat16 if kind == "bf16" else torch.float8_e4m3fn) for t in x]
+
+
+def _plan(rows, hq, hk, page=128, kbn=-1, scores=False, splits=1, keys=KEYS, **kw):
+    import msa_for_sail as msa
+    ws = msa.allocate_graph_workspace(1, hq, num_kv_heads=hk, page_size=page, num_kv_splits=splits, kv_block_num=kbn, max_qo_len=rows)
+    return msa.fmha_sail_plan(_i32([rows]), _i32([keys]), hq, num_kv_heads=hk, page_size=page, kv_block_num=kbn, num_kv_splits=splits, graph_safe=True,
+                              output_maxscore=scores, max_total_q=rows, max_qo_len_override=rows, qo_len_uniform_override=True, max_kv_len_override=700,
+                              qo_offset=_i32([keys - rows]), given_workspace=ws, **kw)
+
+
+# rows, query heads, page, selected pages, scores, splits
+CASES = {"decode": (1, 16, 128, -1, False, 2), "decode of 4 tokens": (4, 16, 128, -1, False, 1), "prompt": (200, 4, 128, -1, False, 1),
+         "prompt in splits": (60, 4, 128, -1, False, 2), "pages of 64": (3, 16, 64, -1, False, 1), "scores of one row": (1, 2, 128, -1, True, 1),
+         "scores of a prompt": (200, 4, 128, -1, True, 1), "scores of many rows": (8, 16, 128, -1, True, 1), "selected": (3, 16, 128, 3, False, 2)}
+
+
+@pytest.mark.parametrize("kind", ["bf16", "e4m3", "kv4"])
+@pytest.mark.parametrize("case", list(CASES))
+def test_a_short_table_reads_as_its_last_page(kind, case):
+    import msa_for_sail as msa
+    from msa_for_sail import api
+    rows, hq, page, kbn, scores, splits = CASES[case]
+    if kind == "kv4" and page != 128:
+        pytest.skip("pages of a 4-bit cache have 128 tokens")
+    hk = 2
+    g = torch.Generator().manual_seed(11)
+    pages = -(-KEYS // page)
+    k, v = _cache(kind, g, pages + 3, hk, page)
+    q = torch.randn(rows, hq, 128, generator=g).to(torch.bfloat16).to(DEV)
+    table = torch.randperm(pages + 3, generator=g)[:pages].to(torch.int32).to(DEV)
+    if kind == "e4m3" and rows > 128:
+        q = q.to(torch.float8_e4m3fn)
+    sel = dict(kv_block_indexes=_i32([0, 2, pages - 1]).expand(rows, hk, 3).contiguous()) if kbn > 0 else {}
+    plan = _plan(rows, hq, hk, page, kbn, scores, splits, use_kv4_cache=kind == "kv4")
+    full = table.clone()
+    full[KEPT:] = table[KEPT - 1]
+    kw = dict(output_o=False) if scores else {}
+    run = lambda t: [x.clone() for x in msa.fmha_sail(q, k, v, plan, kv_indices=t, **kw, **sel) if x is not None]
+    got = run(table[:KEPT].clone())
+    api.last_status()                                           # (the build with bounds checks reports the places past the end)
+    want = run(full)
+    other = run(table)
+    assert len(got) == len(want) == 1
+    assert torch.equal(got[0], want[0]) and not torch.equal(want[0], other[0])
+
+
+def test_a_short_table_of_a_plan_with_pages_first():
+    """Sparse prefill page by page: a host-made plan, whose table is as long as its pages, or shorter where nobody selects the rest."""
+    import msa_for_sail as msa
+    g = torch.Generator().manual_seed(12)
+    k, v = _cache("bf16", g, 9, 2, 128)
+    q = torch.randn(300, 8, 128, generator=g).to(torch.bfloat16).to(DEV)
+    plan = msa.fmha_sail_plan(torch.tensor([300]), torch.tensor([900]), 8, num_kv_heads=2, page_size=128, kv_block_num=4)
+    assert plan[3]["sparse_tc_preferred"]
+    table = _i32([3, 7, 1, 0, 8, 2, 4, 6])
+    blocks = _i32([0, 1, 2, -1]).expand(300, 2, 4).contiguous()
+    want = msa.fmha_sail(q, k, v, plan, kv_indices=table, kv_block_indexes=blocks)[0]
+    assert torch.equal(msa.fmha_sail(q, k, v, plan, kv_indices=table[:3].clone(), kv_block_indexes=blocks)[0], want)
+    last = _i32([3, 7, 7, 7, 7, 7, 7, 7])
+    want = msa.fmha_sail(q, k, v, plan, kv_indices=last, kv_block_indexes=blocks)[0]
+    assert torch.equal(msa.fmha_sail(q, k, v, plan, kv_indices=table[:2].clone(), kv_block_indexes=blocks)[0], want)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "e4m3", "kv4"])
+def test_tables_with_too_few_places_and_attention(kind):
+    """paged_kv_tables counts the pages that its flat table has no place for; attention over such a table stays in the cache."""
+    import msa_for_sail as msa
+    g = torch.Generator().manual_seed(13)
+    k, v = _cache(kind, g, 12, 2, 128)
+    ql, kl = _i32([1, 200]), _i32([300, 700])
+    block_table = torch.randperm(12, generator=g).view(2, 6).to(torch.int32).to(DEV)
+    q = torch.randn(201, 8, 128, generator=g).to(torch.bfloat16).to(DEV)
+
+    def run(places):
+        tabs = msa.paged_kv_tables(ql, kl, block_table, max_total_q=201, max_total_pages=places)
+        ws = msa.allocate_graph_workspace(2, 8, num_kv_heads=2, page_size=128, max_qo_len=200)
+        plan = msa.fmha_sail_plan(ql, kl, 8, num_kv_heads=2, page_size=128, num_kv_splits=1, graph_safe=True, max_total_q=201, max_qo_len_override=200,
+                                  qo_len_uniform_override=False, max_kv_len_override=700, qo_offset=_i32([-1, -1]), given_workspace=ws,
+                                  use_kv4_cache=kind == "kv4")
+        return msa.fmha_sail(q, k, v, plan, kv_indices=tabs["kv_indices"])[0].clone(), int(tabs["num_missing"])
+    want, none = run(9)
+    got, missing = run(4)
+    assert none == 0 and missing == 5
+    assert torch.equal(got[0], want[0]) and torch.isfinite(got.float()).all()
