@@ -1044,6 +1044,11 @@ def _fmha_sail_kv4(q, k, v, plan, kv_indices, kv_block_indexes, q_offset_overrid
             raise ValueError(f"plan allows at most {plan['total_qo_len']} query tokens, q has {nnz_qo}")
     elif plan["total_qo_len"] != nnz_qo:
         raise ValueError(f"plan was made for {plan['total_qo_len']} query tokens, q has {nnz_qo}")
+    pages = plan.get("_kv4_pages")
+    if pages is None:
+        pages = plan["_kv4_pages"] = sum(-(-n // cache.KV4_TILE) for n in plan["_host"]["kv_lens"]) if plan["_host"] is not None else 0
+    if kv_indices.shape[0] < pages and nnz_qo:
+        raise ValueError(f"kv_indices must have the {pages} pages of the plan's sequences, got {kv_indices.shape[0]}")
     if not native:
         with cache._on(dev):
             table = torch.arange(kv_indices.shape[0], dtype=torch.int32, device=dev)
@@ -1093,13 +1098,10 @@ def _fmha_sail_kv4(q, k, v, plan, kv_indices, kv_block_indexes, q_offset_overrid
     q_stride, out_scale = q.stride(), float(v_s * o_s)
     base = plan.get("_kv4_params")            # the sizes that are the same in every call with this plan
     if base is None:
-        plan["_kv4_pages"] = sum(-(-n // cache.KV4_TILE) for n in plan["_host"]["kv_lens"]) if plan["_host"] is not None else 0
         base = plan["_kv4_params"] = bytes(_lib.MsaFmhaParams(
             num_work=plan["num_work"], decode_rows=0 if sparse else rows, num_qo_heads=num_qo_heads, num_kv_heads=num_kv_heads,
             batch=plan["batch_size"], block_m=plan["qo_tile_size"], pack=plan["pack_factor"], page_size=cache.KV4_TILE, num_splits=splits,
             kv_dtype=MSA_DT_KV4, flags=FLAG_OUT_O | FLAG_SPARSE if sparse else FLAG_OUT_O))
-    if kv_indices.shape[0] < plan["_kv4_pages"]:
-        raise ValueError(f"kv_indices must have the {plan['_kv4_pages']} pages of the plan's sequences, got {kv_indices.shape[0]}")
     p = _lib.MsaFmhaParams.from_buffer_copy(base)
     p.qo_start, p.kv_len, p.qo_offset = plan["qo_segment_offsets"].data_ptr(), plan["kv_segment_lens"].data_ptr(), qo_offset.data_ptr()
     p.kv_page_indptr, p.num_logical_pages, p.status = plan["kv_page_indptr"].data_ptr(), kv_indices.shape[0], _status_ptr(dev)

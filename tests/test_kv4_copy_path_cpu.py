@@ -1,0 +1,60 @@
+"""Arguments of attention over a 4-bit cache where it runs on bf16 copies (longer queries, page scores, pages that many tokens share): what is
+refused, is refused before a page is copied.  CPU tensors stand in for those of a GPU; nothing is launched."""
+import contextlib
+
+import pytest
+import torch
+
+
+class Copied(Exception):
+    """The call came as far as copying pages."""
+
+
+@pytest.fixture
+def api(monkeypatch):
+    from msa_for_sail import api, cache
+
+    def copied(*a, **kw):
+        raise Copied
+    monkeypatch.setattr(api, "_num_sms", lambda dev: 148)
+    monkeypatch.setattr(cache, "_same_device", lambda *a, **kw: None)
+    monkeypatch.setattr(cache, "_on", lambda dev: contextlib.nullcontext())
+    monkeypatch.setattr(cache, "unpack_pages", copied)
+    return api
+
+
+# query tokens, keys, options of the plan, what the call adds
+PATHS = {"prompt": ([200, 1], [300, 200], {}, {}), "scores": ([1, 1], [300, 200], dict(output_maxscore=True), dict(output_o=False)),
+         "shared pages": ([300], [600], dict(kv_block_num=2), {}), "prompt of 9 tokens": ([9], [600], {}, {})}
+
+
+def _call(api, path, table=None, **kw):
+    qo, kv, opts, extra = PATHS[path]
+    hq, hk = (64, 4) if path == "prompt of 9 tokens" else (16, 2)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32)
+    plan = api._fmha_sail_plan(i32(qo), i32(kv), hq, hk, page_size=128, device="cpu", use_kv4_cache=True, **opts)
+    q = torch.zeros(sum(qo), hq, 128, dtype=torch.bfloat16)
+    k, v = (torch.zeros(9, hk, 128, 72, dtype=torch.uint8) for _ in range(2))
+    table = torch.arange(5, dtype=torch.int32) if table is None else table
+    args = dict(kv_block_indexes=None, q_offset_override=None, out=None, max_score=None, sm_scale=None, q_scale=None, k_scale=None, v_scale=None,
+                o_scale=None, output_maxscore=True, output_o=True, check_input_valid=False, max_score_dtype=None, lse=None)
+    if "kv_block_num" in opts:
+        args["kv_block_indexes"] = torch.zeros(sum(qo), hk, opts["kv_block_num"], dtype=torch.int32)
+    return api._fmha_sail_kv4(q, k, v, plan, table, **{**args, **extra, **kw})
+
+
+@pytest.mark.parametrize("path", list(PATHS))
+def test_a_table_shorter_than_the_plan_is_refused(api, path):
+    with pytest.raises(Copied):
+        _call(api, path)
+    for n in (4, 1, 0):
+        with pytest.raises(ValueError, match="kv_indices must have the 5 pages"):
+            _call(api, path, table=torch.arange(n, dtype=torch.int32))
+
+
+def test_a_call_without_tokens_needs_no_table(api):
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32)
+    plan = api._fmha_sail_plan(i32([0, 0]), i32([300, 200]), 16, 2, page_size=128, device="cpu", use_kv4_cache=True)
+    k = torch.zeros(9, 2, 128, 72, dtype=torch.uint8)
+    with pytest.raises(Copied):
+        api._fmha_sail_kv4(torch.zeros(0, 16, 128, dtype=torch.bfloat16), k, k, plan, i32([]), *[None] * 9, True, True, False, None, None)
