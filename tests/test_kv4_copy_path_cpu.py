@@ -58,3 +58,12 @@ def test_a_call_without_tokens_needs_no_table(api):
     k = torch.zeros(9, 2, 128, 72, dtype=torch.uint8)
     with pytest.raises(Copied):
         api._fmha_sail_kv4(torch.zeros(0, 16, 128, dtype=torch.bfloat16), k, k, plan, i32([]), *[None] * 9, True, True, False, None, None)
+
+
+@pytest.mark.parametrize("path", list(PATHS))
+def test_offsets_of_another_batch_are_refused(api, path):
+    with pytest.raises(Copied):
+        _call(api, path, q_offset_override=torch.zeros(len(PATHS[path][0]), dtype=torch.int32))
+    for shape in [(len(PATHS[path][0]) + 1,), (0,), (len(PATHS[path][0]), 1)]:
+        with pytest.raises(ValueError, match="q_offset_override must be"):
+            _call(api, path, q_offset_override=torch.zeros(shape, dtype=torch.int32))

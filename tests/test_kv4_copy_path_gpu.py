@@ -36,3 +36,17 @@ def test_a_call_without_tokens():
     plan = msa.fmha_sail_plan(torch.tensor([0, 0]), torch.tensor([300, 200]), 16, num_kv_heads=2, page_size=128, use_kv4_cache=True)
     out, _ = msa.fmha_sail(torch.empty(0, 16, 128, dtype=torch.bfloat16, device=DEV), k, v, plan, kv_indices=none)
     assert out.shape == (0, 16, 128)
+
+
+def test_offsets_of_any_type_and_stride():
+    """An override may be int64, or every second entry of a tensor: it is what it says, entry by entry."""
+    import msa_for_sail as msa
+    b = Batch(102, [140, 3], [300, 200], 8, 2, offsets=[100, 150])
+    q, k, v, table = b.cuda()
+    plan = msa.fmha_sail_plan(torch.tensor(b.qo), torch.tensor(b.kv), 8, num_kv_heads=2, page_size=128, use_kv4_cache=True)
+    wide = torch.tensor([100, -7, 150, -7], device=DEV)
+    for off in (wide[::2], wide[::2].to(torch.int32), wide.to(torch.int32)[::2]):
+        out, _ = msa.fmha_sail(q, k, v, plan, kv_indices=table, q_offset_override=off)
+        ref.check_attention(out, None, b.want(), P_BF16, "offsets")
+    with pytest.raises(ValueError, match="q_offset_override must be"):
+        msa.fmha_sail(q, k, v, plan, kv_indices=table, q_offset_override=wide[:1])
