@@ -303,12 +303,14 @@ typedef struct MsaNormRopeArgs {
 int msa_norm_rope(const MsaNormRopeArgs* args, msa_stream_t stream);
 
 /* Rows of a KV4 cache as bf16 (exact).  whole_pages == 0: out[i][head] = row slot_map[i] (zeros for a negative slot or one past
- * num_pages); != 0: out[i][head][128][128] = page slot_map[i] (left as it was for a page outside [0, num_pages)). */
+ * num_pages); != 0: out[i][head][128][128] = page slot_map[i] (the nearest one for a number outside [0, num_pages)), for the first
+ * *num_used entries or all; what is behind them is left as it was. */
 typedef struct MsaKv4ReadArgs {
   const void* cache;
   void* out;
   const int32_t* slot_map;         /* [rows] device: slots, or pages */
   int32_t* status;
+  const int32_t* num_used;         /* whole_pages: [1] device, entries that count (the last one of kv_page_indptr), or NULL: all */
   int64_t stride_page, stride_head;
   int32_t rows, num_kv_heads, num_pages, whole_pages;
 } MsaKv4ReadArgs;

@@ -417,13 +417,14 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const MsaKv4ReadArgs a) {
 }
 
 // Whole pages, in the order of a page table: out[e, head, 128, 128] = page kv_indices[e].  A block has a (page, head), 16 lanes a row as
-// above, so that the writes of a warp are 512 contiguous bytes; memory bounds it.
+// above, so that the writes of a warp are 512 contiguous bytes; memory bounds it.  A number that is no page is the nearest one, as in
+// the kernels that read 4 bits: what is attended to was written.
 __global__ void __launch_bounds__(256) kv4_unpack_kernel(const MsaKv4ReadArgs a) {
   chain_begin();
   const int l = threadIdx.x & 15;
   const int e = blockIdx.x, h = blockIdx.y;
-  const int page = a.slot_map[e];
-  if (page < 0 || page >= a.num_pages) return;               // behind the last page of a table that is longer than its use
+  if ((a.num_used && e >= *a.num_used) || a.num_pages == 0) return;      // behind the last page of a table that is longer than its use
+  const int page = min(max(chk(a.slot_map[e], 0, a.num_pages, a.status), 0), a.num_pages - 1);
   const unsigned char* tile = static_cast<const unsigned char*>(a.cache) + page * a.stride_page + h * a.stride_head;
   __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) + (static_cast<int64_t>(e) * a.num_kv_heads + h) * (kKvTile * kHeadDim) + 8 * l;
 #pragma unroll

@@ -84,7 +84,7 @@ class MsaNormRopeArgs(ctypes.Structure):
 
 
 class MsaKv4ReadArgs(ctypes.Structure):
-    _fields_ = [("cache", _p), ("out", _p), ("slot_map", _p), ("status", _p), ("stride_page", _i64), ("stride_head", _i64),
+    _fields_ = [("cache", _p), ("out", _p), ("slot_map", _p), ("status", _p), ("num_used", _p), ("stride_page", _i64), ("stride_head", _i64),
                 ("rows", _i32), ("num_kv_heads", _i32), ("num_pages", _i32), ("whole_pages", _i32)]
 
 

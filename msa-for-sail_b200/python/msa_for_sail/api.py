@@ -1061,23 +1061,24 @@ def _fmha_sail_kv4(q, k, v, plan, kv_indices, kv_block_indexes, q_offset_overrid
             if tuple(qo_offset.shape) != (plan["batch_size"],):
                 raise ValueError(f"q_offset_override must be [batch_size={plan['batch_size']}], got {tuple(qo_offset.shape)}")
             qo_offset = qo_offset.to(torch.int32).contiguous()
+    if check_input_valid and plan["_host"] is not None:
+        _validate_fmha_inputs(q, k, k if v is None else v, plan, True, False, num_kv_heads, cache.KV4_TILE, kv_indices, kv_block_indexes, qo_offset)
     if not native:
         with cache._on(dev):
             table = torch.arange(kv_indices.shape[0], dtype=torch.int32, device=dev)
-            kb = cache.unpack_pages(k, kv_indices)
-            vb = cache.unpack_pages(v, kv_indices) if output_o else kb
+            used = plan["kv_page_indptr"].data_ptr() + 4 * plan["batch_size"]
+            kb = cache.unpack_pages(k, kv_indices, used)
+            vb = cache.unpack_pages(v, kv_indices, used) if output_o else kb
             # workspaces of its own: two streams, or two captured graphs, may run one plan at the same time
             plan = PlanInfo(plan, sparse_ws=None)
             for name in ("workspace_o", "workspace_lse"):
                 if plan[name] is not None:
                     plan[name] = torch.empty_like(plan[name])
             return _fmha_sail(q if q.dtype == torch.bfloat16 else q.to(torch.bfloat16), kb, vb, plan, table, kv_block_indexes, qo_offset, out,
-                              max_score, sm_scale, q_scale, k_scale, v_scale, o_scale, output_maxscore, output_o, check_input_valid,
+                              max_score, sm_scale, q_scale, k_scale, v_scale, o_scale, output_maxscore, output_o, False,
                               max_score_dtype, lse)
     if plan["orig_num_qo_heads"] != num_qo_heads or plan["num_kv_heads"] != num_kv_heads:
         raise ValueError("plan head counts do not match q / k")
-    if check_input_valid and plan["_host"] is not None:
-        _validate_fmha_inputs(q, k, v, plan, True, False, num_kv_heads, cache.KV4_TILE, kv_indices, kv_block_indexes, qo_offset)
     if sm_scale is None:
         sm_scale = 1.0 / math.sqrt(128)
     q_s, _ = _scale_arg(q_scale, dev, num_kv_heads)

@@ -87,7 +87,7 @@ def _check_kv4(name, t, num_kv_heads=None):
     return stride
 
 
-def _read(cache, stride, index, out, whole_pages):
+def _read(cache, stride, index, out, whole_pages, num_used=0):
     rows, shape = index.shape[0], cache.shape
     if rows == 0:
         return out
@@ -95,8 +95,8 @@ def _read(cache, stride, index, out, whole_pages):
         return out.zero_()
     dev = cache.device
     _launch(dev, _lib.lib.msa_kv4_read, _lib.kv4_read_args(
-        cache.data_ptr(), out.data_ptr(), index.data_ptr(), _status_ptr(dev) or 0, stride[0], stride[1], rows, shape[1], shape[0], whole_pages),
-        "msa_kv4_read")
+        cache.data_ptr(), out.data_ptr(), index.data_ptr(), _status_ptr(dev) or 0, num_used, stride[0], stride[1], rows, shape[1], shape[0],
+        whole_pages), "msa_kv4_read")
     return out
 
 
@@ -126,10 +126,11 @@ def kv4_read(cache: torch.Tensor, slot_map: torch.Tensor, out: Optional[torch.Te
     return _read(cache, stride, slot_map, out, 0)
 
 
-def unpack_pages(cache, kv_indices):
-    """Pages of a 4-bit cache as bf16 ``[len(kv_indices), Hkv, 128, 128]``; pages outside the cache are left as they were."""
+def unpack_pages(cache, kv_indices, num_used=0):
+    """Pages of a 4-bit cache as bf16 ``[len(kv_indices), Hkv, 128, 128]``, the nearest page for a number that is none.  ``num_used``:
+    where the device has the number of entries that count (0: all do); the pages behind them are left as they were."""
     out = torch.empty(kv_indices.shape[0], cache.shape[1], KV4_TILE, 128, dtype=torch.bfloat16, device=cache.device)
-    return _read(cache, cache.stride(), kv_indices, out, 1)
+    return _read(cache, cache.stride(), kv_indices, out, 1, num_used)
 
 
 # ----------------------------------------------------------------------------

@@ -39,7 +39,7 @@ def _call(api, path, table=None, **kw):
     args = dict(kv_block_indexes=None, q_offset_override=None, out=None, max_score=None, sm_scale=None, q_scale=None, k_scale=None, v_scale=None,
                 o_scale=None, output_maxscore=True, output_o=True, check_input_valid=False, max_score_dtype=None, lse=None)
     if "kv_block_num" in opts:
-        args["kv_block_indexes"] = torch.zeros(sum(qo), hk, opts["kv_block_num"], dtype=torch.int32)
+        args["kv_block_indexes"] = torch.arange(opts["kv_block_num"], dtype=torch.int32).expand(sum(qo), hk, -1)
     return api._fmha_sail_kv4(q, k, v, plan, table, **{**args, **extra, **kw})
 
 
@@ -67,3 +67,12 @@ def test_offsets_of_another_batch_are_refused(api, path):
     for shape in [(len(PATHS[path][0]) + 1,), (0,), (len(PATHS[path][0]), 1)]:
         with pytest.raises(ValueError, match="q_offset_override must be"):
             _call(api, path, q_offset_override=torch.zeros(shape, dtype=torch.int32))
+
+
+@pytest.mark.parametrize("path", list(PATHS))
+def test_checked_inputs_are_those_of_the_caller(api, path):
+    with pytest.raises(Copied):
+        _call(api, path, check_input_valid=True)
+    for bad in (9, -1, 10 ** 6):
+        with pytest.raises(AssertionError, match="outside"):
+            _call(api, path, table=torch.tensor([0, 1, bad, 3, 4], dtype=torch.int32), check_input_valid=True)

@@ -50,3 +50,66 @@ def test_offsets_of_any_type_and_stride():
         ref.check_attention(out, None, b.want(), P_BF16, "offsets")
     with pytest.raises(ValueError, match="q_offset_override must be"):
         msa.fmha_sail(q, k, v, plan, kv_indices=table, q_offset_override=wide[:1])
+
+
+def _paths(seed=103):
+    """(name, batch, plan, what the call adds) of every way to the copies."""
+    prompt = Batch(seed, [200, 1], [300, 200], 16, 2)
+    shared = Batch(seed + 1, [300], [900], 8, 2)
+    few = Batch(seed + 2, [9, 2], [500, 260], 64, 4)
+    return [("prompt", prompt, prompt.plan(), {}), ("scores", prompt, prompt.plan(output_maxscore=True), dict(output_o=False)),
+            ("shared pages", shared, shared.plan(kv_block_num=4), dict(kv_block_indexes=shared.blocks(4).to(DEV))), ("9 tokens", few, few.plan(), {})]
+
+
+def _results(x):
+    return [t.clone() for t in x if t is not None]
+
+
+def _dirty():
+    """What the allocator hands out next holds NaN, as memory that others have used may."""
+    torch.cuda.empty_cache()
+    junk = torch.full((1 << 27,), float("nan"), dtype=torch.bfloat16, device=DEV)
+    torch.cuda.synchronize()
+    del junk
+
+
+@pytest.mark.parametrize("i", range(4))
+def test_a_number_that_is_no_page(i):
+    """Checked, it is refused; else it is the nearest page, never memory that nobody wrote."""
+    import msa_for_sail as msa
+    from msa_for_sail import api
+    name, b, plan, kw = _paths()[i]
+    q, k, v, table = b.cuda()
+    for bad, near in ((10 ** 6, k.shape[0] - 1), (-3, 0), (k.shape[0], k.shape[0] - 1)):
+        wrong, right = table.clone(), table.clone()
+        wrong[1], right[1] = bad, near
+        want = _results(msa.fmha_sail(q, k, v, plan, kv_indices=right, check_input_valid=True, **kw))
+        _dirty()
+        got = _results(msa.fmha_sail(q, k, v, plan, kv_indices=wrong, **kw))
+        api.last_status()                                       # (the build with bounds checks reports the number)
+        assert all(torch.equal(x, y) for x, y in zip(got, want)) and len(got) == len(want) == 1, name
+        with pytest.raises(AssertionError, match="outside"):
+            msa.fmha_sail(q, k, v, plan, kv_indices=wrong, check_input_valid=True, **kw)
+
+
+def test_copies_of_the_pages_that_count():
+    """Entries behind the number that the device has are not copied; numbers that are no pages are the nearest ones."""
+    from msa_for_sail import cache
+    c = ref.random_kv4(torch.Generator().manual_seed(6), 7, 3).to(DEV)
+    want = ref.kv4_values(c)
+    pages, used = _i32([6, -1, 2, 7, 10 ** 6, 4, -1, 5]), _i32([99, 6])
+    got = cache.unpack_pages(c, pages, used[1:].data_ptr()).double().cpu()
+    assert torch.equal(got[:6], want[[6, 0, 2, 6, 6, 4]])
+    assert torch.equal(cache.unpack_pages(c, pages).double().cpu(), want[[6, 0, 2, 6, 6, 4, 0, 5]])
+    assert torch.equal(cache.unpack_pages(c, pages[:3], used.data_ptr()).double().cpu(), want[[6, 0, 2]])
+
+
+@pytest.mark.parametrize("what", ["pages", "table"])
+def test_the_checked_build_reports_what_the_copies_clamp(what):
+    import os
+    import subprocess
+    import sys
+    here = os.path.dirname(os.path.abspath(__file__))
+    r = subprocess.run([sys.executable, os.path.join(here, "checked_kv4_child.py"), what], capture_output=True, text=True, timeout=600,
+                       env=dict(os.environ, MSA_BOUNDS_CHECK="1"))
+    assert r.returncode == 0 and "CHECKED_KV4_OK" in r.stdout, r.stdout[-2000:] + "\n--- stderr ---\n" + r.stderr[-3000:]
