@@ -1065,12 +1065,16 @@ def _fmha_sail_kv4(q, k, v, plan, kv_indices, kv_block_indexes, q_offset_overrid
         _validate_fmha_inputs(q, k, k if v is None else v, plan, True, False, num_kv_heads, cache.KV4_TILE, kv_indices, kv_block_indexes, qo_offset)
     if not native:
         with cache._on(dev):
-            table = torch.arange(kv_indices.shape[0], dtype=torch.int32, device=dev)
-            used = plan["kv_page_indptr"].data_ptr() + 4 * plan["batch_size"]
-            kb = cache.unpack_pages(k, kv_indices, used)
-            vb = cache.unpack_pages(v, kv_indices, used) if output_o else kb
             # workspaces of its own: two streams, or two captured graphs, may run one plan at the same time
             plan = PlanInfo(plan, sparse_ws=None)
+            table = torch.arange(max(1, kv_indices.shape[0]), dtype=torch.int32, device=dev)
+            if kv_indices.shape[0] == 0:      # an empty table has no keys: a page that nobody sees
+                kb = vb = torch.zeros(1, num_kv_heads, cache.KV4_TILE, 128, dtype=torch.bfloat16, device=dev)
+                plan["kv_segment_lens"] = torch.zeros_like(plan["kv_segment_lens"])
+            else:
+                used = plan["kv_page_indptr"].data_ptr() + 4 * plan["batch_size"]
+                kb = cache.unpack_pages(k, kv_indices, used)
+                vb = cache.unpack_pages(v, kv_indices, used) if output_o else kb
             for name in ("workspace_o", "workspace_lse"):
                 if plan[name] is not None:
                     plan[name] = torch.empty_like(plan[name])

@@ -56,7 +56,7 @@ def test_a_call_without_tokens_needs_no_table(api):
     i32 = lambda x: torch.tensor(x, dtype=torch.int32)
     plan = api._fmha_sail_plan(i32([0, 0]), i32([300, 200]), 16, 2, page_size=128, device="cpu", use_kv4_cache=True)
     k = torch.zeros(9, 2, 128, 72, dtype=torch.uint8)
-    with pytest.raises(Copied):
+    with pytest.raises(RuntimeError, match="needs CUDA tensors"):         # as far as the attention over the copies
         api._fmha_sail_kv4(torch.zeros(0, 16, 128, dtype=torch.bfloat16), k, k, plan, i32([]), *[None] * 9, True, True, False, None, None)
 
 
@@ -76,3 +76,20 @@ def test_checked_inputs_are_those_of_the_caller(api, path):
     for bad in (9, -1, 10 ** 6):
         with pytest.raises(AssertionError, match="outside"):
             _call(api, path, table=torch.tensor([0, 1, bad, 3, 4], dtype=torch.int32), check_input_valid=True)
+
+
+def test_an_empty_table_copies_nothing(api, monkeypatch):
+    """Lengths of a device-made plan that an empty table cannot hold: the call goes on with sequences that have no keys."""
+    seen = {}
+
+    def run(q, k, v, plan, kv_indices, *a, **kw):
+        seen.update(k=k, v=v, lens=plan["kv_segment_lens"], table=kv_indices)
+        return None, None
+    monkeypatch.setattr(api, "_fmha_sail", run)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32)
+    plan = api._fmha_sail_plan(i32([200]), i32([600]), 16, 2, page_size=128, device="cpu", use_kv4_cache=True)
+    plan["_host"] = None                                        # as if the lengths had stayed on the device
+    k = torch.zeros(9, 2, 128, 72, dtype=torch.uint8)
+    api._fmha_sail_kv4(torch.zeros(200, 16, 128, dtype=torch.bfloat16), k, k, plan, i32([]), *[None] * 9, True, True, False, None, None)
+    assert seen["k"].shape == seen["v"].shape == (1, 2, 128, 128) and seen["table"].tolist() == [0] and seen["lens"].tolist() == [0]
+    assert plan["kv_segment_lens"].tolist() == [600]

@@ -113,3 +113,35 @@ def test_the_checked_build_reports_what_the_copies_clamp(what):
     r = subprocess.run([sys.executable, os.path.join(here, "checked_kv4_child.py"), what], capture_output=True, text=True, timeout=600,
                        env=dict(os.environ, MSA_BOUNDS_CHECK="1"))
     assert r.returncode == 0 and "CHECKED_KV4_OK" in r.stdout, r.stdout[-2000:] + "\n--- stderr ---\n" + r.stderr[-3000:]
+
+
+@pytest.mark.parametrize("rows,scores,splits", [(200, False, 1), (40, False, 2), (200, True, 1), (1, True, 1), (3, True, 1)])
+def test_an_empty_table_has_no_keys(rows, scores, splits):
+    """As on the kernels that read 4 bits: zeros, an LSE and scores of -inf; rows behind the last sequence stay as they were."""
+    import msa_for_sail as msa
+    hq, pad = 4, 3
+    k, v = (ref.random_kv4(torch.Generator().manual_seed(7), 6, 2).to(DEV) for _ in range(2))
+    q = torch.ones(rows + pad, hq, 128, dtype=torch.bfloat16, device=DEV)
+    ws = msa.allocate_graph_workspace(1, hq, num_kv_heads=2, page_size=128, max_qo_len=rows + pad, num_kv_splits=splits)
+    plan = msa.fmha_sail_plan(_i32([rows]), _i32([600]), hq, num_kv_heads=2, page_size=128, num_kv_splits=splits, graph_safe=True, output_maxscore=scores,
+                              max_total_q=rows + pad, max_qo_len_override=rows, qo_len_uniform_override=True, max_kv_len_override=600, qo_offset=_i32([-1]),
+                              given_workspace=ws, use_kv4_cache=True)
+    none = torch.empty(0, dtype=torch.int32, device=DEV)
+    if scores:
+        _, ms = msa.fmha_sail(q, k, v, plan, kv_indices=none, output_o=False)
+        assert (ms == -float("inf")).all()
+        return
+    out, lse = torch.full((rows + pad, hq, 128), 7.0, dtype=torch.bfloat16, device=DEV), torch.full((rows + pad, hq), 7.0, device=DEV)
+    msa.fmha_sail(q, k, v, plan, kv_indices=none, out=out, lse=lse)
+    assert (out[:rows] == 0).all() and (lse[:rows] == -float("inf")).all()
+    if splits == 1:
+        assert (out[rows:] == 7).all() and (lse[rows:] == 7).all()
+
+
+def test_sequences_without_a_key():
+    import msa_for_sail as msa
+    msa, k, v, none = _empty_batch()
+    plan = msa.fmha_sail_plan(torch.tensor([200, 5]), torch.tensor([0, 0]), 16, num_kv_heads=2, page_size=128, use_kv4_cache=True)
+    lse = torch.empty(205, 16, device=DEV)
+    out, _ = msa.fmha_sail(torch.ones(205, 16, 128, dtype=torch.bfloat16, device=DEV), k, v, plan, kv_indices=none, lse=lse)
+    assert (out == 0).all() and (lse == -float("inf")).all()
