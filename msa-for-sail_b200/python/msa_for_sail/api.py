@@ -692,10 +692,18 @@ def _head_scale(x, device, hkv):
     """Like ``_scale_arg``, without a read of the device: a tensor of one value is spread over the heads there."""
     if not isinstance(x, torch.Tensor):
         return 1.0 if x is None else float(x), None
+    if x.numel() == 1 and not x.is_cuda:
+        return float(x), None
     if x.dtype == torch.float32 and x.numel() == hkv and x.get_device() == device.index and x.is_contiguous():
         return 1.0, x
     assert x.numel() in (1, hkv), f"per-head scale must have {hkv} entries, got {x.numel()}"
     return 1.0, x.reshape(-1).expand(hkv).to(device=device, dtype=torch.float32).contiguous()
+
+
+def _scale_pair(a, b, device, hkv):
+    """Two scales that come as a product, as ``_head_scale`` gives one."""
+    (fa, ta), (fb, tb) = _head_scale(a, device, hkv), _head_scale(b, device, hkv)
+    return fa * fb, tb if ta is None else ta if tb is None else ta * tb
 
 
 def _scale_arg(x, device, hkv):
@@ -754,6 +762,7 @@ def _fmha_sail(
     check_input_valid: bool = False,
     max_score_dtype: Optional[torch.dtype] = None,
     lse: Optional[torch.Tensor] = None,
+    _scales=None,
 ) -> Tuple[Optional[torch.Tensor], Optional[torch.Tensor]]:
     """Internal runner (upstream ``_fmha_sail``, api.py:1221-1477).
 
@@ -838,10 +847,14 @@ def _fmha_sail(
 
     if sm_scale is None:
         sm_scale = 1.0 / math.sqrt(head_dim_qk)
-    q_s, _ = _scale_arg(q_scale, q.device, num_kv_heads)
-    k_s, k_head = _scale_arg(k_scale, q.device, num_kv_heads)
-    v_s, v_head = _scale_arg(v_scale, q.device, num_kv_heads)
-    o_s, _ = _scale_arg(o_scale, q.device, num_kv_heads)
+    if _scales is None:
+        q_s, _ = _scale_arg(q_scale, q.device, num_kv_heads)
+        k_s, k_head = _scale_arg(k_scale, q.device, num_kv_heads)
+        v_s, v_head = _scale_arg(v_scale, q.device, num_kv_heads)
+        o_s, _ = _scale_arg(o_scale, q.device, num_kv_heads)
+    else:                                     # products of scales that stay on the device
+        (k_s, k_head), (v_s, v_head) = _scales
+        q_s = o_s = 1.0
 
     assert output_o or output_maxscore
 
@@ -1063,6 +1076,7 @@ def _fmha_sail_kv4(q, k, v, plan, kv_indices, kv_block_indexes, q_offset_overrid
             qo_offset = qo_offset.to(torch.int32).contiguous()
     if check_input_valid and plan["_host"] is not None:
         _validate_fmha_inputs(q, k, k if v is None else v, plan, True, False, num_kv_heads, cache.KV4_TILE, kv_indices, kv_block_indexes, qo_offset)
+    scales = _scale_pair(q_scale, k_scale, dev, num_kv_heads), _scale_pair(o_scale, v_scale, dev, num_kv_heads)
     if not native:
         with cache._on(dev):
             # workspaces of its own: two streams, or two captured graphs, may run one plan at the same time
@@ -1079,16 +1093,12 @@ def _fmha_sail_kv4(q, k, v, plan, kv_indices, kv_block_indexes, q_offset_overrid
                 if plan[name] is not None:
                     plan[name] = torch.empty_like(plan[name])
             return _fmha_sail(q if q.dtype == torch.bfloat16 else q.to(torch.bfloat16), kb, vb, plan, table, kv_block_indexes, qo_offset, out,
-                              max_score, sm_scale, q_scale, k_scale, v_scale, o_scale, output_maxscore, output_o, False,
-                              max_score_dtype, lse)
+                              max_score, sm_scale, None, None, None, None, output_maxscore, output_o, False, max_score_dtype, lse, scales)
     if plan["orig_num_qo_heads"] != num_qo_heads or plan["num_kv_heads"] != num_kv_heads:
         raise ValueError("plan head counts do not match q / k")
     if sm_scale is None:
         sm_scale = 1.0 / math.sqrt(128)
-    q_s, _ = _scale_arg(q_scale, dev, num_kv_heads)
-    k_s, k_head = _head_scale(k_scale, dev, num_kv_heads)
-    v_s, v_head = _head_scale(v_scale, dev, num_kv_heads)
-    o_s, _ = _scale_arg(o_scale, dev, num_kv_heads)
+    (k_s, k_head), (out_scale, v_head) = scales
     if out is None:
         out = torch.empty(nnz_qo, num_qo_heads, 128, device=dev, dtype=torch.bfloat16)
     else:
@@ -1100,7 +1110,7 @@ def _fmha_sail_kv4(q, k, v, plan, kv_indices, kv_block_indexes, q_offset_overrid
         return out, None
     assert q.stride(2) == 1, "q head_dim must be contiguous"
     splits = plan["num_kv_splits"]
-    q_stride, out_scale = q.stride(), float(v_s * o_s)
+    q_stride = q.stride()
     base = plan.get("_kv4_params")            # the sizes that are the same in every call with this plan
     if base is None:
         base = plan["_kv4_params"] = bytes(_lib.MsaFmhaParams(
@@ -1113,7 +1123,7 @@ def _fmha_sail_kv4(q, k, v, plan, kv_indices, kv_block_indexes, q_offset_overrid
     p.q, p.k, p.v, p.kv_indices = q.data_ptr(), k.data_ptr(), v.data_ptr(), kv_indices.data_ptr() or p.kv_page_indptr     # (an empty table is not read)
     p.q_stride_tok, p.q_stride_head, p.total_q, p.q_dtype = q_stride[0], q_stride[1], nnz_qo, _dt_code(q.dtype)
     p.k_stride_page, p.k_stride_head, p.v_stride_page, p.v_stride_head = k_stride[0], k_stride[1], v_stride[0], v_stride[1]
-    p.kv_extent, p.sm_scale, p.out_scale = k.shape[0], float(q_s * k_s * sm_scale), out_scale
+    p.kv_extent, p.sm_scale, p.out_scale = k.shape[0], float(k_s * sm_scale), out_scale
     if k_head is not None:
         p.k_scale_head = k_head.data_ptr()
     if v_head is not None:

@@ -145,3 +145,69 @@ def test_sequences_without_a_key():
     lse = torch.empty(205, 16, device=DEV)
     out, _ = msa.fmha_sail(torch.ones(205, 16, 128, dtype=torch.bfloat16, device=DEV), k, v, plan, kv_indices=none, lse=lse)
     assert (out == 0).all() and (lse == -float("inf")).all()
+
+
+def _one_value(x, **kw):
+    return torch.tensor([x], device=DEV, **kw)
+
+
+@pytest.mark.parametrize("path", ["prompt", "tokens", "shared pages", "scores"])
+@pytest.mark.parametrize("hk", [1, 2])
+def test_scales_stay_on_the_device(path, hk):
+    """One value for all heads, or one per head, of every scale: nothing is read back, so a graph sees what they become."""
+    import msa_for_sail as msa
+    hq = 8 * hk
+    b = Batch(110, *{"prompt": ([200, 1], [300, 200]), "tokens": ([1, 1], [300, 200]), "shared pages": ([300], [600]), "scores": ([140], [300])}[path],
+              hq, hk, q_dtype=torch.float8_e4m3fn if path in ("prompt", "tokens") else torch.bfloat16)
+    q, k, v, table = b.cuda()
+    kw, want_kw = {}, {}
+    plan = b.plan(**{"shared pages": dict(kv_block_num=2), "scores": dict(output_maxscore=True)}.get(path, {}))
+    if path == "shared pages":
+        blocks = b.blocks(2)
+        kw, want_kw = dict(kv_block_indexes=blocks.to(DEV)), dict(blocks=blocks)
+    if path == "scores":
+        kw = dict(output_o=False)
+    scales = dict(q_scale=_one_value(0.5), k_scale=_one_value(1.5), v_scale=torch.rand(hk, device=DEV) + 0.5, o_scale=_one_value(2.0))
+    run = lambda: [x for x in msa.fmha_sail(q, k, v, plan, kv_indices=table, **scales, **kw) if x is not None][0]
+    run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run()
+    scales["q_scale"].fill_(0.75), scales["k_scale"].fill_(0.25), scales["v_scale"].mul_(3.0), scales["o_scale"].fill_(0.125)
+    graph.replay()
+    torch.cuda.synchronize()
+    if path == "scores":                                        # largest raw products: no scale enters
+        plain = msa.fmha_sail(q, k, v, plan, kv_indices=table, **kw)[1]
+        assert torch.equal(got, plain)
+        return
+    want = b.want(k_scale=torch.full((hk,), 0.75 * 0.25), v_scale=scales["v_scale"] * 0.125, **want_kw)
+    ref.check_attention(got, None, want, P_BF16, path)
+
+
+@pytest.mark.parametrize("path", ["prompt", "tokens"])
+def test_every_form_of_a_scale(path):
+    """Floats, one value in host memory (fp64 too), one value and one per head on the device: the same attention."""
+    import msa_for_sail as msa
+    b = Batch(111, [200 if path == "prompt" else 2], [300], 8, 2)
+    q, k, v, table = b.cuda()
+    plan = b.plan()
+    want = b.want(k_scale=torch.full((2,), 0.5 * 0.25), v_scale=torch.full((2,), 4.0 * 0.5))
+    forms = [lambda x: x, lambda x: torch.tensor(x), lambda x: torch.tensor([x], dtype=torch.float64), _one_value, lambda x: _one_value(x, dtype=torch.bfloat16),
+             lambda x: torch.full((2,), x, device=DEV), lambda x: torch.full((2,), x), lambda x: torch.full((4,), x, device=DEV)[::2]]
+    for i, f in enumerate(forms):
+        lse = torch.empty(b.T, 8, device=DEV)
+        out, _ = msa.fmha_sail(q, k, v, plan, kv_indices=table, q_scale=f(0.5), k_scale=f(0.25), v_scale=f(4.0), o_scale=f(0.5), lse=lse)
+        ref.check_attention(out, lse, want, P_BF16, f"{path}, form {i}")
+    for name in ("q_scale", "k_scale", "v_scale", "o_scale"):
+        with pytest.raises(AssertionError, match="must have 2 entries"):
+            msa.fmha_sail(q, k, v, plan, kv_indices=table, **{name: torch.ones(3, device=DEV)})
+    # one value in host memory does not stop a capture
+    graph, one = torch.cuda.CUDAGraph(), torch.tensor(0.5)
+    first = msa.fmha_sail(q, k, v, plan, kv_indices=table, k_scale=one)[0].clone()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        out, _ = msa.fmha_sail(q, k, v, plan, kv_indices=table, k_scale=one)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, first)
