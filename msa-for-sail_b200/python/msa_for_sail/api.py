@@ -973,7 +973,7 @@ def _fmha_sail(
     p.kv_extent = k.shape[0]
     if use_tc:
         p.work, p.num_work, p.block_m = plan["work_tc"].data_ptr(), plan["num_work_tc"], 256
-    p.status = _status_word(q.device).data_ptr()
+    p.status = _status_ptr(q.device)
     rows = plan["max_qo_len"] * plan["pack_factor"] if kv_block_indexes is None else plan["pack_factor"]
     dt_ok = (q.dtype == torch.bfloat16 and k.dtype == torch.bfloat16) or k.dtype == torch.float8_e4m3fn
     if (_USE_DECODE_TC and not use_tc and output_o != (max_score is not None) and dt_ok

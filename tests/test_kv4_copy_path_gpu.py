@@ -211,3 +211,27 @@ def test_every_form_of_a_scale(path):
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(out, first)
+
+
+@pytest.mark.parametrize("kind", ["kv4", "bf16"])
+def test_first_prompt_of_a_process_inside_a_capture(kind, monkeypatch):
+    """The word that kernels report to is not made inside a capture, where it would belong to the graph and hold anything until a replay."""
+    import msa_for_sail as msa
+    from msa_for_sail import api
+    b = Batch(112, [200, 1], [300, 200], 8, 2)
+    q, k, v, table = b.cuda()
+    if kind == "bf16":
+        k, v = (ref.kv4_values(x).nan_to_num(0.0).to(torch.bfloat16).to(DEV) for x in (b.k, b.v))
+    plan = b.plan()
+    msa.fmha_sail(q, k, v, plan, kv_indices=table)
+    torch.cuda.synchronize()
+    monkeypatch.setattr(api, "_STATUS", {})
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, _ = msa.fmha_sail(q, k, v, plan, kv_indices=table)
+    assert not api._STATUS
+    first, _ = msa.fmha_sail(q, k, v, plan, kv_indices=table)    # before any replay
+    ref.check_attention(first, None, b.want(), P_BF16, "eager")
+    graph.replay()
+    torch.cuda.synchronize()
+    ref.check_attention(out, None, b.want(), P_BF16, "captured")
