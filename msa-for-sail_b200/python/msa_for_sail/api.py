@@ -742,6 +742,16 @@ def _show_params(q, plan, is_paged, page_size, sm_scale, output_o, max_score, kv
     print("[MSA] --format=" + ",".join(f"{k}:{v}" for k, v in fields) + ".", flush=True)
 
 
+def _copy_rows(out, result, plan):
+    """The bf16 result of an unsplit kernel into an fp32 ``out``; the rows behind the last sequence of a padded batch, which no kernel wrote,
+    stay as they were."""
+    if plan["_host"] is None:
+        real = torch.arange(out.shape[0], device=out.device) < plan["qo_segment_offsets"][-1]
+        torch.where(real[:, None, None], result, out, out=out)
+    else:
+        out.copy_(result)
+
+
 def _fmha_sail(
     q: torch.Tensor,
     k: torch.Tensor,
@@ -998,7 +1008,7 @@ def _fmha_sail(
             out.data_ptr(), _dt_code(out.dtype), _ptr(lse), splits, nnz_qo, num_qo_heads, 0, 0,
             out.stride(0), out.stride(1), float(v_s * o_s), stream), "msa_lse_merge_ex")
     elif kernel_out is not None and kernel_out is not out:
-        out.copy_(kernel_out)
+        _copy_rows(out, kernel_out, plan)
     return out, max_score
 
 
@@ -1155,7 +1165,7 @@ def _fmha_sail_kv4(q, k, v, plan, kv_indices, kv_block_indexes, q_offset_overrid
                 p.partial_o, p.partial_lse, _ptr(plan["num_kv_splits_per_row"]), out.data_ptr(), _dt_code(out.dtype), _ptr(lse),
                 splits, nnz_qo, num_qo_heads, out.stride(0), out.stride(1), out_scale, stream), "msa_lse_merge_many")
         elif kernel_out is not out:
-            out.copy_(kernel_out)
+            _copy_rows(out, kernel_out, plan)
     return out, None
 
 

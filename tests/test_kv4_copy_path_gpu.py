@@ -235,3 +235,35 @@ def test_first_prompt_of_a_process_inside_a_capture(kind, monkeypatch):
     graph.replay()
     torch.cuda.synchronize()
     ref.check_attention(out, None, b.want(), P_BF16, "captured")
+
+
+@pytest.mark.parametrize("kind", ["kv4", "bf16"])
+@pytest.mark.parametrize("n", [1, 3, 200])
+@pytest.mark.parametrize("sparse", [False, True])
+def test_fp32_rows_behind_the_last_sequence(kind, n, sparse):
+    """An fp32 result of an unsplit call: rows behind the last sequence of a padded batch stay as they were, bit for bit, and what is between
+    the rows of a wider buffer too."""
+    import msa_for_sail as msa
+    qo, pad, hq = [n, 1, 0], 4, 16
+    b = Batch(113, qo, [500, 130, 0], hq, 2)
+    q, k, v, table = b.cuda()
+    if kind == "bf16":
+        k, v = (ref.kv4_values(x).nan_to_num(0.0).to(torch.bfloat16).to(DEV) for x in (b.k, b.v))
+    T = b.T + pad
+    q = torch.cat([q, torch.full((pad, hq, 128), float("nan"), dtype=torch.bfloat16, device=DEV)])
+    blocks = torch.cat([b.blocks(3), torch.zeros(pad, 2, 3, dtype=torch.int32)])
+    kbn = 3 if sparse else -1
+    ws = msa.allocate_graph_workspace(3, hq, num_kv_heads=2, page_size=128, num_kv_splits=1, kv_block_num=kbn, max_qo_len=n + 2)
+    off = _i32([-1] * 3)
+
+    def run(out):
+        plan = msa.fmha_sail_plan(_i32(qo), _i32(b.kv), hq, num_kv_heads=2, page_size=128, kv_block_num=kbn, num_kv_splits=1, graph_safe=True, max_total_q=T,
+                                  max_qo_len_override=n, qo_len_uniform_override=False, max_kv_len_override=600, qo_offset=off, given_workspace=ws,
+                                  use_kv4_cache=kind == "kv4")
+        msa.fmha_sail(q, k, v, plan, kv_indices=table, out=out, **(dict(kv_block_indexes=blocks.to(DEV)) if sparse else {}))
+
+    was = torch.randn(T, hq + 3, 128, device=DEV)
+    wide = was.clone()
+    run(wide[:, 1:1 + hq])
+    ref.check_attention(wide[:b.T, 1:1 + hq], None, b.want(**(dict(blocks=blocks[:b.T]) if sparse else {})), P_BF16, "real rows")
+    assert torch.equal(wide[b.T:], was[b.T:]) and torch.equal(wide[:, 0], was[:, 0]) and torch.equal(wide[:, 1 + hq:], was[:, 1 + hq:])
