@@ -203,7 +203,8 @@ int msa_plan_dense(const MsaPlanArgs* args, MsaWorkItem* work, int32_t capacity,
  * Everything that sizes a launch is fixed when the graph is built: batch, the number of
  * row tiles per batch item (`row_tiles` >= ceil(max qo_len * pack / block_m)), the split count.
  * One kernel launch on `stream`; reads no device memory on the host, allocates nothing.
- * Fills, for i in [0, batch):  qo_start / kv_start (exclusive prefix sums, [batch + 1]),
+ * Fills, for i in [0, batch):  qo_start / kv_start (exclusive prefix sums, [batch + 1]; qo_start never above max_total_q, where
+ * that is not 0: tokens of lengths that sum to more are in no sequence and in no work item, if qo_start is given),
  * kv_len_out, qo_offset_out (causal: kv_len - qo_len where qo_offset_in is NULL or
  * negative; non-causal: `noncausal_offset`), kv_page_indptr ([batch + 1], pages of
  * `page_size` keys, NULL for ragged K/V), token_batch ([max_total_q], NULL when unused),

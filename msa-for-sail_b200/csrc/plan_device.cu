@@ -15,6 +15,10 @@ __global__ void __launch_bounds__(256) plan_device_kernel(const MsaPlanDeviceArg
   const int G = a.pack;
   const int groups = a.num_qo_heads / G;
   const int S = a.num_splits;
+  // Lengths on the device may outgrow the caller's q and out: tokens past max_total_q are in no sequence (0: no bound).
+  auto bounded = [&](int tokens) -> int {
+    return a.max_total_q > 0 ? static_cast<int>(min(static_cast<unsigned>(tokens), static_cast<unsigned>(a.max_total_q))) : tokens;
+  };
   // Prefix sums over the batch, 256 items at a time: a warp scan and the sums of the warps.  (One thread that walked the
   // batch waited for two loads per item: 5.4 us a plan at 24 sequences.)
   __shared__ int s_sum[8][3];
@@ -60,18 +64,18 @@ __global__ void __launch_bounds__(256) plan_device_kernel(const MsaPlanDeviceArg
       }
     }
     if (b < a.batch) {
-      if (a.qo_start) a.qo_start[b] = start[0];
+      if (a.qo_start) a.qo_start[b] = bounded(start[0]);
       if (a.kv_start) a.kv_start[b] = start[1];
       if (a.kv_page_indptr) a.kv_page_indptr[b] = start[2];
     }
     __syncthreads();
   }
   if (threadIdx.x == 0) {
-    if (a.qo_start) a.qo_start[a.batch] = carry[0];
+    if (a.qo_start) a.qo_start[a.batch] = bounded(carry[0]);
     if (a.kv_start) a.kv_start[a.batch] = carry[1];
     if (a.kv_page_indptr) a.kv_page_indptr[a.batch] = carry[2];
   }
-  const int total_q = carry[0];
+  const int total_q = bounded(carry[0]);
   __syncthreads();                                         // qo_start is read below
   // work items: (((b * RT + r) * groups) + g) * S + s, row tiles in descending order
   if (a.work) {
@@ -88,7 +92,8 @@ __global__ void __launch_bounds__(256) plan_device_kernel(const MsaPlanDeviceArg
         if (off < 0) off = kl - ql;
       }
       const int row0 = (RT - 1 - rr) * bm_eff;
-      const int nrows = max(0, min(bm_eff, ql * G - row0));
+      const int tokens = a.qo_start ? a.qo_start[b + 1] - a.qo_start[b] : ql;
+      const int nrows = max(0, min(bm_eff, tokens * G - row0));
       long long vis = nrows > 0 ? min(static_cast<long long>(kl), static_cast<long long>((row0 + nrows - 1) / G) + off + 1) : 0;
       if (vis < 0) vis = 0;
       const int nt = static_cast<int>((vis + kKvTile - 1) / kKvTile);

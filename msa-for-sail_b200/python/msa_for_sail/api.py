@@ -580,10 +580,10 @@ def _fmha_sail_plan_device(qo_segment_lens, kv_segment_lens, num_qo_heads, hkv, 
     if want_tc:
         t = _lib.MsaPlanDeviceArgs()
         t.qo_len, t.kv_len, t.qo_offset_in = a.qo_len, a.kv_len, a.qo_offset_in
-        t.work = work_tc.data_ptr()
+        t.qo_start, t.work = a.qo_start, work_tc.data_ptr()         # (written again, with the same values)
         t.batch, t.num_qo_heads, t.num_kv_heads = batch, num_qo_heads, hkv
         t.block_m, t.pack, t.num_splits, t.row_tiles = 256, 1, 1, tc_tiles
-        t.page_size, t.causal, t.noncausal_offset, t.max_total_q = page_size, a.causal, a.noncausal_offset, 0
+        t.page_size, t.causal, t.noncausal_offset, t.max_total_q = page_size, a.causal, a.noncausal_offset, max_total_q
         _lib.check(_lib.lib.msa_plan_device(ctypes.byref(t), _stream()), "msa_plan_device")
 
     max_k_tiles = math.ceil(math.ceil(max_kv / KV_TILE) / 128) * 128 if output_maxscore else -1

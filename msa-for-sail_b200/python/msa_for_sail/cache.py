@@ -438,8 +438,9 @@ def paged_kv_tables(
     call, ``slot_map`` (``[max_total_q]``, -1 behind the last token) for the cache write, ``positions`` for the rotation, ``num_held``
     and ``num_free`` (the counts after this step; pass ``num_held_out=num_held, num_free_out=num_free`` to update in place) and
     ``num_missing``: pages and tokens that found no place.  Where that is not zero, missing pages are 0 in ``kv_indices``, places
-    behind the end of a ``kv_indices`` that is too short read as its last page, and the tokens' slots are -1: nothing goes out of
-    bounds, but attention over such a request means nothing.
+    behind the end of a ``kv_indices`` that is too short read as its last page, the tokens' slots are -1, and tokens past
+    ``max_total_q`` are in no sequence of a device-made plan with the same ``max_total_q``: nothing goes out of bounds, but attention
+    over such a request means nothing.
 
     ``out``: a former result of the same sizes, whose tensors are written again (a captured step's fixed addresses)."""
     if not qo_lens.is_cuda:

@@ -103,3 +103,41 @@ def test_tables_with_too_few_places_and_attention(kind):
     got, missing = run(4)
     assert none == 0 and missing == 5
     assert torch.equal(got[0], want[0]) and torch.isfinite(got.float()).all()
+
+
+@pytest.mark.parametrize("kind", ["bf16", "kv4"])
+@pytest.mark.parametrize("ql,hq,scores,splits", [([1, 1, 1, 1], 16, False, 1), ([1, 1, 1, 1], 16, False, 2), ([3, 4, 2, 3], 16, False, 1), ([2, 150, 200, 1], 4, False, 1),
+                                                 ([20, 30, 25, 4], 4, False, 2), ([1, 1, 1, 1], 2, True, 1), ([40, 150, 3, 9], 4, True, 1)])
+def test_tokens_past_the_rows_of_a_plan(kind, ql, hq, scores, splits):
+    """Query lengths on the device may sum to more than max_total_q, as paged_kv_tables counts in num_missing: what is past it is in no sequence.
+    The rows that there are get what they get from lengths that end there, and nothing around q, the result and the scores is touched."""
+    import msa_for_sail as msa
+    g = torch.Generator().manual_seed(14)
+    hk, kl = 2, [300, 500, 260, 129]
+    T = sum(ql[:2]) + (ql[2] + 1) // 2                          # ends inside the third sequence, or behind it
+    cut = [min(n, max(0, T - sum(ql[:i]))) for i, n in enumerate(ql)]
+    k, v = _cache(kind, g, 14, hk, 128)
+    table = torch.randperm(14, generator=g)[:sum(-(-n // 128) for n in kl)].to(torch.int32).to(DEV)
+    q = torch.randn(T + 512, hq, 128, generator=g).to(torch.bfloat16).to(DEV)
+    off = _i32([a - b for a, b in zip(kl, ql)])
+    tabs = msa.paged_kv_tables(_i32(ql), _i32(kl), torch.zeros(4, 4, dtype=torch.int32, device=DEV), max_total_q=T)
+    assert int(tabs["num_missing"]) == sum(ql) - T
+
+    def run(lens):
+        ws = msa.allocate_graph_workspace(4, hq, num_kv_heads=hk, page_size=128, max_qo_len=max(ql), num_kv_splits=splits)
+        plan = msa.fmha_sail_plan(_i32(lens), _i32(kl), hq, num_kv_heads=hk, page_size=128, num_kv_splits=splits, graph_safe=True, output_maxscore=scores,
+                                  max_total_q=T, max_qo_len_override=max(ql), qo_len_uniform_override=False, max_kv_len_override=500, qo_offset=off,
+                                  given_workspace=ws, use_kv4_cache=kind == "kv4")
+        assert plan[3]["qo_segment_offsets"].tolist() == [min(T, sum(ql[:i])) for i in range(5)]
+        if scores:
+            ms = torch.full((hq + 1, plan[3]["max_k_tiles"], T), -float("inf"), device=DEV)
+            msa.fmha_sail(q[:T], k, v, plan, kv_indices=table, output_o=False, max_score=ms[:hq])
+            assert (ms[hq] == -float("inf")).all()
+            return ms[:hq], None
+        out, lse = torch.full((T + 512, hq, 128), 7.0, dtype=torch.bfloat16, device=DEV), torch.full((T + 512, hq), 7.0, device=DEV)
+        msa.fmha_sail(q[:T], k, v, plan, kv_indices=table, out=out[:T], lse=lse[:T])
+        assert (out[T:] == 7).all() and (lse[T:] == 7).all()
+        return out[:T], lse[:T]
+    want, got = run(cut), run(ql)
+    assert torch.equal(got[0], want[0]) and (scores or torch.equal(got[1], want[1]))
+    assert scores or not (got[0] == 7).all(2).any()
