@@ -459,7 +459,8 @@ def _fmha_sail_plan(
             num_work = n
             splits = int(max_splits.value)
             rows = splits * total_q * orig_num_qo_heads
-            if splits == 1 or arena.fits([size for *_, size in up.parts] + [max(1, n) * 8, total_q, rows * 128, rows]):
+            partials = [] if use_kv4_cache else [rows * 128, rows]               # that the plan holds
+            if splits == 1 or arena.fits([size for *_, size in up.parts] + [max(1, n) * 8, total_q] + partials):
                 break
         up.add("work", host[:n], max(1, n) * 8)
         info["_work_host"] = host[:n]
@@ -470,7 +471,7 @@ def _fmha_sail_plan(
         info["tc_preferred"] = info["num_work_tc"] > 0 and (splits == 1 or info["num_work_tc"] * 2 >= num_sms)
 
     up.run(arena, info)
-    if splits > 1:
+    if splits > 1 and not use_kv4_cache:      # (calls over a 4-bit cache bring partials of their own)
         info["workspace_o"] = arena.take(splits * total_q * orig_num_qo_heads * 128, torch.float32)
         info["workspace_lse"] = arena.take(splits * total_q * orig_num_qo_heads, torch.float32)
     else:
@@ -560,7 +561,7 @@ def _fmha_sail_plan_device(qo_segment_lens, kv_segment_lens, num_qo_heads, hkv, 
     tc_tiles = max(1, -(-max_qo // 256))
     n_items_tc = batch * tc_tiles * num_qo_heads if want_tc else 0
     work_tc = arena.take(n_items_tc * 8, torch.int32) if want_tc else None
-    if splits > 1:
+    if splits > 1 and not use_kv4_cache:
         info["workspace_o"] = arena.take(splits * max_total_q * num_qo_heads * 128, torch.float32)
         info["workspace_lse"] = arena.take(splits * max_total_q * num_qo_heads, torch.float32)
     else:
@@ -928,8 +929,12 @@ def _fmha_sail(
     if lse is not None:
         assert lse.dtype == torch.float32 and lse.is_contiguous() and lse.shape == (nnz_qo, num_qo_heads)
     if use_split:
-        p.partial_o = plan["workspace_o"].data_ptr()
-        p.partial_lse = plan["workspace_lse"].data_ptr()
+        part_o, part_lse = plan["workspace_o"], plan["workspace_lse"]
+        if part_o is None:                    # the plan holds none: partials of this call
+            part_o = torch.empty(splits * nnz_qo * num_qo_heads * 128, dtype=torch.float32, device=q.device)
+            part_lse = torch.empty(splits * nnz_qo * num_qo_heads, dtype=torch.float32, device=q.device)
+        p.partial_o = part_o.data_ptr()
+        p.partial_lse = part_lse.data_ptr()
         p.num_splits = splits
     else:
         p.num_splits = 1
@@ -1004,7 +1009,7 @@ def _fmha_sail(
     if use_split:
         spr = plan["num_kv_splits_per_row"]
         _lib.check(_lib.lib.msa_lse_merge_ex(
-            plan["workspace_o"].data_ptr(), MSA_DT_F32, plan["workspace_lse"].data_ptr(), _ptr(spr),
+            p.partial_o, MSA_DT_F32, p.partial_lse, _ptr(spr),
             out.data_ptr(), _dt_code(out.dtype), _ptr(lse), splits, nnz_qo, num_qo_heads, 0, 0,
             out.stride(0), out.stride(1), float(v_s * o_s), stream), "msa_lse_merge_ex")
     elif kernel_out is not None and kernel_out is not out:
@@ -1090,7 +1095,7 @@ def _fmha_sail_kv4(q, k, v, plan, kv_indices, kv_block_indexes, q_offset_overrid
     if not native:
         with cache._on(dev):
             # workspaces of its own: two streams, or two captured graphs, may run one plan at the same time
-            plan = PlanInfo(plan, sparse_ws=None)
+            plan = PlanInfo(plan, sparse_ws=None, workspace_o=None, workspace_lse=None)
             table = torch.arange(max(1, kv_indices.shape[0]), dtype=torch.int32, device=dev)
             if kv_indices.shape[0] == 0:      # an empty table has no keys: a page that nobody sees
                 kb = vb = torch.zeros(1, num_kv_heads, cache.KV4_TILE, 128, dtype=torch.bfloat16, device=dev)
@@ -1099,9 +1104,6 @@ def _fmha_sail_kv4(q, k, v, plan, kv_indices, kv_block_indexes, q_offset_overrid
                 used = plan["kv_page_indptr"].data_ptr() + 4 * plan["batch_size"]
                 kb = cache.unpack_pages(k, kv_indices, used)
                 vb = cache.unpack_pages(v, kv_indices, used) if output_o else kb
-            for name in ("workspace_o", "workspace_lse"):
-                if plan[name] is not None:
-                    plan[name] = torch.empty_like(plan[name])
             return _fmha_sail(q if q.dtype == torch.bfloat16 else q.to(torch.bfloat16), kb, vb, plan, table, kv_block_indexes, qo_offset, out,
                               max_score, sm_scale, None, None, None, None, output_maxscore, output_o, False, max_score_dtype, lse, scales)
     if plan["orig_num_qo_heads"] != num_qo_heads or plan["num_kv_heads"] != num_kv_heads:

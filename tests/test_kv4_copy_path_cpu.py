@@ -93,3 +93,19 @@ def test_an_empty_table_copies_nothing(api, monkeypatch):
     api._fmha_sail_kv4(torch.zeros(200, 16, 128, dtype=torch.bfloat16), k, k, plan, i32([]), *[None] * 9, True, True, False, None, None)
     assert seen["k"].shape == seen["v"].shape == (1, 2, 128, 128) and seen["table"].tolist() == [0] and seen["lens"].tolist() == [0]
     assert plan["kv_segment_lens"].tolist() == [600]
+
+
+@pytest.mark.parametrize("qo,kv,hq,hk", [([1] * 24, [20000] * 23 + [60000], 64, 4), ([1], [1 << 20], 64, 8), ([4] * 8, [20000] * 8, 64, 8), ([20] * 2, [9000] * 2, 16, 4)])
+def test_plans_of_a_4_bit_cache_reserve_no_partials(api, qo, kv, hq, hk):
+    """Its calls allocate their own: a plan holds none, and a workspace without room for any still gets the finer cut."""
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32)
+    make = lambda **kw: api._fmha_sail_plan(i32(qo), i32(kv), hq, hk, page_size=128, device="cpu", use_kv4_cache=True, **kw)
+    free = make()
+    assert free["num_kv_splits"] > 1 and free["workspace_o"] is None and free["workspace_lse"] is None
+    last = max((t for t in free.values() if isinstance(t, torch.Tensor)), key=lambda t: t.data_ptr() + t.numel() * 4)
+    first = min(t.data_ptr() for t in free.values() if isinstance(t, torch.Tensor))
+    ws = torch.empty(last.data_ptr() + last.numel() * 4 - first, dtype=torch.uint8)
+    given = make(given_workspace=ws)
+    assert given["num_kv_splits"] == free["num_kv_splits"] and torch.equal(given["work"], free["work"])
+    with pytest.raises(ValueError, match="too small"):
+        make(given_workspace=ws[:1000])

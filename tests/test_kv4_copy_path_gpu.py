@@ -267,3 +267,33 @@ def test_fp32_rows_behind_the_last_sequence(kind, n, sparse):
     run(wide[:, 1:1 + hq])
     ref.check_attention(wide[:b.T, 1:1 + hq], None, b.want(**(dict(blocks=blocks[:b.T]) if sparse else {})), P_BF16, "real rows")
     assert torch.equal(wide[b.T:], was[b.T:]) and torch.equal(wide[:, 0], was[:, 0]) and torch.equal(wide[:, 1 + hq:], was[:, 1 + hq:])
+
+
+@pytest.mark.parametrize("path", ["tokens", "prompt", "selected", "another cache"])
+@pytest.mark.parametrize("on_device", [False, True])
+def test_partials_are_those_of_a_call(path, on_device):
+    """A plan for a 4-bit cache holds no partials; whatever runs with it, the copies and a cache of another type too, brings its own."""
+    import msa_for_sail as msa
+    qo, kv = {"prompt": ([40, 1], [900, 700])}.get(path, ([1, 2], [900, 700]))
+    b = Batch(114, qo, kv, 16, 4)
+    q, k, v, table = b.cuda()
+    blocks, kbn = (b.blocks(32), 32) if path == "selected" else (None, -1)       # (fewer pages are not cut: a merge costs more)
+    if path == "another cache":
+        k, v = (ref.kv4_values(x).nan_to_num(0.0).to(torch.bfloat16).to(DEV) for x in (b.k, b.v))
+    if on_device:
+        ws = msa.allocate_graph_workspace(2, 16, num_kv_heads=4, page_size=128, max_qo_len=max(qo), kv_block_num=kbn, num_kv_splits=1)
+        plan = msa.fmha_sail_plan(_i32(qo), _i32(kv), 16, num_kv_heads=4, page_size=128, kv_block_num=kbn, num_kv_splits=4, graph_safe=True, max_total_q=b.T,
+                                  max_qo_len_override=max(qo), qo_len_uniform_override=False, max_kv_len_override=900, qo_offset=_i32([-1, -1]),
+                                  given_workspace=ws, use_kv4_cache=True)
+    else:
+        plan = b.plan(num_kv_splits=4, kv_block_num=kbn)
+    assert plan[3]["num_kv_splits"] > 1 and plan[3]["workspace_o"] is None and plan[3]["workspace_lse"] is None
+    lse = torch.empty(b.T, 16, device=DEV)
+    for dtype in (torch.bfloat16, torch.float32):
+        out = torch.empty(b.T, 16, 128, dtype=dtype, device=DEV)
+        msa.fmha_sail(q, k, v, plan, kv_indices=table, out=out, lse=lse, **(dict(kv_block_indexes=blocks.to(DEV)) if blocks is not None else {}))
+        want = b.want(**(dict(blocks=blocks) if blocks is not None else {}))
+        # The decode kernel of a bf16 cache adds up the weights as it has rounded them, each by half a step (2^-8) at most, so their sum is
+        # within 2^-8 of the exact one and its logarithm within -log(1 - 2^-8) < 2^-8 + 2^-16.
+        ref.check_attention(out, None if path == "another cache" else lse, want, P_BF16, path)
+        assert path != "another cache" or ((lse.double().cpu() - want[1]).abs() <= want[3] + 2.0 ** -15 + 2.0 ** -21 * want[1].abs() + 2.0 ** -8 + 2.0 ** -16).all()
