@@ -423,8 +423,9 @@ __global__ void __launch_bounds__(256) kv4_unpack_kernel(const MsaKv4ReadArgs a)
   chain_begin();
   const int l = threadIdx.x & 15;
   const int e = blockIdx.x, h = blockIdx.y;
-  if ((a.num_used && e >= *a.num_used) || a.num_pages == 0) return;      // behind the last page of a table that is longer than its use
-  const int page = min(max(chk(a.slot_map[e], 0, a.num_pages, a.status), 0), a.num_pages - 1);
+  const int entry = a.slot_map[e], used = a.num_used ? *a.num_used : a.rows;         // (on their way together)
+  if (e >= used || a.num_pages == 0) return;                 // behind the last page of a table that is longer than its use
+  const int page = min(max(chk(entry, 0, a.num_pages, a.status), 0), a.num_pages - 1);
   const unsigned char* tile = static_cast<const unsigned char*>(a.cache) + page * a.stride_page + h * a.stride_head;
   __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) + (static_cast<int64_t>(e) * a.num_kv_heads + h) * (kKvTile * kHeadDim) + 8 * l;
 #pragma unroll
