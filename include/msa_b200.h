@@ -278,8 +278,9 @@ int msa_fmha_fwd_split_static(const MsaFmhaParams* params, const int32_t* splits
  *    by positions[axis[n]][token] * turns[n] for pair n; turns[n] = the frequency in turns per position, as a
  *    64-bit fraction (modulo 1).
  *  - cache: row of token t at slot_map[t] = page * page_size + offset; a negative slot, or one past num_pages, writes
- *    nothing.  Slots of one call are distinct.  Keys are computed in 64 bits and rounded to bf16, then divided by k_scale * k_scale_head[head]
- *    and rounded to the cache's type (bf16 caches: as they are); values likewise.
+ *    nothing.  Slots of one call are distinct.  Keys are computed in 64 bits and rounded to 32 and to bf16, then divided by
+ *    k_scale * k_scale_head[head] and rounded to the cache's type (bf16 caches: as they are); values likewise.
+ *  - e4m3 queries: rounded to bf16, divided by q_scale and rounded to e4m3.
  * No upstream counterpart (upstream starts at the attention call). */
 typedef struct MsaNormRopeArgs {
   const void* q; const void* k; const void* v;

@@ -8,9 +8,11 @@
 // wrapping integer product, exact to 2^-64 turns times the position at any position; the cosine and sine of what is left
 // are taken once per token and pair and shared by all heads.
 //
-// Keys that go into a cache are normed and rotated in 64 bits, rounded to bf16 once and quantised from there: which bf16, e4m3 or
-// e2m1 value a key next to a border gets does not depend on the order of a sum.  (They are a tenth of the rows or less.)
-// All else is computed in 32 bits and rounded once.
+// Keys that go into a cache are normed and rotated in 64 bits, rounded to 32 bits, from there to bf16 (the two steps of a cast of a
+// 64-bit tensor; a key within 2^-24 of itself of a border of two bf16 values may become the border and go to the even one), and
+// quantised from there: which bf16, e4m3 or e2m1 value a key next to a border gets does not depend on the order of a sum.  (They are
+// a tenth of the rows or less.)  All else is computed in 32 bits and rounded to bf16; queries in e4m3 are divided by their scale and
+// rounded from there, as a call that quantises bf16 queries does.
 //
 // 4-bit rows: 16 elements share an e4m3 scale s = round(max|x| / 6), at least 2^-9; the codes are the e2m1 roundings of x / s
 // (divisions as IEEE has them: an x on a border goes to the even code).  A NaN makes the scale of its 16 elements NaN.
@@ -116,7 +118,7 @@ __device__ __forceinline__ void norm_rotate_f(uint64_t (&x)[8], const uint64_t (
   }
 }
 
-// 64 bits, rounded to bf16.  cs: of pair i of this lane at 8 i.
+// 64 bits, rounded to 32 and to bf16.  cs: of pair i of this lane at 8 i.
 template <bool PAIRS>
 __device__ __forceinline__ void norm_rotate_d(float (&x)[16], const float (&w)[16], bool norm, float eps, bool turn, const double2* cs) {
   double z[16], r = 1.0;

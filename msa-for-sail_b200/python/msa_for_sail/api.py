@@ -1023,7 +1023,7 @@ def _fmha_sail_kv4(q, k, v, plan, kv_indices, kv_block_indexes, q_offset_overrid
 
     Work items of at most 128 rows (decode; sparse attention where few tokens share a page) read the codes themselves.  Longer
     queries and scores run on a bf16 copy of the table's pages, which is exact: the products of a prompt take far longer than the
-    copy."""
+    copy.  All checks come before either, so that they do not depend on which it is."""
     if kv_indices is None:
         raise ValueError("a 4-bit cache is paged: kv_indices is required")
     if q.dim() != 3 or q.shape[2] != 128:

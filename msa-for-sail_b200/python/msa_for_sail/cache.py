@@ -308,9 +308,9 @@ def qk_norm_rope(
     Without caches returns ``(q, k)`` in bf16.  With ``k_cache``, ``v_cache`` and ``v`` the rows go to ``slot_map[t]`` (int32,
     ``page * page_size + offset``; a negative slot writes nothing; slots of one call are distinct) and the result is ``(q, None)``,
     or ``(q, k_out)`` where that is given.  Caches are bf16 or e4m3 (HND or NHD, as ``fmha_sail`` takes them) or 4-bit
-    (``allocate_kv4_cache``); cached keys are computed in 64 bits and rounded to bf16 before they are quantised.  ``k_scale`` / ``v_scale`` (quantised caches): what
-    the attention call will multiply by, a float or one float32 value per KV head.  ``q_out`` may be ``q`` (in place) or
-    float8_e4m3fn (then ``q / q_scale`` is stored)."""
+    (``allocate_kv4_cache``); cached keys are computed in 64 bits and rounded to bf16 (by way of 32 bits) before they are quantised.
+    ``k_scale`` / ``v_scale`` (quantised caches): what the attention call will multiply by, a float or one float32 value per KV head.
+    ``q_out`` may be ``q`` (in place) or float8_e4m3fn (then ``q``, rounded to bf16, is divided by ``q_scale`` and stored)."""
     if not q.is_cuda:
         raise RuntimeError("qk_norm_rope needs CUDA tensors (there is no CPU path)")
     dev = q.device
