@@ -159,7 +159,8 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
     b = chk(w.batch, 0, p.batch, p.status); head0 = chk(w.head0, 0, p.num_qo_heads, p.status);
     tb = w.kv_tile_begin; te = w.kv_tile_end; split = chk(w.split, 0, p.num_splits, p.status);
     i_base = 0;
-    ntok = p.qo_start[b + 1] - p.qo_start[b];
+    // (lengths on the device may outgrow the rows that the plan and this kernel's tile were made for; G divides 128)
+    ntok = min(p.qo_start[b + 1] - p.qo_start[b], p.decode_rows >> (__ffs(G) - 1));
   } else {
     const int S = p.num_splits;
     int idx = blockIdx.x;

@@ -32,3 +32,8 @@ def test_the_length_travels_with_the_table():
     from msa_for_sail import _lib, api
     assert [n for n, _ in _lib.MsaFmhaParams._fields_][-1] == "num_page_entries"
     assert "p.num_page_entries = kv_indices.data_ptr(), kv_indices.numel()" in inspect.getsource(api._fmha_sail)
+
+
+def test_rows_of_a_decode_tile_are_bounded():
+    """A sequence of a device-made plan may have more tokens than the plan was made for: the tile holds as many rows as were announced."""
+    assert "ntok = min(p.qo_start[b + 1] - p.qo_start[b], p.decode_rows >> (__ffs(G) - 1));" in code("fmha_decode_tc.cu")

@@ -141,3 +141,35 @@ def test_tokens_past_the_rows_of_a_plan(kind, ql, hq, scores, splits):
     want, got = run(cut), run(ql)
     assert torch.equal(got[0], want[0]) and (scores or torch.equal(got[1], want[1]))
     assert scores or not (got[0] == 7).all(2).any()
+
+
+@pytest.mark.parametrize("kind", ["bf16", "e4m3", "kv4"])
+@pytest.mark.parametrize("most,hq,scores,splits", [(1, 16, False, 1), (2, 16, False, 2), (3, 16, False, 1), (8, 32, False, 1), (2, 16, True, 1), (1, 2, True, 1)])
+def test_more_tokens_than_a_plan_has_rows_for(kind, most, hq, scores, splits):
+    """A sequence with more tokens than max_qo_len_override: as many as fill its row tiles are worked on, the rows of the rest stay as they were."""
+    import msa_for_sail as msa
+    g = torch.Generator().manual_seed(15)
+    hk, kl, ql = 2, [300, 500], [40, 1]
+    k, v = _cache(kind, g, 9, hk, 128)
+    table = torch.randperm(9, generator=g)[:7].to(torch.int32).to(DEV)
+    q = torch.randn(41, hq, 128, generator=g).to(torch.bfloat16).to(DEV)
+    off = _i32([200, 499])
+
+    def run(lens, q, most):
+        T = q.shape[0]
+        ws = msa.allocate_graph_workspace(2, hq, num_kv_heads=hk, page_size=128, max_qo_len=40, num_kv_splits=splits)
+        plan = msa.fmha_sail_plan(_i32(lens), _i32(kl), hq, num_kv_heads=hk, page_size=128, num_kv_splits=splits, graph_safe=True, output_maxscore=scores,
+                                  max_total_q=T, max_qo_len_override=most, qo_len_uniform_override=False, max_kv_len_override=500, qo_offset=off,
+                                  given_workspace=ws, use_kv4_cache=kind == "kv4")
+        if scores:
+            ms = torch.full((hq, plan[3]["max_k_tiles"], T), 7.0, device=DEV)
+            msa.fmha_sail(q, k, v, plan, kv_indices=table, output_o=False, max_score=ms)
+            return ms.movedim(2, 0)
+        out = torch.full((T, hq, 128), 7.0, dtype=torch.bfloat16, device=DEV)
+        msa.fmha_sail(q, k, v, plan, kv_indices=table, out=out)
+        return out
+    want = run([most, 1], torch.cat([q[:most], q[40:]]), most)
+    got = run(ql, q, most)
+    assert torch.equal(got[:most], want[:most]) and torch.equal(got[40], want[most])
+    if splits == 1:                                             # (a merge takes the rows of every token)
+        assert (got[39] == 7).all()
