@@ -59,7 +59,8 @@ typedef struct MsaWorkItem {
   int32_t kv_tile_end;    /* one past the last tile                                */
   int32_t split;          /* split index for the partial workspace (0 if unsplit)  */
   int32_t num_rows;       /* packed rows of this item (<= block_m)                  */
-  int32_t reserved;
+  int32_t kv_tile_skip;   /* tiles that no row of a windowed item sees: tile t of the item is tile t of the keys for
+                             t < ceil(sink_tokens / 128), tile t + kv_tile_skip from there on (0 without a window) */
 } MsaWorkItem;
 
 /* Arguments of the FMHA forward.  Field-for-field successor of the upstream
@@ -113,6 +114,9 @@ typedef struct MsaFmhaParams {
   float   out_scale;       /* v_scale * o_scale                                              */
   int32_t num_page_entries; /* length of kv_indices: places past its end read as its last entry; 0 = not given,
                               every place that the lengths reach is read (kv_dtype = MSA_DT_KV4: num_logical_pages) */
+  int32_t window;          /* > 0: row i, at place t = i + qo_offset, sees key j <= t iff j > t - window or j < sink_tokens.
+                              Dense work lists made with the same two numbers, MSA_FLAG_OUT_O only; 0: every key up to t */
+  int32_t sink_tokens;
 } MsaFmhaParams;
 
 /* FMHA forward: dense ragged / dense paged / sparse, optional split-KV partials.
@@ -192,6 +196,8 @@ typedef struct MsaPlanArgs {
   int32_t num_sms;            /* device SM count (adaptive mode target)  */
   int32_t ctas_per_sm;        /* items an SM runs side by side; 0 = 1; < 0: all items cut alike, for two waves of the
                                * SMs, and uncut where there are as many (adaptive mode) */
+  int32_t window;             /* as in MsaFmhaParams: a row tile then has the tiles that its rows see, see kv_tile_skip */
+  int32_t sink_tokens;
 } MsaPlanArgs;
 int msa_plan_dense(const MsaPlanArgs* args, MsaWorkItem* work, int32_t capacity,
                    int32_t* splits_per_row /* [total_q] host */,
@@ -236,6 +242,8 @@ typedef struct MsaPlanDeviceArgs {
   int32_t noncausal_offset;
   int32_t max_total_q;
   int32_t row_tiles;           /* >= 1 */
+  int32_t window;              /* as in MsaPlanArgs */
+  int32_t sink_tokens;
 } MsaPlanDeviceArgs;
 int msa_plan_device(const MsaPlanDeviceArgs* args, msa_stream_t stream);
 
@@ -350,6 +358,97 @@ typedef struct MsaPageTablesArgs {
 int64_t msa_page_tables_workspace_bytes(int32_t batch);
 int msa_page_tables(const MsaPageTablesArgs* args, msa_stream_t stream);
 
+/* Pages of a cache: copies, rows of a block table that share pages, pages given back, pages in use moved together.
+ *
+ * A block table [batch][table_width], table_stride apart, has the page of each page_size tokens of a request; num_held[b] entries of
+ * row b are set, -1 among them for pages given back from the middle.  free_pages[0, *num_free) is the stack of free pages that
+ * msa_page_tables takes from.  shares[p] (NULL: each page is in one row) is the number of rows that hold page p beyond the first.
+ * Everything is on the device, and updated in place; results do not depend on the order of threads.  No upstream counterpart. */
+
+/* One tensor that holds something of every page: a page is `parts` pieces of part_bytes, stride_part bytes apart, from
+ * base + page * stride_page (bytes) on.  Any alignment; multiples of 16 bytes are fastest. */
+typedef struct MsaPageCache {
+  void* base;
+  int64_t stride_page, stride_part;
+  int32_t parts, part_bytes;
+  int32_t token_bytes;             /* bytes of one token in a piece, tokens in order; -1: each piece is a token; 0: neither, such
+                                      pages are copied whole where others are copied up to a token */
+  int32_t reserved;
+} MsaPageCache;
+
+/* Page src[i] to page dst[i] in every cache, for i in [0, count); a number outside [0, num_pages) copies nothing.  A page
+ * of dst is in dst once and not in src. */
+typedef struct MsaPagesCopyArgs {
+  const MsaPageCache* caches;      /* [num_caches] HOST */
+  const int32_t* src;              /* [count] device */
+  const int32_t* dst;
+  int32_t* status;
+  int32_t num_caches, count, num_pages, page_size;
+} MsaPagesCopyArgs;
+int msa_pages_copy(const MsaPagesCopyArgs* args, msa_stream_t stream);
+
+/* Row children[i] becomes a fork of row parents[i]: it shares the full pages of the first kv_len tokens (shares + 1 each), and gets a copy of
+ * the used part of the last page in a page from the stack, in the order of i.  kv_len and num_held of the child are set.
+ * An entry with a negative number does nothing.  Entries whose row is not in the table, is its own parent, holds pages already or was
+ * named as a child before are not made, and counted in num_missing; so is a child for whose last page the stack has none: it ends with its last
+ * full page.  Rows are read as they were before the call. */
+typedef struct MsaPagesForkArgs {
+  const MsaPageCache* caches;      /* [num_caches] HOST */
+  int32_t* block_table;
+  int32_t* num_held;               /* [batch] */
+  int32_t* kv_len;                 /* [batch] */
+  const int32_t* parents;          /* [count] device */
+  const int32_t* children;
+  const int32_t* free_pages;
+  int32_t* num_free;               /* [1] */
+  int32_t* shares;                 /* [num_pages] */
+  int32_t* num_missing;            /* [1] or NULL */
+  int32_t* workspace;              /* msa_pages_fork_workspace_bytes(batch, count) bytes */
+  int64_t table_stride;
+  int32_t num_caches, count, num_pages, page_size, batch, table_width, free_capacity;
+} MsaPagesForkArgs;
+int64_t msa_pages_fork_workspace_bytes(int32_t batch, int32_t count);
+int msa_pages_fork(const MsaPagesForkArgs* args, msa_stream_t stream);
+
+/* Row b keeps the pages of its first kv_len[b] tokens; with a window (as in MsaFmhaParams) also only those that a query at place
+ * kv_len[b] or later sees.  The other entries become -1, their pages lose a share, and those that nobody shares go onto the stack in the order of
+ * the entries (row, then column; of several entries with one page the first).  num_held becomes the pages of the length.
+ * Numbers outside [0, num_pages) are dropped. */
+typedef struct MsaPagesFreeArgs {
+  int32_t* block_table;
+  int32_t* num_held;               /* [batch] */
+  const int32_t* kv_len;           /* [batch] */
+  int32_t* free_pages;             /* [free_capacity] */
+  int32_t* num_free;               /* [1] */
+  int32_t* shares;                 /* [num_pages] or NULL */
+  int32_t* num_freed;              /* [1] or NULL: pages that went onto the stack */
+  int32_t* workspace;              /* msa_pages_free_workspace_bytes(batch, table_width) bytes */
+  int64_t table_stride;
+  int32_t batch, table_width, page_size, free_capacity, num_pages, window, sink_tokens;
+} MsaPagesFreeArgs;
+int64_t msa_pages_free_workspace_bytes(int32_t batch, int32_t table_width);
+int msa_pages_free(const MsaPagesFreeArgs* args, msa_stream_t stream);
+
+/* The pages that rows hold move to the lowest of the places that they and the free pages have: of those in use that lie higher, the lowest goes to
+ * the lowest free place, and so on.  Table, shares and caches follow; the stack has the free pages afterwards, the lowest on
+ * top.  Pages in no row and not on the stack stay where they are.  src / dst: the moves, -1 behind them. */
+typedef struct MsaPagesCompactArgs {
+  const MsaPageCache* caches;      /* [num_caches] HOST */
+  int32_t* block_table;
+  const int32_t* num_held;         /* [batch] */
+  int32_t* free_pages;             /* [free_capacity] */
+  int32_t* num_free;               /* [1] */
+  int32_t* shares;                 /* [num_pages] or NULL */
+  int32_t* src;                    /* [num_pages] */
+  int32_t* dst;
+  int32_t* num_moved;              /* [1] */
+  int32_t* workspace;              /* msa_pages_compact_workspace_bytes(num_pages) bytes */
+  int64_t table_stride;
+  int32_t num_caches, num_pages, page_size, batch, table_width, free_capacity;
+} MsaPagesCompactArgs;
+int64_t msa_pages_compact_workspace_bytes(int32_t num_pages);
+int msa_pages_compact(const MsaPagesCompactArgs* args, msa_stream_t stream);
+
 /* Human-readable text of an MSA_ERR_* code. */
 const char* msa_status_string(int code);
 
@@ -358,7 +457,8 @@ int msa_build_arch(void);
 
 /* sizeof() of the ABI structs as the library was compiled: 0 = MsaFmhaParams,
  * 1 = MsaWorkItem, 2 = MsaPlanArgs, 3 = MsaPlanDeviceArgs, 4 = MsaNormRopeArgs, 5 = MsaKv4ReadArgs,
- * 6 = MsaPageTablesArgs.  Lets a foreign-language binding verify its
+ * 6 = MsaPageTablesArgs, 7 = MsaPageCache, 8 = MsaPagesCopyArgs, 9 = MsaPagesForkArgs, 10 = MsaPagesFreeArgs,
+ * 11 = MsaPagesCompactArgs.  Lets a foreign-language binding verify its
  * own struct declaration at load time. */
 int msa_sizeof(int which);
 

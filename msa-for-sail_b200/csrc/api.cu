@@ -50,6 +50,8 @@ int validate_fmha(const MsaFmhaParams& p, bool own_scratch) {
   if (p.q_dtype != MSA_DT_BF16 && p.q_dtype != MSA_DT_E4M3) return MSA_ERR_UNSUPPORTED;
   if (p.kv_dtype != MSA_DT_BF16 && p.kv_dtype != MSA_DT_E4M3) return MSA_ERR_UNSUPPORTED;
   if (has_s && p.max_score_dtype != MSA_DT_F32 && p.max_score_dtype != MSA_DT_BF16) return MSA_ERR_UNSUPPORTED;
+  if (p.window < 0 || p.sink_tokens < 0 || (p.sink_tokens > 0 && p.window == 0)) return MSA_ERR_BAD_ARG;
+  if (p.window > 0 && (sparse || has_s)) return MSA_ERR_UNSUPPORTED;
   if (sparse) {
     if (!p.kv_block_indexes || !p.token_batch || p.kv_block_num <= 0) return MSA_ERR_BAD_ARG;
     if (p.page_size != msa::kKvTile) return MSA_ERR_UNSUPPORTED;   // a selected block is one 128-key page
@@ -85,7 +87,7 @@ extern "C" int msa_fmha_fwd(const MsaFmhaParams* pp, msa_stream_t stream_) {
 }
 
 namespace msa {
-struct Proto { int b, row0, nrows, ntiles; };      // the rows of one work item and their KV tiles, before any split
+struct Proto { int b, row0, nrows, ntiles, skip; };      // the rows of one work item and their KV tiles, before any split
 
 // Tile times until the last of `slots` workers is done when every item is cut into pieces of `chunk` tiles and the
 // pieces are handed out longest first.  A piece costs three tiles beyond its own (a CTA's dependent index loads, the
@@ -117,6 +119,7 @@ extern "C" int msa_plan_dense(const MsaPlanArgs* a, MsaWorkItem* work, int32_t c
   if (a->num_qo_heads <= 0 || a->num_kv_heads <= 0 || a->num_qo_heads % a->num_kv_heads) return MSA_ERR_BAD_ARG;
   const int G = a->pack;
   if (G < 1 || (a->num_qo_heads / a->num_kv_heads) % G || G > a->block_m) return MSA_ERR_BAD_ARG;
+  if (a->window < 0 || a->sink_tokens < 0 || (a->sink_tokens > 0 && a->window == 0)) return MSA_ERR_BAD_ARG;
   const int groups = a->num_qo_heads / G;
   const int bm_eff = (a->block_m / G) * G;       // a token's heads never straddle two items
 
@@ -127,12 +130,10 @@ extern "C" int msa_plan_dense(const MsaPlanArgs* a, MsaWorkItem* work, int32_t c
     const int rows = a->qo_len[b] * G;
     for (int r0 = 0; r0 < rows; r0 += bm_eff) {
       const int nrows = std::min(bm_eff, rows - r0);
-      const long long i_max = (r0 + nrows - 1) / G;
-      long long vis = std::min<long long>(a->kv_len[b], i_max + a->qo_offset[b] + 1);
-      if (vis < 0) vis = 0;
-      const int nt = static_cast<int>((vis + msa::kKvTile - 1) / msa::kKvTile);
-      protos.push_back({b, r0, nrows, nt});
-      max_tiles = std::max(max_tiles, nt);
+      const long long off = a->qo_offset[b];
+      const msa::WindowSpan span = msa::window_span(r0 / G + off, (r0 + nrows - 1) / G + off, a->kv_len[b], a->window, a->sink_tokens);
+      protos.push_back({b, r0, nrows, span.count, span.skip});
+      max_tiles = std::max(max_tiles, span.count);
     }
   }
   // one chunk size (tiles per split) for the whole plan
@@ -192,7 +193,7 @@ extern "C" int msa_plan_dense(const MsaPlanArgs* a, MsaWorkItem* work, int32_t c
         w.batch = pr.b; w.head0 = g * G; w.row0 = pr.row0;
         w.kv_tile_begin = std::min(pr.ntiles, s * chunk);
         w.kv_tile_end = std::min(pr.ntiles, (s + 1) * chunk);
-        w.split = s; w.num_rows = pr.nrows; w.reserved = 0;
+        w.split = s; w.num_rows = pr.nrows; w.kv_tile_skip = pr.skip;
         items.push_back(w);
       }
   }
@@ -235,6 +236,11 @@ extern "C" int msa_sizeof(int which) {
     case 4: return static_cast<int>(sizeof(MsaNormRopeArgs));
     case 5: return static_cast<int>(sizeof(MsaKv4ReadArgs));
     case 6: return static_cast<int>(sizeof(MsaPageTablesArgs));
+    case 7: return static_cast<int>(sizeof(MsaPageCache));
+    case 8: return static_cast<int>(sizeof(MsaPagesCopyArgs));
+    case 9: return static_cast<int>(sizeof(MsaPagesForkArgs));
+    case 10: return static_cast<int>(sizeof(MsaPagesFreeArgs));
+    case 11: return static_cast<int>(sizeof(MsaPagesCompactArgs));
     default: return -1;
   }
 }

@@ -41,6 +41,31 @@ __device__ __forceinline__ int page_entry(const MsaFmhaParams& p, int at) {
   return chk(p.kv_indices[place], 0, static_cast<int>(p.kv_extent), p.status);
 }
 
+// ---- windows ----
+// With a window W and S sink tokens a row at place t of its sequence sees key j <= t iff j > t - W or j < S.  The tiles that any of a row
+// tile's rows sees are those of the sinks and those from the first key of its first row's window on: the ones between are left out
+// of its work item, so that one range of numbers [0, count) stands for both.  Sums are taken in 64 bits: places may lie far behind the keys.
+struct WindowSpan {
+  int count;                    // tiles of the row tile
+  int skip;                     // tiles left out behind those of the sinks
+};
+__host__ __device__ inline int sink_tiles(int sink_tokens) { return sink_tokens / kKvTile + (sink_tokens % kKvTile != 0); }
+__host__ __device__ inline WindowSpan window_span(long long first_place, long long last_place, int kv_len, int window, int sink_tokens) {
+  long long end = last_place + 1 < kv_len ? last_place + 1 : kv_len;
+  if (end < 0) end = 0;
+  const int tiles = static_cast<int>((end + kKvTile - 1) / kKvTile);
+  if (window <= 0) return {tiles, 0};
+  long long lo = (first_place - window + 1) / kKvTile;
+  if (lo > tiles) lo = tiles;
+  const int skip = lo > sink_tiles(sink_tokens) ? static_cast<int>(lo) - sink_tiles(sink_tokens) : 0;
+  return {tiles - skip, skip};
+}
+// First key of the window of a row at place t, at most `kv_len`.
+__device__ __forceinline__ int window_first(int place, int kv_len, int window) {
+  const long long lo = static_cast<long long>(place) - window + 1;
+  return lo < 0 ? 0 : lo < kv_len ? static_cast<int>(lo) : kv_len;
+}
+
 // ---- kernels of one stream without a gap between them ----
 // A kernel launched with launch_chained() may start while the kernel before it in the stream still runs: once every CTA of
 // that one has called chain_begin() or ended.  chain_begin() comes before anything that touches global memory: it waits

@@ -801,6 +801,7 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
 // (optionally as split partials) or, for the proxy pass, the per-page max score alone
 int fmha_decode_tc_supported(const MsaFmhaParams& p) {
   const bool has_o = (p.flags & MSA_FLAG_OUT_O) != 0, has_s = (p.flags & MSA_FLAG_OUT_SCORE) != 0;
+  if (p.window > 0) return 0;
   if (has_o == has_s) return 0;                                  // O + score together stays on the generic kernel
   if (p.page_size != decode_tc::BN) return 0;
   if (p.kv_dtype == MSA_DT_BF16) { if (p.q_dtype != MSA_DT_BF16) return 0; }

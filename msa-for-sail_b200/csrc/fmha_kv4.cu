@@ -556,6 +556,7 @@ int fmha_kv4_fwd(const MsaFmhaParams& p, cudaStream_t stream) {
   const bool sparse = (p.flags & MSA_FLAG_SPARSE) != 0;
   if (!(p.flags & MSA_FLAG_OUT_O)) return (p.flags & MSA_FLAG_OUT_SCORE) ? MSA_ERR_UNSUPPORTED : MSA_ERR_BAD_ARG;
   if (p.flags & MSA_FLAG_OUT_SCORE) return MSA_ERR_UNSUPPORTED;
+  if (p.window != 0 || p.sink_tokens != 0) return p.window < 0 || p.sink_tokens < 0 || p.window == 0 ? MSA_ERR_BAD_ARG : MSA_ERR_UNSUPPORTED;
   if (!p.q || !p.k || !p.v || !p.qo_start || !p.kv_len || !p.qo_offset || !p.kv_page_indptr || !p.kv_indices) return MSA_ERR_BAD_ARG;
   if (p.total_q < 0 || p.batch < 0 || p.kv_extent < 0 || (!p.out && !p.partial_o)) return MSA_ERR_BAD_ARG;
   if (p.partial_o ? (!p.partial_lse || p.num_splits < 1) : p.num_splits != 1) return MSA_ERR_BAD_ARG;

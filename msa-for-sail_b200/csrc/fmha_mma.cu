@@ -40,7 +40,8 @@ struct Cfg {
   static constexpr int SMEM = Q_BYTES + (RING_BYTES > MERGE_BYTES ? RING_BYTES : MERGE_BYTES) + 1024;
 };
 
-template <int MW, int NW, bool HAS_O, bool KV8>
+// WIN: rows see a window and the first keys only (compiled on its own: the other modes' code stays as it is).
+template <int MW, int NW, bool HAS_O, bool KV8, bool WIN>
 __global__ void __launch_bounds__(32 * MW * NW, 1)
 fmha_mma_kernel(const __grid_constant__ MsaFmhaParams p) {
   using C = Cfg<MW, NW, HAS_O, KV8>;
@@ -66,12 +67,14 @@ fmha_mma_kernel(const __grid_constant__ MsaFmhaParams p) {
   // ---------------- item ----------------
   int b, head0, row0, tb, te, split, i_base, rows_total;   // rows_total: one past the item's last packed row
   const int32_t* blocks = nullptr;
+  [[maybe_unused]] int skip = 0;               // windowed: tiles left out behind those of the sinks
   if (!sparse) {
     if (static_cast<int>(blockIdx.x) >= p.num_work) return;
     const MsaWorkItem w = p.work[blockIdx.x];
     b = chk(w.batch, 0, p.batch, p.status); head0 = chk(w.head0, 0, p.num_qo_heads, p.status); row0 = w.row0;
     tb = w.kv_tile_begin; te = w.kv_tile_end; split = chk(w.split, 0, p.num_splits, p.status);
     i_base = 0;
+    if constexpr (WIN) skip = w.kv_tile_skip;
     rows_total = min((p.qo_start[b + 1] - p.qo_start[b]) * G, w.row0 + w.num_rows);
   } else {
     const int S = p.num_splits;
@@ -95,6 +98,12 @@ fmha_mma_kernel(const __grid_constant__ MsaFmhaParams p) {
   const int page_base = p.page_size > 0 ? p.kv_page_indptr[b] : 0;
   const int kv_base = p.page_size > 0 ? 0 : p.kv_start[b];
   const int ps = p.page_size;
+
+  [[maybe_unused]] int item_from = 0, item_last = 0;          // windowed: what the item's first and last row see
+  if constexpr (WIN) {
+    item_from = window_first(row0 / G + off, kv_len, p.window);
+    item_last = (rows_total - 1) / G + off;
+  }
 
   float scale_log2 = p.sm_scale * kLog2e;
   if (p.k_scale_head) scale_log2 *= p.k_scale_head[kvh];
@@ -134,7 +143,11 @@ fmha_mma_kernel(const __grid_constant__ MsaFmhaParams p) {
   // ---------------- tile source + loader ----------------
   auto tile_src = [&](int j) -> TileSrc {
     TileSrc s;
-    if (!sparse) { s.pos0 = j * kKvTile; s.valid = true; s.lpage = 0; return s; }
+    if (!sparse) {
+      s.pos0 = (WIN && j >= sink_tiles(p.sink_tokens) ? j + skip : j) * kKvTile;
+      s.valid = true; s.lpage = 0;
+      return s;
+    }
     const int blk = blocks[j];
     s.lpage = blk;
     s.pos0 = blk * kKvTile;
@@ -150,7 +163,9 @@ fmha_mma_kernel(const __grid_constant__ MsaFmhaParams p) {
     for (int c = tid; c < kKvTile * CH_PER_ROW; c += NT) {
       const int r = c / CH_PER_ROW, ch = c % CH_PER_ROW;
       const int pos = s.pos0 + r;
-      const bool ok = s.valid && pos < kv_len;
+      bool ok = s.valid && pos < kv_len;
+      // keys that no row of the item sees are zeros: a weight of 0 does not take a NaN out
+      if constexpr (WIN) ok = ok && pos <= item_last && (pos >= item_from || pos < p.sink_tokens);
       int64_t ko = 0, vo = 0;
       if (ok) {
         if (ps > 0) {
@@ -179,6 +194,7 @@ fmha_mma_kernel(const __grid_constant__ MsaFmhaParams p) {
   // ---------------- per-thread row bookkeeping ----------------
   const int r_lo = wm * 16 + (lane >> 2), r_hi = r_lo + 8;
   int lim[2], gtok[2], headr[2];
+  [[maybe_unused]] int from[2];                 // windowed: first key of the row's window
   bool rowok[2];
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
@@ -188,10 +204,16 @@ fmha_mma_kernel(const __grid_constant__ MsaFmhaParams p) {
     headr[e] = head0 + (rowok[e] ? pr % G : 0);
     gtok[e] = qo_base + i;
     lim[e] = rowok[e] ? min(i + off, kv_len - 1) : -1;   // last visible key position
+    if constexpr (WIN) from[e] = rowok[e] ? window_first(i + off, kv_len, p.window) : 0;
   }
   int warp_min_lim = min(lim[0], lim[1]);
+  [[maybe_unused]] int warp_max_from = 0;
+  if constexpr (WIN) warp_max_from = max(from[0], from[1]);
 #pragma unroll
-  for (int o = 16; o >= 1; o >>= 1) warp_min_lim = min(warp_min_lim, __shfl_xor_sync(0xffffffffu, warp_min_lim, o));
+  for (int o = 16; o >= 1; o >>= 1) {
+    warp_min_lim = min(warp_min_lim, __shfl_xor_sync(0xffffffffu, warp_min_lim, o));
+    if constexpr (WIN) warp_max_from = max(warp_max_from, __shfl_xor_sync(0xffffffffu, warp_max_from, o));
+  }
 
   float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};
   float acc_o[16][4];
@@ -281,6 +303,17 @@ fmha_mma_kernel(const __grid_constant__ MsaFmhaParams p) {
         if (c + 1 > lim[0]) acc_s[n][1] = -INFINITY;
         if (c > lim[1]) acc_s[n][2] = -INFINITY;
         if (c + 1 > lim[1]) acc_s[n][3] = -INFINITY;
+      }
+    }
+    if constexpr (WIN) {
+      if (src.pos0 < warp_max_from) {
+#pragma unroll
+        for (int n = 0; n < NTILE_S; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int c = col0 + n * 8 + (e & 1);
+            if (c < from[e >> 1] && c >= p.sink_tokens) acc_s[n][e] = -INFINITY;
+          }
       }
     }
 
@@ -470,10 +503,10 @@ fmha_mma_kernel(const __grid_constant__ MsaFmhaParams p) {
   }
 }
 
-template <int MW, int NW, bool HAS_O, bool KV8>
+template <int MW, int NW, bool HAS_O, bool KV8, bool WIN>
 int launch_cfg(const MsaFmhaParams& p, int grid, cudaStream_t stream) {
   using C = Cfg<MW, NW, HAS_O, KV8>;
-  auto kern = fmha_mma_kernel<MW, NW, HAS_O, KV8>;
+  auto kern = fmha_mma_kernel<MW, NW, HAS_O, KV8, WIN>;
   static bool attr_done[16] = {};                 // per device
   int dev = 0;
   cudaGetDevice(&dev);
@@ -487,12 +520,12 @@ int launch_cfg(const MsaFmhaParams& p, int grid, cudaStream_t stream) {
   return cudaGetLastError() == cudaSuccess ? MSA_OK : MSA_ERR_LAUNCH;
 }
 
-template <bool HAS_O, bool KV8>
+template <bool HAS_O, bool KV8, bool WIN>
 int launch_bm(const MsaFmhaParams& p, int grid, cudaStream_t stream) {
   switch (p.block_m) {
-    case 16: return launch_cfg<1, 4, HAS_O, KV8>(p, grid, stream);
-    case 64: return launch_cfg<4, 1, HAS_O, KV8>(p, grid, stream);
-    case 128: return launch_cfg<8, 1, HAS_O, KV8>(p, grid, stream);
+    case 16: return launch_cfg<1, 4, HAS_O, KV8, WIN>(p, grid, stream);
+    case 64: return launch_cfg<4, 1, HAS_O, KV8, WIN>(p, grid, stream);
+    case 128: return launch_cfg<8, 1, HAS_O, KV8, WIN>(p, grid, stream);
     default: return MSA_ERR_UNSUPPORTED;
   }
 }
@@ -507,8 +540,9 @@ int fmha_mma_launch(const MsaFmhaParams& p, cudaStream_t stream) {
   if (grid64 <= 0) return MSA_OK;
   if (grid64 > 0x7fffffffLL) return MSA_ERR_TOO_LARGE;
   const int grid = static_cast<int>(grid64);
-  if (has_o) return kv8 ? launch_bm<true, true>(p, grid, stream) : launch_bm<true, false>(p, grid, stream);
-  return kv8 ? launch_bm<false, true>(p, grid, stream) : launch_bm<false, false>(p, grid, stream);
+  if (p.window > 0) return kv8 ? launch_bm<true, true, true>(p, grid, stream) : launch_bm<true, false, true>(p, grid, stream);
+  if (has_o) return kv8 ? launch_bm<true, true, false>(p, grid, stream) : launch_bm<true, false, false>(p, grid, stream);
+  return kv8 ? launch_bm<false, true, false>(p, grid, stream) : launch_bm<false, false, false>(p, grid, stream);
 }
 
 }  // namespace msa

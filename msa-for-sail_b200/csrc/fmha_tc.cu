@@ -774,7 +774,7 @@ int make_tma_map_u8(CUtensorMap* m, const void* base, int rank, const uint64_t* 
 
 // Shapes the tcgen05 kernel takes; everything else runs on the mma.sync kernel.
 int fmha_tc_supported(const MsaFmhaParams& p) {
-  if (p.block_m != 256) return 0;
+  if (p.block_m != 256 || p.window > 0) return 0;
   return 1;
 }
 

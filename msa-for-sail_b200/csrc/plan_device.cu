@@ -94,15 +94,15 @@ __global__ void __launch_bounds__(256) plan_device_kernel(const MsaPlanDeviceArg
       const int row0 = (RT - 1 - rr) * bm_eff;
       const int tokens = a.qo_start ? a.qo_start[b + 1] - a.qo_start[b] : ql;
       const int nrows = max(0, min(bm_eff, tokens * G - row0));
-      long long vis = nrows > 0 ? min(static_cast<long long>(kl), static_cast<long long>((row0 + nrows - 1) / G) + off + 1) : 0;
-      if (vis < 0) vis = 0;
-      const int nt = static_cast<int>((vis + kKvTile - 1) / kKvTile);
+      const long long place = off;
+      const WindowSpan span = window_span(place + row0 / G, place + (row0 + nrows - 1) / G, kl, a.window, a.sink_tokens);
+      const int nt = nrows > 0 ? span.count : 0;
       const int chunk = max(1, (nt + S - 1) / S);
       MsaWorkItem w;
       w.batch = b; w.head0 = g * G; w.row0 = row0;
       w.kv_tile_begin = min(nt, s * chunk);
       w.kv_tile_end = min(nt, (s + 1) * chunk);
-      w.split = s; w.num_rows = nrows; w.reserved = 0;
+      w.split = s; w.num_rows = nrows; w.kv_tile_skip = span.skip;
       a.work[idx] = w;
     }
   }
@@ -133,6 +133,7 @@ extern "C" int msa_plan_device(const MsaPlanDeviceArgs* a, msa_stream_t stream) 
   if (a->pack < 1 || (a->num_qo_heads / a->num_kv_heads) % a->pack || a->pack > a->block_m) return MSA_ERR_BAD_ARG;
   if (a->num_splits < 1 || a->max_total_q < 0 || a->row_tiles < 1) return MSA_ERR_BAD_ARG;
   if (a->token_batch && !a->qo_start) return MSA_ERR_BAD_ARG;
+  if (a->window < 0 || a->sink_tokens < 0 || (a->sink_tokens > 0 && a->window == 0)) return MSA_ERR_BAD_ARG;
   if (a->batch == 0) return MSA_OK;
   msa::NvtxRange range("msa_plan_device");
   return msa::launch_chained(msa::plan_device_kernel, 1, 256, 0, static_cast<cudaStream_t>(stream), *a) == cudaSuccess ? MSA_OK : MSA_ERR_LAUNCH;

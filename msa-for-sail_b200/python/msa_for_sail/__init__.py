@@ -20,9 +20,16 @@ from .cache import (  # noqa: F401
     qk_norm_rope,
     rope_plan,
 )
+from .pages import (  # noqa: F401
+    kv_pages_compact,
+    kv_pages_copy,
+    kv_pages_fork,
+    kv_pages_free,
+)
 
 __all__ = ["fmha_sail_plan", "fmha_sail", "sparse_topk_select", "allocate_graph_workspace",
-           "paged_kv_tables", "rope_plan", "qk_norm_rope", "kv_cache_append", "allocate_kv4_cache", "kv4_read"]
+           "paged_kv_tables", "rope_plan", "qk_norm_rope", "kv_cache_append", "allocate_kv4_cache", "kv4_read",
+           "kv_pages_copy", "kv_pages_fork", "kv_pages_free", "kv_pages_compact"]
 __version__ = "0.1.0"
 
 # TVM-FFI global functions minfer.ops.* (upstream __init__.py:20-78); a no-op without tvm_ffi

@@ -28,7 +28,7 @@ _f32 = ctypes.c_float
 
 class MsaWorkItem(ctypes.Structure):
     _fields_ = [("batch", _i32), ("head0", _i32), ("row0", _i32), ("kv_tile_begin", _i32),
-                ("kv_tile_end", _i32), ("split", _i32), ("num_rows", _i32), ("reserved", _i32)]
+                ("kv_tile_end", _i32), ("split", _i32), ("num_rows", _i32), ("kv_tile_skip", _i32)]
 
 
 class MsaFmhaParams(ctypes.Structure):
@@ -48,14 +48,14 @@ class MsaFmhaParams(ctypes.Structure):
         ("num_work", _i32), ("block_m", _i32), ("pack", _i32), ("page_size", _i32),
         ("kv_block_num", _i32), ("num_splits", _i32), ("max_k_tiles", _i32), ("num_logical_pages", _i32), ("decode_rows", _i32),
         ("q_dtype", _i32), ("kv_dtype", _i32), ("max_score_dtype", _i32), ("flags", _i32),
-        ("sm_scale", _f32), ("out_scale", _f32), ("num_page_entries", _i32),
+        ("sm_scale", _f32), ("out_scale", _f32), ("num_page_entries", _i32), ("window", _i32), ("sink_tokens", _i32),
     ]
 
 
 class MsaPlanArgs(ctypes.Structure):
     _fields_ = [("qo_len", _p), ("kv_len", _p), ("qo_offset", _p), ("batch", _i32),
                 ("num_qo_heads", _i32), ("num_kv_heads", _i32), ("block_m", _i32), ("pack", _i32),
-                ("num_splits", _i32), ("num_sms", _i32), ("ctas_per_sm", _i32)]
+                ("num_splits", _i32), ("num_sms", _i32), ("ctas_per_sm", _i32), ("window", _i32), ("sink_tokens", _i32)]
 
 
 class MsaPlanDeviceArgs(ctypes.Structure):
@@ -64,7 +64,7 @@ class MsaPlanDeviceArgs(ctypes.Structure):
                 ("splits_per_row", _p), ("work", _p), ("batch", _i32), ("num_qo_heads", _i32),
                 ("num_kv_heads", _i32), ("block_m", _i32), ("pack", _i32), ("num_splits", _i32),
                 ("page_size", _i32), ("causal", _i32), ("noncausal_offset", _i32), ("max_total_q", _i32),
-                ("row_tiles", _i32)]
+                ("row_tiles", _i32), ("window", _i32), ("sink_tokens", _i32)]
 
 
 class MsaNormRopeArgs(ctypes.Structure):
@@ -95,6 +95,32 @@ class MsaPageTablesArgs(ctypes.Structure):
                 ("table_width", _i32), ("page_size", _i32), ("max_total_q", _i32), ("max_total_pages", _i32), ("free_capacity", _i32)]
 
 
+class MsaPageCache(ctypes.Structure):
+    _fields_ = [("base", _p), ("stride_page", _i64), ("stride_part", _i64), ("parts", _i32), ("part_bytes", _i32), ("token_bytes", _i32), ("reserved", _i32)]
+
+
+class MsaPagesCopyArgs(ctypes.Structure):
+    _fields_ = [("caches", _p), ("src", _p), ("dst", _p), ("status", _p), ("num_caches", _i32), ("count", _i32), ("num_pages", _i32), ("page_size", _i32)]
+
+
+class MsaPagesForkArgs(ctypes.Structure):
+    _fields_ = [("caches", _p), ("block_table", _p), ("num_held", _p), ("kv_len", _p), ("parents", _p), ("children", _p), ("free_pages", _p), ("num_free", _p),
+                ("shares", _p), ("num_missing", _p), ("workspace", _p), ("table_stride", _i64), ("num_caches", _i32), ("count", _i32), ("num_pages", _i32),
+                ("page_size", _i32), ("batch", _i32), ("table_width", _i32), ("free_capacity", _i32)]
+
+
+class MsaPagesFreeArgs(ctypes.Structure):
+    _fields_ = [("block_table", _p), ("num_held", _p), ("kv_len", _p), ("free_pages", _p), ("num_free", _p), ("shares", _p), ("num_freed", _p),
+                ("workspace", _p), ("table_stride", _i64), ("batch", _i32), ("table_width", _i32), ("page_size", _i32), ("free_capacity", _i32),
+                ("num_pages", _i32), ("window", _i32), ("sink_tokens", _i32)]
+
+
+class MsaPagesCompactArgs(ctypes.Structure):
+    _fields_ = [("caches", _p), ("block_table", _p), ("num_held", _p), ("free_pages", _p), ("num_free", _p), ("shares", _p), ("src", _p), ("dst", _p),
+                ("num_moved", _p), ("workspace", _p), ("table_stride", _i64), ("num_caches", _i32), ("num_pages", _i32), ("page_size", _i32),
+                ("batch", _i32), ("table_width", _i32), ("free_capacity", _i32)]
+
+
 def _packer(struct_type):
     """A call that takes the values of all fields in order (0 for NULL) and gives the structure: a third of the time of the constructor."""
     codes = {_p: "Q", _i64: "q", _i32: "i", _f32: "f"}
@@ -104,13 +130,15 @@ def _packer(struct_type):
 
 
 norm_rope_args, kv4_read_args, page_tables_args = map(_packer, (MsaNormRopeArgs, MsaKv4ReadArgs, MsaPageTablesArgs))
+pages_copy_args, pages_fork_args, pages_free_args, pages_compact_args = map(_packer, (MsaPagesCopyArgs, MsaPagesForkArgs, MsaPagesFreeArgs, MsaPagesCompactArgs))
 
 
 #: every symbol include/msa_b200.h declares
 EXPORTS = ("msa_fmha_fwd", "msa_lse_merge", "msa_topk_select", "msa_plan_dense",
            "msa_status_string", "msa_build_arch", "msa_sizeof", "msa_fmha_fwd_split_static",
            "msa_sparse_workspace_bytes", "msa_plan_device", "msa_lse_merge_ex", "msa_lse_merge_many", "msa_norm_rope", "msa_kv4_read",
-           "msa_page_tables", "msa_page_tables_workspace_bytes")
+           "msa_page_tables", "msa_page_tables_workspace_bytes", "msa_pages_copy", "msa_pages_fork", "msa_pages_fork_workspace_bytes",
+           "msa_pages_free", "msa_pages_free_workspace_bytes", "msa_pages_compact", "msa_pages_compact_workspace_bytes")
 
 
 def _load():
@@ -125,7 +153,8 @@ def _load():
     lib.msa_sizeof.argtypes = [ctypes.c_int]
     lib.msa_sizeof.restype = ctypes.c_int
     for which, st in ((0, MsaFmhaParams), (1, MsaWorkItem), (2, MsaPlanArgs), (3, MsaPlanDeviceArgs), (4, MsaNormRopeArgs),
-                      (5, MsaKv4ReadArgs), (6, MsaPageTablesArgs)):
+                      (5, MsaKv4ReadArgs), (6, MsaPageTablesArgs), (7, MsaPageCache), (8, MsaPagesCopyArgs), (9, MsaPagesForkArgs),
+                      (10, MsaPagesFreeArgs), (11, MsaPagesCompactArgs)):
         if lib.msa_sizeof(which) != ctypes.sizeof(st):
             raise ImportError(
                 f"ABI mismatch for {st.__name__}: library {lib.msa_sizeof(which)} bytes, "
@@ -157,6 +186,12 @@ def _load():
     lib.msa_page_tables.restype = ctypes.c_int
     lib.msa_page_tables_workspace_bytes.argtypes = [_i32]
     lib.msa_page_tables_workspace_bytes.restype = _i64
+    for name, st, sizes in (("copy", MsaPagesCopyArgs, 0), ("fork", MsaPagesForkArgs, 2), ("free", MsaPagesFreeArgs, 2), ("compact", MsaPagesCompactArgs, 1)):
+        fn = getattr(lib, "msa_pages_" + name)
+        fn.argtypes, fn.restype = [ctypes.POINTER(st), _p], ctypes.c_int
+        if sizes:
+            fn = getattr(lib, f"msa_pages_{name}_workspace_bytes")
+            fn.argtypes, fn.restype = [_i32] * sizes, _i64
     lib.msa_fmha_fwd_split_static.argtypes = [ctypes.POINTER(MsaFmhaParams), _p, _p]
     lib.msa_fmha_fwd_split_static.restype = ctypes.c_int
     return lib

@@ -184,6 +184,28 @@ def _block_m(rows):
     return 16 if rows <= 16 else (64 if rows <= 64 else 128)
 
 
+def _check_window(window_size, num_sink_tokens, causal, output_maxscore, kv_block_num, use_kv4_cache):
+    """(window, sink tokens) of a plan, (0, 0) for none."""
+    window, sinks = -1 if window_size is None else int(window_size), int(num_sink_tokens)
+    if window == 0 or window < -1 or window > (1 << 31) - 1:
+        raise ValueError(f"window_size must be -1 (no window) or from 1 to 2^31 - 1, got {window_size}")
+    if sinks < 0 or sinks > (1 << 31) - 1:
+        raise ValueError(f"num_sink_tokens must be from 0 to 2^31 - 1, got {num_sink_tokens}")
+    if window == -1:
+        if sinks:
+            raise ValueError("num_sink_tokens belongs to a window_size")
+        return 0, 0
+    if not causal:
+        raise ValueError("window_size requires causal=True: the window ends at the query's own place")
+    if output_maxscore:
+        raise ValueError("window_size computes O only: plan it without output_maxscore")
+    if kv_block_num > 0:
+        raise ValueError("window_size and a selection of pages (kv_block_num) exclude each other")
+    if use_kv4_cache:
+        raise ValueError("window_size needs a bfloat16 or float8_e4m3fn cache")
+    return window, sinks
+
+
 class PlanInfo(dict):
     """Execution plan returned by the planner; pass it unchanged to ``fmha_sail``."""
 
@@ -302,6 +324,8 @@ def _fmha_sail_plan(
     qo_len_uniform_override: Optional[bool] = None,
     max_kv_len_override: int = -1,
     use_kv4_cache: bool = False,
+    window_size: Optional[int] = -1,
+    num_sink_tokens: int = 0,
 ):
     """Internal planner (upstream ``_fmha_sail_plan``, api.py:889-1217).
 
@@ -310,6 +334,7 @@ def _fmha_sail_plan(
     metadata tensors (no buffer is shared between two live plans)."""
     device = torch.cuda.current_device() if device is None else device
     dev = torch.device("cuda", device) if isinstance(device, int) else torch.device(device)
+    window = _check_window(window_size, num_sink_tokens, causal, output_maxscore, kv_block_num, use_kv4_cache)
 
     if graph_safe:
         if max_qo_len_override <= 0:
@@ -338,7 +363,7 @@ def _fmha_sail_plan(
             return _fmha_sail_plan_device(
                 qo_segment_lens, kv_segment_lens, num_qo_heads, hkv_, qo_offset, num_kv_splits, page_size,
                 output_maxscore, kv_block_num, usable_SM_count, causal, use_fp8_kvcache, dev, given_workspace,
-                max_total_q, max_qo_len_override, bool(qo_len_uniform_override), max_kv_len_override, use_kv4_cache)
+                max_total_q, max_qo_len_override, bool(qo_len_uniform_override), max_kv_len_override, use_kv4_cache, window)
         # host-resident lengths: planned on the host below, which reads them
 
     qo_lens = _to_int_list(qo_segment_lens)
@@ -429,7 +454,7 @@ def _fmha_sail_plan(
         if pack == 1 and max_qo > 128 and page_size in (-1, 0, 128):
             args_tc = _lib.MsaPlanArgs(
                 a_q.ctypes.data, a_k.ctypes.data, a_o.ctypes.data, batch, num_qo_heads, hkv, 256, 1,
-                1, num_sms, 0)
+                1, num_sms, 0, *window)
             cap_tc = max(16, (total_q // 256 + batch) * num_qo_heads)
             host_tc = np.empty((cap_tc, 8), np.int32)
             n_tc = _lib.check(_lib.lib.msa_plan_dense(ctypes.byref(args_tc), host_tc.ctypes.data, cap_tc,
@@ -443,7 +468,7 @@ def _fmha_sail_plan(
         for ctas in (shared, -1):
             args = _lib.MsaPlanArgs(
                 a_q.ctypes.data, a_k.ctypes.data, a_o.ctypes.data, batch, num_qo_heads, hkv, block_m, pack,
-                num_kv_splits if num_kv_splits >= 1 else -128, num_sms, ctas)
+                num_kv_splits if num_kv_splits >= 1 else -128, num_sms, ctas, *window)
             cap = 1024
             spr = np.ones(max(1, total_q), np.int32)
             max_splits = _lib._i32(1)
@@ -503,6 +528,7 @@ def _fmha_sail_plan(
         "total_qo_len": total_q,
         "batch_size": batch,
         "causal": causal,
+        "window": window,
         "_host": {"qo_lens": qo_lens, "kv_lens": kv_lens, "qo_offset": offs},
     })
     return info
@@ -510,7 +536,8 @@ def _fmha_sail_plan(
 
 def _fmha_sail_plan_device(qo_segment_lens, kv_segment_lens, num_qo_heads, hkv, qo_offset, num_kv_splits,
                            page_size, output_maxscore, kv_block_num, usable_SM_count, causal, use_fp8_kvcache,
-                           dev, given_workspace, max_total_q, max_qo, qo_len_uniform, max_kv_len_override, use_kv4_cache=False):
+                           dev, given_workspace, max_total_q, max_qo, qo_len_uniform, max_kv_len_override, use_kv4_cache=False,
+                           window=(0, 0)):
     """Graph-safe planner (upstream graph_safe mode, api.py:916-941): the lengths stay on the GPU.
 
     Everything that sizes a launch comes from the arguments -- batch, ``max_qo_len_override`` (the
@@ -577,6 +604,7 @@ def _fmha_sail_plan_device(qo_segment_lens, kv_segment_lens, num_qo_heads, hkv, 
     a.block_m, a.pack, a.num_splits = block_m, pack, splits
     a.page_size, a.causal, a.noncausal_offset = page_size, int(bool(causal)), max(0, max_kv)
     a.max_total_q, a.row_tiles = max_total_q, row_tiles
+    a.window, a.sink_tokens = window
     _lib.check(_lib.lib.msa_plan_device(ctypes.byref(a), _stream()), "msa_plan_device")
     if want_tc:
         t = _lib.MsaPlanDeviceArgs()
@@ -585,6 +613,7 @@ def _fmha_sail_plan_device(qo_segment_lens, kv_segment_lens, num_qo_heads, hkv, 
         t.batch, t.num_qo_heads, t.num_kv_heads = batch, num_qo_heads, hkv
         t.block_m, t.pack, t.num_splits, t.row_tiles = 256, 1, 1, tc_tiles
         t.page_size, t.causal, t.noncausal_offset, t.max_total_q = page_size, a.causal, a.noncausal_offset, max_total_q
+        t.window, t.sink_tokens = window
         _lib.check(_lib.lib.msa_plan_device(ctypes.byref(t), _stream()), "msa_plan_device")
 
     max_k_tiles = math.ceil(math.ceil(max_kv / KV_TILE) / 128) * 128 if output_maxscore else -1
@@ -597,7 +626,7 @@ def _fmha_sail_plan_device(qo_segment_lens, kv_segment_lens, num_qo_heads, hkv, 
         "orig_num_qo_heads": num_qo_heads, "num_kv_heads": hkv, "qo_len_uniform": qo_len_uniform,
         "graph_safe": True, "page_size": page_size, "kv_block_num": kv_block_num if is_sparse else -1,
         "is_sparse": is_sparse, "total_qo_len": max_total_q, "batch_size": batch, "causal": causal,
-        "_host": None,
+        "window": window, "_host": None,
     })
     return info
 
@@ -840,6 +869,9 @@ def _fmha_sail(
     if (plan_page > 0) != is_paged:
         raise ValueError("plan page_size does not match the K/V layout (kv_indices given?)")
 
+    window = plan["window"]
+    if window[0] and q_offset_override is not None:
+        raise ValueError("a plan with window_size has its offsets (qo_offset): q_offset_override cannot change them")
     qo_offset = plan["qo_offset"] if q_offset_override is None else q_offset_override
     if isinstance(qo_offset, int):
         if plan.get("graph_safe", False):
@@ -921,7 +953,7 @@ def _fmha_sail(
     p.kv_len = plan["kv_segment_lens"].data_ptr()
     p.qo_offset = qo_offset.data_ptr()
     splits = plan["num_kv_splits"]
-    use_tc = (plan.get("work_tc") is not None and kv_block_indexes is None
+    use_tc = (plan.get("work_tc") is not None and kv_block_indexes is None and not window[0]
               and q.dtype == k.dtype and k.dtype in (torch.bfloat16, torch.float8_e4m3fn)
               and page_size in (0, 128) and _USE_TC and (plan["tc_preferred"] or _FORCE_TC))
     use_split = output_o and splits > 1 and not use_tc
@@ -991,11 +1023,12 @@ def _fmha_sail(
     p.status = _status_ptr(q.device)
     rows = plan["max_qo_len"] * plan["pack_factor"] if kv_block_indexes is None else plan["pack_factor"]
     dt_ok = (q.dtype == torch.bfloat16 and k.dtype == torch.bfloat16) or k.dtype == torch.float8_e4m3fn
-    if (_USE_DECODE_TC and not use_tc and output_o != (max_score is not None) and dt_ok
+    if (_USE_DECODE_TC and not use_tc and not window[0] and output_o != (max_score is not None) and dt_ok
             and page_size == 128 and 0 < rows <= 128
             and plan["pack_factor"] == num_qo_heads // num_kv_heads and 128 % plan["pack_factor"] == 0):
         p.decode_rows = rows
     p.q_dtype, p.kv_dtype = _dt_code(q.dtype), _dt_code(k.dtype)
+    p.window, p.sink_tokens = window
     p.flags = (FLAG_OUT_O if output_o else 0) | (FLAG_OUT_SCORE if max_score is not None else 0) | \
               (FLAG_SPARSE if kv_block_indexes is not None else 0)
     p.sm_scale = float(q_s * k_s * sm_scale)
@@ -1031,6 +1064,8 @@ def _fmha_sail_kv4(q, k, v, plan, kv_indices, kv_block_indexes, q_offset_overrid
     if q.dtype not in (torch.bfloat16, torch.float8_e4m3fn):
         raise ValueError(f"fmha_sail on a 4-bit cache requires q in bfloat16 or float8_e4m3fn, got {q.dtype}")
     nnz_qo, num_qo_heads, _ = q.shape
+    if plan["window"][0]:
+        raise ValueError("a plan with window_size needs a bfloat16 or float8_e4m3fn cache")
     if plan.get("page_size", -1) != cache.KV4_TILE:
         raise ValueError(f"a 4-bit cache needs a plan with page_size={cache.KV4_TILE}")
     assert output_o or output_maxscore
