@@ -45,6 +45,11 @@ __device__ __forceinline__ float2 e4m3x2_as_float2(uint16_t x) {
   return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
 
+// What two values leave that were rounded to r, as e4m3 (low 16 bits).
+__device__ __forceinline__ uint32_t e4m3_rest(float a, float b, float2 r) {
+  return __nv_cvt_float2_to_fp8x2(make_float2(a - r.x, b - r.y), __NV_SATFINITE, __NV_E4M3);
+}
+
 constexpr int BM = 128, BN = 128;
 constexpr int SUB_BYTES = BM * 128;             // one [128 rows][128 bytes] swizzled sub-tile
 constexpr int NTHREADS = 224;
@@ -59,8 +64,9 @@ constexpr int STAGE_LD = kHeadDim + 4;          // floats per staged O row (padd
 // softmax warp can finish its last tile while P_{n-2} V is still waiting for its V tile, i.e. two phases ahead
 // of the barrier, where a parity wait for phase n - 1 reads phase n - 3 as "done".  O_DONE completes once, after
 // the last P V.
+// V_FIX + 1, + 2: windowed items only.
 enum Bar { Q_FULL = 0, K_FULL = 1, K_EMPTY = 7, V_FULL = 13, V_EMPTY = 19, S_FULL = 25, P_FULL = 27, PV_DONE = 29,
-           V_FIX = 30, O_DONE = 31, NUM_BARS = 32 };
+           O_DONE = 30, V_FIX = 31, NUM_BARS = 34 };
 
 #ifdef MSA_DEBUG_HOOKS
 // diagnostic timeline: when set, every CTA records 16 words (see msa_debug_decode_trace)
@@ -84,21 +90,30 @@ __device__ __forceinline__ unsigned long long global_ns() {
 //         half pages (64 keys): two 64-column S buffers and O fit the 256 columns, so Q K^T of tile
 //         j + 1 still overlaps the softmax of tile j.  The barriers live in rows 16-31 of the Q
 //         tile, which no real row uses.
-template <bool F8, bool QUAD>
+//   WIN   rows see a window and the first keys only; tiles that no row sees are not loaded.
+//   F8 && WIN ("pair"): Q and P are pairs of e4m3 values, x = hi + lo with lo = e4m3(x - hi), both multiplied into the same
+//         accumulator: 8 bits where one value has 4, for MMAs that have nothing else to do.  (A single value puts 2.6 % of noise on
+//         each weight: with a window there are few enough that it shows.)  Q_lo: rows 16-31 of each quadrant of the Q tile (dual),
+//         whose descriptor starts 2 KB later, or a tile of its own.
+template <bool F8, bool QUAD, bool WIN = false>
 struct Cfg {
   static constexpr bool DUAL = F8 && QUAD;
+  static constexpr bool PAIR = F8 && WIN;
   static constexpr int TK = DUAL ? 64 : 128;              // keys per tile
   static constexpr int NSUB = F8 ? 1 : 2;                 // 128-byte-wide sub-tiles per tile
   static constexpr int TILE_BYTES = NSUB * TK * 128;
   static constexpr int RING_BYTES = DUAL ? 48 * 1024 : 96 * 1024;
   static constexpr int STAGES = RING_BYTES / TILE_BYTES;  // bf16 3, e4m3 6 (dual: 6 half pages)
+  static constexpr int V_STAGES = DUAL && WIN ? STAGES - 1 : STAGES;      // room for the barriers, see below
   static constexpr int OFF_Q = 0;
-  // dual: rows 112-127 of the Q tile are never real rows, the K ring may start there
-  static constexpr int OFF_K = DUAL ? SUB_BYTES - 2048 : 2 * SUB_BYTES;
+  [[maybe_unused]] static constexpr int OFF_Q_LO = DUAL ? 2048 : SUB_BYTES;
+  // dual: rows 112-127 of the Q tile are never real rows (pairs: of Q_hi), the K ring may start there
+  static constexpr int OFF_K = DUAL && !PAIR ? SUB_BYTES - 2048 : DUAL ? SUB_BYTES : 2 * SUB_BYTES;
   static constexpr int OFF_V = OFF_K + RING_BYTES;
-  static constexpr int END = OFF_V + RING_BYTES;
-  static constexpr int OFF_BAR = DUAL ? 2048 : END;
-  static constexpr int SMEM_BYTES = (DUAL ? END : END + 1024) + 1024;   // + slack to align the base to 1 KB
+  static constexpr int END = OFF_V + V_STAGES * TILE_BYTES;
+  static constexpr int OFF_BAR = DUAL && !PAIR ? 2048 : END;
+  static constexpr int SMEM_BYTES = (DUAL && !PAIR ? END : END + 1024) + 1024;   // + slack to align the base to 1 KB
+  static_assert(!DUAL || 2 * (SMEM_BYTES + 1024) <= 228 * 1024, "two CTAs fit an SM");
   static constexpr int NBUF = 2;                          // S buffers in TMEM
   static constexpr int TMEM_COLS = DUAL ? 256 : 512;
   static constexpr int O_COL = NBUF * TK;
@@ -107,12 +122,13 @@ struct Cfg {
   static_assert(4 * QUAD_MAX_ROWS * STAGE_LD * 4 <= RING_BYTES, "O staging fits the K ring");
 };
 
-template <bool F8, bool QUAD>
-__global__ void __launch_bounds__(NTHREADS, (Cfg<F8, QUAD>::MIN_CTAS))
+template <bool F8, bool QUAD, bool WIN>
+__global__ void __launch_bounds__(NTHREADS, (Cfg<F8, QUAD, WIN>::MIN_CTAS))
 decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant__ CUtensorMap tm_q,
                  const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v) {
-  using C = Cfg<F8, QUAD>;
-  constexpr int NSUB = C::NSUB, TILE_BYTES = C::TILE_BYTES, STAGES = C::STAGES, NBUF = C::NBUF, TK = C::TK;
+  using C = Cfg<F8, QUAD, WIN>;
+  constexpr int NSUB = C::NSUB, TILE_BYTES = C::TILE_BYTES, STAGES = C::STAGES, V_STAGES = C::V_STAGES, NBUF = C::NBUF, TK = C::TK;
+  constexpr bool PAIR = C::PAIR;
   constexpr int UPP = BN / TK;                      // tiles per page
   constexpr int OFF_Q = C::OFF_Q, OFF_K = C::OFF_K, OFF_V = C::OFF_V, OFF_BAR = C::OFF_BAR;
   extern __shared__ unsigned char smem_raw[];
@@ -144,14 +160,15 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
   constexpr unsigned long long* trace = nullptr;   // the `if (trace)` records below compile to nothing
   constexpr long long clk0 = 0;
 #endif
-  const bool sparse = (p.flags & MSA_FLAG_SPARSE) != 0;
-  const bool has_o = (p.flags & MSA_FLAG_OUT_O) != 0;   // false: score-only pass (no V, no P, no O)
+  const bool sparse = !WIN && (p.flags & MSA_FLAG_SPARSE) != 0;
+  const bool has_o = WIN || (p.flags & MSA_FLAG_OUT_O) != 0;   // false: score-only pass (no V, no P, no O)
   const int G = p.pack;
   const int h_r = p.num_qo_heads / p.num_kv_heads;
 
   chain_begin();
   // ---------------- work item ----------------
   int b, head0, tb, te, split, i_base, ntok;
+  [[maybe_unused]] int skip = 0;            // windowed: pages left out behind those of the sinks
   int blk_first = -1;                       // sparse: this lane's entry of the selected-page list, fetched early
   const int32_t* blocks = nullptr;
   if (!sparse) {
@@ -159,6 +176,7 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
     b = chk(w.batch, 0, p.batch, p.status); head0 = chk(w.head0, 0, p.num_qo_heads, p.status);
     tb = w.kv_tile_begin; te = w.kv_tile_end; split = chk(w.split, 0, p.num_splits, p.status);
     i_base = 0;
+    if constexpr (WIN) skip = w.kv_tile_skip;
     // (lengths on the device may outgrow the rows that the plan and this kernel's tile were made for; G divides 128)
     ntok = min(p.qo_start[b + 1] - p.qo_start[b], p.decode_rows >> (__ffs(G) - 1));
   } else {
@@ -184,6 +202,22 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
   const int kv_len = p.kv_len[b];
   const int off = p.qo_offset[b];
   const int page_base = p.kv_page_indptr[b];
+  // Windowed: the item's tiles of TK keys are numbered without those that no row sees (a half page next to a page's visible half, too):
+  // number t stands for tile t of the keys below sink_t, for t + skip_t from there on.  first_key: of the first row's window, end_key: behind
+  // what the last row sees.
+  [[maybe_unused]] int first_key = 0, end_key = 0, sink_t = 0, skip_t = 0, t_begin = 0, t_end = 0;
+  [[maybe_unused]] auto real_page = [&](int t) { return t < sink_tiles(p.sink_tokens) ? t : t + skip; };
+  if constexpr (WIN) {
+    first_key = window_first(off, kv_len, p.window);
+    end_key = max(0, min(kv_len, off + ntok));
+    sink_t = p.sink_tokens / TK + (p.sink_tokens % TK != 0);
+    skip_t = max(0, first_key / TK - sink_t);
+    auto number = [&](int t) { return t < sink_t ? t : max(sink_t, t - skip_t); };
+    if (tb < te) {
+      t_begin = number(real_page(tb) * UPP);
+      t_end = number(min(real_page(te - 1) * UPP + UPP, (end_key + TK - 1) / TK));
+    }
+  }
   const int n_active_warps = QUAD ? 4 : (nrows + 31) / 32;
 
   // a timeout reported earlier on this device (status word not cleared yet): do not start.  Read by
@@ -196,6 +230,7 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
       mbar_init(bar(K_FULL + s), 1);  mbar_init(bar(K_EMPTY + s), 1);
       mbar_init(bar(V_FULL + s), 1);  mbar_init(bar(V_EMPTY + s), 1);
     }
+    if constexpr (WIN) { mbar_init(bar(V_FIX + 1), 1); mbar_init(bar(V_FIX + 2), 1); }
     for (int s = 0; s < NBUF; ++s) { mbar_init(bar(S_FULL + s), 1); mbar_init(bar(P_FULL + s), 32 * n_active_warps); }
     mbar_init(bar(PV_DONE), 1);
     mbar_init(bar(O_DONE), 1);
@@ -231,6 +266,8 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
         n += __shfl_sync(0xffffffffu, incl, 31);
       }
       if (lane == 0) *s_ntiles = min(n, MAX_SPARSE_TILES * UPP);
+    } else if (WIN) {
+      if (lane == 0) *s_ntiles = max(0, t_end - t_begin);
     } else if (lane == 0) {
       // [tb, te) pages of the sequence, up to the last tile that holds a key
       const int keys = min(te * BN, kv_len) - tb * BN;
@@ -247,7 +284,15 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
   const uint32_t tmem = *tmem_slot;
   const int n_tiles = *s_ntiles;
   if (trace) trace[3] = clock64() - clk0;
-  auto tile_key0 = [&](int j) -> int { return (sparse ? s_tiles[j] : tb * UPP + j) * TK; };   // position of the first key of tile j
+  auto tile_key0 = [&](int j) -> int {                       // position of the first key of tile j
+    if constexpr (WIN) return (t_begin + j < sink_t ? t_begin + j : t_begin + j + skip_t) * TK;
+    return (sparse ? s_tiles[j] : tb * UPP + j) * TK;
+  };
+  // windowed: whether the tile from key0 on holds a key that no row sees.  Those are in three tiles at most: the last of the sinks, the first
+  // of the window, the last.
+  [[maybe_unused]] auto has_unseen = [&](int key0) -> bool {
+    return key0 + TK > end_key || (key0 < first_key && key0 + TK > p.sink_tokens);
+  };
 
   const bool run = *skip_flag == 0;
   if (!run) {
@@ -275,24 +320,38 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
     // page-table entries: one per lane, 32 pages at a time, the next batch already in flight
     int phys_cur = 0, phys_next = 0;
     const int n_pages = (n_tiles + UPP - 1) / UPP;
-    if (!sparse) {
+    [[maybe_unused]] int entry0 = tb;                          // windowed: page (numbered as the item's tiles) that lane 0 has in phys_cur
+    if constexpr (WIN) {
+      phys_cur = tb + lane < te ? page_entry(p, page_base + real_page(tb + lane)) : 0;
+      phys_next = tb + 32 + lane < te ? page_entry(p, page_base + real_page(tb + 32 + lane)) : 0;
+    } else if (!sparse) {
       phys_cur = lane < n_pages ? page_entry(p, page_base + tb + lane) : 0;
       phys_next = 32 + lane < n_pages ? page_entry(p, page_base + tb + 32 + lane) : 0;
     }
+    [[maybe_unused]] int fixes = 0;
     uint32_t fix_phase = 0;
     bool alive = do_k || do_v;
     for (int j = 0; j < n_tiles && alive; ++j) {
       const int st = j % STAGES;
       const int key0 = tile_key0(j);
       const int row_in_page = key0 % BN;
-      const int pg = j / UPP;                                // dense: page index within this item
-      if (!sparse && j > 0 && (j % (32 * UPP)) == 0) {
+      int pg = j / UPP;                                      // dense: page index within this item
+      if constexpr (WIN) {
+        pg = key0 / BN;
+        if (pg >= sink_tiles(p.sink_tokens)) pg -= skip;
+        pg -= entry0;
+        if (pg >= 32) {                                      // (tiles come in order: the next batch begins here)
+          phys_cur = phys_next;
+          entry0 += 32; pg -= 32;
+          phys_next = entry0 + 32 + lane < te ? page_entry(p, page_base + real_page(entry0 + 32 + lane)) : 0;
+        }
+      } else if (!sparse && j > 0 && (j % (32 * UPP)) == 0) {
         phys_cur = phys_next;
         phys_next = pg + 32 + lane < n_pages ? page_entry(p, page_base + tb + pg + 32 + lane) : 0;
       }
       const int phys = sparse ? s_phys[j] : __shfl_sync(0xffffffffu, phys_cur, pg & 31);
       const int valid_rows = min(TK, kv_len - key0);
-      const bool fix = valid_rows < TK;
+      const bool fix = WIN ? has_unseen(key0) : valid_rows < TK;
       if (do_k) {
         alive = mbar_wait_warp(bar(K_EMPTY + st), ((j / STAGES) & 1) ^ 1, abort_flag);
         if (!alive) break;
@@ -306,16 +365,18 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
         __syncwarp();
       }
       if (!do_v) continue;
-      alive = mbar_wait_warp(bar(V_EMPTY + st), ((j / STAGES) & 1) ^ 1, abort_flag);
+      const int vst = j % V_STAGES;
+      alive = mbar_wait_warp(bar(V_EMPTY + vst), ((j / V_STAGES) & 1) ^ 1, abort_flag);
       if (!alive) break;
       if (elect_one()) {
-        const uint32_t vbar = fix ? bar(V_FIX) : bar(V_FULL + st);
+        const uint32_t vbar = fix ? bar(V_FIX + (WIN ? fixes : 0)) : bar(V_FULL + vst);
         mbar_arrive_expect_tx(vbar, TILE_BYTES);
 #pragma unroll
         for (int hlf = 0; hlf < NSUB; ++hlf)
-          tma_load_4d(smem_base + OFF_V + st * TILE_BYTES + hlf * SUB_BYTES, &tm_v, vbar, hlf * SUB_ELEMS, row_in_page, kvh, phys);
+          tma_load_4d(smem_base + OFF_V + vst * TILE_BYTES + hlf * SUB_BYTES, &tm_v, vbar, hlf * SUB_ELEMS, row_in_page, kvh, phys);
       }
       __syncwarp();
+      if constexpr (WIN) { fixes += fix; continue; }         // the other warp's
       if (fix) {                                             // rows past kv_len must read as 0 in V
         alive = mbar_wait_warp(bar(V_FIX), fix_phase, abort_flag);
         fix_phase ^= 1;
@@ -329,6 +390,27 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
           __syncwarp();
           if (lane == 0) mbar_arrive(bar(V_FULL + st));
         }
+      }
+    }
+    if constexpr (WIN) {
+      // Keys that no row sees read as 0 in V: the weight of 0 that they have does not take a NaN out.  The V warp, which has
+      // nothing to load here, sees to it while the loads go on.
+      bool up = warp == V_PRODUCER_WARP;
+      for (int j = 0; j < n_tiles && up; ++j) {
+        const int key0 = tile_key0(j);
+        if (!has_unseen(key0)) continue;
+        up = mbar_wait_warp(bar(V_FIX + fixes), 0, abort_flag, kSpinLimit * static_cast<uint64_t>(n_tiles));
+        ++fixes;
+        if (!up) break;
+        unsigned char* vt = smem_gen + OFF_V + (j % V_STAGES) * TILE_BYTES;
+        for (int c = lane; c < TK * 8 * NSUB; c += 32) {
+          const int r = c / (8 * NSUB), ch = c % (8 * NSUB), key = key0 + r;
+          if (key >= end_key || (key < first_key && key >= p.sink_tokens))
+            *reinterpret_cast<uint4*>(vt + (ch >> 3) * SUB_BYTES + r * 128 + (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(V_FULL + j % V_STAGES));
       }
     }
   } else if (warp == MMA_WARP) {
@@ -349,14 +431,23 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
         if constexpr (F8) mma_ss_f8(sbuf(j), dk_hi | ((qa + o) & 0x3FFF), dk_hi | ((ka + o) & 0x3FFF), IDESC_QK, k > 0);
         else mma_ss(sbuf(j), dk_hi | ((qa + o) & 0x3FFF), dk_hi | ((ka + o) & 0x3FFF), IDESC_QK, k > 0);
       }
+      if constexpr (PAIR) {
+        if (p.q_dtype == MSA_DT_BF16) {
+          const uint32_t ql = (smem_base + C::OFF_Q_LO) >> 4;
+#pragma unroll
+          for (int k = 0; k < KSTEPS; ++k)
+            mma_ss_f8(sbuf(j), dk_hi | ((ql + 2 * k) & 0x3FFF), dk_hi | ((ka + 2 * k) & 0x3FFF), IDESC_QK, 1u);
+        }
+      }
     };
     auto issue_pv = [&](int j) {
-      const uint32_t va = (smem_base + OFF_V + (j % STAGES) * TILE_BYTES) >> 4;
+      const uint32_t va = (smem_base + OFF_V + (j % V_STAGES) * TILE_BYTES) >> 4;
 #pragma unroll
       for (int k = 0; k < PV_STEPS; ++k) {              // P: 8 TMEM columns per MMA in both formats
         const uint64_t vd = dv_hi | ((va + k * (V_KSTEP >> 4)) & 0x3FFF);
         if constexpr (F8) mma_ts_f8(tmem + C::O_COL, sbuf(j) + k * 8, vd, IDESC_PV, (j > 0 || k > 0) ? 1u : 0u);
         else mma_ts(tmem + C::O_COL, sbuf(j) + k * 8, vd, IDESC_PV, (j > 0 || k > 0) ? 1u : 0u);
+        if constexpr (PAIR) mma_ts_f8(tmem + C::O_COL, sbuf(j) + TK / 4 + k * 8, vd, IDESC_PV, 1u);
       }
     };
     // S[j + 1] = Q K_{j+1}^T.  Two S buffers: issued before P_j V_j so it overlaps the softmax of
@@ -382,12 +473,12 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
     for (int j = 0; j < n_tiles && alive; ++j) {
       if (NBUF == 2 && j + 1 < n_tiles) { next_qk(j, alive); if (!alive) break; }
       if (has_o) {
-        alive = mbar_wait_warp(bar(V_FULL + j % STAGES), (j / STAGES) & 1, abort_flag);
+        alive = mbar_wait_warp(bar(V_FULL + j % V_STAGES), (j / V_STAGES) & 1, abort_flag);
         if (alive) alive = mbar_wait_warp(bar(P_FULL + j % NBUF), (j / NBUF) & 1, abort_flag);
         if (!alive) break;
         tc_fence_after();
         if (elect_one()) {
-          issue_pv(j); mma_commit(bar(V_EMPTY + j % STAGES)); mma_commit(bar(PV_DONE));
+          issue_pv(j); mma_commit(bar(V_EMPTY + j % V_STAGES)); mma_commit(bar(PV_DONE));
           if (j == n_tiles - 1) mma_commit(bar(O_DONE));
         }
         __syncwarp();
@@ -405,7 +496,9 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
     const int head = head0 + (row_ok ? r % G : 0);
     const int gtok = qo_base + i;
     const int lim = row_ok ? min(i + off, kv_len - 1) : -1;
-    const float scale_log2 = p.sm_scale * kLog2e * (p.k_scale_head ? p.k_scale_head[kvh] : 1.f);
+    [[maybe_unused]] int from = 0;                           // windowed: first key of this row's window
+    if constexpr (WIN) from = row_ok ? window_first(i + off, kv_len, p.window) : 0;
+    float scale_log2 = p.sm_scale * kLog2e * (p.k_scale_head ? p.k_scale_head[kvh] : 1.f);
     const bool want_score = (p.flags & MSA_FLAG_OUT_SCORE) != 0 && p.max_score != nullptr;
     float m_used = -INFINITY, l_sum = 0.f;
     bool alive = true;
@@ -422,6 +515,46 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
                                    static_cast<int64_t>(gtok) * p.q_stride_tok + static_cast<int64_t>(head) * p.q_stride_head);
 #pragma unroll
             for (int c = 0; c < 8; ++c) chunks[c] = src[c];
+          } else if constexpr (PAIR) {
+            // times a power of two that brings the largest element to [128, 256), so that neither value of a pair runs out of exponents
+            const uint4* src = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.q) +
+                                   static_cast<int64_t>(gtok) * p.q_stride_tok + static_cast<int64_t>(head) * p.q_stride_head);
+            uint32_t top = 0;                                // magnitudes order as their bits do
+#pragma unroll
+            for (int c = 0; c < 16; ++c) {
+              const uint4 x = src[c];
+              const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+              for (int e = 0; e < 4; ++e) top = max(top, max(w[e] & 0x7fffu, (w[e] >> 16) & 0x7fffu));
+            }
+            // (a row of zeros, or with an infinity or NaN, is taken as it is; the factors are normal numbers)
+            int ex = static_cast<int>(top >> 7) - 127 - 7;
+            if (top == 0 || top >= 0x7f80u) ex = 0;
+            ex = min(max(ex, -126), 126);
+            const float up = __uint_as_float(static_cast<uint32_t>(127 - ex) << 23);
+            scale_log2 *= __uint_as_float(static_cast<uint32_t>(127 + ex) << 23);
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+              const uint4 a = src[2 * c], b4 = src[2 * c + 1];
+              const uint32_t w[8] = {a.x, a.y, a.z, a.w, b4.x, b4.y, b4.z, b4.w};
+              uint32_t hi[4], lo[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                uint16_t h[2], l[2];
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
+                  const uint32_t x = w[2 * e + n];
+                  const float2 f = make_float2(__uint_as_float(x << 16) * up, __uint_as_float(x & 0xffff0000u) * up);
+                  h[n] = __nv_cvt_float2_to_fp8x2(f, __NV_SATFINITE, __NV_E4M3);
+                  const float2 r = e4m3x2_as_float2(h[n]);
+                  l[n] = __nv_cvt_float2_to_fp8x2(make_float2(f.x - r.x, f.y - r.y), __NV_SATFINITE, __NV_E4M3);
+                }
+                hi[e] = static_cast<uint32_t>(h[0]) | (static_cast<uint32_t>(h[1]) << 16);
+                lo[e] = static_cast<uint32_t>(l[0]) | (static_cast<uint32_t>(l[1]) << 16);
+              }
+              chunks[c] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+              *reinterpret_cast<uint4*>(smem_gen + C::OFF_Q_LO + trow * 128 + ((c ^ (trow & 7)) << 4)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+            }
           } else {
             const uint4* src = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.q) +
                                    static_cast<int64_t>(gtok) * p.q_stride_tok + static_cast<int64_t>(head) * p.q_stride_head);
@@ -476,6 +609,13 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
           for (int e = 0; e < CW; ++e)
             if (pos0 + e > lim) sv[e] = 0xff800000u;
         }
+        if constexpr (WIN) {
+          if (pos0 < from && pos0 + CW > p.sink_tokens) {
+#pragma unroll
+            for (int e = 0; e < CW; ++e)
+              if (pos0 + e < from && pos0 + e >= p.sink_tokens) sv[e] = 0xff800000u;
+          }
+        }
         float mxs[2] = {-INFINITY, -INFINITY};
 #pragma unroll
         for (int e = 0; e < CW; e += 2)
@@ -504,6 +644,7 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
         if (trace && j == 12) trace[6] = clock64() - clk0;       // ... max / rescale done
         constexpr int PCOLS = F8 ? CW / 4 : CW / 2;          // TMEM columns of this quadrant's P
         uint32_t pk[PCOLS];
+        [[maybe_unused]] uint32_t pl[PCOLS];                 // pairs: the second values
         if constexpr (F8) {
 #pragma unroll
           for (int e = 0; e < CW; e += 4) {
@@ -514,7 +655,12 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
             const uint16_t lo = __nv_cvt_float2_to_fp8x2(make_float2(p0, p1), __NV_SATFINITE, __NV_E4M3);
             const uint16_t hi = __nv_cvt_float2_to_fp8x2(make_float2(p2, p3), __NV_SATFINITE, __NV_E4M3);
             const float2 ra = e4m3x2_as_float2(lo), rb = e4m3x2_as_float2(hi);
-            l0 += ra.x + rb.x; l1 += ra.y + rb.y;
+            if constexpr (PAIR) {
+              l0 += p0 + p2; l1 += p1 + p3;
+              pl[e >> 2] = e4m3_rest(p0, p1, ra) | (e4m3_rest(p2, p3, rb) << 16);
+            } else {
+              l0 += ra.x + rb.x; l1 += ra.y + rb.y;
+            }
             pk[e >> 2] = static_cast<uint32_t>(lo) | (static_cast<uint32_t>(hi) << 16);
           }
         } else {
@@ -533,6 +679,11 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
 #pragma unroll
           for (int c = 0; c < 16; ++c) all[c] = (c >> 2) == warp ? pk[c & 3] : 0u;
           tmem_st16(tS, all);
+          if constexpr (PAIR) {
+#pragma unroll
+            for (int c = 0; c < 16; ++c) all[c] = (c >> 2) == warp ? pl[c & 3] : 0u;
+            tmem_st16(tS + TK / 4, all);
+          }
         } else {
           uint32_t zero[PCOLS];
 #pragma unroll
@@ -570,6 +721,15 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
 #pragma unroll
           for (int e = 0; e < 32; ++e)
             if (pos0 + c * 32 + e > lim) sv[c][e] = 0xff800000u;
+      }
+      if constexpr (WIN) {
+        if (pos0 < from && pos0 + BN > p.sink_tokens) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (pos0 + c * 32 + e < from && pos0 + c * 32 + e >= p.sink_tokens) sv[c][e] = 0xff800000u;
+        }
       }
       float mxs[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -616,6 +776,7 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
       for (int c = 0; c < 4; ++c) {
         if constexpr (F8) {
           uint32_t pk[8];                                   // four e4m3 per TMEM column
+          [[maybe_unused]] uint32_t pl[8];
 #pragma unroll
           for (int e = 0; e < 32; e += 4) {
             const float p0 = exp2_fast(fmaf(__uint_as_float(sv[c][e]), scale_log2, -msafe));
@@ -625,10 +786,16 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
             const uint16_t lo = __nv_cvt_float2_to_fp8x2(make_float2(p0, p1), __NV_SATFINITE, __NV_E4M3);
             const uint16_t hi = __nv_cvt_float2_to_fp8x2(make_float2(p2, p3), __NV_SATFINITE, __NV_E4M3);
             const float2 ra = e4m3x2_as_float2(lo), rb = e4m3x2_as_float2(hi);
-            l0 += ra.x + rb.x; l1 += ra.y + rb.y;
+            if constexpr (PAIR) {
+              l0 += p0 + p2; l1 += p1 + p3;
+              pl[e >> 2] = e4m3_rest(p0, p1, ra) | (e4m3_rest(p2, p3, rb) << 16);
+            } else {
+              l0 += ra.x + rb.x; l1 += ra.y + rb.y;
+            }
             pk[e >> 2] = static_cast<uint32_t>(lo) | (static_cast<uint32_t>(hi) << 16);
           }
           tmem_st8(tS + c * 8, pk);
+          if constexpr (PAIR) tmem_st8(tS + TK / 4 + c * 8, pl);
         } else {
           uint32_t pk[16];
 #pragma unroll
@@ -801,7 +968,6 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
 // (optionally as split partials) or, for the proxy pass, the per-page max score alone
 int fmha_decode_tc_supported(const MsaFmhaParams& p) {
   const bool has_o = (p.flags & MSA_FLAG_OUT_O) != 0, has_s = (p.flags & MSA_FLAG_OUT_SCORE) != 0;
-  if (p.window > 0) return 0;
   if (has_o == has_s) return 0;                                  // O + score together stays on the generic kernel
   if (p.page_size != decode_tc::BN) return 0;
   if (p.kv_dtype == MSA_DT_BF16) { if (p.q_dtype != MSA_DT_BF16) return 0; }
@@ -850,23 +1016,27 @@ int fmha_decode_tc_launch(const MsaFmhaParams& p, cudaStream_t stream) {
         return MSA_ERR_LAUNCH;
     }
   }
-  static bool attr_done[16][4] = {};
+  static bool attr_done[16][8] = {};
   int dev = 0;
   cudaGetDevice(&dev);
   using Kern = void (*)(const MsaFmhaParams, const CUtensorMap, const CUtensorMap, const CUtensorMap);
-  const int variant = (f8 ? 2 : 0) | (quad ? 1 : 0);
+  const int variant = (p.window > 0 ? 4 : 0) | (f8 ? 2 : 0) | (quad ? 1 : 0);
   Kern kern;
   int smem;
   switch (variant) {
-    case 0: kern = decode_tc_kernel<false, false>; smem = Cfg<false, false>::SMEM_BYTES; break;
-    case 1: kern = decode_tc_kernel<false, true>;  smem = Cfg<false, true>::SMEM_BYTES;  break;
-    case 2: kern = decode_tc_kernel<true, false>;  smem = Cfg<true, false>::SMEM_BYTES;  break;
-    default: kern = decode_tc_kernel<true, true>;  smem = Cfg<true, true>::SMEM_BYTES;   break;
+    case 0: kern = decode_tc_kernel<false, false, false>; smem = Cfg<false, false>::SMEM_BYTES; break;
+    case 1: kern = decode_tc_kernel<false, true, false>;  smem = Cfg<false, true>::SMEM_BYTES;  break;
+    case 2: kern = decode_tc_kernel<true, false, false>;  smem = Cfg<true, false>::SMEM_BYTES;  break;
+    case 3: kern = decode_tc_kernel<true, true, false>;   smem = Cfg<true, true>::SMEM_BYTES;   break;
+    case 4: kern = decode_tc_kernel<false, false, true>;  smem = Cfg<false, false, true>::SMEM_BYTES; break;
+    case 5: kern = decode_tc_kernel<false, true, true>;   smem = Cfg<false, true, true>::SMEM_BYTES;  break;
+    case 6: kern = decode_tc_kernel<true, false, true>;   smem = Cfg<true, false, true>::SMEM_BYTES;  break;
+    default: kern = decode_tc_kernel<true, true, true>;   smem = Cfg<true, true, true>::SMEM_BYTES;   break;
   }
   if (dev >= 16 || !attr_done[dev][variant]) {
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
       return MSA_ERR_LAUNCH;
-    if (variant == 3)      // two co-resident CTAs need the whole shared-memory carve-out
+    if ((variant & 3) == 3)      // two co-resident CTAs need the whole shared-memory carve-out
       cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
     if (dev < 16) attr_done[dev][variant] = true;
   }
@@ -879,21 +1049,21 @@ int fmha_decode_tc_occupancy(int f8, int quad) {
   int n = 0;
   cudaError_t e;
   if (f8 && quad) {
-    cudaFuncSetAttribute(decode_tc_kernel<true, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<true, true>::SMEM_BYTES);
-    e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, decode_tc_kernel<true, true>, NTHREADS, Cfg<true, true>::SMEM_BYTES);
+    cudaFuncSetAttribute(decode_tc_kernel<true, true, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<true, true>::SMEM_BYTES);
+    e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, decode_tc_kernel<true, true, false>, NTHREADS, Cfg<true, true>::SMEM_BYTES);
     cudaFuncAttributes fa;
-    if (cudaFuncGetAttributes(&fa, decode_tc_kernel<true, true>) == cudaSuccess)
+    if (cudaFuncGetAttributes(&fa, decode_tc_kernel<true, true, false>) == cudaSuccess)
       fprintf(stderr, "decode_tc_kernel<e4m3, quad>: regs %d static smem %zu dyn smem %d local %zu max threads %d\n", fa.numRegs,
               fa.sharedSizeBytes, Cfg<true, true>::SMEM_BYTES, fa.localSizeBytes, fa.maxThreadsPerBlock);
   } else if (f8) {
-    cudaFuncSetAttribute(decode_tc_kernel<true, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<true, false>::SMEM_BYTES);
-    e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, decode_tc_kernel<true, false>, NTHREADS, Cfg<true, false>::SMEM_BYTES);
+    cudaFuncSetAttribute(decode_tc_kernel<true, false, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<true, false>::SMEM_BYTES);
+    e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, decode_tc_kernel<true, false, false>, NTHREADS, Cfg<true, false>::SMEM_BYTES);
   } else if (quad) {
-    cudaFuncSetAttribute(decode_tc_kernel<false, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<false, true>::SMEM_BYTES);
-    e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, decode_tc_kernel<false, true>, NTHREADS, Cfg<false, true>::SMEM_BYTES);
+    cudaFuncSetAttribute(decode_tc_kernel<false, true, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<false, true>::SMEM_BYTES);
+    e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, decode_tc_kernel<false, true, false>, NTHREADS, Cfg<false, true>::SMEM_BYTES);
   } else {
-    cudaFuncSetAttribute(decode_tc_kernel<false, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<false, false>::SMEM_BYTES);
-    e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, decode_tc_kernel<false, false>, NTHREADS, Cfg<false, false>::SMEM_BYTES);
+    cudaFuncSetAttribute(decode_tc_kernel<false, false, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<false, false>::SMEM_BYTES);
+    e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, decode_tc_kernel<false, false, false>, NTHREADS, Cfg<false, false>::SMEM_BYTES);
   }
   return e == cudaSuccess ? n : -1;
 }

@@ -401,6 +401,8 @@ def _fmha_sail_plan(
         offs = _to_int_list(qo_offset)
         assert len(offs) == batch, f"qo_offset must be [batch_size={batch}], got {len(offs)}"
         offs = [kv_lens[i] - qo_lens[i] if o < 0 else o for i, o in enumerate(offs)]
+    if window[0] and any(o + n > (1 << 31) - 1 for o, n in zip(offs, qo_lens)):
+        raise ValueError("places of queries (qo_offset + qo_segment_lens) must fit int32")
 
     if is_sparse:
         pack = h_r
@@ -1023,7 +1025,7 @@ def _fmha_sail(
     p.status = _status_ptr(q.device)
     rows = plan["max_qo_len"] * plan["pack_factor"] if kv_block_indexes is None else plan["pack_factor"]
     dt_ok = (q.dtype == torch.bfloat16 and k.dtype == torch.bfloat16) or k.dtype == torch.float8_e4m3fn
-    if (_USE_DECODE_TC and not use_tc and not window[0] and output_o != (max_score is not None) and dt_ok
+    if (_USE_DECODE_TC and not use_tc and output_o != (max_score is not None) and dt_ok
             and page_size == 128 and 0 < rows <= 128
             and plan["pack_factor"] == num_qo_heads // num_kv_heads and 128 % plan["pack_factor"] == 0):
         p.decode_rows = rows
