@@ -20,7 +20,7 @@
 //               TMEM; completion is signalled to mbarriers with tcgen05.commit
 //   warp 10     scheduler: the CTA's next work item, from the launch control
 //   warp 11     idle (it completes the third warpgroup so that setmaxnreg can move registers to
-//               the softmax warpgroups: 224 / 224 / 56 per thread)
+//               the softmax warpgroups: 224 / 224 / 56 per thread); with a window it clears values that no row sees
 //
 // TMEM (512 columns): S_A [0,128) S_B [128,256) O_A [256,384) O_B [384,512); P aliases the
 // first 64 columns of its S (32 in e4m3).  Shared memory: Q 64 KB, K 2x32 KB, V 2x32 KB (e4m3:
@@ -31,6 +31,10 @@
 // item run under the last softmax and the epilogue of the one before.  Measured against one CTA per item: 4.38 ->
 // 4.24 ms at 4 x 8 192 tokens x 64 heads in bf16 (under the power cap), 213 -> 193 us at five ragged e4m3 prompts of
 // 95 to 4 333 tokens x 32 heads, where an item has few tiles.
+//
+// With a window (WIN) an item's tiles are those of the first keys (sinks) and those from the first key of its first row's window on.  Q tile B's
+// window starts a tile later and A's ends one earlier, so each leaves out the other's tile.  With e4m3 operands P is a pair of
+// e4m3 values, hi + lo, both multiplied by V (a single one puts 2.6 % of noise on each of the few weights that a window leaves).
 //
 // Every mbarrier wait is bounded; on a timeout the CTA raises an abort flag, reports
 // MSA_STATUS_TIMEOUT in the status word, releases its TMEM and exits.
@@ -70,8 +74,8 @@ struct Cfg {
 };
 
 enum Bar { Q_FULL = 0, K_FULL = 1, K_EMPTY = 5, V_FULL = 9, V_EMPTY = 13, S_FULL = 17, P_FULL = 19, O_FULL = 21,
-           V_FIX = 23, Q_EMPTY = 24, ITEM_FULL = 25, ITEM_EMPTY = 27, NEXT_REQ = 29, NEXT_FULL = 30, NUM_BARS = 31 };
-constexpr int ITEM_READERS = 10;        // warps that take every item: 8 softmax, the producer, the MMA issuer
+           V_FIX = 23, Q_EMPTY = 24, ITEM_FULL = 25, ITEM_EMPTY = 27, NEXT_REQ = 29, NEXT_FULL = 30, V_FIX_STAGE = 31, NUM_BARS = 35 };
+constexpr int ITEM_READERS = 10;        // warps that take every item: 8 softmax, the producer, the MMA issuer (with a window: and warp 11)
 constexpr int NEXT_LEAD = 4;            // K tiles before the end of an item at which the next one is asked for
 
 // One work item as the roles need it, written to shared memory by the scheduler warp
@@ -80,6 +84,10 @@ struct Item {
   int head, kvh, row0, qo_base, ql, kv_len, off;
   int n_tiles[2];                       // KV tiles of Q tile A / B
   int kv0;                              // first entry in the page table (paged) / first key (ragged)
+  // with a window:
+  int skip;                             // tiles left out behind those of the sinks
+  int b_first;                          // Q tile B has no tiles between those of the sinks and this one
+  int first_key, end_key;               // of the first row's window; behind the last key that the last row sees
 };
 
 __device__ __forceinline__ float2 e4m3x2_to_float2(uint16_t x) {
@@ -96,12 +104,14 @@ struct Knobs {            // read only in builds with -DMSA_DEBUG_HOOKS
 
 // HAS_O = false: score-only pass (no V, no P, no O), compiled on its own so that neither path's code is shaped
 // by the other's.
-template <bool F8, bool HAS_O>
+template <bool F8, bool HAS_O, bool WIN>
 __global__ void __launch_bounds__(NTHREADS, 1)
 fmha_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant__ CUtensorMap tm_q,
                const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                const Knobs kn) {
   using C = Cfg<F8>;
+  static_assert(HAS_O || !WIN, "a window computes O");
+  constexpr bool PAIR = F8 && WIN;
   constexpr int TILE_BYTES = C::TILE_BYTES, NSUB = C::NSUB, SUB_ELEMS = C::SUB_ELEMS;
   constexpr int KSTAGES = C::STAGES, VSTAGES = C::STAGES;
   // Score-only pass: K comes in pairs of tiles (256 keys, one MMA of N = 256 per K step) through the space of both rings:
@@ -118,12 +128,12 @@ fmha_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant__ 
   const uint32_t bars = smem_base + OFF_BAR;
   // after the barriers: TMEM address, abort flag, skip flag (the status word already reports a timeout), the
   // answer of the launch control, two work items
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem_gen + OFF_BAR + 272);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem_gen + OFF_BAR + 280);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem_gen + OFF_BAR + 288);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem_gen + OFF_BAR + 296);
   volatile int* skip_flag = abort_flag + 1;
-  const uint32_t next_answer = smem_base + OFF_BAR + 288;
-  Item* items = reinterpret_cast<Item*>(smem_gen + OFF_BAR + 304);
-  static_assert(NUM_BARS * 8 <= 272 && 304 + 2 * sizeof(Item) <= 512, "layout of the last 512 bytes");
+  const uint32_t next_answer = smem_base + OFF_BAR + 304;
+  Item* items = reinterpret_cast<Item*>(smem_gen + OFF_BAR + 320);
+  static_assert(NUM_BARS * 8 <= 288 && 320 + 2 * sizeof(Item) <= 512, "layout of the last 512 bytes");
   auto bar = [&](int i) -> uint32_t { return bars + 8u * i; };
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -159,7 +169,9 @@ fmha_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant__ 
       mbar_init(bar(O_FULL + s), 1);
     }
     mbar_init(bar(V_FIX), 1);  mbar_init(bar(Q_EMPTY), 1);
-    for (int s = 0; s < 2; ++s) { mbar_init(bar(ITEM_FULL + s), 1);  mbar_init(bar(ITEM_EMPTY + s), ITEM_READERS); }
+    for (int s = 0; s < 2; ++s) { mbar_init(bar(ITEM_FULL + s), 1);  mbar_init(bar(ITEM_EMPTY + s), ITEM_READERS + WIN); }
+    if constexpr (WIN)
+      for (int s = 0; s < VSTAGES; ++s) mbar_init(bar(V_FIX_STAGE + s), 1);
     mbar_init(bar(NEXT_REQ), 1);  mbar_init(bar(NEXT_FULL), 1);
     *abort_flag = 0;
     mbar_fence_init();
@@ -187,6 +199,15 @@ fmha_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant__ 
     if (lane == 0) mbar_arrive(bar(ITEM_EMPTY + slot));
     tiles = max(w.n_tiles[0], w.n_tiles[1]);
     return w.valid != 0;
+  };
+
+  // with a window: number of a tile among the keys, whether Q tile x has tile j, whether a tile has keys that no row of the item sees
+  [[maybe_unused]] auto real_tile = [&](const Item& w, int j) -> int { return j < sink_tiles(p.sink_tokens) ? j : j + w.skip; };
+  [[maybe_unused]] auto has_tile = [&](const Item& w, int x, int j) -> bool {
+    return x == 0 ? j < w.n_tiles[0] : j < w.n_tiles[1] && (j < sink_tiles(p.sink_tokens) || j >= w.b_first);
+  };
+  [[maybe_unused]] auto has_unseen = [&](const Item& w, int key0) -> bool {
+    return key0 + BN > w.end_key || (key0 < w.first_key && key0 + BN > p.sink_tokens);
   };
 
   const bool run = *skip_flag == 0;
@@ -252,9 +273,10 @@ fmha_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant__ 
           if (j == stall_tile) { alive = false; break; }    // test hook: whoever waits for this tile runs out of polls
           if (j == max(0, n_total - NEXT_LEAD) && lane == 0) mbar_arrive(bar(NEXT_REQ));
           const int ks = tile % KSTAGES, vs = tile % VSTAGES;
-          const int page = paged ? page_entry(p, page_base + j) : 0;
-          const int valid_rows = min(BN, kv_len - j * BN);
-          const bool fix = valid_rows < BN;                 // tail tile: rows past kv_len must read as 0 in V
+          const int jr = WIN ? real_tile(w, j) : j;
+          const int page = paged ? page_entry(p, page_base + jr) : 0;
+          const int valid_rows = min(BN, kv_len - jr * BN);
+          const bool fix = WIN ? has_unseen(w, jr * BN) : valid_rows < BN;   // tail tile: rows past kv_len must read as 0 in V
           if (lane == 0) trace(3, j, 0);
           alive = mbar_wait_warp(bar(K_EMPTY + ks), ((tile / KSTAGES) & 1) ^ 1, abort_flag, spin_limit);
           if (lane == 0) trace(3, j, 1);
@@ -265,7 +287,7 @@ fmha_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant__ 
             for (int hlf = 0; hlf < NSUB; ++hlf) {
               const uint32_t dst = smem_base + OFF_K + ks * TILE_BYTES + hlf * SUB_BYTES;
               if (paged) tma_load_4d(dst, &tm_k, bar(K_FULL + ks), hlf * SUB_ELEMS, 0, kvh, page);
-              else tma_load_3d(dst, &tm_k, bar(K_FULL + ks), hlf * SUB_ELEMS, kvh, kv_base + j * BN);
+              else tma_load_3d(dst, &tm_k, bar(K_FULL + ks), hlf * SUB_ELEMS, kvh, kv_base + jr * BN);
             }
           }
           __syncwarp();
@@ -273,17 +295,17 @@ fmha_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant__ 
           if (lane == 0) trace(3, j, 2);
           if (!alive) break;
           if (elect_one()) {
-            const uint32_t vbar = fix ? bar(V_FIX) : bar(V_FULL + vs);
+            const uint32_t vbar = !fix ? bar(V_FULL + vs) : WIN ? bar(V_FIX_STAGE + vs) : bar(V_FIX);
             mbar_arrive_expect_tx(vbar, TILE_BYTES);
 #pragma unroll
             for (int hlf = 0; hlf < NSUB; ++hlf) {
               const uint32_t dst = smem_base + OFF_V + vs * TILE_BYTES + hlf * SUB_BYTES;
               if (paged) tma_load_4d(dst, &tm_v, vbar, hlf * SUB_ELEMS, 0, kvh, page);
-              else tma_load_3d(dst, &tm_v, vbar, hlf * SUB_ELEMS, kvh, kv_base + j * BN);
+              else tma_load_3d(dst, &tm_v, vbar, hlf * SUB_ELEMS, kvh, kv_base + jr * BN);
             }
           }
           __syncwarp();
-          if (fix && alive) {
+          if (!WIN && fix && alive) {                       // (with a window: warp 11)
             alive = mbar_wait_warp(bar(V_FIX), fix_phase, abort_flag, spin_limit);
             fix_phase ^= 1;
             if (alive) {
@@ -316,6 +338,7 @@ fmha_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant__ 
       Item w;
       w.valid = idx >= 0;
       w.head = w.kvh = w.row0 = w.qo_base = w.ql = w.kv_len = w.off = w.n_tiles[0] = w.n_tiles[1] = w.kv0 = 0;
+      w.skip = w.b_first = w.first_key = w.end_key = 0;
       if (idx >= 0) {
         const MsaWorkItem mw = p.work[idx];
         const int b = chk(mw.batch, 0, p.batch, p.status);
@@ -335,6 +358,19 @@ fmha_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant__ 
           long long vis = min(static_cast<long long>(w.kv_len), static_cast<long long>(last) + w.off + 1);
           if (vis < 0) vis = 0;
           w.n_tiles[x] = min(mw.kv_tile_end, static_cast<int>((vis + BN - 1) / BN));
+          if constexpr (WIN) {
+            const int sinks = sink_tiles(p.sink_tokens), end = static_cast<int>((vis + BN - 1) / BN);
+            w.skip = mw.kv_tile_skip;
+            w.n_tiles[x] = min(mw.kv_tile_end, end <= sinks ? end : max(sinks, end - w.skip));
+            const int lo = window_first(m0 + w.off, w.kv_len, p.window);
+            if (x == 0) {
+              w.first_key = lo;
+            } else {                                    // (the last tile is one that it has)
+              w.b_first = max(sinks, lo / BN - w.skip);
+              if (w.n_tiles[1] <= w.b_first) w.n_tiles[1] = min(w.n_tiles[1], sinks);
+            }
+            w.end_key = static_cast<int>(vis);
+          }
         }
       }
       if (lane == 0) {
@@ -391,6 +427,12 @@ fmha_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant__ 
         else mma_ts(tmem + 256 + x * kHeadDim, tmem + x * BN + k * 8, vd, IDESC_PV, (!first || k > 0) ? 1u : 0u);
       }
     };
+    [[maybe_unused]] auto issue_pv_lo = [&](int x, uint32_t vt) {   // the second values of P, behind the first ones
+      const uint32_t va = (smem_base + OFF_V + (vt % VSTAGES) * TILE_BYTES) >> 4;
+#pragma unroll
+      for (int k = 0; k < KSTEPS; ++k)
+        mma_ts_f8(tmem + 256 + x * kHeadDim, tmem + x * BN + BN / 4 + k * 8, dv_hi | ((va + k * (V_KSTEP >> 4)) & 0x3FFF), IDESC_PV, 1u);
+    };
     uint32_t tile = 0, q_loads = 0;                    // running counts, as in the producer
     [[maybe_unused]] uint32_t p_par = 0;               // bit x: parity of the next P_FULL + x
     [[maybe_unused]] uint32_t n_s[2] = {0, 0};         // score-only: S pairs issued so far
@@ -437,6 +479,52 @@ fmha_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant__ 
       if (alive) alive = mbar_wait_warp(bar(K_FULL + tile % KSTAGES), (tile / KSTAGES) & 1, abort_flag, spin_limit);
       if (!alive) break;
       tc_fence_after();
+      if constexpr (WIN) {
+        // As below, but each Q tile leaves out tiles: S of tile j + 1 is issued in step j whether or not the Q tile has tile j.
+        if (elect_one()) {
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+            if (has_tile(w, x, 0)) { issue_qk(x, tile); mma_commit(bar(S_FULL + x)); }
+          mma_commit(bar(K_EMPTY + tile % KSTAGES));
+          if (n_total == 1) mma_commit(bar(Q_EMPTY));
+        }
+        __syncwarp();
+        uint32_t begun = 0;                            // bit x: O of Q tile x holds something
+        for (int j = 0; j < n_total && alive; ++j, ++tile) {
+          alive = mbar_wait_warp(bar(V_FULL + tile % VSTAGES), (tile / VSTAGES) & 1, abort_flag, spin_limit);
+          if (alive && j + 1 < n_total)
+            alive = mbar_wait_warp(bar(K_FULL + (tile + 1) % KSTAGES), ((tile + 1) / KSTAGES) & 1, abort_flag, spin_limit);
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const bool now = has_tile(w, x, j), next = has_tile(w, x, j + 1);
+            if (!alive) continue;
+            if (now) {
+              alive = mbar_wait_warp(bar(P_FULL + x), (p_par >> x) & 1, abort_flag, spin_limit);
+              if (!alive) continue;
+              p_par ^= 1u << x;
+            }
+            tc_fence_after();
+            if (elect_one()) {
+              if (now) {
+                issue_pv(x, tile, !((begun >> x) & 1));
+                if constexpr (PAIR) issue_pv_lo(x, tile);
+              }
+              if (next) { issue_qk(x, tile + 1); mma_commit(bar(S_FULL + x)); }
+              if (now && j + 1 == w.n_tiles[x]) mma_commit(bar(O_FULL + x));
+            }
+            __syncwarp();
+            if (now) begun |= 1u << x;
+          }
+          if (!alive) break;
+          if (elect_one()) {
+            mma_commit(bar(V_EMPTY + tile % VSTAGES));
+            if (j + 1 < n_total) mma_commit(bar(K_EMPTY + (tile + 1) % KSTAGES));
+            if (j + 2 == n_total) mma_commit(bar(Q_EMPTY));
+          }
+          __syncwarp();
+        }
+        continue;
+      }
       if (elect_one()) {                               // S of both tiles is free: the last P has been waited for
 #pragma unroll
         for (int x = 0; x < 2; ++x)
@@ -484,6 +572,33 @@ fmha_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant__ 
     }
   } else if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if constexpr (WIN) {
+      // =========================== values that no row sees ===========================
+      // They read as 0: the weight of 0 that they have does not take a NaN out.
+      uint32_t tile = 0, fix_par = 0;
+      bool alive = true;
+      Item w;
+      int n_total = 0;
+      for (uint32_t it = 0; take_item(it, w, n_total, alive); ++it) {
+        for (int j = 0; j < n_total && alive; ++j, ++tile) {
+          const int key0 = real_tile(w, j) * BN;
+          if (!has_unseen(w, key0)) continue;
+          const int vs = tile % VSTAGES;
+          alive = mbar_wait_warp(bar(V_FIX_STAGE + vs), (fix_par >> vs) & 1, abort_flag, item_limit(n_total));
+          if (!alive) break;
+          fix_par ^= 1u << vs;
+          unsigned char* vt = smem_gen + OFF_V + vs * TILE_BYTES;
+          for (int c = lane; c < BN * (NSUB * 8); c += 32) {
+            const int r = c / (NSUB * 8), ch = c % (NSUB * 8), key = key0 + r;
+            if (key >= w.end_key || (key < w.first_key && key >= p.sink_tokens))
+              *reinterpret_cast<uint4*>(vt + (ch >> 3) * SUB_BYTES + r * 128 + (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(V_FULL + vs));
+        }
+      }
+    }
   } else {
     // =========================== softmax / epilogue ===========================
     asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
@@ -503,12 +618,21 @@ fmha_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant__ 
       const bool row_ok = i < w.ql;
       const int gtok = w.qo_base + i;
       const int lim = row_ok ? min(i + off, kv_len - 1) : -1;
+      [[maybe_unused]] int from = 0, from_last = 0;        // with a window: its first key for this row, and for the last row of the tile
+      if constexpr (WIN) {
+        from = window_first(i + off, kv_len, p.window);
+        from_last = window_first(m0 + BM - 1 + off, kv_len, p.window);
+      }
+      [[maybe_unused]] bool begun = false;
       const int nx = x == 0 ? w.n_tiles[0] : w.n_tiles[1];
       const float scale_log2 = p.sm_scale * kLog2e * (p.k_scale_head ? p.k_scale_head[kvh] : 1.f);
       float m_used = -INFINITY, l_sum = 0.f;
       float l_exact = 0.f;                                 // e4m3 only: sum of the unrounded probabilities, for the LSE
 
       for (int j = 0; j < nx && alive; ++j) {
+        if (WIN && !has_tile(w, x, j)) continue;
+        const bool later = WIN ? begun : j > 0;             // not the Q tile's first tile
+        if constexpr (WIN) begun = true;
         if (r == 0) trace(x, j, 0);
         if (HAS_O || (j & 1) == 0) {                       // score-only: S of two tiles at a time
           alive = mbar_wait_warp(bar(S_FULL + x), s_par, abort_flag, spin_limit);
@@ -518,8 +642,8 @@ fmha_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant__ 
         const uint32_t tS = tmem + (HAS_O ? x * BN : x * 2 * BN + (j & 1) * BN) + lane_addr;
         tc_fence_after();
         if (r == 0) trace(x, j, 1);
-        const int pos0 = j * BN;
-        const bool need_mask = (pos0 + BN - 1 > m0 + off) || (pos0 + BN > kv_len);
+        const int pos0 = (WIN ? real_tile(w, j) : j) * BN;
+        const bool need_mask = (pos0 + BN - 1 > m0 + off) || (pos0 + BN > kv_len) || (WIN && pos0 < from_last && pos0 + BN > p.sink_tokens);
         // ---- one read of the whole S row (128 fp32) ----
         uint32_t sv[4][32];
         tmem_ld32(tS, sv[0]);
@@ -537,7 +661,7 @@ fmha_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant__ 
           for (int c = 0; c < 4; ++c)
 #pragma unroll
             for (int e = 0; e < 32; ++e)
-              if (pos0 + c * 32 + e > lim) sv[c][e] = 0xff800000u;     // -inf
+              if (pos0 + c * 32 + e > lim || (WIN && pos0 + c * 32 + e < from && pos0 + c * 32 + e >= p.sink_tokens)) sv[c][e] = 0xff800000u;     // -inf
         }
         auto store_score = [&](const float mx) {
           if (want_score && row_ok && j < p.max_k_tiles) {
@@ -578,7 +702,8 @@ fmha_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant__ 
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             uint32_t pk[F8 ? 8 : 16];
-            [[maybe_unused]] uint16_t held = 0;
+            [[maybe_unused]] uint32_t pl[PAIR ? 8 : 1];
+            [[maybe_unused]] uint16_t held = 0, held_lo = 0;
 #pragma unroll
             for (int e = 0; e < 32; e += 2) {
               if constexpr (decltype(with_max)::value)
@@ -612,7 +737,13 @@ fmha_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant__ 
                 lex2 = f2_add(lex2, f2_pack(p0, p1));
                 const uint16_t pr = __nv_cvt_float2_to_fp8x2(make_float2(p0, p1), __NV_SATFINITE, __NV_E4M3);
                 const float2 rr = e4m3x2_to_float2(pr);
-                lsum2 = f2_add(lsum2, f2_pack(rr.x, rr.y));
+                if constexpr (PAIR) {
+                  const uint16_t lo = __nv_cvt_float2_to_fp8x2(make_float2(p0 - rr.x, p1 - rr.y), __NV_SATFINITE, __NV_E4M3);
+                  if (e & 2) pl[e >> 2] = static_cast<uint32_t>(held_lo) | (static_cast<uint32_t>(lo) << 16);
+                  else held_lo = lo;
+                } else {
+                  lsum2 = f2_add(lsum2, f2_pack(rr.x, rr.y));
+                }
                 if (e & 2) pk[e >> 2] = static_cast<uint32_t>(held) | (static_cast<uint32_t>(pr) << 16);
                 else held = pr;
               } else {
@@ -622,17 +753,19 @@ fmha_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant__ 
             }
             if constexpr (F8) tmem_st8(tS + c * 8, pk);
             else tmem_st16(tS + c * 16, pk);
+            if constexpr (PAIR) tmem_st8(tS + BN / 4 + c * 8, pl);
           }
           float l0, l1;
           f2_unpack(lsum2, l0, l1);
           l_rnd = l0 + l1;
           if constexpr (F8) { f2_unpack(lex2, l0, l1); l_raw = l0 + l1; }
+          if constexpr (PAIR) l_rnd = l_raw;
         };
         // Every tile but the first writes P with the running max while it finds its own max: the max does
         // not sit between the S read and the exponentials, and the guess holds unless the row's max grows
         // by more than the rescale threshold (then P is written again below).
         // (bf16 only: with e4m3 operands the kernel measured 6 % slower this way.)
-        const bool guess = !F8 && j > 0;                              // warp-uniform
+        const bool guess = !F8 && later;                              // warp-uniform
         const float m_guess = ((m_used == -INFINITY) ? 0.f : m_used) - kPOffset;
         if (guess) emit_p(std::true_type{}, m_guess);
         else row_max();
@@ -646,7 +779,7 @@ fmha_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant__ 
         if (!guess || __any_sync(0xffffffffu, bump)) {
           float factor = 1.f;
           if (bump) { factor = exp2_fast(m_used - m_cand); m_used = m_cand; l_sum *= factor; l_exact *= factor; }
-          if (j > 0 && __any_sync(0xffffffffu, bump)) {
+          if (later && __any_sync(0xffffffffu, bump)) {
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
               uint32_t v[32];
@@ -677,7 +810,8 @@ fmha_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant__ 
       if (alive && has_o) {
         tc_fence_after();
         const float vsh = p.v_scale_head ? p.v_scale_head[kvh] : 1.f;
-        const float inv = l_sum > 0.f ? p.out_scale * vsh / l_sum : 0.f;
+        // (a row that saw no key may have the least of what the exponentials give as its sum)
+        const float inv = l_sum > 0.f && (!WIN || m_used != -INFINITY) ? p.out_scale * vsh / l_sum : 0.f;
         __nv_bfloat16* dst = p.out ? static_cast<__nv_bfloat16*>(p.out) + static_cast<int64_t>(gtok) * p.out_stride_tok +
                                          static_cast<int64_t>(head) * p.out_stride_head
                                    : nullptr;
@@ -774,7 +908,7 @@ int make_tma_map_u8(CUtensorMap* m, const void* base, int rank, const uint64_t* 
 
 // Shapes the tcgen05 kernel takes; everything else runs on the mma.sync kernel.
 int fmha_tc_supported(const MsaFmhaParams& p) {
-  if (p.block_m != 256 || p.window > 0) return 0;
+  if (p.block_m != 256) return 0;
   return 1;
 }
 
@@ -816,13 +950,13 @@ int fmha_tc_launch(const MsaFmhaParams& p, cudaStream_t stream) {
     if (!make_map(&tk, p.k, 3, dims, ks, box, f8) || !make_map(&tv, has_o ? p.v : p.k, 3, dims, has_o ? vs : ks, box, f8))
       return MSA_ERR_LAUNCH;
   }
-  static bool attr_done[4][16] = {};
+  static bool attr_done[6][16] = {};
   int dev = 0;
   cudaGetDevice(&dev);
   using KernelFn = void (*)(const MsaFmhaParams, const CUtensorMap, const CUtensorMap, const CUtensorMap, const Knobs);
-  const int variant = (f8 ? 2 : 0) | (has_o ? 1 : 0);
-  const KernelFn kernels[4] = {fmha_tc_kernel<false, false>, fmha_tc_kernel<false, true>, fmha_tc_kernel<true, false>,
-                               fmha_tc_kernel<true, true>};
+  const int variant = p.window > 0 ? (f8 ? 5 : 4) : (f8 ? 2 : 0) | (has_o ? 1 : 0);
+  const KernelFn kernels[6] = {fmha_tc_kernel<false, false, false>, fmha_tc_kernel<false, true, false>, fmha_tc_kernel<true, false, false>,
+                               fmha_tc_kernel<true, true, false>, fmha_tc_kernel<false, true, true>, fmha_tc_kernel<true, true, true>};
   const KernelFn kern = kernels[variant];
   const int smem_bytes = f8 ? Cfg<true>::SMEM_BYTES : Cfg<false>::SMEM_BYTES;
   if (dev >= 16 || !attr_done[variant][dev]) {
