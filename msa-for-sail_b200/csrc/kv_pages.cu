@@ -6,6 +6,8 @@
 // order of the table: results do not depend on how threads are scheduled.
 //
 // The tables are small: launches and chains of dependent reads bound these passes.  The copies are bound by memory.
+#include <cooperative_groups.h>
+
 #include <algorithm>
 #include <climits>
 
@@ -133,6 +135,28 @@ __device__ __forceinline__ int block_scan(int x, int* s_sum, int& total) {
   const int before = __shfl_sync(0xffffffffu, scan - mine, warp);
   __syncthreads();                             // s_sum may be written again
   return before + incl - x;
+}
+
+// One cluster, chained as launch_chained() does.
+template <typename... P, typename... A>
+cudaError_t launch_cluster(void (*kernel)(P...), int ctas, int threads, cudaStream_t stream, A&&... args) {
+  if (ctas == 1) return launch_chained(kernel, 1, threads, 0, stream, args...);
+  if (ctas > 8) {                              // more than every device of the architecture has to take
+    const cudaError_t rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (rc != cudaSuccess) return rc;
+  }
+  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+  cudaStreamIsCapturing(stream, &capture);
+  cudaLaunchAttribute attr[2] = {};
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = capture == cudaStreamCaptureStatusNone ? 1 : 0;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = static_cast<unsigned>(ctas);
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(ctas)); cfg.blockDim = dim3(static_cast<unsigned>(threads)); cfg.stream = stream;
+  cfg.attrs = attr; cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, kernel, P(args)...);
 }
 
 __device__ __forceinline__ int stack_size(const int32_t* num_free, int capacity) { return min(max(__ldcg(num_free), 0), capacity); }
@@ -289,48 +313,100 @@ __device__ __forceinline__ void push(const MsaPagesFreeArgs& a, int page, int pl
   if (a.shares) a.shares[page] = 0;
 }
 
-// Few entries: one CTA walks the table.
-__global__ void __launch_bounds__(kScanThreads) pages_free_small_kernel(const MsaPagesFreeArgs a) {
+// Tables of up to 2^18 entries: the CTAs of one cluster, K entries a thread that stay in registers from step to step; between the steps are
+// barriers of the cluster.  (As launches of their own the steps take longer than the work: 512 rows of 257 pages that other rows share,
+// 17.5 us in five launches.)
+constexpr int kClusterCtas = 16;
+
+template <int K>
+__global__ void __launch_bounds__(kScanThreads) pages_free_cluster_kernel(const MsaPagesFreeArgs a) {
   chain_begin();
+  auto cluster = cooperative_groups::this_cluster();
   __shared__ int s_sum[32];
-  const int tid = threadIdx.x, entries = a.batch * a.table_width;
+  __shared__ int s_warps[K * 32];              // pages that a warp's entries give back, then those of the entries before it in this CTA
+  __shared__ int s_total;
+  __shared__ Kept s_kept[kScanThreads];        // of the rows that this CTA has entries of
+  const int ctas = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int entries = a.batch * a.table_width, e0 = rank * K * kScanThreads + tid;
   const int num_free = stack_size(a.num_free, a.free_capacity);
-  auto visit = [&](int e, auto&& what) {
-    const int b = e / a.table_width, col = e - b * a.table_width;
-    const Kept k = kept_of(a, b);
-    what(page_back(a, k, b, col), given_back(k, col), b, col);
-  };
-  if (a.shares) {
-    for (int e = tid; e < entries; e += kScanThreads) visit(e, [&](int page, bool, int, int) { release(a, page); });
-    __syncthreads();
-    for (int e = tid; e < entries; e += kScanThreads) visit(e, [&](int page, bool, int, int) { claim(a, page, e); });
-    __syncthreads();
+  // (the divisions of a row's limits, made for each entry, would take longest of all)
+  const int row0 = min(e0 - tid, entries) / max(a.table_width, 1);
+  const bool few_rows = K * kScanThreads / max(a.table_width, 1) + 2 <= kScanThreads;
+  if (few_rows && row0 + tid < a.batch) s_kept[tid] = kept_of(a, row0 + tid);
+  __syncthreads();
+  int page[K];
+  unsigned back = 0, own = 0;                  // bit k: entry e0 + k * kScanThreads is given back, and its page goes onto the stack
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int e = e0 + k * kScanThreads;
+    page[k] = -1;
+    if (e < entries) {
+      const int b = e / a.table_width, col = e - b * a.table_width;
+      if (given_back(few_rows ? s_kept[b - row0] : kept_of(a, b), col)) {
+        back |= 1u << k;
+        page[k] = a.block_table[b * a.table_stride + col];
+      }
+    }
   }
-  int at = num_free;
-  for (int e0 = 0; e0 < entries; e0 += kScanThreads) {
-    const int e = e0 + tid;
-    int page = -1;
-    bool mine = false;
-    if (e < entries)
-      visit(e, [&](int pg, bool back, int b, int col) {
-        page = pg;
-        mine = gives(a, pg, e);
-        if (back) a.block_table[b * a.table_stride + col] = -1;
-      });
-    int total;
-    const int rank = block_scan<kScanThreads>(mine, s_sum, total);
-    if (mine) push(a, page, at + rank);
-    at += total;
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+    if (page[k] >= a.num_pages) page[k] = -1;
+  if (a.shares) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) release(a, page[k]);
+    cluster.sync();
+    int share[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) share[k] = page[k] >= 0 ? __ldcg(&a.shares[page[k]]) : 0;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+      if (share[k] < 0) atomicMin(&a.shares[page[k]], INT_MIN + e0 + k * kScanThreads);
+    cluster.sync();
+#pragma unroll
+    for (int k = 0; k < K; ++k) share[k] = page[k] >= 0 ? __ldcg(&a.shares[page[k]]) : 0;
+#pragma unroll
+    for (int k = 0; k < K; ++k) own |= static_cast<unsigned>(share[k] == INT_MIN + e0 + k * kScanThreads) << k;
+  } else {
+#pragma unroll
+    for (int k = 0; k < K; ++k) own |= static_cast<unsigned>(page[k] >= 0) << k;
+  }
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const unsigned who = __ballot_sync(0xffffffffu, (own >> k) & 1);
+    if (lane == 0) s_warps[k * 32 + warp] = __popc(who);
   }
   __syncthreads();
-  for (int b = tid; b < a.batch; b += kScanThreads) a.num_held[b] = kept_of(a, b).end;
-  if (tid == 0) {
-    *a.num_free = min(at, a.free_capacity);
-    if (a.num_freed) *a.num_freed = at - num_free;
+  int total;
+  const int mine = tid < K * 32 ? s_warps[tid] : 0;
+  const int before = block_scan<kScanThreads>(mine, s_sum, total);
+  if (tid < K * 32) s_warps[tid] = before;
+  if (tid == 0) s_total = total;
+  cluster.sync();
+  int at = num_free, all = 0;
+  for (int c = 0; c < ctas; ++c) {
+    const int n = *cluster.map_shared_rank(&s_total, c);
+    if (c < rank) at += n;
+    all += n;
   }
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const unsigned who = __ballot_sync(0xffffffffu, (own >> k) & 1);
+    if ((own >> k) & 1) push(a, page[k], at + s_warps[k * 32 + warp] + __popc(who & ((1u << lane) - 1)));
+    if ((back >> k) & 1) {
+      const int e = e0 + k * kScanThreads, b = e / a.table_width;
+      a.block_table[b * a.table_stride + e - b * a.table_width] = -1;
+    }
+  }
+  for (int b = rank * kScanThreads + tid; b < a.batch; b += ctas * kScanThreads) a.num_held[b] = kept_of(a, b).end;
+  if (rank == 0 && tid == 0) {
+    *a.num_free = min(num_free + all, a.free_capacity);
+    if (a.num_freed) *a.num_freed = all;
+  }
+  cluster.sync();                              // nobody leaves while its s_total may be read
 }
 
-// Many entries: a CTA for 1 024 columns of a row, a kernel for each step.  Workspace: pages given back by each of these chunks, then the size of
+// Long rows, or many: a CTA for 1 024 columns of a row, a kernel for each step.  Workspace: pages given back by each of these chunks, then the size of
 // the stack.
 constexpr int kCols = 4 * kThreads;
 __device__ __forceinline__ int chunks_of(const MsaPagesFreeArgs& a) { return (a.table_width + kCols - 1) / kCols; }
@@ -434,18 +510,29 @@ __host__ __device__ inline Sets sets_of(const MsaPagesCompactArgs& a) {
   return {reinterpret_cast<uint32_t*>(s), reinterpret_cast<uint32_t*>(s + w), s + 2 * w, s + 3 * w, s + 4 * w, s + 5 * w};
 }
 
-__global__ void __launch_bounds__(kThreads) pages_mark_kernel(const MsaPagesCompactArgs a) {
-  chain_begin();
+// Steps, for thread `first` of `step`.
+__device__ __forceinline__ void mark_pages(const MsaPagesCompactArgs& a, int64_t first, int64_t step) {
   const Sets s = sets_of(a);
-  const int64_t first = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x, step = static_cast<int64_t>(gridDim.x) * kThreads;
   const int num_free = stack_size(a.num_free, a.free_capacity);
   auto mark = [&](uint32_t* set, int page) {
     if (static_cast<unsigned>(page) < static_cast<unsigned>(a.num_pages)) atomicOr(&set[page >> 5], 1u << (page & 31));
   };
   for (int64_t i = first; i < num_free; i += step) mark(s.free, a.free_pages[i]);
-  for (int64_t e = first; e < static_cast<int64_t>(a.batch) * a.table_width; e += step) {
-    const int b = static_cast<int>(e / a.table_width), col = static_cast<int>(e % a.table_width);
-    if (col < a.num_held[b]) mark(s.live, a.block_table[b * a.table_stride + col]);
+  constexpr int U = 4;                         // entries on their way
+  const int64_t entries = static_cast<int64_t>(a.batch) * a.table_width;
+  for (int64_t e0 = first; e0 < entries; e0 += U * step) {
+    int page[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t e = e0 + u * step;
+      page[u] = -1;
+      if (e < entries) {
+        const int b = static_cast<int>(e / a.table_width), col = static_cast<int>(e % a.table_width);
+        if (col < a.num_held[b]) page[u] = a.block_table[b * a.table_stride + col];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) mark(s.live, page[u]);
   }
 }
 
@@ -455,8 +542,8 @@ __device__ __forceinline__ uint32_t from_line(int w, int line) {
   return d <= 0 ? 0xffffffffu : d >= 32 ? 0u : 0xffffffffu << d;
 }
 
-__global__ void __launch_bounds__(kScanThreads) pages_rank_kernel(const MsaPagesCompactArgs a) {
-  chain_begin();
+// By one CTA of kScanThreads.
+__device__ __forceinline__ void rank_pages(const MsaPagesCompactArgs& a) {
   const Sets s = sets_of(a);
   __shared__ int s_sum[32];
   __shared__ int s_line;
@@ -508,20 +595,46 @@ __global__ void __launch_bounds__(kScanThreads) pages_rank_kernel(const MsaPages
 }
 
 // The list of moves, and the stack: the lowest page on top.
-__global__ void __launch_bounds__(kThreads) pages_list_kernel(const MsaPagesCompactArgs a) {
-  chain_begin();
+__device__ __forceinline__ void list_pages(const MsaPagesCompactArgs& a, int first, int step) {
   const Sets s = sets_of(a);
-  const int line = s.sums[0], moved = s.sums[1], left = s.sums[2];
-  const int first = blockIdx.x * kThreads + threadIdx.x, step = gridDim.x * kThreads;
+  const int line = __ldcg(&s.sums[0]), moved = __ldcg(&s.sums[1]), left = __ldcg(&s.sums[2]);
   for (int p = first; p < a.num_pages; p += step) {
     const int w = p >> 5;
-    const uint32_t bit = 1u << (p & 31), live = s.live[w], managed = live | s.free[w], above = from_line(w, line);
-    if (live & above & bit) a.src[s.moving[w] + __popc(live & above & (bit - 1))] = p;
-    if (managed & ~live & ~above & bit) a.dst[s.holes[w] + __popc(managed & ~live & ~above & (bit - 1))] = p;
-    if (managed & above & bit) a.free_pages[left - 1 - s.rest[w] - __popc(managed & above & (bit - 1))] = p;
+    const uint32_t bit = 1u << (p & 31), live = __ldcg(&s.live[w]), managed = live | __ldcg(&s.free[w]), above = from_line(w, line);
+    if (live & above & bit) a.src[__ldcg(&s.moving[w]) + __popc(live & above & (bit - 1))] = p;
+    if (managed & ~live & ~above & bit) a.dst[__ldcg(&s.holes[w]) + __popc(managed & ~live & ~above & (bit - 1))] = p;
+    if (managed & above & bit) a.free_pages[left - 1 - __ldcg(&s.rest[w]) - __popc(managed & above & (bit - 1))] = p;
     if (p >= moved) a.src[p] = a.dst[p] = -1;  // (the lists have a place for every page; moves come before)
   }
   if (first == 0) *a.num_free = left;
+}
+
+// Ordinary pools: the CTAs of one cluster.  (8 192 pages, 800 rows: 5 us instead of 15 for a memset and three launches.)
+__global__ void __launch_bounds__(kScanThreads) pages_compact_cluster_kernel(const MsaPagesCompactArgs a) {
+  chain_begin();
+  auto cluster = cooperative_groups::this_cluster();
+  const int first = static_cast<int>(cluster.block_rank()) * kScanThreads + threadIdx.x, step = static_cast<int>(cluster.num_blocks()) * kScanThreads;
+  uint32_t* words = sets_of(a).live;           // and the free ones behind them
+  for (int w = first; w < 2 * words_of(a.num_pages); w += step) words[w] = 0;
+  cluster.sync();
+  mark_pages(a, first, step);
+  cluster.sync();
+  if (cluster.block_rank() == 0) rank_pages(a);
+  cluster.sync();
+  list_pages(a, first, step);
+}
+
+__global__ void __launch_bounds__(kThreads) pages_mark_kernel(const MsaPagesCompactArgs a) {
+  chain_begin();
+  mark_pages(a, static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x, static_cast<int64_t>(gridDim.x) * kThreads);
+}
+__global__ void __launch_bounds__(kScanThreads) pages_rank_kernel(const MsaPagesCompactArgs a) {
+  chain_begin();
+  rank_pages(a);
+}
+__global__ void __launch_bounds__(kThreads) pages_list_kernel(const MsaPagesCompactArgs a) {
+  chain_begin();
+  list_pages(a, blockIdx.x * kThreads + threadIdx.x, gridDim.x * kThreads);
 }
 
 __global__ void __launch_bounds__(kThreads) pages_move_kernel(const __grid_constant__ MsaPagesCompactArgs a, const __grid_constant__ Copies c) {
@@ -670,8 +783,13 @@ extern "C" int msa_pages_free(const MsaPagesFreeArgs* pa, msa_stream_t stream) {
   if (entries > INT_MAX / 2) return MSA_ERR_TOO_LARGE;
   msa::NvtxRange range("msa_pages_free");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (entries <= 16 * kScanThreads)
-    return msa::launch_chained(pages_free_small_kernel, 1, kScanThreads, 0, st, a) == cudaSuccess ? MSA_OK : MSA_ERR_LAUNCH;
+  if (entries <= 16 * kClusterCtas * kScanThreads) {
+    const int k = entries <= kClusterCtas * kScanThreads ? 1 : entries <= 4 * kClusterCtas * kScanThreads ? 4 : 16;
+    int ctas = 1;
+    while (static_cast<int64_t>(ctas) * k * kScanThreads < entries) ctas *= 2;
+    const auto kernel = k == 1 ? pages_free_cluster_kernel<1> : k == 4 ? pages_free_cluster_kernel<4> : pages_free_cluster_kernel<16>;
+    return launch_cluster(kernel, ctas, kScanThreads, st, a) == cudaSuccess ? MSA_OK : MSA_ERR_LAUNCH;
+  }
   const int64_t units = static_cast<int64_t>(a.batch) * ((a.table_width + kCols - 1) / kCols);
   const unsigned grid = static_cast<unsigned>(std::min<int64_t>(units, kCopyCtas));
   cudaError_t rc = cudaSuccess;
@@ -704,10 +822,15 @@ extern "C" int msa_pages_compact(const MsaPagesCompactArgs* pa, msa_stream_t str
   const Sets s = sets_of(a);
   const int64_t entries = static_cast<int64_t>(a.batch) * a.table_width;
   auto grid = [](int64_t n) { return static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>((n + kThreads - 1) / kThreads, kCopyCtas))); };
-  if (a.num_pages > 0 && cudaMemsetAsync(s.live, 0, 8 * static_cast<size_t>(words_of(a.num_pages)), st) != cudaSuccess) return MSA_ERR_LAUNCH;
-  cudaError_t rc = msa::launch_chained(pages_mark_kernel, grid(std::max<int64_t>(entries, a.free_capacity)), kThreads, 0, st, a);
-  if (rc == cudaSuccess) rc = msa::launch_chained(pages_rank_kernel, 1, kScanThreads, 0, st, a);
-  if (rc == cudaSuccess) rc = msa::launch_chained(pages_list_kernel, grid(a.num_pages), kThreads, 0, st, a);
+  cudaError_t rc = cudaSuccess;
+  if (entries <= (1 << 17) && a.num_pages <= (1 << 17)) {
+    rc = launch_cluster(pages_compact_cluster_kernel, kClusterCtas, kScanThreads, st, a);
+  } else {
+    rc = cudaMemsetAsync(s.live, 0, 8 * static_cast<size_t>(words_of(a.num_pages)), st);
+    if (rc == cudaSuccess) rc = msa::launch_chained(pages_mark_kernel, grid(std::max<int64_t>(entries, a.free_capacity)), kThreads, 0, st, a);
+    if (rc == cudaSuccess) rc = msa::launch_chained(pages_rank_kernel, 1, kScanThreads, 0, st, a);
+    if (rc == cudaSuccess) rc = msa::launch_chained(pages_list_kernel, grid(a.num_pages), kThreads, 0, st, a);
+  }
   if (rc != cudaSuccess) return MSA_ERR_LAUNCH;
   Copies list = {};
   list.entries = a.num_pages; list.src = a.src; list.dst = a.dst; list.count = a.num_moved;

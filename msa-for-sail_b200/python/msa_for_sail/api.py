@@ -486,7 +486,7 @@ def _fmha_sail_plan(
             num_work = n
             splits = int(max_splits.value)
             rows = splits * total_q * orig_num_qo_heads
-            partials = [] if use_kv4_cache else [rows * 128, rows]               # that the plan holds
+            partials = [] if use_kv4_cache or window[0] else [rows * 128, rows]  # that the plan holds
             if splits == 1 or arena.fits([size for *_, size in up.parts] + [max(1, n) * 8, total_q] + partials):
                 break
         up.add("work", host[:n], max(1, n) * 8)
@@ -498,7 +498,7 @@ def _fmha_sail_plan(
         info["tc_preferred"] = info["num_work_tc"] > 0 and (splits == 1 or info["num_work_tc"] * 2 >= num_sms)
 
     up.run(arena, info)
-    if splits > 1 and not use_kv4_cache:      # (calls over a 4-bit cache bring partials of their own)
+    if splits > 1 and not use_kv4_cache and not window[0]:      # (calls over a 4-bit cache, or with a window, bring partials of their own)
         info["workspace_o"] = arena.take(splits * total_q * orig_num_qo_heads * 128, torch.float32)
         info["workspace_lse"] = arena.take(splits * total_q * orig_num_qo_heads, torch.float32)
     else:
@@ -590,7 +590,7 @@ def _fmha_sail_plan_device(qo_segment_lens, kv_segment_lens, num_qo_heads, hkv, 
     tc_tiles = max(1, -(-max_qo // 256))
     n_items_tc = batch * tc_tiles * num_qo_heads if want_tc else 0
     work_tc = arena.take(n_items_tc * 8, torch.int32) if want_tc else None
-    if splits > 1 and not use_kv4_cache:
+    if splits > 1 and not use_kv4_cache and not window[0]:
         info["workspace_o"] = arena.take(splits * max_total_q * num_qo_heads * 128, torch.float32)
         info["workspace_lse"] = arena.take(splits * max_total_q * num_qo_heads, torch.float32)
     else:
@@ -819,6 +819,9 @@ def _fmha_sail(
     if k.dtype == torch.uint8:
         return _fmha_sail_kv4(q, k, v, plan_info, kv_indices, kv_block_indexes, q_offset_override, out, max_score, sm_scale,
                               q_scale, k_scale, v_scale, o_scale, output_maxscore, output_o, check_input_valid, max_score_dtype, lse)
+    if plan_info["window"][0]:
+        return _fmha_sail_window(q, k, v, plan_info, kv_indices, kv_block_indexes, q_offset_override, out, max_score, sm_scale, q_scale, k_scale,
+                                 v_scale, o_scale, output_o, check_input_valid, lse)
     nnz_qo, num_qo_heads, head_dim_qk = q.shape
     plan_page = plan_info.get("page_size", -1)
     if kv_indices is None:
@@ -871,9 +874,6 @@ def _fmha_sail(
     if (plan_page > 0) != is_paged:
         raise ValueError("plan page_size does not match the K/V layout (kv_indices given?)")
 
-    window = plan["window"]
-    if window[0] and q_offset_override is not None:
-        raise ValueError("a plan with window_size has its offsets (qo_offset): q_offset_override cannot change them")
     qo_offset = plan["qo_offset"] if q_offset_override is None else q_offset_override
     if isinstance(qo_offset, int):
         if plan.get("graph_safe", False):
@@ -1030,7 +1030,6 @@ def _fmha_sail(
             and plan["pack_factor"] == num_qo_heads // num_kv_heads and 128 % plan["pack_factor"] == 0):
         p.decode_rows = rows
     p.q_dtype, p.kv_dtype = _dt_code(q.dtype), _dt_code(k.dtype)
-    p.window, p.sink_tokens = window
     p.flags = (FLAG_OUT_O if output_o else 0) | (FLAG_OUT_SCORE if max_score is not None else 0) | \
               (FLAG_SPARSE if kv_block_indexes is not None else 0)
     p.sm_scale = float(q_s * k_s * sm_scale)
@@ -1050,6 +1049,124 @@ def _fmha_sail(
     elif kernel_out is not None and kernel_out is not out:
         _copy_rows(out, kernel_out, plan)
     return out, max_score
+
+
+def _window_params(q_dtype, kv_dtype, plan, nhd):
+    """What is the same in every call with this plan and these types, as the bytes of the arguments: the kernel, its work list and the plan's metadata."""
+    page_size, splits, pack = max(0, plan["page_size"]), plan["num_kv_splits"], plan["pack_factor"]
+    h_r = plan["orig_num_qo_heads"] // plan["num_kv_heads"]
+    p = _lib.MsaFmhaParams(qo_start=plan["qo_segment_offsets"].data_ptr(), kv_start=plan["kv_segment_offsets"].data_ptr(),
+                           kv_len=plan["kv_segment_lens"].data_ptr(), qo_offset=plan["qo_offset"].data_ptr(), kv_page_indptr=_ptr(plan["kv_page_indptr"]),
+                           work=_ptr(plan["work"]), num_work=plan["num_work"], block_m=plan["qo_tile_size"], pack=pack, page_size=page_size,
+                           num_splits=splits, num_qo_heads=plan["orig_num_qo_heads"], num_kv_heads=plan["num_kv_heads"], batch=plan["batch_size"],
+                           q_dtype=_dt_code(q_dtype), kv_dtype=_dt_code(kv_dtype), flags=FLAG_OUT_O, window=plan["window"][0], sink_tokens=plan["window"][1])
+    if plan.get("work_tc") is not None and q_dtype == kv_dtype and page_size in (0, 128) and _USE_TC and (plan["tc_preferred"] or _FORCE_TC):
+        p.work, p.num_work, p.block_m, p.num_splits = plan["work_tc"].data_ptr(), plan["num_work_tc"], 256, 1
+    elif _USE_DECODE_TC and page_size == 128 and 0 < plan["max_qo_len"] * pack <= 128 and pack == h_r and 128 % pack == 0:
+        p.decode_rows = plan["max_qo_len"] * pack
+    return bytes(p), p.num_splits
+
+
+def _fmha_sail_window(q, k, v, plan, kv_indices, kv_block_indexes, q_offset_override, out, max_score, sm_scale, q_scale, k_scale, v_scale, o_scale,
+                      output_o, check_input_valid, lse):
+    """``_fmha_sail`` with a plan that has a window: O (and the LSE) only, over bf16 and e4m3 caches, ragged or paged."""
+    if kv_block_indexes is not None or max_score is not None:
+        raise ValueError("window_size computes O over all keys of the window: no kv_block_indexes, no max_score")
+    if q_offset_override is not None:
+        raise ValueError("a plan with window_size has its offsets (qo_offset): q_offset_override cannot change them")
+    if v is None or not output_o:
+        raise ValueError("window_size computes O: v and output_o are required")
+    q_shape, k_shape, q_dtype, k_dtype = q.shape, k.shape, q.dtype, k.dtype
+    paged = kv_indices is not None
+    if len(q_shape) != 3 or q_shape[2] != 128 or k_shape[-1] != 128:
+        raise ValueError("fmha_sail supports head_dim 128 only")
+    plan_page = plan["page_size"]
+    if (plan_page > 0) != paged:
+        raise ValueError("plan page_size does not match the K/V layout (kv_indices given?)")
+    nhd = False
+    if paged:
+        nhd, num_kv_heads, page_size = _detect_paged_kv_layout(k_shape, plan_page)
+    else:
+        if len(k_shape) != 3:
+            raise ValueError(f"ragged K/V must be [total_kv, Hkv, 128], got {tuple(k_shape)}")
+        num_kv_heads = k_shape[1]
+    if v.shape != k_shape:
+        raise ValueError(f"k and v must have the same shape, got {tuple(k_shape)} and {tuple(v.shape)}")
+    if k_dtype != v.dtype or k_dtype not in (torch.bfloat16, torch.float8_e4m3fn) or (q_dtype != torch.bfloat16 and q_dtype != k_dtype):
+        raise ValueError(f"window_size needs k and v in bfloat16 or float8_e4m3fn and q in bfloat16 or their type, got q={q_dtype}, k={k_dtype}, v={v.dtype}")
+    nnz_qo, num_qo_heads, _ = q_shape
+    dev = q.device
+    index = dev.index
+    if any(t is not None and t.get_device() != index for t in (k, v, kv_indices, out, lse, plan["qo_offset"])):
+        cache._same_device(dev, k=k, v=v, kv_indices=kv_indices, out=out, lse=lse, plan=plan["qo_offset"])
+    if plan["_host"] is None:                 # planned on the device: total_qo_len is the bound max_total_q
+        if nnz_qo > plan["total_qo_len"]:
+            raise ValueError(f"plan allows at most {plan['total_qo_len']} query tokens, q has {nnz_qo}")
+    elif plan["total_qo_len"] != nnz_qo:
+        raise ValueError(f"plan was made for {plan['total_qo_len']} query tokens, q has {nnz_qo}")
+    if plan["orig_num_qo_heads"] != num_qo_heads or plan["num_kv_heads"] != num_kv_heads:
+        raise ValueError("plan head counts do not match q / k")
+    if check_input_valid and plan["_host"] is not None:
+        _validate_fmha_inputs(q, k, v, plan, paged, nhd, num_kv_heads, plan_page if paged else 0, kv_indices, None, plan["qo_offset"])
+    if out is None:
+        out = torch.empty(q_shape, device=dev, dtype=torch.bfloat16)
+    elif out.dtype not in (torch.bfloat16, torch.float32) or out.shape != q_shape or out.stride(2) != 1:
+        raise ValueError(f"out must be bfloat16 or float32 {tuple(q_shape)} with a contiguous head_dim, got {out.dtype} {tuple(out.shape)}")
+    if lse is not None and (lse.dtype != torch.float32 or lse.shape != (nnz_qo, num_qo_heads) or not lse.is_contiguous()):
+        raise ValueError(f"lse must be contiguous float32 {(nnz_qo, num_qo_heads)}, got {lse.dtype} {tuple(lse.shape)}")
+    if nnz_qo == 0:
+        return out, None
+    key = (q_dtype, k_dtype, nhd, _USE_TC, _FORCE_TC, _USE_DECODE_TC)
+    kept = plan.setdefault("_window_params", {})
+    base = kept.get(key)
+    if base is None:
+        base = kept[key] = _window_params(q_dtype, k_dtype, plan, nhd)
+    p, splits = _lib.MsaFmhaParams.from_buffer_copy(base[0]), base[1]
+    q_stride, k_stride, v_stride = q.stride(), k.stride(), v.stride()
+    if q_stride[2] != 1 or k_stride[-1] != 1 or v_stride[-1] != 1:
+        raise ValueError("head_dim of q, k and v must be contiguous")
+    p.q, p.k, p.v, p.status = q.data_ptr(), k.data_ptr(), v.data_ptr(), _status_ptr(dev)
+    p.q_stride_tok, p.q_stride_head, p.total_q, p.kv_extent = q_stride[0], q_stride[1], nnz_qo, k_shape[0]
+    if paged:
+        if kv_indices.dtype != torch.int32 or kv_indices.dim() != 1 or not kv_indices.is_contiguous():
+            raise ValueError("kv_indices must be a contiguous int32 vector")
+        p.kv_indices, p.num_page_entries = kv_indices.data_ptr(), kv_indices.shape[0]
+        tok, head = (1, 2) if nhd else (2, 1)
+        p.k_stride_page, p.k_stride_head, p.k_stride_tok = k_stride[0], k_stride[head], k_stride[tok]
+        p.v_stride_page, p.v_stride_head, p.v_stride_tok = v_stride[0], v_stride[head], v_stride[tok]
+    else:
+        p.k_stride_tok, p.k_stride_head, p.v_stride_tok, p.v_stride_head = k_stride[0], k_stride[1], v_stride[0], v_stride[1]
+    if q_scale is None and k_scale is None and v_scale is None and o_scale is None:
+        k_s, out_scale = 1.0, 1.0
+    else:
+        (k_s, k_head), (out_scale, v_head) = _scale_pair(q_scale, k_scale, dev, num_kv_heads), _scale_pair(o_scale, v_scale, dev, num_kv_heads)
+        p.k_scale_head, p.v_scale_head = _ptr(k_head), _ptr(v_head)
+    p.sm_scale, p.out_scale = float(k_s * (0.08838834764831845 if sm_scale is None else sm_scale)), out_scale    # 1 / sqrt(128)
+    if _SHOW_PARAMS:
+        _show_params(q, plan, paged, plan_page, 0.08838834764831845 if sm_scale is None else float(sm_scale), True, None, None)
+    with cache._on(dev):
+        stream = _stream()
+        # partials of its own: two streams, or two captured graphs, may run one plan at the same time
+        kernel_out = out
+        if splits > 1:
+            part = torch.empty(splits * nnz_qo * num_qo_heads * 129, dtype=torch.float32, device=dev)
+            p.partial_o = part.data_ptr()
+            p.partial_lse = part.data_ptr() + splits * nnz_qo * num_qo_heads * 512
+        else:
+            if out.dtype == torch.float32:
+                kernel_out = torch.empty(q_shape, dtype=torch.bfloat16, device=dev)
+            if lse is not None:
+                p.lse = lse.data_ptr()
+            o_stride = kernel_out.stride()
+            p.out, p.out_stride_tok, p.out_stride_head = kernel_out.data_ptr(), o_stride[0], o_stride[1]
+        _lib.check(_lib.lib.msa_fmha_fwd(ctypes.byref(p), stream), "msa_fmha_fwd")
+        if splits > 1:
+            _lib.check(_lib.lib.msa_lse_merge_many(
+                p.partial_o, p.partial_lse, _ptr(plan["num_kv_splits_per_row"]), out.data_ptr(), _dt_code(out.dtype), _ptr(lse),
+                splits, nnz_qo, num_qo_heads, out.stride(0), out.stride(1), out_scale, stream), "msa_lse_merge_many")
+        elif kernel_out is not out:
+            _copy_rows(out, kernel_out, plan)
+    return out, None
 
 
 def _fmha_sail_kv4(q, k, v, plan, kv_indices, kv_block_indexes, q_offset_override, out, max_score, sm_scale, q_scale, k_scale, v_scale,

@@ -12,6 +12,7 @@ updated in place on the current stream of its device; nothing is read back, so t
 No upstream counterpart (upstream starts at the attention call).
 """
 import ctypes
+import functools
 import struct
 from typing import NamedTuple, Optional, Sequence, Union
 
@@ -23,21 +24,22 @@ from .cache import KV4_ROW_BYTES, KV4_TILE, _check_index, _launch
 _CACHE = struct.Struct("@QqqiiiI")
 
 
-def _pieces(name, t, page_size, by_token):
-    """A cache tensor as ``MsaPageCache``s, packed.  ``by_token``: a page may be copied up to a token."""
-    shape, stride, size = t.shape, t.stride(), t.element_size()
+@functools.lru_cache(maxsize=256)
+def _pieces(shape, stride, size, kv4, page_size, by_token):
+    """Pieces of a page of a cache of this shape: (bytes from its start, page stride, stride of pieces, pieces, their bytes, bytes of a token), or
+    None if they are not evenly spaced.  ``by_token``: a page may be copied up to a token."""
     if by_token and len(shape) == 4:
-        if t.dtype == torch.uint8 and tuple(shape[2:]) == (KV4_TILE, KV4_ROW_BYTES) and stride[2:] == (KV4_ROW_BYTES, 1) and page_size == KV4_TILE:
+        if kv4 and shape[2:] == (KV4_TILE, KV4_ROW_BYTES) and stride[2:] == (KV4_ROW_BYTES, 1) and page_size == KV4_TILE:
             # a 4-bit cache: the codes of a page and head, then the scales
-            head, codes = (stride[0], stride[1], shape[1]), KV4_TILE * 64
-            return [_CACHE.pack(t.data_ptr(), *head, codes, 64, 0), _CACHE.pack(t.data_ptr() + codes, *head, KV4_TILE * 8, 8, 0)]
+            codes = KV4_TILE * 64
+            return [(0, stride[0], stride[1], shape[1], codes, 64), (codes, stride[0], stride[1], shape[1], KV4_TILE * 8, 8)]
         if shape[2] == page_size and stride[2:] == (shape[3], 1):             # HND
             row = shape[3] * size
-            return [_CACHE.pack(t.data_ptr(), stride[0] * size, stride[1] * size, shape[1], page_size * row, row, 0)]
+            return [(0, stride[0] * size, stride[1] * size, shape[1], page_size * row, row)]
         if shape[1] == page_size and stride[2:] == (shape[3], 1):             # NHD
             row = shape[2] * shape[3] * size
-            return [_CACHE.pack(t.data_ptr(), stride[0] * size, stride[1] * size, page_size, row, -1, 0)]
-    # pieces: the innermost dimensions as far as they are contiguous; what is left has to be one step
+            return [(0, stride[0] * size, stride[1] * size, page_size, row, -1)]
+    # the innermost dimensions as far as they are contiguous; what is left has to be one step
     length, d = 1, len(shape) - 1
     while d > 0 and (shape[d] == 1 or stride[d] == length):
         length *= shape[d]
@@ -50,52 +52,75 @@ def _pieces(name, t, page_size, by_token):
             parts *= shape[d]
             d -= 1
         if d > 0:
-            raise ValueError(f"{name}: a page must be one piece of memory or evenly spaced pieces, got shape {tuple(shape)}, strides {stride}")
-    return [_CACHE.pack(t.data_ptr(), stride[0] * size, step * size, parts, length * size, 0, 0)]
+            return None
+    return [(0, stride[0] * size, step * size, parts, length * size, 0)]
 
 
 def _cache_list(caches, num_pages, page_size, device, by_token=False):
-    """(packed caches, their number, pages)"""
+    """(packed ``MsaPageCache``s, their number, pages)"""
     if isinstance(caches, torch.Tensor):
         caches = (caches,)
-    packed = []
+    packed, index, like = [], device.index, None
     for i, t in enumerate(caches):
-        name = f"caches[{i}]"
-        if t.get_device() != device.index:
-            raise ValueError(f"{name} is on {t.device}, expected {device}")
-        if t.dim() < 1 or (num_pages is not None and t.shape[0] != num_pages):
-            raise ValueError(f"{name} must have {'pages' if num_pages is None else f'{num_pages} pages'} as its first dimension, got shape {tuple(t.shape)}")
-        num_pages = t.shape[0]
-        if num_pages > 1 and t.stride(0) == 0:
-            raise ValueError(f"{name}: pages must not overlap")
-        if t.numel():
-            packed += _pieces(name, t, page_size, by_token)
+        if t.get_device() != index:
+            raise ValueError(f"caches[{i}] is on {t.device}, expected {device}")
+        layout = t.shape, t.stride(), t.dtype
+        if layout == like:                    # the caches of a model's layers are alike
+            ptr = t.data_ptr()
+            for off, rest in pieces:
+                packed.append(pack(ptr + off, *rest))
+            continue
+        shape, stride, dtype = layout
+        if not shape or (num_pages is not None and shape[0] != num_pages):
+            raise ValueError(f"caches[{i}] must have {'pages' if num_pages is None else f'{num_pages} pages'} as its first dimension, got shape {tuple(shape)}")
+        num_pages = shape[0]
+        if 0 in shape:
+            continue
+        if num_pages > 1 and stride[0] == 0:
+            raise ValueError(f"caches[{i}]: pages must not overlap")
+        pieces = _pieces(shape, stride, dtype.itemsize, dtype is torch.uint8, page_size, by_token)
+        if pieces is None:
+            raise ValueError(f"caches[{i}]: a page must be one piece of memory or evenly spaced pieces, got shape {tuple(shape)}, strides {stride}")
+        like, pack, ptr = layout, _CACHE.pack, t.data_ptr()
+        pieces = [(off, (*rest, 0)) for off, *rest in pieces]
+        for off, rest in pieces:
+            packed.append(pack(ptr + off, *rest))
     return b"".join(packed), len(packed), num_pages
 
 
-def _table(block_table, num_held, free_pages, num_free, page_size):
-    """Checks of what every call but the copy has; (device, rows, width, stride)."""
-    if not block_table.is_cuda:
-        raise RuntimeError("pages of a cache need CUDA tensors (there is no CPU path)")
+def _address(packed):
+    """Where the bytes are, while `packed` lives."""
+    return ctypes.cast(packed, ctypes.c_void_p).value
+
+
+def _vector(name, t, n, device):
+    _check_index(name, t, device)
+    if n is not None and t.shape[0] != n:
+        raise ValueError(f"{name} must have {n} entries, got {t.shape[0]}")
+
+
+def _tables(block_table, page_size, rows, others):
+    """Checks of what every call but the copy has: ``rows``, int32 with an entry for each row of ``block_table``, and ``others``, int32 of given
+    lengths; (device, rows, width, stride)."""
     dev = block_table.device
-    if block_table.dim() != 2 or block_table.dtype != torch.int32 or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
-        raise ValueError(f"block_table must be int32 [B, width] with contiguous rows, got {block_table.dtype} {tuple(block_table.shape)}")
-    B, width = block_table.shape
-    if B > 1 and block_table.stride(0) < width:
+    index = dev.index
+    if dev.type != "cuda":
+        raise RuntimeError("pages of a cache need CUDA tensors (there is no CPU path)")
+    shape, stride, i32 = block_table.shape, block_table.stride(), torch.int32
+    if len(shape) != 2 or block_table.dtype is not i32 or (shape[1] > 1 and stride[1] != 1):
+        raise ValueError(f"block_table must be int32 [B, width] with contiguous rows, got {block_table.dtype} {tuple(shape)}")
+    B, width = shape
+    if B > 1 and stride[0] < width:
         raise ValueError("rows of block_table must not overlap")
-    for name, t, n in (("num_held", num_held, B), ("free_pages", free_pages, None), ("num_free", num_free, 1)):
-        _check_index(name, t, dev)
-        if n is not None and t.shape[0] != n:
-            raise ValueError(f"{name} must have {n} entries, got {t.shape[0]}")
+    for name, t in rows.items():
+        if t.dtype is not i32 or t.shape != (B,) or t.get_device() != index or not t.is_contiguous():
+            _vector(name, t, B, dev)
+    for name, (t, n) in others.items():
+        if t.dtype is not i32 or t.dim() != 1 or t.get_device() != index or not t.is_contiguous() or (n is not None and t.shape[0] != n):
+            _vector(name, t, n, dev)
     if not 1 <= page_size <= (1 << 31) - 1:
         raise ValueError(f"page_size={page_size} must be positive and fit int32")
-    return dev, B, width, block_table.stride(0) if B > 1 else width
-
-
-def _entries(name, t, n, device):
-    _check_index(name, t, device)
-    if t.shape[0] != n:
-        raise ValueError(f"{name} must have {n} entries, got {t.shape[0]}")
+    return dev, B, width, stride[0] if B > 1 else width
 
 
 def kv_pages_copy(caches: Union[torch.Tensor, Sequence[torch.Tensor]], src: torch.Tensor, dst: torch.Tensor) -> None:
@@ -106,16 +131,16 @@ def kv_pages_copy(caches: Union[torch.Tensor, Sequence[torch.Tensor]], src: torc
     entry with a negative number (a list of fixed size) copies nothing, nor does one past the pool.  Entries are copied in any order: a page of
     ``dst`` is there once and is not in ``src``."""
     first = caches if isinstance(caches, torch.Tensor) else caches[0] if len(caches) else src
-    if not first.is_cuda:
-        raise RuntimeError("kv_pages_copy needs CUDA tensors (there is no CPU path)")
     dev = first.device
-    _check_index("src", src, dev)
-    _entries("dst", dst, src.shape[0], dev)
+    if dev.type != "cuda":
+        raise RuntimeError("kv_pages_copy needs CUDA tensors (there is no CPU path)")
+    _vector("src", src, None, dev)
+    _vector("dst", dst, src.shape[0], dev)
     packed, n, num_pages = _cache_list(caches, None, 1, dev)
     if n == 0 or src.shape[0] == 0:
         return
     _launch(dev, _lib.lib.msa_pages_copy, _lib.pages_copy_args(
-        ctypes.cast(packed, ctypes.c_void_p).value, src.data_ptr(), dst.data_ptr(), cache._status_ptr(dev) or 0, n, src.shape[0], num_pages, 1), "msa_pages_copy")
+        _address(packed), src.data_ptr(), dst.data_ptr(), cache._status_ptr(dev) or 0, n, src.shape[0], num_pages, 1), "msa_pages_copy")
 
 
 def kv_pages_fork(block_table: torch.Tensor, num_held: torch.Tensor, kv_lens: torch.Tensor, parents: torch.Tensor, children: torch.Tensor,
@@ -132,18 +157,15 @@ def kv_pages_fork(block_table: torch.Tensor, num_held: torch.Tensor, kv_lens: to
     A child holds nothing before (``kv_pages_free`` it first).  Returns ``num_missing`` (int32 ``[1]``): entries that were not made, since a row is
     not in the table, is its own parent, holds pages already or is a child for the second time, and children that found no page on the
     stack for their last tokens, which end with their last full page (``kv_lens`` says where)."""
-    dev, B, width, stride = _table(block_table, num_held, free_pages, num_free, page_size)
-    _entries("kv_lens", kv_lens, B, dev)
-    _check_index("parents", parents, dev)
-    n = parents.shape[0]
-    _entries("children", children, n, dev)
-    _check_index("shares", shares, dev)
+    n = parents.numel()
+    dev, B, width, stride = _tables(block_table, page_size, {"num_held": num_held, "kv_lens": kv_lens}, {
+        "parents": (parents, n), "children": (children, n), "free_pages": (free_pages, None), "num_free": (num_free, 1), "shares": (shares, None)})
     packed, num, pages = _cache_list(caches, shares.shape[0], page_size, dev, True)
     ws = _lib.check(_lib.lib.msa_pages_fork_workspace_bytes(B, n), "msa_pages_fork_workspace_bytes") // 4
     buf = torch.empty(ws + 1, dtype=torch.int32, device=dev)
     ptr = buf.data_ptr()
     _launch(dev, _lib.lib.msa_pages_fork, _lib.pages_fork_args(
-        ctypes.cast(packed, ctypes.c_void_p).value, block_table.data_ptr(), num_held.data_ptr(), kv_lens.data_ptr(), parents.data_ptr(), children.data_ptr(),
+        _address(packed), block_table.data_ptr(), num_held.data_ptr(), kv_lens.data_ptr(), parents.data_ptr(), children.data_ptr(),
         free_pages.data_ptr(), num_free.data_ptr(), shares.data_ptr(), ptr, ptr + 4, stride, num, n, pages, page_size, B, width, free_pages.shape[0]),
         "msa_pages_fork")
     return buf[:1]
@@ -162,10 +184,10 @@ def kv_pages_free(block_table: torch.Tensor, num_held: torch.Tensor, kv_lens: to
     A page of several rows (``shares``) loses a share for each and goes onto the stack with the last; without ``shares`` each page is in one row.
     Pages are pushed in the order of the rows and their entries.  Returns ``num_freed`` (int32 ``[1]``): how many were pushed.  ``free_pages`` has
     room for every page of the pool."""
-    dev, B, width, stride = _table(block_table, num_held, free_pages, num_free, page_size)
-    _entries("kv_lens", kv_lens, B, dev)
+    others = {"free_pages": (free_pages, None), "num_free": (num_free, 1)}
     if shares is not None:
-        _check_index("shares", shares, dev)
+        others["shares"] = (shares, None)
+    dev, B, width, stride = _tables(block_table, page_size, {"num_held": num_held, "kv_lens": kv_lens}, others)
     window = -1 if window_size is None else int(window_size)
     if window == 0 or window < -1 or window > (1 << 31) - 1:
         raise ValueError(f"window_size must be -1 (no window) or from 1 to 2^31 - 1, got {window_size}")
@@ -198,11 +220,11 @@ def kv_pages_compact(block_table: torch.Tensor, num_held: torch.Tensor, free_pag
     kept for padding, say) stay where they are.  Of the pages in use above the line, the lowest goes to the lowest free place below it, and so on.
     ``block_table``, ``shares`` and the pages of all ``caches`` (as in ``kv_pages_copy``) follow, and the stack is made anew, the lowest page on top.
     The pool has ``num_pages`` pages, by default as many as the caches or ``shares``.  Tables made before (``kv_indices``, slots) are void."""
-    dev, B, width, stride = _table(block_table, num_held, free_pages, num_free, 1)
+    others = {"free_pages": (free_pages, None), "num_free": (num_free, 1)}
     if shares is not None:
-        _check_index("shares", shares, dev)
-        if num_pages is not None and shares.shape[0] != num_pages:
-            raise ValueError(f"shares must have {num_pages} entries, got {shares.shape[0]}")
+        others["shares"] = (shares, num_pages)
+    dev, B, width, stride = _tables(block_table, 1, {"num_held": num_held}, others)
+    if shares is not None:
         num_pages = shares.shape[0]
     packed, num, num_pages = _cache_list(caches, num_pages, 1, dev)
     if num_pages is None or not 0 <= num_pages <= (1 << 31) - 1:
@@ -210,7 +232,7 @@ def kv_pages_compact(block_table: torch.Tensor, num_held: torch.Tensor, free_pag
     ws = _lib.check(_lib.lib.msa_pages_compact_workspace_bytes(num_pages), "msa_pages_compact_workspace_bytes") // 4
     src, dst, num_moved, ws = torch.empty(2 * num_pages + 1 + ws, dtype=torch.int32, device=dev).split_with_sizes([num_pages, num_pages, 1, ws])
     _launch(dev, _lib.lib.msa_pages_compact, _lib.pages_compact_args(
-        ctypes.cast(packed, ctypes.c_void_p).value, block_table.data_ptr(), num_held.data_ptr(), free_pages.data_ptr(), num_free.data_ptr(),
+        _address(packed), block_table.data_ptr(), num_held.data_ptr(), free_pages.data_ptr(), num_free.data_ptr(),
         0 if shares is None else shares.data_ptr(), src.data_ptr(), dst.data_ptr(), num_moved.data_ptr(), ws.data_ptr(), stride, num, num_pages, 1, B, width,
         free_pages.shape[0]), "msa_pages_compact")
     return PageMoves(src, dst, num_moved)

@@ -221,7 +221,7 @@ def test_free_keeps_what_a_windowed_query_sees():
             assert {i for i, p in enumerate(t.tolist()[0][:pages]) if p >= 0} == need, (n, window, sinks)
 
 
-@pytest.mark.parametrize("rows,width,spare", [(1, 1, 0), (4, 9, 40), (50, 30, 0), (200, 20, 3000), (3, 2000, 100), (900, 130, 40000)])
+@pytest.mark.parametrize("rows,width,spare", [(1, 1, 0), (4, 9, 40), (50, 30, 0), (200, 20, 3000), (3, 2000, 100), (900, 130, 40000), (40, 30, 200000), (1300, 130, 500)])
 @pytest.mark.parametrize("sharing", [True, False])
 def test_compact(rows, width, spare, sharing):
     rng = random.Random(rows + width)
