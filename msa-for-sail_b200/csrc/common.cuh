@@ -180,6 +180,19 @@ __device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
   return d;
 }
 
+// Two values as pairs of e4m3 values, hi and lo (low 16 bits each).  hi is the value rounded to 4 significant bits: with t = (2^20 + 1) x,
+// t - (t - x) (Veltkamp's splitting); what it leaves is exact.  No conversion back from e4m3 is needed.  (Where hi is below e4m3's
+// normal numbers its conversion rounds once more, by at most 2^-10 where weights reach 2^4 to 2^8.)
+__device__ __forceinline__ void e4m3_pair(float a, float b, uint32_t& hi, uint32_t& lo) {
+  const uint64_t x = f2_pack(a, b), t = f2_fma(x, f2_pack(1048577.f, 1048577.f), 0), minus = f2_pack(-1.f, -1.f);
+  const uint64_t h = f2_fma(f2_fma(x, minus, t), minus, t), rest = f2_fma(h, minus, x);
+  float h0, h1, l0, l1;
+  f2_unpack(h, h0, h1);
+  f2_unpack(rest, l0, l1);
+  hi = __nv_cvt_float2_to_fp8x2(make_float2(h0, h1), __NV_SATFINITE, __NV_E4M3);
+  lo = __nv_cvt_float2_to_fp8x2(make_float2(l0, l1), __NV_SATFINITE, __NV_E4M3);
+}
+
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));

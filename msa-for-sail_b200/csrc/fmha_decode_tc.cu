@@ -45,11 +45,6 @@ __device__ __forceinline__ float2 e4m3x2_as_float2(uint16_t x) {
   return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
 
-// What two values leave that were rounded to r, as e4m3 (low 16 bits).
-__device__ __forceinline__ uint32_t e4m3_rest(float a, float b, float2 r) {
-  return __nv_cvt_float2_to_fp8x2(make_float2(a - r.x, b - r.y), __NV_SATFINITE, __NV_E4M3);
-}
-
 constexpr int BM = 128, BN = 128;
 constexpr int SUB_BYTES = BM * 128;             // one [128 rows][128 bytes] swizzled sub-tile
 constexpr int NTHREADS = 224;
@@ -93,8 +88,10 @@ __device__ __forceinline__ unsigned long long global_ns() {
 //   WIN   rows see a window and the first keys only; tiles that no row sees are not loaded.
 //   F8 && WIN ("pair"): Q and P are pairs of e4m3 values, x = hi + lo with lo = e4m3(x - hi), both multiplied into the same
 //         accumulator: 8 bits where one value has 4, for MMAs that have nothing else to do.  (A single value puts 2.6 % of noise on
-//         each weight: with a window there are few enough that it shows.)  Q_lo: rows 16-31 of each quadrant of the Q tile (dual),
-//         whose descriptor starts 2 KB later, or a tile of its own.
+//         each weight: with a window there are few enough that it shows.)  Q_lo is a tile of its own, or, with 16 rows (dual), rows 16-31
+//         of each quadrant: one MMA gives both parts of S, in lanes r and r + 16, which exchange what they need and go on as two
+//         softmaxes of half the quadrant's keys each, eight for a row.  (Q_lo as a second MMA there: 80 us instead of 66 for 64
+//         sequences x 8 heads x 2 112 keys.)
 template <bool F8, bool QUAD, bool WIN = false>
 struct Cfg {
   static constexpr bool DUAL = F8 && QUAD;
@@ -106,8 +103,9 @@ struct Cfg {
   static constexpr int STAGES = RING_BYTES / TILE_BYTES;  // bf16 3, e4m3 6 (dual: 6 half pages)
   static constexpr int V_STAGES = DUAL && WIN ? STAGES - 1 : STAGES;      // room for the barriers, see below
   static constexpr int OFF_Q = 0;
-  [[maybe_unused]] static constexpr int OFF_Q_LO = DUAL ? 2048 : SUB_BYTES;
-  // dual: rows 112-127 of the Q tile are never real rows (pairs: of Q_hi), the K ring may start there
+  static constexpr int OFF_Q_LO = SUB_BYTES;              // not dual
+  static constexpr int SPLIT = DUAL && PAIR ? 2 : 1;      // lanes that share a row's columns of a quadrant
+  // dual: rows 112-127 of the Q tile are never real rows (but for pairs), the K ring may start there
   static constexpr int OFF_K = DUAL && !PAIR ? SUB_BYTES - 2048 : DUAL ? SUB_BYTES : 2 * SUB_BYTES;
   static constexpr int OFF_V = OFF_K + RING_BYTES;
   static constexpr int END = OFF_V + V_STAGES * TILE_BYTES;
@@ -120,6 +118,7 @@ struct Cfg {
   static constexpr int MIN_CTAS = DUAL ? 2 : 1;
   static_assert(STAGES <= MAX_STAGES, "barrier table");
   static_assert(4 * QUAD_MAX_ROWS * STAGE_LD * 4 <= RING_BYTES, "O staging fits the K ring");
+  static_assert(4 * SPLIT * QUAD_MAX_ROWS * (STAGE_LD + 2) * 4 <= END - OFF_K, "... of pairs both rings");
 };
 
 template <bool F8, bool QUAD, bool WIN>
@@ -431,7 +430,7 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
         if constexpr (F8) mma_ss_f8(sbuf(j), dk_hi | ((qa + o) & 0x3FFF), dk_hi | ((ka + o) & 0x3FFF), IDESC_QK, k > 0);
         else mma_ss(sbuf(j), dk_hi | ((qa + o) & 0x3FFF), dk_hi | ((ka + o) & 0x3FFF), IDESC_QK, k > 0);
       }
-      if constexpr (PAIR) {
+      if constexpr (PAIR && !QUAD) {
         if (p.q_dtype == MSA_DT_BF16) {
           const uint32_t ql = (smem_base + C::OFF_Q_LO) >> 4;
 #pragma unroll
@@ -488,7 +487,8 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
   } else if (warp < n_active_warps) {
     // =========================== softmax / epilogue ===========================
     const int trow = (warp << 5) | lane;                     // row of the MMA tile == TMEM lane
-    const int r = QUAD ? lane : trow;                        // logical row of the work item
+    const int r = C::SPLIT == 2 ? lane & 15 : QUAD ? lane : trow;        // logical row of the work item
+    const int half = C::SPLIT == 2 ? lane >> 4 : 0;          // which half of the quadrant's columns of the row this lane has
     const uint32_t lane_addr = static_cast<uint32_t>(warp << 5) << 16;
     const uint32_t tO = tmem + C::O_COL + lane_addr;
     const bool row_ok = r < nrows;
@@ -552,8 +552,10 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
                 hi[e] = static_cast<uint32_t>(h[0]) | (static_cast<uint32_t>(h[1]) << 16);
                 lo[e] = static_cast<uint32_t>(l[0]) | (static_cast<uint32_t>(l[1]) << 16);
               }
-              chunks[c] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-              *reinterpret_cast<uint4*>(smem_gen + C::OFF_Q_LO + trow * 128 + ((c ^ (trow & 7)) << 4)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+              if (C::SPLIT == 2 && half) chunks[c] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+              else chunks[c] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+              if constexpr (C::SPLIT == 1)
+                *reinterpret_cast<uint4*>(smem_gen + C::OFF_Q_LO + trow * 128 + ((c ^ (trow & 7)) << 4)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
             }
           } else {
             const uint4* src = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.q) +
@@ -577,7 +579,7 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
           }
         }
         // QUAD: only the real rows are written (rows 16-31 of the first quadrant hold the
-        // barriers; what the MMA reads from unused rows only reaches unused TMEM lanes)
+        // barriers, but for pairs; what the MMA reads from unused rows only reaches unused TMEM lanes)
         if (!QUAD || row_ok) {
 #pragma unroll
           for (int c = 0; c < 8; ++c)
@@ -597,12 +599,26 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
         if (trace && j == 12) trace[4] = clock64() - clk0;       // S of tile 12 ready
         if (trace && j == 13) trace[14] = clock64() - clk0;
         tc_fence_after();
-        constexpr int CW = TK / 4;                           // key columns of a tile per quadrant
-        const int pos0 = tile_key0(j) + warp * CW;
+        constexpr int QW = TK / 4, CW = QW / C::SPLIT;       // key columns of a tile per quadrant, and of this lane
+        const int pos0 = tile_key0(j) + warp * QW + half * CW;
         uint32_t sv[CW];
-        if constexpr (CW == 32) tmem_ld32(tS + warp * CW, sv);
-        else tmem_ld16(tS + warp * CW, sv);
-        tmem_wait_ld();
+        if constexpr (C::SPLIT == 2) {
+          // lane r: q_hi k, lane r + 16: q_lo k (or q k in both, if q is e4m3)
+          uint32_t both[QW];
+          tmem_ld16(tS + warp * QW, both);
+          tmem_wait_ld();
+          const bool pair_q = p.q_dtype == MSA_DT_BF16;
+#pragma unroll
+          for (int e = 0; e < CW; ++e) {
+            const float mine = __uint_as_float(half ? both[CW + e] : both[e]);
+            const float other = __uint_as_float(__shfl_xor_sync(0xffffffffu, half ? both[e] : both[CW + e], 16));
+            sv[e] = __float_as_uint(pair_q ? mine + other : mine);
+          }
+        } else {
+          if constexpr (CW == 32) tmem_ld32(tS + warp * CW, sv);
+          else tmem_ld16(tS + warp * CW, sv);
+          tmem_wait_ld();
+        }
         if (trace && j == 12) trace[5] = clock64() - clk0;       // ... loaded
         if (pos0 + CW - 1 > lim) {
 #pragma unroll
@@ -652,16 +668,20 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
             const float p1 = exp2_fast(fmaf(__uint_as_float(sv[e + 1]), scale_log2, -msafe));
             const float p2 = exp2_fast(fmaf(__uint_as_float(sv[e + 2]), scale_log2, -msafe));
             const float p3 = exp2_fast(fmaf(__uint_as_float(sv[e + 3]), scale_log2, -msafe));
-            const uint16_t lo = __nv_cvt_float2_to_fp8x2(make_float2(p0, p1), __NV_SATFINITE, __NV_E4M3);
-            const uint16_t hi = __nv_cvt_float2_to_fp8x2(make_float2(p2, p3), __NV_SATFINITE, __NV_E4M3);
-            const float2 ra = e4m3x2_as_float2(lo), rb = e4m3x2_as_float2(hi);
             if constexpr (PAIR) {
+              uint32_t a, b, c, d;
+              e4m3_pair(p0, p1, a, b);
+              e4m3_pair(p2, p3, c, d);
               l0 += p0 + p2; l1 += p1 + p3;
-              pl[e >> 2] = e4m3_rest(p0, p1, ra) | (e4m3_rest(p2, p3, rb) << 16);
+              pk[e >> 2] = a | (c << 16);
+              pl[e >> 2] = b | (d << 16);
             } else {
+              const uint16_t lo = __nv_cvt_float2_to_fp8x2(make_float2(p0, p1), __NV_SATFINITE, __NV_E4M3);
+              const uint16_t hi = __nv_cvt_float2_to_fp8x2(make_float2(p2, p3), __NV_SATFINITE, __NV_E4M3);
+              const float2 ra = e4m3x2_as_float2(lo), rb = e4m3x2_as_float2(hi);
               l0 += ra.x + rb.x; l1 += ra.y + rb.y;
+              pk[e >> 2] = static_cast<uint32_t>(lo) | (static_cast<uint32_t>(hi) << 16);
             }
-            pk[e >> 2] = static_cast<uint32_t>(lo) | (static_cast<uint32_t>(hi) << 16);
           }
         } else {
 #pragma unroll
@@ -674,16 +694,20 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
           }
         }
         // P of this quadrant's rows: own keys, zero for the other three quarters of the tile
-        if constexpr (PCOLS == 4) {                           // 16 columns in all: one store
+        if constexpr (C::SPLIT == 2) {
+          const int own = 2 * warp + half;                    // of eight pairs of columns
+          uint32_t all[16];
+#pragma unroll
+          for (int c = 0; c < 16; ++c) all[c] = (c >> 1) == own ? pk[c & 1] : 0u;
+          tmem_st16(tS, all);
+#pragma unroll
+          for (int c = 0; c < 16; ++c) all[c] = (c >> 1) == own ? pl[c & 1] : 0u;
+          tmem_st16(tS + TK / 4, all);
+        } else if constexpr (PCOLS == 4) {                           // 16 columns in all: one store
           uint32_t all[16];
 #pragma unroll
           for (int c = 0; c < 16; ++c) all[c] = (c >> 2) == warp ? pk[c & 3] : 0u;
           tmem_st16(tS, all);
-          if constexpr (PAIR) {
-#pragma unroll
-            for (int c = 0; c < 16; ++c) all[c] = (c >> 2) == warp ? pl[c & 3] : 0u;
-            tmem_st16(tS + TK / 4, all);
-          }
         } else {
           uint32_t zero[PCOLS];
 #pragma unroll
@@ -783,16 +807,20 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
             const float p1 = exp2_fast(fmaf(__uint_as_float(sv[c][e + 1]), scale_log2, -msafe));
             const float p2 = exp2_fast(fmaf(__uint_as_float(sv[c][e + 2]), scale_log2, -msafe));
             const float p3 = exp2_fast(fmaf(__uint_as_float(sv[c][e + 3]), scale_log2, -msafe));
-            const uint16_t lo = __nv_cvt_float2_to_fp8x2(make_float2(p0, p1), __NV_SATFINITE, __NV_E4M3);
-            const uint16_t hi = __nv_cvt_float2_to_fp8x2(make_float2(p2, p3), __NV_SATFINITE, __NV_E4M3);
-            const float2 ra = e4m3x2_as_float2(lo), rb = e4m3x2_as_float2(hi);
             if constexpr (PAIR) {
+              uint32_t a, b, c, d;
+              e4m3_pair(p0, p1, a, b);
+              e4m3_pair(p2, p3, c, d);
               l0 += p0 + p2; l1 += p1 + p3;
-              pl[e >> 2] = e4m3_rest(p0, p1, ra) | (e4m3_rest(p2, p3, rb) << 16);
+              pk[e >> 2] = a | (c << 16);
+              pl[e >> 2] = b | (d << 16);
             } else {
+              const uint16_t lo = __nv_cvt_float2_to_fp8x2(make_float2(p0, p1), __NV_SATFINITE, __NV_E4M3);
+              const uint16_t hi = __nv_cvt_float2_to_fp8x2(make_float2(p2, p3), __NV_SATFINITE, __NV_E4M3);
+              const float2 ra = e4m3x2_as_float2(lo), rb = e4m3x2_as_float2(hi);
               l0 += ra.x + rb.x; l1 += ra.y + rb.y;
+              pk[e >> 2] = static_cast<uint32_t>(lo) | (static_cast<uint32_t>(hi) << 16);
             }
-            pk[e >> 2] = static_cast<uint32_t>(lo) | (static_cast<uint32_t>(hi) << 16);
           }
           tmem_st8(tS + c * 8, pk);
           if constexpr (PAIR) tmem_st8(tS + TK / 4 + c * 8, pl);
@@ -823,9 +851,11 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
     if constexpr (QUAD) {
       // every MMA and every TMA load of this CTA has completed: the K ring is free to stage the
       // four partial results of each row; thread t then combines column t of every row
-      float* stage = reinterpret_cast<float*>(smem_gen + OFF_K);              // [4][nrows][STAGE_LD]
-      float* st_m = reinterpret_cast<float*>(smem_gen + OFF_V);               // [4][QUAD_MAX_ROWS]
-      float* st_l = st_m + 4 * QUAD_MAX_ROWS;
+      constexpr int PARTS = 4 * C::SPLIT;                                     // results of a row
+      float* stage = reinterpret_cast<float*>(smem_gen + OFF_K);              // [PARTS][nrows][STAGE_LD]
+      float* st_m = C::SPLIT == 1 ? reinterpret_cast<float*>(smem_gen + OFF_V) : stage + PARTS * QUAD_MAX_ROWS * STAGE_LD;    // [PARTS][QUAD_MAX_ROWS]
+      float* st_l = st_m + PARTS * QUAD_MAX_ROWS;
+      const int part = C::SPLIT * warp + half;
       if (alive && has_o) {
         tc_fence_after();
 #pragma unroll
@@ -839,14 +869,14 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
             for (int e = 0; e < 32; ++e) v[e] = 0u;
           }
           if (row_ok) {
-            float* dst = stage + (warp * nrows + r) * STAGE_LD + c * 32;
+            float* dst = stage + (part * nrows + r) * STAGE_LD + c * 32;
 #pragma unroll
             for (int e = 0; e < 32; e += 4)
               *reinterpret_cast<float4*>(dst + e) = make_float4(__uint_as_float(v[e]), __uint_as_float(v[e + 1]),
                                                                 __uint_as_float(v[e + 2]), __uint_as_float(v[e + 3]));
           }
         }
-        if (row_ok) { st_m[warp * QUAD_MAX_ROWS + r] = m_used; st_l[warp * QUAD_MAX_ROWS + r] = l_sum; }
+        if (row_ok) { st_m[part * QUAD_MAX_ROWS + r] = m_used; st_l[part * QUAD_MAX_ROWS + r] = l_sum; }
       }
       if (trace) trace[10] = clock64() - clk0;
       asm volatile("bar.sync 1, 128;" ::: "memory");
@@ -858,11 +888,11 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
         const bool to_partial = p.partial_o != nullptr;
         const int c8 = (trow & 15) * 8;
         for (int rr = trow >> 4; rr < nrows; rr += 8) {
-          float mq[4], wq[4], M = -INFINITY, L = 0.f;
+          float mq[PARTS], wq[PARTS], M = -INFINITY, L = 0.f;
 #pragma unroll
-          for (int q = 0; q < 4; ++q) { mq[q] = st_m[q * QUAD_MAX_ROWS + rr]; M = fmaxf(M, mq[q]); }
+          for (int q = 0; q < PARTS; ++q) { mq[q] = st_m[q * QUAD_MAX_ROWS + rr]; M = fmaxf(M, mq[q]); }
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
+          for (int q = 0; q < PARTS; ++q) {
             wq[q] = (mq[q] == -INFINITY) ? 0.f : exp2_fast(mq[q] - M);
             L += st_l[q * QUAD_MAX_ROWS + rr] * wq[q];
           }
@@ -871,7 +901,7 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
 #pragma unroll
           for (int e = 0; e < 8; ++e) acc[e] = 0.f;
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
+          for (int q = 0; q < PARTS; ++q) {
             const float4 a0 = *reinterpret_cast<const float4*>(stage + (q * nrows + rr) * STAGE_LD + c8);
             const float4 a1 = *reinterpret_cast<const float4*>(stage + (q * nrows + rr) * STAGE_LD + c8 + 4);
             const float w = wq[q] * inv;                      // a quadrant that saw no key has weight 0 and O == 0

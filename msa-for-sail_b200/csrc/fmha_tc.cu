@@ -703,7 +703,7 @@ fmha_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant__ 
           for (int c = 0; c < 4; ++c) {
             uint32_t pk[F8 ? 8 : 16];
             [[maybe_unused]] uint32_t pl[PAIR ? 8 : 1];
-            [[maybe_unused]] uint16_t held = 0, held_lo = 0;
+            [[maybe_unused]] uint32_t held = 0, held_lo = 0;
 #pragma unroll
             for (int e = 0; e < 32; e += 2) {
               if constexpr (decltype(with_max)::value)
@@ -735,17 +735,22 @@ fmha_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant__ 
                 // O is normalised by the sum of the probabilities as the MMA sees them (see the decode kernel);
                 // the LSE reports the sum before rounding
                 lex2 = f2_add(lex2, f2_pack(p0, p1));
-                const uint16_t pr = __nv_cvt_float2_to_fp8x2(make_float2(p0, p1), __NV_SATFINITE, __NV_E4M3);
-                const float2 rr = e4m3x2_to_float2(pr);
                 if constexpr (PAIR) {
-                  const uint16_t lo = __nv_cvt_float2_to_fp8x2(make_float2(p0 - rr.x, p1 - rr.y), __NV_SATFINITE, __NV_E4M3);
-                  if (e & 2) pl[e >> 2] = static_cast<uint32_t>(held_lo) | (static_cast<uint32_t>(lo) << 16);
-                  else held_lo = lo;
+                  uint32_t hi, lo;
+                  e4m3_pair(p0, p1, hi, lo);
+                  if (e & 2) {
+                    pk[e >> 2] = held | (hi << 16);
+                    pl[e >> 2] = held_lo | (lo << 16);
+                  } else {
+                    held = hi; held_lo = lo;
+                  }
                 } else {
+                  const uint16_t pr = __nv_cvt_float2_to_fp8x2(make_float2(p0, p1), __NV_SATFINITE, __NV_E4M3);
+                  const float2 rr = e4m3x2_to_float2(pr);
                   lsum2 = f2_add(lsum2, f2_pack(rr.x, rr.y));
+                  if (e & 2) pk[e >> 2] = static_cast<uint32_t>(held) | (static_cast<uint32_t>(pr) << 16);
+                  else held = pr;
                 }
-                if (e & 2) pk[e >> 2] = static_cast<uint32_t>(held) | (static_cast<uint32_t>(pr) << 16);
-                else held = pr;
               } else {
                 lsum2 = f2_add(lsum2, f2_pack(p0, p1));
                 pk[e >> 1] = pack2<false>(p0, p1);
