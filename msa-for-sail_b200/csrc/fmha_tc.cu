@@ -206,6 +206,12 @@ fmha_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant__ 
   [[maybe_unused]] auto has_tile = [&](const Item& w, int x, int j) -> bool {
     return x == 0 ? j < w.n_tiles[0] : j < w.n_tiles[1] && (j < sink_tiles(p.sink_tokens) || j >= w.b_first);
   };
+  // Up to 32 sink tokens in the last of their tiles, with tiles left out behind it: all rows see those keys of the tile, and that is all it is
+  // multiplied for (S and P of 32 columns).
+  [[maybe_unused]] auto is_short = [&](const Item& w, int j) -> bool {
+    const int rest = p.sink_tokens % BN;
+    return w.skip > 0 && j == sink_tiles(p.sink_tokens) - 1 && rest >= 1 && rest <= 32;
+  };
   [[maybe_unused]] auto has_unseen = [&](const Item& w, int key0) -> bool {
     return key0 + BN > w.end_key || (key0 < w.first_key && key0 + BN > p.sink_tokens);
   };
@@ -408,31 +414,36 @@ fmha_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant__ 
     // MN-major V: LBO 16384 B (next sub-tile of head_dim), SBO 1024 B (next 8 keys)
     const uint64_t dk_hi = smem_desc(0, 16, 1024) & 0xFFFFFFFFFFFF0000ull;
     const uint64_t dv_hi = smem_desc(0, SUB_BYTES, 1024) & 0xFFFFFFFFFFFF0000ull;
-    auto issue_qk = [&](int x, uint32_t kt) {
+    auto issue_qk = [&](int x, uint32_t kt, uint32_t idesc) {
       const uint32_t qa = (smem_base + OFF_Q + x * TILE_BYTES) >> 4;
       const uint32_t ka = (smem_base + OFF_K + (kt % KSTAGES) * TILE_BYTES) >> 4;
 #pragma unroll
       for (int k = 0; k < KSTEPS; ++k) {
         const uint32_t o = ((k >> 2) * SUB_BYTES + (k & 3) * 32) >> 4;
-        if constexpr (F8) mma_ss_f8(tmem + x * BN, dk_hi | ((qa + o) & 0x3FFF), dk_hi | ((ka + o) & 0x3FFF), IDESC_QK, k > 0);
-        else mma_ss(tmem + x * BN, dk_hi | ((qa + o) & 0x3FFF), dk_hi | ((ka + o) & 0x3FFF), IDESC_QK, k > 0);
+        if constexpr (F8) mma_ss_f8(tmem + x * BN, dk_hi | ((qa + o) & 0x3FFF), dk_hi | ((ka + o) & 0x3FFF), idesc, k > 0);
+        else mma_ss(tmem + x * BN, dk_hi | ((qa + o) & 0x3FFF), dk_hi | ((ka + o) & 0x3FFF), idesc, k > 0);
       }
     };
-    auto issue_pv = [&](int x, uint32_t vt, bool first) {
+    // (few: the first 32 keys only)
+    auto issue_pv = [&](int x, uint32_t vt, bool first, bool few) {
       const uint32_t va = (smem_base + OFF_V + (vt % VSTAGES) * TILE_BYTES) >> 4;
 #pragma unroll
       for (int k = 0; k < KSTEPS; ++k) {              // P: 8 TMEM columns per MMA in both formats
         const uint64_t vd = dv_hi | ((va + k * (V_KSTEP >> 4)) & 0x3FFF);
         if constexpr (F8) mma_ts_f8(tmem + 256 + x * kHeadDim, tmem + x * BN + k * 8, vd, IDESC_PV, (!first || k > 0) ? 1u : 0u);
         else mma_ts(tmem + 256 + x * kHeadDim, tmem + x * BN + k * 8, vd, IDESC_PV, (!first || k > 0) ? 1u : 0u);
+        if (WIN && few && k + 1 == KSTEPS / 4) break;
       }
     };
-    [[maybe_unused]] auto issue_pv_lo = [&](int x, uint32_t vt) {   // the second values of P, behind the first ones
+    [[maybe_unused]] auto issue_pv_lo = [&](int x, uint32_t vt, bool few) {   // the second values of P, behind the first ones
       const uint32_t va = (smem_base + OFF_V + (vt % VSTAGES) * TILE_BYTES) >> 4;
 #pragma unroll
-      for (int k = 0; k < KSTEPS; ++k)
+      for (int k = 0; k < KSTEPS; ++k) {
         mma_ts_f8(tmem + 256 + x * kHeadDim, tmem + x * BN + BN / 4 + k * 8, dv_hi | ((va + k * (V_KSTEP >> 4)) & 0x3FFF), IDESC_PV, 1u);
+        if (few && k + 1 == KSTEPS / 4) break;
+      }
     };
+    [[maybe_unused]] constexpr uint32_t IDESC_QK_SHORT = F8 ? idesc_e4m3(BM, 32, false, false) : idesc_bf16(BM, 32, false, false);
     uint32_t tile = 0, q_loads = 0;                    // running counts, as in the producer
     [[maybe_unused]] uint32_t p_par = 0;               // bit x: parity of the next P_FULL + x
     [[maybe_unused]] uint32_t n_s[2] = {0, 0};         // score-only: S pairs issued so far
@@ -484,7 +495,7 @@ fmha_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant__ 
         if (elect_one()) {
 #pragma unroll
           for (int x = 0; x < 2; ++x)
-            if (has_tile(w, x, 0)) { issue_qk(x, tile); mma_commit(bar(S_FULL + x)); }
+            if (has_tile(w, x, 0)) { issue_qk(x, tile, is_short(w, 0) ? IDESC_QK_SHORT : IDESC_QK); mma_commit(bar(S_FULL + x)); }
           mma_commit(bar(K_EMPTY + tile % KSTAGES));
           if (n_total == 1) mma_commit(bar(Q_EMPTY));
         }
@@ -506,10 +517,10 @@ fmha_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant__ 
             tc_fence_after();
             if (elect_one()) {
               if (now) {
-                issue_pv(x, tile, !((begun >> x) & 1));
-                if constexpr (PAIR) issue_pv_lo(x, tile);
+                issue_pv(x, tile, !((begun >> x) & 1), is_short(w, j));
+                if constexpr (PAIR) issue_pv_lo(x, tile, is_short(w, j));
               }
-              if (next) { issue_qk(x, tile + 1); mma_commit(bar(S_FULL + x)); }
+              if (next) { issue_qk(x, tile + 1, is_short(w, j + 1) ? IDESC_QK_SHORT : IDESC_QK); mma_commit(bar(S_FULL + x)); }
               if (now && j + 1 == w.n_tiles[x]) mma_commit(bar(O_FULL + x));
             }
             __syncwarp();
@@ -528,7 +539,7 @@ fmha_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant__ 
       if (elect_one()) {                               // S of both tiles is free: the last P has been waited for
 #pragma unroll
         for (int x = 0; x < 2; ++x)
-          if (w.n_tiles[x] > 0) { issue_qk(x, tile); mma_commit(bar(S_FULL + x)); }
+          if (w.n_tiles[x] > 0) { issue_qk(x, tile, IDESC_QK); mma_commit(bar(S_FULL + x)); }
         mma_commit(bar(K_EMPTY + tile % KSTAGES));
         if (n_total == 1) mma_commit(bar(Q_EMPTY));
       }
@@ -552,9 +563,9 @@ fmha_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant__ 
           tc_fence_after();
           if (lane == 0) trace(2, j, x * 4 + 2);
           if (elect_one()) {
-            issue_pv(x, tile, j == 0);
+            issue_pv(x, tile, j == 0, false);
             if (more) {
-              issue_qk(x, tile + 1);
+              issue_qk(x, tile + 1, IDESC_QK);
               mma_commit(bar(S_FULL + x));
             } else {
               mma_commit(bar(O_FULL + x));
@@ -588,7 +599,8 @@ fmha_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant__ 
           if (!alive) break;
           fix_par ^= 1u << vs;
           unsigned char* vt = smem_gen + OFF_V + vs * TILE_BYTES;
-          for (int c = lane; c < BN * (NSUB * 8); c += 32) {
+          const int rows = is_short(w, j) ? 32 : BN;          // that are multiplied
+          for (int c = lane; c < rows * (NSUB * 8); c += 32) {
             const int r = c / (NSUB * 8), ch = c % (NSUB * 8), key = key0 + r;
             if (key >= w.end_key || (key < w.first_key && key >= p.sink_tokens))
               *reinterpret_cast<uint4*>(vt + (ch >> 3) * SUB_BYTES + r * 128 + (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
@@ -642,6 +654,62 @@ fmha_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant__ 
         const uint32_t tS = tmem + (HAS_O ? x * BN : x * 2 * BN + (j & 1) * BN) + lane_addr;
         tc_fence_after();
         if (r == 0) trace(x, j, 1);
+        if constexpr (WIN) {
+          if (is_short(w, j)) {
+            // S of 32 keys, the first `rest` of which every row sees
+            const int rest = p.sink_tokens % BN;
+            uint32_t s32[32];
+            tmem_ld32(tS, s32);
+            tmem_wait_ld();
+            float top = -INFINITY;
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+              if (e >= rest) s32[e] = 0xff800000u;
+              top = fmaxf(top, __uint_as_float(s32[e]));
+            }
+            const float m_cand = fmaxf(m_used, top * scale_log2);
+            const bool bump = (m_cand - m_used) > kRescaleThreshold;
+            float factor = 1.f;
+            if (bump) { factor = exp2_fast(m_used - m_cand); m_used = m_cand; l_sum *= factor; l_exact *= factor; }
+            if (later && __any_sync(0xffffffffu, bump)) {
+#pragma unroll
+              for (int c = 0; c < 4; ++c) {
+                uint32_t v[32];
+                tmem_ld32(tO + c * 32, v);
+                tmem_wait_ld();
+#pragma unroll
+                for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * factor);
+                tmem_st32(tO + c * 32, v);
+              }
+            }
+            const float m_ref = ((m_used == -INFINITY) ? 0.f : m_used) - kPOffset;
+            float l0 = 0.f, l1 = 0.f;
+            uint32_t pk[F8 ? 8 : 16];
+            [[maybe_unused]] uint32_t pl[8];
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+              const float p0 = exp2_fast(fmaf(__uint_as_float(s32[e]), scale_log2, -m_ref));
+              const float p1 = exp2_fast(fmaf(__uint_as_float(s32[e + 1]), scale_log2, -m_ref));
+              l0 += p0; l1 += p1;
+              if constexpr (F8) {
+                uint32_t hi, lo;
+                e4m3_pair(p0, p1, hi, lo);
+                pk[e >> 2] = (e & 2) ? pk[e >> 2] | (hi << 16) : hi;
+                pl[e >> 2] = (e & 2) ? pl[e >> 2] | (lo << 16) : lo;
+              } else {
+                pk[e >> 1] = pack2<false>(p0, p1);
+              }
+            }
+            if constexpr (F8) { tmem_st8(tS, pk); tmem_st8(tS + BN / 4, pl); }
+            else tmem_st16(tS, pk);
+            l_sum += l0 + l1;
+            l_exact += l0 + l1;
+            tmem_wait_st();
+            tc_fence_before();
+            mbar_arrive(bar(P_FULL + x));
+            continue;
+          }
+        }
         const int pos0 = (WIN ? real_tile(w, j) : j) * BN;
         const bool need_mask = (pos0 + BN - 1 > m0 + off) || (pos0 + BN > kv_len) || (WIN && pos0 < from_last && pos0 + BN > p.sink_tokens);
         // ---- one read of the whole S row (128 fp32) ----
@@ -656,12 +724,23 @@ fmha_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant__ 
           tc_fence_before();
           mbar_arrive(bar(P_FULL + x));
         }
-        if (need_mask) {
+        if (WIN && need_mask) {
+          // one bit for each key that the row sees: a test and a select an element, where three comparisons would be needed
+          auto below = [](int n) -> uint32_t { return n <= 0 ? 0u : 0xffffffffu >> (32 - min(n, 32)); };     // the first n bits
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const int k0 = pos0 + c * 32;
+            const uint32_t seen = below(lim + 1 - k0) & (~below(from - k0) | below(p.sink_tokens - k0));
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (!(seen & (1u << e))) sv[c][e] = 0xff800000u;         // -inf
+          }
+        } else if (need_mask) {
 #pragma unroll
           for (int c = 0; c < 4; ++c)
 #pragma unroll
             for (int e = 0; e < 32; ++e)
-              if (pos0 + c * 32 + e > lim || (WIN && pos0 + c * 32 + e < from && pos0 + c * 32 + e >= p.sink_tokens)) sv[c][e] = 0xff800000u;     // -inf
+              if (pos0 + c * 32 + e > lim) sv[c][e] = 0xff800000u;     // -inf
         }
         auto store_score = [&](const float mx) {
           if (want_score && row_ok && j < p.max_k_tiles) {
@@ -710,7 +789,7 @@ fmha_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant__ 
                 mxs[(e >> 1) & 3] = max3(mxs[(e >> 1) & 3], __uint_as_float(sv[c][e]), __uint_as_float(sv[c][e + 1]));
               const uint64_t x2 = f2_fma(f2_pack(__uint_as_float(sv[c][e]), __uint_as_float(sv[c][e + 1])), scale2, negm2);
               float p0, p1;
-              if ((kEmuMask >> ((e >> 1) & 15)) & 1) {
+              if (!PAIR && ((kEmuMask >> ((e >> 1) & 15)) & 1)) {
                 float x0, x1;
                 f2_unpack(x2, x0, x1);
                 const uint64_t xc = f2_pack(fmaxf(x0, -126.f), fmaxf(x1, -126.f));     // also maps -inf

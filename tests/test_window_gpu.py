@@ -92,6 +92,17 @@ class Case:
         return out
 
 
+@pytest.fixture(params=["chosen", "generic", "tcgen05"])
+def kernels(request):
+    """The kernels that a call takes by itself, the generic one, and the tcgen05 ones wherever they can."""
+    from msa_for_sail import api
+    old = api._USE_TC, api._FORCE_TC, api._USE_DECODE_TC
+    if request.param != "chosen":
+        api._USE_TC = api._FORCE_TC = api._USE_DECODE_TC = request.param == "tcgen05"
+    yield request.param
+    api._USE_TC, api._FORCE_TC, api._USE_DECODE_TC = old
+
+
 LAYOUTS = [("ragged", 0), ("hnd", 128), ("nhd", 128), ("hnd", 16), ("nhd", 64)]
 BF, E4 = torch.bfloat16, torch.float8_e4m3fn
 
@@ -116,20 +127,20 @@ def test_a_few_tokens(heads, tokens, types):
 @pytest.mark.parametrize("layout,page", LAYOUTS)
 @pytest.mark.parametrize("types", [(BF, BF), (E4, E4), (BF, E4)])
 @pytest.mark.parametrize("window,sinks", [(1, 0), (64, 1), (127, 4), (128, 128), (300, 0), (513, 200), (10000, 7)])
-def test_prompts(layout, page, types, window, sinks):
+def test_prompts(kernels, layout, page, types, window, sinks):
     Case([700, 129, 1, 256, 0, 300], [700, 1000, 500, 256, 40, 333], 8, 2, window, sinks, layout, page, *types).check()
 
 
 @pytest.mark.parametrize("types", [(BF, BF), (E4, E4)])
-@pytest.mark.parametrize("window,sinks", [(1, 0), (200, 300), (1000, 0), (4096, 4)])
-def test_a_chunk_behind_a_long_prefix(types, window, sinks):
+@pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (200, 300), (1000, 0), (4096, 4), (300, 32), (300, 33), (500, 160), (500, 250), (64, 128)])
+def test_a_chunk_behind_a_long_prefix(kernels, types, window, sinks):
     Case([1000], [9001], 4, 1, window, sinks, "hnd", 128, *types).check()
 
 
 @pytest.mark.parametrize("n", [1, 3, 140, 300])
 @pytest.mark.parametrize("layout,page", [("hnd", 128), ("ragged", 0), ("hnd", 16)])
 @pytest.mark.parametrize("types", [(BF, BF), (E4, E4), (BF, E4)])
-def test_places_before_and_behind_the_keys(n, layout, page, types):
+def test_places_before_and_behind_the_keys(kernels, n, layout, page, types):
     """Offsets of the caller's own: rows before the first key see nothing, rows far behind the last one the sinks alone."""
     kl = [500, 500, 500, 500, 0, 130]
     Case([n] * 6, kl, 8, 2, 100, 40, layout, page, *types, offsets=[700, 450, 5000000, 0, 10, 200]).check()
@@ -154,7 +165,7 @@ def test_a_window_wider_than_the_keys_is_no_window(kw):
     assert (got.float() - plain.float()).abs().max() <= 2 ** -7 * plain.float().abs().max()
 
 
-def test_strides_scales_and_outputs():
+def test_strides_scales_and_outputs(kernels):
     import msa_for_sail as msa
     for types in ((BF, BF), (BF, E4), (E4, E4)):
         for ql, kl in (([1, 1], [700, 2000]), ([300, 200], [700, 2000])):
@@ -189,7 +200,7 @@ def _device_plan(c, max_q, T, splits=1, **kw):
 @pytest.mark.parametrize("splits", [1, 3])
 @pytest.mark.parametrize("layout,page", [("hnd", 128), ("ragged", 0), ("nhd", 16)])
 @pytest.mark.parametrize("types", [(BF, BF), (BF, E4), (E4, E4)])
-def test_device_made_plans(splits, layout, page, types):
+def test_device_made_plans(kernels, splits, layout, page, types):
     for ql, kl, max_q in (([1, 1, 0, 1], [900, 3000 - 7, 10, 128], 1), ([4, 1, 2, 0], [900, 2501, 10, 0], 4), ([300, 1, 140, 0], [900, 2501, 140, 5], 400)):
         c = Case(ql, kl, 8, 2, 257, 3, layout, page, *types)
         c.check(plan=_device_plan(c, max_q, sum(ql), splits))
@@ -250,7 +261,7 @@ def test_two_streams_and_another_current_device():
     assert torch.equal(outs[0], want) and torch.equal(outs[1], want)
 
 
-def test_rows_behind_the_last_sequence_are_left_as_they_were():
+def test_rows_behind_the_last_sequence_are_left_as_they_were(kernels):
     import msa_for_sail as msa
     for types in ((BF, BF), (BF, E4), (E4, E4)):
         for max_q, ql in ((1, [1, 0, 1]), (300, [300, 0, 20])):
@@ -263,7 +274,7 @@ def test_rows_behind_the_last_sequence_are_left_as_they_were():
             ref.check(out[:T], None, c.want(), 2 ** -8, 2 ** -8 if types[0] != types[1] else 0.0)
 
 
-def test_random_batches():
+def test_random_batches(kernels):
     rng = random.Random(5)
     for i in range(30):
         b = rng.choice([1, 2, 5])
@@ -278,7 +289,7 @@ def test_random_batches():
             Case(ql, kl, hq, hk, window, sinks, layout, page, *types, seed=i).check()
 
 
-def test_large_values_and_infinities_outside_the_window():
+def test_large_values_and_infinities_outside_the_window(kernels):
     """What a query does not see may be anything, and a far larger score outside the window is not a maximum."""
     for types in ((BF, BF), (BF, E4), (E4, E4)):
         for n in (1, 200):
