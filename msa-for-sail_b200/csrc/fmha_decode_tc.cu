@@ -80,7 +80,7 @@ __device__ __forceinline__ unsigned long long global_ns() {
 //         [32 w, 32 w + 32) of every tile (its P is zero elsewhere), so all four softmax warps
 //         work on a tile instead of the first lanes of one; the four partial (O, m, l) of a row
 //         are combined in shared memory at the end.
-//   F8 && QUAD ("dual"): half the shared memory and 256 TMEM columns, two CTAs per SM, so the
+//   F8 && QUAD, and with a window bf16 && QUAD ("dual"): half the shared memory and 256 TMEM columns, two CTAs per SM, so the
 //         prologue and epilogue of short work items overlap with another item's loads.  Tiles are
 //         half pages (64 keys): two 64-column S buffers and O fit the 256 columns, so Q K^T of tile
 //         j + 1 still overlaps the softmax of tile j.  The barriers live in rows 16-31 of the Q
@@ -94,11 +94,12 @@ __device__ __forceinline__ unsigned long long global_ns() {
 //         sequences x 8 heads x 2 112 keys.)
 template <bool F8, bool QUAD, bool WIN = false>
 struct Cfg {
-  static constexpr bool DUAL = F8 && QUAD;
+  static constexpr bool DUAL = QUAD && (F8 || WIN);
   static constexpr bool PAIR = F8 && WIN;
   static constexpr int TK = DUAL ? 64 : 128;              // keys per tile
   static constexpr int NSUB = F8 ? 1 : 2;                 // 128-byte-wide sub-tiles per tile
-  static constexpr int TILE_BYTES = NSUB * TK * 128;
+  static constexpr int KV_SUB = TK * 128;                 // one sub-tile of K or V
+  static constexpr int TILE_BYTES = NSUB * KV_SUB;
   static constexpr int RING_BYTES = DUAL ? 48 * 1024 : 96 * 1024;
   static constexpr int STAGES = RING_BYTES / TILE_BYTES;  // bf16 3, e4m3 6 (dual: 6 half pages)
   static constexpr int V_STAGES = DUAL && WIN ? STAGES - 1 : STAGES;      // room for the barriers, see below
@@ -106,7 +107,7 @@ struct Cfg {
   static constexpr int OFF_Q_LO = SUB_BYTES;              // not dual
   static constexpr int SPLIT = DUAL && PAIR ? 2 : 1;      // lanes that share a row's columns of a quadrant
   // dual: rows 112-127 of the Q tile are never real rows (but for pairs), the K ring may start there
-  static constexpr int OFF_K = DUAL && !PAIR ? SUB_BYTES - 2048 : DUAL ? SUB_BYTES : 2 * SUB_BYTES;
+  static constexpr int OFF_K = DUAL && !PAIR ? NSUB * SUB_BYTES - 2048 : DUAL ? SUB_BYTES : 2 * SUB_BYTES;
   static constexpr int OFF_V = OFF_K + RING_BYTES;
   static constexpr int END = OFF_V + V_STAGES * TILE_BYTES;
   static constexpr int OFF_BAR = DUAL && !PAIR ? 2048 : END;
@@ -126,7 +127,7 @@ __global__ void __launch_bounds__(NTHREADS, (Cfg<F8, QUAD, WIN>::MIN_CTAS))
 decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant__ CUtensorMap tm_q,
                  const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v) {
   using C = Cfg<F8, QUAD, WIN>;
-  constexpr int NSUB = C::NSUB, TILE_BYTES = C::TILE_BYTES, STAGES = C::STAGES, V_STAGES = C::V_STAGES, NBUF = C::NBUF, TK = C::TK;
+  constexpr int NSUB = C::NSUB, KV_SUB = C::KV_SUB, TILE_BYTES = C::TILE_BYTES, STAGES = C::STAGES, V_STAGES = C::V_STAGES, NBUF = C::NBUF, TK = C::TK;
   constexpr bool PAIR = C::PAIR;
   constexpr int UPP = BN / TK;                      // tiles per page
   constexpr int OFF_Q = C::OFF_Q, OFF_K = C::OFF_K, OFF_V = C::OFF_V, OFF_BAR = C::OFF_BAR;
@@ -358,7 +359,7 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
           mbar_arrive_expect_tx(bar(K_FULL + st), TILE_BYTES);
 #pragma unroll
           for (int hlf = 0; hlf < NSUB; ++hlf)
-            tma_load_4d(smem_base + OFF_K + st * TILE_BYTES + hlf * SUB_BYTES, &tm_k, bar(K_FULL + st), hlf * SUB_ELEMS,
+            tma_load_4d(smem_base + OFF_K + st * TILE_BYTES + hlf * KV_SUB, &tm_k, bar(K_FULL + st), hlf * SUB_ELEMS,
                         row_in_page, kvh, phys);
         }
         __syncwarp();
@@ -372,7 +373,7 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
         mbar_arrive_expect_tx(vbar, TILE_BYTES);
 #pragma unroll
         for (int hlf = 0; hlf < NSUB; ++hlf)
-          tma_load_4d(smem_base + OFF_V + vst * TILE_BYTES + hlf * SUB_BYTES, &tm_v, vbar, hlf * SUB_ELEMS, row_in_page, kvh, phys);
+          tma_load_4d(smem_base + OFF_V + vst * TILE_BYTES + hlf * KV_SUB, &tm_v, vbar, hlf * SUB_ELEMS, row_in_page, kvh, phys);
       }
       __syncwarp();
       if constexpr (WIN) { fixes += fix; continue; }         // the other warp's
@@ -383,7 +384,7 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
           unsigned char* vt = smem_gen + OFF_V + st * TILE_BYTES;
           for (int c = lane; c < (TK - valid_rows) * 8 * NSUB; c += 32) {
             const int r = valid_rows + c / (8 * NSUB), ch = c % (8 * NSUB);
-            *reinterpret_cast<uint4*>(vt + (ch >> 3) * SUB_BYTES + r * 128 + (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4*>(vt + (ch >> 3) * KV_SUB + r * 128 + (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
           }
           fence_proxy_async_smem();
           __syncwarp();
@@ -405,7 +406,7 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
         for (int c = lane; c < TK * 8 * NSUB; c += 32) {
           const int r = c / (8 * NSUB), ch = c % (8 * NSUB), key = key0 + r;
           if (key >= end_key || (key < first_key && key >= p.sink_tokens))
-            *reinterpret_cast<uint4*>(vt + (ch >> 3) * SUB_BYTES + r * 128 + (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4*>(vt + (ch >> 3) * KV_SUB + r * 128 + (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
         }
         fence_proxy_async_smem();
         __syncwarp();
@@ -417,7 +418,7 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
     constexpr uint32_t IDESC_QK = F8 ? idesc_e4m3(BM, TK, false, false) : idesc_bf16(BM, TK, false, false);
     constexpr uint32_t IDESC_PV = F8 ? idesc_e4m3(BM, kHeadDim, false, true) : idesc_bf16(BM, kHeadDim, false, true);
     const uint64_t dk_hi = smem_desc(0, 16, 1024) & 0xFFFFFFFFFFFF0000ull;
-    const uint64_t dv_hi = smem_desc(0, SUB_BYTES, 1024) & 0xFFFFFFFFFFFF0000ull;
+    const uint64_t dv_hi = smem_desc(0, KV_SUB, 1024) & 0xFFFFFFFFFFFF0000ull;
     constexpr int KEYS_PER_PV = F8 ? 32 : 16;        // keys one P.V MMA contracts over
     constexpr int PV_STEPS = TK / KEYS_PER_PV;
     constexpr int V_KSTEP = KEYS_PER_PV * 128;       // bytes between the key slices of consecutive P.V MMAs
@@ -426,9 +427,10 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
       const uint32_t qa = (smem_base + OFF_Q) >> 4, ka = (smem_base + OFF_K + (j % STAGES) * TILE_BYTES) >> 4;
 #pragma unroll
       for (int k = 0; k < KSTEPS; ++k) {
-        const uint32_t o = ((k >> 2) * SUB_BYTES + (k & 3) * 32) >> 4;      // 32 bytes of head_dim per MMA
-        if constexpr (F8) mma_ss_f8(sbuf(j), dk_hi | ((qa + o) & 0x3FFF), dk_hi | ((ka + o) & 0x3FFF), IDESC_QK, k > 0);
-        else mma_ss(sbuf(j), dk_hi | ((qa + o) & 0x3FFF), dk_hi | ((ka + o) & 0x3FFF), IDESC_QK, k > 0);
+        const uint32_t oq = ((k >> 2) * SUB_BYTES + (k & 3) * 32) >> 4;     // 32 bytes of head_dim per MMA
+        const uint32_t ok = ((k >> 2) * KV_SUB + (k & 3) * 32) >> 4;
+        if constexpr (F8) mma_ss_f8(sbuf(j), dk_hi | ((qa + oq) & 0x3FFF), dk_hi | ((ka + ok) & 0x3FFF), IDESC_QK, k > 0);
+        else mma_ss(sbuf(j), dk_hi | ((qa + oq) & 0x3FFF), dk_hi | ((ka + ok) & 0x3FFF), IDESC_QK, k > 0);
       }
       if constexpr (PAIR && !QUAD) {
         if (p.q_dtype == MSA_DT_BF16) {
@@ -1040,7 +1042,7 @@ int fmha_decode_tc_launch(const MsaFmhaParams& p, cudaStream_t stream) {
       const uint64_t str[2] = {static_cast<uint64_t>(p.q_stride_head) * 2, static_cast<uint64_t>(p.q_stride_tok) * 2};
       const uint32_t box[3] = {64, static_cast<uint32_t>(p.pack), 1};
       if (make_tma_map_bf16(&tq, p.q, 3, dims, str, box) != MSA_OK) return MSA_ERR_LAUNCH;
-      const uint32_t kbox[4] = {64, BN, 1, 1};
+      const uint32_t kbox[4] = {64, static_cast<uint32_t>(quad && p.window > 0 ? Cfg<false, true, true>::TK : BN), 1, 1};
       if (make_tma_map_bf16(&tk, p.k, 4, kd, ks, kbox) != MSA_OK ||
           make_tma_map_bf16(&tv, vptr, 4, kd, has_o ? vs : ks, kbox) != MSA_OK)
         return MSA_ERR_LAUNCH;
@@ -1066,7 +1068,7 @@ int fmha_decode_tc_launch(const MsaFmhaParams& p, cudaStream_t stream) {
   if (dev >= 16 || !attr_done[dev][variant]) {
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
       return MSA_ERR_LAUNCH;
-    if ((variant & 3) == 3)      // two co-resident CTAs need the whole shared-memory carve-out
+    if ((variant & 3) == 3 || variant == 5)      // two co-resident CTAs need the whole shared-memory carve-out
       cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
     if (dev < 16) attr_done[dev][variant] = true;
   }

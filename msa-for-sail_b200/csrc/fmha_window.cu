@@ -1,0 +1,505 @@
+// Windowed attention of up to 16 rows (decode: tokens x query heads of a KV head), streamed at the rate of the memory.
+//
+// Per key and KV head 4 * 128 multiplications are made for each row, so memory is the bound, and what has to be short is the chain from a
+// key's arrival to its place in the sums.  In the tcgen05 decode kernel that chain (load, Q K^T, commit, softmax, store, P V) takes 1 100
+// clocks for 64 keys whatever they hold, most of it hand-overs between warps, and two CTAs of it share an SM: 71 us for 64 sequences x 8
+// heads x 2 100 e4m3 keys, 41 would be the memory's.  Here a warp does all of it itself, on mma.sync, and there are eight warps an SM at
+// different points of it:
+//
+//   S^T = K Q^T     A = 16 keys x 16 elements of K from shared memory, B = Q^T, in registers for the whole item
+//   O^T = V^T P^T   A = 16 elements x 16 keys of V^T, B = P^T: S^T through a transposing register move
+//
+// A warp has a ring of its own, filled by TMA (128-byte swizzle: every read below is free of bank conflicts) with units of 16 bf16 or 32 e4m3
+// keys, 4 KB each of K and V; unit n of an item is warp n % 4's.  It has a softmax of its own; the four states are joined at the end.
+// Units that no row sees are not loaded, so a window costs its keys and at most two units' edges.
+//
+// bf16: P is rounded to bf16 (2^-8), its sum is that of the unrounded weights.  e4m3: elements are converted to f16, which is exact; the order of a
+// contraction is free, so thread t of a group of four takes elements 32 t .. 32 t + 31 of its keys (K), thread group g elements
+// 16 g .. 16 g + 15 (V): whole 16-byte reads.  A query row is multiplied by a power of two that brings its largest element to [2^14, 2^15)
+// (exact in f16 down to 2^-28 of it), P is written as 2^(x - m + 7) in f16 (11 bits down to 2^-21 of the largest weight).
+#include "tc_ptx.cuh"
+
+namespace msa {
+int make_tma_map_bf16(CUtensorMap* m, const void* base, int rank, const uint64_t* dims, const uint64_t* strides_bytes, const uint32_t* box);
+int make_tma_map_u8(CUtensorMap* m, const void* base, int rank, const uint64_t* dims, const uint64_t* strides_bytes, const uint32_t* box);
+
+namespace window {
+namespace {
+
+using namespace tc;
+
+constexpr int kWarps = 4;
+constexpr int kThreads = 32 * kWarps;
+constexpr int kStages = 3;
+constexpr int kHalf = 4096;                                  // K of a unit; V follows
+constexpr int kLdO = kHeadDim + 4;                           // floats of a row of O in shared memory
+constexpr float kRescale = 8.f;
+constexpr float kNoMax = -3e38f;                             // maximum of a row that has seen no key
+
+template <bool F8>
+__host__ __device__ constexpr int unit_keys() { return F8 ? 32 : 16; }
+
+constexpr int OFF_BAR = kWarps * kStages * 2 * kHalf;        // [warp][stage] full
+constexpr int OFF_FAC = OFF_BAR + kWarps * kStages * 8;      // [16] factor of a row's scores
+constexpr int OFF_FLAG = OFF_FAC + 64;                       // abort, skip
+constexpr int SMEM_BYTES = OFF_FLAG + 16 + 1024;             // + slack to align the base to 1 KB
+static_assert(2 * (SMEM_BYTES + 1024) <= 228 * 1024, "two CTAs fit an SM");
+
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+// 16 bytes of a row of a swizzled tile of 128-byte rows
+__device__ __forceinline__ uint32_t swizzled(int row, int chunk) { return static_cast<uint32_t>(row * 128 + ((chunk ^ (row & 7)) << 4)); }
+__device__ __forceinline__ void load_words(const unsigned char* at, uint32_t* w) {
+  const uint4 v = *reinterpret_cast<const uint4*>(at);
+  w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+}
+
+template <int NT, bool F8>
+__global__ void __launch_bounds__(kThreads, 2)
+window_decode_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v) {
+  constexpr int UK = unit_keys<F8>(), STEPS = UK / 16;
+  constexpr int SUB = UK * 128;                              // a half of head_dim of a bf16 unit, all of it in e4m3
+  constexpr float kPOffset = F8 ? 7.f : 0.f;
+  extern __shared__ unsigned char smem_raw[];
+  const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  unsigned char* smem = smem_raw + (smem_base - smem_u32(smem_raw));
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + OFF_FLAG);
+  volatile int* skip_flag = abort_flag + 1;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
+  unsigned char* ring = smem + warp * kStages * 2 * kHalf;
+  const uint32_t ring_u = smem_base + warp * kStages * 2 * kHalf, bars = smem_base + OFF_BAR + warp * kStages * 8;
+
+  // a timeout reported earlier on this device (status word not cleared yet): do not start
+  if (threadIdx.x == kThreads - 1) *skip_flag = (p.status != nullptr && *reinterpret_cast<const volatile int32_t*>(p.status) != 0) ? 1 : 0;
+  if (threadIdx.x == 0) {
+    *abort_flag = 0;
+    for (int s = 0; s < kWarps * kStages; ++s) mbar_init(smem_base + OFF_BAR + 8 * s, 1);
+    mbar_fence_init();
+  }
+
+  // ---------------- the item ----------------
+  const MsaWorkItem w = p.work[blockIdx.x];
+  const int b = chk(w.batch, 0, p.batch, p.status), head0 = chk(w.head0, 0, p.num_qo_heads, p.status), split = chk(w.split, 0, p.num_splits, p.status);
+  const int G = p.pack, kvh = head0 / (p.num_qo_heads / p.num_kv_heads);
+  const int qo_base = p.qo_start[b], kv_len = p.kv_len[b], off = p.qo_offset[b];
+  const bool paged = p.page_size > 0;
+  const int kv0 = paged ? p.kv_page_indptr[b] : p.kv_start[b];
+  const int ntok = min(p.qo_start[b + 1] - qo_base, p.decode_rows / G);      // (lengths on the device may outgrow the rows there are)
+  const int nrows = ntok * G;
+  // Units are numbered without those that no row sees: number n stands for unit n of the keys below sink_u, for n + skip_u from there on.
+  const int first_key = window_first(off, kv_len, p.window);                 // of the first row's window
+  const int end_key = max(0, min(kv_len, off + ntok));                       // behind what the last row sees
+  const int sink_u = p.sink_tokens / UK + (p.sink_tokens % UK != 0), skip_u = max(0, first_key / UK - sink_u);
+  auto number = [&](int u) { return u < sink_u ? u : max(sink_u, u - skip_u); };
+  auto real_tile = [&](int t) { return t < sink_tiles(p.sink_tokens) ? t : t + w.kv_tile_skip; };
+  int begin = 0, end = 0;
+  if (w.kv_tile_begin < w.kv_tile_end && nrows > 0) {
+    begin = number(real_tile(w.kv_tile_begin) * (kKvTile / UK));
+    end = number(min((real_tile(w.kv_tile_end - 1) + 1) * (kKvTile / UK), (end_key + UK - 1) / UK));
+  }
+  begin += warp;                                             // this warp's: every fourth
+  const int n_units = end > begin ? (end - begin + kWarps - 1) / kWarps : 0;
+  auto key_of = [&](int i) { const int n = begin + kWarps * i; return (n < sink_u ? n : n + skip_u) * UK; };
+
+  // ---------------- loads ----------------
+  int phys = 0;                                              // lane i: page of this warp's unit 32 k + i
+  auto load_pages = [&](int i0) { phys = paged && i0 + lane < n_units ? page_entry(p, kv0 + key_of(i0 + lane) / p.page_size) : 0; };
+  auto fetch = [&](int i, int stage) {                       // unit i into a stage that no lane reads any more
+    if ((i & 31) == 0) load_pages(i);
+    const int page = __shfl_sync(0xffffffffu, phys, i & 31), key0 = key_of(i);
+    if (elect_one()) {
+      const uint32_t bar = bars + 8 * stage, dst = ring_u + stage * 2 * kHalf;
+      mbar_arrive_expect_tx(bar, 2 * kHalf);
+#pragma unroll
+      for (int h = 0; h < (F8 ? 1 : 2); ++h) {
+        if (paged) {
+          tma_load_4d(dst + h * SUB, &tm_k, bar, 64 * h, key0 % p.page_size, kvh, page);
+          tma_load_4d(dst + kHalf + h * SUB, &tm_v, bar, 64 * h, key0 % p.page_size, kvh, page);
+        } else {
+          tma_load_3d(dst + h * SUB, &tm_k, bar, 64 * h, kvh, kv0 + key0);
+          tma_load_3d(dst + kHalf + h * SUB, &tm_v, bar, 64 * h, kvh, kv0 + key0);
+        }
+      }
+    }
+    __syncwarp();
+  };
+  __syncthreads();
+  const bool run = *skip_flag == 0;
+  bool alive = run;
+  if (run) {
+#pragma unroll
+    for (int s = 0; s < kStages; ++s)
+      if (s < n_units) fetch(s, s);
+  }
+
+  // ---------------- Q^T: row 8 n + g, as operands ----------------
+  // The factor of the scores is made positive, its sign goes to Q, so that the largest score has the largest exponent; a factor of 0 makes Q 0.
+  const float signed_scale = p.sm_scale * kLog2e * (p.k_scale_head ? p.k_scale_head[kvh] : 1.f);
+  const float scale = signed_scale == 0.f ? 1.f : fabsf(signed_scale);
+  [[maybe_unused]] const uint32_t flip = signed_scale < 0.f ? 0x80008000u : 0u, keep = signed_scale == 0.f ? 0u : 0xffffffffu;
+  uint32_t qf[NT][8][2];
+  float* s_fac = reinterpret_cast<float*>(smem + OFF_FAC);
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int row = min(8 * n + g, max(nrows, 1) - 1);       // rows that are none repeat the last one and are not written
+    const int64_t at = static_cast<int64_t>(qo_base + row / G) * p.q_stride_tok + static_cast<int64_t>(head0 + row % G) * p.q_stride_head;
+    if constexpr (!F8) {
+      const uint32_t* src = reinterpret_cast<const uint32_t*>(static_cast<const __nv_bfloat16*>(p.q) + at);
+#pragma unroll
+      for (int s = 0; s < 8; ++s) {
+        qf[n][s][0] = nrows > 0 ? (src[8 * s + t4] ^ flip) & keep : 0u;
+        qf[n][s][1] = nrows > 0 ? (src[8 * s + 4 + t4] ^ flip) & keep : 0u;
+      }
+    } else {
+      float x[32];                                           // elements 32 t .. 32 t + 31
+      if (p.q_dtype == MSA_DT_E4M3) {
+        uint32_t v[8] = {};
+        if (nrows > 0) {
+          load_words(static_cast<const unsigned char*>(p.q) + at + 32 * t4, v);
+          load_words(static_cast<const unsigned char*>(p.q) + at + 32 * t4 + 16, v + 4);
+        }
+#pragma unroll
+        for (int c = 0; c < 16; ++c) {
+          const uint32_t h = cvt_e4m3x2<true>(static_cast<uint16_t>(v[c >> 1] >> (16 * (c & 1))));
+          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+          x[2 * c] = f.x; x[2 * c + 1] = f.y;
+        }
+      } else {
+        uint32_t v[16] = {};
+        if (nrows > 0) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) load_words(reinterpret_cast<const unsigned char*>(static_cast<const __nv_bfloat16*>(p.q) + at + 32 * t4) + 16 * c, v + 4 * c);
+        }
+#pragma unroll
+        for (int c = 0; c < 16; ++c) { x[2 * c] = __uint_as_float(v[c] << 16); x[2 * c + 1] = __uint_as_float(v[c] & 0xffff0000u); }
+      }
+      float top = 0.f;
+#pragma unroll
+      for (int c = 0; c < 32; ++c) top = fmaxf(top, fabsf(x[c]));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      // exponent of the largest element; a row of zeros or with an infinity is taken as it is; 2^-e is a normal number
+      int e = static_cast<int>(__float_as_uint(top) >> 23) - 127 - 14;
+      if (top == 0.f || !(top < INFINITY)) e = 0;
+      e = max(e, -126);
+      const float up = copysignf(signed_scale == 0.f ? 0.f : __uint_as_float(static_cast<uint32_t>(127 - e) << 23), signed_scale);
+#pragma unroll
+      for (int s = 0; s < 8; ++s) {
+        qf[n][s][0] = pack2<true>(x[4 * s] * up, x[4 * s + 1] * up);
+        qf[n][s][1] = pack2<true>(x[4 * s + 2] * up, x[4 * s + 3] * up);
+      }
+      if (warp == 0 && t4 == 0) s_fac[8 * n + g] = signed_scale == 0.f ? 1.f : scale * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+    }
+  }
+  if constexpr (F8) __syncthreads();
+
+  // of rows 8 n + 2 t4 + c: factor of the scores, first key that the row does not see any more, first key of its window
+  float fac[NT][2];
+  int lim[NT][2], from[NT][2];
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const int r = 8 * n + 2 * t4 + c, tok = min(r, max(nrows, 1) - 1) / G;
+      fac[n][c] = F8 ? s_fac[r] : scale;
+      lim[n][c] = max(0, min(kv_len, tok + off + 1));
+      from[n][c] = window_first(tok + off, kv_len, p.window);
+    }
+  const int lim_first = max(0, min(kv_len, off + 1)), from_last = window_first(off + ntok - 1, kv_len, p.window);
+
+  float m[NT][2];                                            // maximum - kPOffset
+  uint64_t l[NT];                                            // sums of the weights, two floats
+  float o[8][NT][4];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    m[n][0] = m[n][1] = kNoMax;
+    l[n] = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) o[i][n][c] = 0.f;
+  }
+
+  int stage = 0, parity = 0;
+#pragma unroll 1
+  for (int i = 0; i < n_units && alive; ++i) {
+    const int key0 = key_of(i);
+    unsigned char* kt = ring + stage * 2 * kHalf;
+    unsigned char* vt = kt + kHalf;
+    const uint32_t kt_u = ring_u + stage * 2 * kHalf, vt_u = kt_u + kHalf;
+    alive = mbar_wait_warp(bars + 8 * stage, parity, abort_flag);
+    if (!alive) break;
+    // Keys that no row sees read as 0 in V: the weight of 0 that they have does not take a NaN out.
+    const bool unseen = key0 + UK > end_key || (key0 < first_key && key0 + UK > p.sink_tokens);
+    if (unseen) {
+      for (int c = lane; c < UK * (F8 ? 8 : 16); c += 32) {
+        const int r = c / (F8 ? 8 : 16), ch = c % (F8 ? 8 : 16), key = key0 + r;
+        if (key >= end_key || (key < first_key && key >= p.sink_tokens))
+          *reinterpret_cast<uint4*>(vt + (ch >> 3) * SUB + r * 128 + (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
+      }
+      fence_proxy_async_smem();                              // before the next copy into these bytes
+      __syncwarp();
+    }
+    // ---- S^T ----
+    float s[STEPS][NT][4];
+#pragma unroll
+    for (int u = 0; u < STEPS; ++u) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) s[u][n][c] = 0.f;
+      if constexpr (!F8) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          uint32_t a[4];
+          const int ch = 2 * k + (lane >> 4);
+          ldmatrix_x4(kt_u + (ch >> 3) * SUB + swizzled(lane & 15, ch & 7), a[0], a[1], a[2], a[3]);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma_16816<false>(s[u][n], a, qf[n][k][0], qf[n][k][1]);
+        }
+      } else {
+        uint32_t lo[8], hi[8];                               // keys g and g + 8
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          load_words(kt + swizzled(16 * u + g, 2 * t4 + h), lo + 4 * h);
+          load_words(kt + swizzled(16 * u + 8 + g, 2 * t4 + h), hi + 4 * h);
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const uint32_t a[4] = {cvt_e4m3x2<true>(static_cast<uint16_t>(lo[k])), cvt_e4m3x2<true>(static_cast<uint16_t>(hi[k])),
+                                 cvt_e4m3x2<true>(static_cast<uint16_t>(lo[k] >> 16)), cvt_e4m3x2<true>(static_cast<uint16_t>(hi[k] >> 16))};
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma_16816<true>(s[u][n], a, qf[n][k][0], qf[n][k][1]);
+        }
+      }
+    }
+    // ---- softmax: mask, a maximum that may lag, exponents ----
+    if (key0 + UK > lim_first || (key0 < from_last && key0 + UK > p.sink_tokens)) {
+#pragma unroll
+      for (int u = 0; u < STEPS; ++u)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const int key = key0 + 16 * u + 8 * (c >> 1) + g;
+            if (key >= lim[n][c & 1] || (key < from[n][c & 1] && key >= p.sink_tokens)) s[u][n][c] = -INFINITY;
+          }
+    }
+    bool raise = false;
+    float top[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float x = fmaxf(s[0][n][c], s[0][n][c + 2]);
+        if constexpr (STEPS == 2) x = max3(x, s[STEPS - 1][n][c], s[STEPS - 1][n][c + 2]);
+        top[n][c] = x * fac[n][c];
+        raise |= top[n][c] > m[n][c] + (kPOffset + kRescale);
+      }
+    if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float k2[2];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float x = top[n][c];
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+          x = fmaxf(x - kPOffset, m[n][c]);
+          k2[c] = exp2_fast(m[n][c] - x);
+          m[n][c] = x;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) { o[j][n][c] *= k2[c]; o[j][n][c + 2] *= k2[c]; }
+        }
+        l[n] = f2_fma(l[n], f2_pack(k2[0], k2[1]), 0);
+      }
+    }
+    uint32_t pt[STEPS][NT][2];                               // P^T as an operand: keys 0-7, keys 8-15
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const uint64_t f = f2_pack(fac[n][0], fac[n][1]), shift = f2_pack(-m[n][0], -m[n][1]);
+#pragma unroll
+      for (int u = 0; u < STEPS; ++u)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float x0, x1;
+          f2_unpack(f2_fma(f2_pack(s[u][n][2 * h], s[u][n][2 * h + 1]), f, shift), x0, x1);
+          const float p0 = exp2_fast(x0), p1 = exp2_fast(x1);
+          l[n] = f2_add(l[n], f2_pack(p0, p1));
+          pt[u][n][h] = transpose8x8(pack2<F8>(p0, p1));
+        }
+    }
+    // ---- O^T ----
+#pragma unroll
+    for (int u = 0; u < STEPS; ++u) {
+      if constexpr (!F8) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          uint32_t a[4];
+          const int ch = 2 * j + ((lane >> 3) & 1), r = (lane & 7) + ((lane >> 4) << 3);
+          ldmatrix_x4_trans(vt_u + (ch >> 3) * SUB + swizzled(r, ch & 7), a[0], a[1], a[2], a[3]);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma_16816<false>(o[j][n], a, pt[u][n][0], pt[u][n][1]);
+        }
+      } else {
+        uint32_t v[4][4];                                    // keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9
+#pragma unroll
+        for (int r = 0; r < 4; ++r) load_words(vt + swizzled(16 * u + 2 * t4 + (r & 1) + 8 * (r >> 1), g), v[r]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            // an element of two keys side by side: elements 4 j + 2 h and the next one
+            const uint32_t x = __byte_perm(v[0][j], v[1][j], h ? 0x7362 : 0x5140), y = __byte_perm(v[2][j], v[3][j], h ? 0x7362 : 0x5140);
+            const uint32_t a[4] = {cvt_e4m3x2<true>(static_cast<uint16_t>(x)), cvt_e4m3x2<true>(static_cast<uint16_t>(x >> 16)),
+                                   cvt_e4m3x2<true>(static_cast<uint16_t>(y)), cvt_e4m3x2<true>(static_cast<uint16_t>(y >> 16))};
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma_16816<true>(o[2 * j + h][n], a, pt[u][n][0], pt[u][n][1]);
+          }
+      }
+    }
+    __syncwarp();                                            // all lanes have read the stage
+    if (i + kStages < n_units) fetch(i + kStages, stage);
+    if (++stage == kStages) { stage = 0; parity ^= 1; }
+  }
+  float sums[NT][2];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    f2_unpack(l[n], sums[n][0], sums[n][1]);
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int d = 4; d < 32; d <<= 1) sums[n][c] += __shfl_xor_sync(0xffffffffu, sums[n][c], d);
+  }
+  __syncthreads();                                           // the rings are no longer read, and no copy is on its way (but after a timeout)
+  if (*abort_flag) {
+    if (threadIdx.x == 0 && p.status) atomicExch(p.status, MSA_STATUS_TIMEOUT);
+    outlast_async_work();
+    return;
+  }
+  if (!run || nrows <= 0) return;
+  // ---------------- the four states of a row become one ----------------
+  float* s_o = reinterpret_cast<float*>(smem);               // [warp][row][kLdO]
+  float* s_m = s_o + kWarps * 8 * NT * kLdO;                 // [warp][row][2]: maximum - kPOffset, sum
+  static_assert(kWarps * 8 * NT * (kLdO + 2) * 4 <= OFF_BAR, "states fit the rings");
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const int r = warp * 8 * NT + 8 * n + 2 * t4 + c;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if constexpr (F8) {
+          *reinterpret_cast<float2*>(s_o + r * kLdO + 16 * g + 2 * j) = make_float2(o[j][n][c], o[j][n][c + 2]);
+        } else {
+          s_o[r * kLdO + 16 * j + g] = o[j][n][c];
+          s_o[r * kLdO + 16 * j + g + 8] = o[j][n][c + 2];
+        }
+      }
+      if (g == 0) { s_m[2 * r] = m[n][c]; s_m[2 * r + 1] = sums[n][c]; }
+    }
+  __syncthreads();
+  // 16 threads a row, 8 columns each
+  const int c16 = threadIdx.x & 15;
+#pragma unroll
+  for (int r0 = 0; r0 < 8 * NT; r0 += 8) {
+    const int r = r0 + (threadIdx.x >> 4);
+    if (r >= nrows) continue;
+    float top = kNoMax;
+#pragma unroll
+    for (int v = 0; v < kWarps; ++v) top = fmaxf(top, s_m[2 * (v * 8 * NT + r)]);
+    float sum = 0.f, acc[8];
+#pragma unroll
+    for (int c = 0; c < 8; ++c) acc[c] = 0.f;
+#pragma unroll
+    for (int v = 0; v < kWarps; ++v) {
+      const int at = v * 8 * NT + r;
+      const float f = exp2_fast(s_m[2 * at] - top);
+      sum += f * s_m[2 * at + 1];
+#pragma unroll
+      for (int c = 0; c < 8; ++c) acc[c] += f * s_o[at * kLdO + 8 * c16 + c];
+    }
+    const int64_t tok = qo_base + r / G;
+    const int head = head0 + r % G;
+    const bool none = sum == 0.f;
+    const float inv = none ? 0.f : (p.v_scale_head ? p.v_scale_head[kvh] : 1.f) / sum;
+    const float lse = none ? -INFINITY : (top + log2f(sum)) * kLn2;
+    if (p.partial_o) {
+      const int64_t at = (static_cast<int64_t>(split) * p.total_q + tok) * p.num_qo_heads + head;
+      float* dst = p.partial_o + at * kHeadDim + 8 * c16;
+      *reinterpret_cast<float4*>(dst) = make_float4(acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
+      *reinterpret_cast<float4*>(dst + 4) = make_float4(acc[4] * inv, acc[5] * inv, acc[6] * inv, acc[7] * inv);
+      if (c16 == 0) p.partial_lse[at] = lse;
+    } else {
+      const float f = inv * p.out_scale;
+      const uint4 pk = make_uint4(pack2<false>(acc[0] * f, acc[1] * f), pack2<false>(acc[2] * f, acc[3] * f),
+                                  pack2<false>(acc[4] * f, acc[5] * f), pack2<false>(acc[6] * f, acc[7] * f));
+      *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.out) + tok * p.out_stride_tok + head * p.out_stride_head + 8 * c16) = pk;
+      if (p.lse && c16 == 0) p.lse[tok * p.num_qo_heads + head] = lse;
+    }
+  }
+}
+
+template <int NT, bool F8>
+int launch(const MsaFmhaParams& p, cudaStream_t stream) {
+  constexpr int UK = unit_keys<F8>();
+  const uint64_t e = F8 ? 1 : 2;
+  CUtensorMap tk, tv;
+  for (int i = 0; i < 2; ++i) {
+    const void* base = i ? p.v : p.k;
+    const uint64_t tok = (i ? p.v_stride_tok : p.k_stride_tok) * e, head = (i ? p.v_stride_head : p.k_stride_head) * e,
+                   page = (i ? p.v_stride_page : p.k_stride_page) * e;
+    const uint32_t cols = F8 ? 128 : 64;
+    const auto make = F8 ? make_tma_map_u8 : make_tma_map_bf16;
+    int rc;
+    if (p.page_size > 0) {
+      const uint64_t dims[4] = {128, static_cast<uint64_t>(p.page_size), static_cast<uint64_t>(p.num_kv_heads), static_cast<uint64_t>(p.kv_extent)};
+      const uint64_t str[3] = {tok, head, page};
+      const uint32_t box[4] = {cols, UK, 1, 1};
+      rc = make(i ? &tv : &tk, base, 4, dims, str, box);
+    } else {
+      const uint64_t dims[3] = {128, static_cast<uint64_t>(p.num_kv_heads), static_cast<uint64_t>(p.kv_extent)};
+      const uint64_t str[2] = {head, tok};
+      const uint32_t box[3] = {cols, 1, UK};
+      rc = make(i ? &tv : &tk, base, 3, dims, str, box);
+    }
+    if (rc != MSA_OK) return MSA_ERR_LAUNCH;
+  }
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess) return MSA_ERR_LAUNCH;
+  static bool ready[64] = {};
+  if (device < 0 || device >= 64 || !ready[device]) {
+    if (cudaFuncSetAttribute(window_decode_kernel<NT, F8>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES) != cudaSuccess ||
+        cudaFuncSetAttribute(window_decode_kernel<NT, F8>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared) != cudaSuccess)
+      return MSA_ERR_LAUNCH;
+    if (device >= 0 && device < 64) ready[device] = true;
+  }
+  window_decode_kernel<NT, F8><<<p.num_work, kThreads, SMEM_BYTES, stream>>>(p, tk, tv);
+  return cudaGetLastError() == cudaSuccess ? MSA_OK : MSA_ERR_LAUNCH;
+}
+
+}  // namespace
+}  // namespace window
+
+// Windowed items of at most 16 packed rows; pages of whole units, or ragged keys.
+int fmha_window_supported(const MsaFmhaParams& p) {
+  if (p.window <= 0 || (p.flags & MSA_FLAG_SPARSE) || p.block_m != 16 || p.decode_rows < 1 || p.decode_rows > 16) return 0;
+  if (p.pack != p.num_qo_heads / p.num_kv_heads) return 0;
+  const bool f8 = p.kv_dtype == MSA_DT_E4M3;
+  if (p.q_dtype != MSA_DT_BF16 && !(f8 && p.q_dtype == MSA_DT_E4M3)) return 0;
+  if (p.page_size > 0 && p.page_size % (f8 ? window::unit_keys<true>() : window::unit_keys<false>())) return 0;
+  return p.kv_extent > 0;
+}
+
+int fmha_window_launch(const MsaFmhaParams& p, cudaStream_t stream) {
+  using namespace window;
+  if (p.num_work <= 0) return MSA_OK;
+  const bool f8 = p.kv_dtype == MSA_DT_E4M3;
+  if (p.decode_rows <= 8) return f8 ? launch<1, true>(p, stream) : launch<1, false>(p, stream);
+  return f8 ? launch<2, true>(p, stream) : launch<2, false>(p, stream);
+}
+
+}  // namespace msa
