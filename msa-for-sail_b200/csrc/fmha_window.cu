@@ -13,10 +13,13 @@
 // keys, 4 KB each of K and V; unit n of an item is warp n % 4's.  It has a softmax of its own; the four states are joined at the end.
 // Units that no row sees are not loaded, so a window costs its keys and at most two units' edges.
 //
-// bf16: P is rounded to bf16 (2^-8), its sum is that of the unrounded weights.  e4m3: elements are converted to f16, which is exact; the order of a
-// contraction is free, so thread t of a group of four takes elements 32 t .. 32 t + 31 of its keys (K), thread group g elements
-// 16 g .. 16 g + 15 (V): whole 16-byte reads.  A query row is multiplied by a power of two that brings its largest element to [2^14, 2^15)
-// (exact in f16 down to 2^-28 of it), P is written as 2^(x - m + 7) in f16 (11 bits down to 2^-21 of the largest weight).
+// bf16: P is rounded to bf16 (2^-8), its sum is that of the unrounded weights.
+// e4m3: m16n8k32 on the bytes as they are (with K and V converted to f16 the conversions alone took 55 % of the ALU pipe, and an m16n8k16 of f16
+// takes 2.1 clocks an SM where an m16n8k32 of e4m3 takes 1.2).  Q and P are pairs of e4m3 values, hi + lo, both multiplied: 8 bits.  A query
+// row is multiplied by a power of two that brings its largest element to [2^7, 2^8), P is 2^(x - m + 4) and at most 2^8.  The order of
+// a contraction is free: thread t of a group of four takes elements 32 t .. 32 t + 31 of its keys (K), thread group g elements 16 g .. 16 g + 15 of
+// the keys 2 t, 2 t + 8, 2 t + 1, 2 t + 9 (V; four bytes of a key each become four keys of an element by eight byte permutations),
+// which is the order that the transposed bytes of P come in.
 #include "tc_ptx.cuh"
 
 namespace msa {
@@ -33,7 +36,6 @@ constexpr int kThreads = 32 * kWarps;
 constexpr int kStages = 3;
 constexpr int kHalf = 4096;                                  // K of a unit; V follows
 constexpr int kLdO = kHeadDim + 4;                           // floats of a row of O in shared memory
-constexpr float kRescale = 8.f;
 constexpr float kNoMax = -3e38f;                             // maximum of a row that has seen no key
 
 template <bool F8>
@@ -52,6 +54,17 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
 }
 // 16 bytes of a row of a swizzled tile of 128-byte rows
 __device__ __forceinline__ uint32_t swizzled(int row, int chunk) { return static_cast<uint32_t>(row * 128 + ((chunk ^ (row & 7)) << 4)); }
+__device__ __forceinline__ void mma_e4m3(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// Bytes i of four words, as word i.
+__device__ __forceinline__ void transpose_bytes(uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3, uint32_t (&d)[4]) {
+  const uint32_t a = __byte_perm(w0, w1, 0x5140), b = __byte_perm(w2, w3, 0x5140), c = __byte_perm(w0, w1, 0x7362), e = __byte_perm(w2, w3, 0x7362);
+  d[0] = __byte_perm(a, b, 0x5410); d[1] = __byte_perm(a, b, 0x7632);
+  d[2] = __byte_perm(c, e, 0x5410); d[3] = __byte_perm(c, e, 0x7632);
+}
 __device__ __forceinline__ void load_words(const unsigned char* at, uint32_t* w) {
   const uint4 v = *reinterpret_cast<const uint4*>(at);
   w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
@@ -62,7 +75,7 @@ __global__ void __launch_bounds__(kThreads, 2)
 window_decode_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v) {
   constexpr int UK = unit_keys<F8>(), STEPS = UK / 16;
   constexpr int SUB = UK * 128;                              // a half of head_dim of a bf16 unit, all of it in e4m3
-  constexpr float kPOffset = F8 ? 7.f : 0.f;
+  constexpr float kPOffset = F8 ? 4.f : 0.f, kRescale = F8 ? 4.f : 8.f;      // P is at most 2^8
   extern __shared__ unsigned char smem_raw[];
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   unsigned char* smem = smem_raw + (smem_base - smem_u32(smem_raw));
@@ -140,7 +153,8 @@ window_decode_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_const
   const float signed_scale = p.sm_scale * kLog2e * (p.k_scale_head ? p.k_scale_head[kvh] : 1.f);
   const float scale = signed_scale == 0.f ? 1.f : fabsf(signed_scale);
   [[maybe_unused]] const uint32_t flip = signed_scale < 0.f ? 0x80008000u : 0u, keep = signed_scale == 0.f ? 0u : 0xffffffffu;
-  uint32_t qf[NT][8][2];
+  uint32_t qf[NT][8][2];                                     // bf16: [step of 16 elements]; e4m3: [step of 32 elements, + 4: lo]
+  [[maybe_unused]] const bool pair_q = F8 && p.q_dtype == MSA_DT_BF16;
   float* s_fac = reinterpret_cast<float*>(smem + OFF_FAC);
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
@@ -154,42 +168,43 @@ window_decode_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_const
         qf[n][s][1] = nrows > 0 ? (src[8 * s + 4 + t4] ^ flip) & keep : 0u;
       }
     } else {
-      float x[32];                                           // elements 32 t .. 32 t + 31
-      if (p.q_dtype == MSA_DT_E4M3) {
+      int e = 0;                                             // exponent that the row is divided by
+      if (!pair_q) {
         uint32_t v[8] = {};
         if (nrows > 0) {
           load_words(static_cast<const unsigned char*>(p.q) + at + 32 * t4, v);
           load_words(static_cast<const unsigned char*>(p.q) + at + 32 * t4 + 16, v + 4);
         }
 #pragma unroll
-        for (int c = 0; c < 16; ++c) {
-          const uint32_t h = cvt_e4m3x2<true>(static_cast<uint16_t>(v[c >> 1] >> (16 * (c & 1))));
-          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
-          x[2 * c] = f.x; x[2 * c + 1] = f.y;
+        for (int c = 0; c < 8; ++c) {
+          qf[n][c >> 1][c & 1] = (v[c] ^ (flip | (flip >> 8))) & keep;
+          qf[n][4 + (c >> 1)][c & 1] = 0;
         }
       } else {
-        uint32_t v[16] = {};
+        uint32_t v[16] = {};                                 // elements 32 t .. 32 t + 31
         if (nrows > 0) {
 #pragma unroll
           for (int c = 0; c < 4; ++c) load_words(reinterpret_cast<const unsigned char*>(static_cast<const __nv_bfloat16*>(p.q) + at + 32 * t4) + 16 * c, v + 4 * c);
         }
+        uint32_t top = 0;                                    // magnitudes order as their bits do
 #pragma unroll
-        for (int c = 0; c < 16; ++c) { x[2 * c] = __uint_as_float(v[c] << 16); x[2 * c + 1] = __uint_as_float(v[c] & 0xffff0000u); }
-      }
-      float top = 0.f;
+        for (int c = 0; c < 16; ++c) top = max(top, max(v[c] & 0x7fffu, (v[c] >> 16) & 0x7fffu));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        // (a row of zeros, or with an infinity or NaN, is taken as it is; the factors are normal numbers)
+        e = static_cast<int>(top >> 7) - 127 - 7;
+        if (top == 0 || top >= 0x7f80u) e = 0;
+        e = min(max(e, -126), 126);
+        const float up = copysignf(signed_scale == 0.f ? 0.f : __uint_as_float(static_cast<uint32_t>(127 - e) << 23), signed_scale);
 #pragma unroll
-      for (int c = 0; c < 32; ++c) top = fmaxf(top, fabsf(x[c]));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      // exponent of the largest element; a row of zeros or with an infinity is taken as it is; 2^-e is a normal number
-      int e = static_cast<int>(__float_as_uint(top) >> 23) - 127 - 14;
-      if (top == 0.f || !(top < INFINITY)) e = 0;
-      e = max(e, -126);
-      const float up = copysignf(signed_scale == 0.f ? 0.f : __uint_as_float(static_cast<uint32_t>(127 - e) << 23), signed_scale);
+        for (int c = 0; c < 8; ++c) {
+          uint32_t hi[2], lo[2];
 #pragma unroll
-      for (int s = 0; s < 8; ++s) {
-        qf[n][s][0] = pack2<true>(x[4 * s] * up, x[4 * s + 1] * up);
-        qf[n][s][1] = pack2<true>(x[4 * s + 2] * up, x[4 * s + 3] * up);
+          for (int h = 0; h < 2; ++h)
+            e4m3_pair(__uint_as_float(v[2 * c + h] << 16) * up, __uint_as_float(v[2 * c + h] & 0xffff0000u) * up, hi[h], lo[h]);
+          qf[n][c >> 1][c & 1] = hi[0] | (hi[1] << 16);
+          qf[n][4 + (c >> 1)][c & 1] = lo[0] | (lo[1] << 16);
+        }
       }
       if (warp == 0 && t4 == 0) s_fac[8 * n + g] = signed_scale == 0.f ? 1.f : scale * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
     }
@@ -268,11 +283,14 @@ window_decode_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_const
           load_words(kt + swizzled(16 * u + 8 + g, 2 * t4 + h), hi + 4 * h);
         }
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const uint32_t a[4] = {cvt_e4m3x2<true>(static_cast<uint16_t>(lo[k])), cvt_e4m3x2<true>(static_cast<uint16_t>(hi[k])),
-                                 cvt_e4m3x2<true>(static_cast<uint16_t>(lo[k] >> 16)), cvt_e4m3x2<true>(static_cast<uint16_t>(hi[k] >> 16))};
+        for (int k = 0; k < 4; ++k)
 #pragma unroll
-          for (int n = 0; n < NT; ++n) mma_16816<true>(s[u][n], a, qf[n][k][0], qf[n][k][1]);
+          for (int n = 0; n < NT; ++n) mma_e4m3(s[u][n], lo[2 * k], hi[2 * k], lo[2 * k + 1], hi[2 * k + 1], qf[n][k][0], qf[n][k][1]);
+        if (pair_q) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma_e4m3(s[u][n], lo[2 * k], hi[2 * k], lo[2 * k + 1], hi[2 * k + 1], qf[n][4 + k][0], qf[n][4 + k][1]);
         }
       }
     }
@@ -317,47 +335,57 @@ window_decode_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_const
         l[n] = f2_fma(l[n], f2_pack(k2[0], k2[1]), 0);
       }
     }
-    uint32_t pt[STEPS][NT][2];                               // P^T as an operand: keys 0-7, keys 8-15
+    uint32_t pt[STEPS][NT][2];                               // P^T as an operand: keys 0-7, keys 8-15; e4m3: hi, lo of the step's 16 keys
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const uint64_t f = f2_pack(fac[n][0], fac[n][1]), shift = f2_pack(-m[n][0], -m[n][1]);
 #pragma unroll
-      for (int u = 0; u < STEPS; ++u)
+      for (int u = 0; u < STEPS; ++u) {
+        float w0[2], w1[2];                                  // keys g and g + 8 of the rows 2 t, 2 t + 1
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           float x0, x1;
           f2_unpack(f2_fma(f2_pack(s[u][n][2 * h], s[u][n][2 * h + 1]), f, shift), x0, x1);
-          const float p0 = exp2_fast(x0), p1 = exp2_fast(x1);
-          l[n] = f2_add(l[n], f2_pack(p0, p1));
-          pt[u][n][h] = transpose8x8(pack2<F8>(p0, p1));
+          w0[h] = exp2_fast(x0); w1[h] = exp2_fast(x1);
+          l[n] = f2_add(l[n], f2_pack(w0[h], w1[h]));
+          if constexpr (!F8) pt[u][n][h] = transpose8x8(pack2<false>(w0[h], w1[h]));
         }
+        if constexpr (F8) {
+          uint32_t h0, l0, h1, l1;
+          e4m3_pair(w0[0], w0[1], h0, l0);
+          e4m3_pair(w1[0], w1[1], h1, l1);
+          pt[u][n][0] = transpose8x8(h0 | (h1 << 16));
+          pt[u][n][1] = transpose8x8(l0 | (l1 << 16));
+        }
+      }
     }
     // ---- O^T ----
+    if constexpr (!F8) {
 #pragma unroll
-    for (int u = 0; u < STEPS; ++u) {
-      if constexpr (!F8) {
+      for (int j = 0; j < 8; ++j) {
+        uint32_t a[4];
+        const int ch = 2 * j + ((lane >> 3) & 1), r = (lane & 7) + ((lane >> 4) << 3);
+        ldmatrix_x4_trans(vt_u + (ch >> 3) * SUB + swizzled(r, ch & 7), a[0], a[1], a[2], a[3]);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          uint32_t a[4];
-          const int ch = 2 * j + ((lane >> 3) & 1), r = (lane & 7) + ((lane >> 4) << 3);
-          ldmatrix_x4_trans(vt_u + (ch >> 3) * SUB + swizzled(r, ch & 7), a[0], a[1], a[2], a[3]);
+        for (int n = 0; n < NT; ++n) mma_16816<false>(o[j][n], a, pt[0][n][0], pt[0][n][1]);
+      }
+    } else {
+      uint32_t v[2][4][4];                                   // [step][key 2 t, 2 t + 8, 2 t + 1, 2 t + 9][4 elements]
 #pragma unroll
-          for (int n = 0; n < NT; ++n) mma_16816<false>(o[j][n], a, pt[u][n][0], pt[u][n][1]);
-        }
-      } else {
-        uint32_t v[4][4];                                    // keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9
+      for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) load_words(vt + swizzled(16 * u + 2 * t4 + (r & 1) + 8 * (r >> 1), g), v[r]);
+        for (int r = 0; r < 4; ++r) load_words(vt + swizzled(16 * u + 2 * t4 + (r >> 1) + 8 * (r & 1), g), v[u][r]);
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+      for (int j = 0; j < 4; ++j) {
+        uint32_t a[2][4];                                    // elements 4 j .. 4 j + 3 of four keys
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            // an element of two keys side by side: elements 4 j + 2 h and the next one
-            const uint32_t x = __byte_perm(v[0][j], v[1][j], h ? 0x7362 : 0x5140), y = __byte_perm(v[2][j], v[3][j], h ? 0x7362 : 0x5140);
-            const uint32_t a[4] = {cvt_e4m3x2<true>(static_cast<uint16_t>(x)), cvt_e4m3x2<true>(static_cast<uint16_t>(x >> 16)),
-                                   cvt_e4m3x2<true>(static_cast<uint16_t>(y)), cvt_e4m3x2<true>(static_cast<uint16_t>(y >> 16))};
+        for (int u = 0; u < 2; ++u) transpose_bytes(v[u][0][j], v[u][1][j], v[u][2][j], v[u][3][j], a[u]);
 #pragma unroll
-            for (int n = 0; n < NT; ++n) mma_16816<true>(o[2 * j + h][n], a, pt[u][n][0], pt[u][n][1]);
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            mma_e4m3(o[2 * j + h][n], a[0][2 * h], a[0][2 * h + 1], a[1][2 * h], a[1][2 * h + 1], pt[0][n][0], pt[STEPS - 1][n][0]);
+            mma_e4m3(o[2 * j + h][n], a[0][2 * h], a[0][2 * h + 1], a[1][2 * h], a[1][2 * h + 1], pt[0][n][1], pt[STEPS - 1][n][1]);
           }
       }
     }
