@@ -272,6 +272,10 @@ int msa_plan_device(const MsaPlanDeviceArgs* args, msa_stream_t stream);
 int msa_fmha_fwd_split_static(const MsaFmhaParams* params, const int32_t* splits_per_row,
                               msa_stream_t stream);
 
+/* msa_fmha_fwd with split partials (partial_o, partial_lse and num_splits set) and the merge of them, msa_lse_merge_many, into out and lse: one
+ * call.  out_dtype: MSA_DT_BF16 or MSA_DT_F32, strides of out in elements of it. */
+int msa_fmha_fwd_merged(const MsaFmhaParams* params, const int32_t* splits_per_row, int32_t out_dtype, msa_stream_t stream);
+
 /* msa_fmha_fwd with kv_dtype = MSA_DT_KV4: q bf16 or e4m3, paged k and v with page_size 128, MSA_FLAG_OUT_O only (with or
  * without MSA_FLAG_SPARSE), block_m 16 / 64 / 128; up to 128 packed rows per work item.  Longer queries and scores: unpack
  * the pages with msa_kv4_read and run on the copy.  num_logical_pages is the length of kv_indices; entries past it and pages

@@ -89,6 +89,17 @@ extern "C" int msa_fmha_fwd(const MsaFmhaParams* pp, msa_stream_t stream_) {
   return msa::fmha_mma_launch(p, stream);
 }
 
+extern "C" int msa_fmha_fwd_merged(const MsaFmhaParams* pp, const int32_t* splits_per_row, int32_t out_dtype, msa_stream_t stream) {
+  if (!pp || !pp->partial_o || !pp->partial_lse || !pp->out || pp->num_splits < 1) return MSA_ERR_BAD_ARG;
+  if (out_dtype != MSA_DT_BF16 && out_dtype != MSA_DT_F32) return MSA_ERR_UNSUPPORTED;
+  MsaFmhaParams p = *pp;
+  p.out = nullptr;
+  p.lse = nullptr;
+  if (const int rc = msa_fmha_fwd(&p, stream)) return rc;
+  return msa_lse_merge_many(p.partial_o, p.partial_lse, splits_per_row, pp->out, out_dtype, pp->lse, p.num_splits, p.total_q, p.num_qo_heads,
+                            pp->out_stride_tok, pp->out_stride_head, p.out_scale, stream);
+}
+
 namespace msa {
 struct Proto { int b, row0, nrows, ntiles, skip; };      // the rows of one work item and their KV tiles, before any split
 
@@ -112,16 +123,17 @@ static int makespan(const std::vector<Proto>& protos, int groups, int chunk, int
   return last;
 }
 
-// Tiles a piece of windowed decode: windows are short and alike, so that how many rounds of CTAs there are matters most.  In tile times
-// of a CTA that nothing holds up (1.06 us in bf16): a piece costs five beyond its own, a merge three, and memory gives each SM a tile in 1.4
-// (as if all were bf16; e4m3 tiles take their CTA longer than memory).  Measured with 1 to 12 splits: 24 ragged sequences x 4 heads, at
-// most 34 tiles: 41 us uncut, 46 + merge in two, 38 + merge in three, 44 + merge in four; 128 items of 10 tiles: 25, 34, 38 us; 512 of 66: 336 us
-// uncut, 349 in two; one sequence of 10 tiles x 2 heads: 15.4 us uncut, 11.0 in five and in ten.
+// Tiles of a piece of windowed decode.  Windows are short and alike, so that rounds of CTAs and the memory that all of them share decide.  In tile
+// times of a CTA that nothing holds up (1.6 us in bf16, 16 rows): a piece costs three beyond its own, a merge two, memory gives each SM a
+// tile in 0.9 (as if all were bf16), and of the two bounds a part of the smaller one shows as well.  Measured with 1 to 12 splits, merge
+// included: 24 ragged sequences x 4 heads, at most 34 tiles: 60 us uncut, 40, 38 (three), 43, 41 (seven), 47; 128 items of 10 tiles, 64
+// rows: 26, 34, 37 us; 512 of 66: 316, 326, 331 us; 512 of 18 e4m3 tiles: 61, 69, 73 us; one sequence of 10 tiles x 2 heads: 15.7, 11.7, 11.0, 8.3 us
+// (five and ten).
 static int window_chunk(const std::vector<Proto>& protos, int groups, int max_tiles, int slots, int sms, int ceiling) {
-  constexpr int kPieceCost = 5, kMerge = 3;
+  constexpr int kPieceCost = 3, kMerge = 2;
   long long total = 0, items = 0;
   for (const Proto& pr : protos) { total += static_cast<long long>(pr.ntiles) * groups; items += groups; }
-  const double memory = 1.4 * static_cast<double>(total) / sms;
+  const double memory = 0.9 * static_cast<double>(total) / sms + kPieceCost;
   int best = std::max(1, max_tiles);
   if (items >= 8LL * slots) return best;
   double best_cost = 0;
@@ -130,7 +142,8 @@ static int window_chunk(const std::vector<Proto>& protos, int groups, int max_ti
     const int chunk = (max_tiles + s - 1) / s;
     if (chunk == last || (s > 1 && items * s > 16LL * slots)) continue;
     last = chunk;
-    const double cost = std::max(memory + kPieceCost, static_cast<double>(makespan(protos, groups, chunk, slots, kPieceCost))) + (s > 1 ? kMerge : 0);
+    const double ctas = makespan(protos, groups, chunk, slots, kPieceCost);
+    const double cost = std::max(memory, ctas) + 0.15 * std::min(memory, ctas) + (s > 1 ? kMerge : 0);
     if (s == 1 || cost < best_cost) { best = chunk; best_cost = cost; }
   }
   return best;

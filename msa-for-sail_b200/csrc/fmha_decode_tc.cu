@@ -80,46 +80,40 @@ __device__ __forceinline__ unsigned long long global_ns() {
 //         [32 w, 32 w + 32) of every tile (its P is zero elsewhere), so all four softmax warps
 //         work on a tile instead of the first lanes of one; the four partial (O, m, l) of a row
 //         are combined in shared memory at the end.
-//   F8 && QUAD, and with a window bf16 && QUAD ("dual"): half the shared memory and 256 TMEM columns, two CTAs per SM, so the
+//   F8 && QUAD ("dual"): half the shared memory and 256 TMEM columns, two CTAs per SM, so the
 //         prologue and epilogue of short work items overlap with another item's loads.  Tiles are
 //         half pages (64 keys): two 64-column S buffers and O fit the 256 columns, so Q K^T of tile
 //         j + 1 still overlaps the softmax of tile j.  The barriers live in rows 16-31 of the Q
 //         tile, which no real row uses.
-//   WIN   rows see a window and the first keys only; tiles that no row sees are not loaded.
+//   WIN   rows see a window and the first keys only; tiles that no row sees are not loaded.  (More than 16 rows: fewer stream through
+//         the kernel of fmha_window.cu.)
 //   F8 && WIN ("pair"): Q and P are pairs of e4m3 values, x = hi + lo with lo = e4m3(x - hi), both multiplied into the same
 //         accumulator: 8 bits where one value has 4, for MMAs that have nothing else to do.  (A single value puts 2.6 % of noise on
-//         each weight: with a window there are few enough that it shows.)  Q_lo is a tile of its own, or, with 16 rows (dual), rows 16-31
-//         of each quadrant: one MMA gives both parts of S, in lanes r and r + 16, which exchange what they need and go on as two
-//         softmaxes of half the quadrant's keys each, eight for a row.  (Q_lo as a second MMA there: 80 us instead of 66 for 64
-//         sequences x 8 heads x 2 112 keys.)
+//         each weight: with a window there are few enough that it shows.)
 template <bool F8, bool QUAD, bool WIN = false>
 struct Cfg {
-  static constexpr bool DUAL = QUAD && (F8 || WIN);
+  static_assert(!(QUAD && WIN), "windowed items of few rows have a kernel of their own");
+  static constexpr bool DUAL = F8 && QUAD;
   static constexpr bool PAIR = F8 && WIN;
   static constexpr int TK = DUAL ? 64 : 128;              // keys per tile
   static constexpr int NSUB = F8 ? 1 : 2;                 // 128-byte-wide sub-tiles per tile
-  static constexpr int KV_SUB = TK * 128;                 // one sub-tile of K or V
-  static constexpr int TILE_BYTES = NSUB * KV_SUB;
+  static constexpr int TILE_BYTES = NSUB * TK * 128;
   static constexpr int RING_BYTES = DUAL ? 48 * 1024 : 96 * 1024;
   static constexpr int STAGES = RING_BYTES / TILE_BYTES;  // bf16 3, e4m3 6 (dual: 6 half pages)
-  static constexpr int V_STAGES = DUAL && WIN ? STAGES - 1 : STAGES;      // room for the barriers, see below
   static constexpr int OFF_Q = 0;
-  static constexpr int OFF_Q_LO = SUB_BYTES;              // not dual
-  static constexpr int SPLIT = DUAL && PAIR ? 2 : 1;      // lanes that share a row's columns of a quadrant
-  // dual: rows 112-127 of the Q tile are never real rows (but for pairs), the K ring may start there
-  static constexpr int OFF_K = DUAL && !PAIR ? NSUB * SUB_BYTES - 2048 : DUAL ? SUB_BYTES : 2 * SUB_BYTES;
+  [[maybe_unused]] static constexpr int OFF_Q_LO = SUB_BYTES;      // pairs
+  // dual: rows 112-127 of the Q tile are never real rows, the K ring may start there
+  static constexpr int OFF_K = DUAL ? SUB_BYTES - 2048 : 2 * SUB_BYTES;
   static constexpr int OFF_V = OFF_K + RING_BYTES;
-  static constexpr int END = OFF_V + V_STAGES * TILE_BYTES;
-  static constexpr int OFF_BAR = DUAL && !PAIR ? 2048 : END;
-  static constexpr int SMEM_BYTES = (DUAL && !PAIR ? END : END + 1024) + 1024;   // + slack to align the base to 1 KB
-  static_assert(!DUAL || 2 * (SMEM_BYTES + 1024) <= 228 * 1024, "two CTAs fit an SM");
+  static constexpr int END = OFF_V + RING_BYTES;
+  static constexpr int OFF_BAR = DUAL ? 2048 : END;
+  static constexpr int SMEM_BYTES = (DUAL ? END : END + 1024) + 1024;   // + slack to align the base to 1 KB
   static constexpr int NBUF = 2;                          // S buffers in TMEM
   static constexpr int TMEM_COLS = DUAL ? 256 : 512;
   static constexpr int O_COL = NBUF * TK;
   static constexpr int MIN_CTAS = DUAL ? 2 : 1;
   static_assert(STAGES <= MAX_STAGES, "barrier table");
   static_assert(4 * QUAD_MAX_ROWS * STAGE_LD * 4 <= RING_BYTES, "O staging fits the K ring");
-  static_assert(4 * SPLIT * QUAD_MAX_ROWS * (STAGE_LD + 2) * 4 <= END - OFF_K, "... of pairs both rings");
 };
 
 template <bool F8, bool QUAD, bool WIN>
@@ -127,7 +121,7 @@ __global__ void __launch_bounds__(NTHREADS, (Cfg<F8, QUAD, WIN>::MIN_CTAS))
 decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant__ CUtensorMap tm_q,
                  const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v) {
   using C = Cfg<F8, QUAD, WIN>;
-  constexpr int NSUB = C::NSUB, KV_SUB = C::KV_SUB, TILE_BYTES = C::TILE_BYTES, STAGES = C::STAGES, V_STAGES = C::V_STAGES, NBUF = C::NBUF, TK = C::TK;
+  constexpr int NSUB = C::NSUB, TILE_BYTES = C::TILE_BYTES, STAGES = C::STAGES, NBUF = C::NBUF, TK = C::TK;
   constexpr bool PAIR = C::PAIR;
   constexpr int UPP = BN / TK;                      // tiles per page
   constexpr int OFF_Q = C::OFF_Q, OFF_K = C::OFF_K, OFF_V = C::OFF_V, OFF_BAR = C::OFF_BAR;
@@ -202,21 +196,12 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
   const int kv_len = p.kv_len[b];
   const int off = p.qo_offset[b];
   const int page_base = p.kv_page_indptr[b];
-  // Windowed: the item's tiles of TK keys are numbered without those that no row sees (a half page next to a page's visible half, too):
-  // number t stands for tile t of the keys below sink_t, for t + skip_t from there on.  first_key: of the first row's window, end_key: behind
-  // what the last row sees.
-  [[maybe_unused]] int first_key = 0, end_key = 0, sink_t = 0, skip_t = 0, t_begin = 0, t_end = 0;
+  // windowed: first key of the first row's window, end of what the last row sees
+  [[maybe_unused]] int first_key = 0, end_key = 0;
   [[maybe_unused]] auto real_page = [&](int t) { return t < sink_tiles(p.sink_tokens) ? t : t + skip; };
   if constexpr (WIN) {
     first_key = window_first(off, kv_len, p.window);
     end_key = max(0, min(kv_len, off + ntok));
-    sink_t = p.sink_tokens / TK + (p.sink_tokens % TK != 0);
-    skip_t = max(0, first_key / TK - sink_t);
-    auto number = [&](int t) { return t < sink_t ? t : max(sink_t, t - skip_t); };
-    if (tb < te) {
-      t_begin = number(real_page(tb) * UPP);
-      t_end = number(min(real_page(te - 1) * UPP + UPP, (end_key + TK - 1) / TK));
-    }
   }
   const int n_active_warps = QUAD ? 4 : (nrows + 31) / 32;
 
@@ -267,7 +252,10 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
       }
       if (lane == 0) *s_ntiles = min(n, MAX_SPARSE_TILES * UPP);
     } else if (WIN) {
-      if (lane == 0) *s_ntiles = max(0, t_end - t_begin);
+      // (lengths on the device may outgrow the rows of the tile: the last pages may then be nobody's)
+      int last = te;
+      while (last > tb && real_page(last - 1) * BN >= end_key) --last;
+      if (lane == 0) *s_ntiles = max(0, last - tb);
     } else if (lane == 0) {
       // [tb, te) pages of the sequence, up to the last tile that holds a key
       const int keys = min(te * BN, kv_len) - tb * BN;
@@ -285,7 +273,7 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
   const int n_tiles = *s_ntiles;
   if (trace) trace[3] = clock64() - clk0;
   auto tile_key0 = [&](int j) -> int {                       // position of the first key of tile j
-    if constexpr (WIN) return (t_begin + j < sink_t ? t_begin + j : t_begin + j + skip_t) * TK;
+    if constexpr (WIN) return real_page(tb + j) * BN;
     return (sparse ? s_tiles[j] : tb * UPP + j) * TK;
   };
   // windowed: whether the tile from key0 on holds a key that no row sees.  Those are in three tiles at most: the last of the sinks, the first
@@ -320,10 +308,9 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
     // page-table entries: one per lane, 32 pages at a time, the next batch already in flight
     int phys_cur = 0, phys_next = 0;
     const int n_pages = (n_tiles + UPP - 1) / UPP;
-    [[maybe_unused]] int entry0 = tb;                          // windowed: page (numbered as the item's tiles) that lane 0 has in phys_cur
     if constexpr (WIN) {
-      phys_cur = tb + lane < te ? page_entry(p, page_base + real_page(tb + lane)) : 0;
-      phys_next = tb + 32 + lane < te ? page_entry(p, page_base + real_page(tb + 32 + lane)) : 0;
+      phys_cur = lane < n_pages ? page_entry(p, page_base + real_page(tb + lane)) : 0;
+      phys_next = 32 + lane < n_pages ? page_entry(p, page_base + real_page(tb + 32 + lane)) : 0;
     } else if (!sparse) {
       phys_cur = lane < n_pages ? page_entry(p, page_base + tb + lane) : 0;
       phys_next = 32 + lane < n_pages ? page_entry(p, page_base + tb + 32 + lane) : 0;
@@ -335,19 +322,11 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
       const int st = j % STAGES;
       const int key0 = tile_key0(j);
       const int row_in_page = key0 % BN;
-      int pg = j / UPP;                                      // dense: page index within this item
-      if constexpr (WIN) {
-        pg = key0 / BN;
-        if (pg >= sink_tiles(p.sink_tokens)) pg -= skip;
-        pg -= entry0;
-        if (pg >= 32) {                                      // (tiles come in order: the next batch begins here)
-          phys_cur = phys_next;
-          entry0 += 32; pg -= 32;
-          phys_next = entry0 + 32 + lane < te ? page_entry(p, page_base + real_page(entry0 + 32 + lane)) : 0;
-        }
-      } else if (!sparse && j > 0 && (j % (32 * UPP)) == 0) {
+      const int pg = j / UPP;                                // dense: page index within this item
+      if (!sparse && j > 0 && (j % (32 * UPP)) == 0) {
         phys_cur = phys_next;
-        phys_next = pg + 32 + lane < n_pages ? page_entry(p, page_base + tb + pg + 32 + lane) : 0;
+        if constexpr (WIN) phys_next = pg + 32 + lane < n_pages ? page_entry(p, page_base + real_page(tb + pg + 32 + lane)) : 0;
+        else phys_next = pg + 32 + lane < n_pages ? page_entry(p, page_base + tb + pg + 32 + lane) : 0;
       }
       const int phys = sparse ? s_phys[j] : __shfl_sync(0xffffffffu, phys_cur, pg & 31);
       const int valid_rows = min(TK, kv_len - key0);
@@ -359,21 +338,20 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
           mbar_arrive_expect_tx(bar(K_FULL + st), TILE_BYTES);
 #pragma unroll
           for (int hlf = 0; hlf < NSUB; ++hlf)
-            tma_load_4d(smem_base + OFF_K + st * TILE_BYTES + hlf * KV_SUB, &tm_k, bar(K_FULL + st), hlf * SUB_ELEMS,
+            tma_load_4d(smem_base + OFF_K + st * TILE_BYTES + hlf * SUB_BYTES, &tm_k, bar(K_FULL + st), hlf * SUB_ELEMS,
                         row_in_page, kvh, phys);
         }
         __syncwarp();
       }
       if (!do_v) continue;
-      const int vst = j % V_STAGES;
-      alive = mbar_wait_warp(bar(V_EMPTY + vst), ((j / V_STAGES) & 1) ^ 1, abort_flag);
+      alive = mbar_wait_warp(bar(V_EMPTY + st), ((j / STAGES) & 1) ^ 1, abort_flag);
       if (!alive) break;
       if (elect_one()) {
-        const uint32_t vbar = fix ? bar(V_FIX + (WIN ? fixes : 0)) : bar(V_FULL + vst);
+        const uint32_t vbar = fix ? bar(V_FIX + (WIN ? fixes : 0)) : bar(V_FULL + st);
         mbar_arrive_expect_tx(vbar, TILE_BYTES);
 #pragma unroll
         for (int hlf = 0; hlf < NSUB; ++hlf)
-          tma_load_4d(smem_base + OFF_V + vst * TILE_BYTES + hlf * KV_SUB, &tm_v, vbar, hlf * SUB_ELEMS, row_in_page, kvh, phys);
+          tma_load_4d(smem_base + OFF_V + st * TILE_BYTES + hlf * SUB_BYTES, &tm_v, vbar, hlf * SUB_ELEMS, row_in_page, kvh, phys);
       }
       __syncwarp();
       if constexpr (WIN) { fixes += fix; continue; }         // the other warp's
@@ -384,7 +362,7 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
           unsigned char* vt = smem_gen + OFF_V + st * TILE_BYTES;
           for (int c = lane; c < (TK - valid_rows) * 8 * NSUB; c += 32) {
             const int r = valid_rows + c / (8 * NSUB), ch = c % (8 * NSUB);
-            *reinterpret_cast<uint4*>(vt + (ch >> 3) * KV_SUB + r * 128 + (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4*>(vt + (ch >> 3) * SUB_BYTES + r * 128 + (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
           }
           fence_proxy_async_smem();
           __syncwarp();
@@ -402,15 +380,15 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
         up = mbar_wait_warp(bar(V_FIX + fixes), 0, abort_flag, kSpinLimit * static_cast<uint64_t>(n_tiles));
         ++fixes;
         if (!up) break;
-        unsigned char* vt = smem_gen + OFF_V + (j % V_STAGES) * TILE_BYTES;
+        unsigned char* vt = smem_gen + OFF_V + (j % STAGES) * TILE_BYTES;
         for (int c = lane; c < TK * 8 * NSUB; c += 32) {
           const int r = c / (8 * NSUB), ch = c % (8 * NSUB), key = key0 + r;
           if (key >= end_key || (key < first_key && key >= p.sink_tokens))
-            *reinterpret_cast<uint4*>(vt + (ch >> 3) * KV_SUB + r * 128 + (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4*>(vt + (ch >> 3) * SUB_BYTES + r * 128 + (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
         }
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(bar(V_FULL + j % V_STAGES));
+        if (lane == 0) mbar_arrive(bar(V_FULL + j % STAGES));
       }
     }
   } else if (warp == MMA_WARP) {
@@ -418,7 +396,7 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
     constexpr uint32_t IDESC_QK = F8 ? idesc_e4m3(BM, TK, false, false) : idesc_bf16(BM, TK, false, false);
     constexpr uint32_t IDESC_PV = F8 ? idesc_e4m3(BM, kHeadDim, false, true) : idesc_bf16(BM, kHeadDim, false, true);
     const uint64_t dk_hi = smem_desc(0, 16, 1024) & 0xFFFFFFFFFFFF0000ull;
-    const uint64_t dv_hi = smem_desc(0, KV_SUB, 1024) & 0xFFFFFFFFFFFF0000ull;
+    const uint64_t dv_hi = smem_desc(0, SUB_BYTES, 1024) & 0xFFFFFFFFFFFF0000ull;
     constexpr int KEYS_PER_PV = F8 ? 32 : 16;        // keys one P.V MMA contracts over
     constexpr int PV_STEPS = TK / KEYS_PER_PV;
     constexpr int V_KSTEP = KEYS_PER_PV * 128;       // bytes between the key slices of consecutive P.V MMAs
@@ -427,12 +405,11 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
       const uint32_t qa = (smem_base + OFF_Q) >> 4, ka = (smem_base + OFF_K + (j % STAGES) * TILE_BYTES) >> 4;
 #pragma unroll
       for (int k = 0; k < KSTEPS; ++k) {
-        const uint32_t oq = ((k >> 2) * SUB_BYTES + (k & 3) * 32) >> 4;     // 32 bytes of head_dim per MMA
-        const uint32_t ok = ((k >> 2) * KV_SUB + (k & 3) * 32) >> 4;
-        if constexpr (F8) mma_ss_f8(sbuf(j), dk_hi | ((qa + oq) & 0x3FFF), dk_hi | ((ka + ok) & 0x3FFF), IDESC_QK, k > 0);
-        else mma_ss(sbuf(j), dk_hi | ((qa + oq) & 0x3FFF), dk_hi | ((ka + ok) & 0x3FFF), IDESC_QK, k > 0);
+        const uint32_t o = ((k >> 2) * SUB_BYTES + (k & 3) * 32) >> 4;      // 32 bytes of head_dim per MMA
+        if constexpr (F8) mma_ss_f8(sbuf(j), dk_hi | ((qa + o) & 0x3FFF), dk_hi | ((ka + o) & 0x3FFF), IDESC_QK, k > 0);
+        else mma_ss(sbuf(j), dk_hi | ((qa + o) & 0x3FFF), dk_hi | ((ka + o) & 0x3FFF), IDESC_QK, k > 0);
       }
-      if constexpr (PAIR && !QUAD) {
+      if constexpr (PAIR) {
         if (p.q_dtype == MSA_DT_BF16) {
           const uint32_t ql = (smem_base + C::OFF_Q_LO) >> 4;
 #pragma unroll
@@ -442,7 +419,7 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
       }
     };
     auto issue_pv = [&](int j) {
-      const uint32_t va = (smem_base + OFF_V + (j % V_STAGES) * TILE_BYTES) >> 4;
+      const uint32_t va = (smem_base + OFF_V + (j % STAGES) * TILE_BYTES) >> 4;
 #pragma unroll
       for (int k = 0; k < PV_STEPS; ++k) {              // P: 8 TMEM columns per MMA in both formats
         const uint64_t vd = dv_hi | ((va + k * (V_KSTEP >> 4)) & 0x3FFF);
@@ -474,12 +451,12 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
     for (int j = 0; j < n_tiles && alive; ++j) {
       if (NBUF == 2 && j + 1 < n_tiles) { next_qk(j, alive); if (!alive) break; }
       if (has_o) {
-        alive = mbar_wait_warp(bar(V_FULL + j % V_STAGES), (j / V_STAGES) & 1, abort_flag);
+        alive = mbar_wait_warp(bar(V_FULL + j % STAGES), (j / STAGES) & 1, abort_flag);
         if (alive) alive = mbar_wait_warp(bar(P_FULL + j % NBUF), (j / NBUF) & 1, abort_flag);
         if (!alive) break;
         tc_fence_after();
         if (elect_one()) {
-          issue_pv(j); mma_commit(bar(V_EMPTY + j % V_STAGES)); mma_commit(bar(PV_DONE));
+          issue_pv(j); mma_commit(bar(V_EMPTY + j % STAGES)); mma_commit(bar(PV_DONE));
           if (j == n_tiles - 1) mma_commit(bar(O_DONE));
         }
         __syncwarp();
@@ -489,8 +466,7 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
   } else if (warp < n_active_warps) {
     // =========================== softmax / epilogue ===========================
     const int trow = (warp << 5) | lane;                     // row of the MMA tile == TMEM lane
-    const int r = C::SPLIT == 2 ? lane & 15 : QUAD ? lane : trow;        // logical row of the work item
-    const int half = C::SPLIT == 2 ? lane >> 4 : 0;          // which half of the quadrant's columns of the row this lane has
+    const int r = QUAD ? lane : trow;                        // logical row of the work item
     const uint32_t lane_addr = static_cast<uint32_t>(warp << 5) << 16;
     const uint32_t tO = tmem + C::O_COL + lane_addr;
     const bool row_ok = r < nrows;
@@ -554,10 +530,8 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
                 hi[e] = static_cast<uint32_t>(h[0]) | (static_cast<uint32_t>(h[1]) << 16);
                 lo[e] = static_cast<uint32_t>(l[0]) | (static_cast<uint32_t>(l[1]) << 16);
               }
-              if (C::SPLIT == 2 && half) chunks[c] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-              else chunks[c] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-              if constexpr (C::SPLIT == 1)
-                *reinterpret_cast<uint4*>(smem_gen + C::OFF_Q_LO + trow * 128 + ((c ^ (trow & 7)) << 4)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+              chunks[c] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+              *reinterpret_cast<uint4*>(smem_gen + C::OFF_Q_LO + trow * 128 + ((c ^ (trow & 7)) << 4)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
             }
           } else {
             const uint4* src = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.q) +
@@ -581,7 +555,7 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
           }
         }
         // QUAD: only the real rows are written (rows 16-31 of the first quadrant hold the
-        // barriers, but for pairs; what the MMA reads from unused rows only reaches unused TMEM lanes)
+        // barriers; what the MMA reads from unused rows only reaches unused TMEM lanes)
         if (!QUAD || row_ok) {
 #pragma unroll
           for (int c = 0; c < 8; ++c)
@@ -601,38 +575,17 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
         if (trace && j == 12) trace[4] = clock64() - clk0;       // S of tile 12 ready
         if (trace && j == 13) trace[14] = clock64() - clk0;
         tc_fence_after();
-        constexpr int QW = TK / 4, CW = QW / C::SPLIT;       // key columns of a tile per quadrant, and of this lane
-        const int pos0 = tile_key0(j) + warp * QW + half * CW;
+        constexpr int CW = TK / 4;                           // key columns of a tile per quadrant
+        const int pos0 = tile_key0(j) + warp * CW;
         uint32_t sv[CW];
-        if constexpr (C::SPLIT == 2) {
-          // lane r: q_hi k, lane r + 16: q_lo k (or q k in both, if q is e4m3)
-          uint32_t both[QW];
-          tmem_ld16(tS + warp * QW, both);
-          tmem_wait_ld();
-          const bool pair_q = p.q_dtype == MSA_DT_BF16;
-#pragma unroll
-          for (int e = 0; e < CW; ++e) {
-            const float mine = __uint_as_float(half ? both[CW + e] : both[e]);
-            const float other = __uint_as_float(__shfl_xor_sync(0xffffffffu, half ? both[e] : both[CW + e], 16));
-            sv[e] = __float_as_uint(pair_q ? mine + other : mine);
-          }
-        } else {
-          if constexpr (CW == 32) tmem_ld32(tS + warp * CW, sv);
-          else tmem_ld16(tS + warp * CW, sv);
-          tmem_wait_ld();
-        }
+        if constexpr (CW == 32) tmem_ld32(tS + warp * CW, sv);
+        else tmem_ld16(tS + warp * CW, sv);
+        tmem_wait_ld();
         if (trace && j == 12) trace[5] = clock64() - clk0;       // ... loaded
         if (pos0 + CW - 1 > lim) {
 #pragma unroll
           for (int e = 0; e < CW; ++e)
             if (pos0 + e > lim) sv[e] = 0xff800000u;
-        }
-        if constexpr (WIN) {
-          if (pos0 < from && pos0 + CW > p.sink_tokens) {
-#pragma unroll
-            for (int e = 0; e < CW; ++e)
-              if (pos0 + e < from && pos0 + e >= p.sink_tokens) sv[e] = 0xff800000u;
-          }
         }
         float mxs[2] = {-INFINITY, -INFINITY};
 #pragma unroll
@@ -662,7 +615,6 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
         if (trace && j == 12) trace[6] = clock64() - clk0;       // ... max / rescale done
         constexpr int PCOLS = F8 ? CW / 4 : CW / 2;          // TMEM columns of this quadrant's P
         uint32_t pk[PCOLS];
-        [[maybe_unused]] uint32_t pl[PCOLS];                 // pairs: the second values
         if constexpr (F8) {
 #pragma unroll
           for (int e = 0; e < CW; e += 4) {
@@ -670,20 +622,11 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
             const float p1 = exp2_fast(fmaf(__uint_as_float(sv[e + 1]), scale_log2, -msafe));
             const float p2 = exp2_fast(fmaf(__uint_as_float(sv[e + 2]), scale_log2, -msafe));
             const float p3 = exp2_fast(fmaf(__uint_as_float(sv[e + 3]), scale_log2, -msafe));
-            if constexpr (PAIR) {
-              uint32_t a, b, c, d;
-              e4m3_pair(p0, p1, a, b);
-              e4m3_pair(p2, p3, c, d);
-              l0 += p0 + p2; l1 += p1 + p3;
-              pk[e >> 2] = a | (c << 16);
-              pl[e >> 2] = b | (d << 16);
-            } else {
-              const uint16_t lo = __nv_cvt_float2_to_fp8x2(make_float2(p0, p1), __NV_SATFINITE, __NV_E4M3);
-              const uint16_t hi = __nv_cvt_float2_to_fp8x2(make_float2(p2, p3), __NV_SATFINITE, __NV_E4M3);
-              const float2 ra = e4m3x2_as_float2(lo), rb = e4m3x2_as_float2(hi);
-              l0 += ra.x + rb.x; l1 += ra.y + rb.y;
-              pk[e >> 2] = static_cast<uint32_t>(lo) | (static_cast<uint32_t>(hi) << 16);
-            }
+            const uint16_t lo = __nv_cvt_float2_to_fp8x2(make_float2(p0, p1), __NV_SATFINITE, __NV_E4M3);
+            const uint16_t hi = __nv_cvt_float2_to_fp8x2(make_float2(p2, p3), __NV_SATFINITE, __NV_E4M3);
+            const float2 ra = e4m3x2_as_float2(lo), rb = e4m3x2_as_float2(hi);
+            l0 += ra.x + rb.x; l1 += ra.y + rb.y;
+            pk[e >> 2] = static_cast<uint32_t>(lo) | (static_cast<uint32_t>(hi) << 16);
           }
         } else {
 #pragma unroll
@@ -696,16 +639,7 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
           }
         }
         // P of this quadrant's rows: own keys, zero for the other three quarters of the tile
-        if constexpr (C::SPLIT == 2) {
-          const int own = 2 * warp + half;                    // of eight pairs of columns
-          uint32_t all[16];
-#pragma unroll
-          for (int c = 0; c < 16; ++c) all[c] = (c >> 1) == own ? pk[c & 1] : 0u;
-          tmem_st16(tS, all);
-#pragma unroll
-          for (int c = 0; c < 16; ++c) all[c] = (c >> 1) == own ? pl[c & 1] : 0u;
-          tmem_st16(tS + TK / 4, all);
-        } else if constexpr (PCOLS == 4) {                           // 16 columns in all: one store
+        if constexpr (PCOLS == 4) {                           // 16 columns in all: one store
           uint32_t all[16];
 #pragma unroll
           for (int c = 0; c < 16; ++c) all[c] = (c >> 2) == warp ? pk[c & 3] : 0u;
@@ -810,12 +744,12 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
             const float p2 = exp2_fast(fmaf(__uint_as_float(sv[c][e + 2]), scale_log2, -msafe));
             const float p3 = exp2_fast(fmaf(__uint_as_float(sv[c][e + 3]), scale_log2, -msafe));
             if constexpr (PAIR) {
-              uint32_t a, b, c, d;
-              e4m3_pair(p0, p1, a, b);
-              e4m3_pair(p2, p3, c, d);
+              uint32_t hi[2], lo[2];
+              e4m3_pair(p0, p1, hi[0], lo[0]);
+              e4m3_pair(p2, p3, hi[1], lo[1]);
               l0 += p0 + p2; l1 += p1 + p3;
-              pk[e >> 2] = a | (c << 16);
-              pl[e >> 2] = b | (d << 16);
+              pk[e >> 2] = hi[0] | (hi[1] << 16);
+              pl[e >> 2] = lo[0] | (lo[1] << 16);
             } else {
               const uint16_t lo = __nv_cvt_float2_to_fp8x2(make_float2(p0, p1), __NV_SATFINITE, __NV_E4M3);
               const uint16_t hi = __nv_cvt_float2_to_fp8x2(make_float2(p2, p3), __NV_SATFINITE, __NV_E4M3);
@@ -853,11 +787,9 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
     if constexpr (QUAD) {
       // every MMA and every TMA load of this CTA has completed: the K ring is free to stage the
       // four partial results of each row; thread t then combines column t of every row
-      constexpr int PARTS = 4 * C::SPLIT;                                     // results of a row
-      float* stage = reinterpret_cast<float*>(smem_gen + OFF_K);              // [PARTS][nrows][STAGE_LD]
-      float* st_m = C::SPLIT == 1 ? reinterpret_cast<float*>(smem_gen + OFF_V) : stage + PARTS * QUAD_MAX_ROWS * STAGE_LD;    // [PARTS][QUAD_MAX_ROWS]
-      float* st_l = st_m + PARTS * QUAD_MAX_ROWS;
-      const int part = C::SPLIT * warp + half;
+      float* stage = reinterpret_cast<float*>(smem_gen + OFF_K);              // [4][nrows][STAGE_LD]
+      float* st_m = reinterpret_cast<float*>(smem_gen + OFF_V);               // [4][QUAD_MAX_ROWS]
+      float* st_l = st_m + 4 * QUAD_MAX_ROWS;
       if (alive && has_o) {
         tc_fence_after();
 #pragma unroll
@@ -871,14 +803,14 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
             for (int e = 0; e < 32; ++e) v[e] = 0u;
           }
           if (row_ok) {
-            float* dst = stage + (part * nrows + r) * STAGE_LD + c * 32;
+            float* dst = stage + (warp * nrows + r) * STAGE_LD + c * 32;
 #pragma unroll
             for (int e = 0; e < 32; e += 4)
               *reinterpret_cast<float4*>(dst + e) = make_float4(__uint_as_float(v[e]), __uint_as_float(v[e + 1]),
                                                                 __uint_as_float(v[e + 2]), __uint_as_float(v[e + 3]));
           }
         }
-        if (row_ok) { st_m[part * QUAD_MAX_ROWS + r] = m_used; st_l[part * QUAD_MAX_ROWS + r] = l_sum; }
+        if (row_ok) { st_m[warp * QUAD_MAX_ROWS + r] = m_used; st_l[warp * QUAD_MAX_ROWS + r] = l_sum; }
       }
       if (trace) trace[10] = clock64() - clk0;
       asm volatile("bar.sync 1, 128;" ::: "memory");
@@ -890,11 +822,11 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
         const bool to_partial = p.partial_o != nullptr;
         const int c8 = (trow & 15) * 8;
         for (int rr = trow >> 4; rr < nrows; rr += 8) {
-          float mq[PARTS], wq[PARTS], M = -INFINITY, L = 0.f;
+          float mq[4], wq[4], M = -INFINITY, L = 0.f;
 #pragma unroll
-          for (int q = 0; q < PARTS; ++q) { mq[q] = st_m[q * QUAD_MAX_ROWS + rr]; M = fmaxf(M, mq[q]); }
+          for (int q = 0; q < 4; ++q) { mq[q] = st_m[q * QUAD_MAX_ROWS + rr]; M = fmaxf(M, mq[q]); }
 #pragma unroll
-          for (int q = 0; q < PARTS; ++q) {
+          for (int q = 0; q < 4; ++q) {
             wq[q] = (mq[q] == -INFINITY) ? 0.f : exp2_fast(mq[q] - M);
             L += st_l[q * QUAD_MAX_ROWS + rr] * wq[q];
           }
@@ -903,7 +835,7 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
 #pragma unroll
           for (int e = 0; e < 8; ++e) acc[e] = 0.f;
 #pragma unroll
-          for (int q = 0; q < PARTS; ++q) {
+          for (int q = 0; q < 4; ++q) {
             const float4 a0 = *reinterpret_cast<const float4*>(stage + (q * nrows + rr) * STAGE_LD + c8);
             const float4 a1 = *reinterpret_cast<const float4*>(stage + (q * nrows + rr) * STAGE_LD + c8 + 4);
             const float w = wq[q] * inv;                      // a quadrant that saw no key has weight 0 and O == 0
@@ -1007,7 +939,7 @@ int fmha_decode_tc_supported(const MsaFmhaParams& p) {
   if (p.block_m != 16 && p.block_m != 64 && p.block_m != 128) return 0;
   const int h_r = p.num_qo_heads / p.num_kv_heads;
   if (p.pack != h_r || p.pack > 128 || (128 % p.pack) != 0) return 0;
-  if (p.decode_rows <= 0 || p.decode_rows > 128) return 0;       // 0: caller does not want this kernel
+  if (p.decode_rows <= (p.window > 0 ? decode_tc::QUAD_MAX_ROWS : 0) || p.decode_rows > 128) return 0;       // 0: caller does not want this kernel
   if ((p.flags & MSA_FLAG_SPARSE) && p.kv_block_num > decode_tc::MAX_SPARSE_TILES) return 0;
   return 1;
 }
@@ -1042,17 +974,17 @@ int fmha_decode_tc_launch(const MsaFmhaParams& p, cudaStream_t stream) {
       const uint64_t str[2] = {static_cast<uint64_t>(p.q_stride_head) * 2, static_cast<uint64_t>(p.q_stride_tok) * 2};
       const uint32_t box[3] = {64, static_cast<uint32_t>(p.pack), 1};
       if (make_tma_map_bf16(&tq, p.q, 3, dims, str, box) != MSA_OK) return MSA_ERR_LAUNCH;
-      const uint32_t kbox[4] = {64, static_cast<uint32_t>(quad && p.window > 0 ? Cfg<false, true, true>::TK : BN), 1, 1};
+      const uint32_t kbox[4] = {64, BN, 1, 1};
       if (make_tma_map_bf16(&tk, p.k, 4, kd, ks, kbox) != MSA_OK ||
           make_tma_map_bf16(&tv, vptr, 4, kd, has_o ? vs : ks, kbox) != MSA_OK)
         return MSA_ERR_LAUNCH;
     }
   }
-  static bool attr_done[16][8] = {};
+  static bool attr_done[16][6] = {};
   int dev = 0;
   cudaGetDevice(&dev);
   using Kern = void (*)(const MsaFmhaParams, const CUtensorMap, const CUtensorMap, const CUtensorMap);
-  const int variant = (p.window > 0 ? 4 : 0) | (f8 ? 2 : 0) | (quad ? 1 : 0);
+  const int variant = p.window > 0 ? 4 + (f8 ? 1 : 0) : (f8 ? 2 : 0) | (quad ? 1 : 0);
   Kern kern;
   int smem;
   switch (variant) {
@@ -1061,14 +993,12 @@ int fmha_decode_tc_launch(const MsaFmhaParams& p, cudaStream_t stream) {
     case 2: kern = decode_tc_kernel<true, false, false>;  smem = Cfg<true, false>::SMEM_BYTES;  break;
     case 3: kern = decode_tc_kernel<true, true, false>;   smem = Cfg<true, true>::SMEM_BYTES;   break;
     case 4: kern = decode_tc_kernel<false, false, true>;  smem = Cfg<false, false, true>::SMEM_BYTES; break;
-    case 5: kern = decode_tc_kernel<false, true, true>;   smem = Cfg<false, true, true>::SMEM_BYTES;  break;
-    case 6: kern = decode_tc_kernel<true, false, true>;   smem = Cfg<true, false, true>::SMEM_BYTES;  break;
-    default: kern = decode_tc_kernel<true, true, true>;   smem = Cfg<true, true, true>::SMEM_BYTES;   break;
+    default: kern = decode_tc_kernel<true, false, true>;  smem = Cfg<true, false, true>::SMEM_BYTES;  break;
   }
   if (dev >= 16 || !attr_done[dev][variant]) {
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
       return MSA_ERR_LAUNCH;
-    if ((variant & 3) == 3 || variant == 5)      // two co-resident CTAs need the whole shared-memory carve-out
+    if (variant == 3)      // two co-resident CTAs need the whole shared-memory carve-out
       cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
     if (dev < 16) attr_done[dev][variant] = true;
   }

@@ -33,7 +33,6 @@ using namespace tc;
 
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
-constexpr int kStages = 3;
 constexpr int kHalf = 4096;                                  // K of a unit; V follows
 constexpr int kLdO = kHeadDim + 4;                           // floats of a row of O in shared memory
 constexpr float kNoMax = -3e38f;                             // maximum of a row that has seen no key
@@ -41,11 +40,18 @@ constexpr float kNoMax = -3e38f;                             // maximum of a row
 template <bool F8>
 __host__ __device__ constexpr int unit_keys() { return F8 ? 32 : 16; }
 
-constexpr int OFF_BAR = kWarps * kStages * 2 * kHalf;        // [warp][stage] full
-constexpr int OFF_FAC = OFF_BAR + kWarps * kStages * 8;      // [16] factor of a row's scores
-constexpr int OFF_FLAG = OFF_FAC + 64;                       // abort, skip
-constexpr int SMEM_BYTES = OFF_FLAG + 16 + 1024;             // + slack to align the base to 1 KB
-static_assert(2 * (SMEM_BYTES + 1024) <= 228 * 1024, "two CTAs fit an SM");
+template <int NT>
+struct Cfg {
+  // (8 rows leave registers for three CTAs with two stages, 64 e4m3 sequences x 8 heads: 66 us instead of 61)
+  static constexpr int CTAS = 2;                             // that share an SM
+  static constexpr int STAGES = 3;
+  static constexpr int OFF_BAR = kWarps * STAGES * 2 * kHalf;        // [warp][stage] full
+  static constexpr int OFF_FAC = OFF_BAR + kWarps * STAGES * 8;      // [16] factor of a row's scores
+  static constexpr int OFF_FLAG = OFF_FAC + 64;                      // abort, skip
+  static constexpr int SMEM_BYTES = OFF_FLAG + 16 + 1024;            // + slack to align the base to 1 KB
+  static_assert(CTAS * (SMEM_BYTES + 1024) <= 228 * 1024, "they fit an SM");
+  static_assert(kWarps * 8 * NT * (kLdO + 2) * 4 <= OFF_BAR, "states fit the rings");
+};
 
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t y;
@@ -71,8 +77,10 @@ __device__ __forceinline__ void load_words(const unsigned char* at, uint32_t* w)
 }
 
 template <int NT, bool F8>
-__global__ void __launch_bounds__(kThreads, 2)
+__global__ void __launch_bounds__(kThreads, Cfg<NT>::CTAS)
 window_decode_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v) {
+  using C = Cfg<NT>;
+  constexpr int OFF_BAR = C::OFF_BAR, OFF_FAC = C::OFF_FAC, OFF_FLAG = C::OFF_FLAG, kStages = C::STAGES;
   constexpr int UK = unit_keys<F8>(), STEPS = UK / 16;
   constexpr int SUB = UK * 128;                              // a half of head_dim of a bf16 unit, all of it in e4m3
   constexpr float kPOffset = F8 ? 4.f : 0.f, kRescale = F8 ? 4.f : 8.f;      // P is at most 2^8
@@ -286,11 +294,16 @@ window_decode_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_const
         for (int k = 0; k < 4; ++k)
 #pragma unroll
           for (int n = 0; n < NT; ++n) mma_e4m3(s[u][n], lo[2 * k], hi[2 * k], lo[2 * k + 1], hi[2 * k + 1], qf[n][k][0], qf[n][k][1]);
-        if (pair_q) {
+        if (pair_q) {                                        // sums of their own: chains half as long
+          float s2[NT][4] = {};
 #pragma unroll
           for (int k = 0; k < 4; ++k)
 #pragma unroll
-            for (int n = 0; n < NT; ++n) mma_e4m3(s[u][n], lo[2 * k], hi[2 * k], lo[2 * k + 1], hi[2 * k + 1], qf[n][4 + k][0], qf[n][4 + k][1]);
+            for (int n = 0; n < NT; ++n) mma_e4m3(s2[n], lo[2 * k], hi[2 * k], lo[2 * k + 1], hi[2 * k + 1], qf[n][4 + k][0], qf[n][4 + k][1]);
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) s[u][n][c] += s2[n][c];
         }
       }
     }
@@ -381,12 +394,12 @@ window_decode_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_const
 #pragma unroll
         for (int u = 0; u < 2; ++u) transpose_bytes(v[u][0][j], v[u][1][j], v[u][2][j], v[u][3][j], a[u]);
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int part = 0; part < 2; ++part)                 // hi, lo
 #pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            mma_e4m3(o[2 * j + h][n], a[0][2 * h], a[0][2 * h + 1], a[1][2 * h], a[1][2 * h + 1], pt[0][n][0], pt[STEPS - 1][n][0]);
-            mma_e4m3(o[2 * j + h][n], a[0][2 * h], a[0][2 * h + 1], a[1][2 * h], a[1][2 * h + 1], pt[0][n][1], pt[STEPS - 1][n][1]);
-          }
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+              mma_e4m3(o[2 * j + h][n], a[0][2 * h], a[0][2 * h + 1], a[1][2 * h], a[1][2 * h + 1], pt[0][n][part], pt[STEPS - 1][n][part]);
       }
     }
     __syncwarp();                                            // all lanes have read the stage
@@ -412,7 +425,6 @@ window_decode_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_const
   // ---------------- the four states of a row become one ----------------
   float* s_o = reinterpret_cast<float*>(smem);               // [warp][row][kLdO]
   float* s_m = s_o + kWarps * 8 * NT * kLdO;                 // [warp][row][2]: maximum - kPOffset, sum
-  static_assert(kWarps * 8 * NT * (kLdO + 2) * 4 <= OFF_BAR, "states fit the rings");
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -500,12 +512,12 @@ int launch(const MsaFmhaParams& p, cudaStream_t stream) {
   if (cudaGetDevice(&device) != cudaSuccess) return MSA_ERR_LAUNCH;
   static bool ready[64] = {};
   if (device < 0 || device >= 64 || !ready[device]) {
-    if (cudaFuncSetAttribute(window_decode_kernel<NT, F8>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES) != cudaSuccess ||
+    if (cudaFuncSetAttribute(window_decode_kernel<NT, F8>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<NT>::SMEM_BYTES) != cudaSuccess ||
         cudaFuncSetAttribute(window_decode_kernel<NT, F8>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared) != cudaSuccess)
       return MSA_ERR_LAUNCH;
     if (device >= 0 && device < 64) ready[device] = true;
   }
-  window_decode_kernel<NT, F8><<<p.num_work, kThreads, SMEM_BYTES, stream>>>(p, tk, tv);
+  window_decode_kernel<NT, F8><<<p.num_work, kThreads, Cfg<NT>::SMEM_BYTES, stream>>>(p, tk, tv);
   return cudaGetLastError() == cudaSuccess ? MSA_OK : MSA_ERR_LAUNCH;
 }
 

@@ -137,7 +137,7 @@ pages_copy_args, pages_fork_args, pages_free_args, pages_compact_args = map(_pac
 EXPORTS = ("msa_fmha_fwd", "msa_lse_merge", "msa_topk_select", "msa_plan_dense",
            "msa_status_string", "msa_build_arch", "msa_sizeof", "msa_fmha_fwd_split_static",
            "msa_sparse_workspace_bytes", "msa_plan_device", "msa_lse_merge_ex", "msa_lse_merge_many", "msa_norm_rope", "msa_kv4_read",
-           "msa_page_tables", "msa_page_tables_workspace_bytes", "msa_pages_copy", "msa_pages_fork", "msa_pages_fork_workspace_bytes",
+           "msa_page_tables", "msa_page_tables_workspace_bytes", "msa_fmha_fwd_merged", "msa_pages_copy", "msa_pages_fork", "msa_pages_fork_workspace_bytes",
            "msa_pages_free", "msa_pages_free_workspace_bytes", "msa_pages_compact", "msa_pages_compact_workspace_bytes")
 
 
@@ -192,6 +192,8 @@ def _load():
         if sizes:
             fn = getattr(lib, f"msa_pages_{name}_workspace_bytes")
             fn.argtypes, fn.restype = [_i32] * sizes, _i64
+    lib.msa_fmha_fwd_merged.argtypes = [ctypes.POINTER(MsaFmhaParams), _p, _i32, _p]
+    lib.msa_fmha_fwd_merged.restype = ctypes.c_int
     lib.msa_fmha_fwd_split_static.argtypes = [ctypes.POINTER(MsaFmhaParams), _p, _p]
     lib.msa_fmha_fwd_split_static.restype = ctypes.c_int
     return lib

@@ -10,6 +10,7 @@ replaced by one prebuilt C-ABI library of sm_100a kernels (see ``_lib``).
 import ctypes
 import math
 import os
+import struct
 from typing import Optional, Tuple, Union
 
 import numpy as np
@@ -1051,8 +1052,15 @@ def _fmha_sail(
     return out, max_score
 
 
-def _window_params(q_dtype, kv_dtype, plan, nhd):
-    """What is the same in every call with this plan and these types, as the bytes of the arguments: the kernel, its work list and the plan's metadata."""
+_WINDOW_TYPES = (torch.bfloat16, torch.float8_e4m3fn)
+_WINDOW_OUT = (torch.bfloat16, torch.float32)
+_WINDOW_HEAD = struct.Struct("@7Q")           # the arguments' first fields: q, k, v, out, lse, max_score, partial_o
+_WINDOW_STRIDES = struct.Struct("@10q")       # q, k, v, out
+
+
+def _window_params(q_dtype, kv_dtype, plan):
+    """What is the same in every call with this plan and these types: the arguments' bytes (the kernel, its work list, the plan's metadata), the
+    number of splits, and where their number per row is."""
     page_size, splits, pack = max(0, plan["page_size"]), plan["num_kv_splits"], plan["pack_factor"]
     h_r = plan["orig_num_qo_heads"] // plan["num_kv_heads"]
     p = _lib.MsaFmhaParams(qo_start=plan["qo_segment_offsets"].data_ptr(), kv_start=plan["kv_segment_offsets"].data_ptr(),
@@ -1065,7 +1073,7 @@ def _window_params(q_dtype, kv_dtype, plan, nhd):
     elif _USE_DECODE_TC and 0 < plan["max_qo_len"] * pack <= 128 and pack == h_r:
         # up to 16 rows: the streaming kernel, on any pages of whole units; else the tcgen05 decode kernel, on pages of 128 keys
         p.decode_rows = plan["max_qo_len"] * pack
-    return bytes(p), p.num_splits
+    return bytes(p), p.num_splits, _ptr(plan["num_kv_splits_per_row"])
 
 
 def _fmha_sail_window(q, k, v, plan, kv_indices, kv_block_indexes, q_offset_override, out, max_score, sm_scale, q_scale, k_scale, v_scale, o_scale,
@@ -1086,19 +1094,20 @@ def _fmha_sail_window(q, k, v, plan, kv_indices, kv_block_indexes, q_offset_over
         raise ValueError("plan page_size does not match the K/V layout (kv_indices given?)")
     nhd = False
     if paged:
-        nhd, num_kv_heads, page_size = _detect_paged_kv_layout(k_shape, plan_page)
+        nhd, num_kv_heads, _ = _detect_paged_kv_layout(k_shape, plan_page)
     else:
         if len(k_shape) != 3:
             raise ValueError(f"ragged K/V must be [total_kv, Hkv, 128], got {tuple(k_shape)}")
         num_kv_heads = k_shape[1]
     if v.shape != k_shape:
         raise ValueError(f"k and v must have the same shape, got {tuple(k_shape)} and {tuple(v.shape)}")
-    if k_dtype != v.dtype or k_dtype not in (torch.bfloat16, torch.float8_e4m3fn) or (q_dtype != torch.bfloat16 and q_dtype != k_dtype):
+    if k_dtype is not v.dtype or k_dtype not in _WINDOW_TYPES or (q_dtype is not k_dtype and q_dtype is not torch.bfloat16):
         raise ValueError(f"window_size needs k and v in bfloat16 or float8_e4m3fn and q in bfloat16 or their type, got q={q_dtype}, k={k_dtype}, v={v.dtype}")
     nnz_qo, num_qo_heads, _ = q_shape
     dev = q.device
     index = dev.index
-    if any(t is not None and t.get_device() != index for t in (k, v, kv_indices, out, lse, plan["qo_offset"])):
+    if (k.get_device() != index or v.get_device() != index or (paged and kv_indices.get_device() != index) or (out is not None and out.get_device() != index)
+            or (lse is not None and lse.get_device() != index) or plan["qo_offset"].get_device() != index):
         cache._same_device(dev, k=k, v=v, kv_indices=kv_indices, out=out, lse=lse, plan=plan["qo_offset"])
     if plan["_host"] is None:                 # planned on the device: total_qo_len is the bound max_total_q
         if nnz_qo > plan["total_qo_len"]:
@@ -1107,66 +1116,66 @@ def _fmha_sail_window(q, k, v, plan, kv_indices, kv_block_indexes, q_offset_over
         raise ValueError(f"plan was made for {plan['total_qo_len']} query tokens, q has {nnz_qo}")
     if plan["orig_num_qo_heads"] != num_qo_heads or plan["num_kv_heads"] != num_kv_heads:
         raise ValueError("plan head counts do not match q / k")
+    if paged and (kv_indices.dtype is not torch.int32 or kv_indices.dim() != 1 or not kv_indices.is_contiguous()):
+        raise ValueError("kv_indices must be a contiguous int32 vector")
     if check_input_valid and plan["_host"] is not None:
         _validate_fmha_inputs(q, k, v, plan, paged, nhd, num_kv_heads, plan_page if paged else 0, kv_indices, None, plan["qo_offset"])
-    if out is None:
-        out = torch.empty(q_shape, device=dev, dtype=torch.bfloat16)
-    elif out.dtype not in (torch.bfloat16, torch.float32) or out.shape != q_shape or out.stride(2) != 1:
-        raise ValueError(f"out must be bfloat16 or float32 {tuple(q_shape)} with a contiguous head_dim, got {out.dtype} {tuple(out.shape)}")
-    if lse is not None and (lse.dtype != torch.float32 or lse.shape != (nnz_qo, num_qo_heads) or not lse.is_contiguous()):
-        raise ValueError(f"lse must be contiguous float32 {(nnz_qo, num_qo_heads)}, got {lse.dtype} {tuple(lse.shape)}")
-    if nnz_qo == 0:
-        return out, None
-    key = (q_dtype, k_dtype, nhd, _USE_TC, _FORCE_TC, _USE_DECODE_TC)
-    kept = plan.setdefault("_window_params", {})
-    base = kept.get(key)
-    if base is None:
-        base = kept[key] = _window_params(q_dtype, k_dtype, plan, nhd)
-    p, splits = _lib.MsaFmhaParams.from_buffer_copy(base[0]), base[1]
     q_stride, k_stride, v_stride = q.stride(), k.stride(), v.stride()
     if q_stride[2] != 1 or k_stride[-1] != 1 or v_stride[-1] != 1:
         raise ValueError("head_dim of q, k and v must be contiguous")
-    p.q, p.k, p.v, p.status = q.data_ptr(), k.data_ptr(), v.data_ptr(), _status_ptr(dev)
-    p.q_stride_tok, p.q_stride_head, p.total_q, p.kv_extent = q_stride[0], q_stride[1], nnz_qo, k_shape[0]
-    if paged:
-        if kv_indices.dtype != torch.int32 or kv_indices.dim() != 1 or not kv_indices.is_contiguous():
-            raise ValueError("kv_indices must be a contiguous int32 vector")
-        p.kv_indices, p.num_page_entries = kv_indices.data_ptr(), kv_indices.shape[0]
-        tok, head = (1, 2) if nhd else (2, 1)
-        p.k_stride_page, p.k_stride_head, p.k_stride_tok = k_stride[0], k_stride[head], k_stride[tok]
-        p.v_stride_page, p.v_stride_head, p.v_stride_tok = v_stride[0], v_stride[head], v_stride[tok]
+    out_dtype, o_stride = torch.bfloat16, None
+    if out is None:
+        out = torch.empty(q_shape, device=dev, dtype=torch.bfloat16)
     else:
-        p.k_stride_tok, p.k_stride_head, p.v_stride_tok, p.v_stride_head = k_stride[0], k_stride[1], v_stride[0], v_stride[1]
-    if q_scale is None and k_scale is None and v_scale is None and o_scale is None:
-        k_s, out_scale = 1.0, 1.0
-    else:
+        out_dtype, o_stride = out.dtype, out.stride()
+        if out_dtype not in _WINDOW_OUT or out.shape != q_shape or o_stride[2] != 1:
+            raise ValueError(f"out must be bfloat16 or float32 {tuple(q_shape)} with a contiguous head_dim, got {out.dtype} {tuple(out.shape)}")
+    if lse is not None and (lse.dtype is not torch.float32 or lse.shape != (nnz_qo, num_qo_heads) or not lse.is_contiguous()):
+        raise ValueError(f"lse must be contiguous float32 {(nnz_qo, num_qo_heads)}, got {lse.dtype} {tuple(lse.shape)}")
+    if nnz_qo == 0:
+        return out, None
+    kept = plan.get("_window_params")
+    if kept is None:
+        kept = plan["_window_params"] = {}
+    key = (q_dtype, k_dtype, _USE_TC, _FORCE_TC, _USE_DECODE_TC)
+    base = kept.get(key)
+    if base is None:
+        base = kept[key] = _window_params(q_dtype, k_dtype, plan)
+    p, splits = _lib.MsaFmhaParams.from_buffer_copy(base[0]), base[1]
+    sm_scale = 0.08838834764831845 if sm_scale is None else float(sm_scale)     # 1 / sqrt(128)
+    k_s, out_scale = 1.0, 1.0
+    if q_scale is not None or k_scale is not None or v_scale is not None or o_scale is not None:
         (k_s, k_head), (out_scale, v_head) = _scale_pair(q_scale, k_scale, dev, num_kv_heads), _scale_pair(o_scale, v_scale, dev, num_kv_heads)
         p.k_scale_head, p.v_scale_head = _ptr(k_head), _ptr(v_head)
-    p.sm_scale, p.out_scale = float(k_s * (0.08838834764831845 if sm_scale is None else sm_scale)), out_scale    # 1 / sqrt(128)
+    if paged:
+        tok, head = (1, 2) if nhd else (2, 1)
+        p.kv_indices, p.num_page_entries = kv_indices.data_ptr(), kv_indices.shape[0]
+        strides = (q_stride[0], q_stride[1], k_stride[0], k_stride[head], k_stride[tok], v_stride[0], v_stride[head], v_stride[tok])
+    else:
+        strides = (q_stride[0], q_stride[1], 0, k_stride[1], k_stride[0], 0, v_stride[1], v_stride[0])
     if _SHOW_PARAMS:
-        _show_params(q, plan, paged, plan_page, 0.08838834764831845 if sm_scale is None else float(sm_scale), True, None, None)
+        _show_params(q, plan, paged, plan_page, sm_scale, True, None, None)
     with cache._on(dev):
-        stream = _stream()
-        # partials of its own: two streams, or two captured graphs, may run one plan at the same time
-        kernel_out = out
+        kernel_out, part = out, 0
+        if splits > 1:                        # partials of its own: two streams, or two captured graphs, may run one plan at the same time
+            rows = splits * nnz_qo * num_qo_heads
+            partials = torch.empty(rows * 129, dtype=torch.float32, device=dev)
+            part = partials.data_ptr()
+            p.partial_lse = part + rows * 512
+        elif out_dtype is torch.float32:
+            kernel_out, o_stride = torch.empty(q_shape, dtype=torch.bfloat16, device=dev), None
+        if o_stride is None:
+            o_stride = (num_qo_heads * 128, 128)
+        _WINDOW_HEAD.pack_into(p, 0, q.data_ptr(), k.data_ptr(), v.data_ptr(), kernel_out.data_ptr(), 0 if lse is None else lse.data_ptr(), 0, part)
+        _WINDOW_STRIDES.pack_into(p, _lib.MsaFmhaParams.q_stride_tok.offset, *strides, o_stride[0], o_stride[1])
+        p.total_q, p.kv_extent, p.status = nnz_qo, k_shape[0], _status_ptr(dev)
+        p.sm_scale, p.out_scale = k_s * sm_scale, out_scale
         if splits > 1:
-            part = torch.empty(splits * nnz_qo * num_qo_heads * 129, dtype=torch.float32, device=dev)
-            p.partial_o = part.data_ptr()
-            p.partial_lse = part.data_ptr() + splits * nnz_qo * num_qo_heads * 512
+            _lib.check(_lib.lib.msa_fmha_fwd_merged(ctypes.byref(p), base[2], _dt_code(out_dtype), _stream()), "msa_fmha_fwd_merged")
         else:
-            if out.dtype == torch.float32:
-                kernel_out = torch.empty(q_shape, dtype=torch.bfloat16, device=dev)
-            if lse is not None:
-                p.lse = lse.data_ptr()
-            o_stride = kernel_out.stride()
-            p.out, p.out_stride_tok, p.out_stride_head = kernel_out.data_ptr(), o_stride[0], o_stride[1]
-        _lib.check(_lib.lib.msa_fmha_fwd(ctypes.byref(p), stream), "msa_fmha_fwd")
-        if splits > 1:
-            _lib.check(_lib.lib.msa_lse_merge_many(
-                p.partial_o, p.partial_lse, _ptr(plan["num_kv_splits_per_row"]), out.data_ptr(), _dt_code(out.dtype), _ptr(lse),
-                splits, nnz_qo, num_qo_heads, out.stride(0), out.stride(1), out_scale, stream), "msa_lse_merge_many")
-        elif kernel_out is not out:
-            _copy_rows(out, kernel_out, plan)
+            _lib.check(_lib.lib.msa_fmha_fwd(ctypes.byref(p), _stream()), "msa_fmha_fwd")
+            if kernel_out is not out:
+                _copy_rows(out, kernel_out, plan)
     return out, None
 
 
