@@ -30,6 +30,7 @@ int make_tma_map_bf16(CUtensorMap* m, const void* base, int rank, const uint64_t
                       const uint32_t* box);
 int make_tma_map_u8(CUtensorMap* m, const void* base, int rank, const uint64_t* dims, const uint64_t* strides_bytes,
                     const uint32_t* box);
+int fmha_window_rows(const MsaFmhaParams& p);
 
 namespace decode_tc {
 namespace {
@@ -85,8 +86,8 @@ __device__ __forceinline__ unsigned long long global_ns() {
 //         half pages (64 keys): two 64-column S buffers and O fit the 256 columns, so Q K^T of tile
 //         j + 1 still overlaps the softmax of tile j.  The barriers live in rows 16-31 of the Q
 //         tile, which no real row uses.
-//   WIN   rows see a window and the first keys only; tiles that no row sees are not loaded.  (More than 16 rows: fewer stream through
-//         the kernel of fmha_window.cu.)
+//   WIN   rows see a window and the first keys only; tiles that no row sees are not loaded.  (Fewer rows stream through the kernel of
+//         fmha_window.cu.)
 //   F8 && WIN ("pair"): Q and P are pairs of e4m3 values, x = hi + lo with lo = e4m3(x - hi), both multiplied into the same
 //         accumulator: 8 bits where one value has 4, for MMAs that have nothing else to do.  (A single value puts 2.6 % of noise on
 //         each weight: with a window there are few enough that it shows.)
@@ -939,7 +940,7 @@ int fmha_decode_tc_supported(const MsaFmhaParams& p) {
   if (p.block_m != 16 && p.block_m != 64 && p.block_m != 128) return 0;
   const int h_r = p.num_qo_heads / p.num_kv_heads;
   if (p.pack != h_r || p.pack > 128 || (128 % p.pack) != 0) return 0;
-  if (p.decode_rows <= (p.window > 0 ? decode_tc::QUAD_MAX_ROWS : 0) || p.decode_rows > 128) return 0;       // 0: caller does not want this kernel
+  if (p.decode_rows <= (p.window > 0 ? fmha_window_rows(p) : 0) || p.decode_rows > 128) return 0;       // 0: caller does not want this kernel
   if ((p.flags & MSA_FLAG_SPARSE) && p.kv_block_num > decode_tc::MAX_SPARSE_TILES) return 0;
   return 1;
 }

@@ -1,4 +1,4 @@
-// Windowed attention of up to 16 rows (decode: tokens x query heads of a KV head), streamed at the rate of the memory.
+// Windowed attention of up to 32 rows, 16 over an e4m3 cache (decode: tokens x query heads of a KV head), streamed at the rate of the memory.
 //
 // Per key and KV head 4 * 128 multiplications are made for each row, so memory is the bound, and what has to be short is the chain from a
 // key's arrival to its place in the sums.  In the tcgen05 decode kernel that chain (load, Q K^T, commit, softmax, store, P V) takes 1 100
@@ -46,9 +46,14 @@ struct Cfg {
   static constexpr int CTAS = 2;                             // that share an SM
   static constexpr int STAGES = 3;
   static constexpr int OFF_BAR = kWarps * STAGES * 2 * kHalf;        // [warp][stage] full
-  static constexpr int OFF_FAC = OFF_BAR + kWarps * STAGES * 8;      // [16] factor of a row's scores
-  static constexpr int OFF_FLAG = OFF_FAC + 64;                      // abort, skip
-  static constexpr int SMEM_BYTES = OFF_FLAG + 16 + 1024;            // + slack to align the base to 1 KB
+  static constexpr int OFF_FAC = OFF_BAR + kWarps * STAGES * 8;      // [8 NT] factor of a row's scores
+  static constexpr int OFF_LIM = OFF_FAC + 32 * NT;                  // [8 NT] first key that a row does not see any more, first key of its window
+  static constexpr int OFF_FLAG = OFF_LIM + 64 * NT;                 // abort, skip
+  // 32 rows: Q^T in shared memory, [step][8 rows][lane] x 8 bytes, or registers run out
+  static constexpr bool Q_SHARED = NT == 4;
+  static constexpr int OFF_Q = OFF_FLAG + 16;
+  static constexpr int SMEM_BYTES = OFF_Q + (Q_SHARED ? NT * 2048 : 0) + 1024;      // + slack to align the base to 1 KB
+  static_assert(OFF_FAC % 16 == 0 && OFF_Q % 16 == 0, "alignment");
   static_assert(CTAS * (SMEM_BYTES + 1024) <= 228 * 1024, "they fit an SM");
   static_assert(kWarps * 8 * NT * (kLdO + 2) * 4 <= OFF_BAR, "states fit the rings");
 };
@@ -80,7 +85,7 @@ template <int NT, bool F8>
 __global__ void __launch_bounds__(kThreads, Cfg<NT>::CTAS)
 window_decode_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v) {
   using C = Cfg<NT>;
-  constexpr int OFF_BAR = C::OFF_BAR, OFF_FAC = C::OFF_FAC, OFF_FLAG = C::OFF_FLAG, kStages = C::STAGES;
+  constexpr int OFF_BAR = C::OFF_BAR, OFF_FAC = C::OFF_FAC, OFF_LIM = C::OFF_LIM, OFF_FLAG = C::OFF_FLAG, kStages = C::STAGES;
   constexpr int UK = unit_keys<F8>(), STEPS = UK / 16;
   constexpr int SUB = UK * 128;                              // a half of head_dim of a bf16 unit, all of it in e4m3
   constexpr float kPOffset = F8 ? 4.f : 0.f, kRescale = F8 ? 4.f : 8.f;      // P is at most 2^8
@@ -161,19 +166,21 @@ window_decode_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_const
   const float signed_scale = p.sm_scale * kLog2e * (p.k_scale_head ? p.k_scale_head[kvh] : 1.f);
   const float scale = signed_scale == 0.f ? 1.f : fabsf(signed_scale);
   [[maybe_unused]] const uint32_t flip = signed_scale < 0.f ? 0x80008000u : 0u, keep = signed_scale == 0.f ? 0u : 0xffffffffu;
-  uint32_t qf[NT][8][2];                                     // bf16: [step of 16 elements]; e4m3: [step of 32 elements, + 4: lo]
+  uint32_t qf[C::Q_SHARED ? 1 : NT][8][2];                   // bf16: [step of 16 elements]; e4m3: [step of 32 elements, + 4: lo]
   [[maybe_unused]] const bool pair_q = F8 && p.q_dtype == MSA_DT_BF16;
   float* s_fac = reinterpret_cast<float*>(smem + OFF_FAC);
+  // (in shared memory: warp n makes those of rows 8 n .. 8 n + 7)
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
+  for (int n_ = 0; n_ < (C::Q_SHARED ? 1 : NT); ++n_) {
+    const int n = C::Q_SHARED ? warp : n_;
     const int row = min(8 * n + g, max(nrows, 1) - 1);       // rows that are none repeat the last one and are not written
     const int64_t at = static_cast<int64_t>(qo_base + row / G) * p.q_stride_tok + static_cast<int64_t>(head0 + row % G) * p.q_stride_head;
     if constexpr (!F8) {
       const uint32_t* src = reinterpret_cast<const uint32_t*>(static_cast<const __nv_bfloat16*>(p.q) + at);
 #pragma unroll
       for (int s = 0; s < 8; ++s) {
-        qf[n][s][0] = nrows > 0 ? (src[8 * s + t4] ^ flip) & keep : 0u;
-        qf[n][s][1] = nrows > 0 ? (src[8 * s + 4 + t4] ^ flip) & keep : 0u;
+        qf[n_][s][0] = nrows > 0 ? (src[8 * s + t4] ^ flip) & keep : 0u;
+        qf[n_][s][1] = nrows > 0 ? (src[8 * s + 4 + t4] ^ flip) & keep : 0u;
       }
     } else {
       int e = 0;                                             // exponent that the row is divided by
@@ -185,8 +192,8 @@ window_decode_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_const
         }
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
-          qf[n][c >> 1][c & 1] = (v[c] ^ (flip | (flip >> 8))) & keep;
-          qf[n][4 + (c >> 1)][c & 1] = 0;
+          qf[n_][c >> 1][c & 1] = (v[c] ^ (flip | (flip >> 8))) & keep;
+          qf[n_][4 + (c >> 1)][c & 1] = 0;
         }
       } else {
         uint32_t v[16] = {};                                 // elements 32 t .. 32 t + 31
@@ -210,27 +217,34 @@ window_decode_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_const
 #pragma unroll
           for (int h = 0; h < 2; ++h)
             e4m3_pair(__uint_as_float(v[2 * c + h] << 16) * up, __uint_as_float(v[2 * c + h] & 0xffff0000u) * up, hi[h], lo[h]);
-          qf[n][c >> 1][c & 1] = hi[0] | (hi[1] << 16);
-          qf[n][4 + (c >> 1)][c & 1] = lo[0] | (lo[1] << 16);
+          qf[n_][c >> 1][c & 1] = hi[0] | (hi[1] << 16);
+          qf[n_][4 + (c >> 1)][c & 1] = lo[0] | (lo[1] << 16);
         }
       }
-      if (warp == 0 && t4 == 0) s_fac[8 * n + g] = signed_scale == 0.f ? 1.f : scale * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+      if ((C::Q_SHARED || warp == 0) && t4 == 0) s_fac[8 * n + g] = signed_scale == 0.f ? 1.f : scale * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
     }
   }
-  if constexpr (F8) __syncthreads();
+  uint2* s_q = reinterpret_cast<uint2*>(smem + C::OFF_Q) + lane;
+  if constexpr (C::Q_SHARED) {
+#pragma unroll
+    for (int s = 0; s < 8; ++s) s_q[(s * NT + warp) * 32] = make_uint2(qf[0][s][0], qf[0][s][1]);
+  }
+  auto q_of = [&](int n, int s) -> uint2 {
+    if constexpr (C::Q_SHARED) return s_q[(s * NT + n) * 32];
+    else return make_uint2(qf[n][s][0], qf[n][s][1]);
+  };
+  int2* s_lim = reinterpret_cast<int2*>(smem + OFF_LIM);
+  if (threadIdx.x < 8 * NT) {
+    const int tok = min(static_cast<int>(threadIdx.x), max(nrows, 1) - 1) / G;
+    s_lim[threadIdx.x] = make_int2(max(0, min(kv_len, tok + off + 1)), window_first(tok + off, kv_len, p.window));
+  }
+  __syncthreads();
 
-  // of rows 8 n + 2 t4 + c: factor of the scores, first key that the row does not see any more, first key of its window
-  float fac[NT][2];
-  int lim[NT][2], from[NT][2];
+  float fac[NT][2];                                          // of rows 8 n + 2 t4 + c: factor of the scores
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const int r = 8 * n + 2 * t4 + c, tok = min(r, max(nrows, 1) - 1) / G;
-      fac[n][c] = F8 ? s_fac[r] : scale;
-      lim[n][c] = max(0, min(kv_len, tok + off + 1));
-      from[n][c] = window_first(tok + off, kv_len, p.window);
-    }
+    for (int c = 0; c < 2; ++c) fac[n][c] = F8 ? s_fac[8 * n + 2 * t4 + c] : scale;
   const int lim_first = max(0, min(kv_len, off + 1)), from_last = window_first(off + ntok - 1, kv_len, p.window);
 
   float m[NT][2];                                            // maximum - kPOffset
@@ -281,7 +295,10 @@ window_decode_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_const
           const int ch = 2 * k + (lane >> 4);
           ldmatrix_x4(kt_u + (ch >> 3) * SUB + swizzled(lane & 15, ch & 7), a[0], a[1], a[2], a[3]);
 #pragma unroll
-          for (int n = 0; n < NT; ++n) mma_16816<false>(s[u][n], a, qf[n][k][0], qf[n][k][1]);
+          for (int n = 0; n < NT; ++n) {
+            const uint2 q = q_of(n, k);
+            mma_16816<false>(s[u][n], a, q.x, q.y);
+          }
         }
       } else {
         uint32_t lo[8], hi[8];                               // keys g and g + 8
@@ -293,13 +310,19 @@ window_decode_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_const
 #pragma unroll
         for (int k = 0; k < 4; ++k)
 #pragma unroll
-          for (int n = 0; n < NT; ++n) mma_e4m3(s[u][n], lo[2 * k], hi[2 * k], lo[2 * k + 1], hi[2 * k + 1], qf[n][k][0], qf[n][k][1]);
+          for (int n = 0; n < NT; ++n) {
+            const uint2 q = q_of(n, k);
+            mma_e4m3(s[u][n], lo[2 * k], hi[2 * k], lo[2 * k + 1], hi[2 * k + 1], q.x, q.y);
+          }
         if (pair_q) {                                        // sums of their own: chains half as long
           float s2[NT][4] = {};
 #pragma unroll
           for (int k = 0; k < 4; ++k)
 #pragma unroll
-            for (int n = 0; n < NT; ++n) mma_e4m3(s2[n], lo[2 * k], hi[2 * k], lo[2 * k + 1], hi[2 * k + 1], qf[n][4 + k][0], qf[n][4 + k][1]);
+            for (int n = 0; n < NT; ++n) {
+              const uint2 q = q_of(n, 4 + k);
+              mma_e4m3(s2[n], lo[2 * k], hi[2 * k], lo[2 * k + 1], hi[2 * k + 1], q.x, q.y);
+            }
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -310,14 +333,16 @@ window_decode_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_const
     // ---- softmax: mask, a maximum that may lag, exponents ----
     if (key0 + UK > lim_first || (key0 < from_last && key0 + UK > p.sink_tokens)) {
 #pragma unroll
-      for (int u = 0; u < STEPS; ++u)
+      for (int n = 0; n < NT; ++n) {
+        const int4 r = *reinterpret_cast<const int4*>(s_lim + 8 * n + 2 * t4);       // of two rows
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int u = 0; u < STEPS; ++u)
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             const int key = key0 + 16 * u + 8 * (c >> 1) + g;
-            if (key >= lim[n][c & 1] || (key < from[n][c & 1] && key >= p.sink_tokens)) s[u][n][c] = -INFINITY;
+            if (key >= (c & 1 ? r.z : r.x) || (key < (c & 1 ? r.w : r.y) && key >= p.sink_tokens)) s[u][n][c] = -INFINITY;
           }
+      }
     }
     bool raise = false;
     float top[NT][2];
@@ -524,9 +549,11 @@ int launch(const MsaFmhaParams& p, cudaStream_t stream) {
 }  // namespace
 }  // namespace window
 
-// Windowed items of at most 16 packed rows; pages of whole units, or ragged keys.
+// Windowed items of few packed rows (with 32 over an e4m3 cache registers run out: 256 items x 9 pages take 51 us, on the tcgen05 decode
+// kernel 47; bf16: 30 and 42); pages of whole units, or ragged keys.
+int fmha_window_rows(const MsaFmhaParams& p) { return p.kv_dtype == MSA_DT_E4M3 ? 16 : 32; }
 int fmha_window_supported(const MsaFmhaParams& p) {
-  if (p.window <= 0 || (p.flags & MSA_FLAG_SPARSE) || p.block_m != 16 || p.decode_rows < 1 || p.decode_rows > 16) return 0;
+  if (p.window <= 0 || (p.flags & MSA_FLAG_SPARSE) || p.decode_rows < 1 || p.decode_rows > fmha_window_rows(p)) return 0;
   if (p.pack != p.num_qo_heads / p.num_kv_heads) return 0;
   const bool f8 = p.kv_dtype == MSA_DT_E4M3;
   if (p.q_dtype != MSA_DT_BF16 && !(f8 && p.q_dtype == MSA_DT_E4M3)) return 0;
@@ -539,7 +566,8 @@ int fmha_window_launch(const MsaFmhaParams& p, cudaStream_t stream) {
   if (p.num_work <= 0) return MSA_OK;
   const bool f8 = p.kv_dtype == MSA_DT_E4M3;
   if (p.decode_rows <= 8) return f8 ? launch<1, true>(p, stream) : launch<1, false>(p, stream);
-  return f8 ? launch<2, true>(p, stream) : launch<2, false>(p, stream);
+  if (p.decode_rows <= 16) return f8 ? launch<2, true>(p, stream) : launch<2, false>(p, stream);
+  return launch<4, false>(p, stream);
 }
 
 }  // namespace msa

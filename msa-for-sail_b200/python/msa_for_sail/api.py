@@ -467,7 +467,9 @@ def _fmha_sail_plan(
                 info["num_work_tc"] = n_tc
         # Two CTAs of the e4m3 decode kernel share an SM.  A cut at the average load may take more partials than a workspace
         # sized for the plain cut holds: such a workspace gets the plain cut.
-        shared = 1 if max_qo * pack > 16 else (_kv4_ctas(max_qo * pack) if use_kv4_cache else (2 if use_fp8_kvcache or window[0] else 1))
+        # (windowed rows that the streaming kernel takes: two as well)
+        few = max_qo * pack <= (32 if window[0] and not use_fp8_kvcache else 16)
+        shared = 1 if not few else (_kv4_ctas(max_qo * pack) if use_kv4_cache else (2 if use_fp8_kvcache or window[0] else 1))
         for ctas in (shared, -1):
             args = _lib.MsaPlanArgs(
                 a_q.ctypes.data, a_k.ctypes.data, a_o.ctypes.data, batch, num_qo_heads, hkv, block_m, pack,
@@ -1071,7 +1073,7 @@ def _window_params(q_dtype, kv_dtype, plan):
     if plan.get("work_tc") is not None and q_dtype == kv_dtype and page_size in (0, 128) and _USE_TC and (plan["tc_preferred"] or _FORCE_TC):
         p.work, p.num_work, p.block_m, p.num_splits = plan["work_tc"].data_ptr(), plan["num_work_tc"], 256, 1
     elif _USE_DECODE_TC and 0 < plan["max_qo_len"] * pack <= 128 and pack == h_r:
-        # up to 16 rows: the streaming kernel, on any pages of whole units; else the tcgen05 decode kernel, on pages of 128 keys
+        # few rows: the streaming kernel, on any pages of whole units; else the tcgen05 decode kernel, on pages of 128 keys
         p.decode_rows = plan["max_qo_len"] * pack
     return bytes(p), p.num_splits, _ptr(plan["num_kv_splits_per_row"])
 
