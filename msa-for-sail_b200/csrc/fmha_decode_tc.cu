@@ -86,35 +86,38 @@ __device__ __forceinline__ unsigned long long global_ns() {
 //         half pages (64 keys): two 64-column S buffers and O fit the 256 columns, so Q K^T of tile
 //         j + 1 still overlaps the softmax of tile j.  The barriers live in rows 16-31 of the Q
 //         tile, which no real row uses.
-//   WIN   rows see a window and the first keys only; tiles that no row sees are not loaded.  (Fewer rows stream through the kernel of
-//         fmha_window.cu.)
+//   WIN   rows see a window and the first keys only; tiles that no row sees are not loaded.  Dual too: with one CTA an SM the chain
+//         of a tile (S, softmax, P V) is what an SM waits for, 2.1 us in bf16 and 2.5 in e4m3 for 128 keys.  (Fewer rows stream through the
+//         kernel of fmha_window.cu.)
 //   F8 && WIN ("pair"): Q and P are pairs of e4m3 values, x = hi + lo with lo = e4m3(x - hi), both multiplied into the same
 //         accumulator: 8 bits where one value has 4, for MMAs that have nothing else to do.  (A single value puts 2.6 % of noise on
 //         each weight: with a window there are few enough that it shows.)
 template <bool F8, bool QUAD, bool WIN = false>
 struct Cfg {
   static_assert(!(QUAD && WIN), "windowed items of few rows have a kernel of their own");
-  static constexpr bool DUAL = F8 && QUAD;
+  static constexpr bool DUAL = (F8 && QUAD) || WIN;
   static constexpr bool PAIR = F8 && WIN;
   static constexpr int TK = DUAL ? 64 : 128;              // keys per tile
   static constexpr int NSUB = F8 ? 1 : 2;                 // 128-byte-wide sub-tiles per tile
-  static constexpr int TILE_BYTES = NSUB * TK * 128;
-  static constexpr int RING_BYTES = DUAL ? 48 * 1024 : 96 * 1024;
-  static constexpr int STAGES = RING_BYTES / TILE_BYTES;  // bf16 3, e4m3 6 (dual: 6 half pages)
+  static constexpr int KV_SUB = TK * 128;                 // one sub-tile of K or V
+  static constexpr int TILE_BYTES = NSUB * KV_SUB;
+  static constexpr int RING_BYTES = WIN ? 32 * 1024 : DUAL ? 48 * 1024 : 96 * 1024;
+  static constexpr int STAGES = RING_BYTES / TILE_BYTES;  // bf16 3, e4m3 6 (dual: 6 half pages, windowed: 2 and 4)
   static constexpr int OFF_Q = 0;
   [[maybe_unused]] static constexpr int OFF_Q_LO = SUB_BYTES;      // pairs
   // dual: rows 112-127 of the Q tile are never real rows, the K ring may start there
-  static constexpr int OFF_K = DUAL ? SUB_BYTES - 2048 : 2 * SUB_BYTES;
+  static constexpr int OFF_K = DUAL && !WIN ? SUB_BYTES - 2048 : 2 * SUB_BYTES;
   static constexpr int OFF_V = OFF_K + RING_BYTES;
   static constexpr int END = OFF_V + RING_BYTES;
-  static constexpr int OFF_BAR = DUAL ? 2048 : END;
-  static constexpr int SMEM_BYTES = (DUAL ? END : END + 1024) + 1024;   // + slack to align the base to 1 KB
+  static constexpr int OFF_BAR = DUAL && !WIN ? 2048 : END;
+  static constexpr int SMEM_BYTES = (DUAL && !WIN ? END : END + 1024) + 1024;   // + slack to align the base to 1 KB
+  static_assert(!DUAL || 2 * (SMEM_BYTES + 1024) <= 228 * 1024, "two CTAs fit an SM");
   static constexpr int NBUF = 2;                          // S buffers in TMEM
   static constexpr int TMEM_COLS = DUAL ? 256 : 512;
   static constexpr int O_COL = NBUF * TK;
   static constexpr int MIN_CTAS = DUAL ? 2 : 1;
   static_assert(STAGES <= MAX_STAGES, "barrier table");
-  static_assert(4 * QUAD_MAX_ROWS * STAGE_LD * 4 <= RING_BYTES, "O staging fits the K ring");
+  static_assert(!QUAD || 4 * QUAD_MAX_ROWS * STAGE_LD * 4 <= RING_BYTES, "O staging fits the K ring");
 };
 
 template <bool F8, bool QUAD, bool WIN>
@@ -122,7 +125,7 @@ __global__ void __launch_bounds__(NTHREADS, (Cfg<F8, QUAD, WIN>::MIN_CTAS))
 decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant__ CUtensorMap tm_q,
                  const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v) {
   using C = Cfg<F8, QUAD, WIN>;
-  constexpr int NSUB = C::NSUB, TILE_BYTES = C::TILE_BYTES, STAGES = C::STAGES, NBUF = C::NBUF, TK = C::TK;
+  constexpr int NSUB = C::NSUB, KV_SUB = C::KV_SUB, TILE_BYTES = C::TILE_BYTES, STAGES = C::STAGES, NBUF = C::NBUF, TK = C::TK;
   constexpr bool PAIR = C::PAIR;
   constexpr int UPP = BN / TK;                      // tiles per page
   constexpr int OFF_Q = C::OFF_Q, OFF_K = C::OFF_K, OFF_V = C::OFF_V, OFF_BAR = C::OFF_BAR;
@@ -197,12 +200,21 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
   const int kv_len = p.kv_len[b];
   const int off = p.qo_offset[b];
   const int page_base = p.kv_page_indptr[b];
-  // windowed: first key of the first row's window, end of what the last row sees
-  [[maybe_unused]] int first_key = 0, end_key = 0;
+  // Windowed: the item's tiles of TK keys are numbered without those that no row sees (a half page next to a page's visible half, too):
+  // number t stands for tile t of the keys below sink_t, for t + skip_t from there on.  first_key: of the first row's window, end_key: behind
+  // what the last row sees.
+  [[maybe_unused]] int first_key = 0, end_key = 0, sink_t = 0, skip_t = 0, t_begin = 0, t_end = 0;
   [[maybe_unused]] auto real_page = [&](int t) { return t < sink_tiles(p.sink_tokens) ? t : t + skip; };
   if constexpr (WIN) {
     first_key = window_first(off, kv_len, p.window);
     end_key = max(0, min(kv_len, off + ntok));
+    sink_t = p.sink_tokens / TK + (p.sink_tokens % TK != 0);
+    skip_t = max(0, first_key / TK - sink_t);
+    auto number = [&](int t) { return t < sink_t ? t : max(sink_t, t - skip_t); };
+    if (tb < te) {
+      t_begin = number(real_page(tb) * UPP);
+      t_end = number(min(real_page(te - 1) * UPP + UPP, (end_key + TK - 1) / TK));
+    }
   }
   const int n_active_warps = QUAD ? 4 : (nrows + 31) / 32;
 
@@ -253,10 +265,7 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
       }
       if (lane == 0) *s_ntiles = min(n, MAX_SPARSE_TILES * UPP);
     } else if (WIN) {
-      // (lengths on the device may outgrow the rows of the tile: the last pages may then be nobody's)
-      int last = te;
-      while (last > tb && real_page(last - 1) * BN >= end_key) --last;
-      if (lane == 0) *s_ntiles = max(0, last - tb);
+      if (lane == 0) *s_ntiles = max(0, t_end - t_begin);
     } else if (lane == 0) {
       // [tb, te) pages of the sequence, up to the last tile that holds a key
       const int keys = min(te * BN, kv_len) - tb * BN;
@@ -274,7 +283,7 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
   const int n_tiles = *s_ntiles;
   if (trace) trace[3] = clock64() - clk0;
   auto tile_key0 = [&](int j) -> int {                       // position of the first key of tile j
-    if constexpr (WIN) return real_page(tb + j) * BN;
+    if constexpr (WIN) return (t_begin + j < sink_t ? t_begin + j : t_begin + j + skip_t) * TK;
     return (sparse ? s_tiles[j] : tb * UPP + j) * TK;
   };
   // windowed: whether the tile from key0 on holds a key that no row sees.  Those are in three tiles at most: the last of the sinks, the first
@@ -309,9 +318,10 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
     // page-table entries: one per lane, 32 pages at a time, the next batch already in flight
     int phys_cur = 0, phys_next = 0;
     const int n_pages = (n_tiles + UPP - 1) / UPP;
+    [[maybe_unused]] int entry0 = tb;                          // windowed: page (numbered as the item's tiles) that lane 0 has in phys_cur
     if constexpr (WIN) {
-      phys_cur = lane < n_pages ? page_entry(p, page_base + real_page(tb + lane)) : 0;
-      phys_next = 32 + lane < n_pages ? page_entry(p, page_base + real_page(tb + 32 + lane)) : 0;
+      phys_cur = tb + lane < te ? page_entry(p, page_base + real_page(tb + lane)) : 0;
+      phys_next = tb + 32 + lane < te ? page_entry(p, page_base + real_page(tb + 32 + lane)) : 0;
     } else if (!sparse) {
       phys_cur = lane < n_pages ? page_entry(p, page_base + tb + lane) : 0;
       phys_next = 32 + lane < n_pages ? page_entry(p, page_base + tb + 32 + lane) : 0;
@@ -323,11 +333,19 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
       const int st = j % STAGES;
       const int key0 = tile_key0(j);
       const int row_in_page = key0 % BN;
-      const int pg = j / UPP;                                // dense: page index within this item
-      if (!sparse && j > 0 && (j % (32 * UPP)) == 0) {
+      int pg = j / UPP;                                      // dense: page index within this item
+      if constexpr (WIN) {
+        pg = key0 / BN;
+        if (pg >= sink_tiles(p.sink_tokens)) pg -= skip;
+        pg -= entry0;
+        if (pg >= 32) {                                      // (tiles come in order: the next batch begins here)
+          phys_cur = phys_next;
+          entry0 += 32; pg -= 32;
+          phys_next = entry0 + 32 + lane < te ? page_entry(p, page_base + real_page(entry0 + 32 + lane)) : 0;
+        }
+      } else if (!sparse && j > 0 && (j % (32 * UPP)) == 0) {
         phys_cur = phys_next;
-        if constexpr (WIN) phys_next = pg + 32 + lane < n_pages ? page_entry(p, page_base + real_page(tb + pg + 32 + lane)) : 0;
-        else phys_next = pg + 32 + lane < n_pages ? page_entry(p, page_base + tb + pg + 32 + lane) : 0;
+        phys_next = pg + 32 + lane < n_pages ? page_entry(p, page_base + tb + pg + 32 + lane) : 0;
       }
       const int phys = sparse ? s_phys[j] : __shfl_sync(0xffffffffu, phys_cur, pg & 31);
       const int valid_rows = min(TK, kv_len - key0);
@@ -339,7 +357,7 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
           mbar_arrive_expect_tx(bar(K_FULL + st), TILE_BYTES);
 #pragma unroll
           for (int hlf = 0; hlf < NSUB; ++hlf)
-            tma_load_4d(smem_base + OFF_K + st * TILE_BYTES + hlf * SUB_BYTES, &tm_k, bar(K_FULL + st), hlf * SUB_ELEMS,
+            tma_load_4d(smem_base + OFF_K + st * TILE_BYTES + hlf * KV_SUB, &tm_k, bar(K_FULL + st), hlf * SUB_ELEMS,
                         row_in_page, kvh, phys);
         }
         __syncwarp();
@@ -352,7 +370,7 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
         mbar_arrive_expect_tx(vbar, TILE_BYTES);
 #pragma unroll
         for (int hlf = 0; hlf < NSUB; ++hlf)
-          tma_load_4d(smem_base + OFF_V + st * TILE_BYTES + hlf * SUB_BYTES, &tm_v, vbar, hlf * SUB_ELEMS, row_in_page, kvh, phys);
+          tma_load_4d(smem_base + OFF_V + st * TILE_BYTES + hlf * KV_SUB, &tm_v, vbar, hlf * SUB_ELEMS, row_in_page, kvh, phys);
       }
       __syncwarp();
       if constexpr (WIN) { fixes += fix; continue; }         // the other warp's
@@ -363,7 +381,7 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
           unsigned char* vt = smem_gen + OFF_V + st * TILE_BYTES;
           for (int c = lane; c < (TK - valid_rows) * 8 * NSUB; c += 32) {
             const int r = valid_rows + c / (8 * NSUB), ch = c % (8 * NSUB);
-            *reinterpret_cast<uint4*>(vt + (ch >> 3) * SUB_BYTES + r * 128 + (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4*>(vt + (ch >> 3) * KV_SUB + r * 128 + (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
           }
           fence_proxy_async_smem();
           __syncwarp();
@@ -385,7 +403,7 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
         for (int c = lane; c < TK * 8 * NSUB; c += 32) {
           const int r = c / (8 * NSUB), ch = c % (8 * NSUB), key = key0 + r;
           if (key >= end_key || (key < first_key && key >= p.sink_tokens))
-            *reinterpret_cast<uint4*>(vt + (ch >> 3) * SUB_BYTES + r * 128 + (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4*>(vt + (ch >> 3) * KV_SUB + r * 128 + (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
         }
         fence_proxy_async_smem();
         __syncwarp();
@@ -397,7 +415,7 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
     constexpr uint32_t IDESC_QK = F8 ? idesc_e4m3(BM, TK, false, false) : idesc_bf16(BM, TK, false, false);
     constexpr uint32_t IDESC_PV = F8 ? idesc_e4m3(BM, kHeadDim, false, true) : idesc_bf16(BM, kHeadDim, false, true);
     const uint64_t dk_hi = smem_desc(0, 16, 1024) & 0xFFFFFFFFFFFF0000ull;
-    const uint64_t dv_hi = smem_desc(0, SUB_BYTES, 1024) & 0xFFFFFFFFFFFF0000ull;
+    const uint64_t dv_hi = smem_desc(0, KV_SUB, 1024) & 0xFFFFFFFFFFFF0000ull;
     constexpr int KEYS_PER_PV = F8 ? 32 : 16;        // keys one P.V MMA contracts over
     constexpr int PV_STEPS = TK / KEYS_PER_PV;
     constexpr int V_KSTEP = KEYS_PER_PV * 128;       // bytes between the key slices of consecutive P.V MMAs
@@ -406,9 +424,10 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
       const uint32_t qa = (smem_base + OFF_Q) >> 4, ka = (smem_base + OFF_K + (j % STAGES) * TILE_BYTES) >> 4;
 #pragma unroll
       for (int k = 0; k < KSTEPS; ++k) {
-        const uint32_t o = ((k >> 2) * SUB_BYTES + (k & 3) * 32) >> 4;      // 32 bytes of head_dim per MMA
-        if constexpr (F8) mma_ss_f8(sbuf(j), dk_hi | ((qa + o) & 0x3FFF), dk_hi | ((ka + o) & 0x3FFF), IDESC_QK, k > 0);
-        else mma_ss(sbuf(j), dk_hi | ((qa + o) & 0x3FFF), dk_hi | ((ka + o) & 0x3FFF), IDESC_QK, k > 0);
+        const uint32_t oq = ((k >> 2) * SUB_BYTES + (k & 3) * 32) >> 4;     // 32 bytes of head_dim per MMA
+        const uint32_t ok = ((k >> 2) * KV_SUB + (k & 3) * 32) >> 4;
+        if constexpr (F8) mma_ss_f8(sbuf(j), dk_hi | ((qa + oq) & 0x3FFF), dk_hi | ((ka + ok) & 0x3FFF), IDESC_QK, k > 0);
+        else mma_ss(sbuf(j), dk_hi | ((qa + oq) & 0x3FFF), dk_hi | ((ka + ok) & 0x3FFF), IDESC_QK, k > 0);
       }
       if constexpr (PAIR) {
         if (p.q_dtype == MSA_DT_BF16) {
@@ -670,23 +689,22 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
       if (!alive) break;
       tc_fence_after();
       const int pos0 = tile_key0(j);
-      uint32_t sv[4][32];
-      tmem_ld32(tS, sv[0]);
-      tmem_ld32(tS + 32, sv[1]);
-      tmem_ld32(tS + 64, sv[2]);
-      tmem_ld32(tS + 96, sv[3]);
-      tmem_wait_ld();
-      if (pos0 + BN - 1 > lim) {
+      constexpr int NC = TK / 32;
+      uint32_t sv[NC][32];
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
+      for (int c = 0; c < NC; ++c) tmem_ld32(tS + 32 * c, sv[c]);
+      tmem_wait_ld();
+      if (pos0 + TK - 1 > lim) {
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
 #pragma unroll
           for (int e = 0; e < 32; ++e)
             if (pos0 + c * 32 + e > lim) sv[c][e] = 0xff800000u;
       }
       if constexpr (WIN) {
-        if (pos0 < from && pos0 + BN > p.sink_tokens) {
+        if (pos0 < from && pos0 + TK > p.sink_tokens) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
+          for (int c = 0; c < NC; ++c)
 #pragma unroll
             for (int e = 0; e < 32; ++e)
               if (pos0 + c * 32 + e < from && pos0 + c * 32 + e >= p.sink_tokens) sv[c][e] = 0xff800000u;
@@ -694,7 +712,7 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
       }
       float mxs[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int c = 0; c < 4; ++c)
+      for (int c = 0; c < NC; ++c)
 #pragma unroll
         for (int e = 0; e < 32; e += 2)
           mxs[(e >> 1) & 3] = max3(mxs[(e >> 1) & 3], __uint_as_float(sv[c][e]), __uint_as_float(sv[c][e + 1]));
@@ -734,7 +752,7 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
       const float msafe = ((m_used == -INFINITY) ? 0.f : m_used) - kPOffset;
       float l0 = 0.f, l1 = 0.f;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
+      for (int c = 0; c < NC; ++c) {
         if constexpr (F8) {
           uint32_t pk[8];                                   // four e4m3 per TMEM column
           [[maybe_unused]] uint32_t pl[8];
@@ -965,7 +983,7 @@ int fmha_decode_tc_launch(const MsaFmhaParams& p, cudaStream_t stream) {
                             static_cast<uint64_t>(p.v_stride_page) * e};
     const void* vptr = has_o ? p.v : p.k;
     if (f8) {
-      const uint32_t kbox[4] = {128, static_cast<uint32_t>(quad ? Cfg<true, true>::TK : BN), 1, 1};   // dual: half pages
+      const uint32_t kbox[4] = {128, static_cast<uint32_t>(quad ? Cfg<true, true>::TK : p.window > 0 ? Cfg<true, false, true>::TK : BN), 1, 1};   // dual: half pages
       if (make_tma_map_u8(&tk, p.k, 4, kd, ks, kbox) != MSA_OK ||
           make_tma_map_u8(&tv, vptr, 4, kd, has_o ? vs : ks, kbox) != MSA_OK)
         return MSA_ERR_LAUNCH;
@@ -975,7 +993,7 @@ int fmha_decode_tc_launch(const MsaFmhaParams& p, cudaStream_t stream) {
       const uint64_t str[2] = {static_cast<uint64_t>(p.q_stride_head) * 2, static_cast<uint64_t>(p.q_stride_tok) * 2};
       const uint32_t box[3] = {64, static_cast<uint32_t>(p.pack), 1};
       if (make_tma_map_bf16(&tq, p.q, 3, dims, str, box) != MSA_OK) return MSA_ERR_LAUNCH;
-      const uint32_t kbox[4] = {64, BN, 1, 1};
+      const uint32_t kbox[4] = {64, static_cast<uint32_t>(p.window > 0 ? Cfg<false, false, true>::TK : BN), 1, 1};
       if (make_tma_map_bf16(&tk, p.k, 4, kd, ks, kbox) != MSA_OK ||
           make_tma_map_bf16(&tv, vptr, 4, kd, has_o ? vs : ks, kbox) != MSA_OK)
         return MSA_ERR_LAUNCH;
@@ -999,7 +1017,7 @@ int fmha_decode_tc_launch(const MsaFmhaParams& p, cudaStream_t stream) {
   if (dev >= 16 || !attr_done[dev][variant]) {
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
       return MSA_ERR_LAUNCH;
-    if (variant == 3)      // two co-resident CTAs need the whole shared-memory carve-out
+    if (variant >= 3)      // two co-resident CTAs need the whole shared-memory carve-out
       cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
     if (dev < 16) attr_done[dev][variant] = true;
   }

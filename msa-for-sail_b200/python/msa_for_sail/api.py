@@ -467,9 +467,8 @@ def _fmha_sail_plan(
                 info["num_work_tc"] = n_tc
         # Two CTAs of the e4m3 decode kernel share an SM.  A cut at the average load may take more partials than a workspace
         # sized for the plain cut holds: such a workspace gets the plain cut.
-        # (windowed rows that the streaming kernel takes: two as well)
-        few = max_qo * pack <= (32 if window[0] and not use_fp8_kvcache else 16)
-        shared = 1 if not few else (_kv4_ctas(max_qo * pack) if use_kv4_cache else (2 if use_fp8_kvcache or window[0] else 1))
+        # With a window two CTAs share an SM whatever the rows.
+        shared = 2 if window[0] else 1 if max_qo * pack > 16 else (_kv4_ctas(max_qo * pack) if use_kv4_cache else (2 if use_fp8_kvcache else 1))
         for ctas in (shared, -1):
             args = _lib.MsaPlanArgs(
                 a_q.ctypes.data, a_k.ctypes.data, a_o.ctypes.data, batch, num_qo_heads, hkv, block_m, pack,
