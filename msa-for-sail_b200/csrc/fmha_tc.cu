@@ -639,7 +639,7 @@ fmha_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant__ 
       const int nx = x == 0 ? w.n_tiles[0] : w.n_tiles[1];
       const float scale_log2 = p.sm_scale * kLog2e * (p.k_scale_head ? p.k_scale_head[kvh] : 1.f);
       float m_used = -INFINITY, l_sum = 0.f;
-      float l_exact = 0.f;                                 // e4m3 only: sum of the unrounded probabilities, for the LSE
+      float l_exact = 0.f;                                 // e4m3 without pairs: sum of the unrounded probabilities, for the LSE
 
       for (int j = 0; j < nx && alive; ++j) {
         if (WIN && !has_tile(w, x, j)) continue;
@@ -670,7 +670,7 @@ fmha_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant__ 
             const float m_cand = fmaxf(m_used, top * scale_log2);
             const bool bump = (m_cand - m_used) > kRescaleThreshold;
             float factor = 1.f;
-            if (bump) { factor = exp2_fast(m_used - m_cand); m_used = m_cand; l_sum *= factor; l_exact *= factor; }
+            if (bump) { factor = exp2_fast(m_used - m_cand); m_used = m_cand; l_sum *= factor; }
             if (later && __any_sync(0xffffffffu, bump)) {
 #pragma unroll
               for (int c = 0; c < 4; ++c) {
@@ -703,7 +703,6 @@ fmha_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant__ 
             if constexpr (F8) { tmem_st8(tS, pk); tmem_st8(tS + BN / 4, pl); }
             else tmem_st16(tS, pk);
             l_sum += l0 + l1;
-            l_exact += l0 + l1;
             tmem_wait_st();
             tc_fence_before();
             mbar_arrive(bar(P_FULL + x));
@@ -712,6 +711,90 @@ fmha_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant__ 
         }
         const int pos0 = (WIN ? real_tile(w, j) : j) * BN;
         const bool need_mask = (pos0 + BN - 1 > m0 + off) || (pos0 + BN > kv_len) || (WIN && pos0 < from_last && pos0 + BN > p.sink_tokens);
+        // with a window, one bit for each of 32 keys that the row sees: a test and a select an element, where three comparisons would be needed
+        [[maybe_unused]] auto mask32 = [&](uint32_t (&s)[32], int k0) {
+          auto below = [](int n) -> uint32_t { return n <= 0 ? 0u : 0xffffffffu >> (32 - min(n, 32)); };     // the first n bits
+          const uint32_t seen = below(lim + 1 - k0) & (~below(from - k0) | below(p.sink_tokens - k0));
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (!(seen & (1u << e))) s[e] = 0xff800000u;             // -inf
+        };
+        if constexpr (PAIR) {
+          // Half of the row at a time, the second half read twice: with all 128 scores in registers next to the pairs, registers ran out (spills
+          // in every tile).  P: hi in columns 0-31, lo in 32-63, all of them in the half that has been read.
+          auto read = [&](int h, uint32_t (&s)[2][32]) {
+            tmem_ld32(tS + 64 * h, s[0]);
+            tmem_ld32(tS + 64 * h + 32, s[1]);
+            tmem_wait_ld();
+            if (need_mask) { mask32(s[0], pos0 + 64 * h); mask32(s[1], pos0 + 64 * h + 32); }
+          };
+          auto top_of = [&](const uint32_t (&s)[2][32]) -> float {
+            float t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+              for (int e = 0; e < 32; e += 2) t[(e >> 1) & 3] = max3(t[(e >> 1) & 3], __uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1]));
+            return fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+          };
+          uint32_t sv[2][32];
+          read(1, sv);
+          float top = top_of(sv);
+          read(0, sv);
+          top = fmaxf(top, top_of(sv));
+          if (r == 0) trace(x, j, 2);
+          const float m_cand = fmaxf(m_used, top * scale_log2);
+          const bool bump = (m_cand - m_used) > kRescaleThreshold;
+          float factor = 1.f;
+          if (bump) { factor = exp2_fast(m_used - m_cand); m_used = m_cand; l_sum *= factor; }
+          if (later && __any_sync(0xffffffffu, bump)) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              uint32_t v[32];
+              tmem_ld32(tO + c * 32, v);
+              tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * factor);
+              tmem_st32(tO + c * 32, v);
+            }
+          }
+          if (r == 0) trace(x, j, 3);
+          const float m_ref = ((m_used == -INFINITY) ? 0.f : m_used) - kPOffset;
+          const uint64_t scale2 = f2_pack(scale_log2, scale_log2), negm2 = f2_pack(-m_ref, -m_ref);
+          uint64_t sum2 = f2_pack(0.f, 0.f);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if (h) read(1, sv);
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              uint32_t pk[8], pl[8];
+#pragma unroll
+              for (int e = 0; e < 32; e += 4) {
+                uint32_t hi[2], lo[2];
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                  float x0, x1;
+                  f2_unpack(f2_fma(f2_pack(__uint_as_float(sv[c][e + 2 * q]), __uint_as_float(sv[c][e + 2 * q + 1])), scale2, negm2), x0, x1);
+                  const float p0 = exp2_fast(x0), p1 = exp2_fast(x1);
+                  sum2 = f2_add(sum2, f2_pack(p0, p1));
+                  e4m3_pair(p0, p1, hi[q], lo[q]);
+                }
+                pk[e >> 2] = hi[0] | (hi[1] << 16);
+                pl[e >> 2] = lo[0] | (lo[1] << 16);
+              }
+              tmem_st8(tS + 16 * h + 8 * c, pk);
+              tmem_st8(tS + BN / 4 + 16 * h + 8 * c, pl);
+            }
+          }
+          float l0, l1;
+          f2_unpack(sum2, l0, l1);
+          l_sum += l0 + l1;
+          if (r == 0) trace(x, j, 4);
+          tmem_wait_st();
+          tc_fence_before();
+          mbar_arrive(bar(P_FULL + x));
+          if (r == 0) trace(x, j, 5);
+          continue;
+        }
         // ---- one read of the whole S row (128 fp32) ----
         uint32_t sv[4][32];
         tmem_ld32(tS, sv[0]);
@@ -725,16 +808,8 @@ fmha_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant__ 
           mbar_arrive(bar(P_FULL + x));
         }
         if (WIN && need_mask) {
-          // one bit for each key that the row sees: a test and a select an element, where three comparisons would be needed
-          auto below = [](int n) -> uint32_t { return n <= 0 ? 0u : 0xffffffffu >> (32 - min(n, 32)); };     // the first n bits
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const int k0 = pos0 + c * 32;
-            const uint32_t seen = below(lim + 1 - k0) & (~below(from - k0) | below(p.sink_tokens - k0));
-#pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (!(seen & (1u << e))) sv[c][e] = 0xff800000u;         // -inf
-          }
+          for (int c = 0; c < 4; ++c) mask32(sv[c], pos0 + c * 32);
         } else if (need_mask) {
 #pragma unroll
           for (int c = 0; c < 4; ++c)
@@ -781,15 +856,14 @@ fmha_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant__ 
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             uint32_t pk[F8 ? 8 : 16];
-            [[maybe_unused]] uint32_t pl[PAIR ? 8 : 1];
-            [[maybe_unused]] uint32_t held = 0, held_lo = 0;
+            [[maybe_unused]] uint16_t held = 0;
 #pragma unroll
             for (int e = 0; e < 32; e += 2) {
               if constexpr (decltype(with_max)::value)
                 mxs[(e >> 1) & 3] = max3(mxs[(e >> 1) & 3], __uint_as_float(sv[c][e]), __uint_as_float(sv[c][e + 1]));
               const uint64_t x2 = f2_fma(f2_pack(__uint_as_float(sv[c][e]), __uint_as_float(sv[c][e + 1])), scale2, negm2);
               float p0, p1;
-              if (!PAIR && ((kEmuMask >> ((e >> 1) & 15)) & 1)) {
+              if ((kEmuMask >> ((e >> 1) & 15)) & 1) {
                 float x0, x1;
                 f2_unpack(x2, x0, x1);
                 const uint64_t xc = f2_pack(fmaxf(x0, -126.f), fmaxf(x1, -126.f));     // also maps -inf
@@ -814,22 +888,11 @@ fmha_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant__ 
                 // O is normalised by the sum of the probabilities as the MMA sees them (see the decode kernel);
                 // the LSE reports the sum before rounding
                 lex2 = f2_add(lex2, f2_pack(p0, p1));
-                if constexpr (PAIR) {
-                  uint32_t hi, lo;
-                  e4m3_pair(p0, p1, hi, lo);
-                  if (e & 2) {
-                    pk[e >> 2] = held | (hi << 16);
-                    pl[e >> 2] = held_lo | (lo << 16);
-                  } else {
-                    held = hi; held_lo = lo;
-                  }
-                } else {
-                  const uint16_t pr = __nv_cvt_float2_to_fp8x2(make_float2(p0, p1), __NV_SATFINITE, __NV_E4M3);
-                  const float2 rr = e4m3x2_to_float2(pr);
-                  lsum2 = f2_add(lsum2, f2_pack(rr.x, rr.y));
-                  if (e & 2) pk[e >> 2] = static_cast<uint32_t>(held) | (static_cast<uint32_t>(pr) << 16);
-                  else held = pr;
-                }
+                const uint16_t pr = __nv_cvt_float2_to_fp8x2(make_float2(p0, p1), __NV_SATFINITE, __NV_E4M3);
+                const float2 rr = e4m3x2_to_float2(pr);
+                lsum2 = f2_add(lsum2, f2_pack(rr.x, rr.y));
+                if (e & 2) pk[e >> 2] = static_cast<uint32_t>(held) | (static_cast<uint32_t>(pr) << 16);
+                else held = pr;
               } else {
                 lsum2 = f2_add(lsum2, f2_pack(p0, p1));
                 pk[e >> 1] = pack2<false>(p0, p1);
@@ -837,13 +900,11 @@ fmha_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant__ 
             }
             if constexpr (F8) tmem_st8(tS + c * 8, pk);
             else tmem_st16(tS + c * 16, pk);
-            if constexpr (PAIR) tmem_st8(tS + BN / 4 + c * 8, pl);
           }
           float l0, l1;
           f2_unpack(lsum2, l0, l1);
           l_rnd = l0 + l1;
           if constexpr (F8) { f2_unpack(lex2, l0, l1); l_raw = l0 + l1; }
-          if constexpr (PAIR) l_rnd = l_raw;
         };
         // Every tile but the first writes P with the running max while it finds its own max: the max does
         // not sit between the S read and the exponentials, and the guess holds unless the row's max grows
@@ -923,7 +984,7 @@ fmha_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant__ 
         }
         if (row_ok && p.lse)
           p.lse[static_cast<int64_t>(gtok) * p.num_qo_heads + head] =
-              l_sum > 0.f ? (m_used - kPOffset) * kLn2 + __logf(F8 ? l_exact : l_sum) : -INFINITY;
+              l_sum > 0.f ? (m_used - kPOffset) * kLn2 + __logf(F8 && !PAIR ? l_exact : l_sum) : -INFINITY;
       }
     }
   }
