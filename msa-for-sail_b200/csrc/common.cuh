@@ -65,6 +65,8 @@ __device__ __forceinline__ int window_first(int place, int kv_len, int window) {
   const long long lo = static_cast<long long>(place) - window + 1;
   return lo < 0 ? 0 : lo < kv_len ? static_cast<int>(lo) : kv_len;
 }
+// Factor of the scores where masked ones are -inf: -inf * 0 is no number, the smallest one changes no score by as much as its last bit.
+__device__ __forceinline__ float masked_scale(float scale) { return scale == 0.f ? 1.17549435e-38f : scale; }
 
 // ---- kernels of one stream without a gap between them ----
 // A kernel launched with launch_chained() may start while the kernel before it in the stream still runs: once every CTA of

@@ -585,6 +585,7 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
         mbar_arrive(bar(Q_FULL));
       }
     }
+    if constexpr (WIN) scale_log2 = masked_scale(scale_log2);
 
     if constexpr (QUAD) {
       // quadrant `warp` owns key columns [32 warp, 32 warp + 32) of every tile

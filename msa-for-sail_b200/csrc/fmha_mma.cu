@@ -107,6 +107,7 @@ fmha_mma_kernel(const __grid_constant__ MsaFmhaParams p) {
 
   float scale_log2 = p.sm_scale * kLog2e;
   if (p.k_scale_head) scale_log2 *= p.k_scale_head[kvh];
+  if constexpr (WIN) scale_log2 = masked_scale(scale_log2);
 
   // ---------------- Q tile -> shared (compute type) ----------------
   {

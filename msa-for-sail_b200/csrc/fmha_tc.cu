@@ -637,7 +637,8 @@ fmha_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant__ 
       }
       [[maybe_unused]] bool begun = false;
       const int nx = x == 0 ? w.n_tiles[0] : w.n_tiles[1];
-      const float scale_log2 = p.sm_scale * kLog2e * (p.k_scale_head ? p.k_scale_head[kvh] : 1.f);
+      const float scale_all = p.sm_scale * kLog2e * (p.k_scale_head ? p.k_scale_head[kvh] : 1.f);
+      const float scale_log2 = WIN ? masked_scale(scale_all) : scale_all;
       float m_used = -INFINITY, l_sum = 0.f;
       float l_exact = 0.f;                                 // e4m3 without pairs: sum of the unrounded probabilities, for the LSE
 

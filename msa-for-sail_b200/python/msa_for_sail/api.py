@@ -1056,25 +1056,25 @@ def _fmha_sail(
 _WINDOW_TYPES = (torch.bfloat16, torch.float8_e4m3fn)
 _WINDOW_OUT = (torch.bfloat16, torch.float32)
 _WINDOW_HEAD = struct.Struct("@7Q")           # the arguments' first fields: q, k, v, out, lse, max_score, partial_o
+_WINDOW_TABLES = struct.Struct("@6Q")         # qo_start, kv_start, kv_len, qo_offset, kv_page_indptr, kv_indices
 _WINDOW_STRIDES = struct.Struct("@10q")       # q, k, v, out
 
 
 def _window_params(q_dtype, kv_dtype, plan):
-    """What is the same in every call with this plan and these types: the arguments' bytes (the kernel, its work list, the plan's metadata), the
-    number of splits, and where their number per row is."""
+    """What is the same in every call with this plan and these types: the arguments' bytes (the plan's numbers and the choice of a kernel, no
+    addresses), the number of splits, and the name of the work list."""
     page_size, splits, pack = max(0, plan["page_size"]), plan["num_kv_splits"], plan["pack_factor"]
     h_r = plan["orig_num_qo_heads"] // plan["num_kv_heads"]
-    p = _lib.MsaFmhaParams(qo_start=plan["qo_segment_offsets"].data_ptr(), kv_start=plan["kv_segment_offsets"].data_ptr(),
-                           kv_len=plan["kv_segment_lens"].data_ptr(), qo_offset=plan["qo_offset"].data_ptr(), kv_page_indptr=_ptr(plan["kv_page_indptr"]),
-                           work=_ptr(plan["work"]), num_work=plan["num_work"], block_m=plan["qo_tile_size"], pack=pack, page_size=page_size,
-                           num_splits=splits, num_qo_heads=plan["orig_num_qo_heads"], num_kv_heads=plan["num_kv_heads"], batch=plan["batch_size"],
+    p = _lib.MsaFmhaParams(num_work=plan["num_work"], block_m=plan["qo_tile_size"], pack=pack, page_size=page_size, num_splits=splits,
+                           num_qo_heads=plan["orig_num_qo_heads"], num_kv_heads=plan["num_kv_heads"], batch=plan["batch_size"],
                            q_dtype=_dt_code(q_dtype), kv_dtype=_dt_code(kv_dtype), flags=FLAG_OUT_O, window=plan["window"][0], sink_tokens=plan["window"][1])
+    work = "work"
     if plan.get("work_tc") is not None and q_dtype == kv_dtype and page_size in (0, 128) and _USE_TC and (plan["tc_preferred"] or _FORCE_TC):
-        p.work, p.num_work, p.block_m, p.num_splits = plan["work_tc"].data_ptr(), plan["num_work_tc"], 256, 1
+        work, p.num_work, p.block_m, p.num_splits = "work_tc", plan["num_work_tc"], 256, 1
     elif _USE_DECODE_TC and 0 < plan["max_qo_len"] * pack <= 128 and pack == h_r:
         # few rows: the streaming kernel, on any pages of whole units; else the tcgen05 decode kernel, on pages of 128 keys
         p.decode_rows = plan["max_qo_len"] * pack
-    return bytes(p), p.num_splits, _ptr(plan["num_kv_splits_per_row"])
+    return bytes(p), p.num_splits, work
 
 
 def _fmha_sail_window(q, k, v, plan, kv_indices, kv_block_indexes, q_offset_override, out, max_score, sm_scale, q_scale, k_scale, v_scale, o_scale,
@@ -1142,15 +1142,18 @@ def _fmha_sail_window(q, k, v, plan, kv_indices, kv_block_indexes, q_offset_over
     base = kept.get(key)
     if base is None:
         base = kept[key] = _window_params(q_dtype, k_dtype, plan)
-    p, splits = _lib.MsaFmhaParams.from_buffer_copy(base[0]), base[1]
+    p, splits, work = _lib.MsaFmhaParams.from_buffer_copy(base[0]), base[1], plan[base[2]]
     sm_scale = 0.08838834764831845 if sm_scale is None else float(sm_scale)     # 1 / sqrt(128)
     k_s, out_scale = 1.0, 1.0
     if q_scale is not None or k_scale is not None or v_scale is not None or o_scale is not None:
         (k_s, k_head), (out_scale, v_head) = _scale_pair(q_scale, k_scale, dev, num_kv_heads), _scale_pair(o_scale, v_scale, dev, num_kv_heads)
         p.k_scale_head, p.v_scale_head = _ptr(k_head), _ptr(v_head)
+    scale = k_s * sm_scale
+    if not 0 <= scale < math.inf:
+        raise ValueError(f"with window_size the factor of the scores must be a number from 0 on, got {scale}")
     if paged:
         tok, head = (1, 2) if nhd else (2, 1)
-        p.kv_indices, p.num_page_entries = kv_indices.data_ptr(), kv_indices.shape[0]
+        p.num_page_entries = kv_indices.shape[0]
         strides = (q_stride[0], q_stride[1], k_stride[0], k_stride[head], k_stride[tok], v_stride[0], v_stride[head], v_stride[tok])
     else:
         strides = (q_stride[0], q_stride[1], 0, k_stride[1], k_stride[0], 0, v_stride[1], v_stride[0])
@@ -1168,11 +1171,15 @@ def _fmha_sail_window(q, k, v, plan, kv_indices, kv_block_indexes, q_offset_over
         if o_stride is None:
             o_stride = (num_qo_heads * 128, 128)
         _WINDOW_HEAD.pack_into(p, 0, q.data_ptr(), k.data_ptr(), v.data_ptr(), kernel_out.data_ptr(), 0 if lse is None else lse.data_ptr(), 0, part)
+        _WINDOW_TABLES.pack_into(p, _lib.MsaFmhaParams.qo_start.offset, plan["qo_segment_offsets"].data_ptr(), plan["kv_segment_offsets"].data_ptr(),
+                                 plan["kv_segment_lens"].data_ptr(), plan["qo_offset"].data_ptr(), plan["kv_page_indptr"].data_ptr() if paged else 0,
+                                 kv_indices.data_ptr() if paged else 0)
         _WINDOW_STRIDES.pack_into(p, _lib.MsaFmhaParams.q_stride_tok.offset, *strides, o_stride[0], o_stride[1])
         p.total_q, p.kv_extent, p.status = nnz_qo, k_shape[0], _status_ptr(dev)
-        p.sm_scale, p.out_scale = k_s * sm_scale, out_scale
+        p.work = None if work is None else work.data_ptr()
+        p.sm_scale, p.out_scale = scale, out_scale
         if splits > 1:
-            _lib.check(_lib.lib.msa_fmha_fwd_merged(ctypes.byref(p), base[2], _dt_code(out_dtype), _stream()), "msa_fmha_fwd_merged")
+            _lib.check(_lib.lib.msa_fmha_fwd_merged(ctypes.byref(p), _ptr(plan["num_kv_splits_per_row"]), _dt_code(out_dtype), _stream()), "msa_fmha_fwd_merged")
         else:
             _lib.check(_lib.lib.msa_fmha_fwd(ctypes.byref(p), _stream()), "msa_fmha_fwd")
             if kernel_out is not out:

@@ -215,8 +215,8 @@ def test_a_captured_step_sees_new_lengths(max_q):
     ws = msa.allocate_graph_workspace(3, 8, 2, max_qo_len=max_q, page_size=128, num_kv_splits=2)
     out = torch.zeros(T, 8, 128, dtype=torch.bfloat16, device=DEV)
     table = torch.zeros(64, dtype=torch.int32, device=DEV)
-    kc, vc, q = (torch.zeros(64, 2, 128, 128, dtype=torch.bfloat16, device=DEV) for _ in range(2)), None, torch.zeros_like(c.q)
-    kc, vc = kc
+    kc, vc = (torch.zeros(64, 2, 128, 128, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    q = torch.zeros_like(c.q)
 
     def step():
         plan = msa.fmha_sail_plan(ql, kl, 8, num_kv_heads=2, page_size=128, window_size=300, num_sink_tokens=4, num_kv_splits=2, graph_safe=True,
