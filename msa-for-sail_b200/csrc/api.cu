@@ -127,7 +127,7 @@ static int makespan(const std::vector<Proto>& protos, int groups, int chunk, int
 // times of a CTA that nothing holds up (1.6 us in bf16, 16 rows): a piece costs three beyond its own, a merge two, memory gives each SM a
 // tile in 0.9 (as if all were bf16), and of the two bounds a part of the smaller one shows as well.  Measured with 1 to 12 splits, merge
 // included: 24 ragged sequences x 4 heads, at most 34 tiles: 60 us uncut, 40, 38 (three), 43, 41 (seven), 47; 128 items of 10 tiles, 64
-// rows: 26, 34, 37 us; 512 of 66: 316, 326, 331 us; 512 of 18 e4m3 tiles: 61, 69, 73 us; one sequence of 10 tiles x 2 heads: 15.7, 11.7, 11.0, 8.3 us
+// rows: 23, 24, 26 us; 512 of 66: 316, 326, 331 us; 512 of 18 e4m3 tiles: 61, 69, 73 us; one sequence of 10 tiles x 2 heads: 15.7, 11.7, 11.0, 8.3 us
 // (five and ten).
 static int window_chunk(const std::vector<Proto>& protos, int groups, int max_tiles, int slots, int sms, int ceiling) {
   constexpr int kPieceCost = 3, kMerge = 2;

@@ -117,14 +117,20 @@ struct Cfg {
   static constexpr int O_COL = NBUF * TK;
   static constexpr int MIN_CTAS = DUAL ? 2 : 1;
   static_assert(STAGES <= MAX_STAGES, "barrier table");
+  static_assert(!WIN || BM * kHeadDim * 4 <= 2 * RING_BYTES, "O staging fits the rings");
   static_assert(!QUAD || 4 * QUAD_MAX_ROWS * STAGE_LD * 4 <= RING_BYTES, "O staging fits the K ring");
 };
 
-template <bool F8, bool QUAD, bool WIN>
-__global__ void __launch_bounds__(NTHREADS, (Cfg<F8, QUAD, WIN>::MIN_CTAS))
+// PARTS  windowed items: times that the rows are in the MMA tile.  Their warps take 64 / PARTS key columns of each tile, with a softmax of their own
+//        (their P is zero elsewhere), so that all four warps work on up to 64 rows; the parts are joined in shared memory.  32 e4m3 sequences x 64
+//        rows, a warp taking all 64 columns: 27.7 us, two parts 22.6.  0: no window.
+template <bool F8, bool QUAD, int PARTS>
+__global__ void __launch_bounds__(NTHREADS, (Cfg<F8, QUAD, (PARTS > 0)>::MIN_CTAS))
 decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant__ CUtensorMap tm_q,
                  const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v) {
+  constexpr bool WIN = PARTS > 0;
   using C = Cfg<F8, QUAD, WIN>;
+  constexpr int ROWS = WIN ? BM / PARTS : BM;       // of one part
   constexpr int NSUB = C::NSUB, KV_SUB = C::KV_SUB, TILE_BYTES = C::TILE_BYTES, STAGES = C::STAGES, NBUF = C::NBUF, TK = C::TK;
   constexpr bool PAIR = C::PAIR;
   constexpr int UPP = BN / TK;                      // tiles per page
@@ -216,7 +222,7 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
       t_end = number(min(real_page(te - 1) * UPP + UPP, (end_key + TK - 1) / TK));
     }
   }
-  const int n_active_warps = QUAD ? 4 : (nrows + 31) / 32;
+  const int n_active_warps = QUAD ? 4 : WIN ? PARTS * ((nrows + 31) / 32) : (nrows + 31) / 32;
 
   // a timeout reported earlier on this device (status word not cleared yet): do not start.  Read by
   // another thread than the one that sets up the barriers, so the load overlaps that work.
@@ -304,12 +310,12 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
     const bool do_v = has_o && (sparse ? warp == V_PRODUCER_WARP : warp == PRODUCER_WARP);
     if (lane == 0) { tma_prefetch_desc(&tm_q); tma_prefetch_desc(&tm_k); tma_prefetch_desc(&tm_v); }
     if (do_k && n_tiles > 0 && !F8) {                                 // e4m3: the softmax warps convert and place Q
-      constexpr int COPIES = QUAD ? 4 : 1;
+      constexpr int COPIES = QUAD ? 4 : WIN ? PARTS : 1;
       if (lane == 0) mbar_arrive_expect_tx(bar(Q_FULL), COPIES * nrows * 256);
       __syncwarp();
       for (int c = lane; c < ntok * COPIES; c += 32) {       // G rows of one token per box
         const int ti = c / COPIES, quad = c % COPIES;
-        const uint32_t dst = smem_base + OFF_Q + (quad * 32 + ti * G) * 128;
+        const uint32_t dst = smem_base + OFF_Q + (quad * (WIN ? ROWS : 32) + ti * G) * 128;
         tma_load_3d(dst, &tm_q, bar(Q_FULL), 0, head0, qo_base + i_base + ti);
         tma_load_3d(dst + SUB_BYTES, &tm_q, bar(Q_FULL), 64, head0, qo_base + i_base + ti);
       }
@@ -483,10 +489,10 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
       }
       if (NBUF == 1 && j + 1 < n_tiles) { next_qk(j, alive); if (!alive) break; }
     }
-  } else if (warp < n_active_warps) {
+  } else if (WIN ? warp < 4 && (warp * 32) % ROWS < nrows : warp < n_active_warps) {
     // =========================== softmax / epilogue ===========================
     const int trow = (warp << 5) | lane;                     // row of the MMA tile == TMEM lane
-    const int r = QUAD ? lane : trow;                        // logical row of the work item
+    const int r = QUAD ? lane : trow % ROWS;                 // logical row of the work item
     const uint32_t lane_addr = static_cast<uint32_t>(warp << 5) << 16;
     const uint32_t tO = tmem + C::O_COL + lane_addr;
     const bool row_ok = r < nrows;
@@ -683,6 +689,95 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
         if (trace && j == 12) trace[15] = clock64() - clk0;      // ... P_FULL arrived
         if (trace && j == n_tiles - 1) trace[8] = clock64() - clk0;
       }
+    } else if constexpr (WIN) {
+      constexpr int CW = TK / PARTS;                         // key columns of a tile that this warp has
+      const int part = trow / ROWS;
+      for (int j = 0; j < n_tiles && alive; ++j) {
+        const uint32_t tS = tmem + (j % NBUF) * TK + lane_addr;
+        alive = mbar_wait_warp(bar(S_FULL + j % NBUF), (j / NBUF) & 1, abort_flag);
+        if (!alive) break;
+        tc_fence_after();
+        const int pos0 = tile_key0(j) + part * CW;
+        constexpr int LD = CW < 32 ? CW : 32;                // columns of a load
+        uint32_t sv[CW / LD][LD];
+#pragma unroll
+        for (int c = 0; c < CW / LD; ++c) {
+          if constexpr (LD == 16) tmem_ld16(tS + part * CW, sv[c]);
+          else tmem_ld32(tS + part * CW + c * LD, sv[c]);
+        }
+        tmem_wait_ld();
+        if (pos0 + CW - 1 > lim) {
+#pragma unroll
+          for (int e = 0; e < CW; ++e)
+            if (pos0 + e > lim) sv[e / LD][e % LD] = 0xff800000u;
+        }
+        if (pos0 < from && pos0 + CW > p.sink_tokens) {
+#pragma unroll
+          for (int e = 0; e < CW; ++e)
+            if (pos0 + e < from && pos0 + e >= p.sink_tokens) sv[e / LD][e % LD] = 0xff800000u;
+        }
+        float mxs[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int e = 0; e < CW; e += 2) mxs[(e >> 1) & 3] = max3(mxs[(e >> 1) & 3], __uint_as_float(sv[e / LD][e % LD]), __uint_as_float(sv[e / LD][e % LD + 1]));
+        const float mx = fmaxf(fmaxf(mxs[0], mxs[1]), fmaxf(mxs[2], mxs[3]));
+        const float m_cand = fmaxf(m_used, mx * scale_log2);
+        const bool bump = (m_cand - m_used) > kRescaleThreshold;
+        float factor = 1.f;
+        if (bump) { factor = exp2_fast(m_used - m_cand); m_used = m_cand; l_sum *= factor; }
+        if (j > 0 && __any_sync(0xffffffffu, bump)) {
+          // O may still be the target of P_{j-1} V_{j-1}: wait for that MMA before touching it
+          alive = mbar_wait_warp(bar(PV_DONE), (j - 1) & 1, abort_flag);
+          if (!alive) break;
+          tc_fence_after();
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t v[32];
+            tmem_ld32(tO + c * 32, v);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * factor);
+            tmem_st32(tO + c * 32, v);
+          }
+        }
+        const float msafe = ((m_used == -INFINITY) ? 0.f : m_used) - kPOffset;
+        float l0 = 0.f, l1 = 0.f;
+        // P, 32 columns in both formats (bf16: two keys a column; e4m3: four, 16 columns of hi and 16 of lo), zero but for this part's keys
+        constexpr int PER = F8 ? 4 : 2, OWN = CW / PER;      // keys of a column, columns of this part
+        uint32_t pk[OWN];
+        [[maybe_unused]] uint32_t pl[OWN];
+#pragma unroll
+        for (int e = 0; e < CW; e += PER) {
+          const float p0 = exp2_fast(fmaf(__uint_as_float(sv[e / LD][e % LD]), scale_log2, -msafe));
+          const float p1 = exp2_fast(fmaf(__uint_as_float(sv[e / LD][e % LD + 1]), scale_log2, -msafe));
+          if constexpr (F8) {
+            const float p2 = exp2_fast(fmaf(__uint_as_float(sv[e / LD][e % LD + 2]), scale_log2, -msafe));
+            const float p3 = exp2_fast(fmaf(__uint_as_float(sv[e / LD][e % LD + 3]), scale_log2, -msafe));
+            uint32_t hi[2], lo[2];
+            e4m3_pair(p0, p1, hi[0], lo[0]);
+            e4m3_pair(p2, p3, hi[1], lo[1]);
+            l0 += p0 + p2; l1 += p1 + p3;
+            pk[e / PER] = hi[0] | (hi[1] << 16);
+            pl[e / PER] = lo[0] | (lo[1] << 16);
+          } else {
+            const uint32_t pr = pack2<false>(p0, p1);
+            l0 += __uint_as_float(pr << 16); l1 += __uint_as_float(pr & 0xffff0000u);
+            pk[e / PER] = pr;
+          }
+        }
+        constexpr int PCOLS = TK / PER;
+        uint32_t all[32];
+#pragma unroll
+        for (int c = 0; c < PCOLS; ++c) {
+          const bool own = PARTS == 1 || c / OWN == part;
+          all[c] = own ? pk[c % OWN] : 0u;
+          if constexpr (F8) all[PCOLS + c] = own ? pl[c % OWN] : 0u;
+        }
+        tmem_st32(tS, all);
+        l_sum += l0 + l1;
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(bar(P_FULL + j % NBUF));
+      }
     } else {
     for (int j = 0; j < n_tiles && alive; ++j) {
       const uint32_t tS = tmem + (j % NBUF) * TK + lane_addr;
@@ -701,15 +796,6 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
 #pragma unroll
           for (int e = 0; e < 32; ++e)
             if (pos0 + c * 32 + e > lim) sv[c][e] = 0xff800000u;
-      }
-      if constexpr (WIN) {
-        if (pos0 < from && pos0 + TK > p.sink_tokens) {
-#pragma unroll
-          for (int c = 0; c < NC; ++c)
-#pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (pos0 + c * 32 + e < from && pos0 + c * 32 + e >= p.sink_tokens) sv[c][e] = 0xff800000u;
-        }
       }
       float mxs[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -756,30 +842,19 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
       for (int c = 0; c < NC; ++c) {
         if constexpr (F8) {
           uint32_t pk[8];                                   // four e4m3 per TMEM column
-          [[maybe_unused]] uint32_t pl[8];
 #pragma unroll
           for (int e = 0; e < 32; e += 4) {
             const float p0 = exp2_fast(fmaf(__uint_as_float(sv[c][e]), scale_log2, -msafe));
             const float p1 = exp2_fast(fmaf(__uint_as_float(sv[c][e + 1]), scale_log2, -msafe));
             const float p2 = exp2_fast(fmaf(__uint_as_float(sv[c][e + 2]), scale_log2, -msafe));
             const float p3 = exp2_fast(fmaf(__uint_as_float(sv[c][e + 3]), scale_log2, -msafe));
-            if constexpr (PAIR) {
-              uint32_t hi[2], lo[2];
-              e4m3_pair(p0, p1, hi[0], lo[0]);
-              e4m3_pair(p2, p3, hi[1], lo[1]);
-              l0 += p0 + p2; l1 += p1 + p3;
-              pk[e >> 2] = hi[0] | (hi[1] << 16);
-              pl[e >> 2] = lo[0] | (lo[1] << 16);
-            } else {
-              const uint16_t lo = __nv_cvt_float2_to_fp8x2(make_float2(p0, p1), __NV_SATFINITE, __NV_E4M3);
-              const uint16_t hi = __nv_cvt_float2_to_fp8x2(make_float2(p2, p3), __NV_SATFINITE, __NV_E4M3);
-              const float2 ra = e4m3x2_as_float2(lo), rb = e4m3x2_as_float2(hi);
-              l0 += ra.x + rb.x; l1 += ra.y + rb.y;
-              pk[e >> 2] = static_cast<uint32_t>(lo) | (static_cast<uint32_t>(hi) << 16);
-            }
+            const uint16_t lo = __nv_cvt_float2_to_fp8x2(make_float2(p0, p1), __NV_SATFINITE, __NV_E4M3);
+            const uint16_t hi = __nv_cvt_float2_to_fp8x2(make_float2(p2, p3), __NV_SATFINITE, __NV_E4M3);
+            const float2 ra = e4m3x2_as_float2(lo), rb = e4m3x2_as_float2(hi);
+            l0 += ra.x + rb.x; l1 += ra.y + rb.y;
+            pk[e >> 2] = static_cast<uint32_t>(lo) | (static_cast<uint32_t>(hi) << 16);
           }
           tmem_st8(tS + c * 8, pk);
-          if constexpr (PAIR) tmem_st8(tS + TK / 4 + c * 8, pl);
         } else {
           uint32_t pk[16];
 #pragma unroll
@@ -883,6 +958,76 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
         }
       }
       if (trace) trace[12] = clock64() - clk0;
+    } else if constexpr (WIN) {
+      // Every MMA and every TMA load of this CTA has completed: the rings are free to stage the rows' results, all parts, and Q the maxima and
+      // sums.  Chunks of 16 bytes are turned by the row, so that neither side has bank conflicts.
+      float* stage = reinterpret_cast<float*>(smem_gen + OFF_K);              // [BM][kHeadDim]
+      float* st_m = reinterpret_cast<float*>(smem_gen + OFF_Q);               // [BM]
+      float* st_l = st_m + BM;
+      if (alive) {
+        tc_fence_after();
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t v[32];
+          if (n_tiles > 0) {
+            tmem_ld32(tO + c * 32, v);
+            tmem_wait_ld();
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) v[e] = 0u;
+          }
+          if (row_ok) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              *reinterpret_cast<uint4*>(stage + trow * kHeadDim + 4 * ((8 * c + e) ^ (trow & 7))) = make_uint4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+          }
+        }
+        st_m[trow] = m_used; st_l[trow] = l_sum;
+      }
+      asm volatile("bar.sync 1, %0;" ::"r"(32 * n_active_warps) : "memory");
+      if (*abort_flag == 0) {
+        // thread -> (row, columns 4 t and 64 + 4 t): 16 threads a row
+        const float vsh = p.v_scale_head ? p.v_scale_head[kvh] : 1.f;
+        const bool to_partial = p.partial_o != nullptr;
+        const int nth = (PARTS == 4 ? warp : ROWS == 64 ? (warp >> 1) * ((nrows + 31) / 32) + (warp & 1) : warp) * 32 + lane, t = nth & 15;
+        for (int rr = nth >> 4; rr < nrows; rr += 2 * n_active_warps) {
+          float mq[PARTS], M = -INFINITY, L = 0.f;
+#pragma unroll
+          for (int q = 0; q < PARTS; ++q) { mq[q] = st_m[q * ROWS + rr]; M = fmaxf(M, mq[q]); }
+          float wq[PARTS];
+#pragma unroll
+          for (int q = 0; q < PARTS; ++q) {
+            wq[q] = mq[q] == -INFINITY ? 0.f : exp2_fast(mq[q] - M);
+            L += st_l[q * ROWS + rr] * wq[q];
+          }
+          const float inv = L > 0.f ? __fdividef(to_partial ? vsh : p.out_scale * vsh, L) : 0.f;
+          const int gt = qo_base + i_base + rr / G, hd = head0 + rr % G;
+          const float lse = L > 0.f ? (M - kPOffset) * kLn2 + __logf(L) : -INFINITY;   // l carries 2^kPOffset
+          const int64_t prow = (static_cast<int64_t>(split) * p.total_q + gt) * p.num_qo_heads + hd;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int q = 0; q < PARTS; ++q) {
+              const int row = q * ROWS + rr;
+              const float4 a = *reinterpret_cast<const float4*>(stage + row * kHeadDim + 4 * ((16 * h + t) ^ (row & 7)));
+              const float w = wq[q] * inv;                    // a part that saw no key has weight 0 and O == 0
+              acc[0] = fmaf(a.x, w, acc[0]); acc[1] = fmaf(a.y, w, acc[1]); acc[2] = fmaf(a.z, w, acc[2]); acc[3] = fmaf(a.w, w, acc[3]);
+            }
+            const int col = 64 * h + 4 * t;
+            if (to_partial) {
+              *reinterpret_cast<float4*>(p.partial_o + prow * kHeadDim + col) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+            } else if (p.out) {
+              *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.out) + static_cast<int64_t>(gt) * p.out_stride_tok +
+                                        static_cast<int64_t>(hd) * p.out_stride_head + col) = make_uint2(pack2<false>(acc[0], acc[1]), pack2<false>(acc[2], acc[3]));
+            }
+          }
+          if (t == 0) {
+            if (to_partial) p.partial_lse[prow] = lse;
+            else if (p.lse) p.lse[static_cast<int64_t>(gt) * p.num_qo_heads + hd] = lse;
+          }
+        }
+      }
     } else
     if (alive && has_o) {
       tc_fence_after();
@@ -1000,20 +1145,25 @@ int fmha_decode_tc_launch(const MsaFmhaParams& p, cudaStream_t stream) {
         return MSA_ERR_LAUNCH;
     }
   }
-  static bool attr_done[16][6] = {};
+  static bool attr_done[16][10] = {};
   int dev = 0;
   cudaGetDevice(&dev);
   using Kern = void (*)(const MsaFmhaParams, const CUtensorMap, const CUtensorMap, const CUtensorMap);
-  const int variant = p.window > 0 ? 4 + (f8 ? 1 : 0) : (f8 ? 2 : 0) | (quad ? 1 : 0);
+  const int parts = p.decode_rows <= 32 ? 4 : p.decode_rows <= 64 ? 2 : 1;
+  const int variant = p.window > 0 ? 4 + (parts >> 1) * 2 + (f8 ? 1 : 0) : (f8 ? 2 : 0) | (quad ? 1 : 0);
   Kern kern;
   int smem;
   switch (variant) {
-    case 0: kern = decode_tc_kernel<false, false, false>; smem = Cfg<false, false>::SMEM_BYTES; break;
-    case 1: kern = decode_tc_kernel<false, true, false>;  smem = Cfg<false, true>::SMEM_BYTES;  break;
-    case 2: kern = decode_tc_kernel<true, false, false>;  smem = Cfg<true, false>::SMEM_BYTES;  break;
-    case 3: kern = decode_tc_kernel<true, true, false>;   smem = Cfg<true, true>::SMEM_BYTES;   break;
-    case 4: kern = decode_tc_kernel<false, false, true>;  smem = Cfg<false, false, true>::SMEM_BYTES; break;
-    default: kern = decode_tc_kernel<true, false, true>;  smem = Cfg<true, false, true>::SMEM_BYTES;  break;
+    case 0: kern = decode_tc_kernel<false, false, 0>; smem = Cfg<false, false>::SMEM_BYTES; break;
+    case 1: kern = decode_tc_kernel<false, true, 0>;  smem = Cfg<false, true>::SMEM_BYTES;  break;
+    case 2: kern = decode_tc_kernel<true, false, 0>;  smem = Cfg<true, false>::SMEM_BYTES;  break;
+    case 3: kern = decode_tc_kernel<true, true, 0>;   smem = Cfg<true, true>::SMEM_BYTES;   break;
+    case 4: kern = decode_tc_kernel<false, false, 1>; smem = Cfg<false, false, true>::SMEM_BYTES; break;
+    case 5: kern = decode_tc_kernel<true, false, 1>;  smem = Cfg<true, false, true>::SMEM_BYTES;  break;
+    case 6: kern = decode_tc_kernel<false, false, 2>; smem = Cfg<false, false, true>::SMEM_BYTES; break;
+    case 7: kern = decode_tc_kernel<true, false, 2>;  smem = Cfg<true, false, true>::SMEM_BYTES;  break;
+    case 8: kern = decode_tc_kernel<false, false, 4>; smem = Cfg<false, false, true>::SMEM_BYTES; break;
+    default: kern = decode_tc_kernel<true, false, 4>; smem = Cfg<true, false, true>::SMEM_BYTES;  break;
   }
   if (dev >= 16 || !attr_done[dev][variant]) {
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
@@ -1031,21 +1181,21 @@ int fmha_decode_tc_occupancy(int f8, int quad) {
   int n = 0;
   cudaError_t e;
   if (f8 && quad) {
-    cudaFuncSetAttribute(decode_tc_kernel<true, true, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<true, true>::SMEM_BYTES);
-    e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, decode_tc_kernel<true, true, false>, NTHREADS, Cfg<true, true>::SMEM_BYTES);
+    cudaFuncSetAttribute(decode_tc_kernel<true, true, 0>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<true, true>::SMEM_BYTES);
+    e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, decode_tc_kernel<true, true, 0>, NTHREADS, Cfg<true, true>::SMEM_BYTES);
     cudaFuncAttributes fa;
-    if (cudaFuncGetAttributes(&fa, decode_tc_kernel<true, true, false>) == cudaSuccess)
+    if (cudaFuncGetAttributes(&fa, decode_tc_kernel<true, true, 0>) == cudaSuccess)
       fprintf(stderr, "decode_tc_kernel<e4m3, quad>: regs %d static smem %zu dyn smem %d local %zu max threads %d\n", fa.numRegs,
               fa.sharedSizeBytes, Cfg<true, true>::SMEM_BYTES, fa.localSizeBytes, fa.maxThreadsPerBlock);
   } else if (f8) {
-    cudaFuncSetAttribute(decode_tc_kernel<true, false, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<true, false>::SMEM_BYTES);
-    e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, decode_tc_kernel<true, false, false>, NTHREADS, Cfg<true, false>::SMEM_BYTES);
+    cudaFuncSetAttribute(decode_tc_kernel<true, false, 0>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<true, false>::SMEM_BYTES);
+    e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, decode_tc_kernel<true, false, 0>, NTHREADS, Cfg<true, false>::SMEM_BYTES);
   } else if (quad) {
-    cudaFuncSetAttribute(decode_tc_kernel<false, true, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<false, true>::SMEM_BYTES);
-    e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, decode_tc_kernel<false, true, false>, NTHREADS, Cfg<false, true>::SMEM_BYTES);
+    cudaFuncSetAttribute(decode_tc_kernel<false, true, 0>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<false, true>::SMEM_BYTES);
+    e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, decode_tc_kernel<false, true, 0>, NTHREADS, Cfg<false, true>::SMEM_BYTES);
   } else {
-    cudaFuncSetAttribute(decode_tc_kernel<false, false, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<false, false>::SMEM_BYTES);
-    e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, decode_tc_kernel<false, false, false>, NTHREADS, Cfg<false, false>::SMEM_BYTES);
+    cudaFuncSetAttribute(decode_tc_kernel<false, false, 0>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<false, false>::SMEM_BYTES);
+    e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, decode_tc_kernel<false, false, 0>, NTHREADS, Cfg<false, false>::SMEM_BYTES);
   }
   return e == cudaSuccess ? n : -1;
 }

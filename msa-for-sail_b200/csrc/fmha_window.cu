@@ -549,8 +549,9 @@ int launch(const MsaFmhaParams& p, cudaStream_t stream) {
 }  // namespace
 }  // namespace window
 
-// Windowed items of few packed rows (with 32 over an e4m3 cache registers run out: 256 items x 9 pages take 51 us, on the tcgen05 decode
-// kernel 47; bf16: 30 and 42); pages of whole units, or ragged keys.
+// Windowed items of few packed rows; pages of whole units, or ragged keys.  Here and on the tcgen05 decode kernel, windows of 2 048 keys: bf16,
+// 64 sequences x 2 heads x 32 rows 35 and 38 us, 128 x 8 x 32 338 and 362; e4m3, 64 x 2 x 8 rows 22 and 25 us, 16 rows 29 and 26, but one
+// sequence 9.3 and 10.2, 24 of 512 keys 12.3 and 12.8 (and pages of any whole units); with 32 rows over an e4m3 cache registers run out.
 int fmha_window_rows(const MsaFmhaParams& p) { return p.kv_dtype == MSA_DT_E4M3 ? 16 : 32; }
 int fmha_window_supported(const MsaFmhaParams& p) {
   if (p.window <= 0 || (p.flags & MSA_FLAG_SPARSE) || p.decode_rows < 1 || p.decode_rows > fmha_window_rows(p)) return 0;
