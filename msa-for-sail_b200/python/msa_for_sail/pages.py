@@ -177,7 +177,8 @@ def kv_pages_free(block_table: torch.Tensor, num_held: torch.Tensor, kv_lens: to
 
     Row ``b`` keeps the pages of its first ``kv_lens[b]`` tokens: 0 for a request that ended, less than before where drafted tokens were
     rejected.  With ``window_size`` and ``num_sink_tokens`` (as ``fmha_sail_plan`` takes them) it keeps of those only what a query at place
-    ``kv_lens[b]`` or later sees: call it with the length before the new tokens of a step, or after the attention over them.  Entries given back
+    ``kv_lens[b]`` or later sees: call it with the length before the new tokens of a step, or after the attention over them.  (Without a window
+    it sees all of them, sinks or not.)  Entries given back
     become -1 (``paged_kv_tables`` turns those into page 0, which a windowed call does not read) and ``num_held`` the number of pages of
     the length.
 
@@ -191,15 +192,15 @@ def kv_pages_free(block_table: torch.Tensor, num_held: torch.Tensor, kv_lens: to
     window = -1 if window_size is None else int(window_size)
     if window == 0 or window < -1 or window > (1 << 31) - 1:
         raise ValueError(f"window_size must be -1 (no window) or from 1 to 2^31 - 1, got {window_size}")
-    if num_sink_tokens < 0 or num_sink_tokens > (1 << 31) - 1 or (num_sink_tokens and window == -1):
-        raise ValueError(f"num_sink_tokens={num_sink_tokens} must not be negative, fit int32, and belongs to a window_size")
+    if not 0 <= num_sink_tokens <= (1 << 31) - 1:
+        raise ValueError(f"num_sink_tokens must be from 0 to 2^31 - 1, got {num_sink_tokens}")
     ws = _lib.check(_lib.lib.msa_pages_free_workspace_bytes(B, width), "msa_pages_free_workspace_bytes") // 4
     buf = torch.empty(ws + 1, dtype=torch.int32, device=dev)
     ptr = buf.data_ptr()
     _launch(dev, _lib.lib.msa_pages_free, _lib.pages_free_args(
         block_table.data_ptr(), num_held.data_ptr(), kv_lens.data_ptr(), free_pages.data_ptr(), num_free.data_ptr(), 0 if shares is None else shares.data_ptr(),
         ptr, ptr + 4, stride, B, width, page_size, free_pages.shape[0], (1 << 31) - 1 if shares is None else shares.shape[0], max(window, 0),
-        int(num_sink_tokens)), "msa_pages_free")
+        int(num_sink_tokens) if window > 0 else 0), "msa_pages_free")
     return buf[:1]
 
 

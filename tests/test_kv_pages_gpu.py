@@ -199,7 +199,7 @@ def test_free(rows, width, page_size, window, sinks, sharing):
     t = torch.full((rows, width + 2), -77, dtype=torch.int32, device=DEV)
     t[:, :width] = _i32(table).view(rows, width)
     d = dict(held=_i32(held), kv=_i32(now), free=_i32(free), num_free=_i32([num_free]), shares=_i32(shares) if sharing else None)
-    freed = _msa().kv_pages_free(t[:, :width], d["held"], d["kv"], d["free"], d["num_free"], d["shares"], window_size=window, num_sink_tokens=sinks if window > 0 else 0,
+    freed = _msa().kv_pages_free(t[:, :width], d["held"], d["kv"], d["free"], d["num_free"], d["shares"], window_size=window, num_sink_tokens=sinks,
                                  page_size=page_size)
     _ok()
     left, count = ref.free_pages(table, held, now, free, num_free, shares if sharing else None, window, sinks, page_size)
@@ -330,3 +330,58 @@ def test_a_captured_beam_step():
         assert all((c - 1 if c else 0) == s for c, s in zip(count, shares))
         assert sorted(free[:num_free]) == [p for p in range(P) if not count[p]]
     _ok()
+
+
+def test_refused_calls():
+    m = _msa()
+    P, B, width = 8, 2, 4
+    t, held, kv, free, num_free, shares = torch.zeros(B, width, dtype=torch.int32, device=DEV), _i32([2, 1]), _i32([200, 100]), _i32([7] * 8), _i32([5]), _i32([0] * P)
+    cache = _cache("hnd", P)
+    one = _i32([0])
+    other = torch.zeros(8, P, 4, 4, device=DEV).transpose(0, 1)[:, ::2, ::3, ::2]         # no even steps
+    bad = [
+        lambda: m.kv_pages_copy(cache, one, _i32([0, 1])), lambda: m.kv_pages_copy(cache, one.long(), one), lambda: m.kv_pages_copy(cache, one.cpu(), one),
+        lambda: m.kv_pages_copy([cache, cache[:4]], one, one), lambda: m.kv_pages_copy([cache, cache.cpu()], one, one), lambda: m.kv_pages_copy(other, one, one),
+        lambda: m.kv_pages_copy(cache[:1].expand(P, -1, -1, -1), one, one), lambda: m.kv_pages_copy(cache, one[0], one),
+        lambda: m.kv_pages_fork(t, held, kv, one, _i32([0, 1]), free, num_free, shares), lambda: m.kv_pages_fork(t, held[:1], kv, one, one, free, num_free, shares),
+        lambda: m.kv_pages_fork(t, held, kv.long(), one, one, free, num_free, shares), lambda: m.kv_pages_fork(t, held, kv, one, one, free, held, shares),
+        lambda: m.kv_pages_fork(t, held, kv, one, one, free, num_free, shares[:4], cache), lambda: m.kv_pages_fork(t, held, kv, one, one, free, num_free, shares, page_size=0),
+        lambda: m.kv_pages_fork(t.T, held, kv, one, one, free, num_free, shares), lambda: m.kv_pages_fork(t[:1].expand(2, -1), held, kv, one, one, free, num_free, shares),
+        lambda: m.kv_pages_fork(t.long(), held, kv, one, one, free, num_free, shares),
+        lambda: m.kv_pages_free(t, held, kv, free, num_free, window_size=0), lambda: m.kv_pages_free(t, held, kv, free, num_free, window_size=-3),
+        lambda: m.kv_pages_free(t, held, kv, free, num_free, window_size=3, num_sink_tokens=-1), lambda: m.kv_pages_free(t, held, kv, free.cpu(), num_free),
+        lambda: m.kv_pages_free(t, held, kv, free, num_free, shares.float()), lambda: m.kv_pages_free(t, held, kv, free, num_free, page_size=1 << 31),
+        lambda: m.kv_pages_free(t[0], held, kv, free, num_free),
+        lambda: m.kv_pages_compact(t, held, free, num_free), lambda: m.kv_pages_compact(t, held, free, num_free, num_pages=-1),
+        lambda: m.kv_pages_compact(t, held, free, num_free, cache, shares[:4]), lambda: m.kv_pages_compact(t, held, free, num_free, cache, num_pages=4),
+        lambda: m.kv_pages_compact(t, held, free, num_free, shares=shares, num_pages=9)]
+    before = [x.clone() for x in (t, held, kv, free, num_free, shares, cache.view(torch.int16))]
+    for i, call in enumerate(bad):
+        with pytest.raises(ValueError):
+            call()
+            raise AssertionError(f"call {i} was not refused")
+    _ok()
+    for x, y in zip(before, (t, held, kv, free, num_free, shares, cache.view(torch.int16))):
+        assert torch.equal(x, y)
+
+
+def test_two_streams():
+    """Two pools on two streams at once; workspaces are each call's own."""
+    m = _msa()
+    P = 3000
+    streams, pools = [torch.cuda.Stream() for _ in range(2)], []
+    for i in range(2):
+        table = torch.randperm(P, generator=torch.Generator().manual_seed(i))[:2000].view(20, 100).int().to(DEV)
+        rest = torch.tensor(sorted(set(range(P)) - set(table.flatten().tolist())), dtype=torch.int32, device=DEV)
+        free = torch.cat([rest, torch.zeros(2000, dtype=torch.int32, device=DEV)])
+        cache = _cache("e4m3", P, i, 16)
+        pools.append((table, _i32([100] * 20), free, _i32([P - 2000]), cache, cache[table.flatten().long()].clone()))
+    torch.cuda.synchronize()
+    for r in range(3):
+        for s, (t, held, free, num_free, cache, _) in zip(streams, pools):
+            with torch.cuda.stream(s):
+                m.kv_pages_compact(t, held, free, num_free, cache)
+    _ok()
+    for t, held, free, num_free, cache, was in pools:
+        assert sorted(t.flatten().tolist()) == list(range(2000)) and num_free.item() == P - 2000
+        assert torch.equal(_raw(cache[t.flatten().long()]), _raw(was)) and sorted(free[:1000].tolist()) == list(range(2000, P))
