@@ -113,26 +113,27 @@ __global__ void __launch_bounds__(kThreads) pages_copy_kernel(const __grid_const
 // ---------------------------------------------------------------------------------------------------------------------------
 
 // Exclusive prefix of x over the CTA, and the sum of all; s_sum has a word for each warp.  All threads take part.
-template <int THREADS>
-__device__ __forceinline__ int block_scan(int x, int* s_sum, int& total) {
+template <int THREADS, typename T>
+__device__ __forceinline__ T block_scan(T x, T* s_sum, T& total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   constexpr int WARPS = THREADS / 32;
-  int incl = x;
+  T incl = x;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
-    const int v = __shfl_up_sync(0xffffffffu, incl, d);
+    const T v = __shfl_up_sync(0xffffffffu, incl, d);
     if (lane >= d) incl += v;
   }
   if (lane == 31) s_sum[warp] = incl;
   __syncthreads();
-  int mine = lane < WARPS ? s_sum[lane] : 0, scan = mine;
+  const T mine = lane < WARPS ? s_sum[lane] : T(0);
+  T scan = mine;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
-    const int v = __shfl_up_sync(0xffffffffu, scan, d);
+    const T v = __shfl_up_sync(0xffffffffu, scan, d);
     if (lane >= d) scan += v;
   }
   total = __shfl_sync(0xffffffffu, scan, 31);
-  const int before = __shfl_sync(0xffffffffu, scan - mine, warp);
+  const T before = __shfl_sync(0xffffffffu, scan - mine, warp);
   __syncthreads();                             // s_sum may be written again
   return before + incl - x;
 }
@@ -216,7 +217,7 @@ __global__ void __launch_bounds__(kScanThreads) pages_fork_plan_kernel(const Msa
       }
     }
     int total;
-    const int rank = taken + block_scan<kScanThreads>(part > 0, s_sum, total);
+    const int rank = taken + block_scan<kScanThreads>(part > 0 ? 1 : 0, s_sum, total);
     taken += total;
     int dst = -1;
     if (part > 0) {
@@ -477,7 +478,7 @@ __global__ void __launch_bounds__(kThreads) pages_free_push_kernel(const MsaPage
         if (given_back(k, col)) a.block_table[b * a.table_stride + col] = -1;
       }
       int total;
-      const int rank = block_scan<kThreads>(mine, s_sum, total);
+      const int rank = block_scan<kThreads>(mine ? 1 : 0, s_sum, total);
       if (mine) push(a, page, at + rank);
       at += total;
     }
@@ -544,29 +545,43 @@ __device__ __forceinline__ uint32_t from_line(int w, int line) {
 
 // By one CTA of kScanThreads.
 __device__ __forceinline__ void rank_pages(const MsaPagesCompactArgs& a) {
+  // Several counts go through a scan at once, in fields that the pages of one scan (2^15) do not fill.
+  using u64 = unsigned long long;
   const Sets s = sets_of(a);
-  __shared__ int s_sum[32];
+  __shared__ u64 s_sum[32];
   __shared__ int s_line;
   const int tid = threadIdx.x, words = words_of(a.num_pages);
-  int used = 0, total;
+  u64 total;
+  int used = 0, before = 0, mine = 0;          // pages in use; managed ones in the words before this scan's, before this thread's
+  uint32_t managed = 0;
   for (int w0 = 0; w0 < words; w0 += kScanThreads) {
     const int w = w0 + tid;
-    block_scan<kScanThreads>(w < words ? __popc(__ldcg(&s.live[w])) : 0, s_sum, total);
-    used += total;
+    const uint32_t live = w < words ? __ldcg(&s.live[w]) : 0u;
+    managed = w < words ? live | __ldcg(&s.free[w]) : 0u;
+    mine = before + static_cast<int>(block_scan<kScanThreads>(static_cast<u64>(__popc(live)) << 32 | __popc(managed), s_sum, total) & 0xffffffffu);
+    used += static_cast<int>(total >> 32);
+    before += static_cast<int>(total & 0xffffffffu);
   }
   if (tid == 0) s_line = a.num_pages;          // (nothing is free below it: nothing moves)
   __syncthreads();
-  int before = 0;                              // managed pages in the words before
-  for (int w0 = 0; w0 < words && before <= used; w0 += kScanThreads) {
-    const int w = w0 + tid;
-    const uint32_t managed = w < words ? __ldcg(&s.live[w]) | __ldcg(&s.free[w]) : 0u;
-    const int mine = before + block_scan<kScanThreads>(__popc(managed), s_sum, total);
-    before += total;
-    // the managed page with number `used` (from 0) is the first one that does not stay in use
+  // the managed page with number `used` (from 0) is the first one that does not stay in use
+  auto find = [&](int w) {
     if (mine <= used && used < mine + __popc(managed)) {
       uint32_t m = managed;
       for (int n = used - mine; n > 0; --n) m &= m - 1;
       s_line = 32 * w + __ffs(m) - 1;
+    }
+  };
+  if (words <= kScanThreads) {
+    find(tid);
+  } else {
+    before = 0;
+    for (int w0 = 0; w0 < words && before <= used; w0 += kScanThreads) {
+      const int w = w0 + tid;
+      managed = w < words ? __ldcg(&s.live[w]) | __ldcg(&s.free[w]) : 0u;
+      mine = before + static_cast<int>(block_scan<kScanThreads>(static_cast<u64>(__popc(managed)), s_sum, total));
+      before += static_cast<int>(total);
+      find(w);
     }
   }
   __syncthreads();
@@ -574,18 +589,16 @@ __device__ __forceinline__ void rank_pages(const MsaPagesCompactArgs& a) {
   int sums[3] = {0, 0, 0};
   for (int w0 = 0; w0 < words; w0 += kScanThreads) {
     const int w = w0 + tid;
-    int own[3] = {0, 0, 0};
+    u64 own = 0;
     if (w < words) {
-      const uint32_t live = __ldcg(&s.live[w]), managed = live | __ldcg(&s.free[w]), above = from_line(w, line);
-      own[0] = __popc(live & above);
-      own[1] = __popc(managed & ~live & ~above);
-      own[2] = __popc(managed & above);
+      const uint32_t live = __ldcg(&s.live[w]), all = live | __ldcg(&s.free[w]), above = from_line(w, line);
+      own = static_cast<u64>(__popc(live & above)) | static_cast<u64>(__popc(all & ~live & ~above)) << 20 | static_cast<u64>(__popc(all & above)) << 40;
     }
+    const u64 at = block_scan<kScanThreads>(own, s_sum, total);
 #pragma unroll
     for (int i = 0; i < 3; ++i) {
-      const int at = sums[i] + block_scan<kScanThreads>(own[i], s_sum, total);
-      sums[i] += total;
-      if (w < words) (i == 0 ? s.moving : i == 1 ? s.holes : s.rest)[w] = at;
+      if (w < words) (i == 0 ? s.moving : i == 1 ? s.holes : s.rest)[w] = sums[i] + static_cast<int>(at >> (20 * i) & 0xfffff);
+      sums[i] += static_cast<int>(total >> (20 * i) & 0xfffff);
     }
   }
   if (tid == 0) {
@@ -609,8 +622,8 @@ __device__ __forceinline__ void list_pages(const MsaPagesCompactArgs& a, int fir
   if (first == 0) *a.num_free = left;
 }
 
-// Ordinary pools: the CTAs of one cluster.  (8 192 pages, nothing to copy: 15.5 us in a captured graph against 17.4 for a memset and three
-// launches.)
+// Ordinary pools: the CTAs of one cluster.  (8 192 pages, nothing to copy: 14.4 us in a captured graph; 15.5 before the counts shared a scan,
+// when a memset and three launches took 17.4.)
 __global__ void __launch_bounds__(kScanThreads) pages_compact_cluster_kernel(const MsaPagesCompactArgs a) {
   chain_begin();
   auto cluster = cooperative_groups::this_cluster();
