@@ -691,6 +691,7 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
       }
     } else if constexpr (WIN) {
       constexpr int CW = TK / PARTS;                         // key columns of a tile that this warp has
+      constexpr int RC = PARTS == 1 ? 16 : 32;               // columns of O scaled at a time: 64 scores leave no registers for 32
       const int part = trow / ROWS;
       for (int j = 0; j < n_tiles && alive; ++j) {
         const uint32_t tS = tmem + (j % NBUF) * TK + lane_addr;
@@ -730,49 +731,61 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
           if (!alive) break;
           tc_fence_after();
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t v[32];
-            tmem_ld32(tO + c * 32, v);
+          for (int c = 0; c < kHeadDim; c += RC) {
+            uint32_t v[RC];
+            if constexpr (RC == 16) tmem_ld16(tO + c, v);
+            else tmem_ld32(tO + c, v);
             tmem_wait_ld();
 #pragma unroll
-            for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * factor);
-            tmem_st32(tO + c * 32, v);
+            for (int e = 0; e < RC; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * factor);
+            if constexpr (RC == 16) tmem_st16(tO + c, v);
+            else tmem_st32(tO + c, v);
           }
         }
         const float msafe = ((m_used == -INFINITY) ? 0.f : m_used) - kPOffset;
         float l0 = 0.f, l1 = 0.f;
         // P, 32 columns in both formats (bf16: two keys a column; e4m3: four, 16 columns of hi and 16 of lo), zero but for this part's keys
-        constexpr int PER = F8 ? 4 : 2, OWN = CW / PER;      // keys of a column, columns of this part
-        uint32_t pk[OWN];
-        [[maybe_unused]] uint32_t pl[OWN];
+        constexpr int PER = F8 ? 4 : 2, OWN = LD / PER, PCOLS = TK / PER;      // keys of a column, columns of a load's keys, of all
 #pragma unroll
-        for (int e = 0; e < CW; e += PER) {
-          const float p0 = exp2_fast(fmaf(__uint_as_float(sv[e / LD][e % LD]), scale_log2, -msafe));
-          const float p1 = exp2_fast(fmaf(__uint_as_float(sv[e / LD][e % LD + 1]), scale_log2, -msafe));
-          if constexpr (F8) {
-            const float p2 = exp2_fast(fmaf(__uint_as_float(sv[e / LD][e % LD + 2]), scale_log2, -msafe));
-            const float p3 = exp2_fast(fmaf(__uint_as_float(sv[e / LD][e % LD + 3]), scale_log2, -msafe));
-            uint32_t hi[2], lo[2];
-            e4m3_pair(p0, p1, hi[0], lo[0]);
-            e4m3_pair(p2, p3, hi[1], lo[1]);
-            l0 += p0 + p2; l1 += p1 + p3;
-            pk[e / PER] = hi[0] | (hi[1] << 16);
-            pl[e / PER] = lo[0] | (lo[1] << 16);
+        for (int c0 = 0; c0 < CW / LD; ++c0) {
+          uint32_t pk[OWN];
+          [[maybe_unused]] uint32_t pl[OWN];
+#pragma unroll
+          for (int e1 = 0; e1 < LD; e1 += PER) {
+            const int e = c0 * LD + e1;
+            const float p0 = exp2_fast(fmaf(__uint_as_float(sv[e / LD][e % LD]), scale_log2, -msafe));
+            const float p1 = exp2_fast(fmaf(__uint_as_float(sv[e / LD][e % LD + 1]), scale_log2, -msafe));
+            if constexpr (F8) {
+              const float p2 = exp2_fast(fmaf(__uint_as_float(sv[e / LD][e % LD + 2]), scale_log2, -msafe));
+              const float p3 = exp2_fast(fmaf(__uint_as_float(sv[e / LD][e % LD + 3]), scale_log2, -msafe));
+              uint32_t hi[2], lo[2];
+              e4m3_pair(p0, p1, hi[0], lo[0]);
+              e4m3_pair(p2, p3, hi[1], lo[1]);
+              l0 += p0 + p2; l1 += p1 + p3;
+              pk[e1 / PER] = hi[0] | (hi[1] << 16);
+              pl[e1 / PER] = lo[0] | (lo[1] << 16);
+            } else {
+              const uint32_t pr = pack2<false>(p0, p1);
+              l0 += __uint_as_float(pr << 16); l1 += __uint_as_float(pr & 0xffff0000u);
+              pk[e1 / PER] = pr;
+            }
+          }
+          if constexpr (PARTS > 1) {
+            uint32_t all[32];
+#pragma unroll
+            for (int c = 0; c < PCOLS; ++c) {
+              const bool own = c / OWN == part;
+              all[c] = own ? pk[c % OWN] : 0u;
+              if constexpr (F8) all[PCOLS + c] = own ? pl[c % OWN] : 0u;
+            }
+            tmem_st32(tS, all);
+          } else if constexpr (F8) {
+            tmem_st8(tS + c0 * OWN, pk);
+            tmem_st8(tS + PCOLS + c0 * OWN, pl);
           } else {
-            const uint32_t pr = pack2<false>(p0, p1);
-            l0 += __uint_as_float(pr << 16); l1 += __uint_as_float(pr & 0xffff0000u);
-            pk[e / PER] = pr;
+            tmem_st16(tS + c0 * OWN, pk);
           }
         }
-        constexpr int PCOLS = TK / PER;
-        uint32_t all[32];
-#pragma unroll
-        for (int c = 0; c < PCOLS; ++c) {
-          const bool own = PARTS == 1 || c / OWN == part;
-          all[c] = own ? pk[c % OWN] : 0u;
-          if constexpr (F8) all[PCOLS + c] = own ? pl[c % OWN] : 0u;
-        }
-        tmem_st32(tS, all);
         l_sum += l0 + l1;
         tmem_wait_st();
         tc_fence_before();
