@@ -13,6 +13,8 @@ csrc/msa_profiling_interface.hpp:99-157).  Upstream's emitter and parser disagre
 (`num_heads` / `num_qo_heads`, `num_heads_kv` / `num_kv_heads`, `head_dim` / `head_dim_qk`,
 `head_dim_v` / `head_dim_vo`, `topk` / `kv_block_num`): both spellings are accepted here.
 
+A call with a window has ``window_size:1024,num_sink_tokens:4`` behind the last key.
+
 Only the call's shape travels in the line, so the tensors are random.  sparse_mode: Off (O only),
 Full (O and max_score), OnlyScore (max_score only), Sparse (O over kv_block_num selected pages).
 
@@ -92,7 +94,8 @@ def format_line(cfg):
             return f"{v:.6f}"
         return str(v)
     keys = ("dtype", "batch_size", "seqlen_q", "seqlen_k", "qo_offset", "num_qo_heads", "num_kv_heads", "head_dim_qk",
-            "head_dim_vo", "num_kv_splits", "is_paged", "page_size", "causal", "sm_scale", "sparse_mode", "kv_block_num")
+            "head_dim_vo", "num_kv_splits", "is_paged", "page_size", "causal", "sm_scale", "sparse_mode", "kv_block_num",
+            "window_size", "num_sink_tokens")
     return "[MSA] --format=" + ",".join(f"{k}:{one(cfg[k])}" for k in keys if k in cfg) + "."
 
 
@@ -103,15 +106,23 @@ def flops_and_bytes(cfg):
     sq, sk = cfg["seqlen_q"], cfg["seqlen_k"]
     offs = cfg.get("qo_offset") or [k - q for q, k in zip(sq, sk)]
     mode, kbn, page = cfg["sparse_mode"], cfg["kv_block_num"], cfg["page_size"]
-    pairs = 0                                              # visible (query, key) pairs per head
+    window, sinks = cfg.get("window_size", -1), cfg.get("num_sink_tokens", 0)
+    pairs = seen = 0                                       # visible (query, key) pairs per head; keys that some query sees
     for q, k, o in zip(sq, sk, offs):
         for i in range(q):
             vis = min(k, i + o + 1) if cfg["causal"] else k
+            if window > 0:
+                lo = min(max(0, i + o - window + 1), max(vis, 0))
+                pairs += max(vis, 0) - max(0, lo - sinks)
+                continue
             pairs += min(vis, kbn * page) if mode == "Sparse" else max(vis, 0)
+        if window > 0 and q > 0:
+            hi = max(0, min(k, q + o))
+            seen += hi - max(0, min(max(0, o - window + 1), hi) - sinks)
     per_pair = 2 * 128 if mode == "OnlyScore" else 4 * 128
     flops = hq * pairs * per_pair
     total_q = sum(sq)
-    kv_tokens = total_q * kbn * page if mode == "Sparse" else sum(sk)
+    kv_tokens = seen if window > 0 else total_q * kbn * page if mode == "Sparse" else sum(sk)
     kv_bytes = kv_tokens * hk * 128 * e * (1 if mode == "OnlyScore" else 2)
     nbytes = total_q * hq * 128 * e + kv_bytes + (0 if mode == "OnlyScore" else total_q * hq * 128 * 2)
     return flops, nbytes
@@ -147,7 +158,8 @@ def build_case(cfg):
                               num_kv_splits=cfg["num_kv_splits"], causal=bool(cfg["causal"]),
                               qo_offset=i32(offs) if offs else None, use_fp8_kvcache=fp8,
                               output_maxscore=mode in ("Full", "OnlyScore"),
-                              kv_block_num=kbn if mode == "Sparse" else -1)
+                              kv_block_num=kbn if mode == "Sparse" else -1,
+                              window_size=cfg.get("window_size", -1), num_sink_tokens=cfg.get("num_sink_tokens", 0))
     if mode == "Sparse" and cfg.get("selection") == "first":      # the sweep's choice: pages 0 .. k-1 for every token
         n_sel = min(kbn, min((kl + page - 1) // page for kl in sk))
         sel = torch.full((total_q, hk, kbn), -1, dtype=torch.int32, device=dev)

@@ -773,6 +773,8 @@ def _show_params(q, plan, is_paged, page_size, sm_scale, output_o, max_score, kv
               ("is_paged", int(is_paged)), ("page_size", page_size if is_paged else 0), ("causal", int(plan["causal"])),
               ("sm_scale", f"{sm_scale:.6f}"), ("sparse_mode", mode),
               ("kv_block_num", plan["kv_block_num"] if plan["is_sparse"] else 0)]
+    if plan["window"][0]:
+        fields += [("window_size", plan["window"][0]), ("num_sink_tokens", plan["window"][1])]
     print("[MSA] --format=" + ",".join(f"{k}:{v}" for k, v in fields) + ".", flush=True)
 
 
@@ -1371,6 +1373,14 @@ def fmha_sail_plan(
     result) and the ``*_override`` hints.  With
     ``split_prefill_decode`` a decode-first batch is planned as two sub-batches, each with
     the tile shape that suits it.
+
+    ``window_size`` (default -1, none) and ``num_sink_tokens`` (default 0): a query at place ``t`` of its
+    sequence (its row + ``qo_offset``) sees the keys ``j <= t`` with ``j > t - window_size`` or
+    ``j < num_sink_tokens``.  A row that sees none gets zeros and an LSE of -inf.  Tiles that no row of a
+    work item sees are not read, and what a key that no query of its sequence sees holds does not matter
+    (NaN; the place may be in a page that ``kv_pages_free`` took back, whose entry is then any page).
+    bf16 and e4m3 caches, ragged or paged, prompts, decode, device-made plans; ``causal=True`` and O
+    only: no page scores, no selected pages, no 4-bit cache.
     """
     graph_safe = bool(kwargs.get("graph_safe", False))
     if isinstance(qo_offset, int):
@@ -1463,6 +1473,13 @@ def fmha_sail(
     queries, page scores and sparse prefill run on bf16 copies of the pages in ``kv_indices``, which
     live for the call (``len(kv_indices) * Hkv * 32`` KB each for keys and values; planned pages and a
     fixed-address table alike, so a captured prefill has a table no longer than its use).
+
+    With a plan that has a ``window_size``: bf16 or e4m3 ``k``/``v``, ``q`` in bf16 or their type.  Weights are
+    rounded to bf16, or to pairs of e4m3 values with as many bits over an e4m3 cache (bf16 queries too,
+    where rows are few; prompts of bf16 queries over an e4m3 cache run on the generic kernel, with weights in fp16).  The
+    plan has its offsets (no ``q_offset_override``), the factor of the scores (``sm_scale * q_scale *
+    k_scale``) is not negative, and partials of a split are the call's own, so that one plan may run on
+    two streams, or in two graphs, at a time.
     """
     mixed, cut, batch_size, first, second = plan_info
     if not mixed:

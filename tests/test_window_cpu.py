@@ -91,3 +91,24 @@ def test_arguments_of_the_library():
         assert L.lib.msa_plan_device(ctypes.byref(a), None) == BAD, kw
         with pytest.raises(RuntimeError):
             _plan([1], [1], [0], 8, 2, 16, 4, 1, kw.get("window", 0), kw.get("sink_tokens", 0))
+
+
+def test_a_windowed_call_from_its_parameter_line():
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "msa-for-sail_b200", "benchmarks", "run_msa.py")
+    spec = importlib.util.spec_from_file_location("run_msa", path)
+    m = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(m)
+    for q, k, off, window, sinks in [(3, 500, 497, 100, 4), (200, 700, 500, 64, 30), (5, 5, 0, 3, 9), (4, 100, 300, 50, 2), (3, 10, -2, 4, 0), (2, 50, 0, 1, 0)]:
+        cfg = m.parse_format(f"[MSA] --format=seqlen_q:[{q}],seqlen_k:[{k}],qo_offset:[{off}],num_qo_heads:4,kv_block_num:0,window_size:{window},num_sink_tokens:{sinks}.")
+        assert cfg["window_size"] == window and m.parse_format(m.format_line(cfg)) == cfg
+        place = np.arange(q)[:, None] + off
+        j = np.arange(k)[None]
+        see = (j <= place) & ((j > place - window) | (j < sinks))
+        flops, nbytes = m.flops_and_bytes(cfg)
+        assert flops == 4 * 512 * int(see.sum())
+        # from the first query's window to the last query: one stretch of keys, and the sinks
+        lo, hi = max(0, off - window + 1), max(0, min(k, q + off))
+        assert nbytes == 2 * q * 4 * 128 * 2 + int(((j < hi) & ((j >= lo) | (j < sinks))).sum()) * 4 * 128 * 2 * 2
+    assert "window_size" not in m.format_line(m.parse_format("--format=seqlen_q:[2],seqlen_k:[256],num_qo_heads:4"))
