@@ -129,7 +129,13 @@ static int makespan(const std::vector<Proto>& protos, int groups, int chunk, int
 // included: 24 ragged sequences x 4 heads, at most 34 tiles: 60 us uncut, 40, 38 (three), 43, 41 (seven), 47; 128 items of 10 tiles, 64
 // rows: 23, 24, 26 us; 512 of 66: 316, 326, 331 us; 512 of 18 e4m3 tiles: 61, 69, 73 us; one sequence of 10 tiles x 2 heads: 15.7, 11.7, 11.0, 8.3 us
 // (five and ten).
-static int window_chunk(const std::vector<Proto>& protos, int groups, int max_tiles, int slots, int sms, int ceiling) {
+//
+// cluster > 1: a kernel whose CTAs share an uncut item, up to `cluster` of them with half a tile each at least, where all items are on the GPU at once
+// (nine tenths of the places: a cluster stays within a group of SMs).  It needs no merge; joining the states takes half a tile's time.  Uncut so and
+// cut: one sequence x 2 heads, 10 tiles 7.7 and 8.3 us; 16 x 2 x 9 tiles 9.4 and 10.3; 64 x 2 x 9 18.2 and 18.9; 32 x 2 x 33 28.1 and 29.2, but 4 x 2 x 33
+// 11.3 and 9.8, and 48 x 2 x 33 e4m3 ones, of which two CTAs an item fit and not three, 34 and 29. The call is a launch and an allocation less on the
+// host, 13 us instead of 18, for which such losses are taken.
+static int window_chunk(const std::vector<Proto>& protos, int groups, int max_tiles, int slots, int sms, int ceiling, int cluster) {
   constexpr int kPieceCost = 3, kMerge = 2;
   long long total = 0, items = 0;
   for (const Proto& pr : protos) { total += static_cast<long long>(pr.ntiles) * groups; items += groups; }
@@ -145,6 +151,11 @@ static int window_chunk(const std::vector<Proto>& protos, int groups, int max_ti
     const double ctas = makespan(protos, groups, chunk, slots, kPieceCost);
     const double cost = std::max(memory, ctas) + 0.15 * std::min(memory, ctas) + (s > 1 ? kMerge : 0);
     if (s == 1 || cost < best_cost) { best = chunk; best_cost = cost; }
+  }
+  const long long share = std::min<long long>({cluster, 2LL * max_tiles, items > 0 ? slots * 9LL / 10 / items : 0});
+  if (share > 1) {
+    const double ctas = static_cast<double>(max_tiles) / share + kPieceCost + 0.5;
+    if (std::max(memory, ctas) + 0.15 * std::min(memory, ctas) <= best_cost) best = std::max(1, max_tiles);
   }
   return best;
 }
@@ -181,7 +192,7 @@ extern "C" int msa_plan_dense(const MsaPlanArgs* a, MsaWorkItem* work, int32_t c
     chunk = std::max(1, (max_tiles + a->num_splits - 1) / a->num_splits);
   } else if (a->window > 0 && a->ctas_per_sm >= 0) {
     const int sms = a->num_sms > 0 ? a->num_sms : 148;
-    chunk = msa::window_chunk(protos, groups, max_tiles, sms * std::max(1, a->ctas_per_sm), sms, a->num_splits < 0 ? -a->num_splits : 128);
+    chunk = msa::window_chunk(protos, groups, max_tiles, sms * std::max(1, a->ctas_per_sm), sms, a->num_splits < 0 ? -a->num_splits : 128, a->cluster);
   } else {
     const long long items = static_cast<long long>(protos.size()) * groups;
     const int ceiling = a->num_splits < 0 ? -a->num_splits : 128;

@@ -13,6 +13,9 @@
 // keys, 4 KB each of K and V; unit n of an item is warp n % 4's.  It has a softmax of its own; the four states are joined at the end.
 // Units that no row sees are not loaded, so a window costs its keys and at most two units' edges.
 //
+// Where items are few, the CTAs of a cluster share one: unit n is warp n % (4 S)'s of S CTAs, and the S states of a row are joined through
+// distributed shared memory.  There are no partials in memory and no merge to launch.
+//
 // bf16: P is rounded to bf16 (2^-8), its sum is that of the unrounded weights.
 // e4m3: m16n8k32 on the bytes as they are (with K and V converted to f16 the conversions alone took 55 % of the ALU pipe, and an m16n8k16 of f16
 // takes 2.1 clocks an SM where an m16n8k32 of e4m3 takes 1.2).  Q and P are pairs of e4m3 values, hi + lo, both multiplied: 8 bits.  A query
@@ -20,6 +23,10 @@
 // a contraction is free: thread t of a group of four takes elements 32 t .. 32 t + 31 of its keys (K), thread group g elements 16 g .. 16 g + 15 of
 // the keys 2 t, 2 t + 8, 2 t + 1, 2 t + 9 (V; four bytes of a key each become four keys of an element by eight byte permutations),
 // which is the order that the transposed bytes of P come in.
+#include <cooperative_groups.h>
+
+#include <algorithm>
+
 #include "tc_ptx.cuh"
 
 namespace msa {
@@ -36,6 +43,7 @@ constexpr int kThreads = 32 * kWarps;
 constexpr int kHalf = 4096;                                  // K of a unit; V follows
 constexpr int kLdO = kHeadDim + 4;                           // floats of a row of O in shared memory
 constexpr float kNoMax = -3e38f;                             // maximum of a row that has seen no key
+constexpr int kMaxCluster = 16;
 
 template <bool F8>
 __host__ __device__ constexpr int unit_keys() { return F8 ? 32 : 16; }
@@ -48,7 +56,8 @@ struct Cfg {
   static constexpr int OFF_BAR = kWarps * STAGES * 2 * kHalf;        // [warp][stage] full
   static constexpr int OFF_FAC = OFF_BAR + kWarps * STAGES * 8;      // [8 NT] factor of a row's scores
   static constexpr int OFF_LIM = OFF_FAC + 32 * NT;                  // [8 NT] first key that a row does not see any more, first key of its window
-  static constexpr int OFF_FLAG = OFF_LIM + 64 * NT;                 // abort, skip
+                                                                     // (in the end, in a cluster: maximum - kPOffset, sum of the CTA's state)
+  static constexpr int OFF_FLAG = OFF_LIM + 64 * NT;                 // abort, skip, state is good
   // 32 rows: Q^T in shared memory, [step][8 rows][lane] x 8 bytes, or registers run out
   static constexpr bool Q_SHARED = NT == 4;
   static constexpr int OFF_Q = OFF_FLAG + 16;
@@ -94,6 +103,8 @@ window_decode_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_const
   unsigned char* smem = smem_raw + (smem_base - smem_u32(smem_raw));
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + OFF_FLAG);
   volatile int* skip_flag = abort_flag + 1;
+  const auto cluster = cooperative_groups::this_cluster();
+  const int S = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
   unsigned char* ring = smem + warp * kStages * 2 * kHalf;
   const uint32_t ring_u = smem_base + warp * kStages * 2 * kHalf, bars = smem_base + OFF_BAR + warp * kStages * 8;
@@ -107,7 +118,7 @@ window_decode_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_const
   }
 
   // ---------------- the item ----------------
-  const MsaWorkItem w = p.work[blockIdx.x];
+  const MsaWorkItem w = p.work[blockIdx.x / S];
   const int b = chk(w.batch, 0, p.batch, p.status), head0 = chk(w.head0, 0, p.num_qo_heads, p.status), split = chk(w.split, 0, p.num_splits, p.status);
   const int G = p.pack, kvh = head0 / (p.num_qo_heads / p.num_kv_heads);
   const int qo_base = p.qo_start[b], kv_len = p.kv_len[b], off = p.qo_offset[b];
@@ -126,9 +137,10 @@ window_decode_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_const
     begin = number(real_tile(w.kv_tile_begin) * (kKvTile / UK));
     end = number(min((real_tile(w.kv_tile_end - 1) + 1) * (kKvTile / UK), (end_key + UK - 1) / UK));
   }
-  begin += warp;                                             // this warp's: every fourth
-  const int n_units = end > begin ? (end - begin + kWarps - 1) / kWarps : 0;
-  auto key_of = [&](int i) { const int n = begin + kWarps * i; return (n < sink_u ? n : n + skip_u) * UK; };
+  const int step = kWarps * S;
+  begin += kWarps * rank + warp;                             // this warp's: every step-th
+  const int n_units = end > begin ? (end - begin + step - 1) / step : 0;
+  auto key_of = [&](int i) { const int n = begin + step * i; return (n < sink_u ? n : n + skip_u) * UK; };
 
   // ---------------- loads ----------------
   int phys = 0;                                              // lane i: page of this warp's unit 32 k + i
@@ -441,15 +453,18 @@ window_decode_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_const
       for (int d = 4; d < 32; d <<= 1) sums[n][c] += __shfl_xor_sync(0xffffffffu, sums[n][c], d);
   }
   __syncthreads();                                           // the rings are no longer read, and no copy is on its way (but after a timeout)
+  bool good = run;
   if (*abort_flag) {
     if (threadIdx.x == 0 && p.status) atomicExch(p.status, MSA_STATUS_TIMEOUT);
     outlast_async_work();
-    return;
+    good = false;
   }
-  if (!run || nrows <= 0) return;
+  if (nrows <= 0 || (S == 1 && !good)) return;               // (all CTAs of a cluster, or one without any)
   // ---------------- the four states of a row become one ----------------
   float* s_o = reinterpret_cast<float*>(smem);               // [warp][row][kLdO]
   float* s_m = s_o + kWarps * 8 * NT * kLdO;                 // [warp][row][2]: maximum - kPOffset, sum
+  float2* s_c = reinterpret_cast<float2*>(smem + OFF_LIM);
+  int* s_good = reinterpret_cast<int*>(smem + OFF_FLAG) + 2;
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -487,6 +502,12 @@ window_decode_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_const
 #pragma unroll
       for (int c = 0; c < 8; ++c) acc[c] += f * s_o[at * kLdO + 8 * c16 + c];
     }
+    if (S > 1) {                                             // in the place of warp 0's, which no other thread reads
+      *reinterpret_cast<float4*>(s_o + r * kLdO + 8 * c16) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+      *reinterpret_cast<float4*>(s_o + r * kLdO + 8 * c16 + 4) = make_float4(acc[4], acc[5], acc[6], acc[7]);
+      if (c16 == 0) s_c[r] = make_float2(top, sum);
+      continue;
+    }
     const int64_t tok = qo_base + r / G;
     const int head = head0 + r % G;
     const bool none = sum == 0.f;
@@ -506,6 +527,62 @@ window_decode_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_const
       if (p.lse && c16 == 0) p.lse[tok * p.num_qo_heads + head] = lse;
     }
   }
+  if (S == 1) return;
+  // ---------------- the S states of a row become one ----------------
+  if (threadIdx.x == 0) *s_good = good;
+  cluster.sync();
+  const int q = min(lane, S - 1);                            // lane q has what CTA q has of a row
+  if (__all_sync(0xffffffffu, *cluster.map_shared_rank(s_good, q) != 0)) {
+    for (int r = rank + S * warp; r < nrows; r += step) {
+      const float2 c = *cluster.map_shared_rank(s_c + r, q);
+      float top = c.x;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+      const float weight = exp2_fast(c.x - top);
+      float sum = lane < S ? weight * c.y : 0.f;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+      for (int i = 0; i < S; ++i) {
+        const float4 x = *cluster.map_shared_rank(reinterpret_cast<const float4*>(s_o + r * kLdO + 4 * lane), i);
+        const float f = __shfl_sync(0xffffffffu, weight, i);
+        acc.x = fmaf(f, x.x, acc.x); acc.y = fmaf(f, x.y, acc.y); acc.z = fmaf(f, x.z, acc.z); acc.w = fmaf(f, x.w, acc.w);
+      }
+      const int64_t tok = qo_base + r / G;
+      const int head = head0 + r % G;
+      const bool none = sum == 0.f;
+      const float f = none ? 0.f : (p.v_scale_head ? p.v_scale_head[kvh] : 1.f) * p.out_scale / sum;
+      *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.out) + tok * p.out_stride_tok + head * p.out_stride_head + 4 * lane) =
+          make_uint2(pack2<false>(acc.x * f, acc.y * f), pack2<false>(acc.z * f, acc.w * f));
+      if (p.lse && lane == 0) p.lse[tok * p.num_qo_heads + head] = none ? -INFINITY : (top + log2f(sum)) * kLn2;
+    }
+  }
+  cluster.sync();                                            // until nobody reads this CTA's memory
+}
+
+// CTAs that share an item: the most with which all items are on the GPU at once, and with a unit for each warp.
+template <int NT, bool F8>
+int cluster_of(const MsaFmhaParams& p, cudaLaunchConfig_t config, int device) {
+  if (p.partial_o || device < 0 || device >= 64) return 1;
+  static int fit[64][kMaxCluster + 1] = {};                  // clusters of a size that a device holds, + 1
+  const int64_t keys = static_cast<int64_t>(p.window) + p.sink_tokens + p.decode_rows / p.pack;
+  const int64_t most = std::min<int64_t>(kMaxCluster, (keys + kWarps * unit_keys<F8>() - 1) / (kWarps * unit_keys<F8>()));
+  for (int s = static_cast<int>(most); s > 1; --s) {
+    if (static_cast<int64_t>(p.num_work) * s > 148 * Cfg<NT>::CTAS) continue;
+    if (!fit[device][s]) {
+      cudaLaunchAttribute attr = {};
+      attr.id = cudaLaunchAttributeClusterDimension;
+      attr.val.clusterDim.x = s; attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+      config.gridDim = dim3(s);
+      config.attrs = &attr; config.numAttrs = 1;
+      int n = 0;
+      if (cudaOccupancyMaxActiveClusters(&n, window_decode_kernel<NT, F8>, &config) != cudaSuccess) { cudaGetLastError(); n = 0; }
+      fit[device][s] = n + 1;
+    }
+    if (p.num_work < fit[device][s]) return s;
+  }
+  return 1;
 }
 
 template <int NT, bool F8>
@@ -538,12 +615,22 @@ int launch(const MsaFmhaParams& p, cudaStream_t stream) {
   static bool ready[64] = {};
   if (device < 0 || device >= 64 || !ready[device]) {
     if (cudaFuncSetAttribute(window_decode_kernel<NT, F8>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<NT>::SMEM_BYTES) != cudaSuccess ||
-        cudaFuncSetAttribute(window_decode_kernel<NT, F8>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared) != cudaSuccess)
+        cudaFuncSetAttribute(window_decode_kernel<NT, F8>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared) != cudaSuccess ||
+        cudaFuncSetAttribute(window_decode_kernel<NT, F8>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
       return MSA_ERR_LAUNCH;
     if (device >= 0 && device < 64) ready[device] = true;
   }
-  window_decode_kernel<NT, F8><<<p.num_work, kThreads, Cfg<NT>::SMEM_BYTES, stream>>>(p, tk, tv);
-  return cudaGetLastError() == cudaSuccess ? MSA_OK : MSA_ERR_LAUNCH;
+  cudaLaunchConfig_t config = {};
+  config.blockDim = dim3(kThreads);
+  config.dynamicSmemBytes = Cfg<NT>::SMEM_BYTES;
+  config.stream = stream;
+  const int s = cluster_of<NT, F8>(p, config, device);
+  config.gridDim = dim3(static_cast<unsigned>(p.num_work) * s);
+  cudaLaunchAttribute attr = {};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = s; attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  if (s > 1) { config.attrs = &attr; config.numAttrs = 1; }
+  return cudaLaunchKernelEx(&config, window_decode_kernel<NT, F8>, p, tk, tv) == cudaSuccess ? MSA_OK : MSA_ERR_LAUNCH;
 }
 
 }  // namespace

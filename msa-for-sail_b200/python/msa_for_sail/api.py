@@ -467,12 +467,13 @@ def _fmha_sail_plan(
                 info["num_work_tc"] = n_tc
         # Two CTAs of the e4m3 decode kernel share an SM.  A cut at the average load may take more partials than a workspace
         # sized for the plain cut holds: such a workspace gets the plain cut.
-        # With a window two CTAs share an SM whatever the rows.
+        # With a window two CTAs share an SM whatever the rows, and few rows (of either type) over pages of whole units have clusters.
+        cluster = 16 if window[0] and pack == h_r and max_qo * pack <= 16 and (page_size <= 0 or page_size % 32 == 0) else 0
         shared = 2 if window[0] else 1 if max_qo * pack > 16 else (_kv4_ctas(max_qo * pack) if use_kv4_cache else (2 if use_fp8_kvcache else 1))
         for ctas in (shared, -1):
             args = _lib.MsaPlanArgs(
                 a_q.ctypes.data, a_k.ctypes.data, a_o.ctypes.data, batch, num_qo_heads, hkv, block_m, pack,
-                num_kv_splits if num_kv_splits >= 1 else -128, num_sms, ctas, *window)
+                num_kv_splits if num_kv_splits >= 1 else -128, num_sms, ctas, *window, cluster)
             cap = 1024
             spr = np.ones(max(1, total_q), np.int32)
             max_splits = _lib._i32(1)

@@ -29,7 +29,7 @@ class Case:
         g = torch.Generator(device=DEV).manual_seed(seed)
         self.ql, self.kl, self.hq, self.hk, self.window, self.sinks, self.page = ql, kl, hq, hk, window, sinks, page
         self.offsets = offsets
-        offs = [k - q for q, k in zip(ql, kl)] if offsets is None else offsets
+        offs = [k - q if offsets is None or offsets[i] < 0 else offsets[i] for i, (q, k) in enumerate(zip(ql, kl))]     # (negative: the default)
         self.places = [torch.arange(n) + o for n, o in zip(ql, offs)]
         self.q = _randn(g, q_dtype, sum(ql), hq, 128)
         self.scales = {}

@@ -192,3 +192,37 @@ def test_checked_build():
     r = subprocess.run([sys.executable, os.path.join(here, "checked_window_child.py")], capture_output=True, text=True, timeout=600,
                        env=dict(os.environ, MSA_BOUNDS_CHECK="1"))
     assert r.returncode == 0 and "CHECKED_WINDOW_OK" in r.stdout, r.stdout[-3000:] + "\n--- stderr ---\n" + r.stderr[-3000:]
+
+
+@pytest.mark.parametrize("batch,hk,page", [(1, 1, 128), (1, 2, 32), (3, 1, 0), (5, 4, 128), (24, 2, 128), (40, 4, 64), (148, 1, 128)])
+def test_few_items(batch, hk, page):
+    """Uncut items, which the CTAs of clusters share where they are few, and the same cut: one to 128 tiles, ends anywhere, rows that see nothing."""
+    import msa_for_sail as msa
+    layout = "hnd" if page else "ragged"
+    for i, (types, g, n, window, sinks) in enumerate([((BF, BF), 4, 1, 300, 5), ((E4, E4), 8, 2, 129, 0), ((BF, E4), 16, 1, 2500, 70), ((BF, BF), 16, 2, 1, 1), ((BF, BF), 1, 1, 16000, 0)]):
+        lens = [n + (37 * b * (b + i)) % (900 if batch > 8 else 4000) for b in range(batch)]
+        offs = [k - n for k in lens]
+        if batch > 2:
+            offs[1] = -n                                        # stands for the default
+            lens[2] = 0
+            offs[2] = 10
+        c = Case([n] * batch, lens, g * hk, hk, window, sinks, layout, page, *types, offsets=offs, seed=batch + i)
+        out = c.check(num_kv_splits=1)
+        c.check()
+        c.check(num_kv_splits=3)
+        assert torch.equal(c.check(num_kv_splits=1), out)
+
+
+def test_nothing_runs_while_a_status_is_set():
+    """The word says that a wait ran out: whole clusters and single CTAs return, and leave the output."""
+    from msa_for_sail import _lib, api
+    import msa_for_sail as msa
+    for batch in (1, 40):
+        for types in ((BF, BF), (BF, E4), (E4, E4)):
+            c = Case([1] * batch, [1500] * batch, 32, 4, 1000, 4, "hnd", 128, *types)
+            plan = c.plan(num_kv_splits=1)
+            out = torch.full((batch, 32, 128), 7.0, dtype=BF, device=DEV)
+            api._status_word(c.q.device).fill_(_lib.STATUS_TIMEOUT)
+            msa.fmha_sail(c.q, c.k, c.v, plan, kv_indices=c.table, out=out)
+            assert (out == 7).all() and api.last_status() == _lib.STATUS_TIMEOUT
+            c.check(plan=plan)
