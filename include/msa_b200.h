@@ -199,7 +199,8 @@ typedef struct MsaPlanArgs {
   int32_t window;             /* as in MsaFmhaParams: a row tile then has the tiles that its rows see, see kv_tile_skip */
   int32_t sink_tokens;
   int32_t cluster;            /* with a window, adaptive mode: CTAs that may share an uncut item at run time (16: at most 16 packed rows
-                               * over ragged keys or pages of a multiple of 32 keys; else 0); items stay uncut where that is as good */
+                               * over ragged keys or pages of a multiple of 32 keys; 2: at most 128 over pages of 128 keys, `pack`
+                               * dividing 128; else 0); items stay uncut where that is as good */
 } MsaPlanArgs;
 int msa_plan_dense(const MsaPlanArgs* args, MsaWorkItem* work, int32_t capacity,
                    int32_t* splits_per_row /* [total_q] host */,

@@ -124,11 +124,11 @@ static int makespan(const std::vector<Proto>& protos, int groups, int chunk, int
 }
 
 // Tiles of a piece of windowed decode.  Windows are short and alike, so that rounds of CTAs and the memory that all of them share decide.  In tile
-// times of a CTA that nothing holds up (1.6 us in bf16, 16 rows): a piece costs three beyond its own, a merge two, memory gives each SM a
-// tile in 0.9 (as if all were bf16), and of the two bounds a part of the smaller one shows as well.  Measured with 1 to 12 splits, merge
-// included: 24 ragged sequences x 4 heads, at most 34 tiles: 60 us uncut, 40, 38 (three), 43, 41 (seven), 47; 128 items of 10 tiles, 64
-// rows: 23, 24, 26 us; 512 of 66: 316, 326, 331 us; 512 of 18 e4m3 tiles: 61, 69, 73 us; one sequence of 10 tiles x 2 heads: 15.7, 11.7, 11.0, 8.3 us
-// (five and ten).
+// times of a CTA that nothing holds up (1.6 us in bf16, 16 rows; 1.4 times as much for more): a piece costs three beyond its own, a merge two and
+// the partials' way to memory and back, memory gives each SM a tile in 0.9 (as if all were bf16), and of the two bounds a part of the
+// smaller one shows as well.  Measured with 1 to 12 splits, merge included: 24 ragged sequences x 4 heads, at most 34 tiles: 60 us uncut, 40, 38
+// (three), 43, 41 (seven), 47; 128 items of 10 tiles, 64 rows: 23, 24, 27 us; 512 of 66: 316, 326, 331 us; 512 of 18 e4m3 tiles: 61, 69, 73 us; one
+// sequence of 10 tiles x 2 heads: 15.7, 11.7, 11.0, 8.3 us (five and ten).
 //
 // cluster > 1: a kernel whose CTAs share an uncut item, up to `cluster` of them with half a tile each at least, where all items are on the GPU at once
 // (nine tenths of the places: a cluster stays within a group of SMs).  It needs no merge; joining the states takes half a tile's time.  Uncut so and
@@ -139,7 +139,10 @@ static int window_chunk(const std::vector<Proto>& protos, int groups, int max_ti
   constexpr int kPieceCost = 3, kMerge = 2;
   long long total = 0, items = 0;
   for (const Proto& pr : protos) { total += static_cast<long long>(pr.ntiles) * groups; items += groups; }
-  const double memory = 0.9 * static_cast<double>(total) / sms + kPieceCost;
+  long long rows = 0;                                        // of partials, 0.5 KB each: 8 MB in a tile's time
+  bool many = false;
+  for (const Proto& pr : protos) { rows += static_cast<long long>(pr.nrows) * groups; many = many || pr.nrows > 16; }
+  const double memory = 0.9 * static_cast<double>(total) / sms + kPieceCost, slow = many ? 1.4 : 1.0, merge_row = 1024 / 8e6;
   int best = std::max(1, max_tiles);
   if (items >= 8LL * slots) return best;
   double best_cost = 0;
@@ -148,13 +151,13 @@ static int window_chunk(const std::vector<Proto>& protos, int groups, int max_ti
     const int chunk = (max_tiles + s - 1) / s;
     if (chunk == last || (s > 1 && items * s > 16LL * slots)) continue;
     last = chunk;
-    const double ctas = makespan(protos, groups, chunk, slots, kPieceCost);
-    const double cost = std::max(memory, ctas) + 0.15 * std::min(memory, ctas) + (s > 1 ? kMerge : 0);
+    const double ctas = slow * makespan(protos, groups, chunk, slots, kPieceCost);
+    const double cost = std::max(memory, ctas) + 0.15 * std::min(memory, ctas) + (s > 1 ? kMerge + merge_row * s * rows : 0);
     if (s == 1 || cost < best_cost) { best = chunk; best_cost = cost; }
   }
   const long long share = std::min<long long>({cluster, 2LL * max_tiles, items > 0 ? slots * 9LL / 10 / items : 0});
   if (share > 1) {
-    const double ctas = static_cast<double>(max_tiles) / share + kPieceCost + 0.5;
+    const double ctas = slow * (static_cast<double>(max_tiles) / share + kPieceCost + 0.5);
     if (std::max(memory, ctas) + 0.15 * std::min(memory, ctas) <= best_cost) best = std::max(1, max_tiles);
   }
   return best;

@@ -21,6 +21,9 @@
 //
 // Output: normalised partial O (fp32) + natural-log LSE per split, or the final bf16 O when the
 // work item is unsplit.  Every wait is bounded (tc_ptx.cuh).
+#include <cooperative_groups.h>
+
+#include <algorithm>
 #include <cstdio>
 
 #include "tc_ptx.cuh"
@@ -169,6 +172,10 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
   const int G = p.pack;
   const int h_r = p.num_qo_heads / p.num_kv_heads;
 
+  // windowed: the CTAs of a cluster take a share of an uncut item's pages each, and join the rows' states in the end
+  [[maybe_unused]] const auto cluster = cooperative_groups::this_cluster();
+  const int S = WIN ? static_cast<int>(cluster.num_blocks()) : 1, rank = WIN ? static_cast<int>(cluster.block_rank()) : 0;
+
   chain_begin();
   // ---------------- work item ----------------
   int b, head0, tb, te, split, i_base, ntok;
@@ -176,11 +183,16 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
   int blk_first = -1;                       // sparse: this lane's entry of the selected-page list, fetched early
   const int32_t* blocks = nullptr;
   if (!sparse) {
-    const MsaWorkItem w = p.work[blockIdx.x];
+    const MsaWorkItem w = p.work[blockIdx.x / S];
     b = chk(w.batch, 0, p.batch, p.status); head0 = chk(w.head0, 0, p.num_qo_heads, p.status);
     tb = w.kv_tile_begin; te = w.kv_tile_end; split = chk(w.split, 0, p.num_splits, p.status);
     i_base = 0;
-    if constexpr (WIN) skip = w.kv_tile_skip;
+    if constexpr (WIN) {
+      skip = w.kv_tile_skip;
+      const int share = (te - tb + S - 1) / S;
+      tb = min(te, tb + rank * share);
+      te = min(te, tb + share);
+    }
     // (lengths on the device may outgrow the rows that the plan and this kernel's tile were made for; G divides 128)
     ntok = min(p.qo_start[b + 1] - p.qo_start[b], p.decode_rows >> (__ffs(G) - 1));
   } else {
@@ -296,6 +308,59 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
   // of the window, the last.
   [[maybe_unused]] auto has_unseen = [&](int key0) -> bool {
     return key0 + TK > end_key || (key0 < first_key && key0 + TK > p.sink_tokens);
+  };
+
+  // windowed: the states of a row, PARTS of them in each CTA of the cluster, become one.  Rows first, first + step, ..; 16 threads a row, t has columns
+  // 4 t and 64 + 4 t.  Chunks of 16 bytes are turned by the row, so that neither side has bank conflicts.
+  [[maybe_unused]] float* stage = reinterpret_cast<float*>(smem_gen + OFF_K);          // [BM][kHeadDim]
+  [[maybe_unused]] float* st_m = reinterpret_cast<float*>(smem_gen + OFF_Q);           // [BM] maxima, [BM] sums
+  [[maybe_unused]] auto join = [&](int first, int step, int t) {
+    if constexpr (WIN) {
+      const float vsh = p.v_scale_head ? p.v_scale_head[kvh] : 1.f;
+      const bool to_partial = p.partial_o != nullptr;
+      for (int rr = first; rr < nrows; rr += step) {
+        float M = -INFINITY, L = 0.f, acc[8] = {};
+        for (int c = 0; c < S; ++c) {
+          const float* m_of = cluster.map_shared_rank(st_m, c);
+#pragma unroll
+          for (int q = 0; q < PARTS; ++q) M = fmaxf(M, m_of[q * ROWS + rr]);
+        }
+        for (int c = 0; c < S; ++c) {
+          const float *m_of = cluster.map_shared_rank(st_m, c), *o_of = cluster.map_shared_rank(stage, c);
+#pragma unroll
+          for (int q = 0; q < PARTS; ++q) {
+            const int row = q * ROWS + rr;
+            const float mq = m_of[row], w = mq == -INFINITY ? 0.f : exp2_fast(mq - M);     // a part that saw no key has weight 0 and O == 0
+            L = fmaf(m_of[BM + row], w, L);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float4 a = *reinterpret_cast<const float4*>(o_of + row * kHeadDim + 4 * ((16 * h + t) ^ (row & 7)));
+              acc[4 * h] = fmaf(a.x, w, acc[4 * h]); acc[4 * h + 1] = fmaf(a.y, w, acc[4 * h + 1]);
+              acc[4 * h + 2] = fmaf(a.z, w, acc[4 * h + 2]); acc[4 * h + 3] = fmaf(a.w, w, acc[4 * h + 3]);
+            }
+          }
+        }
+        const float inv = L > 0.f ? __fdividef(to_partial ? vsh : p.out_scale * vsh, L) : 0.f;
+        const int gt = qo_base + i_base + rr / G, hd = head0 + rr % G;
+        const float lse = L > 0.f ? (M - kPOffset) * kLn2 + __logf(L) : -INFINITY;   // l carries 2^kPOffset
+        const int64_t prow = (static_cast<int64_t>(split) * p.total_q + gt) * p.num_qo_heads + hd;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float a0 = acc[4 * h] * inv, a1 = acc[4 * h + 1] * inv, a2 = acc[4 * h + 2] * inv, a3 = acc[4 * h + 3] * inv;
+          const int col = 64 * h + 4 * t;
+          if (to_partial) {
+            *reinterpret_cast<float4*>(p.partial_o + prow * kHeadDim + col) = make_float4(a0, a1, a2, a3);
+          } else if (p.out) {
+            *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.out) + static_cast<int64_t>(gt) * p.out_stride_tok +
+                                      static_cast<int64_t>(hd) * p.out_stride_head + col) = make_uint2(pack2<false>(a0, a1), pack2<false>(a2, a3));
+          }
+        }
+        if (t == 0) {
+          if (to_partial) p.partial_lse[prow] = lse;
+          else if (p.lse) p.lse[static_cast<int64_t>(gt) * p.num_qo_heads + hd] = lse;
+        }
+      }
+    }
   };
 
   const bool run = *skip_flag == 0;
@@ -972,11 +1037,7 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
       }
       if (trace) trace[12] = clock64() - clk0;
     } else if constexpr (WIN) {
-      // Every MMA and every TMA load of this CTA has completed: the rings are free to stage the rows' results, all parts, and Q the maxima and
-      // sums.  Chunks of 16 bytes are turned by the row, so that neither side has bank conflicts.
-      float* stage = reinterpret_cast<float*>(smem_gen + OFF_K);              // [BM][kHeadDim]
-      float* st_m = reinterpret_cast<float*>(smem_gen + OFF_Q);               // [BM]
-      float* st_l = st_m + BM;
+      // Every MMA and every TMA load of this CTA has completed: the rings are free to stage the rows' results, all parts, and Q the maxima and sums.
       if (alive) {
         tc_fence_after();
 #pragma unroll
@@ -995,51 +1056,12 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
               *reinterpret_cast<uint4*>(stage + trow * kHeadDim + 4 * ((8 * c + e) ^ (trow & 7))) = make_uint4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
           }
         }
-        st_m[trow] = m_used; st_l[trow] = l_sum;
+        st_m[trow] = m_used; st_m[BM + trow] = l_sum;
       }
-      asm volatile("bar.sync 1, %0;" ::"r"(32 * n_active_warps) : "memory");
-      if (*abort_flag == 0) {
-        // thread -> (row, columns 4 t and 64 + 4 t): 16 threads a row
-        const float vsh = p.v_scale_head ? p.v_scale_head[kvh] : 1.f;
-        const bool to_partial = p.partial_o != nullptr;
-        const int nth = (PARTS == 4 ? warp : ROWS == 64 ? (warp >> 1) * ((nrows + 31) / 32) + (warp & 1) : warp) * 32 + lane, t = nth & 15;
-        for (int rr = nth >> 4; rr < nrows; rr += 2 * n_active_warps) {
-          float mq[PARTS], M = -INFINITY, L = 0.f;
-#pragma unroll
-          for (int q = 0; q < PARTS; ++q) { mq[q] = st_m[q * ROWS + rr]; M = fmaxf(M, mq[q]); }
-          float wq[PARTS];
-#pragma unroll
-          for (int q = 0; q < PARTS; ++q) {
-            wq[q] = mq[q] == -INFINITY ? 0.f : exp2_fast(mq[q] - M);
-            L += st_l[q * ROWS + rr] * wq[q];
-          }
-          const float inv = L > 0.f ? __fdividef(to_partial ? vsh : p.out_scale * vsh, L) : 0.f;
-          const int gt = qo_base + i_base + rr / G, hd = head0 + rr % G;
-          const float lse = L > 0.f ? (M - kPOffset) * kLn2 + __logf(L) : -INFINITY;   // l carries 2^kPOffset
-          const int64_t prow = (static_cast<int64_t>(split) * p.total_q + gt) * p.num_qo_heads + hd;
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            float acc[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int q = 0; q < PARTS; ++q) {
-              const int row = q * ROWS + rr;
-              const float4 a = *reinterpret_cast<const float4*>(stage + row * kHeadDim + 4 * ((16 * h + t) ^ (row & 7)));
-              const float w = wq[q] * inv;                    // a part that saw no key has weight 0 and O == 0
-              acc[0] = fmaf(a.x, w, acc[0]); acc[1] = fmaf(a.y, w, acc[1]); acc[2] = fmaf(a.z, w, acc[2]); acc[3] = fmaf(a.w, w, acc[3]);
-            }
-            const int col = 64 * h + 4 * t;
-            if (to_partial) {
-              *reinterpret_cast<float4*>(p.partial_o + prow * kHeadDim + col) = make_float4(acc[0], acc[1], acc[2], acc[3]);
-            } else if (p.out) {
-              *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.out) + static_cast<int64_t>(gt) * p.out_stride_tok +
-                                        static_cast<int64_t>(hd) * p.out_stride_head + col) = make_uint2(pack2<false>(acc[0], acc[1]), pack2<false>(acc[2], acc[3]));
-            }
-          }
-          if (t == 0) {
-            if (to_partial) p.partial_lse[prow] = lse;
-            else if (p.lse) p.lse[static_cast<int64_t>(gt) * p.num_qo_heads + hd] = lse;
-          }
-        }
+      if (S == 1) {
+        asm volatile("bar.sync 1, %0;" ::"r"(32 * n_active_warps) : "memory");
+        const int nth = (PARTS == 4 ? warp : ROWS == 64 ? (warp >> 1) * ((nrows + 31) / 32) + (warp & 1) : warp) * 32 + lane;
+        if (*abort_flag == 0) join(nth >> 4, 2 * n_active_warps, nth & 15);
       }
     } else
     if (alive && has_o) {
@@ -1084,6 +1106,20 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
         if (to_partial) p.partial_lse[prow] = lse;
         else if (p.lse) p.lse[static_cast<int64_t>(gtok) * p.num_qo_heads + head] = lse;
       }
+    }
+  }
+
+  if constexpr (WIN) {
+    if (S > 1) {
+      __syncthreads();
+      cluster.sync();
+      bool good = true;                                      // no wait of the cluster ran out, and all of it ran
+      for (int c = 0; c < S; ++c) {
+        const volatile int* flags = cluster.map_shared_rank(const_cast<int*>(abort_flag), c);
+        good = good && flags[0] == 0 && flags[1] == 0;
+      }
+      if (good) join((threadIdx.x >> 4) * S + rank, NTHREADS / 16 * S, threadIdx.x & 15);
+      cluster.sync();                                        // until nobody reads this CTA's memory
     }
   }
 
@@ -1185,7 +1221,16 @@ int fmha_decode_tc_launch(const MsaFmhaParams& p, cudaStream_t stream) {
       cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
     if (dev < 16) attr_done[dev][variant] = true;
   }
-  return launch_chained(kern, static_cast<unsigned>(grid64), NTHREADS, smem, stream, p, tq, tk, tv) == cudaSuccess ? MSA_OK : MSA_ERR_LAUNCH;
+  // windowed: two CTAs to an uncut item where all items are on the GPU at once so, in nine tenths of the places (a cluster stays within a group of
+  // SMs).  64 sequences x 2 heads, 17 tiles, 64 bf16 rows 34 us, cut in two and merged 38; 128 e4m3 rows 44 and 50.  More than two lose to a cut
+  // and its merge: 16 x 2 x 5 tiles, 32 e4m3 rows 20 us with eight, 14 with three pieces.
+  int cluster = 1;
+  if (p.window > 0 && !p.partial_o) {
+    const int64_t pages = (static_cast<int64_t>(p.window) + p.decode_rows / p.pack) / BN + p.sink_tokens / BN + 1;
+    cluster = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({2, pages, 2 * 148 * 9 / 10 / grid64})));
+  }
+  return launch_chained_clusters(kern, static_cast<unsigned>(cluster), static_cast<unsigned>(grid64 * cluster), NTHREADS, smem, stream, p, tq, tk, tv) == cudaSuccess
+             ? MSA_OK : MSA_ERR_LAUNCH;
 }
 
 // CTAs of one decode-kernel variant that fit an SM (what the occupancy calculator reports).

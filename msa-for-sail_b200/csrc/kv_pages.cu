@@ -138,26 +138,14 @@ __device__ __forceinline__ T block_scan(T x, T* s_sum, T& total) {
   return before + incl - x;
 }
 
-// One cluster, chained as launch_chained() does.
+// One cluster.
 template <typename... P, typename... A>
 cudaError_t launch_cluster(void (*kernel)(P...), int ctas, int threads, cudaStream_t stream, A&&... args) {
-  if (ctas == 1) return launch_chained(kernel, 1, threads, 0, stream, args...);
   if (ctas > 8) {                              // more than every device of the architecture has to take
     const cudaError_t rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (rc != cudaSuccess) return rc;
   }
-  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
-  cudaStreamIsCapturing(stream, &capture);
-  cudaLaunchAttribute attr[2] = {};
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = capture == cudaStreamCaptureStatusNone ? 1 : 0;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = static_cast<unsigned>(ctas);
-  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(ctas)); cfg.blockDim = dim3(static_cast<unsigned>(threads)); cfg.stream = stream;
-  cfg.attrs = attr; cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, kernel, P(args)...);
+  return launch_chained_clusters(kernel, static_cast<unsigned>(ctas), ctas, threads, 0, stream, args...);
 }
 
 __device__ __forceinline__ int stack_size(const int32_t* num_free, int capacity) { return min(max(__ldcg(num_free), 0), capacity); }

@@ -467,8 +467,14 @@ def _fmha_sail_plan(
                 info["num_work_tc"] = n_tc
         # Two CTAs of the e4m3 decode kernel share an SM.  A cut at the average load may take more partials than a workspace
         # sized for the plain cut holds: such a workspace gets the plain cut.
-        # With a window two CTAs share an SM whatever the rows, and few rows (of either type) over pages of whole units have clusters.
-        cluster = 16 if window[0] and pack == h_r and max_qo * pack <= 16 and (page_size <= 0 or page_size % 32 == 0) else 0
+        # With a window two CTAs share an SM whatever the rows, and clusters share an item: of few rows (whatever the cache's type) over
+        # pages of whole units, of up to 128 rows over pages of 128 keys (pairs).
+        cluster = 0
+        if window[0] and pack == h_r:
+            if max_qo * pack <= 16 and (page_size <= 0 or page_size % 32 == 0):
+                cluster = 16
+            elif max_qo * pack <= 128 and page_size == KV_TILE and 128 % pack == 0:
+                cluster = 2
         shared = 2 if window[0] else 1 if max_qo * pack > 16 else (_kv4_ctas(max_qo * pack) if use_kv4_cache else (2 if use_fp8_kvcache else 1))
         for ctas in (shared, -1):
             args = _lib.MsaPlanArgs(
