@@ -1067,6 +1067,7 @@ _WINDOW_OUT = (torch.bfloat16, torch.float32)
 _WINDOW_HEAD = struct.Struct("@7Q")           # the arguments' first fields: q, k, v, out, lse, max_score, partial_o
 _WINDOW_TABLES = struct.Struct("@6Q")         # qo_start, kv_start, kv_len, qo_offset, kv_page_indptr, kv_indices
 _WINDOW_STRIDES = struct.Struct("@10q")       # q, k, v, out
+_WINDOW_TABLES_AT, _WINDOW_STRIDES_AT = _lib.MsaFmhaParams.qo_start.offset, _lib.MsaFmhaParams.q_stride_tok.offset
 
 
 def _window_params(q_dtype, kv_dtype, plan):
@@ -1180,10 +1181,10 @@ def _fmha_sail_window(q, k, v, plan, kv_indices, kv_block_indexes, q_offset_over
         if o_stride is None:
             o_stride = (num_qo_heads * 128, 128)
         _WINDOW_HEAD.pack_into(p, 0, q.data_ptr(), k.data_ptr(), v.data_ptr(), kernel_out.data_ptr(), 0 if lse is None else lse.data_ptr(), 0, part)
-        _WINDOW_TABLES.pack_into(p, _lib.MsaFmhaParams.qo_start.offset, plan["qo_segment_offsets"].data_ptr(), plan["kv_segment_offsets"].data_ptr(),
+        _WINDOW_TABLES.pack_into(p, _WINDOW_TABLES_AT, plan["qo_segment_offsets"].data_ptr(), plan["kv_segment_offsets"].data_ptr(),
                                  plan["kv_segment_lens"].data_ptr(), plan["qo_offset"].data_ptr(), plan["kv_page_indptr"].data_ptr() if paged else 0,
                                  kv_indices.data_ptr() if paged else 0)
-        _WINDOW_STRIDES.pack_into(p, _lib.MsaFmhaParams.q_stride_tok.offset, *strides, o_stride[0], o_stride[1])
+        _WINDOW_STRIDES.pack_into(p, _WINDOW_STRIDES_AT, *strides, o_stride[0], o_stride[1])
         p.total_q, p.kv_extent, p.status = nnz_qo, k_shape[0], _status_ptr(dev)
         p.work = None if work is None else work.data_ptr()
         p.sm_scale, p.out_scale = scale, out_scale

@@ -88,6 +88,13 @@ def _cache_list(caches, num_pages, page_size, device, by_token=False):
     return b"".join(packed), len(packed), num_pages
 
 
+@functools.lru_cache(maxsize=256)
+def _workspace(name, *sizes):
+    """int32 entries of the workspace of a call of these sizes."""
+    name = f"msa_pages_{name}_workspace_bytes"
+    return _lib.check(getattr(_lib.lib, name)(*sizes), name) // 4
+
+
 def _address(packed):
     """Where the bytes are, while `packed` lives."""
     return ctypes.cast(packed, ctypes.c_void_p).value
@@ -161,8 +168,7 @@ def kv_pages_fork(block_table: torch.Tensor, num_held: torch.Tensor, kv_lens: to
     dev, B, width, stride = _tables(block_table, page_size, {"num_held": num_held, "kv_lens": kv_lens}, {
         "parents": (parents, n), "children": (children, n), "free_pages": (free_pages, None), "num_free": (num_free, 1), "shares": (shares, None)})
     packed, num, pages = _cache_list(caches, shares.shape[0], page_size, dev, True)
-    ws = _lib.check(_lib.lib.msa_pages_fork_workspace_bytes(B, n), "msa_pages_fork_workspace_bytes") // 4
-    buf = torch.empty(ws + 1, dtype=torch.int32, device=dev)
+    buf = torch.empty(_workspace("fork", B, n) + 1, dtype=torch.int32, device=dev)
     ptr = buf.data_ptr()
     _launch(dev, _lib.lib.msa_pages_fork, _lib.pages_fork_args(
         _address(packed), block_table.data_ptr(), num_held.data_ptr(), kv_lens.data_ptr(), parents.data_ptr(), children.data_ptr(),
@@ -194,8 +200,7 @@ def kv_pages_free(block_table: torch.Tensor, num_held: torch.Tensor, kv_lens: to
         raise ValueError(f"window_size must be -1 (no window) or from 1 to 2^31 - 1, got {window_size}")
     if not 0 <= num_sink_tokens <= (1 << 31) - 1:
         raise ValueError(f"num_sink_tokens must be from 0 to 2^31 - 1, got {num_sink_tokens}")
-    ws = _lib.check(_lib.lib.msa_pages_free_workspace_bytes(B, width), "msa_pages_free_workspace_bytes") // 4
-    buf = torch.empty(ws + 1, dtype=torch.int32, device=dev)
+    buf = torch.empty(_workspace("free", B, width) + 1, dtype=torch.int32, device=dev)
     ptr = buf.data_ptr()
     _launch(dev, _lib.lib.msa_pages_free, _lib.pages_free_args(
         block_table.data_ptr(), num_held.data_ptr(), kv_lens.data_ptr(), free_pages.data_ptr(), num_free.data_ptr(), 0 if shares is None else shares.data_ptr(),
@@ -230,7 +235,7 @@ def kv_pages_compact(block_table: torch.Tensor, num_held: torch.Tensor, free_pag
     packed, num, num_pages = _cache_list(caches, num_pages, 1, dev)
     if num_pages is None or not 0 <= num_pages <= (1 << 31) - 1:
         raise ValueError("num_pages is needed where there are neither caches nor shares" if num_pages is None else f"num_pages={num_pages} must fit int32")
-    ws = _lib.check(_lib.lib.msa_pages_compact_workspace_bytes(num_pages), "msa_pages_compact_workspace_bytes") // 4
+    ws = _workspace("compact", num_pages)
     src, dst, num_moved, ws = torch.empty(2 * num_pages + 1 + ws, dtype=torch.int32, device=dev).split_with_sizes([num_pages, num_pages, 1, ws])
     _launch(dev, _lib.lib.msa_pages_compact, _lib.pages_compact_args(
         _address(packed), block_table.data_ptr(), num_held.data_ptr(), free_pages.data_ptr(), num_free.data_ptr(),
