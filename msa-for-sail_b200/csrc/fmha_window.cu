@@ -143,23 +143,30 @@ window_decode_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_const
   auto key_of = [&](int i) { const int n = begin + step * i; return (n < sink_u ? n : n + skip_u) * UK; };
 
   // ---------------- loads ----------------
-  int phys = 0;                                              // lane i: page of this warp's unit 32 k + i
-  auto load_pages = [&](int i0) { phys = paged && i0 + lane < n_units ? page_entry(p, kv0 + key_of(i0 + lane) / p.page_size) : 0; };
+  int phys = 0, row = 0;                                     // lane i: where this warp's unit 32 k + i is, its page and its first row there
+  auto load_pages = [&](int i0) {
+    if (i0 + lane >= n_units) return;
+    const int key0 = key_of(i0 + lane);
+    row = kv0 + key0;
+    if (paged) {
+      const int c = key0 / p.page_size;
+      phys = page_entry(p, kv0 + c);
+      row = key0 - c * p.page_size;
+    }
+  };
   auto fetch = [&](int i, int stage) {                       // unit i into a stage that no lane reads any more
-    if ((i & 31) == 0) load_pages(i);
-    const int page = __shfl_sync(0xffffffffu, phys, i & 31), key0 = key_of(i);
+    if ((i & 31) == 0) { load_pages(i); __syncwarp(); }
+    const int page = __shfl_sync(0xffffffffu, phys, i & 31), first = __shfl_sync(0xffffffffu, row, i & 31);
     if (elect_one()) {
       const uint32_t bar = bars + 8 * stage, dst = ring_u + stage * 2 * kHalf;
       mbar_arrive_expect_tx(bar, 2 * kHalf);
-#pragma unroll
-      for (int h = 0; h < (F8 ? 1 : 2); ++h) {
-        if (paged) {
-          tma_load_4d(dst + h * SUB, &tm_k, bar, 64 * h, key0 % p.page_size, kvh, page);
-          tma_load_4d(dst + kHalf + h * SUB, &tm_v, bar, 64 * h, key0 % p.page_size, kvh, page);
-        } else {
-          tma_load_3d(dst + h * SUB, &tm_k, bar, 64 * h, kvh, kv0 + key0);
-          tma_load_3d(dst + kHalf + h * SUB, &tm_v, bar, 64 * h, kvh, kv0 + key0);
-        }
+      // (both halves of head_dim in one copy: its tensor has them as a dimension)
+      if (paged) {
+        tma_load_5d(dst, &tm_k, bar, 0, first, 0, kvh, page);
+        tma_load_5d(dst + kHalf, &tm_v, bar, 0, first, 0, kvh, page);
+      } else {
+        tma_load_4d(dst, &tm_k, bar, 0, first, 0, kvh);
+        tma_load_4d(dst + kHalf, &tm_v, bar, 0, first, 0, kvh);
       }
     }
     __syncwarp();
@@ -594,19 +601,19 @@ int launch(const MsaFmhaParams& p, cudaStream_t stream) {
     const void* base = i ? p.v : p.k;
     const uint64_t tok = (i ? p.v_stride_tok : p.k_stride_tok) * e, head = (i ? p.v_stride_head : p.k_stride_head) * e,
                    page = (i ? p.v_stride_page : p.k_stride_page) * e;
-    const uint32_t cols = F8 ? 128 : 64;
+    const uint32_t cols = F8 ? 128 : 64, halves = F8 ? 1 : 2;          // of head_dim: 128 bytes each, a swizzled tile of its own
     const auto make = F8 ? make_tma_map_u8 : make_tma_map_bf16;
     int rc;
     if (p.page_size > 0) {
-      const uint64_t dims[4] = {128, static_cast<uint64_t>(p.page_size), static_cast<uint64_t>(p.num_kv_heads), static_cast<uint64_t>(p.kv_extent)};
-      const uint64_t str[3] = {tok, head, page};
-      const uint32_t box[4] = {cols, UK, 1, 1};
-      rc = make(i ? &tv : &tk, base, 4, dims, str, box);
+      const uint64_t dims[5] = {cols, static_cast<uint64_t>(p.page_size), halves, static_cast<uint64_t>(p.num_kv_heads), static_cast<uint64_t>(p.kv_extent)};
+      const uint64_t str[4] = {tok, 128, head, page};
+      const uint32_t box[5] = {cols, UK, halves, 1, 1};
+      rc = make(i ? &tv : &tk, base, 5, dims, str, box);
     } else {
-      const uint64_t dims[3] = {128, static_cast<uint64_t>(p.num_kv_heads), static_cast<uint64_t>(p.kv_extent)};
-      const uint64_t str[2] = {head, tok};
-      const uint32_t box[3] = {cols, 1, UK};
-      rc = make(i ? &tv : &tk, base, 3, dims, str, box);
+      const uint64_t dims[4] = {cols, static_cast<uint64_t>(p.kv_extent), halves, static_cast<uint64_t>(p.num_kv_heads)};
+      const uint64_t str[3] = {tok, 128, head};
+      const uint32_t box[4] = {cols, UK, halves, 1};
+      rc = make(i ? &tv : &tk, base, 4, dims, str, box);
     }
     if (rc != MSA_OK) return MSA_ERR_LAUNCH;
   }
