@@ -303,12 +303,13 @@ __device__ __forceinline__ void push(const MsaPagesFreeArgs& a, int page, int pl
 }
 
 // Tables of up to 2^18 entries: the CTAs of one cluster, K entries a thread that stay in registers from step to step; between the steps are
-// barriers of the cluster.  (8 rows of 257 pages: 5.2 us, 8.3 in launches of their own.  512 rows that share pages: 22 us in a captured graph
+// barriers of the cluster.  (8 rows of 257 pages: 5.2 us, 8.3 in launches of their own.  512 rows that share pages: 20.5 us in a captured graph
 // against 17.5, but 27 a call against 36, whose launches the host cannot keep up with.)
 constexpr int kClusterCtas = 16;
 
 template <int K>
-__global__ void __launch_bounds__(kScanThreads) pages_free_cluster_kernel(const MsaPagesFreeArgs a) {
+__global__ void __launch_bounds__(kScanThreads) pages_free_cluster_kernel(const MsaPagesFreeArgs a, const int span) {
+  // span: entries of a thread, at most K
   chain_begin();
   auto cluster = cooperative_groups::this_cluster();
   __shared__ int s_sum[32];
@@ -317,11 +318,11 @@ __global__ void __launch_bounds__(kScanThreads) pages_free_cluster_kernel(const 
   __shared__ Kept s_kept[kScanThreads];        // of the rows that this CTA has entries of
   const int ctas = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int entries = a.batch * a.table_width, e0 = rank * K * kScanThreads + tid;
+  const int entries = a.batch * a.table_width, e0 = rank * span * kScanThreads + tid;
   const int num_free = stack_size(a.num_free, a.free_capacity);
   // (the divisions of a row's limits, made for each entry, would take longest of all)
   const int row0 = min(e0 - tid, entries) / max(a.table_width, 1);
-  const bool few_rows = K * kScanThreads / max(a.table_width, 1) + 2 <= kScanThreads;
+  const bool few_rows = span * kScanThreads / max(a.table_width, 1) + 2 <= kScanThreads;
   if (few_rows && row0 + tid < a.batch) s_kept[tid] = kept_of(a, row0 + tid);
   __syncthreads();
   int page[K];
@@ -330,7 +331,7 @@ __global__ void __launch_bounds__(kScanThreads) pages_free_cluster_kernel(const 
   for (int k = 0; k < K; ++k) {
     const int e = e0 + k * kScanThreads;
     page[k] = -1;
-    if (e < entries) {
+    if (k < span && e < entries) {
       const int b = e / a.table_width, col = e - b * a.table_width;
       if (given_back(few_rows ? s_kept[b - row0] : kept_of(a, b), col)) {
         back |= 1u << k;
@@ -788,9 +789,10 @@ extern "C" int msa_pages_free(const MsaPagesFreeArgs* pa, msa_stream_t stream) {
   if (entries <= 16 * kClusterCtas * kScanThreads) {
     const int k = entries <= kClusterCtas * kScanThreads ? 1 : entries <= 4 * kClusterCtas * kScanThreads ? 4 : 16;
     int ctas = 1;
-    while (static_cast<int64_t>(ctas) * k * kScanThreads < entries) ctas *= 2;
+    while (ctas < kClusterCtas && static_cast<int64_t>(ctas) * kScanThreads < entries) ctas *= 2;
+    const int span = static_cast<int>((entries + ctas * kScanThreads - 1) / (ctas * kScanThreads));
     const auto kernel = k == 1 ? pages_free_cluster_kernel<1> : k == 4 ? pages_free_cluster_kernel<4> : pages_free_cluster_kernel<16>;
-    return launch_cluster(kernel, ctas, kScanThreads, st, a) == cudaSuccess ? MSA_OK : MSA_ERR_LAUNCH;
+    return launch_cluster(kernel, ctas, kScanThreads, st, a, span) == cudaSuccess ? MSA_OK : MSA_ERR_LAUNCH;
   }
   const int64_t units = static_cast<int64_t>(a.batch) * ((a.table_width + kCols - 1) / kCols);
   const unsigned grid = static_cast<unsigned>(std::min<int64_t>(units, kCopyCtas));
