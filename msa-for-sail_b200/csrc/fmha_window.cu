@@ -1,4 +1,4 @@
-// Windowed attention of up to 32 rows, 16 over an e4m3 cache (decode: tokens x query heads of a KV head), streamed at the rate of the memory.
+// Windowed attention of up to 32 rows, 8 or 16 over an e4m3 cache (decode: tokens x query heads of a KV head), streamed at the rate of the memory.
 //
 // Per key and KV head 4 * 128 multiplications are made for each row, so memory is the bound, and what has to be short is the chain from a
 // key's arrival to its place in the sums.  In the tcgen05 decode kernel that chain (load, Q K^T, commit, softmax, store, P V) takes 1 100
@@ -643,10 +643,14 @@ int launch(const MsaFmhaParams& p, cudaStream_t stream) {
 }  // namespace
 }  // namespace window
 
-// Windowed items of few packed rows; pages of whole units, or ragged keys.  Here and on the tcgen05 decode kernel, windows of 2 048 keys: bf16,
-// 64 sequences x 2 heads x 32 rows 35 and 38 us, 128 x 8 x 32 338 and 362; e4m3, 64 x 2 x 8 rows 22 and 25 us, 16 rows 29 and 26, but one
-// sequence 9.3 and 10.2, 24 of 512 keys 12.3 and 12.8 (and pages of any whole units); with 32 rows over an e4m3 cache registers run out.
-int fmha_window_rows(const MsaFmhaParams& p) { return p.kv_dtype == MSA_DT_E4M3 ? 16 : 32; }
+// Windowed items of few packed rows; pages of whole units, or ragged keys.  Here and on the tcgen05 decode kernel (pages of 128 keys), one token a
+// sequence: bf16, 32 rows, 64 sequences x 2 heads x 2 048 keys 34 and 34 us, 128 x 8 x 4 096 326 and 366; e4m3, 8 rows, 21 and 24, 178 and 229.  16 rows
+// over an e4m3 cache (255 registers) pay while items are few and many CTAs share one: 32 items x 1 024 keys 12.0 and 14.4 us, 64 14.4 and 14.9, 96 18.9
+// and 17.4, 512 50 and 44; with 32 rows registers run out.
+int fmha_window_rows(const MsaFmhaParams& p) {
+  if (p.kv_dtype != MSA_DT_E4M3) return 32;
+  return p.page_size == kKvTile && 128 % p.pack == 0 && p.num_work > 74 ? 8 : 16;
+}
 int fmha_window_supported(const MsaFmhaParams& p) {
   if (p.window <= 0 || (p.flags & MSA_FLAG_SPARSE) || p.decode_rows < 1 || p.decode_rows > fmha_window_rows(p)) return 0;
   if (p.pack != p.num_qo_heads / p.num_kv_heads) return 0;
