@@ -226,3 +226,56 @@ def test_nothing_runs_while_a_status_is_set():
             msa.fmha_sail(c.q, c.k, c.v, plan, kv_indices=c.table, out=out)
             assert (out == 7).all() and api.last_status() == _lib.STATUS_TIMEOUT
             c.check(plan=plan)
+
+
+@pytest.mark.parametrize("splits", [1, 3])
+def test_two_graphs_of_one_plan_at_a_time(splits):
+    import msa_for_sail as msa
+    cases = [Case([1] * 3, [3000, 900, 5000], 32, 4, 1500, 4, seed=s) for s in (1, 2)]
+    plan = cases[0].plan(num_kv_splits=splits)                  # both have its lengths
+    outs = [torch.zeros(3, 32, 128, dtype=BF, device=DEV) for _ in cases]
+    graphs, streams = [], [torch.cuda.Stream() for _ in cases]
+    for c, out in zip(cases, outs):
+        msa.fmha_sail(c.q, c.k, c.v, plan, kv_indices=c.table, out=out)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            for _ in range(20):
+                msa.fmha_sail(c.q, c.k, c.v, plan, kv_indices=c.table, out=out)
+        graphs.append(g)
+    for out in outs:
+        out.zero_()
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    for c, out in zip(cases, outs):
+        ref.check(out, None, c.want(), 2 ** -8)
+
+
+def test_splits_without_a_workspace():
+    """The entry point whose partials are the library's own takes windows too."""
+    import ctypes
+    import msa_for_sail as msa
+    from msa_for_sail import _lib
+    for args in ((32, 4, 1, "hnd", 128, BF, BF), (40, 1, 2, "nhd", 128, BF, E4), (8, 2, 1, "ragged", 0, E4, E4)):
+        hq, hk, n, layout, page, qt, ct = args
+        c = Case([n] * 3, [2000, 700, 90], hq, hk, 600, 5, layout, page, qt, ct)
+        plan = c.plan(num_kv_splits=3)
+        got = []
+        merged = _lib.lib.msa_fmha_fwd_merged
+        _lib.lib.msa_fmha_fwd_merged = lambda p, *a: got.append((_lib.MsaFmhaParams.from_buffer_copy(p._obj), a)) or merged(p, *a)
+        try:
+            want, _ = msa.fmha_sail(c.q, c.k, c.v, plan, kv_indices=c.table)
+        finally:
+            _lib.lib.msa_fmha_fwd_merged = merged
+        (p, a), = got
+        out = torch.zeros_like(want)
+        p.out, p.partial_o, p.partial_lse = out.data_ptr(), None, None
+        assert _lib.lib.msa_fmha_fwd_split_static(ctypes.byref(p), a[0], torch.cuda.current_stream().cuda_stream) == 0
+        torch.cuda.synchronize()
+        mixed = qt is not ct
+        ref.check(out, None, c.want(), 2 ** -8, 2 ** -8 if mixed else 0.0, str(args))
+        ref.check(want, None, c.want(), 2 ** -8, 2 ** -8 if mixed else 0.0, str(args))
