@@ -84,7 +84,8 @@ struct Item {
   int head, kvh, row0, qo_base, ql, kv_len, off;
   int n_tiles[2];                       // KV tiles of Q tile A / B
   int kv0;                              // first entry in the page table (paged) / first key (ragged)
-  // with a window:
+};
+struct WindowItem : Item {
   int skip;                             // tiles left out behind those of the sinks
   int b_first;                          // Q tile B has no tiles between those of the sinks and this one
   int first_key, end_key;               // of the first row's window; behind the last key that the last row sees
@@ -112,6 +113,7 @@ fmha_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant__ 
   using C = Cfg<F8>;
   static_assert(HAS_O || !WIN, "a window computes O");
   constexpr bool PAIR = F8 && WIN;
+  using Item = std::conditional_t<WIN, WindowItem, tc::Item>;
   constexpr int TILE_BYTES = C::TILE_BYTES, NSUB = C::NSUB, SUB_ELEMS = C::SUB_ELEMS;
   constexpr int KSTAGES = C::STAGES, VSTAGES = C::STAGES;
   // Score-only pass: K comes in pairs of tiles (256 keys, one MMA of N = 256 per K step) through the space of both rings:
@@ -202,18 +204,27 @@ fmha_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant__ 
   };
 
   // with a window: number of a tile among the keys, whether Q tile x has tile j, whether a tile has keys that no row of the item sees
-  [[maybe_unused]] auto real_tile = [&](const Item& w, int j) -> int { return j < sink_tiles(p.sink_tokens) ? j : j + w.skip; };
-  [[maybe_unused]] auto has_tile = [&](const Item& w, int x, int j) -> bool {
-    return x == 0 ? j < w.n_tiles[0] : j < w.n_tiles[1] && (j < sink_tiles(p.sink_tokens) || j >= w.b_first);
+  [[maybe_unused]] auto real_tile = [&](const auto& w, int j) -> int {
+    if constexpr (WIN) return j < sink_tiles(p.sink_tokens) ? j : j + w.skip;
+    else return j;
+  };
+  [[maybe_unused]] auto has_tile = [&](const auto& w, int x, int j) -> bool {
+    if constexpr (WIN) return x == 0 ? j < w.n_tiles[0] : j < w.n_tiles[1] && (j < sink_tiles(p.sink_tokens) || j >= w.b_first);
+    else return j < w.n_tiles[x];
   };
   // Up to 32 sink tokens in the last of their tiles, with tiles left out behind it: all rows see those keys of the tile, and that is all it is
   // multiplied for (S and P of 32 columns).
-  [[maybe_unused]] auto is_short = [&](const Item& w, int j) -> bool {
-    const int rest = p.sink_tokens % BN;
-    return w.skip > 0 && j == sink_tiles(p.sink_tokens) - 1 && rest >= 1 && rest <= 32;
+  [[maybe_unused]] auto is_short = [&](const auto& w, int j) -> bool {
+    if constexpr (WIN) {
+      const int rest = p.sink_tokens % BN;
+      return w.skip > 0 && j == sink_tiles(p.sink_tokens) - 1 && rest >= 1 && rest <= 32;
+    } else {
+      return false;
+    }
   };
-  [[maybe_unused]] auto has_unseen = [&](const Item& w, int key0) -> bool {
-    return key0 + BN > w.end_key || (key0 < w.first_key && key0 + BN > p.sink_tokens);
+  [[maybe_unused]] auto has_unseen = [&](const auto& w, int key0) -> bool {
+    if constexpr (WIN) return key0 + BN > w.end_key || (key0 < w.first_key && key0 + BN > p.sink_tokens);
+    else return key0 + BN > w.kv_len;
   };
 
   const bool run = *skip_flag == 0;
@@ -344,7 +355,7 @@ fmha_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant__ 
       Item w;
       w.valid = idx >= 0;
       w.head = w.kvh = w.row0 = w.qo_base = w.ql = w.kv_len = w.off = w.n_tiles[0] = w.n_tiles[1] = w.kv0 = 0;
-      w.skip = w.b_first = w.first_key = w.end_key = 0;
+      if constexpr (WIN) w.skip = w.b_first = w.first_key = w.end_key = 0;
       if (idx >= 0) {
         const MsaWorkItem mw = p.work[idx];
         const int b = chk(mw.batch, 0, p.batch, p.status);
