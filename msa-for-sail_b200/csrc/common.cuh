@@ -190,8 +190,10 @@ __device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
 }
 
 // Two values as pairs of e4m3 values, hi and lo (low 16 bits each).  hi is the value rounded to 4 significant bits: with t = (2^20 + 1) x,
-// t - (t - x) (Veltkamp's splitting); what it leaves is exact.  No conversion back from e4m3 is needed.  (Where hi is below e4m3's
-// normal numbers its conversion rounds once more, by at most 2^-10 where weights reach 2^4 to 2^8.)
+// t - (t - x) (Veltkamp's splitting); what it leaves is exact.  No conversion back from e4m3 is needed.  (Below e4m3's
+// normal numbers, 2^-6, the conversions of hi and lo round by up to 2^-10 each, where the row's largest weight is 2^4 to 2^8: 2^-13 of it at most.
+// Weights four times as large, with a maximum that lags by 2^2 at most instead of 2^4, are not seen in the results, 0.00176 from 64 bits instead
+// of 0.00178, and raise the maximum so often that an e4m3 prompt takes 365 us instead of 336.)
 __device__ __forceinline__ void e4m3_pair(float a, float b, uint32_t& hi, uint32_t& lo) {
   const uint64_t x = f2_pack(a, b), t = f2_fma(x, f2_pack(1048577.f, 1048577.f), 0), minus = f2_pack(-1.f, -1.f);
   const uint64_t h = f2_fma(f2_fma(x, minus, t), minus, t), rest = f2_fma(h, minus, x);
