@@ -174,12 +174,12 @@ __global__ void __launch_bounds__(kScanThreads) pages_fork_plan_kernel(const Msa
   const int num_free = stack_size(a.num_free, a.free_capacity);
   auto is_row = [&](int r) { return static_cast<unsigned>(r) < static_cast<unsigned>(a.batch); };
   if (tid == 0) s_missing = 0;
-  // the first of the entries that name a child has it
+  // the first of the entries that name a child has it (one with a negative parent does nothing, whatever its child)
   for (int i = tid; i < a.count; i += kScanThreads)
     if (is_row(a.children[i])) f.claim[a.children[i]] = INT_MAX;
   __syncthreads();
   for (int i = tid; i < a.count; i += kScanThreads)
-    if (is_row(a.children[i])) atomicMin(&f.claim[a.children[i]], i);
+    if (is_row(a.children[i]) && a.parents[i] >= 0) atomicMin(&f.claim[a.children[i]], i);
   __syncthreads();
   int taken = 0, missing = 0;                  // pages that the entries before need
   for (int i0 = 0; i0 < a.count; i0 += kScanThreads) {
