@@ -641,10 +641,10 @@ fmha_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant__ 
       const bool row_ok = i < w.ql;
       const int gtok = w.qo_base + i;
       const int lim = row_ok ? min(i + off, kv_len - 1) : -1;
-      [[maybe_unused]] int from = 0, from_last = 0;        // with a window: its first key for this row, and for the last row of the tile
-      if constexpr (WIN) {
-        from = window_first(i + off, kv_len, p.window);
-        from_last = window_first(m0 + BM - 1 + off, kv_len, p.window);
+      [[maybe_unused]] int from = 0, from_last = 0;        // with a window: its first key for this row, and for the last row that the tile has
+      if constexpr (WIN) {                                 // (places of rows fit 32 bits, those behind the last row need not)
+        if (row_ok) from = window_first(i + off, kv_len, p.window);
+        if (m0 < w.ql) from_last = window_first(min(m0 + BM, w.ql) - 1 + off, kv_len, p.window);
       }
       [[maybe_unused]] bool begun = false;
       const int nx = x == 0 ? w.n_tiles[0] : w.n_tiles[1];

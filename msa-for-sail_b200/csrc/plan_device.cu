@@ -4,6 +4,8 @@
 // plan.cuh; api.py:916-941).  Everything that sizes a launch is fixed by the caller: batch, the row
 // tiles per batch item, the split count -- hence the work list has a fixed number of items; a row
 // tile past a sequence's rows and a chunk past its key tiles are empty items.
+#include <climits>
+
 #include "common.cuh"
 #include "nvtx_range.h"
 
@@ -19,6 +21,8 @@ __global__ void __launch_bounds__(256) plan_device_kernel(const MsaPlanDeviceArg
   auto bounded = [&](int tokens) -> int {
     return a.max_total_q > 0 ? static_cast<int>(min(static_cast<unsigned>(tokens), static_cast<unsigned>(a.max_total_q))) : tokens;
   };
+  // Offsets on the device may be any: a sequence's places fit 32 bits, its last one is at most 2^31 - 2, as in plans made on the host.
+  auto fitting = [](int off, int ql) -> int { return min(off, INT_MAX - max(ql, 0)); };
   // Prefix sums over the batch, 256 items at a time: a warp scan and the sums of the warps.  (One thread that walked the
   // batch waited for two loads per item: 5.4 us a plan at 24 sequences.)
   __shared__ int s_sum[8][3];
@@ -38,6 +42,7 @@ __global__ void __launch_bounds__(256) plan_device_kernel(const MsaPlanDeviceArg
         else {
           off = a.qo_offset_in ? a.qo_offset_in[b] : -1;
           if (off < 0) off = kl - ql;
+          off = fitting(off, ql);
         }
         a.qo_offset_out[b] = off;
       }
@@ -90,6 +95,7 @@ __global__ void __launch_bounds__(256) plan_device_kernel(const MsaPlanDeviceArg
       else {
         off = a.qo_offset_in ? a.qo_offset_in[b] : -1;
         if (off < 0) off = kl - ql;
+        off = fitting(off, ql);
       }
       const int row0 = (RT - 1 - rr) * bm_eff;
       const int tokens = a.qo_start ? a.qo_start[b + 1] - a.qo_start[b] : ql;
