@@ -190,10 +190,14 @@ __device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
 }
 
 // Two values as pairs of e4m3 values, hi and lo (low 16 bits each).  hi is the value rounded to 4 significant bits: with t = (2^20 + 1) x,
-// t - (t - x) (Veltkamp's splitting); what it leaves is exact.  No conversion back from e4m3 is needed.  (Below e4m3's
-// normal numbers, 2^-6, the conversions of hi and lo round by up to 2^-10 each, where the row's largest weight is 2^4 to 2^8: 2^-13 of it at most.
-// Weights four times as large, with a maximum that lags by 2^2 at most instead of 2^4, are not seen in the results, 0.00176 from 64 bits instead
-// of 0.00178, and raise the maximum so often that an e4m3 prompt takes 365 us instead of 336.)
+// t - (t - x) (Veltkamp's splitting); what it leaves is exact.  No conversion back from e4m3 is needed.  A pair is within 2^-8 x + 1.5 * 2^-10 of x: below
+// e4m3's normal numbers, 2^-6, hi rounds by up to 2^-10, what is left of it by 2^-11, and a weight below 2^-10 is gone.
+//
+// So what weights are relative to must not lie far above most of a row's mass: one heavy key (a sink) with weight 2^4 would leave nothing of thousands
+// of keys ten nats below it, 16 % of the mass with 4 096 of them.  It follows a tile's largest score down as well as up (pair_lowers).  Of a tile of n keys
+// 1.5 * 2^-10 n is lost at most.  That is left so where the tile's weights have a sum of n / 4, or the row's have one of n / 4 for each tile that it
+// has; else it goes down to the tile's largest score.  Either way all that is lost of a row is 1.5 * 2^-8 of its sum at most.  A row of scores that lie
+// within a few nats has such a sum after its first tiles and never gets there.
 __device__ __forceinline__ void e4m3_pair(float a, float b, uint32_t& hi, uint32_t& lo) {
   const uint64_t x = f2_pack(a, b), t = f2_fma(x, f2_pack(1048577.f, 1048577.f), 0), minus = f2_pack(-1.f, -1.f);
   const uint64_t h = f2_fma(f2_fma(x, minus, t), minus, t), rest = f2_fma(h, minus, x);
@@ -208,6 +212,40 @@ __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
   return y;
+}
+
+// What a row's weights are relative to, for pairs of e4m3 values (e4m3_pair): a score equal to it has weight 2^kPairOffset, one kPairRescale (log2)
+// above it raises it.
+constexpr float kPairOffset = 5.f, kPairRescale = 3.8f;
+constexpr float kPairEnough = 0.25f;                         // sum of weights, for each key, of which the loss is small enough
+// Whether it goes down to a tile's largest score: not where `tile`, a lower bound of the sum of the tile's n weights, or `row`, the sum of the row's
+// weights before, is enough (for the tile; for all `tiles`).  Nothing 2^60 below is looked at: fewer than 2^31 keys have no weight there, and sums
+// and O stay finite.  (A tile without a key has top -inf.)
+__device__ __forceinline__ bool pair_lowers(float ref, float top, float tile, float row, int n, int tiles) {
+  const float enough = kPairEnough * static_cast<float>(n), down = ref - top;
+  return tile < enough && row < enough * static_cast<float>(tiles) && down > 0.f && down <= 60.f;
+}
+// The next `ref` of a row, by a thread that has all of it: `top` are the largest scores of N parts of the tile, to be multiplied by `scale`, `sum` is
+// the row's so far, relative to `ref`.  settled: all rows of the warp have enough for all tiles, which only a rise of `ref` changes.
+template <int N>
+__device__ __forceinline__ float pair_reference(float ref, float sum, const float (&top)[N], float scale, int n, int tiles, bool exists, bool& settled) {
+  float best = top[0];
+#pragma unroll
+  for (int i = 1; i < N; ++i) best = fmaxf(best, top[i]);
+  best *= scale;
+  const bool up = best - ref > kPairRescale;
+  float now = up ? best : ref;
+  if (!settled || __any_sync(0xffffffffu, up)) {
+    const float row = up ? sum * exp2_fast(ref - now) : sum;
+    settled = __all_sync(0xffffffffu, row >= kPairEnough * static_cast<float>(n) * static_cast<float>(tiles) || !exists);
+    if (!settled) {
+      float tile = 0.f;
+#pragma unroll
+      for (int i = 0; i < N; ++i) tile += exp2_fast(fmaf(top[i], scale, kPairOffset - now));
+      if (pair_lowers(now, best, tile, row, n, tiles)) now = best;
+    }
+  }
+  return now;
 }
 
 // Row tile [rows][128 x 16-bit]: 16 chunks of 16 bytes per row, chunk index XOR-ed with

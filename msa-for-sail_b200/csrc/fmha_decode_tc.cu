@@ -156,8 +156,8 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
   // within (0, 2^8], and what falls below e4m3's smallest subnormal (2^-9) is a weight under 2^-13
   // of the row's largest.  (Upstream uses the exact max and a 2^8 offset, fmha_common.hpp:567-570;
   // with the exact max nearly every tile of a short work item triggers an O rescale.)
-  constexpr float kRescaleThreshold = F8 ? 4.0f : 8.0f;
-  constexpr float kPOffset = F8 ? 4.0f : 0.0f;
+  constexpr float kRescaleThreshold = F8 ? 4.0f : 8.0f;        // (pairs: pair_reference)
+  constexpr float kPOffset = PAIR ? kPairOffset : F8 ? 4.0f : 0.0f;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 #ifdef MSA_DEBUG_HOOKS
   unsigned long long* trace = (threadIdx.x == 0 && g_trace) ? g_trace + 16ull * blockIdx.x : nullptr;
@@ -758,6 +758,7 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
       constexpr int CW = TK / PARTS;                         // key columns of a tile that this warp has
       constexpr int RC = PARTS == 1 ? 16 : 32;               // columns of O scaled at a time: 64 scores leave no registers for 32
       const int part = trow / ROWS;
+      [[maybe_unused]] bool settled = false;
       for (int j = 0; j < n_tiles && alive; ++j) {
         const uint32_t tS = tmem + (j % NBUF) * TK + lane_addr;
         alive = mbar_wait_warp(bar(S_FULL + j % NBUF), (j / NBUF) & 1, abort_flag);
@@ -785,12 +786,17 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
         float mxs[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
         for (int e = 0; e < CW; e += 2) mxs[(e >> 1) & 3] = max3(mxs[(e >> 1) & 3], __uint_as_float(sv[e / LD][e % LD]), __uint_as_float(sv[e / LD][e % LD + 1]));
-        const float mx = fmaxf(fmaxf(mxs[0], mxs[1]), fmaxf(mxs[2], mxs[3]));
-        const float m_cand = fmaxf(m_used, mx * scale_log2);
-        const bool bump = (m_cand - m_used) > kRescaleThreshold;
+        float m_next;
+        if constexpr (PAIR) {
+          m_next = pair_reference(m_used, l_sum, mxs, scale_log2, CW, n_tiles, row_ok, settled);
+        } else {
+          const float m_cand = fmaxf(m_used, fmaxf(fmaxf(mxs[0], mxs[1]), fmaxf(mxs[2], mxs[3])) * scale_log2);
+          m_next = (m_cand - m_used) > kRescaleThreshold ? m_cand : m_used;
+        }
+        const bool moves = m_next != m_used;
         float factor = 1.f;
-        if (bump) { factor = exp2_fast(m_used - m_cand); m_used = m_cand; l_sum *= factor; }
-        if (j > 0 && __any_sync(0xffffffffu, bump)) {
+        if (moves) { factor = exp2_fast(m_used - m_next); m_used = m_next; l_sum *= factor; }
+        if (j > 0 && __any_sync(0xffffffffu, moves)) {
           // O may still be the target of P_{j-1} V_{j-1}: wait for that MMA before touching it
           alive = mbar_wait_warp(bar(PV_DONE), (j - 1) & 1, abort_flag);
           if (!alive) break;

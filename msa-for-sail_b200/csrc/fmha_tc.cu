@@ -123,7 +123,7 @@ fmha_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant__ 
   constexpr int PAIR_BYTES = 2 * TILE_BYTES;
   static_assert(HAS_O || KSTAGES * PAIR_BYTES <= C::OFF_BAR - C::OFF_K, "pairs of K tiles fit both rings");
   constexpr int OFF_Q = C::OFF_Q, OFF_K = C::OFF_K, OFF_V = C::OFF_V, OFF_BAR = C::OFF_BAR;
-  constexpr float kRescaleThreshold = C::kRescaleThreshold, kPOffset = C::kPOffset;
+  constexpr float kRescaleThreshold = C::kRescaleThreshold, kPOffset = PAIR ? kPairOffset : C::kPOffset;      // (threshold of pairs: pair_reference)
   extern __shared__ unsigned char smem_raw[];
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   unsigned char* smem_gen = smem_raw + (smem_base - smem_u32(smem_raw));
@@ -646,7 +646,7 @@ fmha_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant__ 
         if (row_ok) from = window_first(i + off, kv_len, p.window);
         if (m0 < w.ql) from_last = window_first(min(m0 + BM, w.ql) - 1 + off, kv_len, p.window);
       }
-      [[maybe_unused]] bool begun = false;
+      [[maybe_unused]] bool begun = false, settled = false;
       const int nx = x == 0 ? w.n_tiles[0] : w.n_tiles[1];
       const float scale_all = p.sm_scale * kLog2e * (p.k_scale_head ? p.k_scale_head[kvh] : 1.f);
       const float scale_log2 = WIN ? masked_scale(scale_all) : scale_all;
@@ -679,11 +679,19 @@ fmha_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant__ 
               if (e >= rest) s32[e] = 0xff800000u;
               top = fmaxf(top, __uint_as_float(s32[e]));
             }
-            const float m_cand = fmaxf(m_used, top * scale_log2);
-            const bool bump = (m_cand - m_used) > kRescaleThreshold;
+            float m_next;
+            if constexpr (PAIR) {
+              const float tops[1] = {top};
+              m_next = pair_reference(m_used, l_sum, tops, scale_log2, rest, nx, row_ok, settled);
+              settled = false;                              // (fewer keys than other tiles have)
+            } else {
+              const float m_cand = fmaxf(m_used, top * scale_log2);
+              m_next = (m_cand - m_used) > kRescaleThreshold ? m_cand : m_used;
+            }
+            const bool moves = m_next != m_used;
             float factor = 1.f;
-            if (bump) { factor = exp2_fast(m_used - m_cand); m_used = m_cand; l_sum *= factor; }
-            if (later && __any_sync(0xffffffffu, bump)) {
+            if (moves) { factor = exp2_fast(m_used - m_next); m_used = m_next; l_sum *= factor; }
+            if (later && __any_sync(0xffffffffu, moves)) {
 #pragma unroll
               for (int c = 0; c < 4; ++c) {
                 uint32_t v[32];
@@ -740,25 +748,27 @@ fmha_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant__ 
             tmem_wait_ld();
             if (need_mask) { mask32(s[0], pos0 + 64 * h); mask32(s[1], pos0 + 64 * h + 32); }
           };
-          auto top_of = [&](const uint32_t (&s)[2][32]) -> float {
+          float tops[8];                                    // of 16 scores each
+          auto tops_of = [&](const uint32_t (&s)[2][32], int at) {
             float t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
             for (int c = 0; c < 2; ++c)
 #pragma unroll
               for (int e = 0; e < 32; e += 2) t[(e >> 1) & 3] = max3(t[(e >> 1) & 3], __uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1]));
-            return fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) tops[at + i] = t[i];
           };
           uint32_t sv[2][32];
           read(1, sv);
-          float top = top_of(sv);
+          tops_of(sv, 4);
           read(0, sv);
-          top = fmaxf(top, top_of(sv));
+          tops_of(sv, 0);
           if (r == 0) trace(x, j, 2);
-          const float m_cand = fmaxf(m_used, top * scale_log2);
-          const bool bump = (m_cand - m_used) > kRescaleThreshold;
+          const float m_next = pair_reference(m_used, l_sum, tops, scale_log2, BN, nx, row_ok, settled);
+          const bool moves = m_next != m_used;
           float factor = 1.f;
-          if (bump) { factor = exp2_fast(m_used - m_cand); m_used = m_cand; l_sum *= factor; }
-          if (later && __any_sync(0xffffffffu, bump)) {
+          if (moves) { factor = exp2_fast(m_used - m_next); m_used = m_next; l_sum *= factor; }
+          if (later && __any_sync(0xffffffffu, moves)) {
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
               uint32_t v[32];

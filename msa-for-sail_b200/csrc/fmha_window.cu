@@ -18,8 +18,8 @@
 //
 // bf16: P is rounded to bf16 (2^-8), its sum is that of the unrounded weights.
 // e4m3: m16n8k32 on the bytes as they are (with K and V converted to f16 the conversions alone took 55 % of the ALU pipe, and an m16n8k16 of f16
-// takes 2.1 clocks an SM where an m16n8k32 of e4m3 takes 1.2).  Q and P are pairs of e4m3 values, hi + lo, both multiplied: 8 bits.  A query
-// row is multiplied by a power of two that brings its largest element to [2^7, 2^8), P is 2^(x - m + 4) and at most 2^8.  The order of
+// takes 2.1 clocks an SM where an m16n8k32 of e4m3 takes 1.2).  Q and P are pairs of e4m3 values, hi + lo, both multiplied: 8 bits (e4m3_pair).  A query
+// row is multiplied by a power of two that brings its largest element to [2^7, 2^8), P is 2^(x - m + 5) and at most 2^8.8.  The order of
 // a contraction is free: thread t of a group of four takes elements 32 t .. 32 t + 31 of its keys (K), thread group g elements 16 g .. 16 g + 15 of
 // the keys 2 t, 2 t + 8, 2 t + 1, 2 t + 9 (V; four bytes of a key each become four keys of an element by eight byte permutations),
 // which is the order that the transposed bytes of P come in.
@@ -97,7 +97,7 @@ window_decode_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_const
   constexpr int OFF_BAR = C::OFF_BAR, OFF_FAC = C::OFF_FAC, OFF_LIM = C::OFF_LIM, OFF_FLAG = C::OFF_FLAG, kStages = C::STAGES;
   constexpr int UK = unit_keys<F8>(), STEPS = UK / 16;
   constexpr int SUB = UK * 128;                              // a half of head_dim of a bf16 unit, all of it in e4m3
-  constexpr float kPOffset = F8 ? 4.f : 0.f, kRescale = F8 ? 4.f : 8.f;      // P is at most 2^8
+  constexpr float kPOffset = F8 ? kPairOffset : 0.f, kRescale = F8 ? kPairRescale : 8.f;      // P is at most 2^8, 2^8.8 in e4m3
   extern __shared__ unsigned char smem_raw[];
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   unsigned char* smem = smem_raw + (smem_base - smem_u32(smem_raw));
@@ -280,6 +280,7 @@ window_decode_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_const
   }
 
   int stage = 0, parity = 0;
+  [[maybe_unused]] bool settled = false;
 #pragma unroll 1
   for (int i = 0; i < n_units && alive; ++i) {
     const int key0 = key_of(i);
@@ -375,6 +376,7 @@ window_decode_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_const
         raise |= top[n][c] > m[n][c] + (kPOffset + kRescale);
       }
     if (__any_sync(0xffffffffu, raise)) {
+      settled = false;
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         float k2[2];
@@ -393,29 +395,84 @@ window_decode_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_const
       }
     }
     uint32_t pt[STEPS][NT][2];                               // P^T as an operand: keys 0-7, keys 8-15; e4m3: hi, lo of the step's 16 keys
+    uint64_t unit[NT];                                       // sums of its weights, two rows
+    auto weights = [&]() {
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const uint64_t f = f2_pack(fac[n][0], fac[n][1]), shift = f2_pack(-m[n][0], -m[n][1]);
+      for (int n = 0; n < NT; ++n) {
+        const uint64_t f = f2_pack(fac[n][0], fac[n][1]), shift = f2_pack(-m[n][0], -m[n][1]);
+        unit[n] = 0;
 #pragma unroll
-      for (int u = 0; u < STEPS; ++u) {
-        float w0[2], w1[2];                                  // keys g and g + 8 of the rows 2 t, 2 t + 1
+        for (int u = 0; u < STEPS; ++u) {
+          float w0[2], w1[2];                                // keys g and g + 8 of the rows 2 t, 2 t + 1
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float x0, x1;
-          f2_unpack(f2_fma(f2_pack(s[u][n][2 * h], s[u][n][2 * h + 1]), f, shift), x0, x1);
-          w0[h] = exp2_fast(x0); w1[h] = exp2_fast(x1);
-          l[n] = f2_add(l[n], f2_pack(w0[h], w1[h]));
-          if constexpr (!F8) pt[u][n][h] = transpose8x8(pack2<false>(w0[h], w1[h]));
+          for (int h = 0; h < 2; ++h) {
+            float x0, x1;
+            f2_unpack(f2_fma(f2_pack(s[u][n][2 * h], s[u][n][2 * h + 1]), f, shift), x0, x1);
+            w0[h] = exp2_fast(x0); w1[h] = exp2_fast(x1);
+            unit[n] = f2_add(unit[n], f2_pack(w0[h], w1[h]));
+            if constexpr (!F8) pt[u][n][h] = transpose8x8(pack2<false>(w0[h], w1[h]));
+          }
+          if constexpr (F8) {
+            uint32_t h0, l0, h1, l1;
+            e4m3_pair(w0[0], w0[1], h0, l0);
+            e4m3_pair(w1[0], w1[1], h1, l1);
+            pt[u][n][0] = transpose8x8(h0 | (h1 << 16));
+            pt[u][n][1] = transpose8x8(l0 | (l1 << 16));
+          }
         }
-        if constexpr (F8) {
-          uint32_t h0, l0, h1, l1;
-          e4m3_pair(w0[0], w0[1], h0, l0);
-          e4m3_pair(w1[0], w1[1], h1, l1);
-          pt[u][n][0] = transpose8x8(h0 | (h1 << 16));
-          pt[u][n][1] = transpose8x8(l0 | (l1 << 16));
+      }
+    };
+    weights();
+    if constexpr (F8) {
+      // Pairs: whether the row's sums allow small weights to get lost (pair_lowers).  Once every lane has its share of enough for all units, only a
+      // maximum that rises asks again.
+      if (!settled) {
+        const float enough = kPairEnough * UK * static_cast<float>(n_units);
+        float now[NT][2];
+        bool small = false, all = true;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          float before[2];
+          f2_unpack(unit[n], now[n][0], now[n][1]);
+          f2_unpack(l[n], before[0], before[1]);
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            all &= now[n][c] + before[c] >= enough / 8;
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) now[n][c] += __shfl_xor_sync(0xffffffffu, now[n][c], d);
+            small |= now[n][c] < kPairEnough * UK;
+          }
+        }
+        settled = __all_sync(0xffffffffu, all);
+        if (!settled && __any_sync(0xffffffffu, small)) {
+          bool again = false;
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            float k2[2], before[2];
+            f2_unpack(l[n], before[0], before[1]);
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              float x = top[n][c];
+#pragma unroll
+              for (int d = 4; d < 32; d <<= 1) {
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+                before[c] += __shfl_xor_sync(0xffffffffu, before[c], d);
+              }
+              const bool lowers = pair_lowers(m[n][c] + kPOffset, x, now[n][c], before[c], UK, n_units);
+              again |= lowers;
+              k2[c] = lowers ? exp2_fast(m[n][c] - (x - kPOffset)) : 1.f;
+              if (lowers) m[n][c] = x - kPOffset;
+#pragma unroll
+              for (int j = 0; j < 8; ++j) { o[j][n][c] *= k2[c]; o[j][n][c + 2] *= k2[c]; }
+            }
+            l[n] = f2_fma(l[n], f2_pack(k2[0], k2[1]), 0);
+          }
+          if (__any_sync(0xffffffffu, again)) weights();
         }
       }
     }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) l[n] = f2_add(l[n], unit[n]);
     // ---- O^T ----
     if constexpr (!F8) {
 #pragma unroll

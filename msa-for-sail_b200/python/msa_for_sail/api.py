@@ -1483,8 +1483,9 @@ def fmha_sail(
     fixed-address table alike, so a captured prefill has a table no longer than its use).
 
     With a plan that has a ``window_size``: bf16 or e4m3 ``k``/``v``, ``q`` in bf16 or their type.  Weights are
-    rounded to bf16, or to pairs of e4m3 values with as many bits over an e4m3 cache (bf16 queries too,
-    where rows are few; prompts of bf16 queries over an e4m3 cache run on the generic kernel, with weights in fp16).  The
+    rounded to bf16, or over an e4m3 cache to pairs of e4m3 values (bf16 queries too, where rows are few): each
+    weight within 2^-8 of itself, and what small ones lose beyond that is together at most 1.5 * 2^-8 of their row's sum.
+    Prompts of bf16 queries over an e4m3 cache run on the generic kernel, with weights in fp16.  The
     plan has its offsets (no ``q_offset_override``), the factor of the scores (``sm_scale * q_scale *
     k_scale``) is not negative, and partials of a split are the call's own, so that one plan may run on
     two streams, or in two graphs, at a time.
