@@ -420,8 +420,13 @@ int msa_pages_fork(const MsaPagesForkArgs* args, msa_stream_t stream);
 /* Row b keeps the pages of its first kv_len[b] tokens; with a window (as in MsaFmhaParams) also only those that a query at place
  * kv_len[b] or later sees.  The other entries become -1, their pages lose a share, and those that nobody shares go onto the stack in the order of
  * the entries (row, then column; of several entries with one page the first).  num_held becomes the pages of the length.
- * Numbers outside [0, num_pages) are dropped. */
+ * Numbers outside [0, num_pages) are dropped.
+ *
+ * A row whose length was cut back into a page that other rows hold would write its next token there.  With caches such a row then takes a page from
+ * the stack, in the order of the rows, that gets a copy of its tokens, and gives up its share (the last row, if all that hold the page are such
+ * rows, keeps it).  num_shared: rows that are left with such a page, since the stack had none or there are no caches. */
 typedef struct MsaPagesFreeArgs {
+  const MsaPageCache* caches;      /* [num_caches] HOST; needs shares */
   int32_t* block_table;
   int32_t* num_held;               /* [batch] */
   const int32_t* kv_len;           /* [batch] */
@@ -429,9 +434,10 @@ typedef struct MsaPagesFreeArgs {
   int32_t* num_free;               /* [1] */
   int32_t* shares;                 /* [num_pages] or NULL */
   int32_t* num_freed;              /* [1] or NULL: pages that went onto the stack */
+  int32_t* num_shared;             /* [1] or NULL; needs shares */
   int32_t* workspace;              /* msa_pages_free_workspace_bytes(batch, table_width) bytes */
   int64_t table_stride;
-  int32_t batch, table_width, page_size, free_capacity, num_pages, window, sink_tokens;
+  int32_t num_caches, batch, table_width, page_size, free_capacity, num_pages, window, sink_tokens;
 } MsaPagesFreeArgs;
 int64_t msa_pages_free_workspace_bytes(int32_t batch, int32_t table_width);
 int msa_pages_free(const MsaPagesFreeArgs* args, msa_stream_t stream);

@@ -481,6 +481,88 @@ __global__ void __launch_bounds__(kThreads) pages_free_held_kernel(const MsaPage
   for (int b = blockIdx.x * kThreads + threadIdx.x; b < a.batch; b += gridDim.x * kThreads) a.num_held[b] = kept_of(a, b).end;
 }
 
+// Rows that were cut back into a page that other rows hold (see kept_of: entry len / page_size, partly used).  By one CTA, after all of the above.
+// Workspace, behind the counts: the page of each such row (-1: none), its number among those that go to another page (-1: it does not), then the moves
+// (from, to, tokens), then their number.  shares[p] goes down by one
+// for each such row of p; below zero nobody else holds p, and the last row, whose number is put in the place of the share, keeps it.  (512 rows of 17
+// pages, 8 of them so: 8 us with the copy's launch, in a captured graph.)
+struct Cut {
+  int32_t *page, *rank, *src, *dst, *tokens, *moves;
+};
+__host__ __device__ inline int64_t counts_of(int batch, int width) { return static_cast<int64_t>(batch) * ((static_cast<int64_t>(width) + kCols - 1) / kCols) + 1; }
+__host__ __device__ inline Cut cut_of(const MsaPagesFreeArgs& a) {
+  int32_t* w = a.workspace + counts_of(a.batch, a.table_width);
+  const int64_t n = a.batch;
+  return {w, w + n, w + 2 * n, w + 3 * n, w + 4 * n, w + 5 * n};
+}
+__global__ void __launch_bounds__(kScanThreads) pages_cut_kernel(const MsaPagesFreeArgs a) {
+  chain_begin();
+  const Cut w = cut_of(a);
+  __shared__ int s_sum[32];
+  __shared__ int s_left;
+  const int tid = threadIdx.x;
+  const bool moves = a.num_caches > 0;
+  if (tid == 0) s_left = 0;
+  for (int b = tid; b < a.batch; b += kScanThreads) {
+    const int len = max(a.kv_len[b], 0), col = len / a.page_size;
+    int page = -1;
+    if (len % a.page_size > 0 && col < min(a.num_held[b], a.table_width)) {
+      page = a.block_table[b * a.table_stride + col];
+      if (page < 0 || page >= a.num_pages || __ldcg(&a.shares[page]) <= 0) page = -1;
+    }
+    w.page[b] = page;
+  }
+  __syncthreads();
+  if (moves) {
+    for (int b = tid; b < a.batch; b += kScanThreads)
+      if (w.page[b] >= 0) atomicSub(&a.shares[w.page[b]], 1);
+    __syncthreads();
+    for (int b = tid; b < a.batch; b += kScanThreads)
+      if (w.page[b] >= 0 && __ldcg(&a.shares[w.page[b]]) < 0) atomicMin(&a.shares[w.page[b]], INT_MIN + (a.batch - 1 - b));
+    __syncthreads();
+    const int num_free = stack_size(a.num_free, a.free_capacity);
+    int taken = 0;
+    for (int b0 = 0; b0 < a.batch; b0 += kScanThreads) {
+      const int b = b0 + tid, page = b < a.batch ? w.page[b] : -1;
+      const bool keeps = page >= 0 && __ldcg(&a.shares[page]) == INT_MIN + (a.batch - 1 - b), goes = page >= 0 && !keeps;
+      int total;
+      const int rank = taken + block_scan<kScanThreads>(goes ? 1 : 0, s_sum, total);
+      taken += total;
+      if (b < a.batch) w.rank[b] = goes ? rank : keeps ? -2 : -1;
+    }
+    __syncthreads();
+    for (int b = tid; b < a.batch; b += kScanThreads)
+      if (w.rank[b] == -2) a.shares[w.page[b]] = 0;
+    __syncthreads();
+    for (int b = tid; b < a.batch; b += kScanThreads) {
+      const int rank = w.rank[b];
+      if (rank < 0) continue;
+      const int len = a.kv_len[b];
+      int to = rank < num_free ? a.free_pages[num_free - 1 - rank] : -1;
+      if (static_cast<unsigned>(to) >= static_cast<unsigned>(a.num_pages)) to = -1;
+      w.src[rank] = w.page[b]; w.dst[rank] = to; w.tokens[rank] = len % a.page_size;
+      if (to >= 0) {
+        a.block_table[b * a.table_stride + len / a.page_size] = to;
+        w.page[b] = -1;                        // (it is not counted)
+      } else {
+        atomicAdd(&a.shares[w.page[b]], 1);
+      }
+    }
+    __syncthreads();
+    if (tid == 0) {
+      *w.moves = taken;
+      *a.num_free = num_free - min(taken, num_free);
+    }
+  }
+  if (a.num_shared) {
+    int left = 0;
+    for (int b = tid; b < a.batch; b += kScanThreads) left += w.page[b] >= 0 && __ldcg(&a.shares[w.page[b]]) > 0;
+    if (left) atomicAdd(&s_left, left);
+    __syncthreads();
+    if (tid == 0) *a.num_shared = s_left;
+  }
+}
+
 // ---------------------------------------------------------------------------------------------------------------------------
 // pages in use moved together
 // ---------------------------------------------------------------------------------------------------------------------------
@@ -723,6 +805,31 @@ int check_caches(const MsaPageCache* caches, int num_caches, int num_pages, int 
   return MSA_OK;
 }
 
+// The pages that rows give back.
+int give_back(const MsaPagesFreeArgs& a, int64_t entries, cudaStream_t st) {
+  if (entries <= 16 * kClusterCtas * kScanThreads) {
+    const int k = entries <= kClusterCtas * kScanThreads ? 1 : entries <= 4 * kClusterCtas * kScanThreads ? 4 : 16;
+    int ctas = 1;
+    while (ctas < kClusterCtas && static_cast<int64_t>(ctas) * kScanThreads < entries) ctas *= 2;
+    const int span = static_cast<int>((entries + ctas * kScanThreads - 1) / (ctas * kScanThreads));
+    const auto kernel = k == 1 ? pages_free_cluster_kernel<1> : k == 4 ? pages_free_cluster_kernel<4> : pages_free_cluster_kernel<16>;
+    return launch_cluster(kernel, ctas, kScanThreads, st, a, span) == cudaSuccess ? MSA_OK : MSA_ERR_LAUNCH;
+  }
+  const int64_t units = static_cast<int64_t>(a.batch) * ((a.table_width + kCols - 1) / kCols);
+  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(units, kCopyCtas));
+  cudaError_t rc = cudaSuccess;
+  if (a.shares) {
+    rc = msa::launch_chained(pages_free_step_kernel<0>, grid, kThreads, 0, st, a);
+    if (rc == cudaSuccess) rc = msa::launch_chained(pages_free_step_kernel<1>, grid, kThreads, 0, st, a);
+  }
+  if (rc == cudaSuccess) rc = msa::launch_chained(pages_free_step_kernel<2>, grid, kThreads, 0, st, a);
+  if (rc == cudaSuccess) rc = msa::launch_chained(pages_free_scan_kernel, 1, kScanThreads, 0, st, a);
+  if (rc == cudaSuccess) rc = msa::launch_chained(pages_free_push_kernel, grid, kThreads, 0, st, a);
+  if (rc == cudaSuccess && a.table_width > kCols)
+    rc = msa::launch_chained(pages_free_held_kernel, static_cast<unsigned>(std::min((a.batch + kThreads - 1) / kThreads, 148)), kThreads, 0, st, a);
+  return rc == cudaSuccess ? MSA_OK : MSA_ERR_LAUNCH;
+}
+
 }  // namespace
 }  // namespace pages
 }  // namespace msa
@@ -771,7 +878,7 @@ extern "C" int msa_pages_fork(const MsaPagesForkArgs* pa, msa_stream_t stream) {
 
 extern "C" int64_t msa_pages_free_workspace_bytes(int32_t batch, int32_t table_width) {
   if (batch < 0 || table_width < 0) return MSA_ERR_BAD_ARG;
-  return 4 * (static_cast<int64_t>(batch) * ((static_cast<int64_t>(table_width) + msa::pages::kCols - 1) / msa::pages::kCols) + 1);
+  return 4 * (msa::pages::counts_of(batch, table_width) + 5 * static_cast<int64_t>(batch) + 1);
 }
 
 extern "C" int msa_pages_free(const MsaPagesFreeArgs* pa, msa_stream_t stream) {
@@ -782,31 +889,22 @@ extern "C" int msa_pages_free(const MsaPagesFreeArgs* pa, msa_stream_t stream) {
   if (a.window < 0 || a.sink_tokens < 0 || (a.sink_tokens > 0 && a.window == 0)) return MSA_ERR_BAD_ARG;
   if (!a.num_free || !a.workspace || (a.free_capacity > 0 && !a.free_pages)) return MSA_ERR_BAD_ARG;
   if (a.batch > 0 && (!a.num_held || !a.kv_len || (a.table_width > 0 && !a.block_table))) return MSA_ERR_BAD_ARG;
+  if (const int rc = check_caches(a.caches, a.num_caches, a.num_pages, a.page_size)) return rc;
+  if ((a.num_caches > 0 || a.num_shared) && !a.shares) return MSA_ERR_BAD_ARG;
   const int64_t entries = static_cast<int64_t>(a.batch) * a.table_width;
   if (entries > INT_MAX / 2) return MSA_ERR_TOO_LARGE;
   msa::NvtxRange range("msa_pages_free");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (entries <= 16 * kClusterCtas * kScanThreads) {
-    const int k = entries <= kClusterCtas * kScanThreads ? 1 : entries <= 4 * kClusterCtas * kScanThreads ? 4 : 16;
-    int ctas = 1;
-    while (ctas < kClusterCtas && static_cast<int64_t>(ctas) * kScanThreads < entries) ctas *= 2;
-    const int span = static_cast<int>((entries + ctas * kScanThreads - 1) / (ctas * kScanThreads));
-    const auto kernel = k == 1 ? pages_free_cluster_kernel<1> : k == 4 ? pages_free_cluster_kernel<4> : pages_free_cluster_kernel<16>;
-    return launch_cluster(kernel, ctas, kScanThreads, st, a, span) == cudaSuccess ? MSA_OK : MSA_ERR_LAUNCH;
-  }
-  const int64_t units = static_cast<int64_t>(a.batch) * ((a.table_width + kCols - 1) / kCols);
-  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(units, kCopyCtas));
-  cudaError_t rc = cudaSuccess;
-  if (a.shares) {
-    rc = msa::launch_chained(pages_free_step_kernel<0>, grid, kThreads, 0, st, a);
-    if (rc == cudaSuccess) rc = msa::launch_chained(pages_free_step_kernel<1>, grid, kThreads, 0, st, a);
-  }
-  if (rc == cudaSuccess) rc = msa::launch_chained(pages_free_step_kernel<2>, grid, kThreads, 0, st, a);
-  if (rc == cudaSuccess) rc = msa::launch_chained(pages_free_scan_kernel, 1, kScanThreads, 0, st, a);
-  if (rc == cudaSuccess) rc = msa::launch_chained(pages_free_push_kernel, grid, kThreads, 0, st, a);
-  if (rc == cudaSuccess && a.table_width > kCols)
-    rc = msa::launch_chained(pages_free_held_kernel, static_cast<unsigned>(std::min((a.batch + kThreads - 1) / kThreads, 148)), kThreads, 0, st, a);
-  return rc == cudaSuccess ? MSA_OK : MSA_ERR_LAUNCH;
+  if (const int rc = give_back(a, entries, st)) return rc;
+  if (a.num_caches == 0 && !a.num_shared) return MSA_OK;
+  if (msa::launch_chained(pages_cut_kernel, 1, kScanThreads, 0, st, a) != cudaSuccess) return MSA_ERR_LAUNCH;
+  if (a.num_caches == 0 || a.batch == 0) return MSA_OK;
+  const Cut w = cut_of(a);
+  Copies list = {};
+  list.entries = a.batch; list.src = w.src; list.dst = w.dst; list.tokens = w.tokens; list.count = w.moves;
+  return launch_copies(a.caches, a.num_caches, a.num_pages, a.page_size, list, 1, st, [&](const Copies& c, unsigned grid) {
+    return msa::launch_chained(pages_copy_kernel, grid, kThreads, 0, st, c);
+  });
 }
 
 extern "C" int64_t msa_pages_compact_workspace_bytes(int32_t num_pages) {

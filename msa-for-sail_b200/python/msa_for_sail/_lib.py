@@ -110,9 +110,9 @@ class MsaPagesForkArgs(ctypes.Structure):
 
 
 class MsaPagesFreeArgs(ctypes.Structure):
-    _fields_ = [("block_table", _p), ("num_held", _p), ("kv_len", _p), ("free_pages", _p), ("num_free", _p), ("shares", _p), ("num_freed", _p),
-                ("workspace", _p), ("table_stride", _i64), ("batch", _i32), ("table_width", _i32), ("page_size", _i32), ("free_capacity", _i32),
-                ("num_pages", _i32), ("window", _i32), ("sink_tokens", _i32)]
+    _fields_ = [("caches", _p), ("block_table", _p), ("num_held", _p), ("kv_len", _p), ("free_pages", _p), ("num_free", _p), ("shares", _p), ("num_freed", _p),
+                ("num_shared", _p), ("workspace", _p), ("table_stride", _i64), ("num_caches", _i32), ("batch", _i32), ("table_width", _i32), ("page_size", _i32),
+                ("free_capacity", _i32), ("num_pages", _i32), ("window", _i32), ("sink_tokens", _i32)]
 
 
 class MsaPagesCompactArgs(ctypes.Structure):

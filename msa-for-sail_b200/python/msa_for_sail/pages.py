@@ -158,7 +158,8 @@ def kv_pages_fork(block_table: torch.Tensor, num_held: torch.Tensor, kv_lens: to
     Full pages are shared (``shares`` + 1 each); the last page, where it is partly filled, is taken from the stack, in the order of the entries, and
     the used part is copied in every one of ``caches`` (bf16, e4m3 or any other type as ``[pages, Hkv, page, D]`` or ``[pages, page, Hkv, D]``, 4-bit
     caches; of other tensors with pages as the first dimension the whole page is copied).  So whoever writes next writes into a page of its
-    own.  ``num_held`` and ``kv_lens`` (int32 ``[B]``) of the child are set.
+    own, as long as neither row is cut back into a page that they share (``kv_pages_free`` with ``caches`` sees to that).  ``num_held`` and ``kv_lens``
+    (int32 ``[B]``) of the child are set.
 
     ``parents``, ``children``: int32 ``[n]``; an entry with a negative number does nothing (a list of fixed size).  A row may be the parent of many.
     A child holds nothing before (``kv_pages_free`` it first).  Returns ``num_missing`` (int32 ``[1]``): entries that were not made, since a row is
@@ -178,7 +179,8 @@ def kv_pages_fork(block_table: torch.Tensor, num_held: torch.Tensor, kv_lens: to
 
 
 def kv_pages_free(block_table: torch.Tensor, num_held: torch.Tensor, kv_lens: torch.Tensor, free_pages: torch.Tensor, num_free: torch.Tensor,
-                  shares: Optional[torch.Tensor] = None, *, window_size: int = -1, num_sink_tokens: int = 0, page_size: int = 128) -> torch.Tensor:
+                  shares: Optional[torch.Tensor] = None, *, window_size: int = -1, num_sink_tokens: int = 0, page_size: int = 128,
+                  caches: Union[torch.Tensor, Sequence[torch.Tensor]] = (), num_shared: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Give back the pages that no request needs any more.
 
     Row ``b`` keeps the pages of its first ``kv_lens[b]`` tokens: 0 for a request that ended, less than before where drafted tokens were
@@ -190,21 +192,35 @@ def kv_pages_free(block_table: torch.Tensor, num_held: torch.Tensor, kv_lens: to
 
     A page of several rows (``shares``) loses a share for each and goes onto the stack with the last; without ``shares`` each page is in one row.
     Pages are pushed in the order of the rows and their entries.  Returns ``num_freed`` (int32 ``[1]``): how many were pushed.  ``free_pages`` has
-    room for every page of the pool."""
+    room for every page of the pool.
+
+    A row that is cut back *into* a page it shares (below the length it was forked at, or its fork's) would write its next token into the other rows'
+    page.  With ``caches`` (all of them, as ``kv_pages_fork`` takes them) such a row gets a page of its own from the stack, in the order of the rows, with
+    a copy of its tokens, and gives up its share; of rows that are all cut back into one page the last keeps it.  ``num_shared`` (int32 ``[1]``, set
+    here) counts the rows that are left with such a page: all of them without ``caches``, with them those that found the stack empty.  They must not be
+    written to."""
     others = {"free_pages": (free_pages, None), "num_free": (num_free, 1)}
     if shares is not None:
         others["shares"] = (shares, None)
+    if num_shared is not None:
+        others["num_shared"] = (num_shared, 1)
     dev, B, width, stride = _tables(block_table, page_size, {"num_held": num_held, "kv_lens": kv_lens}, others)
     window = -1 if window_size is None else int(window_size)
     if window == 0 or window < -1 or window > (1 << 31) - 1:
         raise ValueError(f"window_size must be -1 (no window) or from 1 to 2^31 - 1, got {window_size}")
     if not 0 <= num_sink_tokens <= (1 << 31) - 1:
         raise ValueError(f"num_sink_tokens must be from 0 to 2^31 - 1, got {num_sink_tokens}")
+    packed, num = b"", 0
+    if num_shared is not None or len(caches):
+        if shares is None:
+            raise ValueError("caches and num_shared need shares: without them each page is in one row")
+        packed, num, _ = _cache_list(caches, shares.shape[0], page_size, dev, True)
     buf = torch.empty(_workspace("free", B, width) + 1, dtype=torch.int32, device=dev)
     ptr = buf.data_ptr()
     _launch(dev, _lib.lib.msa_pages_free, _lib.pages_free_args(
-        block_table.data_ptr(), num_held.data_ptr(), kv_lens.data_ptr(), free_pages.data_ptr(), num_free.data_ptr(), 0 if shares is None else shares.data_ptr(),
-        ptr, ptr + 4, stride, B, width, page_size, free_pages.shape[0], (1 << 31) - 1 if shares is None else shares.shape[0], max(window, 0),
+        _address(packed) or 0, block_table.data_ptr(), num_held.data_ptr(), kv_lens.data_ptr(), free_pages.data_ptr(), num_free.data_ptr(),
+        0 if shares is None else shares.data_ptr(), ptr, 0 if num_shared is None else num_shared.data_ptr(), ptr + 4, stride, num, B, width, page_size,
+        free_pages.shape[0], (1 << 31) - 1 if shares is None else shares.shape[0], max(window, 0),
         int(num_sink_tokens) if window > 0 else 0), "msa_pages_free")
     return buf[:1]
 
