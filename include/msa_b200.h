@@ -115,6 +115,7 @@ typedef struct MsaFmhaParams {
   int32_t window;          /* > 0: row i, at place t = i + qo_offset, sees key j <= t iff j > t - window or j < sink_tokens.
                               Dense work lists made with the same two numbers, MSA_FLAG_OUT_O only; 0: every key up to t */
   int32_t sink_tokens;
+  int32_t num_sms;         /* with a window: SMs that CTAs which share an item are spread over; 0 = all 148                */
   int32_t num_page_entries; /* length of kv_indices: places past its end read as its last entry; 0 = not given,
                               every place that the lengths reach is read (kv_dtype = MSA_DT_KV4: num_logical_pages) */
 } MsaFmhaParams;

@@ -54,6 +54,7 @@ int validate_fmha(const MsaFmhaParams& p, bool own_scratch) {
   if (has_s && p.max_score_dtype != MSA_DT_F32 && p.max_score_dtype != MSA_DT_BF16) return MSA_ERR_UNSUPPORTED;
   if (p.window < 0 || p.sink_tokens < 0 || (p.sink_tokens > 0 && p.window == 0)) return MSA_ERR_BAD_ARG;
   if (p.window > 0 && (sparse || has_s)) return MSA_ERR_UNSUPPORTED;
+  if (p.num_sms < 0) return MSA_ERR_BAD_ARG;
   if (sparse) {
     if (!p.kv_block_indexes || !p.token_batch || p.kv_block_num <= 0) return MSA_ERR_BAD_ARG;
     if (p.page_size != msa::kKvTile) return MSA_ERR_UNSUPPORTED;   // a selected block is one 128-key page

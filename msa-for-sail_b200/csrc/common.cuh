@@ -65,6 +65,8 @@ __device__ __forceinline__ int window_first(int place, int kv_len, int window) {
   const long long lo = static_cast<long long>(place) - window + 1;
   return lo < 0 ? 0 : lo < kv_len ? static_cast<int>(lo) : kv_len;
 }
+// SMs that the CTAs of a call may be spread over.
+inline int sms_of(const MsaFmhaParams& p) { return p.num_sms > 0 && p.num_sms < 148 ? p.num_sms : 148; }
 // Factor of the scores where masked ones are -inf: -inf * 0 is no number, the smallest one changes no score by as much as its last bit.
 __device__ __forceinline__ float masked_scale(float scale) { return scale == 0.f ? 1.17549435e-38f : scale; }
 

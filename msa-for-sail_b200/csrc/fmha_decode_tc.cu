@@ -1233,7 +1233,7 @@ int fmha_decode_tc_launch(const MsaFmhaParams& p, cudaStream_t stream) {
   int cluster = 1;
   if (p.window > 0 && !p.partial_o) {
     const int64_t pages = (static_cast<int64_t>(p.window) + p.decode_rows / p.pack) / BN + p.sink_tokens / BN + 1;
-    cluster = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({2, pages, 2 * 148 * 9 / 10 / grid64})));
+    cluster = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({2, pages, 2 * sms_of(p) * 9 / 10 / grid64})));
   }
   return launch_chained_clusters(kern, static_cast<unsigned>(cluster), static_cast<unsigned>(grid64 * cluster), NTHREADS, smem, stream, p, tq, tk, tv) == cudaSuccess
              ? MSA_OK : MSA_ERR_LAUNCH;

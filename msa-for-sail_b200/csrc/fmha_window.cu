@@ -633,7 +633,7 @@ int cluster_of(const MsaFmhaParams& p, cudaLaunchConfig_t config, int device) {
   const int64_t keys = static_cast<int64_t>(p.window) + p.sink_tokens + p.decode_rows / p.pack;
   const int64_t most = std::min<int64_t>(kMaxCluster, (keys + kWarps * unit_keys<F8>() - 1) / (kWarps * unit_keys<F8>()));
   for (int s = static_cast<int>(most); s > 1; --s) {
-    if (static_cast<int64_t>(p.num_work) * s > 148 * Cfg<NT>::CTAS) continue;
+    if (static_cast<int64_t>(p.num_work) * s > sms_of(p) * Cfg<NT>::CTAS) continue;
     if (!fit[device][s]) {
       cudaLaunchAttribute attr = {};
       attr.id = cudaLaunchAttributeClusterDimension;
@@ -706,7 +706,7 @@ int launch(const MsaFmhaParams& p, cudaStream_t stream) {
 // and 17.4, 512 50 and 44; with 32 rows registers run out.
 int fmha_window_rows(const MsaFmhaParams& p) {
   if (p.kv_dtype != MSA_DT_E4M3) return 32;
-  return p.page_size == kKvTile && 128 % p.pack == 0 && p.num_work > 74 ? 8 : 16;
+  return p.page_size == kKvTile && 128 % p.pack == 0 && p.num_work > sms_of(p) / 2 ? 8 : 16;
 }
 int fmha_window_supported(const MsaFmhaParams& p) {
   if (p.window <= 0 || (p.flags & MSA_FLAG_SPARSE) || p.decode_rows < 1 || p.decode_rows > fmha_window_rows(p)) return 0;

@@ -48,7 +48,8 @@ class MsaFmhaParams(ctypes.Structure):
         ("num_work", _i32), ("block_m", _i32), ("pack", _i32), ("page_size", _i32),
         ("kv_block_num", _i32), ("num_splits", _i32), ("max_k_tiles", _i32), ("num_logical_pages", _i32), ("decode_rows", _i32),
         ("q_dtype", _i32), ("kv_dtype", _i32), ("max_score_dtype", _i32), ("flags", _i32),
-        ("sm_scale", _f32), ("out_scale", _f32), ("window", _i32), ("sink_tokens", _i32), ("num_page_entries", _i32),
+        ("sm_scale", _f32), ("out_scale", _f32), ("window", _i32), ("sink_tokens", _i32), ("num_sms", _i32),
+        ("num_page_entries", _i32),
     ]
 
 

@@ -539,7 +539,7 @@ def _fmha_sail_plan(
         "total_qo_len": total_q,
         "batch_size": batch,
         "causal": causal,
-        "window": window,
+        "window": window, "num_sms": num_sms,
         "_host": {"qo_lens": qo_lens, "kv_lens": kv_lens, "qo_offset": offs},
     })
     return info
@@ -564,11 +564,11 @@ def _fmha_sail_plan_device(qo_segment_lens, kv_segment_lens, num_qo_heads, hkv, 
             raise ValueError(f"graph_safe=True requires {name} as a contiguous int32 CUDA tensor")
     h_r = num_qo_heads // hkv
     is_sparse = kv_block_num > 0 and page_size > 0
+    num_sms = _num_sms(dev)
+    if usable_SM_count > 0:
+        num_sms = min(num_sms, usable_SM_count)
     if is_sparse:
         pack, block_m = h_r, _block_m(h_r)
-        num_sms = _num_sms(dev)
-        if usable_SM_count > 0:
-            num_sms = min(num_sms, usable_SM_count)
         if use_kv4_cache:
             splits = _kv4_sparse_splits(max_total_q * hkv * -(-h_r // 16), kv_block_num, max(1, num_kv_splits), num_sms, h_r)
         else:
@@ -637,7 +637,7 @@ def _fmha_sail_plan_device(qo_segment_lens, kv_segment_lens, num_qo_heads, hkv, 
         "orig_num_qo_heads": num_qo_heads, "num_kv_heads": hkv, "qo_len_uniform": qo_len_uniform,
         "graph_safe": True, "page_size": page_size, "kv_block_num": kv_block_num if is_sparse else -1,
         "is_sparse": is_sparse, "total_qo_len": max_total_q, "batch_size": batch, "causal": causal,
-        "window": window, "_host": None,
+        "window": window, "num_sms": num_sms, "_host": None,
     })
     return info
 
@@ -1077,7 +1077,8 @@ def _window_params(q_dtype, kv_dtype, plan):
     h_r = plan["orig_num_qo_heads"] // plan["num_kv_heads"]
     p = _lib.MsaFmhaParams(num_work=plan["num_work"], block_m=plan["qo_tile_size"], pack=pack, page_size=page_size, num_splits=splits,
                            num_qo_heads=plan["orig_num_qo_heads"], num_kv_heads=plan["num_kv_heads"], batch=plan["batch_size"],
-                           q_dtype=_dt_code(q_dtype), kv_dtype=_dt_code(kv_dtype), flags=FLAG_OUT_O, window=plan["window"][0], sink_tokens=plan["window"][1])
+                           q_dtype=_dt_code(q_dtype), kv_dtype=_dt_code(kv_dtype), flags=FLAG_OUT_O, window=plan["window"][0], sink_tokens=plan["window"][1],
+                           num_sms=plan["num_sms"])
     work = "work"
     if plan.get("work_tc") is not None and q_dtype == kv_dtype and page_size in (0, 128) and _USE_TC and (plan["tc_preferred"] or _FORCE_TC):
         work, p.num_work, p.block_m, p.num_splits = "work_tc", plan["num_work_tc"], 256, 1
