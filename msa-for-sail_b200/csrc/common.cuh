@@ -67,8 +67,14 @@ __device__ __forceinline__ int window_first(int place, int kv_len, int window) {
 }
 // SMs that the CTAs of a call may be spread over.
 inline int sms_of(const MsaFmhaParams& p) { return p.num_sms > 0 && p.num_sms < 148 ? p.num_sms : 148; }
-// Factor of the scores where masked ones are -inf: -inf * 0 is no number, the smallest one changes no score by as much as its last bit.
-__device__ __forceinline__ float masked_scale(float scale) { return scale == 0.f ? 1.17549435e-38f : scale; }
+// Factor of the scores where masked ones are -inf, a positive number: -inf * 0 is no number, the smallest one changes no score by as much as its last
+// bit.  The sign of a negative one (a head's own scale) goes to Q, or to the scores before they are masked and the largest is sought.
+__device__ __forceinline__ float masked_scale(float scale) { return scale == 0.f ? 1.17549435e-38f : fabsf(scale); }
+template <int N>
+__device__ __forceinline__ void turn_scores(uint32_t (&s)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) s[i] ^= 0x80000000u;
+}
 
 // ---- kernels of one stream without a gap between them ----
 // A kernel launched with launch_chained() may start while the kernel before it in the stream still runs: once every CTA of

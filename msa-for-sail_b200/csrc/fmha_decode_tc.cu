@@ -656,7 +656,8 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
         mbar_arrive(bar(Q_FULL));
       }
     }
-    if constexpr (WIN) scale_log2 = masked_scale(scale_log2);
+    [[maybe_unused]] bool turned = false;
+    if constexpr (WIN) { turned = scale_log2 < 0.f; scale_log2 = masked_scale(scale_log2); }
 
     if constexpr (QUAD) {
       // quadrant `warp` owns key columns [32 warp, 32 warp + 32) of every tile
@@ -773,6 +774,10 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
           else tmem_ld32(tS + part * CW + c * LD, sv[c]);
         }
         tmem_wait_ld();
+        if (turned) {
+#pragma unroll
+          for (int c = 0; c < CW / LD; ++c) turn_scores(sv[c]);
+        }
         if (pos0 + CW - 1 > lim) {
 #pragma unroll
           for (int e = 0; e < CW; ++e)

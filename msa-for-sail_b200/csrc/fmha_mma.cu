@@ -107,7 +107,8 @@ fmha_mma_kernel(const __grid_constant__ MsaFmhaParams p) {
 
   float scale_log2 = p.sm_scale * kLog2e;
   if (p.k_scale_head) scale_log2 *= p.k_scale_head[kvh];
-  if constexpr (WIN) scale_log2 = masked_scale(scale_log2);
+  [[maybe_unused]] bool turned = false;
+  if constexpr (WIN) { turned = scale_log2 < 0.f; scale_log2 = masked_scale(scale_log2); }
 
   // ---------------- Q tile -> shared (compute type) ----------------
   {
@@ -291,6 +292,15 @@ fmha_mma_kernel(const __grid_constant__ MsaFmhaParams p) {
         ldmatrix_x4(smem_u32(tK + swz_off(key, ch)), b0, b1, b2, b3);
         mma_16816<HF>(acc_s[np * 2], qf[ks], b0, b1);
         mma_16816<HF>(acc_s[np * 2 + 1], qf[ks], b2, b3);
+      }
+    }
+
+    if constexpr (WIN) {
+      if (turned) {
+#pragma unroll
+        for (int n = 0; n < NTILE_S; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc_s[n][e] = -acc_s[n][e];
       }
     }
 

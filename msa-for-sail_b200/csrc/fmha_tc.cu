@@ -498,6 +498,20 @@ fmha_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant__ 
         }
         continue;
       }
+      if constexpr (WIN) {
+        // The sign of a head's factor of the scores goes to Q: masked scores are -inf.  (Scores turned by the softmax warps: a chunk 362 -> 405 us,
+        // whether or not there is a sign.)
+        if (alive && p.sm_scale * (p.k_scale_head ? p.k_scale_head[w.kvh] : 1.f) < 0.f) {
+          const uint32_t sign = F8 ? 0x80808080u : 0x80008000u;
+          uint4* q = reinterpret_cast<uint4*>(smem_gen + OFF_Q);
+          for (int i = lane; i < 2 * TILE_BYTES / 16; i += 32) {
+            const uint4 v = q[i];
+            q[i] = make_uint4(v.x ^ sign, v.y ^ sign, v.z ^ sign, v.w ^ sign);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+        }
+      }
       if (alive) alive = mbar_wait_warp(bar(K_FULL + tile % KSTAGES), (tile / KSTAGES) & 1, abort_flag, spin_limit);
       if (!alive) break;
       tc_fence_after();

@@ -1488,8 +1488,8 @@ def fmha_sail(
     weight within 2^-8 of itself, and what small ones lose beyond that is together at most 1.5 * 2^-8 of their row's sum.
     Prompts of bf16 queries over an e4m3 cache run on the generic kernel, with weights in fp16.  The
     plan has its offsets (no ``q_offset_override``), the factor of the scores (``sm_scale * q_scale *
-    k_scale``) is not negative, and partials of a split are the call's own, so that one plan may run on
-    two streams, or in two graphs, at a time.
+    k_scale``) is not negative as a float (per head, in a tensor, it may have any sign on every kernel), and
+    partials of a split are the call's own, so that one plan may run on two streams, or in two graphs, at a time.
     """
     mixed, cut, batch_size, first, second = plan_info
     if not mixed:
