@@ -277,7 +277,8 @@ int msa_fmha_fwd_split_static(const MsaFmhaParams* params, const int32_t* splits
                               msa_stream_t stream);
 
 /* msa_fmha_fwd with split partials (partial_o, partial_lse and num_splits set) and the merge of them, msa_lse_merge_many, into out and lse: one
- * call.  out_dtype: MSA_DT_BF16 or MSA_DT_F32, strides of out in elements of it. */
+ * call.  out_dtype: MSA_DT_BF16 or MSA_DT_F32, strides of out in elements of it; its rows begin at multiples of 16 bytes, as in an unsplit call.
+ * What the merge would refuse is refused before anything is launched. */
 int msa_fmha_fwd_merged(const MsaFmhaParams* params, const int32_t* splits_per_row, int32_t out_dtype, msa_stream_t stream);
 
 /* msa_fmha_fwd with kv_dtype = MSA_DT_KV4: q bf16 or e4m3, paged k and v with page_size 128, MSA_FLAG_OUT_O only (with or

@@ -93,6 +93,12 @@ extern "C" int msa_fmha_fwd(const MsaFmhaParams* pp, msa_stream_t stream_) {
 extern "C" int msa_fmha_fwd_merged(const MsaFmhaParams* pp, const int32_t* splits_per_row, int32_t out_dtype, msa_stream_t stream) {
   if (!pp || !pp->partial_o || !pp->partial_lse || !pp->out || pp->num_splits < 1) return MSA_ERR_BAD_ARG;
   if (out_dtype != MSA_DT_BF16 && out_dtype != MSA_DT_F32) return MSA_ERR_UNSUPPORTED;
+  // all that the merge asks for, before anything is launched; `out` as in an unsplit call, rows that begin at multiples of 16 bytes
+  const int oe = out_dtype == MSA_DT_BF16 ? 2 : 4;
+  if ((reinterpret_cast<uintptr_t>(pp->partial_o) & 15) || (reinterpret_cast<uintptr_t>(pp->out) & 15) || pp->out_stride_tok * oe % 16 ||
+      pp->out_stride_head * oe % 16)
+    return MSA_ERR_BAD_ARG;
+  if (static_cast<int64_t>(pp->total_q) * pp->num_qo_heads > 0x7fffffffLL) return MSA_ERR_TOO_LARGE;
   MsaFmhaParams p = *pp;
   p.out = nullptr;
   p.lse = nullptr;

@@ -1177,6 +1177,9 @@ def _fmha_sail_window(q, k, v, plan, kv_indices, kv_block_indexes, q_offset_over
             partials = torch.empty(rows * 129, dtype=torch.float32, device=dev)
             part = partials.data_ptr()
             p.partial_lse = part + rows * 512
+            # (an fp32 result may have any strides, as where it is converted below; a bf16 one has rows that begin at multiples of 16 bytes on both paths)
+            if out_dtype is torch.float32 and (out.data_ptr() | o_stride[0] * 4 | o_stride[1] * 4) & 15:
+                kernel_out, o_stride = torch.empty(q_shape, dtype=torch.float32, device=dev), None
         elif out_dtype is torch.float32:
             kernel_out, o_stride = torch.empty(q_shape, dtype=torch.bfloat16, device=dev), None
         if o_stride is None:
@@ -1191,6 +1194,8 @@ def _fmha_sail_window(q, k, v, plan, kv_indices, kv_block_indexes, q_offset_over
         p.sm_scale, p.out_scale = scale, out_scale
         if splits > 1:
             _lib.check(_lib.lib.msa_fmha_fwd_merged(ctypes.byref(p), _ptr(plan["num_kv_splits_per_row"]), _dt_code(out_dtype), _stream()), "msa_fmha_fwd_merged")
+            if kernel_out is not out:
+                out.copy_(kernel_out)
         else:
             _lib.check(_lib.lib.msa_fmha_fwd(ctypes.byref(p), _stream()), "msa_fmha_fwd")
             if kernel_out is not out:
