@@ -1070,13 +1070,13 @@ _WINDOW_STRIDES = struct.Struct("@10q")       # q, k, v, out
 _WINDOW_TABLES_AT, _WINDOW_STRIDES_AT = _lib.MsaFmhaParams.qo_start.offset, _lib.MsaFmhaParams.q_stride_tok.offset
 
 
-def _window_params(q_dtype, kv_dtype, plan):
+def _window_params(q_dtype, kv_dtype, num_kv_heads, plan):
     """What is the same in every call with this plan and these types: the arguments' bytes (the plan's numbers and the choice of a kernel, no
     addresses), the number of splits, and the name of the work list."""
     page_size, splits, pack = max(0, plan["page_size"]), plan["num_kv_splits"], plan["pack_factor"]
-    h_r = plan["orig_num_qo_heads"] // plan["num_kv_heads"]
+    h_r = plan["orig_num_qo_heads"] // num_kv_heads
     p = _lib.MsaFmhaParams(num_work=plan["num_work"], block_m=plan["qo_tile_size"], pack=pack, page_size=page_size, num_splits=splits,
-                           num_qo_heads=plan["orig_num_qo_heads"], num_kv_heads=plan["num_kv_heads"], batch=plan["batch_size"],
+                           num_qo_heads=plan["orig_num_qo_heads"], num_kv_heads=num_kv_heads, batch=plan["batch_size"],
                            q_dtype=_dt_code(q_dtype), kv_dtype=_dt_code(kv_dtype), flags=FLAG_OUT_O, window=plan["window"][0], sink_tokens=plan["window"][1],
                            num_sms=plan["num_sms"])
     work = "work"
@@ -1126,8 +1126,11 @@ def _fmha_sail_window(q, k, v, plan, kv_indices, kv_block_indexes, q_offset_over
             raise ValueError(f"plan allows at most {plan['total_qo_len']} query tokens, q has {nnz_qo}")
     elif plan["total_qo_len"] != nnz_qo:
         raise ValueError(f"plan was made for {plan['total_qo_len']} query tokens, q has {nnz_qo}")
-    if plan["orig_num_qo_heads"] != num_qo_heads or plan["num_kv_heads"] != num_kv_heads:
+    if plan["orig_num_qo_heads"] != num_qo_heads:
         raise ValueError("plan head counts do not match q / k")
+    if plan["num_kv_heads"] != num_kv_heads:  # (a plan made without num_kv_heads: as in _fmha_sail)
+        if plan.get("kv_heads_given", True) or plan["pack_factor"] != 1 or num_kv_heads == 0 or num_qo_heads % num_kv_heads:
+            raise ValueError("plan head counts do not match q / k")
     if paged and (kv_indices.dtype is not torch.int32 or kv_indices.dim() != 1 or not kv_indices.is_contiguous()):
         raise ValueError("kv_indices must be a contiguous int32 vector")
     if check_input_valid and plan["_host"] is not None:
@@ -1149,10 +1152,10 @@ def _fmha_sail_window(q, k, v, plan, kv_indices, kv_block_indexes, q_offset_over
     kept = plan.get("_window_params")
     if kept is None:
         kept = plan["_window_params"] = {}
-    key = (q_dtype, k_dtype, _USE_TC, _FORCE_TC, _USE_DECODE_TC)
+    key = (q_dtype, k_dtype, num_kv_heads, _USE_TC, _FORCE_TC, _USE_DECODE_TC)
     base = kept.get(key)
     if base is None:
-        base = kept[key] = _window_params(q_dtype, k_dtype, plan)
+        base = kept[key] = _window_params(q_dtype, k_dtype, num_kv_heads, plan)
     p, splits, work = _lib.MsaFmhaParams.from_buffer_copy(base[0]), base[1], plan[base[2]]
     sm_scale = 0.08838834764831845 if sm_scale is None else float(sm_scale)     # 1 / sqrt(128)
     k_s, out_scale = 1.0, 1.0
