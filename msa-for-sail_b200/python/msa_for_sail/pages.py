@@ -33,10 +33,12 @@ def _pieces(shape, stride, size, kv4, page_size, by_token):
             # a 4-bit cache: the codes of a page and head, then the scales
             codes = KV4_TILE * 64
             return [(0, stride[0], stride[1], shape[1], codes, 64), (codes, stride[0], stride[1], shape[1], KV4_TILE * 8, 8)]
-        if shape[2] == page_size and stride[2:] == (shape[3], 1):             # HND
+        # (both dimensions as long as a page: either could be the tokens, the page is copied whole)
+        hnd, nhd = shape[2] == page_size != shape[1], shape[1] == page_size != shape[2]
+        if hnd and stride[2:] == (shape[3], 1):
             row = shape[3] * size
             return [(0, stride[0] * size, stride[1] * size, shape[1], page_size * row, row)]
-        if shape[1] == page_size and stride[2:] == (shape[3], 1):             # NHD
+        if nhd and stride[2:] == (shape[3], 1):
             row = shape[2] * shape[3] * size
             return [(0, stride[0] * size, stride[1] * size, page_size, row, -1)]
     # the innermost dimensions as far as they are contiguous; what is left has to be one step
@@ -156,8 +158,10 @@ def kv_pages_fork(block_table: torch.Tensor, num_held: torch.Tensor, kv_lens: to
     """Make row ``children[i]`` a fork of row ``parents[i]``: a request with the same first ``kv_lens[parent]`` tokens.
 
     Full pages are shared (``shares`` + 1 each); the last page, where it is partly filled, is taken from the stack, in the order of the entries, and
-    the used part is copied in every one of ``caches`` (bf16, e4m3 or any other type as ``[pages, Hkv, page, D]`` or ``[pages, page, Hkv, D]``, 4-bit
-    caches; of other tensors with pages as the first dimension the whole page is copied).  So whoever writes next writes into a page of its
+    the used part is copied in every one of ``caches``: 4-bit caches, and tensors of any type with four dimensions that are taken as ``[pages, Hkv, page, D]``
+    if the third is ``page_size``, as ``[pages, page, Hkv, D]`` if the second is.  Of other tensors with pages as the first dimension, and where both
+    are, the whole page is copied; one with four dimensions and such a length that means something else (keys with the tokens last, say) is given as
+    a view, ``t.flatten(1)``.  So whoever writes next writes into a page of its
     own, as long as neither row is cut back into a page that they share (``kv_pages_free`` with ``caches`` sees to that).  ``num_held`` and ``kv_lens``
     (int32 ``[B]``) of the child are set.
 

@@ -193,3 +193,16 @@ def test_rows_cut_back_needs_shares():
         with pytest.raises(ValueError):
             msa.kv_pages_free(*t, _i32([0] * 4), page_size=16, **kw)
     assert t[0].tolist() == [[0, 1]] and t[2].tolist() == [20]
+
+
+def test_forks_copy_whole_pages_where_the_tokens_could_be_either_dimension():
+    P, page = 6, 16
+    both = torch.randint(0, 256, (P, page, page, 8), dtype=torch.uint8, device=DEV)              # heads or tokens
+    last = torch.randint(0, 256, (P, 3, page, page), dtype=torch.uint8, device=DEV)              # tokens last: given as a view
+    want = [both.clone(), last.clone()]
+    table, free = _i32([[2], [-1]]), _i32([4])
+    _msa().kv_pages_fork(table, _i32([1, 0]), _i32([5, 0]), _i32([0]), _i32([1]), free, _i32([1]), _i32([0] * P), [both, last.flatten(1)], page)
+    for t, w in zip((both, last), want):
+        w[4] = w[2]
+        assert torch.equal(t, w)
+    assert table.tolist() == [[2], [4]]
