@@ -23,6 +23,7 @@ constexpr int kScanThreads = 1024;
 constexpr int kChunk = 16384;                  // bytes of a piece of a page that a CTA copies at a time
 constexpr int kMaxCaches = 64;                 // of one launch
 constexpr int kCopyCtas = 148 * 8;
+constexpr int kMostIndex = INT_MAX - (1 << 20);               // of rows, columns, pages: the kernels' loops step by less than 2^20 beyond it, in 32 bits
 
 // ---------------------------------------------------------------------------------------------------------------------------
 // copies
@@ -863,7 +864,7 @@ extern "C" int msa_pages_fork(const MsaPagesForkArgs* pa, msa_stream_t stream) {
   if (!a.num_free || !a.workspace || (a.count > 0 && (!a.parents || !a.children))) return MSA_ERR_BAD_ARG;
   if (a.batch > 0 && (!a.num_held || !a.kv_len || (a.table_width > 0 && !a.block_table))) return MSA_ERR_BAD_ARG;
   if ((a.free_capacity > 0 && !a.free_pages) || (a.num_pages > 0 && !a.shares)) return MSA_ERR_BAD_ARG;
-  if (a.count > (1 << 24)) return MSA_ERR_TOO_LARGE;
+  if (a.count > (1 << 24) || a.table_width > kMostIndex) return MSA_ERR_TOO_LARGE;
   msa::NvtxRange range("msa_pages_fork");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (msa::launch_chained(pages_fork_plan_kernel, 1, kScanThreads, 0, st, a) != cudaSuccess) return MSA_ERR_LAUNCH;
@@ -892,7 +893,7 @@ extern "C" int msa_pages_free(const MsaPagesFreeArgs* pa, msa_stream_t stream) {
   if (const int rc = check_caches(a.caches, a.num_caches, a.num_pages, a.page_size)) return rc;
   if ((a.num_caches > 0 || a.num_shared) && !a.shares) return MSA_ERR_BAD_ARG;
   const int64_t entries = static_cast<int64_t>(a.batch) * a.table_width;
-  if (entries > INT_MAX / 2) return MSA_ERR_TOO_LARGE;
+  if (entries > INT_MAX / 2 || a.batch > kMostIndex) return MSA_ERR_TOO_LARGE;
   msa::NvtxRange range("msa_pages_free");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (const int rc = give_back(a, entries, st)) return rc;
@@ -919,6 +920,7 @@ extern "C" int msa_pages_compact(const MsaPagesCompactArgs* pa, msa_stream_t str
   if (a.batch < 0 || a.table_width < 0 || a.table_stride < a.table_width || a.free_capacity < 0) return MSA_ERR_BAD_ARG;
   if (!a.num_free || !a.workspace || !a.num_moved || (a.free_capacity > 0 && !a.free_pages) || (a.num_pages > 0 && (!a.src || !a.dst))) return MSA_ERR_BAD_ARG;
   if (a.batch > 0 && (!a.num_held || (a.table_width > 0 && !a.block_table))) return MSA_ERR_BAD_ARG;
+  if (a.num_pages > kMostIndex || a.batch > kMostIndex || a.table_width > kMostIndex) return MSA_ERR_TOO_LARGE;
   msa::NvtxRange range("msa_pages_compact");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const Sets s = sets_of(a);
