@@ -203,9 +203,9 @@ __device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
 //
 // So what weights are relative to must not lie far above most of a row's mass: one heavy key (a sink) with weight 2^4 would leave nothing of thousands
 // of keys ten nats below it, 16 % of the mass with 4 096 of them.  It follows a tile's largest score down as well as up (pair_lowers).  Of a tile of n keys
-// 1.5 * 2^-10 n is lost at most.  That is left so where the tile's weights have a sum of n / 4, or the row's have one of n / 4 for each tile that it
-// has; else it goes down to the tile's largest score.  Either way all that is lost of a row is 1.5 * 2^-8 of its sum at most.  A row of scores that lie
-// within a few nats has such a sum after its first tiles and never gets there.
+// 1.5 * 2^-10 n is lost at most.  That is left so where the tile's weights have a sum of n / 4, or the row's have one of a quarter of its keys so far; else
+// it goes down to the tile's largest score.  Either way all that is lost of a row is 1.5 * 2^-8 of its sum at most.  A row of scores that lie within a few
+// nats has such a sum throughout.
 __device__ __forceinline__ void e4m3_pair(float a, float b, uint32_t& hi, uint32_t& lo) {
   const uint64_t x = f2_pack(a, b), t = f2_fma(x, f2_pack(1048577.f, 1048577.f), 0), minus = f2_pack(-1.f, -1.f);
   const uint64_t h = f2_fma(f2_fma(x, minus, t), minus, t), rest = f2_fma(h, minus, x);
@@ -223,41 +223,45 @@ __device__ __forceinline__ float exp2_fast(float x) {
 }
 
 // What a row's weights are relative to, for pairs of e4m3 values (e4m3_pair): a score equal to it has weight 2^kPairOffset, one kPairRescale (log2)
-// above it raises it.
-constexpr float kPairOffset = 5.f, kPairRescale = 3.8f;
+// above it raises it, to kPairRise below that score.
+constexpr float kPairOffset = 5.f, kPairRescale = 3.8f, kPairRise = 2.8f;
 constexpr float kPairEnough = 0.25f;                         // sum of weights, for each key, of which the loss is small enough
-// Whether it goes down to a tile's largest score: not where `tile`, a lower bound of the sum of the tile's n weights, or `row`, the sum of the row's
-// weights before, is enough (for the tile; for all `tiles`).  Nothing 2^60 below is looked at: fewer than 2^31 keys have no weight there, and sums
-// and O stay finite.  (A tile without a key has top -inf.)
-__device__ __forceinline__ bool pair_lowers(float ref, float top, float tile, float row, int n, int tiles) {
-  const float enough = kPairEnough * static_cast<float>(n), down = ref - top;
-  return tile < enough && row < enough * static_cast<float>(tiles) && down > 0.f && down <= 60.f;
+// It goes down to a tile's largest score where neither `tile`, (a lower bound of) the sum of the tile's n weights, is enough for the tile's keys, nor that
+// and `row`, the sum of the row's weights before, for these and `lossy` keys before.  Nothing 2^60 below is looked at: fewer than 2^31 keys have no weight
+// there, and sums and O stay finite.  (A tile without a key has top -inf.)
+__device__ __forceinline__ bool pair_lowers(float ref, float top, float tile, float row, int n, float lossy) {
+  const float down = ref - top;
+  return tile < kPairEnough * static_cast<float>(n) && row + tile < kPairEnough * (lossy + static_cast<float>(n)) && down > 0.f && down <= 60.f;
 }
 // The next `ref` of a row, by a thread that has all of it: `top` are the largest scores of N parts of the tile, to be multiplied by `scale`, `sum` is
-// the row's so far, relative to `ref`.  settled: all rows of the warp have enough for all tiles, which only a rise of `ref` changes.
+// the row's so far, relative to `ref`.  lossy: keys so far, as far as what they lost weighs now (it moves with the sum).  settled: all rows of the warp
+// have enough for what they lost and for the `left` keys from this tile on, which only a rise of `ref` changes.
 template <int N>
-__device__ __forceinline__ float pair_reference(float ref, float sum, const float (&top)[N], float scale, int n, int tiles, bool exists, bool& settled) {
+__device__ __forceinline__ float pair_reference(float ref, float sum, float& lossy, const float (&top)[N], float scale, int n, int left, bool exists, bool& settled) {
   float best = top[0];
 #pragma unroll
   for (int i = 1; i < N; ++i) best = fmaxf(best, top[i]);
   best *= scale;
   const bool up = best - ref > kPairRescale;
-  float now = up ? best : ref;
+  float now = up ? (ref == -INFINITY ? best : best - kPairRise) : ref;
   if (!settled || __any_sync(0xffffffffu, up)) {
-    const float row = up ? sum * exp2_fast(ref - now) : sum;
-    settled = __all_sync(0xffffffffu, row >= kPairEnough * static_cast<float>(n) * static_cast<float>(tiles) || !exists);
-    if (!settled) {
+    const float f = up ? exp2_fast(ref - now) : 1.f, row = sum * f;
+    lossy *= f;
+    settled = __all_sync(0xffffffffu, row >= kPairEnough * (lossy + static_cast<float>(left)) || !exists);
+    if (!settled && !__all_sync(0xffffffffu, row >= kPairEnough * (lossy + static_cast<float>(n)) || !exists)) {
       float tile = 0.f;
 #pragma unroll
       for (int i = 0; i < N; ++i) tile += exp2_fast(fmaf(top[i], scale, kPairOffset - now));
-      if (pair_lowers(now, best, tile, row, n, tiles)) now = best;
+      if (pair_lowers(now, best, tile, row, n, lossy)) {
+        lossy *= exp2_fast(now - best);
+        now = best;
+      }
     }
   }
+  lossy += static_cast<float>(n);
   return now;
 }
 
-// Row tile [rows][128 x 16-bit]: 16 chunks of 16 bytes per row, chunk index XOR-ed with
-// (row & 7) so that ldmatrix reads and 16-byte row writes are bank-conflict free.
 __device__ __forceinline__ uint32_t swz_off(int row, int chunk) {
   return static_cast<uint32_t>(row * 256 + ((chunk ^ (row & 7)) << 4));
 }

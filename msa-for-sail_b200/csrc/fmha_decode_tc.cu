@@ -760,6 +760,7 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
       constexpr int RC = PARTS == 1 ? 16 : 32;               // columns of O scaled at a time: 64 scores leave no registers for 32
       const int part = trow / ROWS;
       [[maybe_unused]] bool settled = false;
+      [[maybe_unused]] float lossy = 0.f;
       for (int j = 0; j < n_tiles && alive; ++j) {
         const uint32_t tS = tmem + (j % NBUF) * TK + lane_addr;
         alive = mbar_wait_warp(bar(S_FULL + j % NBUF), (j / NBUF) & 1, abort_flag);
@@ -793,7 +794,7 @@ decode_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant_
         for (int e = 0; e < CW; e += 2) mxs[(e >> 1) & 3] = max3(mxs[(e >> 1) & 3], __uint_as_float(sv[e / LD][e % LD]), __uint_as_float(sv[e / LD][e % LD + 1]));
         float m_next;
         if constexpr (PAIR) {
-          m_next = pair_reference(m_used, l_sum, mxs, scale_log2, CW, n_tiles, row_ok, settled);
+          m_next = pair_reference(m_used, l_sum, lossy, mxs, scale_log2, CW, (n_tiles - j) * CW, row_ok, settled);
         } else {
           const float m_cand = fmaxf(m_used, fmaxf(fmaxf(mxs[0], mxs[1]), fmaxf(mxs[2], mxs[3])) * scale_log2);
           m_next = (m_cand - m_used) > kRescaleThreshold ? m_cand : m_used;

@@ -103,6 +103,18 @@ struct Knobs {            // read only in builds with -DMSA_DEBUG_HOOKS
   uint32_t spin_limit;         // > 0: polls a bounded wait makes before it gives up (instead of kSpinLimit)
 };
 
+// The sign of all elements of a tile in shared memory, by a warp.
+__device__ __noinline__ void turn_tile(unsigned char* tile, int bytes, uint32_t sign) {
+  uint4* q = reinterpret_cast<uint4*>(tile);
+#pragma unroll 1
+  for (int i = threadIdx.x & 31; i < bytes / 16; i += 32) {
+    const uint4 v = q[i];
+    q[i] = make_uint4(v.x ^ sign, v.y ^ sign, v.z ^ sign, v.w ^ sign);
+  }
+  fence_proxy_async_smem();
+  __syncwarp();
+}
+
 // HAS_O = false: score-only pass (no V, no P, no O), compiled on its own so that neither path's code is shaped
 // by the other's.
 template <bool F8, bool HAS_O, bool WIN>
@@ -463,6 +475,8 @@ fmha_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant__ 
     int n_total = 0;
     for (uint32_t it = 0; take_item(it, w, n_total, alive); ++it) {
       if (n_total == 0) continue;
+      [[maybe_unused]] bool turned = false;            // (read while Q is on its way)
+      if constexpr (WIN) turned = p.sm_scale * (p.k_scale_head ? p.k_scale_head[w.kvh] : 1.f) < 0.f;
       alive = mbar_wait_warp(bar(Q_FULL), q_loads & 1, abort_flag, spin_limit);
       ++q_loads;
       if constexpr (!HAS_O) {
@@ -501,16 +515,7 @@ fmha_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant__ 
       if constexpr (WIN) {
         // The sign of a head's factor of the scores goes to Q: masked scores are -inf.  (Scores turned by the softmax warps: a chunk 362 -> 405 us,
         // whether or not there is a sign.)
-        if (alive && p.sm_scale * (p.k_scale_head ? p.k_scale_head[w.kvh] : 1.f) < 0.f) {
-          const uint32_t sign = F8 ? 0x80808080u : 0x80008000u;
-          uint4* q = reinterpret_cast<uint4*>(smem_gen + OFF_Q);
-          for (int i = lane; i < 2 * TILE_BYTES / 16; i += 32) {
-            const uint4 v = q[i];
-            q[i] = make_uint4(v.x ^ sign, v.y ^ sign, v.z ^ sign, v.w ^ sign);
-          }
-          fence_proxy_async_smem();
-          __syncwarp();
-        }
+        if (__builtin_expect(alive && turned, 0)) turn_tile(smem_gen + OFF_Q, 2 * TILE_BYTES, F8 ? 0x80808080u : 0x80008000u);
       }
       if (alive) alive = mbar_wait_warp(bar(K_FULL + tile % KSTAGES), (tile / KSTAGES) & 1, abort_flag, spin_limit);
       if (!alive) break;
@@ -661,6 +666,7 @@ fmha_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant__ 
         if (m0 < w.ql) from_last = window_first(min(m0 + BM, w.ql) - 1 + off, kv_len, p.window);
       }
       [[maybe_unused]] bool begun = false, settled = false;
+      [[maybe_unused]] float lossy = 0.f;
       const int nx = x == 0 ? w.n_tiles[0] : w.n_tiles[1];
       const float scale_all = p.sm_scale * kLog2e * (p.k_scale_head ? p.k_scale_head[kvh] : 1.f);
       const float scale_log2 = WIN ? masked_scale(scale_all) : scale_all;
@@ -696,8 +702,7 @@ fmha_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant__ 
             float m_next;
             if constexpr (PAIR) {
               const float tops[1] = {top};
-              m_next = pair_reference(m_used, l_sum, tops, scale_log2, rest, nx, row_ok, settled);
-              settled = false;                              // (fewer keys than other tiles have)
+              m_next = pair_reference(m_used, l_sum, lossy, tops, scale_log2, rest, (nx - j) * BN, row_ok, settled);
             } else {
               const float m_cand = fmaxf(m_used, top * scale_log2);
               m_next = (m_cand - m_used) > kRescaleThreshold ? m_cand : m_used;
@@ -778,7 +783,7 @@ fmha_tc_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_constant__ 
           read(0, sv);
           tops_of(sv, 0);
           if (r == 0) trace(x, j, 2);
-          const float m_next = pair_reference(m_used, l_sum, tops, scale_log2, BN, nx, row_ok, settled);
+          const float m_next = pair_reference(m_used, l_sum, lossy, tops, scale_log2, BN, (nx - j) * BN, row_ok, settled);
           const bool moves = m_next != m_used;
           float factor = 1.f;
           if (moves) { factor = exp2_fast(m_used - m_next); m_used = m_next; l_sum *= factor; }

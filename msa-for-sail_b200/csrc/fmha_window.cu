@@ -280,7 +280,7 @@ window_decode_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_const
   }
 
   int stage = 0, parity = 0;
-  [[maybe_unused]] bool settled = false;
+  [[maybe_unused]] bool settled = !F8;
 #pragma unroll 1
   for (int i = 0; i < n_units && alive; ++i) {
     const int key0 = key_of(i);
@@ -375,104 +375,69 @@ window_decode_kernel(const __grid_constant__ MsaFmhaParams p, const __grid_const
         top[n][c] = x * fac[n][c];
         raise |= top[n][c] > m[n][c] + (kPOffset + kRescale);
       }
-    if (__any_sync(0xffffffffu, raise)) {
-      settled = false;
+    if (!settled || __any_sync(0xffffffffu, raise)) {
+      bool enough = true;
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         float k2[2];
+        [[maybe_unused]] float sum[2];
+        if constexpr (F8) f2_unpack(l[n], sum[0], sum[1]);
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           float x = top[n][c];
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
-          x = fmaxf(x - kPOffset, m[n][c]);
-          k2[c] = exp2_fast(m[n][c] - x);
-          m[n][c] = x;
+          float now;
+          if constexpr (F8) {
+            // pairs: up, or down where the row's sums do not allow small weights to get lost (pair_lowers; all units' keys count from the start,
+            // which takes no registers); the unit's sum is that of the largest weights of four keys at least
+            const bool up = x > m[n][c] + (kPOffset + kRescale);
+            now = up ? x - (m[n][c] == kNoMax ? kPOffset : kPOffset + kPairRise) : m[n][c];
+            float tile = exp2_fast(top[n][c] - now);
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) {
+              tile += __shfl_xor_sync(0xffffffffu, tile, d);
+              sum[c] += __shfl_xor_sync(0xffffffffu, sum[c], d);
+            }
+            const float row = sum[c] * exp2_fast(m[n][c] - now), all = static_cast<float>(UK) * static_cast<float>(n_units);
+            if (pair_lowers(now + kPOffset, x, tile, row, UK, all - UK)) now = x - kPOffset;
+            enough &= row >= kPairEnough * all;
+          } else {
+            now = fmaxf(x - kPOffset, m[n][c]);
+          }
+          k2[c] = exp2_fast(m[n][c] - now);
+          m[n][c] = now;
 #pragma unroll
           for (int j = 0; j < 8; ++j) { o[j][n][c] *= k2[c]; o[j][n][c + 2] *= k2[c]; }
         }
         l[n] = f2_fma(l[n], f2_pack(k2[0], k2[1]), 0);
       }
+      if constexpr (F8) settled = __all_sync(0xffffffffu, enough);     // once all rows have enough for all units, only a maximum that rises asks again
     }
     uint32_t pt[STEPS][NT][2];                               // P^T as an operand: keys 0-7, keys 8-15; e4m3: hi, lo of the step's 16 keys
-    uint64_t unit[NT];                                       // sums of its weights, two rows
-    auto weights = [&]() {
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const uint64_t f = f2_pack(fac[n][0], fac[n][1]), shift = f2_pack(-m[n][0], -m[n][1]);
-        unit[n] = 0;
+    for (int n = 0; n < NT; ++n) {
+      const uint64_t f = f2_pack(fac[n][0], fac[n][1]), shift = f2_pack(-m[n][0], -m[n][1]);
 #pragma unroll
-        for (int u = 0; u < STEPS; ++u) {
-          float w0[2], w1[2];                                // keys g and g + 8 of the rows 2 t, 2 t + 1
+      for (int u = 0; u < STEPS; ++u) {
+        float w0[2], w1[2];                                  // keys g and g + 8 of the rows 2 t, 2 t + 1
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            float x0, x1;
-            f2_unpack(f2_fma(f2_pack(s[u][n][2 * h], s[u][n][2 * h + 1]), f, shift), x0, x1);
-            w0[h] = exp2_fast(x0); w1[h] = exp2_fast(x1);
-            unit[n] = f2_add(unit[n], f2_pack(w0[h], w1[h]));
-            if constexpr (!F8) pt[u][n][h] = transpose8x8(pack2<false>(w0[h], w1[h]));
-          }
-          if constexpr (F8) {
-            uint32_t h0, l0, h1, l1;
-            e4m3_pair(w0[0], w0[1], h0, l0);
-            e4m3_pair(w1[0], w1[1], h1, l1);
-            pt[u][n][0] = transpose8x8(h0 | (h1 << 16));
-            pt[u][n][1] = transpose8x8(l0 | (l1 << 16));
-          }
+        for (int h = 0; h < 2; ++h) {
+          float x0, x1;
+          f2_unpack(f2_fma(f2_pack(s[u][n][2 * h], s[u][n][2 * h + 1]), f, shift), x0, x1);
+          w0[h] = exp2_fast(x0); w1[h] = exp2_fast(x1);
+          l[n] = f2_add(l[n], f2_pack(w0[h], w1[h]));
+          if constexpr (!F8) pt[u][n][h] = transpose8x8(pack2<false>(w0[h], w1[h]));
         }
-      }
-    };
-    weights();
-    if constexpr (F8) {
-      // Pairs: whether the row's sums allow small weights to get lost (pair_lowers).  Once every lane has its share of enough for all units, only a
-      // maximum that rises asks again.
-      if (!settled) {
-        const float enough = kPairEnough * UK * static_cast<float>(n_units);
-        float now[NT][2];
-        bool small = false, all = true;
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          float before[2];
-          f2_unpack(unit[n], now[n][0], now[n][1]);
-          f2_unpack(l[n], before[0], before[1]);
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            all &= now[n][c] + before[c] >= enough / 8;
-#pragma unroll
-            for (int d = 4; d < 32; d <<= 1) now[n][c] += __shfl_xor_sync(0xffffffffu, now[n][c], d);
-            small |= now[n][c] < kPairEnough * UK;
-          }
-        }
-        settled = __all_sync(0xffffffffu, all);
-        if (!settled && __any_sync(0xffffffffu, small)) {
-          bool again = false;
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            float k2[2], before[2];
-            f2_unpack(l[n], before[0], before[1]);
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              float x = top[n][c];
-#pragma unroll
-              for (int d = 4; d < 32; d <<= 1) {
-                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
-                before[c] += __shfl_xor_sync(0xffffffffu, before[c], d);
-              }
-              const bool lowers = pair_lowers(m[n][c] + kPOffset, x, now[n][c], before[c], UK, n_units);
-              again |= lowers;
-              k2[c] = lowers ? exp2_fast(m[n][c] - (x - kPOffset)) : 1.f;
-              if (lowers) m[n][c] = x - kPOffset;
-#pragma unroll
-              for (int j = 0; j < 8; ++j) { o[j][n][c] *= k2[c]; o[j][n][c + 2] *= k2[c]; }
-            }
-            l[n] = f2_fma(l[n], f2_pack(k2[0], k2[1]), 0);
-          }
-          if (__any_sync(0xffffffffu, again)) weights();
+        if constexpr (F8) {
+          uint32_t h0, l0, h1, l1;
+          e4m3_pair(w0[0], w0[1], h0, l0);
+          e4m3_pair(w1[0], w1[1], h1, l1);
+          pt[u][n][0] = transpose8x8(h0 | (h1 << 16));
+          pt[u][n][1] = transpose8x8(l0 | (l1 << 16));
         }
       }
     }
-#pragma unroll
-    for (int n = 0; n < NT; ++n) l[n] = f2_add(l[n], unit[n]);
     // ---- O^T ----
     if constexpr (!F8) {
 #pragma unroll
