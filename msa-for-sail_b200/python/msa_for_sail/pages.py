@@ -222,7 +222,7 @@ def kv_pages_free(block_table: torch.Tensor, num_held: torch.Tensor, kv_lens: to
     buf = torch.empty(_workspace("free", B, width) + 1, dtype=torch.int32, device=dev)
     ptr = buf.data_ptr()
     _launch(dev, _lib.lib.msa_pages_free, _lib.pages_free_args(
-        _address(packed) or 0, block_table.data_ptr(), num_held.data_ptr(), kv_lens.data_ptr(), free_pages.data_ptr(), num_free.data_ptr(),
+        _address(packed) if num else 0, block_table.data_ptr(), num_held.data_ptr(), kv_lens.data_ptr(), free_pages.data_ptr(), num_free.data_ptr(),
         0 if shares is None else shares.data_ptr(), ptr, 0 if num_shared is None else num_shared.data_ptr(), ptr + 4, stride, num, B, width, page_size,
         free_pages.shape[0], (1 << 31) - 1 if shares is None else shares.shape[0], max(window, 0),
         int(num_sink_tokens) if window > 0 else 0), "msa_pages_free")
