@@ -666,12 +666,13 @@ int launch(const MsaFmhaParams& p, cudaStream_t stream) {
 }  // namespace window
 
 // Windowed items of few packed rows; pages of whole units, or ragged keys.  Here and on the tcgen05 decode kernel (pages of 128 keys), one token a
-// sequence: bf16, 32 rows, 64 sequences x 2 heads x 2 048 keys 34 and 34 us, 128 x 8 x 4 096 326 and 366; e4m3, 8 rows, 21 and 24, 178 and 229.  16 rows
-// over an e4m3 cache (255 registers) pay while items are few and many CTAs share one: 32 items x 1 024 keys 12.0 and 14.4 us, 64 14.4 and 14.9, 96 18.9
-// and 17.4, 512 50 and 44; with 32 rows registers run out.
+// sequence: bf16, 32 rows, 64 sequences x 2 heads x 2 048 keys 34 and 34 us, 128 x 8 x 4 096 326 and 366; e4m3, 8 rows, 64 x 1 x 2 048 15.2 and 22.3,
+// 128 x 8 x 4 096 186 and 285.  16 rows over an e4m3 cache (255 registers) pay while items are few and three CTAs or more share one: windows of 1 024 keys, 32
+// items 14.1 and 16.4 us, 80 17.6 and 19.7, 96 21.8 and 20.3, 512 61 and 55; of 4 096, 32 21.6 and 33.6, 80 36.5 and 43.9, 96 51 and 45, 512 166 and 148;
+// of 512, within 5 % from 64 items on.  With 32 rows registers run out.
 int fmha_window_rows(const MsaFmhaParams& p) {
   if (p.kv_dtype != MSA_DT_E4M3) return 32;
-  return p.page_size == kKvTile && 128 % p.pack == 0 && p.num_work > sms_of(p) / 2 ? 8 : 16;
+  return p.page_size == kKvTile && 128 % p.pack == 0 && p.num_work > sms_of(p) * 3 / 5 ? 8 : 16;
 }
 int fmha_window_supported(const MsaFmhaParams& p) {
   if (p.window <= 0 || (p.flags & MSA_FLAG_SPARSE) || p.decode_rows < 1 || p.decode_rows > fmha_window_rows(p)) return 0;
