@@ -262,6 +262,8 @@ __device__ __forceinline__ float pair_reference(float ref, float sum, float& los
   return now;
 }
 
+// Row tile [rows][128 x 16-bit]: 16 chunks of 16 bytes per row, chunk index XOR-ed with
+// (row & 7) so that ldmatrix reads and 16-byte row writes are bank-conflict free.
 __device__ __forceinline__ uint32_t swz_off(int row, int chunk) {
   return static_cast<uint32_t>(row * 256 + ((chunk ^ (row & 7)) << 4));
 }

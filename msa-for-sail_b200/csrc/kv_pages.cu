@@ -484,9 +484,8 @@ __global__ void __launch_bounds__(kThreads) pages_free_held_kernel(const MsaPage
 
 // Rows that were cut back into a page that other rows hold (see kept_of: entry len / page_size, partly used).  By one CTA, after all of the above.
 // Workspace, behind the counts: the page of each such row (-1: none), its number among those that go to another page (-1: it does not), then the moves
-// (from, to, tokens), then their number.  shares[p] goes down by one
-// for each such row of p; below zero nobody else holds p, and the last row, whose number is put in the place of the share, keeps it.  (512 rows of 17
-// pages, 8 of them so: 8 us with the copy's launch, in a captured graph.)
+// (from, to, tokens), then their number.  shares[p] goes down by one for each such row of p; below zero nobody else holds p, and the last row, whose
+// number is put in the place of the share, keeps it.  (512 rows of 17 pages, 8 of them so: 8 us with the copy's launch, in a captured graph.)
 struct Cut {
   int32_t *page, *rank, *src, *dst, *tokens, *moves;
 };

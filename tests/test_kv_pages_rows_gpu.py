@@ -111,8 +111,8 @@ def _holders(rng, rows, width, page):
 @pytest.mark.parametrize("rows,width,page", [(1, 3, 16), (4, 3, 16), (60, 5, 16), (3000, 3, 16), (40, 9, 128), (3, 90000, 16)])
 @pytest.mark.parametrize("moving", [True, False])
 @pytest.mark.parametrize("short", [False, True])
-@pytest.mark.parametrize("seed", [1, 2])
-def test_rows_cut_back_into_a_shared_page(rows, width, page, moving, short, seed):
+@pytest.mark.parametrize("window,sinks,seed", [(-1, 0, 1), (-1, 0, 2), (20, 5, 3)])
+def test_rows_cut_back_into_a_shared_page(rows, width, page, moving, short, window, sinks, seed):
     import pages_ref as ref
     rng = random.Random(seed * 100 + rows)
     table, held, kv, free, shares, P = _holders(rng, rows, width, page)
@@ -126,8 +126,8 @@ def test_rows_cut_back_into_a_shared_page(rows, width, page, moving, short, seed
               torch.randint(0, 256, (P, 5), dtype=torch.uint8, device=DEV)]
     want = [c.clone() for c in caches]
     left = _i32([-3])
-    freed = _msa().kv_pages_free(**d, page_size=page, caches=caches if moving else (), num_shared=left)
-    num_free, n = ref.free_pages(table, held, kv, free, num_free, shares, -1, 0, page)
+    freed = _msa().kv_pages_free(**d, window_size=window, num_sink_tokens=sinks, page_size=page, caches=caches if moving else (), num_shared=left)
+    num_free, n = ref.free_pages(table, held, kv, free, num_free, shares, window, sinks, page)
     moves, num_free, still = _cut(table, held, kv, free, num_free, shares, page, moving)
     assert freed.item() == n and left.item() == still and d["num_free"].item() == num_free
     assert d["block_table"].tolist() == table and d["num_held"].tolist() == held and d["shares"].tolist() == shares and d["kv_lens"].tolist() == kv
