@@ -206,3 +206,55 @@ def test_forks_copy_whole_pages_where_the_tokens_could_be_either_dimension():
         w[4] = w[2]
         assert torch.equal(t, w)
     assert table.tolist() == [[2], [4]]
+
+
+@pytest.mark.parametrize("rows,width,seed", [(2, 3, 1), (5, 6, 2), (5, 3, 3), (20, 3, 4), (20, 6, 5), (20, 6, 6)])
+def test_requests_keep_their_tokens(rows, width, seed):
+    """Requests that grow, fork, are cut back anywhere, end and move: each reads its own tokens throughout, and no page is lost or held twice."""
+    msa, rng, page, P = _msa(), random.Random(seed), 16, rows * width + 4
+    table, held, kv = torch.full((rows, width), -1, dtype=torch.int32, device=DEV), _i32([0] * rows), _i32([0] * rows)
+    free, num_free, shares, left = _i32(rng.sample(range(P), P)), _i32([P]), _i32([0] * P), _i32([0])
+    cache = torch.zeros(P, 1, page, 1, dtype=torch.int32, device=DEV)          # a number for each token
+    tokens, last = [[] for _ in range(rows)], 0
+    for _ in range(60):
+        op = rng.choice(["grow", "grow", "fork", "cut", "end", "compact"])
+        if op == "grow":
+            ql = [min(rng.randint(0, 20), width * page - len(t)) if t or rng.random() < 0.5 else 0 for t in tokens]
+            if sum(-(-(len(t) + q) // page) - -(-len(t) // page) for t, q in zip(tokens, ql)) > num_free.item():
+                continue
+            kv += _i32(ql)
+            slots = msa.paged_kv_tables(_i32(ql), kv, table, held, free, num_free, max_total_q=max(1, sum(ql)), page_size=page, num_held_out=held,
+                                        num_free_out=num_free)["slot_map"][:sum(ql)]
+            cache.view(-1)[slots.long()] = torch.arange(last, last + sum(ql), dtype=torch.int32, device=DEV)
+            for t, q in zip(tokens, ql):
+                t += range(last, last + q)
+                last += q
+        elif op == "fork":
+            empty, full = [b for b in range(rows) if not tokens[b]], [b for b in range(rows) if tokens[b]]
+            if not empty or not full:
+                continue
+            children = rng.sample(empty, rng.randint(1, len(empty)))
+            parents = [rng.choice(full) for _ in children]
+            if sum(len(tokens[p]) % page > 0 for p in parents) > num_free.item():
+                continue
+            at = rng.randint(0, len(children))
+            entries = children[:at] + [rng.randrange(rows)] + children[at:], parents[:at] + [-1] + parents[at:]      # one that does nothing
+            assert msa.kv_pages_fork(table, held, kv, _i32(entries[1]), _i32(entries[0]), free, num_free, shares, cache, page).item() == 0
+            for p, c in zip(parents, children):
+                tokens[c] = list(tokens[p])
+        elif op == "compact":
+            msa.kv_pages_compact(table, held, free, num_free, cache, shares)
+        else:
+            tokens = [t if rng.random() < 0.4 else t[:0 if op == "end" else rng.randint(0, len(t))] for t in tokens]
+            kv.copy_(_i32([len(t) for t in tokens]))
+            msa.kv_pages_free(table, held, kv, free, num_free, shares, page_size=page, caches=cache, num_shared=left)
+            assert left.item() == 0                             # (the pool has a page for every entry of the table)
+        rows_of, used, data, holders = table.tolist(), held.tolist(), cache.view(P, page).tolist(), {}
+        for b, t in enumerate(tokens):
+            pages = rows_of[b][:used[b]]
+            assert len(pages) == -(-len(t) // page) and [x for p in pages for x in data[p]][:len(t)] == t, op
+            for p in pages:
+                holders[p] = holders.get(p, 0) + 1
+            assert len(t) % page == 0 or shares[pages[-1]].item() == 0, op
+        stack = free.tolist()[:num_free.item()]
+        assert sorted(stack + list(holders)) == list(range(P)) and shares.tolist() == [holders.get(p, 1) - 1 for p in range(P)], op
